@@ -10,7 +10,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libgdnx.so"
 
-GDNX_OK, GDNX_EINVAL, GDNX_ELAUNCH, GDNX_ETIMEOUT, GDNX_EUNSUPPORTED, GDNX_EWORKSPACE = range(6)
+GDNX_OK, GDNX_EINVAL, GDNX_ELAUNCH, GDNX_ETIMEOUT, GDNX_EUNSUPPORTED, GDNX_EWORKSPACE, GDNX_ENOPAGES = range(7)
 GDNX_F32, GDNX_BF16, GDNX_F16 = 0, 1, 2
 GDNX_MODE_GDN3, GDNX_MODE_KMD2 = 0, 1
 GDNX_DECAY_GAMMA, GDNX_DECAY_LOG, GDNX_DECAY_BRAIDED = 0, 1, 2
@@ -21,7 +21,9 @@ GDNX_COMPACT_SVD, GDNX_COMPACT_SKETCH = 0, 1
 EXPORTED = ("gdnx_scan_fwd", "gdnx_scan_fwd_noalloc", "gdnx_scan_noalloc_status", "gdnx_scan_workspace_bytes", "gdnx_kr_scan_fwd", "gdnx_compact",
             "gdnx_decode_step", "gdnx_epilogue", "gdnx_gdn3_prologue", "gdnx_kmd2_prologue", "gdnx_scan_bwd", "gdnx_scan_bwd_workspace_bytes", "gdnx_status_string", "gdnx_version",
             "gdnx_epilogue_scatter", "gdnx_device_alloc", "gdnx_device_free", "gdnx_ipc_handle", "gdnx_ipc_open",
-            "gdnx_ipc_close")
+            "gdnx_ipc_close", "gdnx_attn_fwd", "gdnx_attn_bwd", "gdnx_attn_bwd_workspace_bytes", "gdnx_cache_fork",
+            "gdnx_cache_extend", "gdnx_cache_write", "gdnx_cache_truncate", "gdnx_cache_trim", "gdnx_cache_compact",
+            "gdnx_cache_workspace_bytes", "gdnx_paged_decode", "gdnx_paged_decode_workspace_bytes")
 
 
 class View(C.Structure):
@@ -115,6 +117,35 @@ class Kmd2PrologueArgs(C.Structure):
                 ("beta_e_out", C.c_void_p), ("beta_w_out", C.c_void_p), ("theta_ws", C.c_void_p)]
 
 
+class AttnArgs(C.Structure):
+    _fields_ = [("B", C.c_int64), ("Tq", C.c_int64), ("Tk", C.c_int64), ("H", C.c_int64), ("Hk", C.c_int64),
+                ("D", C.c_int64), ("window", C.c_int64), ("sinks", C.c_int64), ("scale", C.c_float),
+                ("q", View), ("k", View), ("v", View), ("lengths", C.c_void_p),
+                ("y", C.c_void_p), ("y_dtype", C.c_int32),
+                ("y_sb", C.c_int64), ("y_st", C.c_int64), ("y_sh", C.c_int64),
+                ("lse", C.c_void_p), ("error", C.c_void_p)]
+
+
+class AttnBwdArgs(C.Structure):
+    _fields_ = [("fwd", AttnArgs), ("dy", View), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class Cache(C.Structure):
+    _fields_ = [("kv", C.c_void_p), ("dtype", C.c_int32), ("page", C.c_int32),
+                ("L", C.c_int64), ("pages", C.c_int64), ("Hk", C.c_int64), ("D", C.c_int64),
+                ("slots", C.c_int64), ("width", C.c_int64),
+                ("table", C.c_void_p), ("lengths", C.c_void_p), ("refs", C.c_void_p), ("status", C.c_void_p)]
+
+
+class PagedDecodeArgs(C.Structure):
+    _fields_ = [("cache", Cache), ("B", C.c_int64), ("H", C.c_int64), ("layer", C.c_int64),
+                ("window", C.c_int64), ("sinks", C.c_int64), ("max_len", C.c_int64), ("scale", C.c_float),
+                ("q", View), ("rows", C.c_void_p), ("y", C.c_void_p), ("y_dtype", C.c_int32),
+                ("y_sb", C.c_int64), ("y_sh", C.c_int64), ("error", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 _lib = None
 
 
@@ -163,6 +194,25 @@ def load(path: Path = LIB_PATH):
     lib.gdnx_ipc_close.restype = C.c_int
     lib.gdnx_scan_bwd_workspace_bytes.argtypes = [C.POINTER(ScanBwdArgs)]
     lib.gdnx_scan_bwd_workspace_bytes.restype = C.c_size_t
+    lib.gdnx_attn_fwd.argtypes = [C.POINTER(AttnArgs), C.c_void_p]
+    lib.gdnx_attn_fwd.restype = C.c_int
+    lib.gdnx_attn_bwd_workspace_bytes.argtypes = [C.POINTER(AttnBwdArgs)]
+    lib.gdnx_attn_bwd_workspace_bytes.restype = C.c_size_t
+    lib.gdnx_attn_bwd.argtypes = [C.POINTER(AttnBwdArgs), C.c_void_p]
+    lib.gdnx_attn_bwd.restype = C.c_int
+    cache, ptr, size, i64 = C.POINTER(Cache), C.c_void_p, C.c_size_t, C.c_int64
+    lib.gdnx_cache_workspace_bytes.argtypes = [cache, i64]
+    lib.gdnx_cache_workspace_bytes.restype = size
+    for name, types in (("fork", [cache, i64, ptr, ptr, ptr]), ("extend", [cache, i64, ptr, ptr, ptr, size, ptr]),
+                        ("write", [cache, i64, i64, i64, C.POINTER(View), C.POINTER(View), ptr, ptr, ptr]),
+                        ("truncate", [cache, i64, ptr, ptr, ptr]), ("trim", [cache, i64, ptr, i64, i64, ptr]),
+                        ("compact", [cache, ptr, size, ptr])):
+        fn = getattr(lib, "gdnx_cache_" + name)
+        fn.argtypes, fn.restype = types, C.c_int
+    lib.gdnx_paged_decode_workspace_bytes.argtypes = [C.POINTER(PagedDecodeArgs)]
+    lib.gdnx_paged_decode_workspace_bytes.restype = size
+    lib.gdnx_paged_decode.argtypes = [C.POINTER(PagedDecodeArgs), C.c_void_p]
+    lib.gdnx_paged_decode.restype = C.c_int
     lib.gdnx_status_string.argtypes = [C.c_int]
     lib.gdnx_status_string.restype = C.c_char_p
     lib.gdnx_version.argtypes = []

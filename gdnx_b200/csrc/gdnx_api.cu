@@ -79,9 +79,184 @@ Path select_path(const gdnx_scan_args& a) {
   return Path::kGeneral;
 }
 
+// ---- windowed attention and the paged cache ----
+
+constexpr int64_t kMaxTokens = (int64_t)1 << 30;  // positions and their distances stay in int32
+
+// A [B,T,H,D] operand: its pointer may be null where it has no elements.
+bool heads_ok(const gdnx_view& v, int dtype, int64_t D) {
+  return is_device_ptr(v.ptr) && v.dtype == dtype && v.dim == D && v.sb >= 0 && v.st >= 0 && v.sh >= 0;
+}
+
+gdnx_status check_attn(const gdnx_attn_args& a) {
+  if (a.B < 0 || a.Tq < 0 || a.Tk < a.Tq || a.H <= 0 || a.Hk <= 0 || a.D <= 0) return GDNX_EINVAL;
+  if (a.H % a.Hk || a.window < 1 || a.sinks < 0) return GDNX_EINVAL;
+  if (!(a.scale > 0.f) || a.scale > 3.0e38f || !dtype_ok(a.q.dtype) || !dtype_ok(a.y_dtype)) return GDNX_EINVAL;
+  if (a.D > 128 || a.D % 8 || a.Tk > kMaxTokens || a.B > 65535 || a.H > 65535) return GDNX_EUNSUPPORTED;
+  if (a.B == 0 || a.Tk == 0) return GDNX_OK;
+  if (!heads_ok(a.k, a.q.dtype, a.D) || !heads_ok(a.v, a.q.dtype, a.D)) return GDNX_EINVAL;
+  if (a.Tq > 0 && (!heads_ok(a.q, a.q.dtype, a.D) || !is_device_ptr(a.y))) return GDNX_EINVAL;
+  if (a.y_sb < 0 || a.y_st < 0 || a.y_sh < 0) return GDNX_EINVAL;
+  if (a.lengths && !is_device_ptr(a.lengths)) return GDNX_EINVAL;
+  if (a.lse && a.Tq > 0 && !is_device_ptr(a.lse)) return GDNX_EINVAL;
+  if (a.error && !is_device_ptr(a.error)) return GDNX_EINVAL;
+  return GDNX_OK;
+}
+
+// Window and sinks beyond the sequence say no more than its length does.
+gdnx_attn_args clamp_attn(const gdnx_attn_args& a) {
+  gdnx_attn_args c = a;
+  if (c.window > c.Tk) c.window = c.Tk;
+  if (c.sinks > c.Tk) c.sinks = c.Tk;
+  return c;
+}
+
+gdnx_status check_cache(const gdnx_cache* c) {
+  if (!c) return GDNX_EINVAL;
+  if (!dtype_ok(c->dtype) || c->L <= 0 || c->pages < 0 || c->Hk <= 0 || c->D <= 0 || c->slots <= 0 || c->width <= 0)
+    return GDNX_EINVAL;
+  if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128) return GDNX_EUNSUPPORTED;
+  if (c->D > 128 || c->D % 8 || c->slots > (1 << 18) || c->width > (1 << 20) || c->width * c->page > kMaxTokens ||
+      c->pages > ((int64_t)1 << 30))
+    return GDNX_EUNSUPPORTED;
+  if (c->pages && (!is_device_ptr(c->kv) || reinterpret_cast<uintptr_t>(c->kv) % 16 || !is_device_ptr(c->refs)))
+    return GDNX_EINVAL;
+  if (!is_device_ptr(c->table) || !is_device_ptr(c->lengths) || !is_device_ptr(c->status)) return GDNX_EINVAL;
+  return GDNX_OK;
+}
+
+// A list of n slots with one more list beside it.
+gdnx_status check_rows(const gdnx_cache* c, int64_t n, const int32_t* rows, const int32_t* more) {
+  const gdnx_status s = check_cache(c);
+  if (s != GDNX_OK) return s;
+  if (n < 0 || n > c->slots) return GDNX_EINVAL;
+  if (n && (!is_device_ptr(rows) || !is_device_ptr(more))) return GDNX_EINVAL;
+  return GDNX_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+gdnx_status gdnx_attn_fwd(const gdnx_attn_args* a, void* stream) {
+  if (!a) return GDNX_EINVAL;
+  const gdnx_status s = check_attn(*a);
+  if (s != GDNX_OK || a->B == 0 || a->Tq == 0) return s;
+  return gdnx::launch_attn_fwd_simt(clamp_attn(*a), (cudaStream_t)stream);
+}
+
+size_t gdnx_attn_bwd_workspace_bytes(const gdnx_attn_bwd_args* g) {
+  if (!g || g->fwd.B <= 0 || g->fwd.Tq <= 0 || g->fwd.H <= 0) return 0;
+  return (size_t)(g->fwd.B * g->fwd.H * g->fwd.Tq) * sizeof(float);
+}
+
+gdnx_status gdnx_attn_bwd(const gdnx_attn_bwd_args* g, void* stream) {
+  if (!g) return GDNX_EINVAL;
+  const gdnx_attn_args& a = g->fwd;
+  const gdnx_status s = check_attn(a);
+  if (s != GDNX_OK || a.B == 0 || a.Tk == 0) return s;
+  if (!is_device_ptr(g->dk) || !is_device_ptr(g->dv)) return GDNX_EINVAL;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (a.Tq == 0) {  // nothing was read: the gradients are zero
+    const size_t bytes = (size_t)(a.B * a.Tk * a.Hk * a.D) * (a.k.dtype == GDNX_F32 ? 4 : 2);
+    return cudaMemsetAsync(g->dk, 0, bytes, st) == cudaSuccess && cudaMemsetAsync(g->dv, 0, bytes, st) == cudaSuccess
+               ? GDNX_OK : GDNX_ELAUNCH;
+  }
+  if (!heads_ok(g->dy, a.q.dtype, a.D) || !is_device_ptr(g->dq) || !a.lse) return GDNX_EINVAL;
+  if (g->workspace_bytes < gdnx_attn_bwd_workspace_bytes(g) || !is_device_ptr(g->workspace)) return GDNX_EWORKSPACE;
+  gdnx_attn_bwd_args c = *g;
+  c.fwd = clamp_attn(a);
+  float* delta = static_cast<float*>(g->workspace);
+  const gdnx_status d = gdnx::launch_attn_delta(c, delta, st);
+  return d != GDNX_OK ? d : gdnx::launch_attn_bwd_simt(c, delta, st);
+}
+
+size_t gdnx_cache_workspace_bytes(const gdnx_cache* c, int64_t n) {
+  return !c || n < 0 || c->pages < 0 ? 0 : gdnx::cache_workspace_bytes(*c, n);
+}
+
+gdnx_status gdnx_cache_fork(const gdnx_cache* c, int64_t n, const int32_t* src, const int32_t* dst, void* stream) {
+  const gdnx_status s = check_rows(c, n, src, dst);
+  return s != GDNX_OK || n == 0 ? s : gdnx::launch_cache_fork(*c, n, src, dst, (cudaStream_t)stream);
+}
+
+gdnx_status gdnx_cache_extend(const gdnx_cache* c, int64_t n, const int32_t* rows, const int32_t* counts,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  const gdnx_status s = check_rows(c, n, rows, counts);
+  if (s != GDNX_OK || n == 0) return s;
+  if (workspace_bytes < gdnx_cache_workspace_bytes(c, n) || !is_device_ptr(workspace)) return GDNX_EWORKSPACE;
+  return gdnx::launch_cache_extend(*c, n, rows, counts, workspace, (cudaStream_t)stream);
+}
+
+gdnx_status gdnx_cache_write(const gdnx_cache* c, int64_t layer, int64_t n, int64_t T, const gdnx_view* k,
+                             const gdnx_view* v, const int32_t* rows, const int32_t* counts, void* stream) {
+  const gdnx_status s = check_cache(c);
+  if (s != GDNX_OK) return s;
+  if (layer < 0 || layer >= c->L || n < 0 || T < 0 || !k || !v) return GDNX_EINVAL;
+  if (n == 0 || T == 0) return GDNX_OK;
+  if (!heads_ok(*k, c->dtype, c->D) || !heads_ok(*v, c->dtype, c->D) || !is_device_ptr(rows)) return GDNX_EINVAL;
+  if (counts && !is_device_ptr(counts)) return GDNX_EINVAL;
+  return gdnx::launch_cache_write(*c, layer, n, T, *k, *v, rows, counts, (cudaStream_t)stream);
+}
+
+gdnx_status gdnx_cache_truncate(const gdnx_cache* c, int64_t n, const int32_t* rows, const int32_t* lengths,
+                                void* stream) {
+  const gdnx_status s = check_rows(c, n, rows, lengths);
+  return s != GDNX_OK || n == 0 ? s : gdnx::launch_cache_truncate(*c, n, rows, lengths, (cudaStream_t)stream);
+}
+
+gdnx_status gdnx_cache_trim(const gdnx_cache* c, int64_t n, const int32_t* rows, int64_t window, int64_t sinks,
+                            void* stream) {
+  const gdnx_status s = check_rows(c, n, rows, rows);
+  if (s != GDNX_OK) return s;
+  if (window < 1 || sinks < 0) return GDNX_EINVAL;
+  return n == 0 ? GDNX_OK : gdnx::launch_cache_trim(*c, n, rows, window, sinks, (cudaStream_t)stream);
+}
+
+gdnx_status gdnx_cache_compact(const gdnx_cache* c, void* workspace, size_t workspace_bytes, void* stream) {
+  const gdnx_status s = check_cache(c);
+  if (s != GDNX_OK || c->pages == 0) return s;
+  if (workspace_bytes < gdnx_cache_workspace_bytes(c, 0) || !is_device_ptr(workspace)) return GDNX_EWORKSPACE;
+  return gdnx::launch_cache_compact(*c, workspace, (cudaStream_t)stream);
+}
+
+// The decode's arguments with window and sinks kept within the longest sequence.
+static gdnx_paged_decode_args clamp_decode(const gdnx_paged_decode_args& a) {
+  gdnx_paged_decode_args c = a;
+  const int64_t most = a.cache.width * a.cache.page;
+  if (c.window > most) c.window = most;
+  if (c.sinks > most) c.sinks = most;
+  return c;
+}
+
+static gdnx_status check_decode(const gdnx_paged_decode_args& a) {
+  const gdnx_status s = check_cache(&a.cache);
+  if (s != GDNX_OK) return s;
+  if (a.B < 0 || a.H <= 0 || a.H % a.cache.Hk || a.layer < 0 || a.layer >= a.cache.L || a.window < 1 || a.sinks < 0 ||
+      a.max_len < 0 || !(a.scale > 0.f) || a.scale > 3.0e38f || !dtype_ok(a.y_dtype))
+    return GDNX_EINVAL;
+  if (a.B > 65535 || a.H > 65535) return GDNX_EUNSUPPORTED;
+  if (!a.rows && a.B > a.cache.slots) return GDNX_EINVAL;
+  if (a.B == 0) return GDNX_OK;
+  if (!heads_ok(a.q, a.cache.dtype, a.cache.D) || !is_device_ptr(a.y) || a.y_sb < 0 || a.y_sh < 0) return GDNX_EINVAL;
+  if (a.rows && !is_device_ptr(a.rows)) return GDNX_EINVAL;
+  if (a.error && !is_device_ptr(a.error)) return GDNX_EINVAL;
+  return GDNX_OK;
+}
+
+size_t gdnx_paged_decode_workspace_bytes(const gdnx_paged_decode_args* a) {
+  if (!a || a->B <= 0 || a->H <= 0 || a->cache.Hk <= 0 || a->window < 1 || a->sinks < 0) return 0;
+  return gdnx::paged_decode_workspace_bytes(clamp_decode(*a));
+}
+
+gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* a, void* stream) {
+  if (!a) return GDNX_EINVAL;
+  const gdnx_status s = check_decode(*a);
+  if (s != GDNX_OK || a->B == 0) return s;
+  const size_t need = gdnx_paged_decode_workspace_bytes(a);
+  if (need && (a->workspace_bytes < need || !is_device_ptr(a->workspace))) return GDNX_EWORKSPACE;
+  return gdnx::launch_paged_decode(clamp_decode(*a), (cudaStream_t)stream);
+}
 
 const char* gdnx_status_string(gdnx_status s) {
   switch (s) {
@@ -91,6 +266,7 @@ const char* gdnx_status_string(gdnx_status s) {
     case GDNX_ETIMEOUT: return "GDNX_ETIMEOUT: a bounded device-side wait ran out";
     case GDNX_EUNSUPPORTED: return "GDNX_EUNSUPPORTED: no kernel for this configuration in this build";
     case GDNX_EWORKSPACE: return "GDNX_EWORKSPACE: workspace missing or too small";
+    case GDNX_ENOPAGES: return "GDNX_ENOPAGES: the cache's pool or page table has no room";
   }
   return "GDNX_UNKNOWN";
 }

@@ -14,6 +14,24 @@ constexpr int kMaxPeerOuts = 8;  // destinations of the scattering lane routing
 gdnx_status launch_epilogue_scatter(const gdnx_epilogue_args& a, void* const* outs, int n, cudaStream_t st);
 gdnx_status launch_proj_prologue(const gdnx_prologue_args& a, cudaStream_t st);
 gdnx_status launch_kmd2_prologue(const gdnx_kmd2_prologue_args& a, cudaStream_t st);
+// Windowed attention (attn_simt.cu: CUDA cores, every type and layout) and its gradients.
+gdnx_status launch_attn_fwd_simt(const gdnx_attn_args& a, cudaStream_t st);
+gdnx_status launch_attn_delta(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st);
+gdnx_status launch_attn_bwd_simt(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st);
+// Paged cache (paged_cache.cu) and the attention that reads it (paged_decode.cu).
+size_t cache_workspace_bytes(const gdnx_cache& c, int64_t n);
+gdnx_status launch_cache_fork(const gdnx_cache& c, int64_t n, const int32_t* src, const int32_t* dst, cudaStream_t st);
+gdnx_status launch_cache_extend(const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* counts, void* ws,
+                                cudaStream_t st);
+gdnx_status launch_cache_write(const gdnx_cache& c, int64_t layer, int64_t n, int64_t T, const gdnx_view& k,
+                               const gdnx_view& v, const int32_t* rows, const int32_t* counts, cudaStream_t st);
+gdnx_status launch_cache_truncate(const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* lengths,
+                                  cudaStream_t st);
+gdnx_status launch_cache_trim(const gdnx_cache& c, int64_t n, const int32_t* rows, int64_t window, int64_t sinks,
+                              cudaStream_t st);
+gdnx_status launch_cache_compact(const gdnx_cache& c, void* ws, cudaStream_t st);
+size_t paged_decode_workspace_bytes(const gdnx_paged_decode_args& a);
+gdnx_status launch_paged_decode(const gdnx_paged_decode_args& a, cudaStream_t st);
 // Backward of the dense scan (scan_backward.cu).
 bool scan_bwd_supported(const gdnx_scan_bwd_args& a);
 size_t scan_bwd_workspace_bytes(const gdnx_scan_bwd_args& a);

@@ -42,7 +42,8 @@ typedef enum {
   GDNX_ELAUNCH = 2,      /* CUDA launch or attribute error                         */
   GDNX_ETIMEOUT = 3,     /* a bounded device-side wait ran out (error word set)   */
   GDNX_EUNSUPPORTED = 4, /* valid request this build has no kernel for            */
-  GDNX_EWORKSPACE = 5    /* workspace missing or too small                        */
+  GDNX_EWORKSPACE = 5,   /* workspace missing or too small                        */
+  GDNX_ENOPAGES = 6      /* a cache's pool or page table has no room (device word) */
 } gdnx_status;
 
 typedef enum { GDNX_F32 = 0, GDNX_BF16 = 1, GDNX_F16 = 2 } gdnx_dtype;
@@ -396,6 +397,116 @@ typedef struct {
 } gdnx_kmd2_prologue_args;
 
 GDNX_API gdnx_status gdnx_kmd2_prologue(const gdnx_kmd2_prologue_args* args, void* stream);
+
+/* Causal attention with a sliding window and sink tokens, the exact short-range read
+ * that stands beside the recurrent state.  Query i stands at position p = Tk - Tq + i
+ * (a prompt, or the end of one whose beginning is already known) and sees key j where
+ *   j <= p,  j < lengths[b],  and  p - j < window  or  j < sinks;
+ * a query with p >= lengths[b] is padding: its output is 0, its lse -inf, and what its
+ * rows of q, dy, k and v hold (NaN included) reaches no output.
+ *   y_i = sum_j softmax_j(scale q_i.k_j) v_j ;  query head h reads key head h / (H / Hk).
+ * Scores, softmax statistics and sums are fp32; 16-bit inputs run on the tensor cores
+ * where TMA can address them, other types and layouts on the CUDA cores. */
+typedef struct {
+  int64_t B, Tq, Tk, H, Hk, D; /* Tq <= Tk; H a multiple of Hk; D <= 128, a multiple of 8 */
+  int64_t window, sinks;       /* window >= 1 (Tk or more: plain causal), sinks >= 0       */
+  float scale;
+  gdnx_view q;                 /* [B,Tq,H,D]  (sb, st, sh)                                 */
+  gdnx_view k, v;              /* [B,Tk,Hk,D], the type of q                               */
+  const int32_t* lengths;      /* [B] device, clamped to 0..Tk; NULL = all Tk              */
+  void* y;                     /* [B,Tq,H,D] */
+  int32_t y_dtype;
+  int64_t y_sb, y_st, y_sh;
+  float* lse;                  /* [B,H,Tq] log of the sum of exponentials; NULL = not kept */
+  int32_t* error;              /* device word that takes GDNX_ETIMEOUT; NULL = none        */
+} gdnx_attn_args;
+
+GDNX_API gdnx_status gdnx_attn_fwd(const gdnx_attn_args* args, void* stream);
+
+/* Its gradients.  `fwd` holds the forward's arguments, its output y and its lse.
+ * dq [B,Tq,H,D], dk, dv [B,Tk,Hk,D] are contiguous, in the inputs' type; gradients of
+ * shared key heads are summed over their query heads.  No atomics: the same inputs give
+ * the same bits. */
+typedef struct {
+  gdnx_attn_args fwd;
+  gdnx_view dy;                /* [B,Tq,H,D], the type of q */
+  void* dq;
+  void* dk;
+  void* dv;
+  void* workspace;
+  size_t workspace_bytes;
+} gdnx_attn_bwd_args;
+
+GDNX_API size_t gdnx_attn_bwd_workspace_bytes(const gdnx_attn_bwd_args* args);
+GDNX_API gdnx_status gdnx_attn_bwd(const gdnx_attn_bwd_args* args, void* stream);
+
+/* A paged key/value cache, all of it caller-owned device memory.  A slot is one sequence;
+ * page table[s][i] holds its tokens i*page .. i*page+page-1, one key head after another,
+ * of every layer.  refs counts the slots that hold a page; a page with refs 0 is free.
+ * The page operations below run on the device without host synchronisation.  A call that
+ * cannot be carried out changes nothing and sets *status (GDNX_ENOPAGES: pool or table too
+ * small; GDNX_EINVAL: a slot out of range or named twice, a negative count); while
+ * *status is not 0 the operations do nothing, so a step can be enqueued whole and
+ * checked once. */
+typedef struct {
+  void* kv;                    /* [L, 2, pages, Hk, page, D], 16-byte aligned */
+  int32_t dtype;
+  int32_t page;                /* 16, 32, 64 or 128 tokens */
+  int64_t L, pages, Hk, D;     /* D <= 128, a multiple of 8 */
+  int64_t slots, width;        /* width = pages a slot can hold */
+  int32_t* table;              /* [slots, width], -1 = no page */
+  int32_t* lengths;            /* [slots] */
+  int32_t* refs;               /* [pages] */
+  int32_t* status;             /* one word */
+} gdnx_cache;
+
+GDNX_API size_t gdnx_cache_workspace_bytes(const gdnx_cache* cache, int64_t n);
+/* dst[i] releases its pages and becomes a copy of src[i] that shares src's pages. */
+GDNX_API gdnx_status gdnx_cache_fork(const gdnx_cache* cache, int64_t n, const int32_t* src, const int32_t* dst,
+                                     void* stream);
+/* Room for counts[i] more tokens in slot rows[i]: free pages, the lowest index first, in
+ * the order of rows.  A partly filled last page that other slots share is copied first
+ * (every layer), so that writes stay private. */
+GDNX_API gdnx_status gdnx_cache_extend(const gdnx_cache* cache, int64_t n, const int32_t* rows, const int32_t* counts,
+                                       void* workspace, size_t workspace_bytes, void* stream);
+/* k, v [n,T,Hk,D] become tokens length-count .. length-1 of slot rows[i] in `layer`
+ * (count = counts[i] <= T, or T where counts is NULL; further tokens of a row are ignored). */
+GDNX_API gdnx_status gdnx_cache_write(const gdnx_cache* cache, int64_t layer, int64_t n, int64_t T, const gdnx_view* k,
+                                      const gdnx_view* v, const int32_t* rows, const int32_t* counts, void* stream);
+/* Slot rows[i] keeps its first lengths[i] tokens (0 frees it). */
+GDNX_API gdnx_status gdnx_cache_truncate(const gdnx_cache* cache, int64_t n, const int32_t* rows,
+                                         const int32_t* lengths, void* stream);
+/* Releases the pages of slots rows[i] that hold no sink and nothing that the last token or
+ * a later one sees through `window`. */
+GDNX_API gdnx_status gdnx_cache_trim(const gdnx_cache* cache, int64_t n, const int32_t* rows, int64_t window,
+                                     int64_t sinks, void* stream);
+/* Moves the live pages at or above index n_live down into the free ones below it (in
+ * order), so that the n_live live pages are the pool's first. */
+GDNX_API gdnx_status gdnx_cache_compact(const gdnx_cache* cache, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of one new token per query row over a cache: row i of q reads slot rows[i],
+ * whose last token it is (the token's own key and value are written before the call).
+ * It sees token j < length where length - 1 - j < window or j < sinks; tokens on released
+ * pages are not seen.  A row that sees nothing (length 0, a slot out of range) gives 0.
+ * The visible tokens are split over CTAs, and the parts joined in a fixed order. */
+typedef struct {
+  gdnx_cache cache;
+  int64_t B, H, layer;
+  int64_t window, sinks;       /* window >= 1 */
+  int64_t max_len;             /* no slot is longer: sizes the split; 0 = width * page */
+  float scale;
+  gdnx_view q;                 /* [B,H,D] (sb, sh), the cache's type */
+  const int32_t* rows;         /* [B] device; NULL = slots 0..B-1 */
+  void* y;                     /* [B,H,D] */
+  int32_t y_dtype;
+  int64_t y_sb, y_sh;
+  int32_t* error;              /* device word that takes GDNX_ETIMEOUT; NULL = none */
+  void* workspace;
+  size_t workspace_bytes;
+} gdnx_paged_decode_args;
+
+GDNX_API size_t gdnx_paged_decode_workspace_bytes(const gdnx_paged_decode_args* args);
+GDNX_API gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* args, void* stream);
 
 GDNX_API const char* gdnx_status_string(gdnx_status s);
 

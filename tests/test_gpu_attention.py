@@ -1,0 +1,231 @@
+"""Windowed attention (``gdnx_attn_fwd`` / ``gdnx_attn_bwd``) against the 64-bit oracle.
+
+Tolerances (relative 2-norm).  fp32: a score is off by a few 2^-24 of its size (below 10), sums of n <= 1000
+terms by about sqrt(n) 2^-24: 1e-5 holds both with room.  16-bit types round the output once (rms 0.29 of a
+spacing: 1.7e-3 in bfloat16, 2.1e-4 in float16) and the weights once before the product with V, whose relative
+error is the same and independent: 2.4e-3 and 3e-4 together, twice that is allowed.  The gradients round P and
+dS, and read y rounded: four such errors, so again twice the forward's."""
+import pytest
+import torch
+
+from gdnx_b200 import _lib as L
+from gdnx_b200 import ops
+from oracle import attention as A
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+TOL = {"f32": 1e-5, "bf16": 5e-3, "f16": 6e-4}
+TOL_GRAD = {"f32": 2e-5, "bf16": 1e-2, "f16": 1.2e-3}
+
+
+def rel(a, b):
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    return ((a - b).norm() / b.norm().clamp_min(1e-30)).item()
+
+
+def make(B, Tq, Tk, H, Hk, D, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda T, h: torch.randn(B, T, h, D, generator=g).to(TYPES[dtype]).to(DEV)  # noqa: E731
+    return r(Tq, H), r(Tk, Hk), r(Tk, Hk), r(Tq, H)
+
+
+def check(q, k, v, dy, dtype, **mask):
+    """Forward, lse and gradients against the oracle."""
+    y, lse = ops.window_attention(q, k, v, return_lse=True, **mask)
+    yo, lo = A.window_attention(q, k, v, **mask)
+    assert y.dtype == q.dtype and rel(y, yo) < TOL[dtype]
+    seen = torch.isfinite(lo)
+    assert torch.equal(torch.isfinite(lse).cpu(), seen)
+    # the scores' own rounding: products of 16-bit values are exact in fp32
+    assert (lse.cpu().double()[seen] - lo[seen]).abs().max().item() < 1e-4 if seen.any() else True
+    if dy is None:
+        return
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    yt = ops.window_attention_train(q, k, v, **mask)
+    assert torch.equal(yt.detach(), y)
+    for x, g, go in zip((q, k, v), torch.autograd.grad(yt, (q, k, v), dy), A.window_attention_grads(q, k, v, dy, **mask)):
+        assert g.shape == x.shape and g.dtype == x.dtype
+        assert torch.isfinite(g).all()
+        assert rel(g, go) < TOL_GRAD[dtype] or go.norm() < 1e-12 and g.norm() < 1e-5
+
+
+SHAPES = [  # B, Tq, Tk, H, Hk, D, window, sinks
+    (1, 1, 1, 1, 1, 64, 1, 0),            # one token
+    (2, 1, 300, 4, 2, 64, 50, 3),         # one query at the end of a long sequence
+    (1, 130, 130, 2, 1, 128, 1, 0),       # a window of one: every query sees itself
+    (1, 200, 200, 2, 2, 128, 1, 5),       # and the sinks
+    (2, 257, 257, 4, 2, 64, 64, 4),       # one row past a tile
+    (1, 384, 384, 6, 3, 128, 100, 0),     # window edges inside tiles
+    (1, 500, 500, 2, 1, 96, 129, 130),    # sinks over more than one tile, a head size that is padded
+    (1, 300, 300, 5, 1, 80, 1000, 4),     # window beyond the sequence: plain causal
+    (2, 100, 421, 4, 4, 32, 333, 17),     # a continued prompt
+    (1, 129, 640, 16, 1, 128, 200, 64),   # 16 query heads of one key head
+    (1, 640, 640, 2, 1, 8, 200, 1000),    # sinks beyond the sequence; the smallest head
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_attention_and_gradients(shape, dtype):
+    B, Tq, Tk, H, Hk, D, window, sinks = shape
+    check(*make(B, Tq, Tk, H, Hk, D, dtype, seed=Tk), dtype, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Tq,Tk,D", [(260, 260, 128), (70, 260, 64)])
+def test_padding_holds_nan_and_reaches_nothing(Tq, Tk, D, dtype):
+    """Lengths 0, 1, inside a tile, a tile's edge and full; what lies beyond them is NaN."""
+    n = [0, 1, 128, 201, Tk, 64]
+    q, k, v, dy = make(len(n), Tq, Tk, 4, 2, D, dtype, seed=5)
+    for b, m in enumerate(n):
+        k[b, m:] = float("nan")
+        v[b, m:] = float("inf")
+        q[b, max(0, m - (Tk - Tq)):] = float("nan")
+        dy[b, max(0, m - (Tk - Tq)):] = float("nan")
+    lengths = torch.tensor(n, dtype=torch.int32, device=DEV)
+    check(q, k, v, dy, dtype, window=90, sinks=4, lengths=lengths)
+    y = ops.window_attention(q, k, v, window=90, sinks=4, lengths=lengths)
+    for b, m in enumerate(n):
+        assert (y[b, max(0, m - (Tk - Tq)):] == 0).all()
+
+
+def test_lengths_out_of_range_are_clamped():
+    q, k, v, _ = make(2, 40, 40, 2, 2, 64, "bf16")
+    y = ops.window_attention(q, k, v, lengths=torch.tensor([-3, 99], dtype=torch.int32, device=DEV))
+    assert (y[0] == 0).all() and torch.equal(y[1], ops.window_attention(q, k, v)[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_orders(dtype):
+    """Heads before tokens, a slice of a wider projection, an odd row stride, a shared batch."""
+    q, k, v, dy = make(2, 150, 150, 4, 2, 64, dtype, seed=3)
+    mask = dict(window=70, sinks=2)
+    want = ops.window_attention(q, k, v, **mask)
+    heads_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    assert torch.equal(ops.window_attention(*heads_first, **mask), want)
+    wide = torch.cat([q.flatten(2), k.flatten(2), v.flatten(2)], -1)
+    a = wide[..., :256].unflatten(2, (4, 64)), wide[..., 256:384].unflatten(2, (2, 64)), wide[..., 384:].unflatten(2, (2, 64))
+    assert torch.equal(ops.window_attention(*a, **mask), want)
+    check(*a, dy.transpose(1, 2).contiguous().transpose(1, 2), dtype, **mask)
+    odd = torch.empty(2, 150, 4, 67, dtype=q.dtype, device=DEV)[..., 1:65]
+    odd.copy_(q)
+    check(odd, k, v, dy, dtype, **mask)
+    check(q, k[:1].expand(2, -1, -1, -1), v[:, :, :1].expand(-1, -1, 2, -1), dy, dtype, **mask)
+
+
+def test_gradients_of_broadcast_inputs_are_summed():
+    q, k, v, dy = make(3, 90, 90, 4, 4, 64, "f32", seed=8)
+    k1, v1 = k[:1].detach().requires_grad_(), v[:, :, :1].detach().requires_grad_()
+    y = ops.window_attention_train(q, k1.expand(3, -1, -1, -1), v1.expand(-1, -1, 4, -1), window=30, sinks=2)
+    dk, dv = torch.autograd.grad(y, (k1, v1), dy)
+    _, gk, gv = A.window_attention_grads(q, k1.expand(3, -1, -1, -1), v1.expand(-1, -1, 4, -1), dy, window=30, sinks=2)
+    assert rel(dk, gk.sum(0, keepdim=True)) < 2e-5 and rel(dv, gv.sum(2, keepdim=True)) < 2e-5
+
+
+def test_gradient_of_a_sum_is_taken():
+    """A cotangent with stride 0 everywhere."""
+    q, k, v, _ = make(1, 50, 50, 2, 2, 64, "f32", seed=9)
+    v.requires_grad_()
+    ops.window_attention_train(q, k, v, window=20).sum().backward()
+    _, _, gv = A.window_attention_grads(q, k, v, torch.ones_like(q), window=20)
+    assert rel(v.grad, gv) < 2e-5
+
+
+def test_gradients_against_differences():
+    """fp32: the loss's change over +-h along random directions against the gradient's share in them.  With h = 1e-2
+    the third-order term is below h^2 = 1e-4 of the slope, the rounding of a loss of about 100 below 1e-5 / h."""
+    q, k, v, dy = make(1, 70, 70, 2, 1, 32, "f32", seed=11)
+    mask = dict(window=33, sinks=2)
+    xs = [t.detach().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.window_attention_train(*xs, **mask), xs, dy)
+    loss = lambda t: (ops.window_attention(*t, **mask).double() * dy.double()).sum().item()  # noqa: E731
+    h = 1e-2
+    for i, g in enumerate(grads):
+        e = torch.randn(g.shape, generator=torch.Generator().manual_seed(i)).to(DEV)
+        e = e / e.norm()
+        up, down = [q, k, v], [q, k, v]
+        up[i], down[i] = up[i] + h * e, down[i] - h * e
+        slope = (loss(up) - loss(down)) / (2 * h)
+        assert abs(slope - (g.double() * e.double()).sum().item()) < 2e-3 * g.double().norm().item()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_scores_and_scale(dtype):
+    """Scores of hundreds: the running maximum has to carry them."""
+    q, k, v, dy = make(1, 200, 200, 2, 1, 64, dtype, seed=12)
+    y = ops.window_attention(q * 8, k * 8, v, window=150, scale=0.5)
+    yo, _ = A.window_attention(q * 8, k * 8, v, window=150, scale=0.5)
+    # a score of 500 carries 500 2^-24 = 3e-5 into its weight
+    assert rel(y, yo) < max(TOL[dtype], 1e-4)
+
+
+def test_same_inputs_give_the_same_bits():
+    q, k, v, dy = make(2, 700, 700, 8, 2, 128, "bf16", seed=13)
+    runs = []
+    for _ in range(3):
+        xs = [t.detach().requires_grad_() for t in (q, k, v)]
+        y = ops.window_attention_train(*xs, window=200, sinks=4)
+        runs.append([y.detach(), *torch.autograd.grad(y, xs, dy)])
+    for other in runs[1:]:
+        for a, b in zip(runs[0], other):
+            assert torch.equal(a, b)
+
+
+def test_out_dtype_and_out():
+    q, k, v, _ = make(2, 150, 150, 4, 2, 128, "bf16", seed=14)
+    yo, _ = A.window_attention(q, k, v, window=60)
+    y32 = ops.window_attention(q, k, v, window=60, out_dtype=torch.float32)
+    assert y32.dtype == torch.float32 and rel(y32, yo) < TOL["bf16"]
+    buf = torch.full((2, 150, 4, 160), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = buf[..., 16:144]
+    assert ops.window_attention(q, k, v, window=60, out=out) is out
+    assert rel(out, yo) < TOL["bf16"] and (buf[..., :16] == 7).all() and (buf[..., 144:] == 7).all()
+    odd = torch.full((2, 150, 4, 131), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.window_attention(q, k, v, window=60, out=odd[..., 1:129])
+    assert rel(odd[..., 1:129], yo) < TOL["bf16"] and (odd[..., :1] == 7).all() and (odd[..., 129:] == 7).all()
+
+
+def test_on_another_stream():
+    q, k, v, _ = make(1, 300, 300, 4, 2, 64, "bf16", seed=15)
+    want = ops.window_attention(q, k, v, window=100)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y = ops.window_attention(q * 1, k, v, window=100)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(y, want)
+
+
+def test_empty_sizes():
+    q, k, v, _ = make(2, 3, 5, 2, 1, 64, "bf16")
+    assert ops.window_attention(q[:0], k[:0], v[:0]).shape == (0, 3, 2, 64)
+    assert ops.window_attention(q[:, :0], k[:, :0], v[:, :0]).shape == (2, 0, 2, 64)
+    xs = [t.detach().requires_grad_() for t in (q[:, :0], k, v)]
+    y = ops.window_attention_train(*xs)
+    dq, dk, dv = torch.autograd.grad(y, xs, torch.zeros_like(y))
+    assert dq.shape == (2, 0, 2, 64) and (dk == 0).all() and (dv == 0).all()
+
+
+def test_refusals():
+    q, k, v, _ = make(2, 8, 8, 4, 2, 64, "bf16")
+    bad = [dict(window=0), dict(sinks=-1), dict(lengths=torch.zeros(3, dtype=torch.int32, device=DEV)),
+           dict(lengths=torch.zeros(2, dtype=torch.int64, device=DEV)), dict(lengths=torch.zeros(2, dtype=torch.int32)),
+           dict(out=torch.empty(2, 8, 4, 32, dtype=q.dtype, device=DEV))]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            ops.window_attention(q, k, v, **kw)
+    for a in ((q, k[:, :4], v[:, :4]), (q, k[:1], v[:1]), (q[:, :, :3], k, v), (q, k, v[:, :4]), (q[0], k, v),
+              (q, k[..., :32], v[..., :32]), (q.transpose(2, 3), k, v)):
+        with pytest.raises(ValueError):
+            ops.window_attention(*a)
+    for a in ((q.float(), k, v), (q, k, v.half()), (q.double(), k.double(), v.double())):
+        with pytest.raises(TypeError):
+            ops.window_attention(*a)
+    with pytest.raises(L.GdnxError) as e:
+        ops.window_attention(q, k, v, scale=-1.0)
+    assert e.value.status == L.GDNX_EINVAL
+    wide = torch.zeros(1, 4, 1, 136, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(L.GdnxError) as e:
+        ops.window_attention(wide, wide, wide)
+    assert e.value.status == L.GDNX_EUNSUPPORTED
