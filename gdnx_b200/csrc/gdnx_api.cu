@@ -142,7 +142,13 @@ gdnx_status gdnx_attn_fwd(const gdnx_attn_args* a, void* stream) {
   if (!a) return GDNX_EINVAL;
   const gdnx_status s = check_attn(*a);
   if (s != GDNX_OK || a->B == 0 || a->Tq == 0) return s;
-  return gdnx::launch_attn_fwd_simt(clamp_attn(*a), (cudaStream_t)stream);
+  const gdnx_attn_args c = clamp_attn(*a);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (c.q.dtype != GDNX_F32) {
+    const gdnx_status t = gdnx::launch_attn_fwd_tc(c, st);
+    if (t != GDNX_EUNSUPPORTED) return t;
+  }
+  return gdnx::launch_attn_fwd_simt(c, st);
 }
 
 size_t gdnx_attn_bwd_workspace_bytes(const gdnx_attn_bwd_args* g) {

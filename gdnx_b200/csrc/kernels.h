@@ -16,6 +16,8 @@ gdnx_status launch_proj_prologue(const gdnx_prologue_args& a, cudaStream_t st);
 gdnx_status launch_kmd2_prologue(const gdnx_kmd2_prologue_args& a, cudaStream_t st);
 // Windowed attention (attn_simt.cu: CUDA cores, every type and layout) and its gradients.
 gdnx_status launch_attn_fwd_simt(const gdnx_attn_args& a, cudaStream_t st);
+// Tensor-core forward (attn_fwd.cu); GDNX_EUNSUPPORTED where TMA cannot address the operands.
+gdnx_status launch_attn_fwd_tc(const gdnx_attn_args& a, cudaStream_t st);
 gdnx_status launch_attn_delta(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st);
 gdnx_status launch_attn_bwd_simt(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st);
 // Paged cache (paged_cache.cu) and the attention that reads it (paged_decode.cu).
