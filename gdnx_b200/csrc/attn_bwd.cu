@@ -1,0 +1,688 @@
+// Windowed attention, gradients, on the tensor cores (16-bit inputs that TMA can address).
+//
+// Two kernels recompute P from lse and write every gradient once, in a fixed order: seven
+// products of a tile instead of five, against atomics (whose order would show in the bits)
+// or dQ partials of T x W / 128 fp32 rows.
+//   attn_dkv: 128 keys of a key head; over its query heads and the query tiles that see them
+//     S^T = K Q^T, dP^T = V dY^T; P^T = exp(c S^T - lse), dS^T = P^T (dP^T - delta) packed
+//     16-bit over the columns of S^T and dP^T; dV += P^T dY, dK += dS^T Q.
+//   attn_dq: 128 queries of a head; over the key tiles that they see
+//     S = Q K^T (two buffers), dP = dY V^T; dS over S's columns; dQ += dS K.
+// Accumulators stay in tensor memory (fp32).  Warpgroups 0 and 1 own the two halves of a
+// tile's columns (every lane's row in both), warp 8 issues the products, warp 9 the loads.
+// In attn_dkv dV(t) and S(t+1) run while the rows form dS(t), dK(t) and dP(t+1) while they
+// form P(t+1).
+//
+// A key tile that holds sinks is seen by every later query, far more than the others; its
+// iterations (and all tiles' where there are few) are cut into parts that leave fp32
+// partial sums, which attn_dkv_join adds in order.
+//
+// Weights and dS are rounded to bf16 for the products, like the inputs themselves; dS of
+// float16 inputs could leave float16's range, so those take the CUDA-core kernels.
+#include "attn_tc.cuh"
+#include "kernels.h"
+
+namespace gdnx {
+namespace {
+
+using namespace attn;
+
+constexpr int NTHREADS = 384;
+constexpr int SLOTS = 5;        // streamed tiles in flight
+constexpr uint32_t STAT = TM * 4;  // bytes of one statistic of a tile's queries
+
+struct BwdParams {
+  TileMap q, k, v, dy;
+  gdnx_attn_args a;
+  void *dq, *dk, *dv;
+  const float *lse2, *delta;  // [B,H,qpad]: log2-domain lse (+inf where padding) and delta (0)
+  float* part;                // partial dK, dV of cut tiles: [item][2][128][64 DB]
+  int qtiles, ktiles, nst;    // nst: key tiles that hold sinks
+  int seg_sink, seg;          // parts of such a tile and of the others
+};
+
+struct Bars {
+  uint64_t full[SLOTS], empty[SLOTS], res[2], stat_full[2], stat_empty[2], s_full[2], dp_full, p_ready, ds_ready[2],
+      dp_read, o_full, fix, done;
+};
+
+template <int DB>
+struct Layout {
+  static constexpr uint32_t TILE = DB * BLOCK_BYTES;
+  static constexpr uint32_t RES = 0, RING = 2 * TILE, STATS = RING + SLOTS * TILE, BARS = STATS + 4 * STAT,
+                            END = BARS + 512;
+  static constexpr size_t SMEM = END + 512;  // the base is 1024-aligned: there is no static shared memory
+};
+
+// Bits lo..hi (inclusive) of the 32-bit word that holds columns 32w..32w+31.
+GDNX_DEV uint32_t range_bits(int lo, int hi, int w) {
+  lo = max(lo - 32 * w, 0);
+  hi = min(hi - 32 * w, 31);
+  return lo > hi ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+}
+
+// D (+)= P X with P's columns in two halves, each over the start of its half of 128 columns.
+GDNX_DEV void mma_halves(uint32_t d, uint32_t p, uint32_t x, uint32_t idesc, bool acc) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    tc::mma_bf16_ts(d, p + (k < 4 ? 8 * k : 64 + 8 * (k - 4)), tc::smem_desc(x + k * 2048, BLOCK_BYTES, 1024), idesc,
+                    acc || k > 0);
+}
+
+// Rows r0.. of a landed tile to zero: padding rows meet weights of 0, so they must not hold NaN.
+template <int DB>
+GDNX_DEV void zero_rows(uint8_t* tile, int r0, int lane) {
+  for (int x = lane; x < (TM - r0) * DB * 8; x += 32) {
+    const int row = r0 + x / (DB * 8), c = x % (DB * 8);
+    *reinterpret_cast<uint4*>(tile + (c / 8) * BLOCK_BYTES + row * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+  }
+  tc::fence_async_smem();
+  __syncwarp();
+}
+
+// One streamed tile into the ring (whole warp): rows t0.. of head h, rows from `valid` on
+// (in the tensor's own rows, below `rows`) to zero.
+template <int DB>
+GDNX_DEV bool stream_tile(uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag, uint32_t cnt,
+                          const TileMap& m, int t0, int64_t h, int64_t b, int valid, int64_t rows, uint32_t& nfix) {
+  using Lo = Layout<DB>;
+  const uint32_t sl = cnt % SLOTS;
+  const int lane = threadIdx.x % 32;
+  if (!warp_wait(&bar.empty[sl], (cnt / SLOTS & 1) ^ 1, abort_flag)) return false;
+  const bool fix = valid < rows && t0 + TM > valid;
+  if (lane == 0) {
+    const uint32_t mb = tc::smem_u32(fix ? &bar.fix : &bar.full[sl]);
+    pipe::expect_tx(mb, Lo::TILE);
+    load_rows<DB>(smem + Lo::RING + sl * Lo::TILE, m, t0, h, b, mb);
+  }
+  if (fix) {
+    if (!warp_wait(&bar.fix, nfix++ & 1, abort_flag)) return false;
+    zero_rows<DB>(base + Lo::RING + sl * Lo::TILE, max(0, valid - t0), lane);
+    if (lane == 0) pipe::mbar_arrive(&bar.full[sl]);
+  }
+  return true;
+}
+
+GDNX_DEV void init_bars(Bars& bar) {
+  for (int i = 0; i < SLOTS; ++i) {
+    tc::mbar_init(&bar.full[i], 1);
+    tc::mbar_init(&bar.empty[i], 1);
+  }
+  for (int i = 0; i < 2; ++i) {
+    tc::mbar_init(&bar.res[i], 1);
+    tc::mbar_init(&bar.stat_full[i], 1);
+    tc::mbar_init(&bar.stat_empty[i], 256);
+    tc::mbar_init(&bar.s_full[i], 1);
+    tc::mbar_init(&bar.ds_ready[i], 256);
+  }
+  tc::mbar_init(&bar.dp_full, 1);
+  tc::mbar_init(&bar.p_ready, 256);
+  tc::mbar_init(&bar.dp_read, 256);
+  tc::mbar_init(&bar.o_full, 1);
+  tc::mbar_init(&bar.fix, 1);
+  tc::mbar_init(&bar.done, 1);
+}
+
+// 32 accumulator values of one row, scaled, to 16-bit or fp32 memory (columns below D only).
+template <bool F32>
+GDNX_DEV void store32(void* dst, int64_t at, const float* o, float scale, int left) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 8) {
+    if (e >= left) continue;
+    if (F32) {
+      float4* p = reinterpret_cast<float4*>(static_cast<float*>(dst) + at + e);
+      p[0] = make_float4(o[e] * scale, o[e + 1] * scale, o[e + 2] * scale, o[e + 3] * scale);
+      p[1] = make_float4(o[e + 4] * scale, o[e + 5] * scale, o[e + 6] * scale, o[e + 7] * scale);
+    } else {
+      uint4 u;
+      u.x = tc::pack_bf16(o[e] * scale, o[e + 1] * scale);
+      u.y = tc::pack_bf16(o[e + 2] * scale, o[e + 3] * scale);
+      u.z = tc::pack_bf16(o[e + 4] * scale, o[e + 5] * scale);
+      u.w = tc::pack_bf16(o[e + 6] * scale, o[e + 7] * scale);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(dst) + at + e) = u;
+    }
+  }
+}
+
+// ------------------------------- dK and dV -----------------------------------
+
+// One CTA's work: a key tile, and the part t0..t1-1 of its (query head, query tile) list.
+struct KeyItem {
+  int b, hk, kt, j0, len, seg, nseg, qlo, nq, t0, t1;
+};
+
+GDNX_DEV KeyItem key_item(const BwdParams& P) {
+  const gdnx_attn_args& a = P.a;
+  KeyItem w;
+  const int G = (int)(a.H / a.Hk), off = (int)(a.Tk - a.Tq), bh = (int)(a.B * a.Hk);
+  int n = blockIdx.x;
+  const int sink_items = bh * P.nst * P.seg_sink;
+  const bool sink = n < sink_items;
+  if (!sink) n -= sink_items;
+  w.nseg = sink ? P.seg_sink : P.seg;
+  const int who = n % bh;  // key heads side by side: their queries' tiles are shared in L2
+  n /= bh;
+  w.seg = n % w.nseg;
+  w.kt = n / w.nseg + (sink ? 0 : P.nst);
+  w.b = who / (int)a.Hk;
+  w.hk = who % (int)a.Hk;
+  w.j0 = w.kt * TM;
+  w.len = seq_len(a, w.b);
+  const int rows = min((int)a.Tq, w.len - off);
+  int hi = rows;
+  if (w.j0 >= a.sinks) hi = (int)min((int64_t)rows, (int64_t)w.j0 + TM - 1 + a.window - off);
+  w.qlo = max(w.j0 - off, 0) / TM;
+  w.nq = w.j0 < w.len ? max(0, (hi + TM - 1) / TM - w.qlo) : 0;
+  const int64_t all = (int64_t)G * w.nq;
+  w.t0 = (int)(all * w.seg / w.nseg);
+  w.t1 = (int)(all * (w.seg + 1) / w.nseg);
+  return w;
+}
+
+constexpr uint32_t K_S = 0, K_DP = 128, K_DV = 256, K_DK = 384;  // tensor-memory columns
+
+template <int DB>
+GDNX_DEV void keys_rows(const BwdParams& P, const KeyItem& w, const uint8_t* base, uint32_t tmem, Bars& bar,
+                        volatile int* abort_flag) {
+  using Lo = Layout<DB>;
+  const gdnx_attn_args& a = P.a;
+  const int r = threadIdx.x % 128, half = threadIdx.x / 128;
+  const uint32_t lane_at = (uint32_t)(r / 32 * 32) << 16;
+  const uint32_t tS = tmem + lane_at + K_S + half * 64, tP = tmem + lane_at + K_DP + half * 64;
+  const int off = (int)(a.Tk - a.Tq), window = (int)a.window, sinks = (int)a.sinks, len = w.len;
+  const float c2 = a.scale * kLog2e;
+  const int j = w.j0 + r;
+  const int last = j >= len ? -1 : (j < sinks ? len - 1 : (int)min((int64_t)len - 1, (int64_t)j + window - 1));
+  const bool none = window == 1 && sinks == 0;  // every query sees one key: dS is 0
+  for (int t = w.t0; t < w.t1; ++t) {
+    const uint32_t it = t - w.t0, ss = it & 1;
+    const int p0 = (w.qlo + t % w.nq) * TM + off + half * 64;  // position of this half's first column
+    const float* lse = reinterpret_cast<const float*>(base + Lo::STATS + ss * 2 * STAT) + half * 64;
+    const float* del = lse + TM;
+    if (!warp_wait(&bar.stat_full[ss], it / 2 & 1, abort_flag) || !warp_wait(&bar.s_full[0], it & 1, abort_flag)) return;
+    tc::fence_after();
+    float s[64];
+    tmem_ld64(tS, s);
+    const bool whole = p0 >= w.j0 + TM - 1 && p0 + 64 <= len && w.j0 + TM <= len &&
+                       (p0 + 63 - w.j0 < window || w.j0 + TM <= sinks);
+    uint32_t on[2] = {0xffffffffu, 0xffffffffu};
+#pragma unroll
+    for (int e = 0; e < 64; e += 4) {
+      const float4 z = *reinterpret_cast<const float4*>(lse + e);
+      s[e] = ex2(fmaf(s[e], c2, -z.x));
+      s[e + 1] = ex2(fmaf(s[e + 1], c2, -z.y));
+      s[e + 2] = ex2(fmaf(s[e + 2], c2, -z.z));
+      s[e + 3] = ex2(fmaf(s[e + 3], c2, -z.w));
+    }
+    if (!whole) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        on[q] = range_bits(j - p0, last - p0, q);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!(on[q] >> e & 1)) s[32 * q + e] = 0.f;
+      }
+      if (p0 == 0) on[0] &= ~1u;  // position 0 sees one key
+      if (none) on[0] = on[1] = 0;
+    }
+    uint32_t pk[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
+    tmem_st32u(tS, pk);
+    tc::fence_before();
+    pipe::mbar_arrive(&bar.p_ready);
+    if (!warp_wait(&bar.dp_full, it & 1, abort_flag)) return;
+    tc::fence_after();
+    float d[64];
+    tmem_ld64(tP, d);
+#pragma unroll
+    for (int e = 0; e < 64; e += 4) {
+      const float4 z = *reinterpret_cast<const float4*>(del + e);
+      s[e] *= d[e] - z.x;
+      s[e + 1] *= d[e + 1] - z.y;
+      s[e + 2] *= d[e + 2] - z.z;
+      s[e + 3] *= d[e + 3] - z.w;
+    }
+    if (!whole) {
+#pragma unroll
+      for (int e = 0; e < 64; ++e)
+        if (!(on[e / 32] >> (e % 32) & 1)) s[e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
+    tmem_st32u(tP, pk);
+    tc::fence_before();
+    pipe::mbar_arrive(&bar.ds_ready[0]);
+    pipe::mbar_arrive(&bar.stat_empty[ss]);
+  }
+  // warpgroup 0 writes dV, warpgroup 1 dK
+  if (w.t1 > w.t0) {
+    if (!warp_wait(&bar.o_full, 0, abort_flag)) return;
+    tc::fence_after();
+  }
+  const uint32_t tO = tmem + lane_at + (half ? K_DK : K_DV);
+  const float scale = half ? a.scale : 1.f;
+#pragma unroll
+  for (int d = 0; d < 2 * DB; ++d) {
+    float o[32];
+    if (w.t1 > w.t0) tc::tmem_ld32(tO + 32 * d, o);
+    else
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = 0.f;
+    if (w.nseg > 1) {
+      float* dst = P.part + ((int64_t)blockIdx.x * 2 + half) * TM * 64 * DB;
+      store32<true>(dst, (int64_t)r * 64 * DB + 32 * d, o, scale, 32);
+    } else if (j < a.Tk) {
+      store32<false>(half ? P.dk : P.dv, (((int64_t)w.b * a.Tk + j) * a.Hk + w.hk) * a.D + 32 * d, o, scale,
+                     (int)a.D - 32 * d);
+    }
+  }
+}
+
+template <int DB>
+GDNX_DEV void keys_products(const KeyItem& w, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+  using Lo = Layout<DB>;
+  constexpr uint32_t ID_S = idesc16(true, 128, 128, false, false), ID_O = idesc16(true, 128, 64 * DB, false, true);
+  const int n = w.t1 - w.t0;
+  const auto slot = [&](uint32_t c) { return smem + Lo::RING + c % SLOTS * Lo::TILE; };
+  const auto landed = [&](uint32_t c) { return pipe::wait_or_abort(&bar.full[c % SLOTS], c / SLOTS & 1, abort_flag); };
+  const auto scores = [&](int t) {
+    if (!landed(2 * t)) return false;
+    mma_abt<DB>(tmem + K_S, smem + Lo::RES, slot(2 * t), ID_S);
+    tc::commit(&bar.s_full[0]);
+    return true;
+  };
+  const auto dprobs = [&](int t) {
+    if (!landed(2 * t + 1)) return false;
+    mma_abt<DB>(tmem + K_DP, smem + Lo::RES + Lo::TILE, slot(2 * t + 1), ID_S);
+    tc::commit(&bar.dp_full);
+    return true;
+  };
+  if (n == 0) return;
+  if (!pipe::wait_or_abort(&bar.res[0], 0, abort_flag) || !scores(0)) return;
+  if (!pipe::wait_or_abort(&bar.res[1], 0, abort_flag) || !dprobs(0)) return;
+  for (int t = 0; t < n; ++t) {
+    if (!pipe::wait_or_abort(&bar.p_ready, t & 1, abort_flag)) return;
+    tc::fence_after();
+    mma_halves(tmem + K_DV, tmem + K_S, slot(2 * t + 1), ID_O, t > 0);
+    tc::commit(&bar.empty[(2 * t + 1) % SLOTS]);
+    if (t + 1 < n && !scores(t + 1)) return;
+    if (!pipe::wait_or_abort(&bar.ds_ready[0], t & 1, abort_flag)) return;
+    tc::fence_after();
+    mma_halves(tmem + K_DK, tmem + K_DP, slot(2 * t), ID_O, t > 0);
+    tc::commit(&bar.empty[(2 * t) % SLOTS]);
+    if (t + 1 < n && !dprobs(t + 1)) return;
+  }
+  tc::commit(&bar.o_full);
+}
+
+template <int DB>
+GDNX_DEV void keys_loads(const BwdParams& P, const KeyItem& w, uint8_t* base, uint32_t smem, Bars& bar,
+                         volatile int* abort_flag) {
+  using Lo = Layout<DB>;
+  const gdnx_attn_args& a = P.a;
+  const int lane = threadIdx.x % 32, G = (int)(a.H / a.Hk), off = (int)(a.Tk - a.Tq);
+  const int rows = min((int)a.Tq, w.len - off);
+  uint32_t nfix = 0;
+  if (w.t1 == w.t0) return;
+  if (lane == 0)
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t mb = tc::smem_u32(&bar.res[i]);
+      pipe::expect_tx(mb, Lo::TILE);
+      load_rows<DB>(smem + Lo::RES + i * Lo::TILE, i ? P.v : P.k, w.j0, w.hk, w.b, mb);
+    }
+  for (int t = w.t0; t < w.t1; ++t) {
+    const uint32_t it = t - w.t0, ss = it & 1;
+    const int h = w.hk * G + t / w.nq, qt = w.qlo + t % w.nq;
+    if (!stream_tile<DB>(base, smem, bar, abort_flag, 2 * it, P.q, qt * TM, h, w.b, rows, a.Tq, nfix)) return;
+    if (!warp_wait(&bar.stat_empty[ss], (it / 2 & 1) ^ 1, abort_flag)) return;
+    if (lane == 0) {
+      const uint32_t mb = tc::smem_u32(&bar.stat_full[ss]), dst = smem + Lo::STATS + ss * 2 * STAT;
+      const int64_t at = ((int64_t)w.b * a.H + h) * P.qtiles * TM + qt * TM;
+      pipe::expect_tx(mb, 2 * STAT);
+      pipe::bulk_load(dst, P.lse2 + at, STAT, mb);
+      pipe::bulk_load(dst + STAT, P.delta + at, STAT, mb);
+    }
+    if (!stream_tile<DB>(base, smem, bar, abort_flag, 2 * it + 1, P.dy, qt * TM, h, w.b, rows, a.Tq, nfix)) return;
+  }
+}
+
+// ---------------------------------- dQ ---------------------------------------
+
+struct QueryItem {
+  int b, h, hk, i0, p0, len;
+  KeyTiles kt;
+};
+
+GDNX_DEV QueryItem query_item(const BwdParams& P) {
+  const gdnx_attn_args& a = P.a;
+  int64_t n = blockIdx.x;
+  const int h = (int)(n % a.H);
+  n /= a.H;
+  const int b = (int)(n % a.B), qt = P.qtiles - 1 - (int)(n / a.B);  // those that see most first
+  const int off = (int)(a.Tk - a.Tq), len = seq_len(a, b);
+  return {b, h, h / (int)(a.H / a.Hk), qt * TM, qt * TM + off, len,
+          KeyTiles(qt * TM + off, min(qt * TM + TM, (int)a.Tq) - 1 + off, len, (int)a.window, (int)a.sinks, TM)};
+}
+
+constexpr uint32_t Q_S = 0, Q_DP = 256, Q_DQ = 384;  // S has two buffers
+
+template <int DB>
+GDNX_DEV void queries_rows(const BwdParams& P, const QueryItem& w, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+  const gdnx_attn_args& a = P.a;
+  const int r = threadIdx.x % 128, half = threadIdx.x / 128;
+  const uint32_t lane_at = (uint32_t)(r / 32 * 32) << 16;
+  const uint32_t tS = tmem + lane_at + Q_S + half * 64, tP = tmem + lane_at + Q_DP + half * 64;
+  const int window = (int)a.window, sinks = (int)a.sinks, len = w.len, p = w.p0 + r, i = w.i0 + r;
+  const float c2 = a.scale * kLog2e;
+  const int64_t at = ((int64_t)w.b * a.H + w.h) * P.qtiles * TM + i;
+  const float lse2 = P.lse2[at], del = P.delta[at];
+  const bool one = sees_one(p, window, sinks);
+  for (int t = 0; t < w.kt.count; ++t) {
+    const uint32_t buf = t & 1;
+    const int j0 = w.kt.tile(t) * TM, c0 = j0 + half * 64;  // this half's first key
+    if (!warp_wait(&bar.s_full[buf], t / 2 & 1, abort_flag)) return;
+    tc::fence_after();
+    float s[64];
+    tmem_ld64(tS + buf * 128, s);
+    const bool whole = c0 + 63 <= w.p0 && w.p0 + TM <= len && (w.p0 + TM - 1 - c0 < window || c0 + 64 <= sinks);
+#pragma unroll
+    for (int e = 0; e < 64; ++e) s[e] = ex2(fmaf(s[e], c2, -lse2));
+    if (!warp_wait(&bar.dp_full, t & 1, abort_flag)) return;
+    tc::fence_after();
+    float d[64];
+    tmem_ld64(tP, d);
+    tc::fence_before();
+    pipe::mbar_arrive(&bar.dp_read);
+#pragma unroll
+    for (int e = 0; e < 64; ++e) s[e] *= d[e] - del;
+    if (!whole) {
+      const int hi = p < len && !one ? p - c0 : -1;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t on = range_bits(p - window + 1 - c0, hi, q) | range_bits(0, min(sinks - 1 - c0, hi), q);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!(on >> e & 1)) s[32 * q + e] = 0.f;
+      }
+    }
+    uint32_t pk[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
+    tmem_st32u(tS + buf * 128, pk);
+    tc::fence_before();
+    pipe::mbar_arrive(&bar.ds_ready[buf]);
+  }
+  if (w.kt.count) {
+    if (!warp_wait(&bar.o_full, 0, abort_flag)) return;
+    tc::fence_after();
+  }
+#pragma unroll
+  for (int d = 0; d < DB; ++d) {  // each warpgroup takes half of the columns
+    float o[32];
+    const int c = 32 * (half * DB + d);
+    if (w.kt.count) tc::tmem_ld32(tmem + lane_at + Q_DQ + c, o);
+    else
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = 0.f;
+    if (i < a.Tq) store32<false>(P.dq, (((int64_t)w.b * a.Tq + i) * a.H + w.h) * a.D + c, o, a.scale, (int)a.D - c);
+  }
+}
+
+template <int DB>
+GDNX_DEV void queries_products(const QueryItem& w, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+  using Lo = Layout<DB>;
+  constexpr uint32_t ID_S = idesc16(true, 128, 128, false, false), ID_O = idesc16(true, 128, 64 * DB, false, true);
+  const int n = w.kt.count;
+  const auto slot = [&](uint32_t c) { return smem + Lo::RING + c % SLOTS * Lo::TILE; };
+  const auto landed = [&](uint32_t c) { return pipe::wait_or_abort(&bar.full[c % SLOTS], c / SLOTS & 1, abort_flag); };
+  const auto scores = [&](int t) {
+    if (!landed(2 * t)) return false;
+    mma_abt<DB>(tmem + Q_S + (t & 1) * 128, smem + Lo::RES, slot(2 * t), ID_S);
+    tc::commit(&bar.s_full[t & 1]);
+    return true;
+  };
+  const auto dprobs = [&](int t) {
+    if (!landed(2 * t + 1)) return false;
+    mma_abt<DB>(tmem + Q_DP, smem + Lo::RES + Lo::TILE, slot(2 * t + 1), ID_S);
+    tc::commit(&bar.dp_full);
+    tc::commit(&bar.empty[(2 * t + 1) % SLOTS]);
+    return true;
+  };
+  if (n == 0) return;
+  if (!pipe::wait_or_abort(&bar.res[0], 0, abort_flag) || !scores(0)) return;
+  if (!pipe::wait_or_abort(&bar.res[1], 0, abort_flag) || !dprobs(0)) return;
+  if (n > 1 && !scores(1)) return;
+  for (int t = 0; t < n; ++t) {
+    if (t + 1 < n) {
+      if (!pipe::wait_or_abort(&bar.dp_read, t & 1, abort_flag)) return;
+      tc::fence_after();
+      if (!dprobs(t + 1)) return;
+    }
+    if (!pipe::wait_or_abort(&bar.ds_ready[t & 1], t / 2 & 1, abort_flag)) return;
+    tc::fence_after();
+    mma_halves(tmem + Q_DQ, tmem + Q_S + (t & 1) * 128, slot(2 * t), ID_O, t > 0);
+    tc::commit(&bar.empty[(2 * t) % SLOTS]);
+    if (t + 2 < n && !scores(t + 2)) return;
+  }
+  tc::commit(&bar.o_full);
+}
+
+template <int DB>
+GDNX_DEV void queries_loads(const BwdParams& P, const QueryItem& w, uint8_t* base, uint32_t smem, Bars& bar,
+                            volatile int* abort_flag) {
+  using Lo = Layout<DB>;
+  const gdnx_attn_args& a = P.a;
+  uint32_t nfix = 0;
+  if (w.kt.count == 0) return;
+  if (threadIdx.x % 32 == 0)
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t mb = tc::smem_u32(&bar.res[i]);
+      pipe::expect_tx(mb, Lo::TILE);
+      load_rows<DB>(smem + Lo::RES + i * Lo::TILE, i ? P.dy : P.q, w.i0, w.h, w.b, mb);
+    }
+  for (int t = 0; t < w.kt.count; ++t) {
+    const int j0 = w.kt.tile(t) * TM;
+    // K is also the right factor of dS K: its padding rows must not hold NaN
+    if (!stream_tile<DB>(base, smem, bar, abort_flag, 2 * t, P.k, j0, w.hk, w.b, w.len, a.Tk, nfix) ||
+        !stream_tile<DB>(base, smem, bar, abort_flag, 2 * t + 1, P.v, j0, w.hk, w.b, (int)a.Tk, a.Tk, nfix))
+      return;
+  }
+}
+
+// The frame of both kernels.
+template <int DB, bool KEYS>
+__global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_constant__ BwdParams P) {
+  using Lo = Layout<DB>;
+  extern __shared__ __align__(1024) uint8_t base[];
+  Bars& bar = *reinterpret_cast<Bars*>(base + Lo::BARS);
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(base + Lo::BARS + 448);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(base + Lo::BARS + 452);
+  static_assert(sizeof(Bars) <= 448, "barriers fit their place");
+  const uint32_t smem = tc::smem_u32(base);
+  const int warp = threadIdx.x / 32;
+  if (threadIdx.x == 0) {
+    *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
+    init_bars(bar);
+  }
+  if (warp == 8) tc::tmem_alloc(tmem_at, 512);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_at;
+  if (smem % 1024 == 0) {
+    if (KEYS) {
+      const KeyItem w = key_item(P);
+      if (warp < 8) keys_rows<DB>(P, w, base, tmem, bar, abort_flag);
+      else if (warp == 8 && threadIdx.x % 32 == 0) keys_products<DB>(w, smem, tmem, bar, abort_flag);
+      else if (warp == 9) keys_loads<DB>(P, w, base, smem, bar, abort_flag);
+    } else {
+      const QueryItem w = query_item(P);
+      if (warp < 8) queries_rows<DB>(P, w, tmem, bar, abort_flag);
+      else if (warp == 8 && threadIdx.x % 32 == 0) queries_products<DB>(w, smem, tmem, bar, abort_flag);
+      else if (warp == 9) queries_loads<DB>(P, w, base, smem, bar, abort_flag);
+    }
+  }
+  if (warp == 8 && threadIdx.x % 32 == 0) {  // every product issued has ended
+    tc::commit(&bar.done);
+    tc::mbar_wait(&bar.done, 0);
+  }
+  if (warp == 9 && *abort_flag)  // let the copies in flight land
+    for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 8) tc::tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
+}
+
+// Sums of cut tiles' parts: one thread for each (tile, key, value).
+template <int DB>
+__global__ void __launch_bounds__(256) attn_dkv_join_kernel(const BwdParams P, int first, int tiles) {
+  const gdnx_attn_args& a = P.a;
+  const int bh = (int)(a.B * a.Hk), W = 64 * DB, nseg = first == 0 && P.nst > 0 ? P.seg_sink : P.seg;
+  const int64_t item0 = first == 0 ? 0 : (int64_t)bh * P.nst * P.seg_sink;
+  const int64_t all = (int64_t)tiles * bh * 2 * TM * W;
+  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
+    const int d = (int)(x % W), r = (int)(x / W % TM), side = (int)(x / (W * TM) % 2);
+    const int who = (int)(x / (2 * W * TM) % bh), tile = (int)(x / ((int64_t)2 * W * TM * bh));
+    const int64_t j = (int64_t)(first + tile) * TM + r;
+    if (j >= a.Tk || d >= a.D) continue;
+    float sum = 0.f;
+    for (int s = 0; s < nseg; ++s)
+      sum += P.part[(((item0 + ((int64_t)tile * nseg + s) * bh + who) * 2 + side) * TM + r) * W + d];
+    st_from_f32(side ? P.dk : P.dv, GDNX_BF16, ((who / a.Hk * a.Tk + j) * a.Hk + who % a.Hk) * a.D + d, sum);
+  }
+}
+
+// lse in the log2 domain and delta = sum_d dy y, padded to whole tiles of queries: eight lanes
+// for each row.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_stats_kernel(const gdnx_attn_bwd_args g, float* lse2, float* delta,
+                                                         int qpad) {
+  const gdnx_attn_args& a = g.fwd;
+  const int64_t n = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
+  if (n >= a.B * a.H * qpad) return;  // whole groups of eight
+  const int64_t i = n % qpad, h = n / qpad % a.H, b = n / qpad / a.H;
+  const bool on = i < a.Tq && i + a.Tk - a.Tq < seq_len(a, b);
+  float s = 0.f;
+  if (on) {
+    const uint16_t* y = static_cast<const uint16_t*>(a.y) + b * a.y_sb + i * a.y_st + h * a.y_sh;
+    const uint16_t* dy = static_cast<const uint16_t*>(g.dy.ptr) + b * g.dy.sb + i * g.dy.st + h * g.dy.sh;
+    for (int d = threadIdx.x % 8 * 8; d < a.D; d += 64) {
+      const uint4 u = *reinterpret_cast<const uint4*>(y + d), v = *reinterpret_cast<const uint4*>(dy + d);
+      const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s = fmaf(__uint_as_float(uw[e] << 16), __uint_as_float(vw[e] << 16), s);
+        s = fmaf(__uint_as_float(uw[e] & 0xffff0000u), __uint_as_float(vw[e] & 0xffff0000u), s);
+      }
+    }
+  }
+  const uint32_t mask = 0xffu << (threadIdx.x % 32 / 8 * 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(mask, s, o);
+  if (threadIdx.x % 8 == 0) {
+    lse2[n] = on ? a.lse[(b * a.H + h) * a.Tq + i] * kLog2e : INFINITY;
+    delta[n] = s;
+  }
+}
+
+// How the key tiles' iterations are cut: a part is about a full SM's share of all of them, at
+// least eight iterations; tiles that hold sinks are cut to the others' length.
+void plan(BwdParams& P) {
+  const gdnx_attn_args& a = P.a;
+  const int64_t G = a.H / a.Hk, bh = a.B * a.Hk;
+  P.qtiles = (int)((a.Tq + TM - 1) / TM);
+  P.ktiles = (int)((a.Tk + TM - 1) / TM);
+  P.nst = (int)((a.sinks + TM - 1) / TM);
+  int64_t near = (a.window + TM - 1) / TM + 1;
+  if (near > P.qtiles) near = P.qtiles;
+  const int64_t it = G * near, it_sink = G * P.qtiles;
+  const int64_t total = bh * (P.nst * it_sink + (P.ktiles - P.nst) * it);
+  int64_t share = (total + 147) / 148;
+  if (share < 8) share = 8;
+  if (share > it) share = it > 8 ? it : 8;
+  const auto cut = [&](int64_t n) {
+    const int64_t s = (n + share - 1) / share;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+  };
+  P.seg = cut(it);
+  P.seg_sink = cut(it_sink);
+}
+
+size_t stats_floats(const BwdParams& P) { return (size_t)P.a.B * P.a.H * P.qtiles * TM; }
+
+int64_t items_of(const BwdParams& P) {
+  return P.a.B * P.a.Hk * ((int64_t)P.nst * P.seg_sink + (int64_t)(P.ktiles - P.nst) * P.seg);
+}
+
+// Floats of partial sums: the cut tiles' items come first in the grid where only sinks are cut.
+size_t part_floats(const BwdParams& P) {
+  const size_t one = (size_t)2 * TM * (P.a.D > 64 ? 128 : 64);
+  if (P.seg > 1) return (size_t)items_of(P) * one;
+  return P.seg_sink > 1 ? (size_t)P.a.B * P.a.Hk * P.nst * P.seg_sink * one : 0;
+}
+
+template <int DB>
+gdnx_status run(const gdnx_attn_bwd_args& g, BwdParams& P, cudaStream_t st) {
+  const gdnx_attn_args& a = P.a;
+  const auto keys = attn_bwd_tc_kernel<DB, true>;
+  const auto queries = attn_bwd_tc_kernel<DB, false>;
+  constexpr int smem = (int)Layout<DB>::SMEM;
+  if (cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return GDNX_ELAUNCH;
+  }
+  const int64_t rows = (int64_t)stats_floats(P);
+  attn_stats_kernel<__nv_bfloat16><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(
+      g, const_cast<float*>(P.lse2), const_cast<float*>(P.delta), P.qtiles * TM);
+  keys<<<(unsigned)items_of(P), NTHREADS, smem, st>>>(P);
+  const int bh = (int)(a.B * a.Hk);
+  const auto join = [&](int first, int tiles) {
+    const int64_t blocks = ((int64_t)tiles * bh * 2 * TM * 64 * DB + 255) / 256;
+    attn_dkv_join_kernel<DB><<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st>>>(P, first, tiles);
+  };
+  if (P.nst > 0 && P.seg_sink > 1) join(0, P.nst);
+  if (P.ktiles > P.nst && P.seg > 1) join(P.nst, P.ktiles - P.nst);
+  queries<<<(unsigned)((int64_t)P.qtiles * a.B * a.H), NTHREADS, smem, st>>>(P);
+  return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
+}
+
+}  // namespace
+
+size_t attn_bwd_tc_workspace_bytes(const gdnx_attn_args& a) {
+  BwdParams P;
+  P.a = a;
+  plan(P);
+  return (2 * stats_floats(P) + part_floats(P)) * sizeof(float);
+}
+
+gdnx_status launch_attn_bwd_tc(const gdnx_attn_bwd_args& g, cudaStream_t st) {
+  const gdnx_attn_args& a = g.fwd;
+  const auto wide = [](const void* p, int64_t b, int64_t t, int64_t h) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && b % 8 == 0 && t % 8 == 0 && h % 8 == 0;
+  };
+  if (a.q.dtype != GDNX_BF16 || a.y_dtype != GDNX_BF16 || !wide(a.y, a.y_sb, a.y_st, a.y_sh) ||
+      !wide(g.dy.ptr, g.dy.sb, g.dy.st, g.dy.sh) || !wide(g.dq, 0, 0, 0) || !wide(g.dk, 0, 0, 0) ||
+      !wide(g.dv, 0, 0, 0) || !wide(g.workspace, 0, 0, 0))
+    return GDNX_EUNSUPPORTED;
+  BwdParams P;
+  if (!make_tile_map(a.q, a.B, a.Tq, a.H, a.D, &P.q) || !make_tile_map(a.k, a.B, a.Tk, a.Hk, a.D, &P.k) ||
+      !make_tile_map(a.v, a.B, a.Tk, a.Hk, a.D, &P.v) || !make_tile_map(g.dy, a.B, a.Tq, a.H, a.D, &P.dy))
+    return GDNX_EUNSUPPORTED;
+  P.a = a;
+  P.dq = g.dq;
+  P.dk = g.dk;
+  P.dv = g.dv;
+  plan(P);
+  float* ws = static_cast<float*>(g.workspace);
+  P.lse2 = ws;
+  P.delta = ws + stats_floats(P);
+  P.part = ws + 2 * stats_floats(P);
+  return a.D > 64 ? run<2>(g, P, st) : run<1>(g, P, st);
+}
+
+}  // namespace gdnx

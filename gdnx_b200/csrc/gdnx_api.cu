@@ -88,12 +88,17 @@ bool heads_ok(const gdnx_view& v, int dtype, int64_t D) {
   return is_device_ptr(v.ptr) && v.dtype == dtype && v.dim == D && v.sb >= 0 && v.st >= 0 && v.sh >= 0;
 }
 
-gdnx_status check_attn(const gdnx_attn_args& a) {
+gdnx_status check_attn_sizes(const gdnx_attn_args& a) {
   if (a.B < 0 || a.Tq < 0 || a.Tk < a.Tq || a.H <= 0 || a.Hk <= 0 || a.D <= 0) return GDNX_EINVAL;
   if (a.H % a.Hk || a.window < 1 || a.sinks < 0) return GDNX_EINVAL;
   if (!(a.scale > 0.f) || a.scale > 3.0e38f || !dtype_ok(a.q.dtype) || !dtype_ok(a.y_dtype)) return GDNX_EINVAL;
   if (a.D > 128 || a.D % 8 || a.Tk > kMaxTokens || a.B > 65535 || a.H > 65535) return GDNX_EUNSUPPORTED;
-  if (a.B == 0 || a.Tk == 0) return GDNX_OK;
+  return GDNX_OK;
+}
+
+gdnx_status check_attn(const gdnx_attn_args& a) {
+  const gdnx_status s = check_attn_sizes(a);
+  if (s != GDNX_OK || a.B == 0 || a.Tk == 0) return s;
   if (!heads_ok(a.k, a.q.dtype, a.D) || !heads_ok(a.v, a.q.dtype, a.D)) return GDNX_EINVAL;
   if (a.Tq > 0 && (!heads_ok(a.q, a.q.dtype, a.D) || !is_device_ptr(a.y))) return GDNX_EINVAL;
   if (a.y_sb < 0 || a.y_st < 0 || a.y_sh < 0) return GDNX_EINVAL;
@@ -152,7 +157,8 @@ gdnx_status gdnx_attn_fwd(const gdnx_attn_args* a, void* stream) {
 }
 
 size_t gdnx_attn_bwd_workspace_bytes(const gdnx_attn_bwd_args* g) {
-  if (!g || g->fwd.B <= 0 || g->fwd.Tq <= 0 || g->fwd.H <= 0) return 0;
+  if (!g || check_attn_sizes(g->fwd) != GDNX_OK || g->fwd.B == 0 || g->fwd.Tq == 0) return 0;
+  if (g->fwd.q.dtype == GDNX_BF16) return gdnx::attn_bwd_tc_workspace_bytes(clamp_attn(g->fwd));
   return (size_t)(g->fwd.B * g->fwd.H * g->fwd.Tq) * sizeof(float);
 }
 
@@ -172,6 +178,10 @@ gdnx_status gdnx_attn_bwd(const gdnx_attn_bwd_args* g, void* stream) {
   if (g->workspace_bytes < gdnx_attn_bwd_workspace_bytes(g) || !is_device_ptr(g->workspace)) return GDNX_EWORKSPACE;
   gdnx_attn_bwd_args c = *g;
   c.fwd = clamp_attn(a);
+  if (a.q.dtype == GDNX_BF16) {
+    const gdnx_status t = gdnx::launch_attn_bwd_tc(c, st);
+    if (t != GDNX_EUNSUPPORTED) return t;
+  }
   float* delta = static_cast<float*>(g->workspace);
   const gdnx_status d = gdnx::launch_attn_delta(c, delta, st);
   return d != GDNX_OK ? d : gdnx::launch_attn_bwd_simt(c, delta, st);

@@ -18,6 +18,9 @@ gdnx_status launch_kmd2_prologue(const gdnx_kmd2_prologue_args& a, cudaStream_t 
 gdnx_status launch_attn_fwd_simt(const gdnx_attn_args& a, cudaStream_t st);
 // Tensor-core forward (attn_fwd.cu); GDNX_EUNSUPPORTED where TMA cannot address the operands.
 gdnx_status launch_attn_fwd_tc(const gdnx_attn_args& a, cudaStream_t st);
+// Tensor-core gradients of bfloat16 inputs (attn_bwd.cu); GDNX_EUNSUPPORTED likewise.
+size_t attn_bwd_tc_workspace_bytes(const gdnx_attn_args& a);
+gdnx_status launch_attn_bwd_tc(const gdnx_attn_bwd_args& g, cudaStream_t st);
 gdnx_status launch_attn_delta(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st);
 gdnx_status launch_attn_bwd_simt(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st);
 // Paged cache (paged_cache.cu) and the attention that reads it (paged_decode.cu).
