@@ -30,6 +30,7 @@ GDNX_DEV int seq_len(const gdnx_attn_args& a, int64_t b) {
 // then the window's own.
 struct KeyTiles {
   int nsink, lo, count;
+  GDNX_DEV KeyTiles() : nsink(0), lo(0), count(0) {}
   GDNX_DEV KeyTiles(int p0, int p1, int len, int window, int sinks, int BK) {
     const int last = min(p1, len - 1);
     if (p0 >= len || last < 0) {

@@ -248,7 +248,7 @@ static gdnx_paged_decode_args clamp_decode(const gdnx_paged_decode_args& a) {
 static gdnx_status check_decode(const gdnx_paged_decode_args& a) {
   const gdnx_status s = check_cache(&a.cache);
   if (s != GDNX_OK) return s;
-  if (a.B < 0 || a.H <= 0 || a.H % a.cache.Hk || a.layer < 0 || a.layer >= a.cache.L || a.window < 1 || a.sinks < 0 ||
+  if (a.cache.pages < 1 || a.B < 0 || a.H <= 0 || a.H % a.cache.Hk || a.layer < 0 || a.layer >= a.cache.L || a.window < 1 || a.sinks < 0 ||
       a.max_len < 0 || !(a.scale > 0.f) || a.scale > 3.0e38f || !dtype_ok(a.y_dtype))
     return GDNX_EINVAL;
   if (a.B > 65535 || a.H > 65535) return GDNX_EUNSUPPORTED;
@@ -262,7 +262,9 @@ static gdnx_status check_decode(const gdnx_paged_decode_args& a) {
 
 size_t gdnx_paged_decode_workspace_bytes(const gdnx_paged_decode_args* a) {
   if (!a || a->B <= 0 || a->H <= 0 || a->cache.Hk <= 0 || a->window < 1 || a->sinks < 0) return 0;
-  return gdnx::paged_decode_workspace_bytes(clamp_decode(*a));
+  if (check_cache(&a->cache) != GDNX_OK || a->H % a->cache.Hk) return 0;
+  const gdnx_paged_decode_args c = clamp_decode(*a);
+  return c.cache.dtype == GDNX_F32 ? gdnx::paged_decode_workspace_bytes(c) : gdnx::paged_decode_tc_workspace_bytes(c);
 }
 
 gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* a, void* stream) {
@@ -271,7 +273,9 @@ gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* a, void* stream) {
   if (s != GDNX_OK || a->B == 0) return s;
   const size_t need = gdnx_paged_decode_workspace_bytes(a);
   if (need && (a->workspace_bytes < need || !is_device_ptr(a->workspace))) return GDNX_EWORKSPACE;
-  return gdnx::launch_paged_decode(clamp_decode(*a), (cudaStream_t)stream);
+  const gdnx_paged_decode_args c = clamp_decode(*a);
+  return c.cache.dtype == GDNX_F32 ? gdnx::launch_paged_decode(c, (cudaStream_t)stream)
+                                   : gdnx::launch_paged_decode_tc(c, (cudaStream_t)stream);
 }
 
 const char* gdnx_status_string(gdnx_status s) {

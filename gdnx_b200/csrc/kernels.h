@@ -37,6 +37,9 @@ gdnx_status launch_cache_trim(const gdnx_cache& c, int64_t n, const int32_t* row
 gdnx_status launch_cache_compact(const gdnx_cache& c, void* ws, cudaStream_t st);
 size_t paged_decode_workspace_bytes(const gdnx_paged_decode_args& a);
 gdnx_status launch_paged_decode(const gdnx_paged_decode_args& a, cudaStream_t st);
+// 16-bit caches, on the tensor cores (paged_decode_tc.cu).
+size_t paged_decode_tc_workspace_bytes(const gdnx_paged_decode_args& a);
+gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t st);
 // Backward of the dense scan (scan_backward.cu).
 bool scan_bwd_supported(const gdnx_scan_bwd_args& a);
 size_t scan_bwd_workspace_bytes(const gdnx_scan_bwd_args& a);

@@ -1,4 +1,5 @@
-// Attention of one new token per sequence over a paged key/value cache.
+// Attention of one new token per sequence over a paged key/value cache of 32-bit values, on
+// the CUDA cores (all arithmetic fp32).
 //
 //   y = sum_j softmax_j(scale q.k_j) v_j   over the visible tokens j of the slot.
 // The visible tokens are walked in tiles of 64 positions, split evenly over the CTAs of one
@@ -22,35 +23,11 @@ constexpr int WARPS = NT / 32;
 constexpr int GB = 4;         // query heads of one CTA
 constexpr int MAX_SPLITS = 128;
 
-// Eight consecutive values as fp32.
-template <typename T>
-GDNX_DEV void load8(float (&x)[8], const T* p);
-template <>
-GDNX_DEV void load8<float>(float (&x)[8], const float* p) {
+// Eight consecutive values.
+GDNX_DEV void load8(float (&x)[8], const float* p) {
   const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
   x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
   x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-template <>
-GDNX_DEV void load8<__nv_bfloat16>(float (&x)[8], const __nv_bfloat16* p) {
-  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-template <>
-GDNX_DEV void load8<__half>(float (&x)[8], const __half* p) {
-  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-  }
 }
 
 struct Dec {
@@ -68,7 +45,7 @@ GDNX_DEV int dec_length(const Dec& P, int64_t b, int& row) {
   return (int)(n < 0 ? 0 : (n > most ? most : n));
 }
 
-template <int LPK, typename T>  // lanes per key: 8 (D <= 64) or 16 (D <= 128)
+template <int LPK>  // lanes per key: 8 (D <= 64) or 16 (D <= 128)
 __global__ void __launch_bounds__(NT) paged_decode_kernel(const Dec P) {
   constexpr int KPW = 32 / LPK;              // tokens of one pass of a warp
   constexpr int PASSES = TILE / WARPS / KPW;  // passes of a warp over its part of a tile
@@ -100,9 +77,9 @@ __global__ void __launch_bounds__(NT) paged_decode_kernel(const Dec P) {
                     : 0.f;
     }
   }
-  const T* kv = reinterpret_cast<const T*>(c.kv);
+  const float* kv = static_cast<const float*>(c.kv);
   const int64_t side = c.pages * c.Hk * page * D;  // one layer's keys or values
-  const T* kbase = kv + a.layer * 2 * side + hk * page * D + dl * 8;
+  const float* kbase = kv + a.layer * 2 * side + hk * page * D + dl * 8;
   const int32_t* table = c.table + (int64_t)row * c.width;
   for (int t = t0; t < t1; ++t) {
     const int j0 = kt.tile(t) * TILE + warp * (TILE / WARPS) + sub;
@@ -243,20 +220,8 @@ gdnx_status launch_paged_decode(const gdnx_paged_decode_args& a, cudaStream_t st
   P.part = static_cast<float*>(a.workspace);
   P.stat = P.part + a.B * a.H * P.splits * a.cache.D;
   const dim3 grid((unsigned)P.splits, (unsigned)(a.cache.Hk * P.groups), (unsigned)a.B);
-  const bool wide = a.cache.D > 64;
-  switch (a.cache.dtype) {
-    case GDNX_BF16:
-      if (wide) paged_decode_kernel<16, __nv_bfloat16><<<grid, NT, 0, st>>>(P);
-      else paged_decode_kernel<8, __nv_bfloat16><<<grid, NT, 0, st>>>(P);
-      break;
-    case GDNX_F16:
-      if (wide) paged_decode_kernel<16, __half><<<grid, NT, 0, st>>>(P);
-      else paged_decode_kernel<8, __half><<<grid, NT, 0, st>>>(P);
-      break;
-    default:
-      if (wide) paged_decode_kernel<16, float><<<grid, NT, 0, st>>>(P);
-      else paged_decode_kernel<8, float><<<grid, NT, 0, st>>>(P);
-  }
+  if (a.cache.D > 64) paged_decode_kernel<16><<<grid, NT, 0, st>>>(P);
+  else paged_decode_kernel<8><<<grid, NT, 0, st>>>(P);
   if (cudaGetLastError() != cudaSuccess) return GDNX_ELAUNCH;
   if (P.splits > 1) {
     paged_decode_join_kernel<<<(unsigned)(a.B * a.H), 128, 0, st>>>(P);

@@ -1,0 +1,612 @@
+// Attention of one new token per sequence over a paged cache, on the tensor cores (16-bit
+// caches).  The bytes of K and V bound it; the products only have to keep out of their way.
+//
+// Work.  A unit is one sequence and key head (and group of up to NH of its query heads); its
+// visible tokens are walked in tiles of 128 positions.  All units' tiles in a row are cut
+// evenly over the CTAs (one on each SM), so that mixed lengths leave none waiting: a CTA takes
+// the end of one unit, whole units, the beginning of another.  Whole units are written at
+// once; parts leave maximum, sum and unnormalised output, and a second kernel joins them in
+// order.  Every CTA finds its range from the lengths by itself.
+//
+// A tile.  With the keys as rows the products are narrow and nothing is padded to 128 but the
+// heads to NH:  S^T [128 keys x NH] = K Q^T,  O^T [128 dims x NH] += V^T P  (V read with its
+// rows as K; of head sizes up to 64 lanes 64.. read shifted rows and are not used).  Thread j owns key j: p_h = 2^(c s_jh - m_h), written 16-bit to shared memory as the
+// right factor.  The maxima m are those of the first tile and move only when some score lies
+// more than 8 above (p stays below 2^8), so a tile costs one vote and no reduction; sums stay
+// in the threads until the unit ends.
+//
+// Pages come by TMA, one box for each page and 64 dims; pages that hold nothing visible are not
+// fetched.  Rows that are not visible are masked in S and zeroed in V, since what unwritten
+// and released pages hold may be NaN.
+#include "attn_tc.cuh"
+#include "kernels.h"
+
+namespace gdnx {
+namespace {
+
+using namespace attn;
+
+constexpr int NTHREADS = 192;   // four warps of keys, one that issues products, one that loads
+
+struct DecParams {
+  CUtensorMap kv;  // {D, Hk * page, L * 2 * pages}
+  gdnx_paged_decode_args a;
+  float* part;     // [grid][2][NH][128] unnormalised outputs of a CTA's first and last unit
+  float* stat;     // [grid][2][NH][2] maximum (log2 domain) and sum
+  int grid, groups;
+  int vec_q;       // q's rows are 16-byte aligned
+};
+
+struct Bars {
+  uint64_t full[12], empty[12], q_ready[2], s_full[2], p_ready[2], pv_done, done;
+};
+
+// The place of a CTA in the row of all tiles: its tiles t0..t1-1, the sequence b that holds t0
+// and the tiles of the sequences before b.  Tiles are ordered by sequence, unit, tile.
+struct Range {
+  int64_t t0, t1, before, b;
+};
+
+template <int NH>
+struct Small {
+  Bars bar;
+  Range range;
+  float red[4 * NH];
+  uint32_t tmem_at;
+  int abort_flag;
+};
+
+template <int DB, int NH>
+struct Layout {
+  static constexpr int SLOTS = DB == 2 ? 6 : 12;  // K and V tiles in flight
+  static constexpr uint32_t TILE = DB * BLOCK_BYTES;
+  static constexpr uint32_t QB = DB * NH * 128, PB = 2 * NH * 128;  // a Q tile, a P tile
+  static constexpr uint32_t RING = 0, Q = SLOTS * TILE, P = Q + 2 * QB, SMALL = P + 2 * PB;
+  // no static shared memory: the base is 1024-aligned
+  static constexpr size_t SMEM = SMALL + sizeof(Small<NH>);
+  static constexpr int TMEM = NH == 16 ? 64 : 128;  // columns: S twice, O
+};
+
+// Visible tokens of one sequence.
+struct Seq {
+  int row, len;
+  KeyTiles kt;
+};
+
+GDNX_DEV int slot_length(const gdnx_paged_decode_args& a, int64_t b, int& row) {
+  const gdnx_cache& c = a.cache;
+  row = a.rows ? a.rows[b] : (int)b;
+  if (row < 0 || row >= c.slots) return 0;
+  const int64_t n = c.lengths[row], most = c.width * c.page;
+  return (int)(n < 0 ? 0 : (n > most ? most : n));
+}
+
+GDNX_DEV Seq make_seq(const gdnx_paged_decode_args& a, int64_t b) {
+  int row;
+  const int len = slot_length(a, b, row);
+  return {row, len, KeyTiles(len - 1, len - 1, len, (int)a.window, (int)a.sinks, TM)};
+}
+
+GDNX_DEV int tiles_of(const gdnx_paged_decode_args& a, int64_t b) { return make_seq(a, b).kt.count; }
+
+// One warp finds the range: tiles of all sequences, 32 at a time.
+GDNX_DEV Range find_range(const DecParams& P, int units) {
+  const int lane = threadIdx.x % 32;
+  int64_t total = 0;
+  for (int64_t b = lane; b < P.a.B; b += 32) total += tiles_of(P.a, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  total *= units;
+  const int64_t per = (total + P.grid - 1) / P.grid;
+  Range r;
+  r.t0 = min((int64_t)blockIdx.x * per, total);
+  r.t1 = min(r.t0 + per, total);
+  r.b = r.before = 0;
+  if (r.t0 >= r.t1) return r;
+  int64_t before = 0;
+  for (int64_t base = 0; base < P.a.B; base += 32) {
+    const int64_t b = base + lane;
+    const int64_t n = b < P.a.B ? (int64_t)tiles_of(P.a, b) * units : 0;
+    int64_t s = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    const uint32_t here = __ballot_sync(0xffffffffu, before + s > r.t0);
+    if (here) {
+      const int who = __ffs(here) - 1;
+      r.b = base + who;
+      r.before = before + __shfl_sync(0xffffffffu, s - n, who);
+      return r;
+    }
+    before += __shfl_sync(0xffffffffu, s, 31);
+  }
+  return r;
+}
+
+// Walks the units of a range: every role sees the same sequence of segments.
+struct Walk {
+  const DecParams& P;
+  int units;
+  int64_t t, t1, b, before;
+  Seq seq;
+  int unit, ta, tb;  // segment: tiles ta..tb-1 of `unit` of sequence b
+  GDNX_DEV Walk(const DecParams& P_, int units_, const Range& r)
+      : P(P_), units(units_), t(r.t0), t1(r.t1), b(r.b), before(r.before), seq(), unit(0), ta(0), tb(0) {
+    if (t < t1) seq = make_seq(P.a, b);
+  }
+  GDNX_DEV bool next() {
+    if (t >= t1) return false;
+    while (t >= before + (int64_t)seq.kt.count * units) {
+      before += (int64_t)seq.kt.count * units;
+      seq = make_seq(P.a, ++b);
+    }
+    const int n = seq.kt.count;
+    unit = (int)((t - before) / n);
+    ta = (int)((t - before) % n);
+    tb = (int)min((int64_t)n, ta + (t1 - t));
+    t += tb - ta;
+    return true;
+  }
+  GDNX_DEV bool whole() const { return ta == 0 && tb == seq.kt.count; }
+};
+
+GDNX_DEV bool key_seen(int j, int len, int window, int sinks) {
+  return j < len && (len - 1 - j < window || j < sinks);
+}
+
+// Page ids of a tile's pages, or -1 where nothing visible is there (lane < npp).
+GDNX_DEV int page_id(const DecParams& P, const Seq& s, int kt, int i) {
+  const gdnx_cache& c = P.a.cache;
+  const int64_t first = (int64_t)kt * TM + i * c.page;
+  if (first >= s.len || !(first + c.page > (int64_t)s.len - P.a.window || first < P.a.sinks)) return -1;
+  const int p = c.table[(int64_t)s.row * c.width + first / c.page];
+  return p >= 0 && p < c.pages ? p : -1;
+}
+
+GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(mbar)
+      : "memory");
+}
+
+template <int DB, int NH>
+GDNX_DEV void run_loads(const DecParams& P, Walk w, uint32_t smem, Bars& bar, volatile int* abort_flag) {
+  using Lo = Layout<DB, NH>;
+  const gdnx_cache& c = P.a.cache;
+  const int lane = threadIdx.x % 32, npp = TM / c.page, page = c.page;
+  const int ahead = 32 / npp;  // tiles whose page ids one load of the warp covers
+  const uint32_t box = (uint32_t)page * 128;
+  uint32_t cnt = 0;
+  while (w.next()) {
+    const int hk = w.unit / P.groups;
+    int ids = -1;
+    for (int t = w.ta; t < w.tb; ++t) {
+      const int k = (t - w.ta) % ahead;
+      if (k == 0) {
+        const int mine = t + lane / npp;
+        ids = mine < w.tb ? page_id(P, w.seq, w.seq.kt.tile(mine), lane % npp) : -1;
+      }
+      const int pg = lane / DB, d = lane % DB;
+      const int id = __shfl_sync(0xffffffffu, ids, (k * npp + pg) & 31);
+      const bool go = pg < npp && id >= 0;
+      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, go)) * box;
+#pragma unroll
+      for (int side = 0; side < 2; ++side, ++cnt) {
+        const uint32_t sl = cnt % Lo::SLOTS, mb = tc::smem_u32(&bar.full[sl]);
+        if (!warp_wait(&bar.empty[sl], (cnt / Lo::SLOTS & 1) ^ 1, abort_flag)) return;
+        if (lane == 0) pipe::expect_tx(mb, bytes);
+        __syncwarp();
+        if (go)
+          tma_load_3d(smem + Lo::RING + sl * Lo::TILE + d * BLOCK_BYTES + pg * box, &P.kv, d * 64, hk * page,
+                      (int)((P.a.layer * 2 + side) * c.pages + id), mb);
+      }
+    }
+  }
+}
+
+template <int DB, int NH, bool BF16>
+GDNX_DEV void run_products(const DecParams& P, Walk w, uint32_t smem, uint32_t tmem, Bars& bar,
+                           volatile int* abort_flag) {
+  using Lo = Layout<DB, NH>;
+  constexpr uint32_t ID_S = idesc16(BF16, 128, NH, false, false), ID_O = idesc16(BF16, 128, NH, true, false);
+  // S(t+1) goes out before P(t) is waited for, so the rows may be done with t+1 by then: p_ready
+  // has a barrier for each parity of t
+  uint32_t nt = 0, seg = 0;  // tiles and segments so far
+  bool pend = false, first = false;
+  const auto values = [&]() {  // O^T += V^T P of the tile before
+    if (!pend) return true;
+    const uint32_t t = nt - 1, vc = 2 * t + 1, sl = vc % Lo::SLOTS;
+    if (!pipe::wait_or_abort(&bar.full[sl], vc / Lo::SLOTS & 1, abort_flag)) return false;
+    if (!pipe::wait_or_abort(&bar.p_ready[t & 1], t / 2 & 1, abort_flag)) return false;
+    tc::fence_after();
+    const uint32_t v = smem + Lo::RING + sl * Lo::TILE, p = smem + Lo::P + (t & 1) * Lo::PB;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      tc::mma_bf16(tmem + 2 * NH, tc::smem_desc(v + k * 2048, DB == 2 ? BLOCK_BYTES : 1024, 1024),
+                   tc::smem_desc(p + (k / 4) * NH * 128 + (k % 4) * 32, 16, 1024), ID_O, !first || k > 0);
+    tc::commit(&bar.pv_done);
+    tc::commit(&bar.empty[sl]);
+    pend = false;
+    return true;
+  };
+  for (; w.next(); ++seg) {
+    for (int t = w.ta; t < w.tb; ++t) {
+      const uint32_t kc = 2 * nt, sl = kc % Lo::SLOTS;
+      if (t == w.ta) {
+        // the last unit's output is read before its successor's first product by p_ready
+        if (!values()) return;
+        if (!pipe::wait_or_abort(&bar.q_ready[seg & 1], seg / 2 & 1, abort_flag)) return;
+      }
+      if (!pipe::wait_or_abort(&bar.full[sl], kc / Lo::SLOTS & 1, abort_flag)) return;
+      tc::fence_after();
+      const uint32_t k = smem + Lo::RING + sl * Lo::TILE, q = smem + Lo::Q + (seg & 1) * Lo::QB;
+#pragma unroll
+      for (int x = 0; x < 4 * DB; ++x)
+        tc::mma_bf16(tmem + (nt & 1) * NH, tc::smem_desc(k + (x / 4) * BLOCK_BYTES + (x % 4) * 32, 16, 1024),
+                     tc::smem_desc(q + (x / 4) * NH * 128 + (x % 4) * 32, 16, 1024), ID_S, x > 0);
+      tc::commit(&bar.s_full[nt & 1]);
+      tc::commit(&bar.empty[sl]);
+      if (!values()) return;
+      ++nt;
+      pend = true;
+      first = t == w.ta;
+    }
+  }
+  values();
+}
+
+// Heads of one unit.
+struct Heads {
+  int h0, n;
+  GDNX_DEV Heads(const DecParams& P, int unit, int NH) {
+    const int G = (int)(P.a.H / P.a.cache.Hk), g = unit % P.groups;
+    h0 = unit / P.groups * G + g * NH;
+    n = min(NH, G - g * NH);
+  }
+};
+
+// The unit's query rows as a K-major tile of NH rows (rows beyond its heads zero).
+template <int DB, int NH>
+GDNX_DEV void stage_q(const DecParams& P, const Walk& w, uint8_t* dst) {
+  const gdnx_paged_decode_args& a = P.a;
+  const Heads hd(P, w.unit, NH);
+  const int D = (int)a.cache.D;
+  for (int x = threadIdx.x; x < NH * DB * 8; x += 128) {
+    const int h = x / (DB * 8), c = x % (DB * 8);
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (h < hd.n && c * 8 < D) {
+      const uint16_t* src = static_cast<const uint16_t*>(a.q.ptr) + w.b * a.q.sb + (hd.h0 + h) * a.q.sh + c * 8;
+      if (P.vec_q) {
+        u = *reinterpret_cast<const uint4*>(src);
+      } else {
+        u.x = src[0] | (uint32_t)src[1] << 16;
+        u.y = src[2] | (uint32_t)src[3] << 16;
+        u.z = src[4] | (uint32_t)src[5] << 16;
+        u.w = src[6] | (uint32_t)src[7] << 16;
+      }
+    }
+    *reinterpret_cast<uint4*>(dst + tc::sw128(h, c, NH)) = u;
+  }
+}
+
+GDNX_DEV void tmem_ld(uint32_t at, float (&v)[16]) { tc::tmem_ld16(at, v); }
+GDNX_DEV void tmem_ld(uint32_t at, float (&v)[32]) { tc::tmem_ld32(at, v); }
+GDNX_DEV void tmem_st(uint32_t at, float (&v)[16]) { tc::tmem_st16u(at, reinterpret_cast<const uint32_t*>(v)); }
+GDNX_DEV void tmem_st(uint32_t at, float (&v)[32]) { tc::tmem_st32(at, v); }
+
+template <int DB, int NH, bool BF16>
+GDNX_DEV void run_keys(const DecParams& P, Walk w, uint8_t* base, uint32_t tmem, Bars& bar, float* red,
+                       volatile int* abort_flag) {
+  using Lo = Layout<DB, NH>;
+  const gdnx_paged_decode_args& a = P.a;
+  const int r = threadIdx.x, lane = r % 32, warp = r / 32, D = (int)a.cache.D;
+  const uint32_t lane_at = (uint32_t)(warp * 32) << 16;
+  const float c2 = a.scale * kLog2e;
+  const int window = (int)a.window, sinks = (int)a.sinks;
+  uint32_t nt = 0, seg = 0;
+  bool ok = true;  // a wait that gave up is told at the next vote, where all four warps leave
+  Walk ahead = w;  // the segment whose queries are staged next
+  const auto stage = [&](uint32_t s) {
+    if (!ahead.next()) return;
+    stage_q<DB, NH>(P, ahead, base + Lo::Q + (s & 1) * Lo::QB);
+    tc::fence_async_smem();
+    pipe::mbar_arrive(&bar.q_ready[s & 1]);
+  };
+  stage(0);
+  for (; w.next(); ++seg) {
+    stage(seg + 1);  // its buffer's products (two segments back) have all been read
+    const Heads hd(P, w.unit, NH);
+    float m[NH], l[NH];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+    }
+    for (int t = w.ta; t < w.tb; ++t, ++nt) {
+      const int j0 = w.seq.kt.tile(t) * TM, j = j0 + r;
+      // a released page inside the visible range is not seen either
+      bool seen = key_seen(j, w.seq.len, window, sinks);
+      if (seen) {
+        const int p = a.cache.table[(int64_t)w.seq.row * a.cache.width + j / a.cache.page];
+        seen = p >= 0 && p < a.cache.pages;
+      }
+      ok = ok && warp_wait(&bar.s_full[nt & 1], nt / 2 & 1, abort_flag);
+      tc::fence_after();
+      float s[NH];
+      tmem_ld(tmem + lane_at + (nt & 1) * NH, s);
+      bool over = t == w.ta || !ok;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        s[h] = seen ? s[h] * c2 : -INFINITY;
+        if (h < hd.n) over |= s[h] > m[h] + 8.f;
+      }
+      if (pipe::group_any(1, 128, over)) {
+        // new maxima: of each warp's keys, then of the four warps
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          if (h >= hd.n) continue;
+          float x = s[h];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+          if (lane == 0) red[warp * NH + h] = x;
+        }
+        if (pipe::group_any(1, 128, !ok)) return;
+        float o[NH];
+        if (t > w.ta) {
+          ok = warp_wait(&bar.pv_done, (nt - 1) & 1, abort_flag);
+          tc::fence_after();
+          tmem_ld(tmem + lane_at + 2 * NH, o);
+        }
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          if (h >= hd.n) continue;
+          const float x = fmaxf(fmaxf(fmaxf(red[h], red[NH + h]), fmaxf(red[2 * NH + h], red[3 * NH + h])), m[h]);
+          const float corr = x == -INFINITY ? 1.f : ex2(m[h] - x);
+          m[h] = x;
+          l[h] *= corr;
+          if (t > w.ta) o[h] *= corr;
+        }
+        if (t > w.ta) tmem_st(tmem + lane_at + 2 * NH, o);
+        if (pipe::group_any(1, 128, !ok)) return;  // and red may be written again
+      }
+      uint8_t* pt = base + Lo::P + (nt & 1) * Lo::PB + (r / 64) * NH * 128 + r % 8 * 2;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        if (h >= hd.n) continue;
+        const float p = ex2(s[h] - (m[h] == -INFINITY ? 0.f : m[h]));
+        l[h] += p;
+        *reinterpret_cast<uint16_t*>(pt + h * 128 + (((r % 64 / 8) ^ (h & 7)) << 4)) = (uint16_t)pack2<BF16>(p, 0.f);
+      }
+      if (__any_sync(0xffffffffu, !seen)) {
+        const uint32_t vc = 2 * nt + 1, sl = vc % Lo::SLOTS;
+        ok = warp_wait(&bar.full[sl], vc / Lo::SLOTS & 1, abort_flag);
+        if (!seen && ok)
+#pragma unroll
+          for (int c = 0; c < DB * 8; ++c)
+            *reinterpret_cast<uint4*>(base + Lo::RING + sl * Lo::TILE + (c / 8) * BLOCK_BYTES + r * 128 + c % 8 * 16) =
+                make_uint4(0, 0, 0, 0);
+      }
+      tc::fence_async_smem();
+      tc::fence_before();
+      pipe::mbar_arrive(&bar.p_ready[nt & 1]);
+    }
+    // the unit's sums, then its output: lane d of tensor memory holds dimension d
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      if (h >= hd.n) continue;
+      const float x = warp_sum(l[h]);
+      if (lane == 0) red[warp * NH + h] = x;
+    }
+    if (pipe::group_any(1, 128, !ok)) return;
+    ok = warp_wait(&bar.pv_done, (nt - 1) & 1, abort_flag);
+    tc::fence_after();
+    float o[NH];
+    tmem_ld(tmem + lane_at + 2 * NH, o);
+    const bool whole = w.whole();
+    // a part that goes on in the next CTA is this CTA's last, any other its first
+    const int64_t at = ((int64_t)blockIdx.x * 2 + (w.tb < w.seq.kt.count && w.ta == 0 ? 1 : 0)) * NH;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      if (h >= hd.n) continue;
+      const float sum = red[h] + red[NH + h] + red[2 * NH + h] + red[3 * NH + h];
+      if (whole) {
+        const float inv = sum > 0.f ? 1.f / sum : sum != sum ? sum : 0.f;
+        if (r < D) st_from_f32(a.y, a.y_dtype, w.b * a.y_sb + (hd.h0 + h) * a.y_sh + r, sum == 0.f ? 0.f : o[h] * inv);
+      } else {
+        P.part[(at + h) * 128 + r] = o[h];
+        if (r == 0) {
+          P.stat[(at + h) * 2] = m[h];
+          P.stat[(at + h) * 2 + 1] = sum;
+        }
+      }
+    }
+    if (pipe::group_any(1, 128, !ok)) return;  // and red may be written again
+  }
+}
+
+template <int DB, int NH, bool BF16>
+__global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __grid_constant__ DecParams P) {
+  using Lo = Layout<DB, NH>;
+  extern __shared__ __align__(1024) uint8_t base[];
+  Small<NH>& sm = *reinterpret_cast<Small<NH>*>(base + Lo::SMALL);
+  Bars& bar = sm.bar;
+  volatile int* abort_flag = &sm.abort_flag;
+  const uint32_t smem = tc::smem_u32(base);
+  const int warp = threadIdx.x / 32, units = (int)P.a.cache.Hk * P.groups;
+  if (warp == 0) {
+    const Range r = find_range(P, units);
+    if (threadIdx.x == 0) sm.range = r;
+  } else if (warp == 4) {
+    tc::tmem_alloc(&sm.tmem_at, Lo::TMEM);
+  } else if (threadIdx.x == 160) {
+    *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
+    for (int i = 0; i < Lo::SLOTS; ++i) {
+      tc::mbar_init(&bar.full[i], 1);
+      tc::mbar_init(&bar.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&bar.q_ready[i], 128);
+      tc::mbar_init(&bar.s_full[i], 1);
+      tc::mbar_init(&bar.p_ready[i], 128);
+    }
+    tc::mbar_init(&bar.pv_done, 1);
+    tc::mbar_init(&bar.done, 1);
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = sm.tmem_at;
+  const Walk w(P, units, sm.range);
+  if (*abort_flag) {
+  } else if (warp < 4) {
+    run_keys<DB, NH, BF16>(P, w, base, tmem, bar, sm.red, abort_flag);
+  } else if (warp == 4) {
+    if (threadIdx.x % 32 == 0) {
+      run_products<DB, NH, BF16>(P, w, smem, tmem, bar, abort_flag);
+      tc::commit(&bar.done);  // every product issued has ended before tensor memory is freed
+      tc::mbar_wait(&bar.done, 0);
+    }
+  } else {
+    run_loads<DB, NH>(P, w, smem, bar, abort_flag);
+    if (*abort_flag)  // let the copies in flight land
+      for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
+  }
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 4) tc::tmem_dealloc(tmem, Lo::TMEM);
+  if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
+}
+
+// Joins a unit's parts, CTA after CTA, and writes the zeros of sequences that see nothing:
+// one block for each sequence and query head.
+template <int NH>
+__global__ void __launch_bounds__(128) paged_decode_join_kernel(const DecParams P) {
+  const gdnx_paged_decode_args& a = P.a;
+  __shared__ long long sums[2][4];
+  const int64_t h = blockIdx.x % a.H, b = blockIdx.x / a.H;
+  const int units = (int)a.cache.Hk * P.groups, D = (int)a.cache.D, d = threadIdx.x;
+  // tiles before this sequence, and of all
+  long long s0 = 0, s1 = 0;
+  for (int64_t i = threadIdx.x; i < a.B; i += 128) {
+    const int n = tiles_of(a, i);
+    s1 += n;
+    if (i < b) s0 += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+  }
+  if (threadIdx.x % 32 == 0) {
+    sums[0][threadIdx.x / 32] = s0;
+    sums[1][threadIdx.x / 32] = s1;
+  }
+  __syncthreads();
+  const int64_t before = (sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3]) * units;
+  const int64_t total = (sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3]) * units;
+  const int64_t per = (total + P.grid - 1) / P.grid;
+  const int n = tiles_of(a, b);
+  const int64_t out = b * a.y_sb + h * a.y_sh + d;
+  if (n == 0) {
+    if (d < D) st_from_f32(a.y, a.y_dtype, out, 0.f);
+    return;
+  }
+  const int G = (int)(a.H / a.cache.Hk), g = (int)(h % G);
+  const int64_t unit = h / G * P.groups + g / NH, first = before + unit * n, last = first + n - 1;
+  const int64_t c0 = first / per, c1 = last / per;
+  if (c0 == c1) return;  // one CTA had it whole
+  float m = -INFINITY, sum = 0.f, y = 0.f;
+  for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, P.stat[((c * 2 + (c == c0)) * NH + g % NH) * 2]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int64_t c = c0; c <= c1; ++c) {
+    const int64_t at = (c * 2 + (c == c0)) * NH + g % NH;
+    const float w = exp2f(P.stat[at * 2] - ref);
+    sum = fmaf(w, P.stat[at * 2 + 1], sum);
+    y = fmaf(w, P.part[at * 128 + d], y);
+  }
+  if (d < D) st_from_f32(a.y, a.y_dtype, out, sum == 0.f ? 0.f : y / sum);
+}
+
+struct Plan {
+  int nh, groups, grid;
+};
+
+Plan plan(const gdnx_paged_decode_args& a, int sms) {
+  Plan p;
+  const int64_t G = a.H / a.cache.Hk;
+  p.nh = G > 16 ? 32 : 16;
+  p.groups = (int)((G + p.nh - 1) / p.nh);
+  int64_t most = a.cache.width * a.cache.page;
+  if (a.max_len > 0 && a.max_len < most) most = a.max_len;
+  const int64_t tiles = a.B * a.cache.Hk * p.groups * ((most + TM - 1) / TM);
+  const int64_t ctas = (int64_t)sms;
+  p.grid = (int)(tiles < ctas ? (tiles > 0 ? tiles : 1) : ctas);
+  return p;
+}
+
+int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 148;
+  }
+  return sms;
+}
+
+template <int DB, int NH, bool BF16>
+gdnx_status launch(const DecParams& P, cudaStream_t st) {
+  const auto kernel = paged_decode_tc_kernel<DB, NH, BF16>;
+  constexpr int smem = (int)Layout<DB, NH>::SMEM;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return GDNX_ELAUNCH;
+  }
+  kernel<<<(unsigned)P.grid, NTHREADS, smem, st>>>(P);
+  paged_decode_join_kernel<NH><<<(unsigned)(P.a.B * P.a.H), 128, 0, st>>>(P);
+  return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
+}
+
+template <bool BF16>
+gdnx_status launch(const DecParams& P, int nh, cudaStream_t st) {
+  if (P.a.cache.D > 64) return nh == 16 ? launch<2, 16, BF16>(P, st) : launch<2, 32, BF16>(P, st);
+  return nh == 16 ? launch<1, 16, BF16>(P, st) : launch<1, 32, BF16>(P, st);
+}
+
+}  // namespace
+
+size_t paged_decode_tc_workspace_bytes(const gdnx_paged_decode_args& a) {
+  const Plan p = plan(a, sm_count());
+  return (size_t)p.grid * 2 * p.nh * (128 + 2) * sizeof(float);
+}
+
+gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t st) {
+  const gdnx_cache& c = a.cache;
+  const EncodeTiledFn enc = encode_fn();
+  if (!enc) return GDNX_ELAUNCH;
+  if (c.L * 2 * c.pages > ((int64_t)1 << 31) - 1 || c.Hk * c.page * c.D * 2 >= ((int64_t)1 << 40))
+    return GDNX_EUNSUPPORTED;
+  DecParams P;
+  const cuuint64_t dims[3] = {(cuuint64_t)c.D, (cuuint64_t)(c.Hk * c.page), (cuuint64_t)(c.L * 2 * c.pages)};
+  const cuuint64_t strides[2] = {(cuuint64_t)c.D * 2, (cuuint64_t)(c.Hk * c.page * c.D) * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)c.page, 1}, es[3] = {1, 1, 1};
+  if (enc(&P.kv, c.dtype == GDNX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, c.kv,
+          dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return GDNX_EINVAL;
+  const Plan p = plan(a, sm_count());
+  P.a = a;
+  P.grid = p.grid;
+  P.groups = p.groups;
+  P.part = static_cast<float*>(a.workspace);
+  P.stat = P.part + (size_t)p.grid * 2 * p.nh * 128;
+  P.vec_q = reinterpret_cast<uintptr_t>(a.q.ptr) % 16 == 0 && a.q.sb % 8 == 0 && a.q.sh % 8 == 0;
+  return c.dtype == GDNX_BF16 ? launch<true>(P, p.nh, st) : launch<false>(P, p.nh, st);
+}
+
+}  // namespace gdnx
