@@ -38,7 +38,7 @@ struct DecParams {
 };
 
 struct Bars {
-  uint64_t full[12], empty[12], q_ready[2], s_full[2], p_ready[2], pv_done, done;
+  uint64_t full[12], empty[12], q_ready[2], s_full[2], p_ready[2], pv_done[2], done;
 };
 
 // The place of a CTA in the row of all tiles: its tiles t0..t1-1, the sequence b that holds t0
@@ -212,8 +212,9 @@ GDNX_DEV void run_products(const DecParams& P, Walk w, uint32_t smem, uint32_t t
                            volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   constexpr uint32_t ID_S = idesc16(BF16, 128, NH, false, false), ID_O = idesc16(BF16, 128, NH, true, false);
-  // S(t+1) goes out before P(t) is waited for, so the rows may be done with t+1 by then: p_ready
-  // has a barrier for each parity of t
+  // S(t+1) goes out before P(t) is waited for, so the rows may be done with t+1 by then, and
+  // they skip most of pv_done: both have a barrier for each parity of t, which cannot be lapped
+  // (S(t+2) follows PV(t))
   uint32_t nt = 0, seg = 0;  // tiles and segments so far
   bool pend = false, first = false;
   const auto values = [&]() {  // O^T += V^T P of the tile before
@@ -227,7 +228,7 @@ GDNX_DEV void run_products(const DecParams& P, Walk w, uint32_t smem, uint32_t t
     for (int k = 0; k < 8; ++k)
       tc::mma_bf16(tmem + 2 * NH, tc::smem_desc(v + k * 2048, DB == 2 ? BLOCK_BYTES : 1024, 1024),
                    tc::smem_desc(p + (k / 4) * NH * 128 + (k % 4) * 32, 16, 1024), ID_O, !first || k > 0);
-    tc::commit(&bar.pv_done);
+    tc::commit(&bar.pv_done[t & 1]);
     tc::commit(&bar.empty[sl]);
     pend = false;
     return true;
@@ -292,12 +293,32 @@ GDNX_DEV void stage_q(const DecParams& P, const Walk& w, uint8_t* dst) {
   }
 }
 
-GDNX_DEV void tmem_ld(uint32_t at, float (&v)[16]) { tc::tmem_ld16(at, v); }
-GDNX_DEV void tmem_ld(uint32_t at, float (&v)[32]) { tc::tmem_ld32(at, v); }
-GDNX_DEV void tmem_st(uint32_t at, float (&v)[16]) { tc::tmem_st16u(at, reinterpret_cast<const uint32_t*>(v)); }
-GDNX_DEV void tmem_st(uint32_t at, float (&v)[32]) { tc::tmem_st32(at, v); }
+// NC columns of a thread's lane, in the widths of a tensor-memory move (4 and 8 at once).
+template <int NC>
+GDNX_DEV void tmem_ld(uint32_t at, float (&v)[NC]) {
+#pragma unroll
+  for (int i = 0; i < NC; i += 4)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3])
+                 : "r"(at + i)
+                 : "memory");
+}
+template <>
+GDNX_DEV void tmem_ld<16>(uint32_t at, float (&v)[16]) { tc::tmem_ld16(at, v); }
+template <>
+GDNX_DEV void tmem_ld<32>(uint32_t at, float (&v)[32]) { tc::tmem_ld32(at, v); }
+template <int NC>
+GDNX_DEV void tmem_st(uint32_t at, const float (&v)[NC]) {
+#pragma unroll
+  for (int i = 0; i < NC; i += 4)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n\ttcgen05.wait::st.sync.aligned;"
+                 :
+                 : "r"(at + i), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3])
+                 : "memory");
+}
 
-template <int DB, int NH, bool BF16>
+// NC: heads that a thread works on, the unit's rounded up (the others' columns are not used).
+template <int DB, int NH, int NC, bool BF16>
 GDNX_DEV void run_keys(const DecParams& P, Walk w, uint8_t* base, uint32_t tmem, Bars& bar, float* red,
                        volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
@@ -319,9 +340,9 @@ GDNX_DEV void run_keys(const DecParams& P, Walk w, uint8_t* base, uint32_t tmem,
   for (; w.next(); ++seg) {
     stage(seg + 1);  // its buffer's products (two segments back) have all been read
     const Heads hd(P, w.unit, NH);
-    float m[NH], l[NH];
+    float m[NC], l[NC];
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
+    for (int h = 0; h < NC; ++h) {
       m[h] = -INFINITY;
       l[h] = 0.f;
     }
@@ -335,34 +356,32 @@ GDNX_DEV void run_keys(const DecParams& P, Walk w, uint8_t* base, uint32_t tmem,
       }
       ok = ok && warp_wait(&bar.s_full[nt & 1], nt / 2 & 1, abort_flag);
       tc::fence_after();
-      float s[NH];
+      float s[NC];
       tmem_ld(tmem + lane_at + (nt & 1) * NH, s);
       bool over = t == w.ta || !ok;
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
+      for (int h = 0; h < NC; ++h) {
         s[h] = seen ? s[h] * c2 : -INFINITY;
-        if (h < hd.n) over |= s[h] > m[h] + 8.f;
+        over |= s[h] > m[h] + 8.f;
       }
       if (pipe::group_any(1, 128, over)) {
         // new maxima: of each warp's keys, then of the four warps
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          if (h >= hd.n) continue;
+        for (int h = 0; h < NC; ++h) {
           float x = s[h];
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
           if (lane == 0) red[warp * NH + h] = x;
         }
         if (pipe::group_any(1, 128, !ok)) return;
-        float o[NH];
+        float o[NC];
         if (t > w.ta) {
-          ok = warp_wait(&bar.pv_done, (nt - 1) & 1, abort_flag);
+          ok = warp_wait(&bar.pv_done[(nt - 1) & 1], (nt - 1) / 2 & 1, abort_flag);
           tc::fence_after();
           tmem_ld(tmem + lane_at + 2 * NH, o);
         }
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          if (h >= hd.n) continue;
+        for (int h = 0; h < NC; ++h) {
           const float x = fmaxf(fmaxf(fmaxf(red[h], red[NH + h]), fmaxf(red[2 * NH + h], red[3 * NH + h])), m[h]);
           const float corr = x == -INFINITY ? 1.f : ex2(m[h] - x);
           m[h] = x;
@@ -374,8 +393,7 @@ GDNX_DEV void run_keys(const DecParams& P, Walk w, uint8_t* base, uint32_t tmem,
       }
       uint8_t* pt = base + Lo::P + (nt & 1) * Lo::PB + (r / 64) * NH * 128 + r % 8 * 2;
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        if (h >= hd.n) continue;
+      for (int h = 0; h < NC; ++h) {
         const float p = ex2(s[h] - (m[h] == -INFINITY ? 0.f : m[h]));
         l[h] += p;
         *reinterpret_cast<uint16_t*>(pt + h * 128 + (((r % 64 / 8) ^ (h & 7)) << 4)) = (uint16_t)pack2<BF16>(p, 0.f);
@@ -395,21 +413,20 @@ GDNX_DEV void run_keys(const DecParams& P, Walk w, uint8_t* base, uint32_t tmem,
     }
     // the unit's sums, then its output: lane d of tensor memory holds dimension d
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      if (h >= hd.n) continue;
+    for (int h = 0; h < NC; ++h) {
       const float x = warp_sum(l[h]);
       if (lane == 0) red[warp * NH + h] = x;
     }
     if (pipe::group_any(1, 128, !ok)) return;
-    ok = warp_wait(&bar.pv_done, (nt - 1) & 1, abort_flag);
+    ok = warp_wait(&bar.pv_done[(nt - 1) & 1], (nt - 1) / 2 & 1, abort_flag);
     tc::fence_after();
-    float o[NH];
+    float o[NC];
     tmem_ld(tmem + lane_at + 2 * NH, o);
     const bool whole = w.whole();
     // a part that goes on in the next CTA is this CTA's last, any other its first
     const int64_t at = ((int64_t)blockIdx.x * 2 + (w.tb < w.seq.kt.count && w.ta == 0 ? 1 : 0)) * NH;
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
+    for (int h = 0; h < NC; ++h) {
       if (h >= hd.n) continue;
       const float sum = red[h] + red[NH + h] + red[2 * NH + h] + red[3 * NH + h];
       if (whole) {
@@ -427,8 +444,9 @@ GDNX_DEV void run_keys(const DecParams& P, Walk w, uint8_t* base, uint32_t tmem,
   }
 }
 
-template <int DB, int NH, bool BF16>
+template <int DB, int NC, bool BF16>
 __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __grid_constant__ DecParams P) {
+  constexpr int NH = NC > 16 ? 32 : 16;
   using Lo = Layout<DB, NH>;
   extern __shared__ __align__(1024) uint8_t base[];
   Small<NH>& sm = *reinterpret_cast<Small<NH>*>(base + Lo::SMALL);
@@ -451,8 +469,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
       tc::mbar_init(&bar.q_ready[i], 128);
       tc::mbar_init(&bar.s_full[i], 1);
       tc::mbar_init(&bar.p_ready[i], 128);
+      tc::mbar_init(&bar.pv_done[i], 1);
     }
-    tc::mbar_init(&bar.pv_done, 1);
     tc::mbar_init(&bar.done, 1);
   }
   tc::fence_before();
@@ -462,7 +480,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   const Walk w(P, units, sm.range);
   if (*abort_flag) {
   } else if (warp < 4) {
-    run_keys<DB, NH, BF16>(P, w, base, tmem, bar, sm.red, abort_flag);
+    run_keys<DB, NH, NC, BF16>(P, w, base, tmem, bar, sm.red, abort_flag);
   } else if (warp == 4) {
     if (threadIdx.x % 32 == 0) {
       run_products<DB, NH, BF16>(P, w, smem, tmem, bar, abort_flag);
@@ -483,16 +501,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
 }
 
 // Joins a unit's parts, CTA after CTA, and writes the zeros of sequences that see nothing:
-// one block for each sequence and query head.
+// one block for each sequence and query head.  Each of its warps sums a contiguous run of the
+// parts; the runs are added in order.
+constexpr int JOIN_WARPS = 8;
+
 template <int NH>
-__global__ void __launch_bounds__(128) paged_decode_join_kernel(const DecParams P) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_decode_join_kernel(const DecParams P) {
   const gdnx_paged_decode_args& a = P.a;
-  __shared__ long long sums[2][4];
+  __shared__ long long sums[2][JOIN_WARPS];
+  __shared__ float red_m[JOIN_WARPS], red_l[JOIN_WARPS], red_o[JOIN_WARPS][128];
   const int64_t h = blockIdx.x % a.H, b = blockIdx.x / a.H;
-  const int units = (int)a.cache.Hk * P.groups, D = (int)a.cache.D, d = threadIdx.x;
+  const int units = (int)a.cache.Hk * P.groups, D = (int)a.cache.D, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   // tiles before this sequence, and of all
   long long s0 = 0, s1 = 0;
-  for (int64_t i = threadIdx.x; i < a.B; i += 128) {
+  for (int64_t i = threadIdx.x; i < a.B; i += JOIN_WARPS * 32) {
     const int n = tiles_of(a, i);
     s1 += n;
     if (i < b) s0 += n;
@@ -502,34 +524,67 @@ __global__ void __launch_bounds__(128) paged_decode_join_kernel(const DecParams 
     s0 += __shfl_xor_sync(0xffffffffu, s0, o);
     s1 += __shfl_xor_sync(0xffffffffu, s1, o);
   }
-  if (threadIdx.x % 32 == 0) {
-    sums[0][threadIdx.x / 32] = s0;
-    sums[1][threadIdx.x / 32] = s1;
+  if (lane == 0) {
+    sums[0][warp] = s0;
+    sums[1][warp] = s1;
   }
-  __syncthreads();
-  const int64_t before = (sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3]) * units;
-  const int64_t total = (sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3]) * units;
-  const int64_t per = (total + P.grid - 1) / P.grid;
   const int n = tiles_of(a, b);
-  const int64_t out = b * a.y_sb + h * a.y_sh + d;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < JOIN_WARPS; ++i) {
+    before += sums[0][i];
+    total += sums[1][i];
+  }
+  const int64_t per = (total * units + P.grid - 1) / P.grid;
+  const int64_t out = b * a.y_sb + h * a.y_sh;
   if (n == 0) {
-    if (d < D) st_from_f32(a.y, a.y_dtype, out, 0.f);
+    for (int d = threadIdx.x; d < D; d += JOIN_WARPS * 32) st_from_f32(a.y, a.y_dtype, out + d, 0.f);
     return;
   }
   const int G = (int)(a.H / a.cache.Hk), g = (int)(h % G);
-  const int64_t unit = h / G * P.groups + g / NH, first = before + unit * n, last = first + n - 1;
-  const int64_t c0 = first / per, c1 = last / per;
+  const int64_t unit = h / G * P.groups + g / NH, first = before * units + unit * n, last = first + n - 1;
+  const int c0 = (int)(first / per), c1 = (int)(last / per);
   if (c0 == c1) return;  // one CTA had it whole
-  float m = -INFINITY, sum = 0.f, y = 0.f;
-  for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, P.stat[((c * 2 + (c == c0)) * NH + g % NH) * 2]);
+  const auto place = [&](int c) { return ((int64_t)c * 2 + (c == c0)) * NH + g % NH; };
+  const int parts = c1 - c0 + 1, run = (parts + JOIN_WARPS - 1) / JOIN_WARPS;
+  const int r0 = c0 + warp * run, r1 = min(r0 + run, c1 + 1);
+  float m = -INFINITY, l = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = r0 + lane; c < r1; c += 32) m = fmaxf(m, P.stat[place(c) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float ref = m == -INFINITY ? 0.f : m;
-  for (int64_t c = c0; c <= c1; ++c) {
-    const int64_t at = (c * 2 + (c == c0)) * NH + g % NH;
+#pragma unroll 4
+  for (int c = r0; c < r1; ++c) {
+    const int64_t at = place(c);
     const float w = exp2f(P.stat[at * 2] - ref);
-    sum = fmaf(w, P.stat[at * 2 + 1], sum);
-    y = fmaf(w, P.part[at * 128 + d], y);
+    const float4 x = *reinterpret_cast<const float4*>(P.part + at * 128 + lane * 4);
+    l = fmaf(w, P.stat[at * 2 + 1], l);
+    y.x = fmaf(w, x.x, y.x);
+    y.y = fmaf(w, x.y, y.y);
+    y.z = fmaf(w, x.z, y.z);
+    y.w = fmaf(w, x.w, y.w);
   }
-  if (d < D) st_from_f32(a.y, a.y_dtype, out, sum == 0.f ? 0.f : y / sum);
+  *reinterpret_cast<float4*>(&red_o[warp][lane * 4]) = y;
+  if (lane == 0) {
+    red_m[warp] = m;
+    red_l[warp] = l;
+  }
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= D) return;
+  float top = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+  for (int i = 0; i < JOIN_WARPS; ++i) top = fmaxf(top, red_m[i]);
+  if (top == -INFINITY) top = 0.f;
+#pragma unroll
+  for (int i = 0; i < JOIN_WARPS; ++i) {
+    const float w = exp2f(red_m[i] - top);
+    sum = fmaf(w, red_l[i], sum);
+    v = fmaf(w, red_o[i][d], v);
+  }
+  st_from_f32(a.y, a.y_dtype, out + d, sum == 0.f ? 0.f : v / sum);
 }
 
 struct Plan {
@@ -559,23 +614,31 @@ int sm_count() {
   return sms;
 }
 
-template <int DB, int NH, bool BF16>
+template <int DB, int NC, bool BF16>
 gdnx_status launch(const DecParams& P, cudaStream_t st) {
-  const auto kernel = paged_decode_tc_kernel<DB, NH, BF16>;
+  constexpr int NH = NC > 16 ? 32 : 16;
+  const auto kernel = paged_decode_tc_kernel<DB, NC, BF16>;
   constexpr int smem = (int)Layout<DB, NH>::SMEM;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
     return GDNX_ELAUNCH;
   }
   kernel<<<(unsigned)P.grid, NTHREADS, smem, st>>>(P);
-  paged_decode_join_kernel<NH><<<(unsigned)(P.a.B * P.a.H), 128, 0, st>>>(P);
+  paged_decode_join_kernel<NH><<<(unsigned)(P.a.B * P.a.H), JOIN_WARPS * 32, 0, st>>>(P);
   return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
 }
 
+template <int DB, bool BF16>
+gdnx_status launch_heads(const DecParams& P, cudaStream_t st) {
+  const int64_t G = P.a.H / P.a.cache.Hk;
+  if (G <= 4) return launch<DB, 4, BF16>(P, st);
+  if (G <= 8) return launch<DB, 8, BF16>(P, st);
+  return G <= 16 ? launch<DB, 16, BF16>(P, st) : launch<DB, 32, BF16>(P, st);
+}
+
 template <bool BF16>
-gdnx_status launch(const DecParams& P, int nh, cudaStream_t st) {
-  if (P.a.cache.D > 64) return nh == 16 ? launch<2, 16, BF16>(P, st) : launch<2, 32, BF16>(P, st);
-  return nh == 16 ? launch<1, 16, BF16>(P, st) : launch<1, 32, BF16>(P, st);
+gdnx_status launch_type(const DecParams& P, cudaStream_t st) {
+  return P.a.cache.D > 64 ? launch_heads<2, BF16>(P, st) : launch_heads<1, BF16>(P, st);
 }
 
 }  // namespace
@@ -606,7 +669,7 @@ gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t
   P.part = static_cast<float*>(a.workspace);
   P.stat = P.part + (size_t)p.grid * 2 * p.nh * 128;
   P.vec_q = reinterpret_cast<uintptr_t>(a.q.ptr) % 16 == 0 && a.q.sb % 8 == 0 && a.q.sh % 8 == 0;
-  return c.dtype == GDNX_BF16 ? launch<true>(P, p.nh, st) : launch<false>(P, p.nh, st);
+  return c.dtype == GDNX_BF16 ? launch_type<true>(P, st) : launch_type<false>(P, st);
 }
 
 }  // namespace gdnx
