@@ -63,10 +63,10 @@ GDNX_DEV uint32_t range_bits(int lo, int hi, int w) {
 
 // D (+)= P X with P's columns in two halves, each over the start of its half of 128 columns.
 GDNX_DEV void mma_halves(uint32_t d, uint32_t p, uint32_t x, uint32_t idesc, bool acc) {
+  const uint64_t dx = tc::smem_desc(x, BLOCK_BYTES, 1024);
 #pragma unroll
   for (int k = 0; k < 8; ++k)
-    tc::mma_bf16_ts(d, p + (k < 4 ? 8 * k : 64 + 8 * (k - 4)), tc::smem_desc(x + k * 2048, BLOCK_BYTES, 1024), idesc,
-                    acc || k > 0);
+    tc::mma_bf16_ts(d, p + (k < 4 ? 8 * k : 64 + 8 * (k - 4)), dx + k * (2048 >> 4), idesc, acc || k > 0);
 }
 
 // Rows r0.. of a landed tile to zero: padding rows meet weights of 0, so they must not hold NaN.

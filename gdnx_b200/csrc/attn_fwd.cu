@@ -6,10 +6,14 @@
 //   S_s = Q_s K^T (tcgen05, fp32 in tensor memory) -> registers, one query per thread:
 //   m = max, p = 2^(c (s - m)), l += p -> P_s packed 16-bit over S_s's columns ->
 //   O_s += P_s V (tcgen05, P from tensor memory, V read with its rows as K).
-// While one stage's 128 threads take exponentials, the tensor cores work for the other.
+// While one stage's rows take exponentials, the tensor cores work for the other.
 // Warps 0-3 and 4-7 are the stages' rows, warp 8 issues the products, warp 9 the TMA loads
-// (Q of each stage, K and V through one ring).  The product warp puts PV(t) and S(t+1) of a
-// stage in one run, so S(t+1) complete means PV(t) complete and O at rest.
+// (Q of each stage, K and V through one ring).  A stage's PV(t) and S(t+1) are
+// issued in order, so S(t+1) complete means PV(t) complete and O at rest.
+//
+// The exponentials are what the tensor cores wait for: 128 x 128 of them a tile take the
+// special-function units as long as its two products take the tensor cores.  So an eighth of
+// them goes to the FMA pipes instead (ex2_poly), scaling and sums run two to an instruction.
 //
 // The maximum is lazy: P is taken against the last m that O was scaled to, and O is rescaled
 // only when the new maximum is more than 8 above it in log2 (P stays below 2^8, exact in
@@ -24,72 +28,82 @@ namespace {
 
 using namespace attn;
 
-constexpr int NTHREADS = 384;  // three warpgroups: a stage's rows each, and the warps that issue
+constexpr int NTHREADS = 384;  // a warpgroup for each stage's rows, and the warps that issue
 constexpr uint32_t T_S = 0, T_O = 256;  // tensor-memory columns: S_0, S_1, then O_0, O_1
 
 struct FwdParams {
-  TileMap q, k, v;
+  TileMap q, k, v, y;
   gdnx_attn_args a;
   int64_t items;
+  int tma_y;                   // 16-bit outputs leave through shared memory and TMA
   int pairs, units, by_heads;  // stage pairs of a key head; blocks (or block pairs) of queries
 };
 
-// One stage of a work item: head, first row, the key tiles of its rows.
-struct Stage {
-  int h, i0, p0, p1, lo, hi;  // hi < 0: sees nothing
-  bool valid;
-};
-
+// A work item: its two stages' heads and rows, and the key tiles that either sees as one
+// sequence.  (Scalars and selects: an array indexed by the stage would live in memory.)
 struct Item {
-  int b, hk, len, nst;  // nst: tiles that hold sinks
-  Stage s[2];
-  int nsink, lo, count;  // the tiles either stage sees, as one sequence
-  GDNX_DEV int tile(int i) const { return i < nsink ? i : lo + i - nsink; }
-  GDNX_DEV bool active(int st, int kt) const {
-    const Stage& x = s[st];
-    return kt <= x.hi && (kt >= x.lo || kt < nst);
-  }
+  int b, hk, len, off, Tq, nst;  // nst: tiles that hold sinks
+  int h0, i0, di;                // stage 1: head h0 + dh or rows i0 + di
+  int dh, lo0, lo1, hi0, hi1;    // a stage's window tiles; hi < 0: sees nothing
+  int nsink, count;
+  GDNX_DEV int head(int st) const { return st ? h0 + dh : h0; }
+  GDNX_DEV int row(int st) const { return st ? i0 + di : i0; }
+  GDNX_DEV bool valid(int st) const { return row(st) < Tq; }
+  GDNX_DEV int lo(int st) const { return st ? lo1 : lo0; }
+  GDNX_DEV int hi(int st) const { return st ? hi1 : hi0; }
+  GDNX_DEV int tile(int i) const { return i < nsink ? i : lo0 + i - nsink; }
+  GDNX_DEV bool active(int st, int kt) const { return kt <= hi(st) && (kt >= lo(st) || kt < nst); }
 };
 
-GDNX_DEV Item make_item(const FwdParams& P, int64_t n) {
+GDNX_DEV Item make_item(const FwdParams& P, int64_t item) {
   const gdnx_attn_args& a = P.a;
   Item w;
-  const int Hk = (int)a.Hk, G = (int)(a.H / a.Hk), off = (int)(a.Tk - a.Tq), window = (int)a.window;
-  const int pr = (int)(n % P.pairs);
-  n /= P.pairs;
-  w.hk = (int)(n % Hk);
-  n /= Hk;
-  w.b = (int)(n % a.B);
-  const int u = P.units - 1 - (int)(n / a.B);  // the blocks that see most first
-  w.len = seq_len(a, w.b);
+  const int Hk = (int)a.Hk, G = (int)a.H / Hk, B = (int)a.B, window = (int)a.window;
+  // the grid's items fit 31 bits
+  unsigned n = (unsigned)item;
+  const int pr = (int)(n % (unsigned)P.pairs);
+  n /= (unsigned)P.pairs;
+  w.hk = (int)(n % (unsigned)Hk);
+  n /= (unsigned)Hk;
+  w.b = (int)(n % (unsigned)B);
+  const int u = P.units - 1 - (int)(n / (unsigned)B);  // the blocks that see most first
+  w.len = uniform(seq_len(a, w.b));
+  w.off = (int)(a.Tk - a.Tq);
+  w.Tq = (int)a.Tq;
   w.nst = (int)((a.sinks + TM - 1) / TM);
-#pragma unroll
-  for (int st = 0; st < 2; ++st) {
-    Stage& x = w.s[st];
-    x.h = P.by_heads ? w.hk * G + 2 * pr + st : w.hk * G + pr;
-    x.i0 = (P.by_heads ? u : 2 * u + st) * TM;
-    x.valid = x.i0 < a.Tq;
-    x.p0 = x.i0 + off;
-    x.p1 = min(x.i0 + TM, (int)a.Tq) - 1 + off;
-    x.lo = max(0, x.p0 - window + 1) / TM;
-    x.hi = x.valid && x.p0 < w.len ? min(x.p1, w.len - 1) / TM : -1;
-  }
-  w.lo = w.s[0].lo;
-  w.nsink = min(w.nst, w.lo);
-  w.count = w.s[0].hi < 0 ? 0 : w.nsink + max(w.s[0].hi, w.s[1].hi) - w.lo + 1;
+  w.h0 = P.by_heads ? w.hk * G + 2 * pr : w.hk * G + pr;
+  w.dh = P.by_heads ? 1 : 0;
+  w.i0 = (P.by_heads ? u : 2 * u) * TM;
+  w.di = P.by_heads ? 0 : TM;
+  const auto span = [&](int row, int& lo, int& hi) {
+    const int p0 = row + w.off, p1 = min(row + TM, w.Tq) - 1 + w.off;
+    lo = max(0, p0 - window + 1) / TM;
+    hi = row < w.Tq && p0 < w.len ? min(p1, w.len - 1) / TM : -1;
+  };
+  span(w.i0, w.lo0, w.hi0);
+  span(w.i0 + w.di, w.lo1, w.hi1);
+  w.nsink = min(w.nst, w.lo0);
+  w.count = w.hi0 < 0 ? 0 : w.nsink + max(w.hi0, w.hi1) - w.lo0 + 1;
   return w;
 }
 
-template <int DB>
-struct Layout {
-  static constexpr int SLOTS = DB == 2 ? 5 : 8;  // K and V tiles in flight
-  static constexpr uint32_t TILE = DB * BLOCK_BYTES;
-  static constexpr uint32_t Q = 0, KV = 2 * TILE, END = KV + SLOTS * TILE;
-  static constexpr size_t SMEM = END + 1024;
-};
-
 struct Bars {
   uint64_t kv_full[8], kv_empty[8], q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2], fix, done;
+};
+
+struct Small {
+  Bars bar;
+  uint32_t tmem_at;
+  int abort_flag;
+};
+
+template <int DB>
+struct Layout {
+  static constexpr int SLOTS = DB == 2 ? 4 : 8;  // K and V tiles in flight
+  static constexpr uint32_t TILE = DB * BLOCK_BYTES;
+  // Q of both stages, the ring, and for each row warp 32 rows x 64 values on their way out
+  static constexpr uint32_t Q = 0, KV = 2 * TILE, OUT = KV + SLOTS * TILE, SMALL = OUT + 8 * 4096;
+  static constexpr size_t SMEM = SMALL + sizeof(Small);  // no static shared memory: the base is 1024-aligned
 };
 
 // Bits lo..hi (inclusive, any integers) of the 32-bit word that holds columns 32w..32w+31.
@@ -99,178 +113,196 @@ GDNX_DEV uint32_t range_bits(int lo, int hi, int w) {
   return lo > hi ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
 }
 
-GDNX_DEV void store8(void* y, int dtype, int64_t at, const float* x) {
-  if (dtype == GDNX_F32) {
-    float4* p = reinterpret_cast<float4*>(static_cast<float*>(y) + at);
-    p[0] = make_float4(x[0], x[1], x[2], x[3]);
-    p[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    uint4 u;
-    if (dtype == GDNX_BF16) {
-      u.x = pack2<true>(x[0], x[1]); u.y = pack2<true>(x[2], x[3]);
-      u.z = pack2<true>(x[4], x[5]); u.w = pack2<true>(x[6], x[7]);
-    } else {
-      u.x = pack2<false>(x[0], x[1]); u.y = pack2<false>(x[2], x[3]);
-      u.z = pack2<false>(x[4], x[5]); u.w = pack2<false>(x[6], x[7]);
-    }
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + at) = u;
+// Weights of 32 columns: p = 2^(c2 s - mc), summed, packed 16-bit.  One pair in eight is taken on
+// the FMA pipes (where masked scores give 2^-125: nothing beside a weight that counts).
+template <bool BF16>
+GDNX_DEV void weights32(const float* s, float c2, float mc, float2& sum, uint32_t* pk) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(c2, c2), make_float2(-mc, -mc));
+    const float2 p = e % 8 == 3 ? ex2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+    sum = add2(sum, p);
+    pk[e] = pack2<BF16>(p.x, p.y);
   }
 }
 
-// The rows of one stage: scores to weights, tile after tile, and the output.
+// 32 values of a row as 16-bit words.
+GDNX_DEV void pack_row(uint32_t* u, const float* o, int dtype) {
+  if (dtype == GDNX_BF16) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) u[e] = pack2<true>(o[2 * e], o[2 * e + 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) u[e] = pack2<false>(o[2 * e], o[2 * e + 1]);
+  }
+}
+
+// One stage's rows, one for each thread.
 template <int DB, bool BF16>
-GDNX_DEV void run_rows(const FwdParams& P, int st, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+  using Lo = Layout<DB>;
   const gdnx_attn_args& a = P.a;
-  const int r = threadIdx.x % 128;
+  const int r = threadIdx.x % 128, lane = r % 32, warp = threadIdx.x / 32, st = warp / 4;
   const uint32_t lane_at = (uint32_t)(r / 32 * 32) << 16;
   const uint32_t tS = tmem + T_S + st * 128 + lane_at, tO = tmem + T_O + st * 128 + lane_at;
   const int window = (int)a.window, sinks = (int)a.sinks, D = (int)a.D;
   const float c2 = a.scale * kLog2e;
+  uint8_t* out = base + Lo::OUT + warp * 4096;
   uint32_t nS = 0, nO = 0;
   for (int64_t n = blockIdx.x; n < P.items; n += gridDim.x) {
     const Item w = make_item(P, n);
-    const Stage& x = w.s[st];
-    if (!x.valid) continue;
-    float m = -INFINITY, l = 0.f;
-    const int p = x.p0 + r;
+    if (!w.valid(st)) continue;
+    const int row = w.row(st), head = w.head(st), p0 = row + w.off, p = p0 + r;
+    float m = -INFINITY, l = 0.f;  // the maximum that O and l are scaled to, the sum
     for (int i = 0; i < w.count; ++i) {
       const int kt = w.tile(i), j0 = kt * TM;
       if (!w.active(st, kt)) continue;
       if (!warp_wait(&bar.s_full[st], nS++ & 1, abort_flag)) return;
       tc::fence_after();
-      float s[128];
+      float s[128], t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       tmem_ld128(tS, s);
-      // every row sees the whole tile?
-      const bool whole = j0 + TM - 1 <= x.p0 && j0 + TM <= w.len &&
-                         (x.p0 + TM - 1 - j0 < window || j0 + TM <= sinks);
-      if (!whole) {
-        const int hi = p < w.len ? min(p, w.len - 1) - j0 : -1;
+      uint32_t used = 0xf;  // chunks of which some row of the warp sees a column
+      // does every row see the whole tile?
+      if (!(j0 + TM - 1 <= p0 && p0 + TM <= w.len && (p0 + TM - 1 - j0 < window || j0 + TM <= sinks))) {
+        // visible columns: lo..hi, and those up to sk
+        const int hi = p < w.len ? p - j0 : -1, lo = p - window + 1 - j0, sk = min(sinks - 1 - j0, hi);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t on = range_bits(p - window + 1 - j0, hi, q) | range_bits(0, min(sinks - 1 - j0, hi), q);
+          const uint32_t on = range_bits(lo, hi, q) | range_bits(0, sk, q);
+          if (!__any_sync(0xffffffffu, on)) {
+            used &= ~(1u << q);
+          } else if (!__all_sync(0xffffffffu, on == 0xffffffffu)) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!(on >> e & 1)) s[32 * q + e] = -INFINITY;
+            for (int e = 0; e < 32; ++e)
+              if (!(on >> e & 1)) s[32 * q + e] = -INFINITY;
+          }
         }
       }
-      float mx[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) mx[q] = s[q];
+      for (int q = 0; q < 4; ++q) {
+        if (!(used >> q & 1)) continue;
 #pragma unroll
-      for (int e = 4; e < 128; e += 4)
+        for (int e = 0; e < 32; e += 8)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], s[e + q]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          for (int f = 0; f < 4; ++f) t[f] = fmaxf(fmaxf(t[f], s[32 * q + e + f]), s[32 * q + e + f + 4]);
+      }
+      const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
       const bool grow = m != -INFINITY && (top - m) * c2 > 8.f;
       if (__any_sync(0xffffffffu, grow)) {
         const float corr = grow ? ex2((m - top) * c2) : 1.f;
         l *= corr;
         if (grow) m = top;
+#pragma unroll 1
+        for (int d = 0; d < 64 * DB; d += 16) {
+          float o[16];
+          tc::tmem_ld16(tO + d, o);
 #pragma unroll
-        for (int d = 0; d < 2 * DB; ++d) {
-          float o[32];
-          tc::tmem_ld32(tO + 32 * d, o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= corr;
-          tc::tmem_st32(tO + 32 * d, o);
+          for (int e = 0; e < 16; ++e) o[e] *= corr;
+          tc::tmem_st16u(tO + d, reinterpret_cast<const uint32_t*>(o));
         }
       }
       if (m == -INFINITY) m = top;
       const float mc = m == -INFINITY ? 0.f : m * c2;
-      float sum[2] = {0.f, 0.f};
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float x0 = ex2(fmaf(s[64 * half + 2 * e], c2, -mc)), x1 = ex2(fmaf(s[64 * half + 2 * e + 1], c2, -mc));
-          sum[0] += x0;
-          sum[1] += x1;
-          pk[e] = pack2<BF16>(x0, x1);
-        }
-        tmem_st32u(tS + 32 * half, pk);
+      for (int q = 0; q < 4; ++q) {
+        uint32_t pk[16] = {};
+        if (used >> q & 1) weights32<BF16>(s + 32 * q, c2, mc, sum, pk);
+        tc::tmem_st16u(tS + 16 * q, pk);
       }
-      l += sum[0] + sum[1];
       tc::fence_before();
       pipe::mbar_arrive(&bar.p_ready[st]);
+      l += sum.x + sum.y;
     }
-    if (x.hi >= 0) {
+    if (w.hi(st) >= 0) {
       if (!warp_wait(&bar.o_full[st], nO++ & 1, abort_flag)) return;
       tc::fence_after();
     }
-    const int i = x.i0 + r;
     if (p >= w.len) l = 0.f;  // padding
+    const int i = row + r;
     const float inv = l > 0.f ? 1.f / l : l != l ? l : 0.f;
-    const int64_t at = w.b * a.y_sb + (int64_t)i * a.y_st + x.h * a.y_sh;
+#pragma unroll 1
+    for (int d = 0; d < 64 * DB; d += 64) {
+      float o[64];
+      if (w.hi(st) >= 0) tmem_ld64(tO + d, o);
 #pragma unroll
-    for (int d = 0; d < 2 * DB; ++d) {
-      float o[32];
-      if (x.hi >= 0) tc::tmem_ld32(tO + 32 * d, o);
+      for (int e = 0; e < 64; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
+      if (P.tma_y) {
+        uint32_t u[32];
+        pack_row(u, o, a.y_dtype);
+        pack_row(u + 16, o + 32, a.y_dtype);
+        if (lane == 0) pipe::bulk_wait_read();  // the store before has read the staging rows
+        __syncwarp();
 #pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
-      if (i < a.Tq) {
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4*>(out + tc::sw128(lane, e, 32)) =
+              make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
+        tc::fence_async_smem();
+        __syncwarp();
+        if (lane == 0 && row + r / 32 * 32 < a.Tq) {
+          tma_store_4d(&P.y.map, d, P.y.use_h ? head : 0, row + r / 32 * 32, P.y.use_b ? w.b : 0, tc::smem_u32(out));
+          pipe::bulk_commit();
+        }
+      } else if (i < a.Tq) {  // fp32
+        float* dst = static_cast<float*>(a.y) + w.b * a.y_sb + (int64_t)i * a.y_st + head * a.y_sh + d;
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
-          if (32 * d + e < D) store8(a.y, a.y_dtype, at + 32 * d + e, o + e);
+        for (int e = 0; e < 64; e += 4)
+          if (d + e < D) *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
       }
     }
     if (a.lse && i < a.Tq)
-      a.lse[((int64_t)w.b * a.H + x.h) * a.Tq + i] = l == 0.f ? -INFINITY : (m * c2 + log2f(l)) * kLn2;
+      a.lse[((int64_t)w.b * a.H + head) * a.Tq + i] = l == 0.f ? -INFINITY : (m * c2 + log2f(l)) * kLn2;
   }
 }
 
-// One thread issues every product.  Per tile and stage: PV of the stage's previous tile (its
-// weights are ready), then S of this one.
+// The warp that issues the products: for each tile and stage PV of the tile before, once its
+// weights are there, and S of this one, in one run.  In order, S(t+1) complete means PV(t)
+// complete.  All waits but the one for the weights come first.
 template <int DB, bool BF16>
 GDNX_DEV void run_products(const FwdParams& P, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
   using Lo = Layout<DB>;
   constexpr uint32_t ID_S = idesc16(BF16, 128, 128, false, false), ID_O = idesc16(BF16, 128, 64 * DB, false, true);
   uint32_t cnt = 0, nP[2] = {0, 0}, nQ[2] = {0, 0};
-  bool pend[2] = {false, false}, first[2] = {false, false}, last[2] = {false, false};
-  uint32_t v_of[2] = {0, 0}, old_v = 0;
-  bool have_old = false;
-  const auto flush = [&](int st) {  // the pending PV of a stage
-    if (!pend[st]) return true;
-    const uint32_t sl = v_of[st] % Lo::SLOTS;
-    if (!pipe::wait_or_abort(&bar.kv_full[sl], v_of[st] / Lo::SLOTS & 1, abort_flag)) return false;
-    if (!pipe::wait_or_abort(&bar.p_ready[st], nP[st]++ & 1, abort_flag)) return false;
-    tc::fence_after();
-    mma_px(tmem + T_O + st * 128, tmem + T_S + st * 128, smem + Lo::KV + sl * Lo::TILE, ID_O, !first[st]);
-    if (last[st]) tc::commit(&bar.o_full[st]);
-    pend[st] = false;
-    return true;
-  };
   for (int64_t n = blockIdx.x; n < P.items; n += gridDim.x) {
     const Item w = make_item(P, n);
-    bool begun[2] = {false, false};
-    for (int i = 0; i < w.count; ++i) {
-      const int kt = w.tile(i);
-      const uint32_t kc = cnt, ksl = kc % Lo::SLOTS;
-      cnt += 2;
+    if (w.count == 0) continue;
+    bool begun[2] = {false, false}, pend[2] = {false, false}, acc[2] = {false, false};
+    uint32_t old = 0;      // V's slot of the tile before
+    for (int i = 0; i <= w.count; ++i) {
+      const bool more = i < w.count;
+      const int kt = more ? w.tile(i) : 1 << 29;
+      const uint32_t ksl = cnt % Lo::SLOTS, k = smem + Lo::KV + ksl * Lo::TILE, v = smem + Lo::KV + old * Lo::TILE;
+      if (more && !warp_wait(&bar.kv_full[ksl], cnt / Lo::SLOTS & 1, abort_flag)) return;
+      if (i > 0 && !warp_wait(&bar.kv_full[old], (cnt - 1) / Lo::SLOTS & 1, abort_flag)) return;
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        if (!flush(st)) return;
-        if (st == 0 && !pipe::wait_or_abort(&bar.kv_full[ksl], kc / Lo::SLOTS & 1, abort_flag)) return;
-        if (st == 1 && have_old) tc::commit(&bar.kv_empty[old_v % Lo::SLOTS]);
-        if (!w.active(st, kt)) continue;
-        if (!begun[st] && !pipe::wait_or_abort(&bar.q_full[st], nQ[st]++ & 1, abort_flag)) return;
-        first[st] = !begun[st];
-        begun[st] = true;
-        last[st] = kt == w.s[st].hi;
+        const uint32_t tS = tmem + T_S + st * 128, tO = tmem + T_O + st * 128;
+        const bool on = more && w.active(st, kt);
+        if (on && !begun[st] && !warp_wait(&bar.q_full[st], nQ[st]++ & 1, abort_flag)) return;
+        if (pend[st] && !warp_wait(&bar.p_ready[st], nP[st]++ & 1, abort_flag)) return;
         tc::fence_after();
-        mma_abt<DB>(tmem + T_S + st * 128, smem + Lo::Q + st * Lo::TILE, smem + Lo::KV + ksl * Lo::TILE, ID_S);
-        tc::commit(&bar.s_full[st]);
-        if (last[st]) tc::commit(&bar.q_empty[st]);
-        pend[st] = true;
-        v_of[st] = kc + 1;
+        if (elect_one()) {
+          if (pend[st]) {
+            mma_px<8>(tO, tS, v, ID_O, acc[st]);
+            if (!on) tc::commit(&bar.o_full[st]);  // a stage's tiles have no gap
+          }
+          if (st == 1 && i > 0) tc::commit(&bar.kv_empty[old]);
+          if (on) {
+            mma_abt<DB>(tS, smem + Lo::Q + st * Lo::TILE, k, ID_S);
+            tc::commit(&bar.s_full[st]);
+            if (kt == w.hi(st)) tc::commit(&bar.q_empty[st]);
+          }
+          if (st == 1 && more) tc::commit(&bar.kv_empty[ksl]);
+        }
+        __syncwarp();
+        acc[st] = acc[st] || pend[st];
+        begun[st] = begun[st] || on;
+        pend[st] = on;
       }
-      tc::commit(&bar.kv_empty[ksl]);
-      old_v = kc + 1;
-      have_old = true;
+      old = (cnt + 1) % Lo::SLOTS;
+      if (more) cnt += 2;
     }
   }
-  if (!flush(0) || !flush(1)) return;
-  if (have_old) tc::commit(&bar.kv_empty[old_v % Lo::SLOTS]);
 }
 
 // The warp that loads: K(0), Q, V(0), K(1), V(1), ... of each item.
@@ -310,12 +342,12 @@ GDNX_DEV void run_loads(const FwdParams& P, uint8_t* base, uint32_t smem, Bars& 
         if (i == 0 && side == 0) {
 #pragma unroll
           for (int st = 0; st < 2; ++st) {
-            if (w.s[st].hi < 0) continue;
+            if (w.hi(st) < 0) continue;
             if (!warp_wait(&bar.q_empty[st], (nQ[st]++ & 1) ^ 1, abort_flag)) return;
             if (lane == 0) {
               const uint32_t mb = tc::smem_u32(&bar.q_full[st]);
               pipe::expect_tx(mb, Lo::TILE);
-              load_rows<DB>(smem + Lo::Q + st * Lo::TILE, P.q, w.s[st].i0, w.s[st].h, w.b, mb);
+              load_rows<DB>(smem + Lo::Q + st * Lo::TILE, P.q, w.row(st), w.head(st), w.b, mb);
             }
           }
         }
@@ -327,15 +359,14 @@ GDNX_DEV void run_loads(const FwdParams& P, uint8_t* base, uint32_t smem, Bars& 
 template <int DB, bool BF16>
 __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_constant__ FwdParams P) {
   using Lo = Layout<DB>;
-  extern __shared__ uint8_t raw[];
-  __shared__ Bars bar;
-  __shared__ uint32_t tmem_at;
-  __shared__ int abort_flag;
-  uint8_t* base = tc::align_smem(raw, 1024);
-  const uint32_t smem = tc::smem_u32(base);
-  const int warp = threadIdx.x / 32;
+  extern __shared__ __align__(1024) uint8_t base[];
+  Small& sm = *reinterpret_cast<Small*>(base + Lo::SMALL);
+  Bars& bar = sm.bar;
+  volatile int* abort_flag = &sm.abort_flag;
+  const uint32_t smem = uniform(tc::smem_u32(base));
+  const int warp = uniform(threadIdx.x / 32);
   if (threadIdx.x == 0) {
-    abort_flag = 0;
+    *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
     for (int i = 0; i < 8; ++i) {
       tc::mbar_init(&bar.kv_full[i], 1);
       tc::mbar_init(&bar.kv_empty[i], 1);
@@ -350,28 +381,31 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
     tc::mbar_init(&bar.fix, 1);
     tc::mbar_init(&bar.done, 1);
   }
-  if (warp == 8) tc::tmem_alloc(&tmem_at, 512);
+  if (warp == 8) tc::tmem_alloc(&sm.tmem_at, 512);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const uint32_t tmem = tmem_at;
-  // 384 threads start with 168 registers each: 2 x 128 x 208 + 128 x 88 is just that
-  if (warp < 8) {
-    regs_up<208>();
-    run_rows<DB, BF16>(P, warp / 4, tmem, bar, &abort_flag);
+  const uint32_t tmem = uniform(sm.tmem_at);
+  if (smem % 1024) {  // never entered: the base is aligned
+  } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 216 + 128 x 72 is just that
+    regs_up<216>();
+    run_rows<DB, BF16>(P, base, tmem, bar, abort_flag);
+    if (threadIdx.x % 32 == 0) pipe::bulk_wait_all();
   } else {
-    regs_down<88>();
-    uint32_t issued = 0;
-    if (warp == 8 && threadIdx.x % 32 == 0) {
-      run_products<DB, BF16>(P, smem, tmem, bar, &abort_flag);
-      tc::commit(&bar.done);  // every product issued has ended before tensor memory is freed
+    regs_down<72>();
+    if (warp == 8) {
+      run_products<DB, BF16>(P, smem, tmem, bar, abort_flag);
+      __syncwarp();
+      if (elect_one()) tc::commit(&bar.done);  // every product issued has ended before tensor memory is freed
       tc::mbar_wait(&bar.done, 0);
-    }
-    if (warp == 9) run_loads<DB>(P, base, smem, bar, &abort_flag, issued);
-    if (warp == 9 && abort_flag && threadIdx.x % 32 == 0) {  // let the copies in flight land
-      for (uint32_t c = issued > Lo::SLOTS ? issued - Lo::SLOTS : 0; c < issued; ++c)
-        tc::mbar_wait(&bar.kv_full[c % Lo::SLOTS], c / Lo::SLOTS & 1, 1u << 16);
-      for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
+    } else if (warp == 9) {
+      uint32_t issued = 0;
+      run_loads<DB>(P, base, smem, bar, abort_flag, issued);
+      if (*abort_flag && threadIdx.x % 32 == 0) {  // let the copies in flight land
+        for (uint32_t c = issued > Lo::SLOTS ? issued - Lo::SLOTS : 0; c < issued; ++c)
+          tc::mbar_wait(&bar.kv_full[c % Lo::SLOTS], c / Lo::SLOTS & 1, 1u << 16);
+        for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
+      }
     }
   }
   __syncwarp();
@@ -379,7 +413,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
   __syncthreads();
   tc::fence_after();
   if (warp == 8) tc::tmem_dealloc(tmem, 512);
-  if (threadIdx.x == 0 && abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
+  if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
 }
 
 template <int DB, bool BF16>
@@ -403,12 +437,18 @@ gdnx_status launch_attn_fwd_tc(const gdnx_attn_args& a, cudaStream_t st) {
   if (!make_tile_map(a.q, a.B, a.Tq, a.H, a.D, &P.q) || !make_tile_map(a.k, a.B, a.Tk, a.Hk, a.D, &P.k) ||
       !make_tile_map(a.v, a.B, a.Tk, a.Hk, a.D, &P.v))
     return GDNX_EUNSUPPORTED;
+  P.tma_y = a.y_dtype != GDNX_F32;
+  if (P.tma_y) {
+    gdnx_view y = {a.y, a.y_dtype, (int32_t)a.D, a.y_sb, a.y_st, a.y_sh, 0, 0};
+    if (!make_tile_map(y, a.B, a.Tq, a.H, a.D, &P.y, 32)) return GDNX_EUNSUPPORTED;
+  }
   P.a = a;
   const int G = (int)(a.H / a.Hk), blocks = (int)((a.Tq + TM - 1) / TM);
   P.by_heads = G % 2 == 0;
   P.pairs = P.by_heads ? G / 2 : G;
   P.units = P.by_heads ? blocks : (blocks + 1) / 2;
   P.items = (int64_t)P.units * a.B * a.Hk * P.pairs;
+  if (P.items >= ((int64_t)1 << 31)) return GDNX_EUNSUPPORTED;
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)

@@ -46,23 +46,42 @@ __host__ __device__ constexpr uint32_t idesc16(bool bf16, int M, int N, bool a_m
          ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// D[128 x 128] = A B^T over the head dimension: both tiles K-major in shared memory.
+// A value that all lanes of a converged warp hold alike, in a form that the compiler knows to be
+// uniform (what is loaded from memory or found from the thread index it does not).
+template <typename T>
+GDNX_DEV T uniform(T x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// One lane of a converged warp.  Products are issued by a whole warp that keeps its state
+// uniform, with only the instructions themselves under the elected lane: their operands then
+// stay in uniform registers (issued from a divergent thread, each product waits for its
+// operands to be moved there, and the issue takes longer than the product runs).
+GDNX_DEV bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
+}
+
+// The issuing thread is one thread: descriptors are built once and stepped by constants (their
+// address field counts 16-byte units), which keeps a product's issue well below its run time.
+
+// D[128 x N] = A B^T over the head dimension: both tiles K-major in shared memory.
 template <int DB>
 GDNX_DEV void mma_abt(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+  const uint64_t da = tc::smem_desc(a, 16, 1024), db = tc::smem_desc(b, 16, 1024);
 #pragma unroll
   for (int k = 0; k < 4 * DB; ++k) {
-    const uint32_t at = (k / 4) * BLOCK_BYTES + (k % 4) * 32;
-    tc::mma_bf16(d, tc::smem_desc(a + at, 16, 1024), tc::smem_desc(b + at, 16, 1024), idesc, k > 0);
+    const uint32_t at = ((k / 4) * BLOCK_BYTES + (k % 4) * 32) >> 4;
+    tc::mma_bf16(d, da + at, db + at, idesc, k > 0);
   }
 }
 
-// D[128 x 64 DB] (+)= P X: P [128 x 128] packed 16-bit in tensor memory, X a tile read with
-// its rows as K.  `acc`: whether D holds a sum already.
-template <int KSTEPS = 8>
+// D[128 x 64 DB] (+)= P X over 16 STEPS keys: P packed 16-bit in tensor memory, X rows of a tile
+// read with its rows as K.  `acc`: whether D holds a sum already.
+template <int STEPS>
 GDNX_DEV void mma_px(uint32_t d, uint32_t p, uint32_t x, uint32_t idesc, bool acc) {
+  const uint64_t dx = tc::smem_desc(x, BLOCK_BYTES, 1024);
 #pragma unroll
-  for (int k = 0; k < KSTEPS; ++k)
-    tc::mma_bf16_ts(d, p + 8 * k, tc::smem_desc(x + k * 2048, BLOCK_BYTES, 1024), idesc, acc || k > 0);
+  for (int k = 0; k < STEPS; ++k) tc::mma_bf16_ts(d, p + 8 * k, dx + k * (2048 >> 4), idesc, acc || k > 0);
 }
 
 // Bounded wait by a whole warp, which leaves together.
@@ -90,7 +109,7 @@ GDNX_DEV float ex2(float x) {
 }
 
 // 32 lanes x 128 consecutive 32-bit columns of tensor memory (the wait is in the same statement, as in tc.cuh).
-GDNX_DEV void tmem_ld128(uint32_t taddr, float (&v)[128]) {
+GDNX_DEV void tmem_ld128(uint32_t taddr, float* v) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -124,7 +143,7 @@ GDNX_DEV void tmem_ld128(uint32_t taddr, float (&v)[128]) {
 }
 
 // 32 lanes x 64 consecutive 32-bit columns of tensor memory (the wait is in the same statement, as in tc.cuh).
-GDNX_DEV void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+GDNX_DEV void tmem_ld64(uint32_t taddr, float* v) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -184,6 +203,59 @@ GDNX_DEV void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
       : "memory");
 }
 
+GDNX_DEV void tmem_st8u(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n\t"
+      "tcgen05.wait::st.sync.aligned;"
+      :
+      : "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+      : "memory");
+}
+
+GDNX_DEV void tma_store_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(src)
+               : "memory");
+}
+
+// Two fp32 operations in one instruction.
+GDNX_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+GDNX_DEV float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// 2^x of two values on the FMA pipes, for x <= 120; below -125 it stays at 2^-125.  x = n + f with
+// |f| <= 1/2 (n by rounding x + 1.5 2^23), 2^f by the polynomial of degree 4 whose relative
+// error over the interval is least (2.6e-6, Remez exchange), n added to the exponent.
+GDNX_DEV float2 ex2_poly(float2 x) {
+  constexpr float kRound = 12582912.f;
+  x.x = fmaxf(x.x, -125.f);
+  x.y = fmaxf(x.y, -125.f);
+  const float2 r = add2(x, make_float2(kRound, kRound));
+  const float2 n = add2(r, make_float2(-kRound, -kRound));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 p = fma2(f, make_float2(0.009570102207f, 0.009570102207f), make_float2(0.05591785908f, 0.05591785908f));
+  p = fma2(p, f, make_float2(0.2402474433f, 0.2402474433f));
+  p = fma2(p, f, make_float2(0.6931217909f, 0.6931217909f));
+  p = fma2(p, f, make_float2(0.9999992847f, 0.9999992847f));
+  p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23));
+  p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23));
+  return p;
+}
+
 // ------------------------------- host side ----------------------------------
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -202,9 +274,10 @@ inline EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// 4-D map {D, head, token, batch} over a [B,T,H,D] view of 16-bit values, box {64, 1, 128, 1},
+// 4-D map {D, head, token, batch} over a [B,T,H,D] view of 16-bit values, box {64, 1, rows, 1},
 // 128-byte swizzle, zeros outside.  False where TMA cannot address the view.
-inline bool make_tile_map(const gdnx_view& v, int64_t B, int64_t T, int64_t H, int64_t D, TileMap* m) {
+inline bool make_tile_map(const gdnx_view& v, int64_t B, int64_t T, int64_t H, int64_t D, TileMap* m,
+                          int rows = TM) {
   if ((v.dtype != GDNX_BF16 && v.dtype != GDNX_F16) || reinterpret_cast<uintptr_t>(v.ptr) % 16 || D % 8) return false;
   const EncodeTiledFn enc = encode_fn();
   if (!enc) return false;
@@ -218,7 +291,7 @@ inline bool make_tile_map(const gdnx_view& v, int64_t B, int64_t T, int64_t H, i
                                  m->use_b ? (cuuint64_t)v.sb * 2 : row};
   for (int i = 0; i < 3; ++i)
     if (strides[i] == 0 || strides[i] % 16 || strides[i] >= (1ull << 40)) return false;
-  const cuuint32_t box[4] = {64, 1, (cuuint32_t)TM, 1};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
   const cuuint32_t es[4] = {1, 1, 1, 1};
   return enc(&m->map, v.dtype == GDNX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
              const_cast<void*>(v.ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,

@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   tc::fence_after();
   const uint32_t tmem = sm.tmem_at;
   const Walk w(P, units, sm.range);
-  if (*abort_flag) {
+  if (smem % 1024) {  // never entered: the base is aligned
   } else if (warp < 4) {
     run_keys<DB, NH, NC, BF16>(P, w, base, tmem, bar, sm.red, abort_flag);
   } else if (warp == 4) {
