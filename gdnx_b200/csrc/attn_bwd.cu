@@ -167,7 +167,7 @@ GDNX_DEV KeyItem key_item(const BwdParams& P) {
   w.b = who / (int)a.Hk;
   w.hk = who % (int)a.Hk;
   w.j0 = w.kt * TM;
-  w.len = seq_len(a, w.b);
+  w.len = uniform(seq_len(a, w.b));
   const int rows = min((int)a.Tq, w.len - off);
   int hi = rows;
   if (w.j0 >= a.sinks) hi = (int)min((int64_t)rows, (int64_t)w.j0 + TM - 1 + a.window - off);
@@ -285,35 +285,47 @@ GDNX_DEV void keys_products(const KeyItem& w, uint32_t smem, uint32_t tmem, Bars
   constexpr uint32_t ID_S = idesc16(true, 128, 128, false, false), ID_O = idesc16(true, 128, 64 * DB, false, true);
   const int n = w.t1 - w.t0;
   const auto slot = [&](uint32_t c) { return smem + Lo::RING + c % SLOTS * Lo::TILE; };
-  const auto landed = [&](uint32_t c) { return pipe::wait_or_abort(&bar.full[c % SLOTS], c / SLOTS & 1, abort_flag); };
+  const auto landed = [&](uint32_t c) { return warp_wait(&bar.full[c % SLOTS], c / SLOTS & 1, abort_flag); };
   const auto scores = [&](int t) {
     if (!landed(2 * t)) return false;
-    mma_abt<DB>(tmem + K_S, smem + Lo::RES, slot(2 * t), ID_S);
-    tc::commit(&bar.s_full[0]);
+    if (elect_one()) {
+      mma_abt<DB>(tmem + K_S, smem + Lo::RES, slot(2 * t), ID_S);
+      tc::commit(&bar.s_full[0]);
+    }
+    __syncwarp();
     return true;
   };
   const auto dprobs = [&](int t) {
     if (!landed(2 * t + 1)) return false;
-    mma_abt<DB>(tmem + K_DP, smem + Lo::RES + Lo::TILE, slot(2 * t + 1), ID_S);
-    tc::commit(&bar.dp_full);
+    if (elect_one()) {
+      mma_abt<DB>(tmem + K_DP, smem + Lo::RES + Lo::TILE, slot(2 * t + 1), ID_S);
+      tc::commit(&bar.dp_full);
+    }
+    __syncwarp();
     return true;
   };
   if (n == 0) return;
-  if (!pipe::wait_or_abort(&bar.res[0], 0, abort_flag) || !scores(0)) return;
-  if (!pipe::wait_or_abort(&bar.res[1], 0, abort_flag) || !dprobs(0)) return;
+  if (!warp_wait(&bar.res[0], 0, abort_flag) || !scores(0)) return;
+  if (!warp_wait(&bar.res[1], 0, abort_flag) || !dprobs(0)) return;
   for (int t = 0; t < n; ++t) {
-    if (!pipe::wait_or_abort(&bar.p_ready, t & 1, abort_flag)) return;
+    if (!warp_wait(&bar.p_ready, t & 1, abort_flag)) return;
     tc::fence_after();
-    mma_halves(tmem + K_DV, tmem + K_S, slot(2 * t + 1), ID_O, t > 0);
-    tc::commit(&bar.empty[(2 * t + 1) % SLOTS]);
+    if (elect_one()) {
+      mma_halves(tmem + K_DV, tmem + K_S, slot(2 * t + 1), ID_O, t > 0);
+      tc::commit(&bar.empty[(2 * t + 1) % SLOTS]);
+    }
+    __syncwarp();
     if (t + 1 < n && !scores(t + 1)) return;
-    if (!pipe::wait_or_abort(&bar.ds_ready[0], t & 1, abort_flag)) return;
+    if (!warp_wait(&bar.ds_ready[0], t & 1, abort_flag)) return;
     tc::fence_after();
-    mma_halves(tmem + K_DK, tmem + K_DP, slot(2 * t), ID_O, t > 0);
-    tc::commit(&bar.empty[(2 * t) % SLOTS]);
+    if (elect_one()) {
+      mma_halves(tmem + K_DK, tmem + K_DP, slot(2 * t), ID_O, t > 0);
+      tc::commit(&bar.empty[(2 * t) % SLOTS]);
+    }
+    __syncwarp();
     if (t + 1 < n && !dprobs(t + 1)) return;
   }
-  tc::commit(&bar.o_full);
+  if (elect_one()) tc::commit(&bar.o_full);
 }
 
 template <int DB>
@@ -360,7 +372,7 @@ GDNX_DEV QueryItem query_item(const BwdParams& P) {
   const int h = (int)(n % a.H);
   n /= a.H;
   const int b = (int)(n % a.B), qt = P.qtiles - 1 - (int)(n / a.B);  // those that see most first
-  const int off = (int)(a.Tk - a.Tq), len = seq_len(a, b);
+  const int off = (int)(a.Tk - a.Tq), len = uniform(seq_len(a, b));
   return {b, h, h / (int)(a.H / a.Hk), qt * TM, qt * TM + off, len,
           KeyTiles(qt * TM + off, min(qt * TM + TM, (int)a.Tq) - 1 + off, len, (int)a.window, (int)a.sinks, TM)};
 }
@@ -435,37 +447,46 @@ GDNX_DEV void queries_products(const QueryItem& w, uint32_t smem, uint32_t tmem,
   constexpr uint32_t ID_S = idesc16(true, 128, 128, false, false), ID_O = idesc16(true, 128, 64 * DB, false, true);
   const int n = w.kt.count;
   const auto slot = [&](uint32_t c) { return smem + Lo::RING + c % SLOTS * Lo::TILE; };
-  const auto landed = [&](uint32_t c) { return pipe::wait_or_abort(&bar.full[c % SLOTS], c / SLOTS & 1, abort_flag); };
+  const auto landed = [&](uint32_t c) { return warp_wait(&bar.full[c % SLOTS], c / SLOTS & 1, abort_flag); };
   const auto scores = [&](int t) {
     if (!landed(2 * t)) return false;
-    mma_abt<DB>(tmem + Q_S + (t & 1) * 128, smem + Lo::RES, slot(2 * t), ID_S);
-    tc::commit(&bar.s_full[t & 1]);
+    if (elect_one()) {
+      mma_abt<DB>(tmem + Q_S + (t & 1) * 128, smem + Lo::RES, slot(2 * t), ID_S);
+      tc::commit(&bar.s_full[t & 1]);
+    }
+    __syncwarp();
     return true;
   };
   const auto dprobs = [&](int t) {
     if (!landed(2 * t + 1)) return false;
-    mma_abt<DB>(tmem + Q_DP, smem + Lo::RES + Lo::TILE, slot(2 * t + 1), ID_S);
-    tc::commit(&bar.dp_full);
-    tc::commit(&bar.empty[(2 * t + 1) % SLOTS]);
+    if (elect_one()) {
+      mma_abt<DB>(tmem + Q_DP, smem + Lo::RES + Lo::TILE, slot(2 * t + 1), ID_S);
+      tc::commit(&bar.dp_full);
+      tc::commit(&bar.empty[(2 * t + 1) % SLOTS]);
+    }
+    __syncwarp();
     return true;
   };
   if (n == 0) return;
-  if (!pipe::wait_or_abort(&bar.res[0], 0, abort_flag) || !scores(0)) return;
-  if (!pipe::wait_or_abort(&bar.res[1], 0, abort_flag) || !dprobs(0)) return;
+  if (!warp_wait(&bar.res[0], 0, abort_flag) || !scores(0)) return;
+  if (!warp_wait(&bar.res[1], 0, abort_flag) || !dprobs(0)) return;
   if (n > 1 && !scores(1)) return;
   for (int t = 0; t < n; ++t) {
     if (t + 1 < n) {
-      if (!pipe::wait_or_abort(&bar.dp_read, t & 1, abort_flag)) return;
+      if (!warp_wait(&bar.dp_read, t & 1, abort_flag)) return;
       tc::fence_after();
       if (!dprobs(t + 1)) return;
     }
-    if (!pipe::wait_or_abort(&bar.ds_ready[t & 1], t / 2 & 1, abort_flag)) return;
+    if (!warp_wait(&bar.ds_ready[t & 1], t / 2 & 1, abort_flag)) return;
     tc::fence_after();
-    mma_halves(tmem + Q_DQ, tmem + Q_S + (t & 1) * 128, slot(2 * t), ID_O, t > 0);
-    tc::commit(&bar.empty[(2 * t) % SLOTS]);
+    if (elect_one()) {
+      mma_halves(tmem + Q_DQ, tmem + Q_S + (t & 1) * 128, slot(2 * t), ID_O, t > 0);
+      tc::commit(&bar.empty[(2 * t) % SLOTS]);
+    }
+    __syncwarp();
     if (t + 2 < n && !scores(t + 2)) return;
   }
-  tc::commit(&bar.o_full);
+  if (elect_one()) tc::commit(&bar.o_full);
 }
 
 template <int DB>
@@ -499,8 +520,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_c
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(base + Lo::BARS + 448);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(base + Lo::BARS + 452);
   static_assert(sizeof(Bars) <= 448, "barriers fit their place");
-  const uint32_t smem = tc::smem_u32(base);
-  const int warp = threadIdx.x / 32;
+  const uint32_t smem = uniform(tc::smem_u32(base));
+  const int warp = uniform(threadIdx.x / 32);
   if (threadIdx.x == 0) {
     *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
     init_bars(bar);
@@ -509,22 +530,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_c
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const uint32_t tmem = *tmem_at;
+  const uint32_t tmem = uniform(*tmem_at);
   if (smem % 1024 == 0) {
     if (KEYS) {
       const KeyItem w = key_item(P);
       if (warp < 8) keys_rows<DB>(P, w, base, tmem, bar, abort_flag);
-      else if (warp == 8 && threadIdx.x % 32 == 0) keys_products<DB>(w, smem, tmem, bar, abort_flag);
+      else if (warp == 8) keys_products<DB>(w, smem, tmem, bar, abort_flag);
       else if (warp == 9) keys_loads<DB>(P, w, base, smem, bar, abort_flag);
     } else {
       const QueryItem w = query_item(P);
       if (warp < 8) queries_rows<DB>(P, w, tmem, bar, abort_flag);
-      else if (warp == 8 && threadIdx.x % 32 == 0) queries_products<DB>(w, smem, tmem, bar, abort_flag);
+      else if (warp == 8) queries_products<DB>(w, smem, tmem, bar, abort_flag);
       else if (warp == 9) queries_loads<DB>(P, w, base, smem, bar, abort_flag);
     }
   }
-  if (warp == 8 && threadIdx.x % 32 == 0) {  // every product issued has ended
-    tc::commit(&bar.done);
+  if (warp == 8) {  // every product issued has ended
+    __syncwarp();
+    if (elect_one()) tc::commit(&bar.done);
     tc::mbar_wait(&bar.done, 0);
   }
   if (warp == 9 && *abort_flag)  // let the copies in flight land

@@ -113,17 +113,44 @@ GDNX_DEV uint32_t range_bits(int lo, int hi, int w) {
   return lo > hi ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
 }
 
-// Weights of 32 columns: p = 2^(c2 s - mc), summed, packed 16-bit.  One pair in eight is taken on
+// Weights of N columns: p = 2^(c2 s - mc), summed, packed 16-bit.  One pair in eight is taken on
 // the FMA pipes (where masked scores give 2^-125: nothing beside a weight that counts).
-template <bool BF16>
-GDNX_DEV void weights32(const float* s, float c2, float mc, float2& sum, uint32_t* pk) {
+template <bool BF16, int N>
+GDNX_DEV void weights(const float* s, float c2, float mc, float2& sum, uint32_t* pk) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
+  for (int e = 0; e < N / 2; ++e) {
     const float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(c2, c2), make_float2(-mc, -mc));
     const float2 p = e % 8 == 3 ? ex2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
     sum = add2(sum, p);
     pk[e] = pack2<BF16>(p.x, p.y);
   }
+}
+
+// A row's running state: the maximum that O and l are scaled to, and the sum.
+struct Row {
+  float m, l;
+};
+
+// Takes a tile's maximum into the row, rescaling O where it lies too far above the old one.
+// Returns what the tile's scores (times c2) are taken against.
+template <int DB>
+GDNX_DEV float take_max(Row& w, float top, float c2, uint32_t tO) {
+  const bool grow = w.m != -INFINITY && (top - w.m) * c2 > 8.f;
+  if (__any_sync(0xffffffffu, grow)) {
+    const float corr = grow ? ex2((w.m - top) * c2) : 1.f;
+    w.l *= corr;
+    if (grow) w.m = top;
+#pragma unroll 1
+    for (int d = 0; d < 64 * DB; d += 16) {
+      float o[16];
+      tc::tmem_ld16(tO + d, o);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] *= corr;
+      tc::tmem_st16u(tO + d, reinterpret_cast<const uint32_t*>(o));
+    }
+  }
+  if (w.m == -INFINITY) w.m = top;
+  return w.m == -INFINITY ? 0.f : w.m * c2;
 }
 
 // 32 values of a row as 16-bit words.
@@ -152,74 +179,73 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
   for (int64_t n = blockIdx.x; n < P.items; n += gridDim.x) {
     const Item w = make_item(P, n);
     if (!w.valid(st)) continue;
-    const int row = w.row(st), head = w.head(st), p0 = row + w.off, p = p0 + r;
-    float m = -INFINITY, l = 0.f;  // the maximum that O and l are scaled to, the sum
+    const int i0 = w.row(st), head = w.head(st), p0 = i0 + w.off, p = p0 + r;
+    Row row = {-INFINITY, 0.f};
     for (int i = 0; i < w.count; ++i) {
       const int kt = w.tile(i), j0 = kt * TM;
       if (!w.active(st, kt)) continue;
       if (!warp_wait(&bar.s_full[st], nS++ & 1, abort_flag)) return;
       tc::fence_after();
-      float s[128], t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      tmem_ld128(tS, s);
-      uint32_t used = 0xf;  // chunks of which some row of the warp sees a column
+      float2 sum = make_float2(0.f, 0.f);
       // does every row see the whole tile?
-      if (!(j0 + TM - 1 <= p0 && p0 + TM <= w.len && (p0 + TM - 1 - j0 < window || j0 + TM <= sinks))) {
+      if (j0 + TM - 1 <= p0 && p0 + TM <= w.len && (p0 + TM - 1 - j0 < window || j0 + TM <= sinks)) {
+        float s[128], t[4];
+        tmem_ld128(tS, s);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) t[f] = s[f];
+#pragma unroll
+        for (int e = 4; e < 128; e += 4)
+#pragma unroll
+          for (int f = 0; f < 4; ++f) t[f] = fmaxf(t[f], s[e + f]);
+        const float mc = take_max<DB>(row, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), c2, tO);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[32];
+          weights<BF16, 64>(s + 64 * half, c2, mc, sum, pk);
+          tmem_st32u(tS + 32 * half, pk);
+        }
+      } else {
+        // chunk by chunk of 32 columns: what no row of the warp sees costs nothing
         // visible columns: lo..hi, and those up to sk
         const int hi = p < w.len ? p - j0 : -1, lo = p - window + 1 - j0, sk = min(sinks - 1 - j0, hi);
-#pragma unroll
+        uint32_t used = 0;
+        float top = -INFINITY;
+#pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           const uint32_t on = range_bits(lo, hi, q) | range_bits(0, sk, q);
-          if (!__any_sync(0xffffffffu, on)) {
-            used &= ~(1u << q);
-          } else if (!__all_sync(0xffffffffu, on == 0xffffffffu)) {
+          if (!__any_sync(0xffffffffu, on)) continue;
+          used |= 1u << q;
+          float s[32];
+          tc::tmem_ld32(tS + 32 * q, s);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) top = fmaxf(top, on >> e & 1 ? s[e] : -INFINITY);
+        }
+        const float mc = take_max<DB>(row, top, c2, tO);
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          uint32_t pk[16] = {};
+          if (used >> q & 1) {
+            const uint32_t on = range_bits(lo, hi, q) | range_bits(0, sk, q);
+            float s[32];
+            tc::tmem_ld32(tS + 32 * q, s);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (!(on >> e & 1)) s[32 * q + e] = -INFINITY;
+              if (!(on >> e & 1)) s[e] = -INFINITY;
+            weights<BF16, 32>(s, c2, mc, sum, pk);
           }
+          tc::tmem_st16u(tS + 16 * q, pk);  // over scores that have been read
         }
       }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (!(used >> q & 1)) continue;
-#pragma unroll
-        for (int e = 0; e < 32; e += 8)
-#pragma unroll
-          for (int f = 0; f < 4; ++f) t[f] = fmaxf(fmaxf(t[f], s[32 * q + e + f]), s[32 * q + e + f + 4]);
-      }
-      const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-      const bool grow = m != -INFINITY && (top - m) * c2 > 8.f;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float corr = grow ? ex2((m - top) * c2) : 1.f;
-        l *= corr;
-        if (grow) m = top;
-#pragma unroll 1
-        for (int d = 0; d < 64 * DB; d += 16) {
-          float o[16];
-          tc::tmem_ld16(tO + d, o);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] *= corr;
-          tc::tmem_st16u(tO + d, reinterpret_cast<const uint32_t*>(o));
-        }
-      }
-      if (m == -INFINITY) m = top;
-      const float mc = m == -INFINITY ? 0.f : m * c2;
-      float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t pk[16] = {};
-        if (used >> q & 1) weights32<BF16>(s + 32 * q, c2, mc, sum, pk);
-        tc::tmem_st16u(tS + 16 * q, pk);
-      }
+      row.l += sum.x + sum.y;
       tc::fence_before();
       pipe::mbar_arrive(&bar.p_ready[st]);
-      l += sum.x + sum.y;
     }
     if (w.hi(st) >= 0) {
       if (!warp_wait(&bar.o_full[st], nO++ & 1, abort_flag)) return;
       tc::fence_after();
     }
-    if (p >= w.len) l = 0.f;  // padding
-    const int i = row + r;
+    const float l = p < w.len ? row.l : 0.f;  // padding
+    const int i = i0 + r;
     const float inv = l > 0.f ? 1.f / l : l != l ? l : 0.f;
 #pragma unroll 1
     for (int d = 0; d < 64 * DB; d += 64) {
@@ -239,8 +265,8 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
               make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
         tc::fence_async_smem();
         __syncwarp();
-        if (lane == 0 && row + r / 32 * 32 < a.Tq) {
-          tma_store_4d(&P.y.map, d, P.y.use_h ? head : 0, row + r / 32 * 32, P.y.use_b ? w.b : 0, tc::smem_u32(out));
+        if (lane == 0 && i0 + r / 32 * 32 < a.Tq) {
+          tma_store_4d(&P.y.map, d, P.y.use_h ? head : 0, i0 + r / 32 * 32, P.y.use_b ? w.b : 0, tc::smem_u32(out));
           pipe::bulk_commit();
         }
       } else if (i < a.Tq) {  // fp32
@@ -251,7 +277,7 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
       }
     }
     if (a.lse && i < a.Tq)
-      a.lse[((int64_t)w.b * a.H + head) * a.Tq + i] = l == 0.f ? -INFINITY : (m * c2 + log2f(l)) * kLn2;
+      a.lse[((int64_t)w.b * a.H + head) * a.Tq + i] = l == 0.f ? -INFINITY : (row.m * c2 + log2f(l)) * kLn2;
   }
 }
 
@@ -387,12 +413,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
   tc::fence_after();
   const uint32_t tmem = uniform(sm.tmem_at);
   if (smem % 1024) {  // never entered: the base is aligned
-  } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 216 + 128 x 72 is just that
-    regs_up<216>();
+  } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 232 + 128 x 40 is just that
+    regs_up<232>();
     run_rows<DB, BF16>(P, base, tmem, bar, abort_flag);
     if (threadIdx.x % 32 == 0) pipe::bulk_wait_all();
   } else {
-    regs_down<72>();
+    regs_down<40>();
     if (warp == 8) {
       run_products<DB, BF16>(P, smem, tmem, bar, abort_flag);
       __syncwarp();
