@@ -653,11 +653,8 @@ gdnx_status run(const gdnx_attn_bwd_args& g, BwdParams& P, cudaStream_t st) {
   const auto keys = attn_bwd_tc_kernel<DB, true>;
   const auto queries = attn_bwd_tc_kernel<DB, false>;
   constexpr int smem = (int)Layout<DB>::SMEM;
-  if (cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-      cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-    cudaGetLastError();
-    return GDNX_ELAUNCH;
-  }
+  static std::atomic<uint64_t> done_keys, done_queries;
+  if (!allow_smem(keys, smem, done_keys) || !allow_smem(queries, smem, done_queries)) return GDNX_ELAUNCH;
   const int64_t rows = (int64_t)stats_floats(P);
   attn_stats_kernel<__nv_bfloat16><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(
       g, const_cast<float*>(P.lse2), const_cast<float*>(P.delta), P.qtiles * TM);

@@ -445,10 +445,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
 template <int DB, bool BF16>
 gdnx_status launch(const FwdParams& P, int sms, cudaStream_t st) {
   const auto kernel = attn_fwd_tc_kernel<DB, BF16>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Layout<DB>::SMEM) != cudaSuccess) {
-    cudaGetLastError();
-    return GDNX_ELAUNCH;
-  }
+  static std::atomic<uint64_t> done;
+  if (!allow_smem(kernel, (int)Layout<DB>::SMEM, done)) return GDNX_ELAUNCH;
   const unsigned grid = (unsigned)(P.items < sms ? P.items : sms);
   kernel<<<grid, NTHREADS, Layout<DB>::SMEM, st>>>(P);
   return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
@@ -475,10 +473,7 @@ gdnx_status launch_attn_fwd_tc(const gdnx_attn_args& a, cudaStream_t st) {
   P.units = P.by_heads ? blocks : (blocks + 1) / 2;
   P.items = (int64_t)P.units * a.B * a.Hk * P.pairs;
   if (P.items >= ((int64_t)1 << 31)) return GDNX_EUNSUPPORTED;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return GDNX_ELAUNCH;
+  const int sms = sm_count();
   const bool bf16 = a.q.dtype == GDNX_BF16;
   if (a.D > 64) return bf16 ? launch<2, true>(P, sms, st) : launch<2, false>(P, sms, st);
   return bf16 ? launch<1, true>(P, sms, st) : launch<1, false>(P, sms, st);

@@ -7,6 +7,7 @@
 // Head sizes below a multiple of 64 are filled with zeros by TMA, as rows beyond T are.
 #pragma once
 
+#include <atomic>
 #include <cuda.h>
 
 #include "attn_common.cuh"
@@ -272,6 +273,35 @@ inline EncodeTiledFn encode_fn() {
     return EncodeTiledFn(nullptr);
   }();
   return fn;
+}
+
+// The device's number of SMs, and whether a kernel may use `smem` bytes of dynamic shared memory
+// there (set on its first launch on a device: `done` has a bit for each).
+inline int sm_count() {
+  static std::atomic<int> sms[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 148;
+  int n = sms[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+      cudaGetLastError();
+      return 148;
+    }
+    sms[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+template <typename F>
+bool allow_smem(F kernel, int smem, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  if (dev < 64) done.fetch_or(1ull << dev);
+  return true;
 }
 
 // 4-D map {D, head, token, batch} over a [B,T,H,D] view of 16-bit values, box {64, 1, rows, 1},

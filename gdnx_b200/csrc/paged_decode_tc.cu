@@ -604,25 +604,13 @@ Plan plan(const gdnx_paged_decode_args& a, int sms) {
   return p;
 }
 
-int sm_count() {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return 148;
-  }
-  return sms;
-}
-
 template <int DB, int NC, bool BF16>
 gdnx_status launch(const DecParams& P, cudaStream_t st) {
   constexpr int NH = NC > 16 ? 32 : 16;
   const auto kernel = paged_decode_tc_kernel<DB, NC, BF16>;
   constexpr int smem = (int)Layout<DB, NH>::SMEM;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-    cudaGetLastError();
-    return GDNX_ELAUNCH;
-  }
+  static std::atomic<uint64_t> done;
+  if (!allow_smem(kernel, smem, done)) return GDNX_ELAUNCH;
   kernel<<<(unsigned)P.grid, NTHREADS, smem, st>>>(P);
   paged_decode_join_kernel<NH><<<(unsigned)(P.a.B * P.a.H), JOIN_WARPS * 32, 0, st>>>(P);
   return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;

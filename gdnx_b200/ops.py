@@ -890,66 +890,77 @@ def gdn3_scan_train(q, k, v, b_gate, w_gate, decay, *, decay_kind="gamma", state
 _ERRORS = {}
 
 
-def _error_word(device):
-    """Address of the word that takes a device error of the attention kernels on ``device``
+def _error_word(index: int) -> int:
+    """Address of the word that takes a device error of the attention kernels on device ``index``
     (one per device, read by :func:`device_status`; it stays set)."""
-    word = _ERRORS.get(device.index)
+    word = _ERRORS.get(index)
     if word is None:
-        word = torch.zeros(4, dtype=torch.uint8, device=device)
-        torch.cuda.current_stream(device).synchronize()  # other streams write it too
-        _ERRORS[device.index] = word
+        word = torch.zeros(4, dtype=torch.uint8, device=torch.device("cuda", index))
+        torch.cuda.current_stream(index).synchronize()  # other streams write it too
+        _ERRORS[index] = word
     return word.data_ptr()
+
+
+def _enqueue(name: str, index: int, *args) -> None:
+    """Call a C entry point with device ``index`` current and that device's current stream."""
+    fn = getattr(L.load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        L.check(fn(*args, stream), name)
+    else:
+        with torch.cuda.device(index):
+            L.check(fn(*args, stream), name)
 
 
 def _heads_view(t: torch.Tensor) -> L.View:
     """View of a [B,T,H,D] tensor."""
-    s = t.stride()
-    if t.shape[-1] > 1 and s[-1] != 1:
+    sb, st, sh, sd = t.stride()
+    d = t.shape[3]
+    if sd != 1 and d > 1:
         raise ValueError("the last dim of every input must be contiguous")
-    return L.View(t.data_ptr(), _DT[t.dtype], t.shape[-1], s[0], s[1], s[2], 0, 0)
+    return L.View(t.data_ptr(), _DT[t.dtype], d, sb, st, sh)
 
 
-def _same_device(first, *ts):
+def _on_device(index: int, *ts) -> None:
+    """All of ``ts`` (None: absent) on CUDA device ``index``."""
     for t in ts:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
+            _require_cuda(t)
             raise ValueError("all tensors must be on one device")
 
 
-def _index32(t, n, name, device):
-    """A contiguous int32 vector of n (any n where None) on ``device``."""
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+def _index32(t, n, name, index):
+    """Address of a contiguous int32 vector of n (any n where None) on device ``index``."""
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
         raise ValueError(f"{name} must be a contiguous int32 vector" + ("" if n is None else f" of {n}"))
-    _require_cuda(t)
-    if t.device != device:
-        raise ValueError("all tensors must be on one device")
-    return t
+    _on_device(index, t)
+    return t.data_ptr()
 
 
 def _attn_args(q, k, v, window, sinks, scale, lengths):
     _require_cuda(q, k, v, lengths)
-    _same_device(q, k, v, lengths)
+    index = q.get_device()
+    _on_device(index, k, v, lengths)
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         raise ValueError("q must be [B,Tq,H,D], k and v [B,Tk,Hk,D]")
     B, Tq, H, D = q.shape
-    Tk, Hk = k.shape[1:3]
-    if k.shape[0] != B or k.shape[3] != D or Hk == 0 or H % Hk:
+    Bk, Tk, Hk, Dk = k.shape
+    if Bk != B or Dk != D or Hk == 0 or H % Hk:
         raise ValueError("k and v must have q's batch and head size, and a number of heads that divides q's")
     if Tq > Tk:
         raise ValueError("the queries are the last Tq of Tk positions: Tq must not exceed Tk")
-    if q.dtype not in _DT or k.dtype != q.dtype or v.dtype != q.dtype:
+    dt = q.dtype
+    if dt not in _DT or k.dtype is not dt or v.dtype is not dt:
         raise TypeError("q, k and v must be all float32, all bfloat16 or all float16")
-    window = max(Tk, 1) if window is None else window
+    if window is None:
+        window = max(Tk, 1)
     if window < 1 or sinks < 0:
         raise ValueError("window must be at least 1 (None: no window), sinks at least 0")
-    a = L.AttnArgs()
-    a.B, a.Tq, a.Tk, a.H, a.Hk, a.D = B, Tq, Tk, H, Hk, D
-    a.window, a.sinks = min(window, 1 << 62), min(sinks, 1 << 62)
-    a.scale = D ** -0.5 if scale is None else scale
-    a.q, a.k, a.v = _heads_view(q), _heads_view(k), _heads_view(v)
-    if lengths is not None:
-        a.lengths = _index32(lengths, B, "lengths", q.device).data_ptr()
-    a.error = _error_word(q.device)
-    return a
+    n = None if lengths is None else _index32(lengths, B, "lengths", index)
+    a = L.AttnArgs(B, Tq, Tk, H, Hk, D, min(window, 1 << 62), min(sinks, 1 << 62), D ** -0.5 if scale is None else scale,
+                   _heads_view(q), _heads_view(k), _heads_view(v), n)
+    a.error = _error_word(index)
+    return a, index
 
 
 def window_attention(q, k, v, *, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
@@ -964,21 +975,21 @@ def window_attention(q, k, v, *, window: Optional[int] = None, sinks: int = 0, s
     sequences: keys from there on are not seen, and queries from there on give zeros, whatever the
     padding holds.  ``scale`` defaults to D ** -0.5.  Returns y [B,Tq,H,D] (and the log of the sum
     of exponentials [B,H,Tq] fp32 if asked, -inf where a row is padding)."""
-    a = _attn_args(q, k, v, window, sinks, scale, lengths)
-    y = out if out is not None else torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
-    if out is not None:
-        _require_cuda(out)
-        _same_device(q, out)
-        if out.shape != q.shape or out.dtype not in _DT or (out.shape[-1] > 1 and out.stride(-1) != 1):
+    a, index = _attn_args(q, k, v, window, sinks, scale, lengths)
+    if out is None:
+        y = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+    else:
+        y = out
+        _on_device(index, y)
+        if y.shape != q.shape or y.dtype not in _DT or (y.shape[-1] > 1 and y.stride(-1) != 1):
             raise ValueError("out must be [B,Tq,H,D] with a contiguous last dim")
     a.y, a.y_dtype = y.data_ptr(), _DT[y.dtype]
-    a.y_sb, a.y_st, a.y_sh = y.stride()[:3]
+    a.y_sb, a.y_st, a.y_sh, _ = y.stride()
     lse = None
     if return_lse:
         lse = torch.empty(a.B, a.H, a.Tq, dtype=torch.float32, device=q.device)
         a.lse = lse.data_ptr()
-    with torch.cuda.device(q.device):
-        L.check(L.load().gdnx_attn_fwd(C.byref(a), C.c_void_p(_stream(q.device))), "gdnx_attn_fwd")
+    _enqueue("gdnx_attn_fwd", index, C.byref(a))
     return (y, lse) if return_lse else y
 
 
@@ -994,23 +1005,18 @@ class _WindowAttentionFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         q, k, v, y, lse, lengths = ctx.saved_tensors
-        g = L.AttnBwdArgs()
-        g.fwd = a = _attn_args(q, k, v, *ctx.mask, lengths)
+        a, index = _attn_args(q, k, v, *ctx.mask, lengths)
         a.y, a.y_dtype = y.data_ptr(), _DT[y.dtype]
-        a.y_sb, a.y_st, a.y_sh = y.stride()[:3]
+        a.y_sb, a.y_st, a.y_sh, _ = y.stride()
         a.lse = lse.data_ptr()
-        g.fwd = a
         if dy.shape[-1] > 1 and dy.stride(-1) != 1:
             dy = dy.contiguous()
-        g.dy = _heads_view(dy)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        g.dq, g.dk, g.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        lib = L.load()
-        need = lib.gdnx_attn_bwd_workspace_bytes(C.byref(g))
+        g = L.AttnBwdArgs(a, _heads_view(dy), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+        need = L.load().gdnx_attn_bwd_workspace_bytes(C.byref(g))
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
         g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel()
-        with torch.cuda.device(q.device):
-            L.check(lib.gdnx_attn_bwd(C.byref(g), C.c_void_p(_stream(q.device))), "gdnx_attn_bwd")
+        _enqueue("gdnx_attn_bwd", index, C.byref(g))
         return dq, dk, dv, None, None, None, None
 
 
@@ -1047,34 +1053,30 @@ class PagedCache:
                           torch.zeros(pages, **i32), torch.zeros(1, **i32))
 
 
-def _cache_struct(c: PagedCache) -> L.Cache:
+def _cache_struct(c: PagedCache):
+    """The cache as the C ABI takes it, and its device's index."""
     kv, table = c.kv, c.table
     _require_cuda(kv)
+    index = kv.get_device()
     if kv.dim() != 6 or kv.shape[1] != 2 or not kv.is_contiguous() or kv.dtype not in _DT:
         raise ValueError("kv must be contiguous [L, 2, pages, Hk, page, D] in float32, bfloat16 or float16")
-    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or not table.is_cuda:
-        raise ValueError("table must be a contiguous int32 CUDA tensor [slots, width]")
-    _same_device(kv, table)
-    dev = kv.device
-    n_l, _, pages, hk, page, d = kv.shape
+    if table.dtype is not torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise ValueError("table must be a contiguous int32 tensor [slots, width]")
+    _on_device(index, table)
+    layers, _, pages, hk, page, d = kv.shape
     slots, width = table.shape
-    return L.Cache(kv.data_ptr(), _DT[kv.dtype], page, n_l, pages, hk, d, slots, width, table.data_ptr(),
-                   _index32(c.lengths, slots, "lengths", dev).data_ptr(),
-                   _index32(c.refs, pages, "refs", dev).data_ptr(),
-                   _index32(c.status, 1, "status", dev).data_ptr())
+    return L.Cache(kv.data_ptr(), _DT[kv.dtype], page, layers, pages, hk, d, slots, width, table.data_ptr(),
+                   _index32(c.lengths, slots, "lengths", index), _index32(c.refs, pages, "refs", index),
+                   _index32(c.status, 1, "status", index)), index
 
 
-def _cache_rows(rows, c, name="rows", n=None):
-    t = _index32(rows, n, name, c.kv.device)
-    if t.shape[0] > c.table.shape[0]:
+def _cache_rows(rows, s, index, name="rows"):
+    """Address and number of a list of slots."""
+    at = _index32(rows, None, name, index)
+    n = rows.shape[0]
+    if n > s.slots:
         raise ValueError(f"{name} names more slots than there are")
-    return t
-
-
-def _cache_call(name, c, *args):
-    dev = c.kv.device
-    with torch.cuda.device(dev):
-        L.check(getattr(L.load(), name)(*args, C.c_void_p(_stream(dev))), name)
+    return at, n
 
 
 def cache_check(cache: PagedCache) -> None:
@@ -1088,23 +1090,21 @@ def cache_check(cache: PagedCache) -> None:
 def cache_fork(cache: PagedCache, src: torch.Tensor, dst: torch.Tensor) -> None:
     """Slot ``dst[i]`` releases what it holds and becomes a copy of slot ``src[i]`` that shares its
     pages.  ``src``, ``dst``: int32 vectors; no slot twice in ``dst`` nor in both."""
-    s = _cache_struct(cache)
-    dst = _cache_rows(dst, cache, "dst")
-    src = _index32(src, dst.shape[0], "src", cache.kv.device)
-    _cache_call("gdnx_cache_fork", cache, C.byref(s), dst.shape[0], src.data_ptr(), dst.data_ptr())
+    s, index = _cache_struct(cache)
+    to, n = _cache_rows(dst, s, index, "dst")
+    _enqueue("gdnx_cache_fork", index, C.byref(s), n, _index32(src, n, "src", index), to)
 
 
 def cache_extend(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor) -> None:
     """Room for ``counts[i]`` more tokens in slot ``rows[i]`` (int32 vectors, each slot once): its
     length grows, and it takes free pages, the lowest first, in the order of ``rows``.  A partly
     filled last page that other slots share is copied first, in every layer."""
-    s = _cache_struct(cache)
-    rows = _cache_rows(rows, cache)
-    n = rows.shape[0]
-    counts = _index32(counts, n, "counts", cache.kv.device)
+    s, index = _cache_struct(cache)
+    at, n = _cache_rows(rows, s, index)
+    more = _index32(counts, n, "counts", index)
     need = L.load().gdnx_cache_workspace_bytes(C.byref(s), n)
     ws = torch.empty(need, dtype=torch.uint8, device=cache.kv.device)
-    _cache_call("gdnx_cache_extend", cache, C.byref(s), n, rows.data_ptr(), counts.data_ptr(), ws.data_ptr(), need)
+    _enqueue("gdnx_cache_extend", index, C.byref(s), n, at, more, ws.data_ptr(), need)
 
 
 def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, *, layer: int = 0,
@@ -1112,30 +1112,27 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, rows: torch
     """The keys and values ``k``, ``v`` [n,T,Hk,D] of slot ``rows[i]``'s last T tokens in ``layer``
     (after :func:`cache_extend`); with ``counts`` [n] int32, row i's first ``counts[i]`` of T are its
     last ``counts[i]`` tokens (a right-padded prompt)."""
-    s = _cache_struct(cache)
-    _require_cuda(k, v)
-    _same_device(cache.kv, k, v)
-    rows = _index32(rows, None, "rows", cache.kv.device)
+    s, index = _cache_struct(cache)
+    _on_device(index, k, v)
+    at = _index32(rows, None, "rows", index)
     n = rows.shape[0]
-    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != n or k.shape[2:] != (s.Hk, s.D):
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != n or k.shape[2] != s.Hk or k.shape[3] != s.D:
         raise ValueError("k and v must be [n,T,Hk,D] with the cache's heads")
-    if k.dtype != cache.kv.dtype or v.dtype != cache.kv.dtype:
+    if k.dtype is not cache.kv.dtype or v.dtype is not cache.kv.dtype:
         raise TypeError("k and v must have the cache's type")
     if not 0 <= layer < s.L:
         raise ValueError("no such layer")
-    kv, vv = _heads_view(k), _heads_view(v)
-    cp = None if counts is None else _index32(counts, n, "counts", cache.kv.device).data_ptr()
-    _cache_call("gdnx_cache_write", cache, C.byref(s), layer, n, k.shape[1], C.byref(kv), C.byref(vv), rows.data_ptr(),
-                cp)
+    first = None if counts is None else _index32(counts, n, "counts", index)
+    _enqueue("gdnx_cache_write", index, C.byref(s), layer, n, k.shape[1], C.byref(_heads_view(k)),
+             C.byref(_heads_view(v)), at, first)
 
 
 def cache_truncate(cache: PagedCache, rows: torch.Tensor, lengths: torch.Tensor) -> None:
     """Slot ``rows[i]`` keeps its first ``lengths[i]`` tokens (int32 vectors, each slot once) and
     releases the pages beyond; 0 frees the slot."""
-    s = _cache_struct(cache)
-    rows = _cache_rows(rows, cache)
-    lengths = _index32(lengths, rows.shape[0], "lengths", cache.kv.device)
-    _cache_call("gdnx_cache_truncate", cache, C.byref(s), rows.shape[0], rows.data_ptr(), lengths.data_ptr())
+    s, index = _cache_struct(cache)
+    at, n = _cache_rows(rows, s, index)
+    _enqueue("gdnx_cache_truncate", index, C.byref(s), n, at, _index32(lengths, n, "lengths", index))
 
 
 def cache_trim(cache: PagedCache, rows: torch.Tensor, *, window: int, sinks: int = 0) -> None:
@@ -1143,18 +1140,18 @@ def cache_trim(cache: PagedCache, rows: torch.Tensor, *, window: int, sinks: int
     or a later one sees through ``window``."""
     if window < 1 or sinks < 0:
         raise ValueError("window must be at least 1, sinks at least 0")
-    s = _cache_struct(cache)
-    rows = _cache_rows(rows, cache)
-    _cache_call("gdnx_cache_trim", cache, C.byref(s), rows.shape[0], rows.data_ptr(), window, sinks)
+    s, index = _cache_struct(cache)
+    at, n = _cache_rows(rows, s, index)
+    _enqueue("gdnx_cache_trim", index, C.byref(s), n, at, window, sinks)
 
 
 def cache_compact(cache: PagedCache) -> None:
     """Moves the live pages down so that they are the pool's first: page for page in order, those
     above the live count into the free ones below it."""
-    s = _cache_struct(cache)
+    s, index = _cache_struct(cache)
     need = L.load().gdnx_cache_workspace_bytes(C.byref(s), 0)
     ws = torch.empty(need, dtype=torch.uint8, device=cache.kv.device)
-    _cache_call("gdnx_cache_compact", cache, C.byref(s), ws.data_ptr(), need)
+    _enqueue("gdnx_cache_compact", index, C.byref(s), ws.data_ptr(), need)
 
 
 def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Optional[torch.Tensor] = None,
@@ -1166,44 +1163,42 @@ def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Op
     the slot's tokens within ``window`` (None: all) and the first ``sinks``; tokens on released pages
     are not seen.  A slot of length 0 gives zeros.  ``max_len``, if known, is the longest slot's
     length; it only sizes the split over the cache's length.  Returns [B,H,D]."""
-    s = _cache_struct(cache)
-    _require_cuda(q, out)
-    _same_device(cache.kv, q, out)
-    if q.dim() != 3 or q.shape[2] != s.D or q.shape[1] == 0 or q.shape[1] % s.Hk:
+    s, index = _cache_struct(cache)
+    _on_device(index, q)
+    if q.dim() != 3:
+        raise ValueError("q must be [B,H,D]")
+    B, H, D = q.shape
+    if D != s.D or H == 0 or H % s.Hk:
         raise ValueError("q must be [B,H,D] with the cache's head size and H a multiple of its heads")
-    if q.dtype != cache.kv.dtype:
+    if q.dtype is not cache.kv.dtype:
         raise TypeError("q must have the cache's type")
-    window = (1 << 62) if window is None else window
+    if window is None:
+        window = 1 << 62
     if window < 1 or sinks < 0:
         raise ValueError("window must be at least 1 (None: no window), sinks at least 0")
     if not 0 <= layer < s.L:
         raise ValueError("no such layer")
-    B, H, D = q.shape
-    dev = q.device
-    y = out if out is not None else torch.empty(q.shape, dtype=out_dtype or q.dtype, device=dev)
-    if out is not None and (out.shape != q.shape or out.dtype not in _DT or out.stride(-1) != 1):
-        raise ValueError("out must be [B,H,D] with a contiguous last dim")
-    if q.stride(-1) != 1:
+    if out is None:
+        y = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+    else:
+        y = out
+        _on_device(index, y)
+        if y.shape != q.shape or y.dtype not in _DT or y.stride(-1) != 1:
+            raise ValueError("out must be [B,H,D] with a contiguous last dim")
+    qb, qh, qd = q.stride()
+    if qd != 1:
         raise ValueError("the last dim of every input must be contiguous")
-    a = L.PagedDecodeArgs()
-    a.cache = s
-    a.B, a.H, a.layer, a.window, a.sinks = B, H, layer, min(window, 1 << 62), min(sinks, 1 << 62)
-    a.max_len = max_len or 0
-    a.scale = D ** -0.5 if scale is None else scale
-    a.q = L.View(q.data_ptr(), _DT[q.dtype], D, q.stride(0), 0, q.stride(1), 0, 0)
-    if rows is not None:
-        a.rows = _index32(rows, B, "rows", dev).data_ptr()
-    elif B > s.slots:
+    if rows is None and B > s.slots:
         raise ValueError("more queries than slots")
-    a.y, a.y_dtype = y.data_ptr(), _DT[y.dtype]
-    a.y_sb, a.y_sh = y.stride()[:2]
-    a.error = _error_word(dev)
-    lib = L.load()
-    need = lib.gdnx_paged_decode_workspace_bytes(C.byref(a))
+    yb, yh, _ = y.stride()
+    a = L.PagedDecodeArgs(s, B, H, layer, min(window, 1 << 62), min(sinks, 1 << 62), max_len or 0,
+                          D ** -0.5 if scale is None else scale, L.View(q.data_ptr(), _DT[q.dtype], D, qb, 0, qh),
+                          None if rows is None else _index32(rows, B, "rows", index), y.data_ptr(), _DT[y.dtype], yb, yh,
+                          _error_word(index))
+    need = L.load().gdnx_paged_decode_workspace_bytes(C.byref(a))
     ws = None
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    with torch.cuda.device(dev):
-        L.check(lib.gdnx_paged_decode(C.byref(a), C.c_void_p(_stream(dev))), "gdnx_paged_decode")
+    _enqueue("gdnx_paged_decode", index, C.byref(a))
     return y
