@@ -6,7 +6,8 @@
 // evenly over the CTAs (one on each SM), so that mixed lengths leave none waiting: a CTA takes
 // the end of one unit, whole units, the beginning of another.  Whole units are written at
 // once; parts leave maximum, sum and unnormalised output, and a second kernel joins them in
-// order.  Every CTA finds its range from the lengths by itself.
+// order.  Every CTA finds its range from the lengths by itself.  Where no unit can have more
+// than four tiles, a CTA takes whole units and there is nothing to join.
 //
 // A tile.  With the keys as rows the products are narrow and nothing is padded to 128 but the
 // heads to NH:  S^T [128 keys x NH] = K Q^T,  O^T [128 dims x NH] += V^T P  (V read with its
@@ -26,31 +27,40 @@ namespace {
 
 using namespace attn;
 
-constexpr int NTHREADS = 192;   // four warps of keys, one that issues products, one that loads
+constexpr int NTHREADS = 224;  // four warps of keys, one that issues products, one that loads, one for the queries
+constexpr int WHOLE_TILES = 4;  // units of up to so many tiles are not cut
+
+// A unit that was cut: its parts lie in CTAs c0..c1.  c1 < 0: none.
+struct Joint {
+  int b, unit, c0, c1;
+};
 
 struct DecParams {
   CUtensorMap kv;  // {D, Hk * page, L * 2 * pages}
   gdnx_paged_decode_args a;
   float* part;     // [grid][2][NH][128] unnormalised outputs of a CTA's first and last unit
   float* stat;     // [grid][2][NH][2] maximum (log2 domain) and sum
+  Joint* joint;    // [grid] the unit cut in several parts that ends in a CTA
   int grid, groups;
+  int whole;       // no unit is cut: a CTA takes whole units
   int vec_q;       // q's rows are 16-byte aligned
 };
 
 struct Bars {
-  uint64_t full[12], empty[12], q_ready[2], s_full[2], p_ready[2], pv_done[2], done;
+  uint64_t full[12], empty[12], q_ready[2], q_empty[2], s_full[2], p_ready[2], pv_done[2], done;
 };
 
 // The place of a CTA in the row of all tiles: its tiles t0..t1-1, the sequence b that holds t0
 // and the tiles of the sequences before b.  Tiles are ordered by sequence, unit, tile.
 struct Range {
-  int64_t t0, t1, before, b;
+  int64_t t0, t1, before, b, per;
 };
 
 template <int NH>
 struct Small {
   Bars bar;
   Range range;
+  long long sums[NTHREADS / 32];
   float red[4 * NH];
   uint32_t tmem_at;
   int abort_flag;
@@ -89,40 +99,50 @@ GDNX_DEV Seq make_seq(const gdnx_paged_decode_args& a, int64_t b) {
 
 GDNX_DEV int tiles_of(const gdnx_paged_decode_args& a, int64_t b) { return make_seq(a, b).kt.count; }
 
-// One warp finds the range: tiles of all sequences, 32 at a time.
-GDNX_DEV Range find_range(const DecParams& P, int units) {
-  const int lane = threadIdx.x % 32;
-  int64_t total = 0;
-  for (int64_t b = lane; b < P.a.B; b += 32) total += tiles_of(P.a, b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  total *= units;
-  const int64_t per = (total + P.grid - 1) / P.grid;
-  Range r;
-  r.t0 = min((int64_t)blockIdx.x * per, total);
-  r.t1 = min(r.t0 + per, total);
-  r.b = r.before = 0;
-  if (r.t0 >= r.t1) return r;
-  int64_t before = 0;
-  for (int64_t base = 0; base < P.a.B; base += 32) {
-    const int64_t b = base + lane;
-    const int64_t n = b < P.a.B ? (int64_t)tiles_of(P.a, b) * units : 0;
-    int64_t s = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
+// The CTA finds its range: every thread adds up a run of sequences, and the one whose run holds
+// the range's first tile walks to its sequence.  (Whole units: t0 and t1 count units.)
+GDNX_DEV void find_range(const DecParams& P, int units, Range& out, long long* sums) {
+  if (P.whole) {
+    if (threadIdx.x == 0) {
+      const int64_t all = P.a.B * units;
+      out = {all * blockIdx.x / P.grid, all * (blockIdx.x + 1) / P.grid, 0, 0, 0};
     }
-    const uint32_t here = __ballot_sync(0xffffffffu, before + s > r.t0);
-    if (here) {
-      const int who = __ffs(here) - 1;
-      r.b = base + who;
-      r.before = before + __shfl_sync(0xffffffffu, s - n, who);
-      return r;
-    }
-    before += __shfl_sync(0xffffffffu, s, 31);
+    __syncthreads();
+    return;
   }
-  return r;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int64_t run = (P.a.B + NTHREADS - 1) / NTHREADS;
+  const int64_t b0 = min((int64_t)threadIdx.x * run, P.a.B), b1 = min(b0 + run, P.a.B);
+  long long mine = 0;
+  for (int64_t b = b0; b < b1; ++b) mine += tiles_of(P.a, b);
+  long long s = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += y;
+  }
+  if (lane == 31) sums[warp] = s;
+  if (threadIdx.x == 0) out = {0, 0, 0, 0, 1};
+  __syncthreads();
+  long long before = s - mine, total = 0;
+#pragma unroll
+  for (int i = 0; i < NTHREADS / 32; ++i) {
+    if (i < warp) before += sums[i];
+    total += sums[i];
+  }
+  total *= units;
+  before *= units;
+  const long long per = (total + P.grid - 1) / P.grid, t0 = min(blockIdx.x * per, total);
+  if (t0 < total && t0 >= before && t0 < before + mine * units) {
+    int64_t b = b0;
+    for (; b + 1 < b1; ++b) {
+      const long long n = (long long)tiles_of(P.a, b) * units;
+      if (t0 < before + n) break;
+      before += n;
+    }
+    out = {t0, min(t0 + per, total), before, b, per};
+  }
+  __syncthreads();
 }
 
 // Walks the units of a range: every role sees the same sequence of segments.
@@ -134,9 +154,20 @@ struct Walk {
   int unit, ta, tb;  // segment: tiles ta..tb-1 of `unit` of sequence b
   GDNX_DEV Walk(const DecParams& P_, int units_, const Range& r)
       : P(P_), units(units_), t(r.t0), t1(r.t1), b(r.b), before(r.before), seq(), unit(0), ta(0), tb(0) {
-    if (t < t1) seq = make_seq(P.a, b);
+    if (t < t1 && !P.whole) seq = make_seq(P.a, b);
   }
   GDNX_DEV bool next() {
+    if (P.whole) {
+      for (; t < t1; ++t) {
+        b = t / units;
+        unit = (int)(t % units);
+        seq = make_seq(P.a, b);
+        if ((tb = seq.kt.count) == 0) continue;
+        ++t;
+        return true;
+      }
+      return false;
+    }
     if (t >= t1) return false;
     while (t >= before + (int64_t)seq.kt.count * units) {
       before += (int64_t)seq.kt.count * units;
@@ -170,6 +201,17 @@ GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, 
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(mbar)
       : "memory");
+}
+
+// Zeros for the sequences that see nothing.
+GDNX_DEV void write_zeros(const DecParams& P) {
+  const gdnx_paged_decode_args& a = P.a;
+  const int D = (int)a.cache.D, n = (int)a.H * D;
+  for (int64_t b = blockIdx.x; b < a.B; b += P.grid) {
+    if (tiles_of(a, b) > 0) continue;
+    for (int x = threadIdx.x % 32; x < n; x += 32)
+      st_from_f32(a.y, a.y_dtype, b * a.y_sb + x / D * a.y_sh + x % D, 0.f);
+  }
 }
 
 template <int DB, int NH>
@@ -220,16 +262,20 @@ GDNX_DEV void run_products(const DecParams& P, Walk w, uint32_t smem, uint32_t t
   const auto values = [&]() {  // O^T += V^T P of the tile before
     if (!pend) return true;
     const uint32_t t = nt - 1, vc = 2 * t + 1, sl = vc % Lo::SLOTS;
-    if (!pipe::wait_or_abort(&bar.full[sl], vc / Lo::SLOTS & 1, abort_flag)) return false;
-    if (!pipe::wait_or_abort(&bar.p_ready[t & 1], t / 2 & 1, abort_flag)) return false;
+    if (!warp_wait(&bar.full[sl], vc / Lo::SLOTS & 1, abort_flag)) return false;
+    if (!warp_wait(&bar.p_ready[t & 1], t / 2 & 1, abort_flag)) return false;
     tc::fence_after();
-    const uint32_t v = smem + Lo::RING + sl * Lo::TILE, p = smem + Lo::P + (t & 1) * Lo::PB;
+    if (elect_one()) {
+      const uint64_t v = tc::smem_desc(smem + Lo::RING + sl * Lo::TILE, DB == 2 ? BLOCK_BYTES : 1024, 1024);
+      const uint64_t p = tc::smem_desc(smem + Lo::P + (t & 1) * Lo::PB, 16, 1024);
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      tc::mma_bf16(tmem + 2 * NH, tc::smem_desc(v + k * 2048, DB == 2 ? BLOCK_BYTES : 1024, 1024),
-                   tc::smem_desc(p + (k / 4) * NH * 128 + (k % 4) * 32, 16, 1024), ID_O, !first || k > 0);
-    tc::commit(&bar.pv_done[t & 1]);
-    tc::commit(&bar.empty[sl]);
+      for (int k = 0; k < 8; ++k)
+        tc::mma_bf16(tmem + 2 * NH, v + k * (2048 >> 4), p + (((k / 4) * NH * 128 + (k % 4) * 32) >> 4), ID_O,
+                     !first || k > 0);
+      tc::commit(&bar.pv_done[t & 1]);
+      tc::commit(&bar.empty[sl]);
+    }
+    __syncwarp();
     pend = false;
     return true;
   };
@@ -239,17 +285,22 @@ GDNX_DEV void run_products(const DecParams& P, Walk w, uint32_t smem, uint32_t t
       if (t == w.ta) {
         // the last unit's output is read before its successor's first product by p_ready
         if (!values()) return;
-        if (!pipe::wait_or_abort(&bar.q_ready[seg & 1], seg / 2 & 1, abort_flag)) return;
+        if (!warp_wait(&bar.q_ready[seg & 1], seg / 2 & 1, abort_flag)) return;
       }
-      if (!pipe::wait_or_abort(&bar.full[sl], kc / Lo::SLOTS & 1, abort_flag)) return;
+      if (!warp_wait(&bar.full[sl], kc / Lo::SLOTS & 1, abort_flag)) return;
       tc::fence_after();
-      const uint32_t k = smem + Lo::RING + sl * Lo::TILE, q = smem + Lo::Q + (seg & 1) * Lo::QB;
+      if (elect_one()) {
+        const uint64_t k = tc::smem_desc(smem + Lo::RING + sl * Lo::TILE, 16, 1024);
+        const uint64_t q = tc::smem_desc(smem + Lo::Q + (seg & 1) * Lo::QB, 16, 1024);
 #pragma unroll
-      for (int x = 0; x < 4 * DB; ++x)
-        tc::mma_bf16(tmem + (nt & 1) * NH, tc::smem_desc(k + (x / 4) * BLOCK_BYTES + (x % 4) * 32, 16, 1024),
-                     tc::smem_desc(q + (x / 4) * NH * 128 + (x % 4) * 32, 16, 1024), ID_S, x > 0);
-      tc::commit(&bar.s_full[nt & 1]);
-      tc::commit(&bar.empty[sl]);
+        for (int x = 0; x < 4 * DB; ++x)
+          tc::mma_bf16(tmem + (nt & 1) * NH, k + (((x / 4) * BLOCK_BYTES + (x % 4) * 32) >> 4),
+                       q + (((x / 4) * NH * 128 + (x % 4) * 32) >> 4), ID_S, x > 0);
+        tc::commit(&bar.s_full[nt & 1]);
+        tc::commit(&bar.empty[sl]);
+        if (t + 1 == w.tb) tc::commit(&bar.q_empty[seg & 1]);
+      }
+      __syncwarp();
       if (!values()) return;
       ++nt;
       pend = true;
@@ -269,13 +320,14 @@ struct Heads {
   }
 };
 
-// The unit's query rows as a K-major tile of NH rows (rows beyond its heads zero).
+// The unit's query rows as a K-major tile of NH rows (rows beyond its heads zero), by one warp.
 template <int DB, int NH>
 GDNX_DEV void stage_q(const DecParams& P, const Walk& w, uint8_t* dst) {
   const gdnx_paged_decode_args& a = P.a;
   const Heads hd(P, w.unit, NH);
   const int D = (int)a.cache.D;
-  for (int x = threadIdx.x; x < NH * DB * 8; x += 128) {
+#pragma unroll 4
+  for (int x = threadIdx.x % 32; x < NH * DB * 8; x += 32) {
     const int h = x / (DB * 8), c = x % (DB * 8);
     uint4 u = make_uint4(0, 0, 0, 0);
     if (h < hd.n && c * 8 < D) {
@@ -290,6 +342,17 @@ GDNX_DEV void stage_q(const DecParams& P, const Walk& w, uint8_t* dst) {
       }
     }
     *reinterpret_cast<uint4*>(dst + tc::sw128(h, c, NH)) = u;
+  }
+}
+
+template <int DB, int NH>
+GDNX_DEV void run_queries(const DecParams& P, Walk w, uint8_t* base, Bars& bar, volatile int* abort_flag) {
+  using Lo = Layout<DB, NH>;
+  for (uint32_t seg = 0; w.next(); ++seg) {
+    if (!warp_wait(&bar.q_empty[seg & 1], (seg / 2 & 1) ^ 1, abort_flag)) return;
+    stage_q<DB, NH>(P, w, base + Lo::Q + (seg & 1) * Lo::QB);
+    tc::fence_async_smem();
+    pipe::mbar_arrive(&bar.q_ready[seg & 1]);
   }
 }
 
@@ -319,7 +382,7 @@ GDNX_DEV void tmem_st(uint32_t at, const float (&v)[NC]) {
 
 // NC: heads that a thread works on, the unit's rounded up (the others' columns are not used).
 template <int DB, int NH, int NC, bool BF16>
-GDNX_DEV void run_keys(const DecParams& P, Walk w, uint8_t* base, uint32_t tmem, Bars& bar, float* red,
+GDNX_DEV void run_keys(const DecParams& P, Walk w, int64_t per, uint8_t* base, uint32_t tmem, Bars& bar, float* red,
                        volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   const gdnx_paged_decode_args& a = P.a;
@@ -327,18 +390,10 @@ GDNX_DEV void run_keys(const DecParams& P, Walk w, uint8_t* base, uint32_t tmem,
   const uint32_t lane_at = (uint32_t)(warp * 32) << 16;
   const float c2 = a.scale * kLog2e;
   const int window = (int)a.window, sinks = (int)a.sinks;
-  uint32_t nt = 0, seg = 0;
+  uint32_t nt = 0;
   bool ok = true;  // a wait that gave up is told at the next vote, where all four warps leave
-  Walk ahead = w;  // the segment whose queries are staged next
-  const auto stage = [&](uint32_t s) {
-    if (!ahead.next()) return;
-    stage_q<DB, NH>(P, ahead, base + Lo::Q + (s & 1) * Lo::QB);
-    tc::fence_async_smem();
-    pipe::mbar_arrive(&bar.q_ready[s & 1]);
-  };
-  stage(0);
-  for (; w.next(); ++seg) {
-    stage(seg + 1);  // its buffer's products (two segments back) have all been read
+  if (r == 0 && !P.whole) P.joint[blockIdx.x] = {0, 0, 0, -1};
+  while (w.next()) {
     const Heads hd(P, w.unit, NH);
     float m[NC], l[NC];
 #pragma unroll
@@ -440,6 +495,8 @@ GDNX_DEV void run_keys(const DecParams& P, Walk w, uint8_t* base, uint32_t tmem,
         }
       }
     }
+    if (r == 0 && w.ta > 0 && w.tb == w.seq.kt.count)  // the unit's last part
+      P.joint[blockIdx.x] = {(int)w.b, w.unit, (int)((w.before + (int64_t)w.unit * w.seq.kt.count) / per), (int)blockIdx.x};
     if (pipe::group_any(1, 128, !ok)) return;  // and red may be written again
   }
 }
@@ -452,12 +509,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   Small<NH>& sm = *reinterpret_cast<Small<NH>*>(base + Lo::SMALL);
   Bars& bar = sm.bar;
   volatile int* abort_flag = &sm.abort_flag;
-  const uint32_t smem = tc::smem_u32(base);
-  const int warp = threadIdx.x / 32, units = (int)P.a.cache.Hk * P.groups;
-  if (warp == 0) {
-    const Range r = find_range(P, units);
-    if (threadIdx.x == 0) sm.range = r;
-  } else if (warp == 4) {
+  const uint32_t smem = uniform(tc::smem_u32(base));
+  const int warp = uniform(threadIdx.x / 32), units = (int)P.a.cache.Hk * P.groups;
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may be set up; it waits for this grid's end
+  if (warp == 4) {
     tc::tmem_alloc(&sm.tmem_at, Lo::TMEM);
   } else if (threadIdx.x == 160) {
     *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
@@ -466,7 +521,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
       tc::mbar_init(&bar.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&bar.q_ready[i], 128);
+      tc::mbar_init(&bar.q_ready[i], 32);
+      tc::mbar_init(&bar.q_empty[i], 1);
       tc::mbar_init(&bar.s_full[i], 1);
       tc::mbar_init(&bar.p_ready[i], 128);
       tc::mbar_init(&bar.pv_done[i], 1);
@@ -474,21 +530,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
     tc::mbar_init(&bar.done, 1);
   }
   tc::fence_before();
-  __syncthreads();
+  find_range(P, units, sm.range, sm.sums);  // synchronises
   tc::fence_after();
-  const uint32_t tmem = sm.tmem_at;
+  const uint32_t tmem = uniform(sm.tmem_at);
   const Walk w(P, units, sm.range);
   if (smem % 1024) {  // never entered: the base is aligned
   } else if (warp < 4) {
-    run_keys<DB, NH, NC, BF16>(P, w, base, tmem, bar, sm.red, abort_flag);
+    run_keys<DB, NH, NC, BF16>(P, w, sm.range.per, base, tmem, bar, sm.red, abort_flag);
   } else if (warp == 4) {
-    if (threadIdx.x % 32 == 0) {
-      run_products<DB, NH, BF16>(P, w, smem, tmem, bar, abort_flag);
-      tc::commit(&bar.done);  // every product issued has ended before tensor memory is freed
-      tc::mbar_wait(&bar.done, 0);
-    }
+    run_products<DB, NH, BF16>(P, w, smem, tmem, bar, abort_flag);
+    __syncwarp();
+    if (elect_one()) tc::commit(&bar.done);  // every product issued has ended before tensor memory is freed
+    tc::mbar_wait(&bar.done, 0);
+  } else if (warp == 6) {
+    run_queries<DB, NH>(P, w, base, bar, abort_flag);
   } else {
     run_loads<DB, NH>(P, w, smem, bar, abort_flag);
+    write_zeros(P);
     if (*abort_flag)  // let the copies in flight land
       for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
   }
@@ -500,55 +558,24 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
 }
 
-// Joins a unit's parts, CTA after CTA, and writes the zeros of sequences that see nothing:
-// one block for each sequence and query head.  Each of its warps sums a contiguous run of the
-// parts; the runs are added in order.
+// Joins a cut unit's parts, CTA after CTA: block (c, g) head g of the unit that ends in CTA c.
+// Each warp sums a contiguous run of the parts; the runs are added in order.
 constexpr int JOIN_WARPS = 8;
 
 template <int NH>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_decode_join_kernel(const DecParams P) {
   const gdnx_paged_decode_args& a = P.a;
-  __shared__ long long sums[2][JOIN_WARPS];
   __shared__ float red_m[JOIN_WARPS], red_l[JOIN_WARPS], red_o[JOIN_WARPS][128];
-  const int64_t h = blockIdx.x % a.H, b = blockIdx.x / a.H;
-  const int units = (int)a.cache.Hk * P.groups, D = (int)a.cache.D, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  // tiles before this sequence, and of all
-  long long s0 = 0, s1 = 0;
-  for (int64_t i = threadIdx.x; i < a.B; i += JOIN_WARPS * 32) {
-    const int n = tiles_of(a, i);
-    s1 += n;
-    if (i < b) s0 += n;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-    s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-  }
-  if (lane == 0) {
-    sums[0][warp] = s0;
-    sums[1][warp] = s1;
-  }
-  const int n = tiles_of(a, b);
-  __syncthreads();
-  int64_t before = 0, total = 0;
-#pragma unroll
-  for (int i = 0; i < JOIN_WARPS; ++i) {
-    before += sums[0][i];
-    total += sums[1][i];
-  }
-  const int64_t per = (total * units + P.grid - 1) / P.grid;
-  const int64_t out = b * a.y_sb + h * a.y_sh;
-  if (n == 0) {
-    for (int d = threadIdx.x; d < D; d += JOIN_WARPS * 32) st_from_f32(a.y, a.y_dtype, out + d, 0.f);
-    return;
-  }
-  const int G = (int)(a.H / a.cache.Hk), g = (int)(h % G);
-  const int64_t unit = h / G * P.groups + g / NH, first = before * units + unit * n, last = first + n - 1;
-  const int c0 = (int)(first / per), c1 = (int)(last / per);
-  if (c0 == c1) return;  // one CTA had it whole
-  const auto place = [&](int c) { return ((int64_t)c * 2 + (c == c0)) * NH + g % NH; };
-  const int parts = c1 - c0 + 1, run = (parts + JOIN_WARPS - 1) / JOIN_WARPS;
-  const int r0 = c0 + warp * run, r1 = min(r0 + run, c1 + 1);
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, D = (int)a.cache.D, g = blockIdx.y;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are there
+  const Joint j = P.joint[blockIdx.x];
+  if (j.c1 < 0) return;
+  const Heads hd(P, j.unit, NH);
+  if (g >= hd.n) return;
+  const int64_t out = j.b * a.y_sb + (hd.h0 + g) * a.y_sh;
+  const auto place = [&](int c) { return ((int64_t)c * 2 + (c == j.c0)) * NH + g; };
+  const int parts = j.c1 - j.c0 + 1, run = (parts + JOIN_WARPS - 1) / JOIN_WARPS;
+  const int r0 = j.c0 + warp * run, r1 = min(r0 + run, j.c1 + 1);
   float m = -INFINITY, l = 0.f;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int c = r0 + lane; c < r1; c += 32) m = fmaxf(m, P.stat[place(c) * 2]);
@@ -588,7 +615,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_decode_join_kernel(cons
 }
 
 struct Plan {
-  int nh, groups, grid;
+  int nh, groups, grid, whole;
 };
 
 Plan plan(const gdnx_paged_decode_args& a, int sms) {
@@ -598,9 +625,14 @@ Plan plan(const gdnx_paged_decode_args& a, int sms) {
   p.groups = (int)((G + p.nh - 1) / p.nh);
   int64_t most = a.cache.width * a.cache.page;
   if (a.max_len > 0 && a.max_len < most) most = a.max_len;
-  const int64_t tiles = a.B * a.cache.Hk * p.groups * ((most + TM - 1) / TM);
-  const int64_t ctas = (int64_t)sms;
-  p.grid = (int)(tiles < ctas ? (tiles > 0 ? tiles : 1) : ctas);
+  int64_t n = (most + TM - 1) / TM;  // tiles of a unit, at most
+  const int64_t seen = (a.window + TM - 1) / TM + 1 + (a.sinks + TM - 1) / TM;
+  if (seen < n) n = seen;
+  const int64_t units = a.B * a.cache.Hk * p.groups;
+  // Short units are not cut: a few more tiles in a row take less time than a join.
+  p.whole = n <= WHOLE_TILES;
+  const int64_t ctas = p.whole ? units : units * n;
+  p.grid = (int)(ctas < sms ? (ctas > 0 ? ctas : 1) : sms);
   return p;
 }
 
@@ -612,7 +644,19 @@ gdnx_status launch(const DecParams& P, cudaStream_t st) {
   static std::atomic<uint64_t> done;
   if (!allow_smem(kernel, smem, done)) return GDNX_ELAUNCH;
   kernel<<<(unsigned)P.grid, NTHREADS, smem, st>>>(P);
-  paged_decode_join_kernel<NH><<<(unsigned)(P.a.B * P.a.H), JOIN_WARPS * 32, 0, st>>>(P);
+  if (!P.whole) {
+    cudaLaunchAttribute early;  // set up while the parts are made
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    const int64_t G = P.a.H / P.a.cache.Hk;
+    cfg.gridDim = dim3((unsigned)P.grid, (unsigned)(G < NH ? G : NH));
+    cfg.blockDim = dim3(JOIN_WARPS * 32);
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<NH>, P);
+  }
   return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
 }
 
@@ -633,7 +677,7 @@ gdnx_status launch_type(const DecParams& P, cudaStream_t st) {
 
 size_t paged_decode_tc_workspace_bytes(const gdnx_paged_decode_args& a) {
   const Plan p = plan(a, sm_count());
-  return (size_t)p.grid * 2 * p.nh * (128 + 2) * sizeof(float);
+  return p.whole ? 0 : (size_t)p.grid * (2 * p.nh * (128 + 2) * sizeof(float) + sizeof(Joint));
 }
 
 gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t st) {
@@ -656,6 +700,8 @@ gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t
   P.groups = p.groups;
   P.part = static_cast<float*>(a.workspace);
   P.stat = P.part + (size_t)p.grid * 2 * p.nh * 128;
+  P.joint = reinterpret_cast<Joint*>(P.stat + (size_t)p.grid * 2 * p.nh * 2);
+  P.whole = p.whole;
   P.vec_q = reinterpret_cast<uintptr_t>(a.q.ptr) % 16 == 0 && a.q.sb % 8 == 0 && a.q.sh % 8 == 0;
   return c.dtype == GDNX_BF16 ? launch_type<true>(P, st) : launch_type<false>(P, st);
 }
