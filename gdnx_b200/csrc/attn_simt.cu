@@ -34,10 +34,25 @@ GDNX_DEV float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(
 template <>
 GDNX_DEV float to_f32<__half>(__half x) { return __half2float(x); }
 
-// Rows r0..r0+63 of head h (rows at or beyond `rows` as zeros) into dst [64][DP + 4].
+// Rows r0..r0+63 of head h (rows at or beyond `rows` as zeros) into dst [64][DP + 4].  Aligned
+// 32-bit rows go by 16-byte asynchronous copies (landed after `wait_tiles`), others by value.
 template <int DP, typename T>
 GDNX_DEV void load_tile(float* dst, const gdnx_view& v, int64_t b, int64_t h, int r0, int rows, int D) {
   const T* base = reinterpret_cast<const T*>(v.ptr) + b * v.sb + h * v.sh;
+  if (sizeof(T) == 4 && reinterpret_cast<uintptr_t>(base) % 16 == 0 && v.st % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < BT * DP / 4 / NT; ++k) {
+      const int i = k * NT + threadIdx.x, r = i / (DP / 4), d = i % (DP / 4) * 4;
+      const bool on = r0 + r < rows && d < D;
+      const T* src = on ? base + (int64_t)(r0 + r) * v.st + d : base;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                       static_cast<uint32_t>(__cvta_generic_to_shared(dst + r * (DP + 4) + d))),
+                   "l"(src), "r"(on ? 16 : 0)
+                   : "memory");
+    }
+    return;
+  }
+#pragma unroll 8
   for (int i = threadIdx.x; i < BT * DP; i += NT) {
     const int r = i / DP, d = i % DP;
     float x = 0.f;
@@ -45,16 +60,20 @@ GDNX_DEV void load_tile(float* dst, const gdnx_view& v, int64_t b, int64_t h, in
     dst[r * (DP + 4) + d] = x;
   }
 }
+// This thread's asynchronous copies have landed (a barrier makes them everyone's).
+GDNX_DEV void wait_tiles() {
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+}
 
-// s[a][c] = sum_d A[ty*4+a][d] B[tx+16c][d]
+// s[a][c] = sum_{d < D} A[ty*4+a][d] B[tx+16c][d]  (D a multiple of 8)
 template <int DP>
-GDNX_DEV void dot_tile(float (&s)[4][4], const float* A, const float* B, int ty, int tx) {
+GDNX_DEV void dot_tile(float (&s)[4][4], const float* A, const float* B, int ty, int tx, int D) {
 #pragma unroll
   for (int a = 0; a < 4; ++a)
 #pragma unroll
     for (int c = 0; c < 4; ++c) s[a][c] = 0.f;
 #pragma unroll 4
-  for (int d = 0; d < DP; d += 4) {
+  for (int d = 0; d < D; d += 4) {
     float4 x[4], y[4];
 #pragma unroll
     for (int a = 0; a < 4; ++a) x[a] = *reinterpret_cast<const float4*>(A + (ty * 4 + a) * (DP + 4) + d);
@@ -135,9 +154,10 @@ __global__ void __launch_bounds__(NT) attn_fwd_simt_kernel(const gdnx_attn_args 
     const int j0 = kt.tile(t) * BT;
     __syncthreads();
     load_tile<DP, T>(KV, a.k, b, hk, j0, len, D);
+    wait_tiles();
     __syncthreads();
     float s[4][4];
-    dot_tile<DP>(s, Q, KV, ty, tx);
+    dot_tile<DP>(s, Q, KV, ty, tx, D);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int p = i0 + ty * 4 + r + off;
@@ -164,6 +184,7 @@ __global__ void __launch_bounds__(NT) attn_fwd_simt_kernel(const gdnx_attn_args 
     }
     __syncthreads();
     load_tile<DP, T>(KV, a.v, b, hk, j0, len, D);
+    wait_tiles();
     __syncthreads();
     acc_tile<DP>(o, W, KV, ty, tx);
   }
@@ -237,12 +258,14 @@ __global__ void __launch_bounds__(NT) attn_dq_simt_kernel(const gdnx_attn_bwd_ar
     float dp[4][4], s[4][4];
     __syncthreads();
     load_tile<DP, T>(KV, a.v, b, hk, j0, len, D);
+    wait_tiles();
     __syncthreads();
-    dot_tile<DP>(dp, Y, KV, ty, tx);
+    dot_tile<DP>(dp, Y, KV, ty, tx, D);
     __syncthreads();
     load_tile<DP, T>(KV, a.k, b, hk, j0, len, D);
+    wait_tiles();
     __syncthreads();
-    dot_tile<DP>(s, Q, KV, ty, tx);
+    dot_tile<DP>(s, Q, KV, ty, tx, D);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -301,10 +324,11 @@ __global__ void __launch_bounds__(NT) attn_dkv_simt_kernel(const gdnx_attn_bwd_a
       __syncthreads();
       load_tile<DP, T>(Q, a.q, b, h, i0, rows, D);
       load_tile<DP, T>(Y, g.dy, b, h, i0, rows, D);
+      wait_tiles();
       __syncthreads();
       float s[4][4], dp[4][4];  // [query ty*4+r][key tx+16c]
-      dot_tile<DP>(s, Q, K, ty, tx);
-      dot_tile<DP>(dp, Y, V, ty, tx);
+      dot_tile<DP>(s, Q, K, ty, tx, D);
+      dot_tile<DP>(dp, Y, V, ty, tx, D);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = i0 + ty * 4 + r;
