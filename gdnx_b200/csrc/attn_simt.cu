@@ -25,6 +25,17 @@ constexpr int BT = 64;        // rows of every tile
 constexpr int NT = 256;       // threads
 constexpr int LDP = BT + 4;   // row stride of the weight tile (16-byte rows, conflict-free)
 
+// Blocks run over heads, then batch rows, then tiles: those of one tile, which cost alike, side
+// by side, and the tiles with most work first (the last queries; the first keys).
+struct Block {
+  int64_t b, h;
+  int tile;
+};
+GDNX_DEV Block block_of(int64_t heads, int64_t B) {
+  const int64_t n = blockIdx.x;
+  return {n / heads % B, n % heads, (int)(n / (heads * B))};
+}
+
 template <typename T>
 GDNX_DEV float to_f32(T x);
 template <>
@@ -135,8 +146,9 @@ __global__ void __launch_bounds__(NT) attn_fwd_simt_kernel(const gdnx_attn_args 
   float* KV = Q + BT * (DP + 4);
   float* W = KV + BT * (DP + 4);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int i0 = blockIdx.x * BT, D = (int)a.D;
-  const int64_t h = blockIdx.y, b = blockIdx.z, hk = h / (a.H / a.Hk);
+  const Block blk = block_of(a.H, a.B);
+  const int i0 = ((int)((a.Tq + BT - 1) / BT) - 1 - blk.tile) * BT, D = (int)a.D;
+  const int64_t h = blk.h, b = blk.b, hk = h / (a.H / a.Hk);
   const int off = (int)(a.Tk - a.Tq), len = seq_len(a, b);
   const int window = (int)a.window, sinks = (int)a.sinks;
   const float c2 = a.scale * kLog2e;
@@ -235,8 +247,9 @@ __global__ void __launch_bounds__(NT) attn_dq_simt_kernel(const gdnx_attn_bwd_ar
   float* KV = Y + BT * (DP + 4);
   float* W = KV + BT * (DP + 4);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int i0 = blockIdx.x * BT, D = (int)a.D;
-  const int64_t h = blockIdx.y, b = blockIdx.z, hk = h / (a.H / a.Hk);
+  const Block blk = block_of(a.H, a.B);
+  const int i0 = ((int)((a.Tq + BT - 1) / BT) - 1 - blk.tile) * BT, D = (int)a.D;
+  const int64_t h = blk.h, b = blk.b, hk = h / (a.H / a.Hk);
   const int off = (int)(a.Tk - a.Tq), len = seq_len(a, b);
   const int window = (int)a.window, sinks = (int)a.sinks;
   const float c2 = a.scale * kLog2e;
@@ -302,8 +315,9 @@ __global__ void __launch_bounds__(NT) attn_dkv_simt_kernel(const gdnx_attn_bwd_a
   float* Y = Q + BT * (DP + 4);
   float* W = Y + BT * (DP + 4);  // P^T, then dS^T: [key][query]
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int j0 = blockIdx.x * BT, D = (int)a.D;
-  const int64_t hk = blockIdx.y, b = blockIdx.z, G = a.H / a.Hk;
+  const Block blk = block_of(a.Hk, a.B);
+  const int j0 = blk.tile * BT, D = (int)a.D;
+  const int64_t hk = blk.h, b = blk.b, G = a.H / a.Hk;
   const int off = (int)(a.Tk - a.Tq), len = seq_len(a, b);
   const int window = (int)a.window, sinks = (int)a.sinks;
   const float c2 = a.scale * kLog2e;
@@ -372,6 +386,8 @@ __global__ void __launch_bounds__(NT) attn_dkv_simt_kernel(const gdnx_attn_bwd_a
 
 constexpr size_t smem_of(int dp, int tiles) { return ((size_t)tiles * BT * (dp + 4) + BT * LDP) * sizeof(float); }
 
+dim3 blocks(int64_t T, int64_t heads, int64_t B) { return dim3((unsigned)((T + BT - 1) / BT * heads * B)); }
+
 template <typename F>
 gdnx_status run(F kernel, dim3 grid, size_t smem, cudaStream_t st, void** args) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
@@ -386,7 +402,7 @@ template <int DP, typename T>
 gdnx_status fwd(const gdnx_attn_args& a, cudaStream_t st) {
   gdnx_attn_args arg = a;
   void* p[] = {&arg};
-  return run(attn_fwd_simt_kernel<DP, T>, dim3((unsigned)((a.Tq + BT - 1) / BT), (unsigned)a.H, (unsigned)a.B),
+  return run(attn_fwd_simt_kernel<DP, T>, blocks(a.Tq, a.H, a.B),
              smem_of(DP, 2), st, p);
 }
 
@@ -396,9 +412,9 @@ gdnx_status bwd(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st) {
   void* p[] = {&arg, &delta};
   const gdnx_attn_args& a = g.fwd;
   gdnx_status s = run(attn_dq_simt_kernel<DP, T>,
-                      dim3((unsigned)((a.Tq + BT - 1) / BT), (unsigned)a.H, (unsigned)a.B), smem_of(DP, 3), st, p);
+                      blocks(a.Tq, a.H, a.B), smem_of(DP, 3), st, p);
   if (s != GDNX_OK) return s;
-  return run(attn_dkv_simt_kernel<DP, T>, dim3((unsigned)((a.Tk + BT - 1) / BT), (unsigned)a.Hk, (unsigned)a.B),
+  return run(attn_dkv_simt_kernel<DP, T>, blocks(a.Tk, a.Hk, a.B),
              smem_of(DP, 4), st, p);
 }
 
