@@ -35,7 +35,7 @@ struct BwdParams {
   TileMap q, k, v, dy;
   gdnx_attn_args a;
   void *dq, *dk, *dv;
-  const float *lse2, *delta;  // [B,H,qpad]: log2-domain lse (+inf where padding) and delta (0)
+  const float *lse2, *delta;  // [B,H,qpad]: minus lse in the log2 domain (-inf where padding), minus delta (0)
   float* part;                // partial dK, dV of cut tiles: [item][2][128][64 DB]
   int qtiles, ktiles, nst;    // nst: key tiles that hold sinks
   int seg_sink, seg;          // parts of such a tile and of the others
@@ -206,13 +206,16 @@ GDNX_DEV void keys_rows(const BwdParams& P, const KeyItem& w, const uint8_t* bas
     const bool whole = p0 >= w.j0 + TM - 1 && p0 + 64 <= len && w.j0 + TM <= len &&
                        (p0 + 63 - w.j0 < window || w.j0 + TM <= sinks);
     uint32_t on[2] = {0xffffffffu, 0xffffffffu};
+    const float2 cc = make_float2(c2, c2);
 #pragma unroll
-    for (int e = 0; e < 64; e += 4) {
+    for (int e = 0; e < 64; e += 4) {  // every other pair on the FMA pipes
       const float4 z = *reinterpret_cast<const float4*>(lse + e);
-      s[e] = ex2(fmaf(s[e], c2, -z.x));
-      s[e + 1] = ex2(fmaf(s[e + 1], c2, -z.y));
-      s[e + 2] = ex2(fmaf(s[e + 2], c2, -z.z));
-      s[e + 3] = ex2(fmaf(s[e + 3], c2, -z.w));
+      const float2 x = fma2(make_float2(s[e], s[e + 1]), cc, make_float2(z.x, z.y));
+      const float2 y = ex2_poly(fma2(make_float2(s[e + 2], s[e + 3]), cc, make_float2(z.z, z.w)));
+      s[e] = ex2(x.x);
+      s[e + 1] = ex2(x.y);
+      s[e + 2] = y.x;
+      s[e + 3] = y.y;
     }
     if (!whole) {
 #pragma unroll
@@ -238,10 +241,12 @@ GDNX_DEV void keys_rows(const BwdParams& P, const KeyItem& w, const uint8_t* bas
 #pragma unroll
     for (int e = 0; e < 64; e += 4) {
       const float4 z = *reinterpret_cast<const float4*>(del + e);
-      s[e] *= d[e] - z.x;
-      s[e + 1] *= d[e + 1] - z.y;
-      s[e + 2] *= d[e + 2] - z.z;
-      s[e + 3] *= d[e + 3] - z.w;
+      const float2 x = mul2(make_float2(s[e], s[e + 1]), add2(make_float2(d[e], d[e + 1]), make_float2(z.x, z.y)));
+      const float2 y = mul2(make_float2(s[e + 2], s[e + 3]), add2(make_float2(d[e + 2], d[e + 3]), make_float2(z.z, z.w)));
+      s[e] = x.x;
+      s[e + 1] = x.y;
+      s[e + 2] = y.x;
+      s[e + 3] = y.y;
     }
     if (!whole) {
 #pragma unroll
@@ -390,6 +395,7 @@ GDNX_DEV void queries_rows(const BwdParams& P, const QueryItem& w, uint32_t tmem
   const int64_t at = ((int64_t)w.b * a.H + w.h) * P.qtiles * TM + i;
   const float lse2 = P.lse2[at], del = P.delta[at];
   const bool one = sees_one(p, window, sinks);
+  const float2 cc = make_float2(c2, c2);
   for (int t = 0; t < w.kt.count; ++t) {
     const uint32_t buf = t & 1;
     const int j0 = w.kt.tile(t) * TM, c0 = j0 + half * 64;  // this half's first key
@@ -399,7 +405,14 @@ GDNX_DEV void queries_rows(const BwdParams& P, const QueryItem& w, uint32_t tmem
     tmem_ld64(tS + buf * 128, s);
     const bool whole = c0 + 63 <= w.p0 && w.p0 + TM <= len && (w.p0 + TM - 1 - c0 < window || c0 + 64 <= sinks);
 #pragma unroll
-    for (int e = 0; e < 64; ++e) s[e] = ex2(fmaf(s[e], c2, -lse2));
+    for (int e = 0; e < 64; e += 4) {  // every other pair on the FMA pipes
+      const float2 x = fma2(make_float2(s[e], s[e + 1]), cc, make_float2(lse2, lse2));
+      const float2 y = ex2_poly(fma2(make_float2(s[e + 2], s[e + 3]), cc, make_float2(lse2, lse2)));
+      s[e] = ex2(x.x);
+      s[e + 1] = ex2(x.y);
+      s[e + 2] = y.x;
+      s[e + 3] = y.y;
+    }
     if (!warp_wait(&bar.dp_full, t & 1, abort_flag)) return;
     tc::fence_after();
     float d[64];
@@ -407,7 +420,11 @@ GDNX_DEV void queries_rows(const BwdParams& P, const QueryItem& w, uint32_t tmem
     tc::fence_before();
     pipe::mbar_arrive(&bar.dp_read);
 #pragma unroll
-    for (int e = 0; e < 64; ++e) s[e] *= d[e] - del;
+    for (int e = 0; e < 64; e += 2) {
+      const float2 x = mul2(make_float2(s[e], s[e + 1]), add2(make_float2(d[e], d[e + 1]), make_float2(del, del)));
+      s[e] = x.x;
+      s[e + 1] = x.y;
+    }
     if (!whole) {
       const int hi = p < len && !one ? p - c0 : -1;
 #pragma unroll
@@ -578,7 +595,7 @@ __global__ void __launch_bounds__(256) attn_dkv_join_kernel(const BwdParams P, i
   }
 }
 
-// lse in the log2 domain and delta = sum_d dy y, padded to whole tiles of queries: eight lanes
+// Minus lse in the log2 domain and minus delta = sum_d dy y, padded to whole tiles of queries: eight lanes
 // for each row.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const gdnx_attn_bwd_args g, float* lse2, float* delta,
@@ -606,8 +623,8 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const gdnx_attn_bwd_arg
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(mask, s, o);
   if (threadIdx.x % 8 == 0) {
-    lse2[n] = on ? a.lse[(b * a.H + h) * a.Tq + i] * kLog2e : INFINITY;
-    delta[n] = s;
+    lse2[n] = on ? -a.lse[(b * a.H + h) * a.Tq + i] * kLog2e : -INFINITY;
+    delta[n] = -s;
   }
 }
 

@@ -238,6 +238,15 @@ GDNX_DEV float2 add2(float2 a, float2 b) {
   return d;
 }
 
+GDNX_DEV float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // 2^x of two values on the FMA pipes, for x <= 120; below -125 it stays at 2^-125.  x = n + f with
 // |f| <= 1/2 (n by rounding x + 1.5 2^23), 2^f by the polynomial of degree 4 whose relative
 // error over the interval is least (2.6e-6, Remez exchange), n added to the exponent.
