@@ -39,10 +39,11 @@ struct BwdParams {
   float* part;                // partial dK, dV of cut tiles: [item][2][128][64 DB]
   int qtiles, ktiles, nst;    // nst: key tiles that hold sinks
   int seg_sink, seg;          // parts of such a tile and of the others
+  unsigned queries;           // items of attn_dq
 };
 
 struct Bars {
-  uint64_t full[SLOTS], empty[SLOTS], res[2], stat_full[2], stat_empty[2], s_full[2], dp_full, p_ready, ds_ready[2],
+  uint64_t full[SLOTS], empty[SLOTS], res[2], res_empty[2], stat_full[2], stat_empty[2], s_full[2], dp_full, p_ready, ds_ready[2],
       dp_read, o_full, fix, done;
 };
 
@@ -110,6 +111,7 @@ GDNX_DEV void init_bars(Bars& bar) {
   }
   for (int i = 0; i < 2; ++i) {
     tc::mbar_init(&bar.res[i], 1);
+    tc::mbar_init(&bar.res_empty[i], 1);
     tc::mbar_init(&bar.stat_full[i], 1);
     tc::mbar_init(&bar.stat_empty[i], 256);
     tc::mbar_init(&bar.s_full[i], 1);
@@ -371,12 +373,11 @@ struct QueryItem {
   KeyTiles kt;
 };
 
-GDNX_DEV QueryItem query_item(const BwdParams& P) {
+GDNX_DEV QueryItem query_item(const BwdParams& P, unsigned n) {
   const gdnx_attn_args& a = P.a;
-  int64_t n = blockIdx.x;
-  const int h = (int)(n % a.H);
-  n /= a.H;
-  const int b = (int)(n % a.B), qt = P.qtiles - 1 - (int)(n / a.B);  // those that see most first
+  const int h = (int)(n % (unsigned)a.H);
+  n /= (unsigned)a.H;
+  const int b = (int)(n % (unsigned)a.B), qt = P.qtiles - 1 - (int)(n / (unsigned)a.B);  // those that see most first
   const int off = (int)(a.Tk - a.Tq), len = uniform(seq_len(a, b));
   return {b, h, h / (int)(a.H / a.Hk), qt * TM, qt * TM + off, len,
           KeyTiles(qt * TM + off, min(qt * TM + TM, (int)a.Tq) - 1 + off, len, (int)a.window, (int)a.sinks, TM)};
@@ -384,147 +385,169 @@ GDNX_DEV QueryItem query_item(const BwdParams& P) {
 
 constexpr uint32_t Q_S = 0, Q_DP = 256, Q_DQ = 384;  // S has two buffers
 
+// A persistent CTA takes item after item: tiles are counted through (T), so that the loads and
+// the first products of an item run under the one before.
 template <int DB>
-GDNX_DEV void queries_rows(const BwdParams& P, const QueryItem& w, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void queries_rows(const BwdParams& P, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
   const gdnx_attn_args& a = P.a;
   const int r = threadIdx.x % 128, half = threadIdx.x / 128;
   const uint32_t lane_at = (uint32_t)(r / 32 * 32) << 16;
   const uint32_t tS = tmem + lane_at + Q_S + half * 64, tP = tmem + lane_at + Q_DP + half * 64;
-  const int window = (int)a.window, sinks = (int)a.sinks, len = w.len, p = w.p0 + r, i = w.i0 + r;
+  const int window = (int)a.window, sinks = (int)a.sinks;
   const float c2 = a.scale * kLog2e;
-  const int64_t at = ((int64_t)w.b * a.H + w.h) * P.qtiles * TM + i;
-  const float lse2 = P.lse2[at], del = P.delta[at];
-  const bool one = sees_one(p, window, sinks);
   const float2 cc = make_float2(c2, c2);
-  for (int t = 0; t < w.kt.count; ++t) {
-    const uint32_t buf = t & 1;
-    const int j0 = w.kt.tile(t) * TM, c0 = j0 + half * 64;  // this half's first key
-    if (!warp_wait(&bar.s_full[buf], t / 2 & 1, abort_flag)) return;
-    tc::fence_after();
-    float s[64];
-    tmem_ld64(tS + buf * 128, s);
-    const bool whole = c0 + 63 <= w.p0 && w.p0 + TM <= len && (w.p0 + TM - 1 - c0 < window || c0 + 64 <= sinks);
+  uint32_t T = 0, items = 0;
+  for (unsigned n = blockIdx.x; n < P.queries; n += gridDim.x) {
+    const QueryItem w = query_item(P, n);
+    const int len = w.len, p = w.p0 + r, i = w.i0 + r;
+    const int64_t at = ((int64_t)w.b * a.H + w.h) * P.qtiles * TM + i;
+    const float lse2 = P.lse2[at], del = P.delta[at];
+    const bool one = sees_one(p, window, sinks);
+    for (int t = 0; t < w.kt.count; ++t, ++T) {
+      const uint32_t buf = T & 1;
+      const int j0 = w.kt.tile(t) * TM, c0 = j0 + half * 64;  // this half's first key
+      if (!warp_wait(&bar.s_full[buf], T / 2 & 1, abort_flag)) return;
+      tc::fence_after();
+      float s[64];
+      tmem_ld64(tS + buf * 128, s);
+      const bool whole = c0 + 63 <= w.p0 && w.p0 + TM <= len && (w.p0 + TM - 1 - c0 < window || c0 + 64 <= sinks);
 #pragma unroll
-    for (int e = 0; e < 64; e += 4) {  // every other pair on the FMA pipes
-      const float2 x = fma2(make_float2(s[e], s[e + 1]), cc, make_float2(lse2, lse2));
-      const float2 y = ex2_poly(fma2(make_float2(s[e + 2], s[e + 3]), cc, make_float2(lse2, lse2)));
-      s[e] = ex2(x.x);
-      s[e + 1] = ex2(x.y);
-      s[e + 2] = y.x;
-      s[e + 3] = y.y;
-    }
-    if (!warp_wait(&bar.dp_full, t & 1, abort_flag)) return;
-    tc::fence_after();
-    float d[64];
-    tmem_ld64(tP, d);
-    tc::fence_before();
-    pipe::mbar_arrive(&bar.dp_read);
-#pragma unroll
-    for (int e = 0; e < 64; e += 2) {
-      const float2 x = mul2(make_float2(s[e], s[e + 1]), add2(make_float2(d[e], d[e + 1]), make_float2(del, del)));
-      s[e] = x.x;
-      s[e + 1] = x.y;
-    }
-    if (!whole) {
-      const int hi = p < len && !one ? p - c0 : -1;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const uint32_t on = range_bits(p - window + 1 - c0, hi, q) | range_bits(0, min(sinks - 1 - c0, hi), q);
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (!(on >> e & 1)) s[32 * q + e] = 0.f;
+      for (int e = 0; e < 64; e += 4) {  // every other pair on the FMA pipes
+        const float2 x = fma2(make_float2(s[e], s[e + 1]), cc, make_float2(lse2, lse2));
+        const float2 y = ex2_poly(fma2(make_float2(s[e + 2], s[e + 3]), cc, make_float2(lse2, lse2)));
+        s[e] = ex2(x.x);
+        s[e + 1] = ex2(x.y);
+        s[e + 2] = y.x;
+        s[e + 3] = y.y;
       }
+      if (!warp_wait(&bar.dp_full, T & 1, abort_flag)) return;
+      tc::fence_after();
+      float d[64];
+      tmem_ld64(tP, d);
+      tc::fence_before();
+      pipe::mbar_arrive(&bar.dp_read);
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) {
+        const float2 x = mul2(make_float2(s[e], s[e + 1]), add2(make_float2(d[e], d[e + 1]), make_float2(del, del)));
+        s[e] = x.x;
+        s[e + 1] = x.y;
+      }
+      if (!whole) {
+        const int hi = p < len && !one ? p - c0 : -1;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t on = range_bits(p - window + 1 - c0, hi, q) | range_bits(0, min(sinks - 1 - c0, hi), q);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!(on >> e & 1)) s[32 * q + e] = 0.f;
+        }
+      }
+      uint32_t pk[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
+      tmem_st32u(tS + buf * 128, pk);
+      tc::fence_before();
+      pipe::mbar_arrive(&bar.ds_ready[buf]);
     }
-    uint32_t pk[32];
+    if (w.kt.count) {
+      if (!warp_wait(&bar.o_full, items++ & 1, abort_flag)) return;
+      tc::fence_after();
+    }
 #pragma unroll
-    for (int e = 0; e < 32; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
-    tmem_st32u(tS + buf * 128, pk);
-    tc::fence_before();
-    pipe::mbar_arrive(&bar.ds_ready[buf]);
-  }
-  if (w.kt.count) {
-    if (!warp_wait(&bar.o_full, 0, abort_flag)) return;
-    tc::fence_after();
-  }
+    for (int d = 0; d < DB; ++d) {  // each warpgroup takes half of the columns
+      float o[32];
+      const int c = 32 * (half * DB + d);
+      if (w.kt.count) tc::tmem_ld32(tmem + lane_at + Q_DQ + c, o);
+      else
 #pragma unroll
-  for (int d = 0; d < DB; ++d) {  // each warpgroup takes half of the columns
-    float o[32];
-    const int c = 32 * (half * DB + d);
-    if (w.kt.count) tc::tmem_ld32(tmem + lane_at + Q_DQ + c, o);
-    else
-#pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = 0.f;
-    if (i < a.Tq) store32<false>(P.dq, (((int64_t)w.b * a.Tq + i) * a.H + w.h) * a.D + c, o, a.scale, (int)a.D - c);
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+      if (i < a.Tq) store32<false>(P.dq, (((int64_t)w.b * a.Tq + i) * a.H + w.h) * a.D + c, o, a.scale, (int)a.D - c);
+    }
   }
 }
 
 template <int DB>
-GDNX_DEV void queries_products(const QueryItem& w, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void queries_products(const BwdParams& P, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
   using Lo = Layout<DB>;
   constexpr uint32_t ID_S = idesc16(true, 128, 128, false, false), ID_O = idesc16(true, 128, 64 * DB, false, true);
-  const int n = w.kt.count;
+  uint32_t T = 0, items = 0;  // tiles before this item; items with tiles
   const auto slot = [&](uint32_t c) { return smem + Lo::RING + c % SLOTS * Lo::TILE; };
   const auto landed = [&](uint32_t c) { return warp_wait(&bar.full[c % SLOTS], c / SLOTS & 1, abort_flag); };
-  const auto scores = [&](int t) {
-    if (!landed(2 * t)) return false;
+  const auto scores = [&](int t, bool last) {
+    const uint32_t c = 2 * (T + t), buf = (T + t) & 1;
+    if (!landed(c)) return false;
     if (elect_one()) {
-      mma_abt<DB>(tmem + Q_S + (t & 1) * 128, smem + Lo::RES, slot(2 * t), ID_S);
-      tc::commit(&bar.s_full[t & 1]);
+      mma_abt<DB>(tmem + Q_S + buf * 128, smem + Lo::RES, slot(c), ID_S);
+      tc::commit(&bar.s_full[buf]);
+      if (last) tc::commit(&bar.res_empty[0]);
     }
     __syncwarp();
     return true;
   };
-  const auto dprobs = [&](int t) {
-    if (!landed(2 * t + 1)) return false;
-    if (elect_one()) {
-      mma_abt<DB>(tmem + Q_DP, smem + Lo::RES + Lo::TILE, slot(2 * t + 1), ID_S);
-      tc::commit(&bar.dp_full);
-      tc::commit(&bar.empty[(2 * t + 1) % SLOTS]);
-    }
-    __syncwarp();
-    return true;
-  };
-  if (n == 0) return;
-  if (!warp_wait(&bar.res[0], 0, abort_flag) || !scores(0)) return;
-  if (!warp_wait(&bar.res[1], 0, abort_flag) || !dprobs(0)) return;
-  if (n > 1 && !scores(1)) return;
-  for (int t = 0; t < n; ++t) {
-    if (t + 1 < n) {
-      if (!warp_wait(&bar.dp_read, t & 1, abort_flag)) return;
-      tc::fence_after();
-      if (!dprobs(t + 1)) return;
-    }
-    if (!warp_wait(&bar.ds_ready[t & 1], t / 2 & 1, abort_flag)) return;
+  const auto dprobs = [&](int t, bool last) {
+    const uint32_t c = 2 * (T + t) + 1;
+    if (!landed(c)) return false;
+    if (T + t > 0 && !warp_wait(&bar.dp_read, (T + t - 1) & 1, abort_flag)) return false;
     tc::fence_after();
     if (elect_one()) {
-      mma_halves(tmem + Q_DQ, tmem + Q_S + (t & 1) * 128, slot(2 * t), ID_O, t > 0);
-      tc::commit(&bar.empty[(2 * t) % SLOTS]);
+      mma_abt<DB>(tmem + Q_DP, smem + Lo::RES + Lo::TILE, slot(c), ID_S);
+      tc::commit(&bar.dp_full);
+      tc::commit(&bar.empty[c % SLOTS]);
+      if (last) tc::commit(&bar.res_empty[1]);
     }
     __syncwarp();
-    if (t + 2 < n && !scores(t + 2)) return;
+    return true;
+  };
+  for (unsigned it = blockIdx.x; it < P.queries; it += gridDim.x) {
+    const int n = query_item(P, it).kt.count;
+    if (n == 0) continue;
+    if (!warp_wait(&bar.res[0], items & 1, abort_flag) || !scores(0, n == 1)) return;
+    if (!warp_wait(&bar.res[1], items & 1, abort_flag) || !dprobs(0, n == 1)) return;
+    ++items;
+    if (n > 1 && !scores(1, n == 2)) return;
+    for (int t = 0; t < n; ++t) {
+      if (t + 1 < n && !dprobs(t + 1, t + 2 == n)) return;
+      const uint32_t buf = (T + t) & 1, c = 2 * (T + t);
+      if (!warp_wait(&bar.ds_ready[buf], (T + t) / 2 & 1, abort_flag)) return;
+      tc::fence_after();
+      if (elect_one()) {
+        mma_halves(tmem + Q_DQ, tmem + Q_S + buf * 128, slot(c), ID_O, t > 0);
+        tc::commit(&bar.empty[c % SLOTS]);
+        if (t + 1 == n) tc::commit(&bar.o_full);
+      }
+      __syncwarp();
+      if (t + 2 < n && !scores(t + 2, t + 3 == n)) return;
+    }
+    T += n;
   }
-  if (elect_one()) tc::commit(&bar.o_full);
 }
 
 template <int DB>
-GDNX_DEV void queries_loads(const BwdParams& P, const QueryItem& w, uint8_t* base, uint32_t smem, Bars& bar,
-                            volatile int* abort_flag) {
+GDNX_DEV void queries_loads(const BwdParams& P, uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag) {
   using Lo = Layout<DB>;
   const gdnx_attn_args& a = P.a;
-  uint32_t nfix = 0;
-  if (w.kt.count == 0) return;
-  if (threadIdx.x % 32 == 0)
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t mb = tc::smem_u32(&bar.res[i]);
-      pipe::expect_tx(mb, Lo::TILE);
-      load_rows<DB>(smem + Lo::RES + i * Lo::TILE, i ? P.dy : P.q, w.i0, w.h, w.b, mb);
+  uint32_t nfix = 0, T = 0, items = 0;
+  for (unsigned n = blockIdx.x; n < P.queries; n += gridDim.x) {
+    const QueryItem w = query_item(P, n);
+    for (int t = 0; t < w.kt.count; ++t, ++T) {
+      const int j0 = w.kt.tile(t) * TM;
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        // K is also the right factor of dS K: its padding rows must not hold NaN
+        if (!stream_tile<DB>(base, smem, bar, abort_flag, 2 * T + side, side ? P.v : P.k, j0, w.hk, w.b,
+                             side ? (int)a.Tk : w.len, a.Tk, nfix))
+          return;
+        if (t == 0) {  // Q beside the first K, dY beside the first V
+          if (!warp_wait(&bar.res_empty[side], (items & 1) ^ 1, abort_flag)) return;
+          if (threadIdx.x % 32 == 0) {
+            const uint32_t mb = tc::smem_u32(&bar.res[side]);
+            pipe::expect_tx(mb, Lo::TILE);
+            load_rows<DB>(smem + Lo::RES + side * Lo::TILE, side ? P.dy : P.q, w.i0, w.h, w.b, mb);
+          }
+        }
+      }
     }
-  for (int t = 0; t < w.kt.count; ++t) {
-    const int j0 = w.kt.tile(t) * TM;
-    // K is also the right factor of dS K: its padding rows must not hold NaN
-    if (!stream_tile<DB>(base, smem, bar, abort_flag, 2 * t, P.k, j0, w.hk, w.b, w.len, a.Tk, nfix) ||
-        !stream_tile<DB>(base, smem, bar, abort_flag, 2 * t + 1, P.v, j0, w.hk, w.b, (int)a.Tk, a.Tk, nfix))
-      return;
+    if (w.kt.count) ++items;
   }
 }
 
@@ -555,10 +578,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_c
       else if (warp == 8) keys_products<DB>(w, smem, tmem, bar, abort_flag);
       else if (warp == 9) keys_loads<DB>(P, w, base, smem, bar, abort_flag);
     } else {
-      const QueryItem w = query_item(P);
-      if (warp < 8) queries_rows<DB>(P, w, tmem, bar, abort_flag);
-      else if (warp == 8) queries_products<DB>(w, smem, tmem, bar, abort_flag);
-      else if (warp == 9) queries_loads<DB>(P, w, base, smem, bar, abort_flag);
+      if (warp < 8) queries_rows<DB>(P, tmem, bar, abort_flag);
+      else if (warp == 8) queries_products<DB>(P, smem, tmem, bar, abort_flag);
+      else if (warp == 9) queries_loads<DB>(P, base, smem, bar, abort_flag);
     }
   }
   if (warp == 8) {  // every product issued has ended
@@ -636,6 +658,7 @@ void plan(BwdParams& P) {
   P.qtiles = (int)((a.Tq + TM - 1) / TM);
   P.ktiles = (int)((a.Tk + TM - 1) / TM);
   P.nst = (int)((a.sinks + TM - 1) / TM);
+  P.queries = (unsigned)(P.qtiles * a.B * a.H);
   int64_t near = (a.window + TM - 1) / TM + 1;
   if (near > P.qtiles) near = P.qtiles;
   const int64_t it = G * near, it_sink = G * P.qtiles;
@@ -683,7 +706,8 @@ gdnx_status run(const gdnx_attn_bwd_args& g, BwdParams& P, cudaStream_t st) {
   };
   if (P.nst > 0 && P.seg_sink > 1) join(0, P.nst);
   if (P.ktiles > P.nst && P.seg > 1) join(P.nst, P.ktiles - P.nst);
-  queries<<<(unsigned)((int64_t)P.qtiles * a.B * a.H), NTHREADS, smem, st>>>(P);
+  const unsigned sms = (unsigned)sm_count();
+  queries<<<P.queries < sms ? P.queries : sms, NTHREADS, smem, st>>>(P);
   return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
 }
 
