@@ -8,8 +8,8 @@
 //     16-bit over the columns of S^T and dP^T; dV += P^T dY, dK += dS^T Q.
 //   attn_dq: 128 queries of a head; over the key tiles that they see
 //     S = Q K^T (two buffers), dP = dY V^T; dS over S's columns; dQ += dS K.
-// Accumulators stay in tensor memory (fp32).  Warpgroups 0 and 1 own the two halves of a
-// tile's columns (every lane's row in both), warp 8 issues the products, warp 9 the loads.
+// Accumulators stay in tensor memory (fp32).  Warpgroups 0 to 3 own 32 of a tile's 128
+// columns each (every lane's row in all), warp 16 issues the products, warp 17 the loads.
 // In attn_dkv dV(t) and S(t+1) run while the rows form dS(t), dK(t) and dP(t+1) while they
 // form P(t+1).
 //
@@ -27,7 +27,7 @@ namespace {
 
 using namespace attn;
 
-constexpr int NTHREADS = 384;
+constexpr int NTHREADS = 640;  // four warpgroups of rows, and the warps that issue
 constexpr int SLOTS = 5;        // streamed tiles in flight
 constexpr uint32_t STAT = TM * 4;  // bytes of one statistic of a tile's queries
 
@@ -62,12 +62,12 @@ GDNX_DEV uint32_t range_bits(int lo, int hi, int w) {
   return lo > hi ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
 }
 
-// D (+)= P X with P's columns in two halves, each over the start of its half of 128 columns.
-GDNX_DEV void mma_halves(uint32_t d, uint32_t p, uint32_t x, uint32_t idesc, bool acc) {
+// D (+)= P X with P's columns in four quarters, each over the start of its 32 of 128 columns.
+GDNX_DEV void mma_quarters(uint32_t d, uint32_t p, uint32_t x, uint32_t idesc, bool acc) {
   const uint64_t dx = tc::smem_desc(x, BLOCK_BYTES, 1024);
 #pragma unroll
   for (int k = 0; k < 8; ++k)
-    tc::mma_bf16_ts(d, p + (k < 4 ? 8 * k : 64 + 8 * (k - 4)), dx + k * (2048 >> 4), idesc, acc || k > 0);
+    tc::mma_bf16_ts(d, p + 32 * (k / 2) + 8 * (k % 2), dx + k * (2048 >> 4), idesc, acc || k > 0);
 }
 
 // Rows r0.. of a landed tile to zero: padding rows meet weights of 0, so they must not hold NaN.
@@ -81,15 +81,28 @@ GDNX_DEV void zero_rows(uint8_t* tile, int r0, int lane) {
   __syncwarp();
 }
 
-// One streamed tile into the ring (whole warp): rows t0.. of head h, rows from `valid` on
-// (in the tensor's own rows, below `rows`) to zero.
+// A place in the ring: its slot, and how often the slot was used before.
+struct Place {
+  uint32_t sl, use;
+};
+// attn_dkv: Q and dY of its tiles in turn through all five slots.
+GDNX_DEV Place keys_place(uint32_t c) { return {c % SLOTS, c / SLOTS}; }
+// attn_dq: K through three slots and V through two.  K(t) stays until dQ(t), V(t) only until
+// dP(t): in one ring V(t+2) would take K(t)'s slot, and its load would stand between dQ(t) and
+// dP(t+2).
+GDNX_DEV Place queries_place(uint32_t t, int side) {
+  return side ? Place{3 + t % 2, t / 2} : Place{t % 3, t / 3};
+}
+
+// One streamed tile (whole warp): rows t0.. of head h, rows from `valid` on (in the tensor's own
+// rows, below `rows`) to zero.
 template <int DB>
-GDNX_DEV bool stream_tile(uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag, uint32_t cnt,
+GDNX_DEV bool stream_tile(uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag, Place at,
                           const TileMap& m, int t0, int64_t h, int64_t b, int valid, int64_t rows, uint32_t& nfix) {
   using Lo = Layout<DB>;
-  const uint32_t sl = cnt % SLOTS;
+  const uint32_t sl = at.sl;
   const int lane = threadIdx.x % 32;
-  if (!warp_wait(&bar.empty[sl], (cnt / SLOTS & 1) ^ 1, abort_flag)) return false;
+  if (!warp_wait(&bar.empty[sl], (at.use & 1) ^ 1, abort_flag)) return false;
   const bool fix = valid < rows && t0 + TM > valid;
   if (lane == 0) {
     const uint32_t mb = tc::smem_u32(fix ? &bar.fix : &bar.full[sl]);
@@ -113,23 +126,23 @@ GDNX_DEV void init_bars(Bars& bar) {
     tc::mbar_init(&bar.res[i], 1);
     tc::mbar_init(&bar.res_empty[i], 1);
     tc::mbar_init(&bar.stat_full[i], 1);
-    tc::mbar_init(&bar.stat_empty[i], 256);
+    tc::mbar_init(&bar.stat_empty[i], 512);
     tc::mbar_init(&bar.s_full[i], 1);
-    tc::mbar_init(&bar.ds_ready[i], 256);
+    tc::mbar_init(&bar.ds_ready[i], 512);
   }
   tc::mbar_init(&bar.dp_full, 1);
-  tc::mbar_init(&bar.p_ready, 256);
-  tc::mbar_init(&bar.dp_read, 256);
+  tc::mbar_init(&bar.p_ready, 512);
+  tc::mbar_init(&bar.dp_read, 512);
   tc::mbar_init(&bar.o_full, 1);
   tc::mbar_init(&bar.fix, 1);
   tc::mbar_init(&bar.done, 1);
 }
 
-// 32 accumulator values of one row, scaled, to 16-bit or fp32 memory (columns below D only).
-template <bool F32>
-GDNX_DEV void store32(void* dst, int64_t at, const float* o, float scale, int left) {
+// N accumulator values of one row, scaled, to 16-bit or fp32 memory (columns below D only).
+template <bool F32, int N>
+GDNX_DEV void store_row(void* dst, int64_t at, const float* o, float scale, int left) {
 #pragma unroll
-  for (int e = 0; e < 32; e += 8) {
+  for (int e = 0; e < N; e += 8) {
     if (e >= left) continue;
     if (F32) {
       float4* p = reinterpret_cast<float4*>(static_cast<float*>(dst) + at + e);
@@ -188,9 +201,9 @@ GDNX_DEV void keys_rows(const BwdParams& P, const KeyItem& w, const uint8_t* bas
                         volatile int* abort_flag) {
   using Lo = Layout<DB>;
   const gdnx_attn_args& a = P.a;
-  const int r = threadIdx.x % 128, half = threadIdx.x / 128;
+  const int r = threadIdx.x % 128, part = threadIdx.x / 128;
   const uint32_t lane_at = (uint32_t)(r / 32 * 32) << 16;
-  const uint32_t tS = tmem + lane_at + K_S + half * 64, tP = tmem + lane_at + K_DP + half * 64;
+  const uint32_t tS = tmem + lane_at + K_S + part * 32, tP = tmem + lane_at + K_DP + part * 32;
   const int off = (int)(a.Tk - a.Tq), window = (int)a.window, sinks = (int)a.sinks, len = w.len;
   const float c2 = a.scale * kLog2e;
   const int j = w.j0 + r;
@@ -198,19 +211,19 @@ GDNX_DEV void keys_rows(const BwdParams& P, const KeyItem& w, const uint8_t* bas
   const bool none = window == 1 && sinks == 0;  // every query sees one key: dS is 0
   for (int t = w.t0; t < w.t1; ++t) {
     const uint32_t it = t - w.t0, ss = it & 1;
-    const int p0 = (w.qlo + t % w.nq) * TM + off + half * 64;  // position of this half's first column
-    const float* lse = reinterpret_cast<const float*>(base + Lo::STATS + ss * 2 * STAT) + half * 64;
+    const int p0 = (w.qlo + t % w.nq) * TM + off + part * 32;  // position of this quarter's first column
+    const float* lse = reinterpret_cast<const float*>(base + Lo::STATS + ss * 2 * STAT) + part * 32;
     const float* del = lse + TM;
     if (!warp_wait(&bar.stat_full[ss], it / 2 & 1, abort_flag) || !warp_wait(&bar.s_full[0], it & 1, abort_flag)) return;
     tc::fence_after();
-    float s[64];
-    tmem_ld64(tS, s);
-    const bool whole = p0 >= w.j0 + TM - 1 && p0 + 64 <= len && w.j0 + TM <= len &&
-                       (p0 + 63 - w.j0 < window || w.j0 + TM <= sinks);
-    uint32_t on[2] = {0xffffffffu, 0xffffffffu};
+    float s[32];
+    tc::tmem_ld32(tS, s);
+    const bool whole = p0 >= w.j0 + TM - 1 && p0 + 32 <= len && w.j0 + TM <= len &&
+                       (p0 + 31 - w.j0 < window || w.j0 + TM <= sinks);
+    uint32_t on = 0xffffffffu;
     const float2 cc = make_float2(c2, c2);
 #pragma unroll
-    for (int e = 0; e < 64; e += 4) {  // every other pair on the FMA pipes
+    for (int e = 0; e < 32; e += 4) {  // every other pair on the FMA pipes
       const float4 z = *reinterpret_cast<const float4*>(lse + e);
       const float2 x = fma2(make_float2(s[e], s[e + 1]), cc, make_float2(z.x, z.y));
       const float2 y = ex2_poly(fma2(make_float2(s[e + 2], s[e + 3]), cc, make_float2(z.z, z.w)));
@@ -220,28 +233,25 @@ GDNX_DEV void keys_rows(const BwdParams& P, const KeyItem& w, const uint8_t* bas
       s[e + 3] = y.y;
     }
     if (!whole) {
+      on = range_bits(j - p0, last - p0, 0);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        on[q] = range_bits(j - p0, last - p0, q);
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (!(on[q] >> e & 1)) s[32 * q + e] = 0.f;
-      }
-      if (p0 == 0) on[0] &= ~1u;  // position 0 sees one key
-      if (none) on[0] = on[1] = 0;
+      for (int e = 0; e < 32; ++e)
+        if (!(on >> e & 1)) s[e] = 0.f;
+      if (p0 == 0) on &= ~1u;  // position 0 sees one key
+      if (none) on = 0;
     }
-    uint32_t pk[32];
+    uint32_t pk[16];
 #pragma unroll
-    for (int e = 0; e < 32; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
-    tmem_st32u(tS, pk);
+    for (int e = 0; e < 16; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
+    tc::tmem_st16u(tS, pk);
     tc::fence_before();
     pipe::mbar_arrive(&bar.p_ready);
     if (!warp_wait(&bar.dp_full, it & 1, abort_flag)) return;
     tc::fence_after();
-    float d[64];
-    tmem_ld64(tP, d);
+    float d[32];
+    tc::tmem_ld32(tP, d);
 #pragma unroll
-    for (int e = 0; e < 64; e += 4) {
+    for (int e = 0; e < 32; e += 4) {
       const float4 z = *reinterpret_cast<const float4*>(del + e);
       const float2 x = mul2(make_float2(s[e], s[e + 1]), add2(make_float2(d[e], d[e + 1]), make_float2(z.x, z.y)));
       const float2 y = mul2(make_float2(s[e + 2], s[e + 3]), add2(make_float2(d[e + 2], d[e + 3]), make_float2(z.z, z.w)));
@@ -252,36 +262,37 @@ GDNX_DEV void keys_rows(const BwdParams& P, const KeyItem& w, const uint8_t* bas
     }
     if (!whole) {
 #pragma unroll
-      for (int e = 0; e < 64; ++e)
-        if (!(on[e / 32] >> (e % 32) & 1)) s[e] = 0.f;
+      for (int e = 0; e < 32; ++e)
+        if (!(on >> e & 1)) s[e] = 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < 32; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
-    tmem_st32u(tP, pk);
+    for (int e = 0; e < 16; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
+    tc::tmem_st16u(tP, pk);
     tc::fence_before();
     pipe::mbar_arrive(&bar.ds_ready[0]);
     pipe::mbar_arrive(&bar.stat_empty[ss]);
   }
-  // warpgroup 0 writes dV, warpgroup 1 dK
+  // warpgroups 0 and 1 write dV, 2 and 3 dK, half of the columns each
   if (w.t1 > w.t0) {
     if (!warp_wait(&bar.o_full, 0, abort_flag)) return;
     tc::fence_after();
   }
-  const uint32_t tO = tmem + lane_at + (half ? K_DK : K_DV);
-  const float scale = half ? a.scale : 1.f;
+  const int side = part / 2;
+  const uint32_t tO = tmem + lane_at + (side ? K_DK : K_DV);
+  const float scale = side ? a.scale : 1.f;
 #pragma unroll
-  for (int d = 0; d < 2 * DB; ++d) {
+  for (int d = 0; d < DB; ++d) {
     float o[32];
-    if (w.t1 > w.t0) tc::tmem_ld32(tO + 32 * d, o);
+    const int c = 32 * (part % 2 * DB + d);
+    if (w.t1 > w.t0) tc::tmem_ld32(tO + c, o);
     else
 #pragma unroll
       for (int e = 0; e < 32; ++e) o[e] = 0.f;
     if (w.nseg > 1) {
-      float* dst = P.part + ((int64_t)blockIdx.x * 2 + half) * TM * 64 * DB;
-      store32<true>(dst, (int64_t)r * 64 * DB + 32 * d, o, scale, 32);
+      float* dst = P.part + ((int64_t)blockIdx.x * 2 + side) * TM * 64 * DB;
+      store_row<true, 32>(dst, (int64_t)r * 64 * DB + c, o, scale, 32);
     } else if (j < a.Tk) {
-      store32<false>(half ? P.dk : P.dv, (((int64_t)w.b * a.Tk + j) * a.Hk + w.hk) * a.D + 32 * d, o, scale,
-                     (int)a.D - 32 * d);
+      store_row<false, 32>(side ? P.dk : P.dv, (((int64_t)w.b * a.Tk + j) * a.Hk + w.hk) * a.D + c, o, scale, (int)a.D - c);
     }
   }
 }
@@ -318,7 +329,7 @@ GDNX_DEV void keys_products(const KeyItem& w, uint32_t smem, uint32_t tmem, Bars
     if (!warp_wait(&bar.p_ready, t & 1, abort_flag)) return;
     tc::fence_after();
     if (elect_one()) {
-      mma_halves(tmem + K_DV, tmem + K_S, slot(2 * t + 1), ID_O, t > 0);
+      mma_quarters(tmem + K_DV, tmem + K_S, slot(2 * t + 1), ID_O, t > 0);
       tc::commit(&bar.empty[(2 * t + 1) % SLOTS]);
     }
     __syncwarp();
@@ -326,7 +337,7 @@ GDNX_DEV void keys_products(const KeyItem& w, uint32_t smem, uint32_t tmem, Bars
     if (!warp_wait(&bar.ds_ready[0], t & 1, abort_flag)) return;
     tc::fence_after();
     if (elect_one()) {
-      mma_halves(tmem + K_DK, tmem + K_DP, slot(2 * t), ID_O, t > 0);
+      mma_quarters(tmem + K_DK, tmem + K_DP, slot(2 * t), ID_O, t > 0);
       tc::commit(&bar.empty[(2 * t) % SLOTS]);
     }
     __syncwarp();
@@ -353,7 +364,7 @@ GDNX_DEV void keys_loads(const BwdParams& P, const KeyItem& w, uint8_t* base, ui
   for (int t = w.t0; t < w.t1; ++t) {
     const uint32_t it = t - w.t0, ss = it & 1;
     const int h = w.hk * G + t / w.nq, qt = w.qlo + t % w.nq;
-    if (!stream_tile<DB>(base, smem, bar, abort_flag, 2 * it, P.q, qt * TM, h, w.b, rows, a.Tq, nfix)) return;
+    if (!stream_tile<DB>(base, smem, bar, abort_flag, keys_place(2 * it), P.q, qt * TM, h, w.b, rows, a.Tq, nfix)) return;
     if (!warp_wait(&bar.stat_empty[ss], (it / 2 & 1) ^ 1, abort_flag)) return;
     if (lane == 0) {
       const uint32_t mb = tc::smem_u32(&bar.stat_full[ss]), dst = smem + Lo::STATS + ss * 2 * STAT;
@@ -362,7 +373,7 @@ GDNX_DEV void keys_loads(const BwdParams& P, const KeyItem& w, uint8_t* base, ui
       pipe::bulk_load(dst, P.lse2 + at, STAT, mb);
       pipe::bulk_load(dst + STAT, P.delta + at, STAT, mb);
     }
-    if (!stream_tile<DB>(base, smem, bar, abort_flag, 2 * it + 1, P.dy, qt * TM, h, w.b, rows, a.Tq, nfix)) return;
+    if (!stream_tile<DB>(base, smem, bar, abort_flag, keys_place(2 * it + 1), P.dy, qt * TM, h, w.b, rows, a.Tq, nfix)) return;
   }
 }
 
@@ -390,9 +401,9 @@ constexpr uint32_t Q_S = 0, Q_DP = 256, Q_DQ = 384;  // S has two buffers
 template <int DB>
 GDNX_DEV void queries_rows(const BwdParams& P, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
   const gdnx_attn_args& a = P.a;
-  const int r = threadIdx.x % 128, half = threadIdx.x / 128;
+  const int r = threadIdx.x % 128, part = threadIdx.x / 128;
   const uint32_t lane_at = (uint32_t)(r / 32 * 32) << 16;
-  const uint32_t tS = tmem + lane_at + Q_S + half * 64, tP = tmem + lane_at + Q_DP + half * 64;
+  const uint32_t tS = tmem + lane_at + Q_S + part * 32, tP = tmem + lane_at + Q_DP + part * 32;
   const int window = (int)a.window, sinks = (int)a.sinks;
   const float c2 = a.scale * kLog2e;
   const float2 cc = make_float2(c2, c2);
@@ -405,14 +416,14 @@ GDNX_DEV void queries_rows(const BwdParams& P, uint32_t tmem, Bars& bar, volatil
     const bool one = sees_one(p, window, sinks);
     for (int t = 0; t < w.kt.count; ++t, ++T) {
       const uint32_t buf = T & 1;
-      const int j0 = w.kt.tile(t) * TM, c0 = j0 + half * 64;  // this half's first key
+      const int j0 = w.kt.tile(t) * TM, c0 = j0 + part * 32;  // this quarter's first key
       if (!warp_wait(&bar.s_full[buf], T / 2 & 1, abort_flag)) return;
       tc::fence_after();
-      float s[64];
-      tmem_ld64(tS + buf * 128, s);
-      const bool whole = c0 + 63 <= w.p0 && w.p0 + TM <= len && (w.p0 + TM - 1 - c0 < window || c0 + 64 <= sinks);
+      float s[32];
+      tc::tmem_ld32(tS + buf * 128, s);
+      const bool whole = c0 + 31 <= w.p0 && w.p0 + TM <= len && (w.p0 + TM - 1 - c0 < window || c0 + 32 <= sinks);
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {  // every other pair on the FMA pipes
+      for (int e = 0; e < 32; e += 4) {  // every other pair on the FMA pipes
         const float2 x = fma2(make_float2(s[e], s[e + 1]), cc, make_float2(lse2, lse2));
         const float2 y = ex2_poly(fma2(make_float2(s[e + 2], s[e + 3]), cc, make_float2(lse2, lse2)));
         s[e] = ex2(x.x);
@@ -422,30 +433,27 @@ GDNX_DEV void queries_rows(const BwdParams& P, uint32_t tmem, Bars& bar, volatil
       }
       if (!warp_wait(&bar.dp_full, T & 1, abort_flag)) return;
       tc::fence_after();
-      float d[64];
-      tmem_ld64(tP, d);
+      float d[32];
+      tc::tmem_ld32(tP, d);
       tc::fence_before();
       pipe::mbar_arrive(&bar.dp_read);
 #pragma unroll
-      for (int e = 0; e < 64; e += 2) {
+      for (int e = 0; e < 32; e += 2) {
         const float2 x = mul2(make_float2(s[e], s[e + 1]), add2(make_float2(d[e], d[e + 1]), make_float2(del, del)));
         s[e] = x.x;
         s[e + 1] = x.y;
       }
       if (!whole) {
         const int hi = p < len && !one ? p - c0 : -1;
+        const uint32_t on = range_bits(p - window + 1 - c0, hi, 0) | range_bits(0, min(sinks - 1 - c0, hi), 0);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint32_t on = range_bits(p - window + 1 - c0, hi, q) | range_bits(0, min(sinks - 1 - c0, hi), q);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!(on >> e & 1)) s[32 * q + e] = 0.f;
-        }
+        for (int e = 0; e < 32; ++e)
+          if (!(on >> e & 1)) s[e] = 0.f;
       }
-      uint32_t pk[32];
+      uint32_t pk[16];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
-      tmem_st32u(tS + buf * 128, pk);
+      for (int e = 0; e < 16; ++e) pk[e] = tc::pack_bf16(s[2 * e], s[2 * e + 1]);
+      tc::tmem_st16u(tS + buf * 128, pk);
       tc::fence_before();
       pipe::mbar_arrive(&bar.ds_ready[buf]);
     }
@@ -454,14 +462,15 @@ GDNX_DEV void queries_rows(const BwdParams& P, uint32_t tmem, Bars& bar, volatil
       tc::fence_after();
     }
 #pragma unroll
-    for (int d = 0; d < DB; ++d) {  // each warpgroup takes half of the columns
-      float o[32];
-      const int c = 32 * (half * DB + d);
-      if (w.kt.count) tc::tmem_ld32(tmem + lane_at + Q_DQ + c, o);
+    for (int d = 0; d < 16 * DB; d += 16) {  // each warpgroup takes a quarter of the columns
+      float o[16];
+      const int c = 16 * DB * part + d;
+      if (w.kt.count) tc::tmem_ld16(tmem + lane_at + Q_DQ + c, o);
       else
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0.f;
-      if (i < a.Tq) store32<false>(P.dq, (((int64_t)w.b * a.Tq + i) * a.H + w.h) * a.D + c, o, a.scale, (int)a.D - c);
+        for (int e = 0; e < 16; ++e) o[e] = 0.f;
+      if (i < a.Tq)
+        store_row<false, 16>(P.dq, (((int64_t)w.b * a.Tq + i) * a.H + w.h) * a.D + c, o, a.scale, (int)a.D - c);
     }
   }
 }
@@ -471,10 +480,11 @@ GDNX_DEV void queries_products(const BwdParams& P, uint32_t smem, uint32_t tmem,
   using Lo = Layout<DB>;
   constexpr uint32_t ID_S = idesc16(true, 128, 128, false, false), ID_O = idesc16(true, 128, 64 * DB, false, true);
   uint32_t T = 0, items = 0;  // tiles before this item; items with tiles
-  const auto slot = [&](uint32_t c) { return smem + Lo::RING + c % SLOTS * Lo::TILE; };
-  const auto landed = [&](uint32_t c) { return warp_wait(&bar.full[c % SLOTS], c / SLOTS & 1, abort_flag); };
+  const auto slot = [&](Place at) { return smem + Lo::RING + at.sl * Lo::TILE; };
+  const auto landed = [&](Place at) { return warp_wait(&bar.full[at.sl], at.use & 1, abort_flag); };
   const auto scores = [&](int t, bool last) {
-    const uint32_t c = 2 * (T + t), buf = (T + t) & 1;
+    const Place c = queries_place(T + t, 0);
+    const uint32_t buf = (T + t) & 1;
     if (!landed(c)) return false;
     if (elect_one()) {
       mma_abt<DB>(tmem + Q_S + buf * 128, smem + Lo::RES, slot(c), ID_S);
@@ -485,14 +495,14 @@ GDNX_DEV void queries_products(const BwdParams& P, uint32_t smem, uint32_t tmem,
     return true;
   };
   const auto dprobs = [&](int t, bool last) {
-    const uint32_t c = 2 * (T + t) + 1;
+    const Place c = queries_place(T + t, 1);
     if (!landed(c)) return false;
     if (T + t > 0 && !warp_wait(&bar.dp_read, (T + t - 1) & 1, abort_flag)) return false;
     tc::fence_after();
     if (elect_one()) {
       mma_abt<DB>(tmem + Q_DP, smem + Lo::RES + Lo::TILE, slot(c), ID_S);
       tc::commit(&bar.dp_full);
-      tc::commit(&bar.empty[c % SLOTS]);
+      tc::commit(&bar.empty[c.sl]);
       if (last) tc::commit(&bar.res_empty[1]);
     }
     __syncwarp();
@@ -507,12 +517,13 @@ GDNX_DEV void queries_products(const BwdParams& P, uint32_t smem, uint32_t tmem,
     if (n > 1 && !scores(1, n == 2)) return;
     for (int t = 0; t < n; ++t) {
       if (t + 1 < n && !dprobs(t + 1, t + 2 == n)) return;
-      const uint32_t buf = (T + t) & 1, c = 2 * (T + t);
+      const Place c = queries_place(T + t, 0);
+      const uint32_t buf = (T + t) & 1;
       if (!warp_wait(&bar.ds_ready[buf], (T + t) / 2 & 1, abort_flag)) return;
       tc::fence_after();
       if (elect_one()) {
-        mma_halves(tmem + Q_DQ, tmem + Q_S + buf * 128, slot(c), ID_O, t > 0);
-        tc::commit(&bar.empty[c % SLOTS]);
+        mma_quarters(tmem + Q_DQ, tmem + Q_S + buf * 128, slot(c), ID_O, t > 0);
+        tc::commit(&bar.empty[c.sl]);
         if (t + 1 == n) tc::commit(&bar.o_full);
       }
       __syncwarp();
@@ -534,7 +545,7 @@ GDNX_DEV void queries_loads(const BwdParams& P, uint8_t* base, uint32_t smem, Ba
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
         // K is also the right factor of dS K: its padding rows must not hold NaN
-        if (!stream_tile<DB>(base, smem, bar, abort_flag, 2 * T + side, side ? P.v : P.k, j0, w.hk, w.b,
+        if (!stream_tile<DB>(base, smem, bar, abort_flag, queries_place(T, side), side ? P.v : P.k, j0, w.hk, w.b,
                              side ? (int)a.Tk : w.len, a.Tk, nfix))
           return;
         if (t == 0) {  // Q beside the first K, dY beside the first V
@@ -566,7 +577,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_c
     *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
     init_bars(bar);
   }
-  if (warp == 8) tc::tmem_alloc(tmem_at, 512);
+  if (warp == 16) tc::tmem_alloc(tmem_at, 512);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -574,27 +585,27 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_c
   if (smem % 1024 == 0) {
     if (KEYS) {
       const KeyItem w = key_item(P);
-      if (warp < 8) keys_rows<DB>(P, w, base, tmem, bar, abort_flag);
-      else if (warp == 8) keys_products<DB>(w, smem, tmem, bar, abort_flag);
-      else if (warp == 9) keys_loads<DB>(P, w, base, smem, bar, abort_flag);
+      if (warp < 16) keys_rows<DB>(P, w, base, tmem, bar, abort_flag);
+      else if (warp == 16) keys_products<DB>(w, smem, tmem, bar, abort_flag);
+      else if (warp == 17) keys_loads<DB>(P, w, base, smem, bar, abort_flag);
     } else {
-      if (warp < 8) queries_rows<DB>(P, tmem, bar, abort_flag);
-      else if (warp == 8) queries_products<DB>(P, smem, tmem, bar, abort_flag);
-      else if (warp == 9) queries_loads<DB>(P, base, smem, bar, abort_flag);
+      if (warp < 16) queries_rows<DB>(P, tmem, bar, abort_flag);
+      else if (warp == 16) queries_products<DB>(P, smem, tmem, bar, abort_flag);
+      else if (warp == 17) queries_loads<DB>(P, base, smem, bar, abort_flag);
     }
   }
-  if (warp == 8) {  // every product issued has ended
+  if (warp == 16) {  // every product issued has ended
     __syncwarp();
     if (elect_one()) tc::commit(&bar.done);
     tc::mbar_wait(&bar.done, 0);
   }
-  if (warp == 9 && *abort_flag)  // let the copies in flight land
+  if (warp == 17 && *abort_flag)  // let the copies in flight land
     for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
   __syncwarp();
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 8) tc::tmem_dealloc(tmem, 512);
+  if (warp == 16) tc::tmem_dealloc(tmem, 512);
   if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
 }
 
