@@ -10,6 +10,7 @@
 // whatever the thread order); a second kernel moves the pages.
 #include "common.cuh"
 #include "kernels.h"
+#include "launch.cuh"
 
 namespace gdnx {
 namespace {
@@ -78,6 +79,8 @@ template <int OP>
 __global__ void __launch_bounds__(ROW_NT) cache_rows_kernel(const gdnx_cache c, int64_t n, const int32_t* rows,
                                                             const int32_t* arg, int64_t window, int64_t sinks) {
   extern __shared__ uint32_t seen[];
+  dependents_may_start();
+  wait_for_earlier();
   if (*c.status != 0) return;
   if (!rows_ok(seen, c, n, rows, OP == kFork ? arg : nullptr, OP == kTruncate ? arg : nullptr)) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *c.status = GDNX_EINVAL;
@@ -151,6 +154,8 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
   __shared__ int sums[32];
   __shared__ int ncopy;
   const Plan w(ws, c.pages, n);
+  dependents_may_start();
+  wait_for_earlier();
   if (threadIdx.x == 0) {
     w.head[0] = 0;
     ncopy = 0;
@@ -246,6 +251,8 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
 __global__ void __launch_bounds__(NT) cache_compact_kernel(const gdnx_cache c, void* ws) {
   __shared__ int sums[32];
   const Plan w(ws, c.pages, 0);
+  dependents_may_start();
+  wait_for_earlier();
   if (threadIdx.x == 0) w.head[0] = 0;
   if (*c.status != 0) return;
   int64_t live = 0;
@@ -293,6 +300,8 @@ __global__ void __launch_bounds__(NT) cache_compact_kernel(const gdnx_cache c, v
 __global__ void __launch_bounds__(COPY_NT) cache_copy_kernel(const gdnx_cache c, void* ws, int64_t n, int64_t run,
                                                              int rename) {
   const Plan w(ws, c.pages, n);
+  dependents_may_start();
+  wait_for_earlier();
   const int m = w.head[0];
   if (m == 0) return;
   if (rename) {
@@ -329,6 +338,8 @@ template <typename V>
 __global__ void __launch_bounds__(256) cache_write_kernel(const gdnx_cache c, int64_t layer, int64_t n, int64_t T,
                                                           const gdnx_view k, const gdnx_view v, const int32_t* rows,
                                                           const int32_t* counts, int es) {
+  dependents_may_start();
+  wait_for_earlier();
   if (*c.status != 0) return;
   const int per = (int)(c.D * es / sizeof(V));  // pieces of one head
   const int64_t all = n * T * c.Hk * per * 2;
@@ -352,14 +363,13 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const gdnx_cache c, in
 
 size_t seen_bytes(const gdnx_cache& c) { return (size_t)((c.slots + 31) / 32) * 4; }
 
-gdnx_status launched() { return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH; }
+gdnx_status launched(cudaError_t e) { return e == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH; }
 
 int elem(int dtype) { return dtype == GDNX_F32 ? 4 : 2; }
 
 gdnx_status copy_pages(const gdnx_cache& c, void* ws, int64_t n, int rename, cudaStream_t st) {
   const int64_t run = c.Hk * c.page * c.D * elem(c.dtype);
-  cache_copy_kernel<<<148 * 8, COPY_NT, 0, st>>>(c, ws, n, run, rename);
-  return launched();
+  return launched(launch_early(cache_copy_kernel, dim3(148 * 8), dim3(COPY_NT), 0, st, c, ws, n, run, rename));
 }
 
 }  // namespace
@@ -367,32 +377,31 @@ gdnx_status copy_pages(const gdnx_cache& c, void* ws, int64_t n, int rename, cud
 size_t cache_workspace_bytes(const gdnx_cache& c, int64_t n) { return Plan::bytes(c.pages, n); }
 
 gdnx_status launch_cache_fork(const gdnx_cache& c, int64_t n, const int32_t* src, const int32_t* dst, cudaStream_t st) {
-  cache_rows_kernel<kFork><<<(unsigned)n, ROW_NT, seen_bytes(c), st>>>(c, n, dst, src, 0, 0);
-  return launched();
+  return launched(launch_early(cache_rows_kernel<kFork>, dim3((unsigned)n), dim3(ROW_NT), seen_bytes(c), st, c, n, dst,
+                               src, 0, 0));
 }
 
 gdnx_status launch_cache_truncate(const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* lengths,
                                   cudaStream_t st) {
-  cache_rows_kernel<kTruncate><<<(unsigned)n, ROW_NT, seen_bytes(c), st>>>(c, n, rows, lengths, 0, 0);
-  return launched();
+  return launched(launch_early(cache_rows_kernel<kTruncate>, dim3((unsigned)n), dim3(ROW_NT), seen_bytes(c), st, c, n,
+                               rows, lengths, 0, 0));
 }
 
 gdnx_status launch_cache_trim(const gdnx_cache& c, int64_t n, const int32_t* rows, int64_t window, int64_t sinks,
                               cudaStream_t st) {
-  cache_rows_kernel<kTrim><<<(unsigned)n, ROW_NT, seen_bytes(c), st>>>(c, n, rows, nullptr, window, sinks);
-  return launched();
+  return launched(launch_early(cache_rows_kernel<kTrim>, dim3((unsigned)n), dim3(ROW_NT), seen_bytes(c), st, c, n, rows,
+                               nullptr, window, sinks));
 }
 
 gdnx_status launch_cache_extend(const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* counts, void* ws,
                                 cudaStream_t st) {
-  cache_extend_kernel<<<1, NT, seen_bytes(c), st>>>(c, n, rows, counts, ws);
-  if (cudaGetLastError() != cudaSuccess) return GDNX_ELAUNCH;
+  if (launch_early(cache_extend_kernel, dim3(1), dim3(NT), seen_bytes(c), st, c, n, rows, counts, ws) != cudaSuccess)
+    return GDNX_ELAUNCH;
   return copy_pages(c, ws, n, 0, st);
 }
 
 gdnx_status launch_cache_compact(const gdnx_cache& c, void* ws, cudaStream_t st) {
-  cache_compact_kernel<<<1, NT, 0, st>>>(c, ws);
-  if (cudaGetLastError() != cudaSuccess) return GDNX_ELAUNCH;
+  if (launch_early(cache_compact_kernel, dim3(1), dim3(NT), 0, st, c, ws) != cudaSuccess) return GDNX_ELAUNCH;
   return copy_pages(c, ws, 0, 1, st);
 }
 
@@ -406,10 +415,8 @@ gdnx_status launch_cache_write(const gdnx_cache& c, int64_t layer, int64_t n, in
   const int64_t all = n * T * c.Hk * (v16 ? c.D / vec : c.D) * 2;
   const int64_t most = 148 * 64;
   const unsigned grid = (unsigned)((all + 255) / 256 < most ? (all + 255) / 256 : most);
-  if (v16) cache_write_kernel<uint4><<<grid, 256, 0, st>>>(c, layer, n, T, k, v, rows, counts, es);
-  else if (es == 4) cache_write_kernel<uint32_t><<<grid, 256, 0, st>>>(c, layer, n, T, k, v, rows, counts, es);
-  else cache_write_kernel<uint16_t><<<grid, 256, 0, st>>>(c, layer, n, T, k, v, rows, counts, es);
-  return launched();
+  const auto kernel = v16 ? cache_write_kernel<uint4> : es == 4 ? cache_write_kernel<uint32_t> : cache_write_kernel<uint16_t>;
+  return launched(launch_early(kernel, dim3(grid), dim3(256), 0, st, c, layer, n, T, k, v, rows, counts, es));
 }
 
 }  // namespace gdnx

@@ -21,6 +21,7 @@
 // and released pages hold may be NaN.
 #include "attn_tc.cuh"
 #include "kernels.h"
+#include "launch.cuh"
 
 namespace gdnx {
 namespace {
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   volatile int* abort_flag = &sm.abort_flag;
   const uint32_t smem = uniform(tc::smem_u32(base));
   const int warp = uniform(threadIdx.x / 32), units = (int)P.a.cache.Hk * P.groups;
-  asm volatile("griddepcontrol.launch_dependents;");  // the join may be set up; it waits for this grid's end
+  dependents_may_start();
   if (warp == 4) {
     tc::tmem_alloc(&sm.tmem_at, Lo::TMEM);
   } else if (threadIdx.x == 160) {
@@ -530,6 +531,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
     tc::mbar_init(&bar.done, 1);
   }
   tc::fence_before();
+  wait_for_earlier();
   find_range(P, units, sm.range, sm.sums);  // synchronises
   tc::fence_after();
   const uint32_t tmem = uniform(sm.tmem_at);
@@ -567,7 +569,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_decode_join_kernel(cons
   const gdnx_paged_decode_args& a = P.a;
   __shared__ float red_m[JOIN_WARPS], red_l[JOIN_WARPS], red_o[JOIN_WARPS][128];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, D = (int)a.cache.D, g = blockIdx.y;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are there
+  dependents_may_start();
+  wait_for_earlier();  // the parts are there
   const Joint j = P.joint[blockIdx.x];
   if (j.c1 < 0) return;
   const Heads hd(P, j.unit, NH);
@@ -643,21 +646,11 @@ gdnx_status launch(const DecParams& P, cudaStream_t st) {
   constexpr int smem = (int)Layout<DB, NH>::SMEM;
   static std::atomic<uint64_t> done;
   if (!allow_smem(kernel, smem, done)) return GDNX_ELAUNCH;
-  kernel<<<(unsigned)P.grid, NTHREADS, smem, st>>>(P);
-  if (!P.whole) {
-    cudaLaunchAttribute early;  // set up while the parts are made
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    const int64_t G = P.a.H / P.a.cache.Hk;
-    cfg.gridDim = dim3((unsigned)P.grid, (unsigned)(G < NH ? G : NH));
-    cfg.blockDim = dim3(JOIN_WARPS * 32);
-    cfg.stream = st;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<NH>, P);
-  }
-  return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
+  if (launch_early(kernel, dim3((unsigned)P.grid), dim3(NTHREADS), smem, st, P) != cudaSuccess) return GDNX_ELAUNCH;
+  if (P.whole) return GDNX_OK;
+  const int64_t G = P.a.H / P.a.cache.Hk;
+  return launch_early(paged_decode_join_kernel<NH>, dim3((unsigned)P.grid, (unsigned)(G < NH ? G : NH)),
+                      dim3(JOIN_WARPS * 32), 0, st, P) == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
 }
 
 template <int DB, bool BF16>
