@@ -229,3 +229,21 @@ def test_refusals():
     with pytest.raises(L.GdnxError) as e:
         ops.window_attention(wide, wide, wide)
     assert e.value.status == L.GDNX_EUNSUPPORTED
+
+
+def test_offsets_beyond_32_bits():
+    """Batch rows more than 2^31 elements apart, for the inputs and the output."""
+    far = (1 << 31) + 64
+    n = 40 * 2 * 64
+    bufs = [torch.empty(far + n, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    parts = [make(2, 40, 40, 2, 2, 64, "bf16", seed=20)[i] for i in range(3)]
+    q, out = (b.as_strided((2, 40, 2, 64), (far, 128, 64, 1)) for b in bufs)
+    q.copy_(parts[0])
+    ops.window_attention(q, parts[1], parts[2], window=9, sinks=1, out=out)
+    assert torch.equal(out, ops.window_attention(*parts, window=9, sinks=1))
+    f = [t.float() for t in parts]
+    del bufs, q, out
+    buf = torch.empty(far + n, dtype=torch.float32, device=DEV)
+    q = buf.as_strided((2, 40, 2, 64), (far, 128, 64, 1))
+    q.copy_(f[0])
+    assert torch.equal(ops.window_attention(q, f[1], f[2], window=9), ops.window_attention(*f, window=9))

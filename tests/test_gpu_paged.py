@@ -302,3 +302,28 @@ def test_refusals():
     assert e.value.status == L.GDNX_EUNSUPPORTED
     with pytest.raises(ValueError):
         ops.cache_compact(ops.PagedCache(c.kv.transpose(3, 4), c.table, c.lengths, c.refs, c.status))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_pool_beyond_32_bits(dtype):
+    """Pages that start more than 2^32 bytes (and 2^31 values) into the pool."""
+    pages = 70000 if dtype == "bf16" else 36000
+    c = ops.PagedCache.zeros(1, 8, 2, 64, 128, slots=2, width=4, dtype=TYPES[dtype], device=DEV)
+    kv = torch.empty(1, 2, pages, 2, 64, 128, dtype=TYPES[dtype], device=DEV)
+    c = ops.PagedCache(kv, c.table, c.lengths, torch.zeros(pages, dtype=torch.int32, device=DEV), c.status)
+    c.refs[: pages - 6] = 1  # held elsewhere: the new pages are the pool's last
+    T = 150
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(2, T, 2, 128, generator=g).to(TYPES[dtype]).to(DEV) for _ in range(2))
+    q = torch.randn(2, 4, 128, generator=g).to(TYPES[dtype]).to(DEV)
+    rows = i32(0, 1)
+    ops.cache_extend(c, rows, i32(T, T))
+    ops.cache_write(c, k, v, rows)
+    assert int(c.table.max()) == pages - 1
+    want = ops.window_attention(q[:, None], k, v)[:, 0]
+    y = ops.paged_decode(q, c)
+    assert rel(y, want) < 2 * TOL[dtype]  # two roundings apart at most
+    c.refs[: pages - 6] = 0
+    ops.cache_compact(c)
+    assert int(c.table.max()) == 5 and torch.equal(ops.paged_decode(q, c), y)
+    ops.cache_check(c)
