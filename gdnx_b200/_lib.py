@@ -123,7 +123,7 @@ class AttnArgs(C.Structure):
                 ("q", View), ("k", View), ("v", View), ("lengths", C.c_void_p),
                 ("y", C.c_void_p), ("y_dtype", C.c_int32),
                 ("y_sb", C.c_int64), ("y_st", C.c_int64), ("y_sh", C.c_int64),
-                ("lse", C.c_void_p), ("error", C.c_void_p)]
+                ("lse", C.c_void_p), ("y_rest", C.c_void_p), ("error", C.c_void_p)]
 
 
 class AttnBwdArgs(C.Structure):

@@ -644,11 +644,14 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const gdnx_attn_bwd_arg
     const uint16_t* dy = static_cast<const uint16_t*>(g.dy.ptr) + b * g.dy.sb + i * g.dy.st + h * g.dy.sh;
     for (int d = threadIdx.x % 8 * 8; d < a.D; d += 64) {
       const uint4 u = *reinterpret_cast<const uint4*>(y + d), v = *reinterpret_cast<const uint4*>(dy + d);
-      const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+      uint4 z = make_uint4(0, 0, 0, 0);
+      if (a.y_rest) z = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.y_rest) + ((b * a.Tq + i) * a.H + h) * a.D + d);
+      const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w}, zw[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s = fmaf(__uint_as_float(uw[e] << 16), __uint_as_float(vw[e] << 16), s);
-        s = fmaf(__uint_as_float(uw[e] & 0xffff0000u), __uint_as_float(vw[e] & 0xffff0000u), s);
+        s = fmaf(__uint_as_float(uw[e] << 16) + __uint_as_float(zw[e] << 16), __uint_as_float(vw[e] << 16), s);
+        s = fmaf(__uint_as_float(uw[e] & 0xffff0000u) + __uint_as_float(zw[e] & 0xffff0000u),
+                 __uint_as_float(vw[e] & 0xffff0000u), s);
       }
     }
   }
@@ -738,7 +741,8 @@ gdnx_status launch_attn_bwd_tc(const gdnx_attn_bwd_args& g, cudaStream_t st) {
   };
   if (a.q.dtype != GDNX_BF16 || a.y_dtype != GDNX_BF16 || !wide(a.y, a.y_sb, a.y_st, a.y_sh) ||
       !wide(g.dy.ptr, g.dy.sb, g.dy.st, g.dy.sh) || !wide(g.dq, 0, 0, 0) || !wide(g.dk, 0, 0, 0) ||
-      !wide(g.dv, 0, 0, 0) || !wide(g.workspace, 0, 0, 0))
+      !wide(g.dv, 0, 0, 0) || !wide(g.workspace, 0, 0, 0) ||
+      !wide(a.y_rest, 0, 0, 0))
     return GDNX_EUNSUPPORTED;
   BwdParams P;
   if (!make_tile_map(a.q, a.B, a.Tq, a.H, a.D, &P.q) || !make_tile_map(a.k, a.B, a.Tk, a.Hk, a.D, &P.k) ||

@@ -32,7 +32,7 @@ constexpr int NTHREADS = 384;  // a warpgroup for each stage's rows, and the war
 constexpr uint32_t T_S = 0, T_O = 256;  // tensor-memory columns: S_0, S_1, then O_0, O_1
 
 struct FwdParams {
-  TileMap q, k, v, y;
+  TileMap q, k, v, y, rest;
   gdnx_attn_args a;
   int64_t items;
   int tma_y;                   // 16-bit outputs leave through shared memory and TMA
@@ -126,6 +126,18 @@ GDNX_DEV void weights(const float* s, float c2, float mc, float2& sum, uint32_t*
   }
 }
 
+// 64 values less what `u` holds of them.
+GDNX_DEV void subtract_row(float* o, const uint32_t* u, int dtype) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) {
+    float2 x;
+    if (dtype == GDNX_BF16) x = make_float2(__uint_as_float(u[e] << 16), __uint_as_float(u[e] & 0xffff0000u));
+    else x = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+    o[2 * e] -= x.x;
+    o[2 * e + 1] -= x.y;
+  }
+}
+
 // A row's running state: the maximum that O and l are scaled to, and the sum.
 struct Row {
   float m, l;
@@ -165,7 +177,7 @@ GDNX_DEV void pack_row(uint32_t* u, const float* o, int dtype) {
 }
 
 // One stage's rows, one for each thread.
-template <int DB, bool BF16>
+template <int DB, bool BF16, bool REST>
 GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
   using Lo = Layout<DB>;
   const gdnx_attn_args& a = P.a;
@@ -245,7 +257,7 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
       tc::fence_after();
     }
     const float l = p < w.len ? row.l : 0.f;  // padding
-    const int i = i0 + r;
+    const int i = i0 + r, row0 = i0 + r / 32 * 32;
     const float inv = l > 0.f ? 1.f / l : l != l ? l : 0.f;
 #pragma unroll 1
     for (int d = 0; d < 64 * DB; d += 64) {
@@ -254,20 +266,24 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
 #pragma unroll
       for (int e = 0; e < 64; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
       if (P.tma_y) {
-        uint32_t u[32];
-        pack_row(u, o, a.y_dtype);
-        pack_row(u + 16, o + 32, a.y_dtype);
-        if (lane == 0) pipe::bulk_wait_read();  // the store before has read the staging rows
-        __syncwarp();
+        for (int rest = 0; rest < (REST ? 2 : 1); ++rest) {  // y, and what its rounding left
+          uint32_t u[32];
+          pack_row(u, o, a.y_dtype);
+          pack_row(u + 16, o + 32, a.y_dtype);
+          if (lane == 0) pipe::bulk_wait_read();  // the store before has read the staging rows
+          __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          *reinterpret_cast<uint4*>(out + tc::sw128(lane, e, 32)) =
-              make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
-        tc::fence_async_smem();
-        __syncwarp();
-        if (lane == 0 && i0 + r / 32 * 32 < a.Tq) {
-          tma_store_4d(&P.y.map, d, P.y.use_h ? head : 0, i0 + r / 32 * 32, P.y.use_b ? w.b : 0, tc::smem_u32(out));
-          pipe::bulk_commit();
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(out + tc::sw128(lane, e, 32)) =
+                make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
+          tc::fence_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < a.Tq) {
+            if (rest) tma_store_4d(&P.rest.map, d, P.rest.use_h ? head : 0, row0, P.rest.use_b ? w.b : 0, tc::smem_u32(out));
+            else tma_store_4d(&P.y.map, d, P.y.use_h ? head : 0, row0, P.y.use_b ? w.b : 0, tc::smem_u32(out));
+            pipe::bulk_commit();
+          }
+          if (REST) subtract_row(o, u, a.y_dtype);
         }
       } else if (i < a.Tq) {  // fp32
         float* dst = static_cast<float*>(a.y) + w.b * a.y_sb + (int64_t)i * a.y_st + head * a.y_sh + d;
@@ -382,7 +398,7 @@ GDNX_DEV void run_loads(const FwdParams& P, uint8_t* base, uint32_t smem, Bars& 
   }
 }
 
-template <int DB, bool BF16>
+template <int DB, bool BF16, bool REST>
 __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_constant__ FwdParams P) {
   using Lo = Layout<DB>;
   extern __shared__ __align__(1024) uint8_t base[];
@@ -415,7 +431,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
   if (smem % 1024) {  // never entered: the base is aligned
   } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 232 + 128 x 40 is just that
     regs_up<232>();
-    run_rows<DB, BF16>(P, base, tmem, bar, abort_flag);
+    run_rows<DB, BF16, REST>(P, base, tmem, bar, abort_flag);
     if (threadIdx.x % 32 == 0) pipe::bulk_wait_all();
   } else {
     regs_down<40>();
@@ -442,14 +458,19 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
   if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
 }
 
-template <int DB, bool BF16>
+template <int DB, bool BF16, bool REST>
 gdnx_status launch(const FwdParams& P, int sms, cudaStream_t st) {
-  const auto kernel = attn_fwd_tc_kernel<DB, BF16>;
+  const auto kernel = attn_fwd_tc_kernel<DB, BF16, REST>;
   static std::atomic<uint64_t> done;
   if (!allow_smem(kernel, (int)Layout<DB>::SMEM, done)) return GDNX_ELAUNCH;
   const unsigned grid = (unsigned)(P.items < sms ? P.items : sms);
   kernel<<<grid, NTHREADS, Layout<DB>::SMEM, st>>>(P);
   return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
+}
+
+template <int DB, bool BF16>
+gdnx_status launch(const FwdParams& P, int sms, cudaStream_t st) {
+  return P.a.y_rest ? launch<DB, BF16, true>(P, sms, st) : launch<DB, BF16, false>(P, sms, st);
 }
 
 }  // namespace
@@ -465,6 +486,10 @@ gdnx_status launch_attn_fwd_tc(const gdnx_attn_args& a, cudaStream_t st) {
   if (P.tma_y) {
     gdnx_view y = {a.y, a.y_dtype, (int32_t)a.D, a.y_sb, a.y_st, a.y_sh, 0, 0};
     if (!make_tile_map(y, a.B, a.Tq, a.H, a.D, &P.y, 32)) return GDNX_EUNSUPPORTED;
+    if (a.y_rest) {
+      y = {a.y_rest, a.y_dtype, (int32_t)a.D, a.Tq * a.H * a.D, a.H * a.D, a.D, 0, 0};
+      if (!make_tile_map(y, a.B, a.Tq, a.H, a.D, &P.rest, 32)) return GDNX_EUNSUPPORTED;
+    }
   }
   P.a = a;
   const int G = (int)(a.H / a.Hk), blocks = (int)((a.Tq + TM - 1) / TM);

@@ -139,6 +139,11 @@ GDNX_DEV float half_warp_sum(float x) {
   return x;
 }
 
+// x in a 16-bit type and back.
+GDNX_DEV float rounded(float x, int dtype) {
+  return dtype == GDNX_BF16 ? __bfloat162float(__float2bfloat16_rn(x)) : __half2float(__float2half_rn(x));
+}
+
 template <int DP, typename T>
 __global__ void __launch_bounds__(NT) attn_fwd_simt_kernel(const gdnx_attn_args a) {
   extern __shared__ float sm[];
@@ -211,7 +216,10 @@ __global__ void __launch_bounds__(NT) attn_fwd_simt_kernel(const gdnx_attn_args 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = g * 64 + tx * 4 + e;
-        if (d < D) st_from_f32(a.y, a.y_dtype, row + d, o[r][g * 4 + e] * inv);
+        if (d >= D) continue;
+        const float y = o[r][g * 4 + e] * inv;
+        st_from_f32(a.y, a.y_dtype, row + d, y);
+        if (a.y_rest) st_from_f32(a.y_rest, a.y_dtype, ((b * a.Tq + i) * a.H + h) * D + d, y - rounded(y, a.y_dtype));
       }
     if (a.lse && tx == 0)
       a.lse[(b * a.H + h) * a.Tq + i] = l[r] > 0.f ? (m[r] + log2f(l[r])) * kLn2 : -INFINITY;
@@ -228,8 +236,11 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const gdnx_attn_bwd_arg
   float s = 0.f;
   if (i + a.Tk - a.Tq < seq_len(a, b)) {
     const int64_t ry = b * a.y_sb + i * a.y_st + h * a.y_sh, rd = b * g.dy.sb + i * g.dy.st + h * g.dy.sh;
-    for (int d = lane; d < a.D; d += 32)
-      s = fmaf(ld_as_f32(a.y, a.y_dtype, ry + d), ld_as_f32(g.dy.ptr, g.dy.dtype, rd + d), s);
+    for (int d = lane; d < a.D; d += 32) {
+      float y = ld_as_f32(a.y, a.y_dtype, ry + d);
+      if (a.y_rest) y += ld_as_f32(a.y_rest, a.y_dtype, ((b * a.Tq + i) * a.H + h) * a.D + d);
+      s = fmaf(y, ld_as_f32(g.dy.ptr, g.dy.dtype, rd + d), s);
+    }
     s = warp_sum(s);
   }
   if (lane == 0) delta[(b * a.H + h) * a.Tq + i] = s;

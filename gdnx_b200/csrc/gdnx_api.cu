@@ -105,6 +105,7 @@ gdnx_status check_attn(const gdnx_attn_args& a) {
   if (a.y_sb < 0 || a.y_st < 0 || a.y_sh < 0) return GDNX_EINVAL;
   if (a.lengths && !is_device_ptr(a.lengths)) return GDNX_EINVAL;
   if (a.lse && a.Tq > 0 && !is_device_ptr(a.lse)) return GDNX_EINVAL;
+  if (a.y_rest && a.Tq > 0 && (!is_device_ptr(a.y_rest) || a.y_dtype == GDNX_F32)) return GDNX_EINVAL;
   if (a.error && !is_device_ptr(a.error)) return GDNX_EINVAL;
   return GDNX_OK;
 }

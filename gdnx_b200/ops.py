@@ -975,6 +975,12 @@ def window_attention(q, k, v, *, window: Optional[int] = None, sinks: int = 0, s
     sequences: keys from there on are not seen, and queries from there on give zeros, whatever the
     padding holds.  ``scale`` defaults to D ** -0.5.  Returns y [B,Tq,H,D] (and the log of the sum
     of exponentials [B,H,Tq] fp32 if asked, -inf where a row is padding)."""
+    y, lse, _ = _window_attention(q, k, v, window, sinks, scale, lengths, out, out_dtype, return_lse, False)
+    return (y, lse) if return_lse else y
+
+
+def _window_attention(q, k, v, window, sinks, scale, lengths, out, out_dtype, keep_lse, keep_rest):
+    """y, the log of the sum of exponentials and what y's rounding left (None where not kept)."""
     a, index = _attn_args(q, k, v, window, sinks, scale, lengths)
     if out is None:
         y = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
@@ -985,30 +991,35 @@ def window_attention(q, k, v, *, window: Optional[int] = None, sinks: int = 0, s
             raise ValueError("out must be [B,Tq,H,D] with a contiguous last dim")
     a.y, a.y_dtype = y.data_ptr(), _DT[y.dtype]
     a.y_sb, a.y_st, a.y_sh, _ = y.stride()
-    lse = None
-    if return_lse:
+    lse = rest = None
+    if keep_lse:
         lse = torch.empty(a.B, a.H, a.Tq, dtype=torch.float32, device=q.device)
         a.lse = lse.data_ptr()
+    if keep_rest and y.dtype is not torch.float32:
+        rest = torch.empty(q.shape, dtype=y.dtype, device=q.device)
+        a.y_rest = rest.data_ptr()
     _enqueue("gdnx_attn_fwd", index, C.byref(a))
-    return (y, lse) if return_lse else y
+    return y, lse, rest
 
 
 class _WindowAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, scale, lengths):
-        y, lse = window_attention(q, k, v, window=window, sinks=sinks, scale=scale, lengths=lengths, return_lse=True)
-        ctx.save_for_backward(q, k, v, y, lse, lengths)
+        y, lse, rest = _window_attention(q, k, v, window, sinks, scale, lengths, None, None, True, True)
+        ctx.save_for_backward(q, k, v, y, lse, rest, lengths)
         ctx.mask = (window, sinks, scale)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        q, k, v, y, lse, lengths = ctx.saved_tensors
+        if torch.is_grad_enabled():  # create_graph=True
+            raise RuntimeError("window_attention_train is differentiable once")
+        q, k, v, y, lse, rest, lengths = ctx.saved_tensors
         a, index = _attn_args(q, k, v, *ctx.mask, lengths)
         a.y, a.y_dtype = y.data_ptr(), _DT[y.dtype]
         a.y_sb, a.y_st, a.y_sh, _ = y.stride()
         a.lse = lse.data_ptr()
+        a.y_rest = None if rest is None else rest.data_ptr()
         if dy.shape[-1] > 1 and dy.stride(-1) != 1:
             dy = dy.contiguous()
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))

@@ -418,12 +418,15 @@ typedef struct {
   int32_t y_dtype;
   int64_t y_sb, y_st, y_sh;
   float* lse;                  /* [B,H,Tq] log of the sum of exponentials; NULL = not kept */
+  void* y_rest;                /* [B,Tq,H,D] contiguous, y's (16-bit) type: what y's rounding
+                                  left, for the backward; NULL = not kept                  */
   int32_t* error;              /* device word that takes GDNX_ETIMEOUT; NULL = none        */
 } gdnx_attn_args;
 
 GDNX_API gdnx_status gdnx_attn_fwd(const gdnx_attn_args* args, void* stream);
 
-/* Its gradients.  `fwd` holds the forward's arguments, its output y and its lse.
+/* Its gradients.  `fwd` holds the forward's arguments, its output y and its lse, and where it
+ * kept it y_rest: sum_d dy y then is as exact as y was before it was rounded.
  * dq [B,Tq,H,D], dk, dv [B,Tk,Hk,D] are contiguous, in the inputs' type; gradients of
  * shared key heads are summed over their query heads.  No atomics: the same inputs give
  * the same bits. */

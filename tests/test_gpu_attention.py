@@ -172,6 +172,14 @@ def test_same_inputs_give_the_same_bits():
             assert torch.equal(a, b)
 
 
+def test_gradient_of_a_gradient_is_refused():
+    q, k, v, dy = make(1, 20, 20, 2, 2, 64, "f32")
+    q.requires_grad_()
+    y = ops.window_attention_train(q, k, v)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(y, q, dy, create_graph=True)
+
+
 def test_out_dtype_and_out():
     q, k, v, _ = make(2, 150, 150, 4, 2, 128, "bf16", seed=14)
     yo, _ = A.window_attention(q, k, v, window=60)
