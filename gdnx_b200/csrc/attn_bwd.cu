@@ -636,12 +636,13 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const gdnx_attn_bwd_arg
   const gdnx_attn_args& a = g.fwd;
   const int64_t n = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
   if (n >= a.B * a.H * qpad) return;  // whole groups of eight
-  const int64_t i = n % qpad, h = n / qpad % a.H, b = n / qpad / a.H;
+  const int64_t h = n % a.H, i = n / a.H % qpad, b = n / a.H / qpad;  // heads side by side, as they lie in memory
   const bool on = i < a.Tq && i + a.Tk - a.Tq < seq_len(a, b);
   float s = 0.f;
   if (on) {
     const uint16_t* y = static_cast<const uint16_t*>(a.y) + b * a.y_sb + i * a.y_st + h * a.y_sh;
     const uint16_t* dy = static_cast<const uint16_t*>(g.dy.ptr) + b * g.dy.sb + i * g.dy.st + h * g.dy.sh;
+#pragma unroll 2
     for (int d = threadIdx.x % 8 * 8; d < a.D; d += 64) {
       const uint4 u = *reinterpret_cast<const uint4*>(y + d), v = *reinterpret_cast<const uint4*>(dy + d);
       uint4 z = make_uint4(0, 0, 0, 0);
@@ -659,8 +660,9 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const gdnx_attn_bwd_arg
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(mask, s, o);
   if (threadIdx.x % 8 == 0) {
-    lse2[n] = on ? -a.lse[(b * a.H + h) * a.Tq + i] * kLog2e : -INFINITY;
-    delta[n] = -s;
+    const int64_t at = (b * a.H + h) * qpad + i;
+    lse2[at] = on ? -a.lse[(b * a.H + h) * a.Tq + i] * kLog2e : -INFINITY;
+    delta[at] = -s;
   }
 }
 
