@@ -983,7 +983,7 @@ def _window_attention(q, k, v, window, sinks, scale, lengths, out, out_dtype, ke
     """y, the log of the sum of exponentials and what y's rounding left (None where not kept)."""
     a, index = _attn_args(q, k, v, window, sinks, scale, lengths)
     if out is None:
-        y = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+        y = q.new_empty(q.shape) if out_dtype is None else q.new_empty(q.shape, dtype=out_dtype)
     else:
         y = out
         _on_device(index, y)
@@ -993,10 +993,10 @@ def _window_attention(q, k, v, window, sinks, scale, lengths, out, out_dtype, ke
     a.y_sb, a.y_st, a.y_sh, _ = y.stride()
     lse = rest = None
     if keep_lse:
-        lse = torch.empty(a.B, a.H, a.Tq, dtype=torch.float32, device=q.device)
+        lse = q.new_empty((a.B, a.H, a.Tq), dtype=torch.float32)
         a.lse = lse.data_ptr()
     if keep_rest and y.dtype is not torch.float32:
-        rest = torch.empty(q.shape, dtype=y.dtype, device=q.device)
+        rest = y.new_empty(q.shape)
         a.y_rest = rest.data_ptr()
     _enqueue("gdnx_attn_fwd", index, C.byref(a))
     return y, lse, rest
@@ -1022,10 +1022,10 @@ class _WindowAttentionFn(torch.autograd.Function):
         a.y_rest = None if rest is None else rest.data_ptr()
         if dy.shape[-1] > 1 and dy.stride(-1) != 1:
             dy = dy.contiguous()
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         g = L.AttnBwdArgs(a, _heads_view(dy), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
         need = L.load().gdnx_attn_bwd_workspace_bytes(C.byref(g))
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(max(need, 16), dtype=torch.uint8)
         g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel()
         _enqueue("gdnx_attn_bwd", index, C.byref(g))
         return dq, dk, dv, None, None, None, None
@@ -1114,7 +1114,7 @@ def cache_extend(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor) ->
     at, n = _cache_rows(rows, s, index)
     more = _index32(counts, n, "counts", index)
     need = L.load().gdnx_cache_workspace_bytes(C.byref(s), n)
-    ws = torch.empty(need, dtype=torch.uint8, device=cache.kv.device)
+    ws = rows.new_empty(need, dtype=torch.uint8)
     _enqueue("gdnx_cache_extend", index, C.byref(s), n, at, more, ws.data_ptr(), need)
 
 
@@ -1161,7 +1161,7 @@ def cache_compact(cache: PagedCache) -> None:
     above the live count into the free ones below it."""
     s, index = _cache_struct(cache)
     need = L.load().gdnx_cache_workspace_bytes(C.byref(s), 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=cache.kv.device)
+    ws = cache.table.new_empty(need, dtype=torch.uint8)
     _enqueue("gdnx_cache_compact", index, C.byref(s), ws.data_ptr(), need)
 
 
@@ -1190,7 +1190,7 @@ def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Op
     if not 0 <= layer < s.L:
         raise ValueError("no such layer")
     if out is None:
-        y = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+        y = q.new_empty(q.shape) if out_dtype is None else q.new_empty(q.shape, dtype=out_dtype)
     else:
         y = out
         _on_device(index, y)
@@ -1209,7 +1209,7 @@ def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Op
     need = L.load().gdnx_paged_decode_workspace_bytes(C.byref(a))
     ws = None
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(need, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     _enqueue("gdnx_paged_decode", index, C.byref(a))
     return y
