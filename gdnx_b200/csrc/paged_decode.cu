@@ -1,233 +1,289 @@
-// Attention of one new token per sequence over a paged key/value cache of 32-bit values, on
-// the CUDA cores (all arithmetic fp32).
+// Attention of one new token per sequence over a paged cache of 32-bit values, on the CUDA cores
+// (all arithmetic fp32; the work of a call is cut as in paged_decode.cuh).
 //
-//   y = sum_j softmax_j(scale q.k_j) v_j   over the visible tokens j of the slot.
-// The visible tokens are walked in tiles of 64 positions, split evenly over the CTAs of one
-// (sequence, key head, group of query heads); each CTA leaves its running maximum, sum and
-// unnormalised output, and a second kernel joins the parts in order:
-//   m = max_s m_s;  y = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
-// The bytes of K and V bound it.  A warp reads one token's row with D / 8 lanes, eight values
-// a lane, and holds the G query heads of the key head in registers, so each byte of K and V
-// is read once for up to GB = 4 heads.
-#include "attn_common.cuh"
-#include "kernels.h"
+// The bytes of K and V bound it, so the loads run by themselves: one warp copies the keys and
+// values of 32 tokens at a time into a ring of six stages (a head's tokens of one page are one
+// contiguous run: bulk asynchronous copies), 160 KB ahead of the eight warps that use them.
+// Each of these takes four of a stage's tokens, 32 / LPK at a time; LPK lanes share a token, eight
+// values of its row each, and hold the unit's NH query heads and outputs for them:
+//   s = c q.k (a sum over LPK lanes);  p = 2^(s - m);  l += p;  o += p v
+// with the maximum m moved only where a score lies more than 8 above it (a vote of the warp).
+// The groups' (m, l, o) are joined when the unit ends.
+#include "paged_decode.cuh"
 
 namespace gdnx {
 namespace {
 
-using namespace attn;
+constexpr int WARPS = 8;                     // that use the loads
+constexpr int NTHREADS = WARPS * 32 + 32;
+constexpr int SUB = 32;                      // tokens of a stage
+constexpr int STAGES = 6;
+constexpr uint32_t SIDE = SUB * 128 * 4;     // bytes of a stage's keys or values, at most
+constexpr float kLazy = 8.f;
 
-constexpr int TILE = 64;      // tokens of one step of a CTA
-constexpr int NT = 128;
-constexpr int WARPS = NT / 32;
-constexpr int GB = 4;         // query heads of one CTA
-constexpr int MAX_SPLITS = 128;
-
-// Eight consecutive values.
-GDNX_DEV void load8(float (&x)[8], const float* p) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-
-struct Dec {
-  gdnx_paged_decode_args a;
-  int splits, groups;  // parts of a sequence; CTAs of GB query heads for one key head
-  float* part;         // [B, H, splits, D] unnormalised outputs
-  float* stat;         // [B, H, splits, 2] maximum (log2 domain) and sum
+template <int NH>
+struct Small {
+  float o[WARPS][NH][128], m[WARPS][NH], l[WARPS][NH];
+  uint64_t full[STAGES], empty[STAGES];
+  Range range;
+  long long sums[NTHREADS / 32];
+  int ok[STAGES];  // which halves of a stage's tokens lie on pages
+  int abort_flag;
 };
 
-GDNX_DEV int dec_length(const Dec& P, int64_t b, int& row) {
-  const gdnx_cache& c = P.a.cache;
-  row = P.a.rows ? P.a.rows[b] : (int)b;
-  if (row < 0 || row >= c.slots) return 0;
-  const int64_t n = c.lengths[row], most = c.width * c.page;
-  return (int)(n < 0 ? 0 : (n > most ? most : n));
+// Does the sequence's newest token see any of tokens j..j+31?
+GDNX_DEV bool sub_seen(int j, int len, int64_t window, int64_t sinks) {
+  return j < len && (j + SUB > (int64_t)len - window || j < sinks);
 }
 
-template <int LPK>  // lanes per key: 8 (D <= 64) or 16 (D <= 128)
-__global__ void __launch_bounds__(NT) paged_decode_kernel(const Dec P) {
-  constexpr int KPW = 32 / LPK;              // tokens of one pass of a warp
-  constexpr int PASSES = TILE / WARPS / KPW;  // passes of a warp over its part of a tile
-  __shared__ float red_o[WARPS * KPW][GB][LPK * 8];
-  __shared__ float red_m[WARPS * KPW][GB], red_l[WARPS * KPW][GB];
-  const gdnx_paged_decode_args& a = P.a;
-  const gdnx_cache& c = a.cache;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, sub = lane / LPK, dl = lane % LPK;
-  const int split = blockIdx.x, D = (int)c.D, G = (int)(a.H / c.Hk);
-  const int64_t b = blockIdx.z, hk = blockIdx.y / P.groups;
-  const int g0 = (int)(blockIdx.y % P.groups) * GB, ng = min(GB, G - g0);
-  int row;
-  const int len = dec_length(P, b, row);
-  const int window = (int)a.window, sinks = (int)a.sinks, page = c.page;
-  const KeyTiles kt(len - 1, len - 1, len, window, sinks, TILE);
-  const int per = (kt.count + P.splits - 1) / P.splits, t0 = split * per, t1 = min(kt.count, t0 + per);
-  const bool mine = dl * 8 < D;  // lanes beyond a narrow head hold zeros
-  const float c2 = a.scale * kLog2e;
-  float q[GB][8], o[GB][8], m[GB], l[GB];
-#pragma unroll
-  for (int g = 0; g < GB; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      o[g][e] = 0.f;
-      q[g][e] = (g < ng && mine)
-                    ? ld_as_f32(a.q.ptr, a.q.dtype, b * a.q.sb + (hk * G + g0 + g) * a.q.sh + dl * 8 + e) * c2
-                    : 0.f;
-    }
-  }
+template <int NH>
+GDNX_DEV void load_stages(const DecParams& P, Walk w, uint8_t* ring, Small<NH>& sm) {
+  const gdnx_cache& c = P.a.cache;
+  const int lane = threadIdx.x % 32, page = c.page, npp = TM / page, ahead = 32 / npp, D = (int)c.D;
+  const int runs = page < SUB ? SUB / page : 1, tokens = SUB / runs;  // contiguous runs of a stage
   const float* kv = static_cast<const float*>(c.kv);
-  const int64_t side = c.pages * c.Hk * page * D;  // one layer's keys or values
-  const float* kbase = kv + a.layer * 2 * side + hk * page * D + dl * 8;
-  const int32_t* table = c.table + (int64_t)row * c.width;
-  for (int t = t0; t < t1; ++t) {
-    const int j0 = kt.tile(t) * TILE + warp * (TILE / WARPS) + sub;
-    float s[PASSES][GB];
-    int64_t at[PASSES];
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int j = j0 + i * KPW;
-      at[i] = -1;
-      if (j < len && (len - 1 - j < window || j < sinks)) {
-        const int p = table[j / page];
-        if (p >= 0 && p < c.pages) at[i] = ((int64_t)p * c.Hk * page + j % page) * D;
+  uint32_t n = 0;
+  while (w.next()) {
+    const int hk = w.unit / P.groups;
+    int ids = -1;
+    for (int t = w.ta; t < w.tb; ++t) {
+      const int k = (t - w.ta) % ahead;
+      if (k == 0) {
+        const int mine = t + lane / npp;
+        ids = mine < w.tb ? page_id(P, w.seq, w.seq.kt.tile(mine), lane % npp) : -1;
       }
-    }
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      float x[8] = {};
-      if (at[i] >= 0 && mine) load8(x, kbase + at[i]);
-#pragma unroll
-      for (int g = 0; g < GB; ++g) {
-        float d = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d = fmaf(q[g][e], x[e], d);
-#pragma unroll
-        for (int sh = LPK / 2; sh > 0; sh >>= 1) d += __shfl_xor_sync(0xffffffffu, d, sh);
-        s[i][g] = at[i] >= 0 ? d : -INFINITY;
+      for (int s = 0; s < TM / SUB; ++s) {
+        const int j = w.seq.kt.tile(t) * TM + s * SUB;
+        if (!sub_seen(j, w.seq.len, P.a.window, P.a.sinks)) continue;
+        const uint32_t st = n % STAGES;
+        if (!warp_wait(&sm.empty[st], (n / STAGES & 1) ^ 1, &sm.abort_flag)) return;
+        ++n;
+        // lane: side and run
+        const int run = lane / 2 % 2, side = lane % 2;
+        const int id = __shfl_sync(0xffffffffu, ids, (k * npp + (s * SUB + run * tokens) / page) & 31);
+        const bool go = lane < 4 && run < runs && id >= 0;
+        const uint32_t got = __ballot_sync(0xffffffffu, go);
+        const uint32_t bar = tc::smem_u32(&sm.full[st]), bytes = (uint32_t)(tokens * D * 4);
+        if (lane == 0) {
+          sm.ok[st] = runs == 1 ? (got & 1 ? 3 : 0) : (int)((got & 1) | (got >> 1 & 2));
+          pipe::expect_tx(bar, __popc(got) * bytes);
+        }
+        __syncwarp();
+        if (go) {
+          const int64_t row = ((((P.a.layer * 2 + side) * c.pages + id) * c.Hk + hk) * page + (j + run * tokens) % page);
+          pipe::bulk_load(tc::smem_u32(ring) + st * 2 * SIDE + side * SIDE + run * tokens * D * 4, kv + row * D, bytes, bar);
+        }
       }
-    }
-#pragma unroll
-    for (int g = 0; g < GB; ++g) {
-      float mx = m[g];
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) mx = fmaxf(mx, s[i][g]);
-      const float base = mx == -INFINITY ? 0.f : mx, corr = exp2f(m[g] - base);
-      m[g] = mx;
-      l[g] *= corr;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[g][e] *= corr;
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        s[i][g] = exp2f(s[i][g] - base);
-        l[g] += s[i][g];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      float x[8] = {};
-      if (at[i] >= 0 && mine) load8(x, kbase + side + at[i]);
-#pragma unroll
-      for (int g = 0; g < GB; ++g)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[g][e] = fmaf(s[i][g], x[e], o[g][e]);
     }
   }
-  // join the CTA's WARPS * KPW partial results
-  const int part = warp * KPW + sub;
+}
+
+template <int LPK, int NH>
+GDNX_DEV void use_stages(const DecParams& P, Walk w, int64_t per, const uint8_t* ring, Small<NH>& sm) {
+  constexpr int KPW = 32 / LPK, PASSES = SUB / WARPS / KPW;
+  const gdnx_paged_decode_args& a = P.a;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, sub = lane / LPK, dl = lane % LPK, D = (int)a.cache.D;
+  const int d0 = 4 * dl, d1 = 4 * (LPK + dl);  // this lane's two runs of four values
+  const int window = (int)a.window, sinks = (int)a.sinks;
+  const float c2 = a.scale * kLog2e;
+  uint32_t n = 0;
+  bool ok = true;  // a wait that gave up is told at the next vote, where all warps leave
+  if (threadIdx.x == 0 && !P.whole) P.joint[blockIdx.x] = {0, 0, 0, -1};
+  while (w.next()) {
+    const Heads hd(P, w.unit, NH);
+    float q[NH][8], o[NH][8], m[NH], l[NH];
 #pragma unroll
-  for (int g = 0; g < GB; ++g) {
+    for (int h = 0; h < NH; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+      const float* row = static_cast<const float*>(a.q.ptr) + w.b * a.q.sb + (hd.h0 + h) * a.q.sh;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) red_o[part][g][dl * 8 + e] = o[g][e];
-    if (dl == 0) {
-      red_m[part][g] = m[g];
-      red_l[part][g] = l[g];
+      for (int e = 0; e < 8; ++e) {
+        const int d = (e < 4 ? d0 : d1 - 4) + e;
+        o[h][e] = 0.f;
+        q[h][e] = h < hd.n && d < D ? row[d] * c2 : 0.f;
+      }
     }
+    for (int t = w.ta; t < w.tb; ++t) {
+      for (int s = 0; s < TM / SUB; ++s) {
+        const int j0 = w.seq.kt.tile(t) * TM + s * SUB;
+        if (!sub_seen(j0, w.seq.len, a.window, a.sinks)) continue;
+        const uint32_t st = n % STAGES;
+        ok = ok && warp_wait(&sm.full[st], n / STAGES & 1, &sm.abort_flag);
+        ++n;
+        if (!ok) continue;
+        const int on_page = *const_cast<volatile int*>(&sm.ok[st]);
+        const float* kt = reinterpret_cast<const float*>(ring + st * 2 * SIDE);
+        const float* vt = reinterpret_cast<const float*>(ring + st * 2 * SIDE + SIDE);
+        float x[PASSES][NH];
+        bool seen[PASSES], over = false;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+          const int r = warp * (SUB / WARPS) + i * KPW + sub, j = j0 + r;
+          seen[i] = key_seen(j, w.seq.len, window, sinks) && (on_page >> (r / 16) & 1);
+          float4 k0 = make_float4(0.f, 0.f, 0.f, 0.f), k1 = k0;
+          if (seen[i] && d0 < D) k0 = *reinterpret_cast<const float4*>(kt + r * D + d0);
+          if (seen[i] && d1 < D) k1 = *reinterpret_cast<const float4*>(kt + r * D + d1);
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            float d = q[h][0] * k0.x;
+            d = fmaf(q[h][1], k0.y, d);
+            d = fmaf(q[h][2], k0.z, d);
+            d = fmaf(q[h][3], k0.w, d);
+            d = fmaf(q[h][4], k1.x, d);
+            d = fmaf(q[h][5], k1.y, d);
+            d = fmaf(q[h][6], k1.z, d);
+            d = fmaf(q[h][7], k1.w, d);
+#pragma unroll
+            for (int z = LPK / 2; z > 0; z >>= 1) d += __shfl_xor_sync(0xffffffffu, d, z);
+            x[i][h] = seen[i] ? d : -INFINITY;
+            over |= x[i][h] > m[h] + kLazy;
+          }
+        }
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            float top = m[h];
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) top = fmaxf(top, x[i][h]);
+            const float corr = top == -INFINITY ? 1.f : exp2f(m[h] - top);
+            m[h] = top;
+            l[h] *= corr;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[h][e] *= corr;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+          const int r = warp * (SUB / WARPS) + i * KPW + sub;
+          float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
+          if (seen[i] && d0 < D) v0 = *reinterpret_cast<const float4*>(vt + r * D + d0);
+          if (seen[i] && d1 < D) v1 = *reinterpret_cast<const float4*>(vt + r * D + d1);
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            const float p = x[i][h] == -INFINITY ? 0.f : exp2f(x[i][h] - m[h]);
+            l[h] += p;
+            o[h][0] = fmaf(p, v0.x, o[h][0]);
+            o[h][1] = fmaf(p, v0.y, o[h][1]);
+            o[h][2] = fmaf(p, v0.z, o[h][2]);
+            o[h][3] = fmaf(p, v0.w, o[h][3]);
+            o[h][4] = fmaf(p, v1.x, o[h][4]);
+            o[h][5] = fmaf(p, v1.y, o[h][5]);
+            o[h][6] = fmaf(p, v1.z, o[h][6]);
+            o[h][7] = fmaf(p, v1.w, o[h][7]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) pipe::mbar_arrive(&sm.empty[st]);
+      }
+    }
+    // the groups of a warp, then the warps in order
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      float top = m[h];
+#pragma unroll
+      for (int z = LPK; z < 32; z <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, z));
+      const float corr = top == -INFINITY ? 0.f : exp2f(m[h] - top);
+      l[h] *= corr;
+#pragma unroll
+      for (int z = LPK; z < 32; z <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], z);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        o[h][e] *= corr;
+#pragma unroll
+        for (int z = LPK; z < 32; z <<= 1) o[h][e] += __shfl_xor_sync(0xffffffffu, o[h][e], z);
+      }
+      if (sub == 0) {
+        *reinterpret_cast<float4*>(&sm.o[warp][h][d0]) = make_float4(o[h][0], o[h][1], o[h][2], o[h][3]);
+        *reinterpret_cast<float4*>(&sm.o[warp][h][d1]) = make_float4(o[h][4], o[h][5], o[h][6], o[h][7]);
+        if (dl == 0) {
+          sm.m[warp][h] = top;
+          sm.l[warp][h] = l[h];
+        }
+      }
+    }
+    if (pipe::group_any(1, WARPS * 32, !ok)) return;
+    const bool whole = w.whole();
+    // a part that goes on in the next CTA is this CTA's last, any other its first
+    const int64_t at = ((int64_t)blockIdx.x * 2 + (w.tb < w.seq.kt.count && w.ta == 0 ? 1 : 0)) * NH;
+    for (int i = threadIdx.x; i < hd.n * D; i += WARPS * 32) {
+      const int h = i / D, d = i % D;
+      float top = -INFINITY, sum = 0.f, y = 0.f;
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) top = fmaxf(top, sm.m[k][h]);
+      const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) {
+        const float z = exp2f(sm.m[k][h] - ref);
+        sum = fmaf(z, sm.l[k][h], sum);
+        y = fmaf(z, sm.o[k][h][d], y);
+      }
+      if (whole) {
+        st_from_f32(a.y, a.y_dtype, w.b * a.y_sb + (hd.h0 + h) * a.y_sh + d, sum == 0.f ? 0.f : y / sum);
+      } else {
+        P.part[(at + h) * 128 + d] = y;
+        if (d == 0) {
+          P.stat[(at + h) * 2] = top;
+          P.stat[(at + h) * 2 + 1] = sum;
+        }
+      }
+    }
+    if (threadIdx.x == 0 && w.ta > 0 && w.tb == w.seq.kt.count)  // the unit's last part
+      P.joint[blockIdx.x] = {(int)w.b, w.unit, (int)((w.before + (int64_t)w.unit * w.seq.kt.count) / per), (int)blockIdx.x};
+    if (pipe::group_any(1, WARPS * 32, !ok)) return;  // what was joined may be written again
+  }
+}
+
+template <int LPK, int NH>
+__global__ void __launch_bounds__(NTHREADS, 1) paged_decode_kernel(const DecParams P) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  Small<NH>& sm = *reinterpret_cast<Small<NH>*>(ring + STAGES * 2 * SIDE);
+  const int warp = threadIdx.x / 32, units = (int)P.a.cache.Hk * P.groups;
+  dependents_may_start();
+  if (threadIdx.x == 0) {
+    sm.abort_flag = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      tc::mbar_init(&sm.full[i], 1);
+      tc::mbar_init(&sm.empty[i], WARPS);
+    }
+  }
+  wait_for_earlier();
+  find_range<NTHREADS>(P, units, sm.range, sm.sums);  // synchronises
+  const Walk w(P, units, sm.range);
+  if (warp < WARPS) {
+    use_stages<LPK, NH>(P, w, sm.range.per, ring, sm);
+  } else {
+    load_stages<NH>(P, w, ring, sm);
+    write_zeros(P);
+    if (*const_cast<volatile int*>(&sm.abort_flag))  // let the copies in flight land
+      for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < ng * D; x += NT) {
-    const int g = x / D, d = x % D;
-    float mx = -INFINITY, sum = 0.f, y = 0.f;
-#pragma unroll
-    for (int k = 0; k < WARPS * KPW; ++k) mx = fmaxf(mx, red_m[k][g]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-    for (int k = 0; k < WARPS * KPW; ++k) {
-      const float w = exp2f(red_m[k][g] - base);
-      sum = fmaf(w, red_l[k][g], sum);
-      y = fmaf(w, red_o[k][g][d], y);
-    }
-    const int64_t h = hk * G + g0 + g;
-    if (P.splits == 1) {
-      st_from_f32(a.y, a.y_dtype, b * a.y_sb + h * a.y_sh + d, sum > 0.f ? y / sum : 0.f);
-    } else {
-      const int64_t at = (b * a.H + h) * P.splits + split;
-      P.part[at * D + d] = y;
-      if (d == 0) {
-        P.stat[2 * at] = mx;
-        P.stat[2 * at + 1] = sum;
-      }
-    }
-  }
+  if (threadIdx.x == 0 && sm.abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
 }
 
-// One CTA for each (sequence, query head).
-__global__ void __launch_bounds__(128) paged_decode_join_kernel(const Dec P) {
-  const gdnx_paged_decode_args& a = P.a;
-  const int64_t h = blockIdx.x % a.H, b = blockIdx.x / a.H, at = (b * a.H + h) * P.splits;
-  const int D = (int)a.cache.D;
-  float mx = -INFINITY, sum = 0.f, y = 0.f;
-  for (int s = 0; s < P.splits; ++s) mx = fmaxf(mx, P.stat[2 * (at + s)]);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  const int d = threadIdx.x;
-  for (int s = 0; s < P.splits; ++s) {
-    const float w = exp2f(P.stat[2 * (at + s)] - base);
-    sum = fmaf(w, P.stat[2 * (at + s) + 1], sum);
-    if (d < D) y = fmaf(w, P.part[(at + s) * D + d], y);
-  }
-  if (d < D) st_from_f32(a.y, a.y_dtype, b * a.y_sb + h * a.y_sh + d, sum > 0.f ? y / sum : 0.f);
+template <int LPK, int NH>
+gdnx_status launch(const DecParams& P, cudaStream_t st) {
+  constexpr int smem = (int)(STAGES * 2 * SIDE + sizeof(Small<NH>));
+  const auto kernel = paged_decode_kernel<LPK, NH>;
+  static std::atomic<uint64_t> done;
+  if (!allow_smem(kernel, smem, done)) return GDNX_ELAUNCH;
+  if (launch_early(kernel, dim3((unsigned)P.grid), dim3(NTHREADS), smem, st, P) != cudaSuccess) return GDNX_ELAUNCH;
+  return join_parts<NH>(P, st);
 }
 
-// Parts of a sequence: about four CTAs for each SM, and at least two tiles for each part.
-int split_count(const gdnx_paged_decode_args& a, int groups) {
-  const gdnx_cache& c = a.cache;
-  int64_t most = c.width * c.page;
-  if (a.max_len > 0 && a.max_len < most) most = a.max_len;
-  int64_t tiles = (most + TILE - 1) / TILE;
-  const int64_t seen = (a.window + TILE - 1) / TILE + 1 + (a.sinks + TILE - 1) / TILE;
-  if (seen < tiles) tiles = seen;
-  const int64_t ctas = a.B * c.Hk * groups;
-  int64_t s = (148 * 4 + ctas - 1) / ctas;
-  if (s > (tiles + 1) / 2) s = (tiles + 1) / 2;
-  return (int)(s < 1 ? 1 : s > MAX_SPLITS ? MAX_SPLITS : s);
-}
-
-int group_count(const gdnx_paged_decode_args& a) { return (int)((a.H / a.cache.Hk + GB - 1) / GB); }
+// Query heads of a unit.
+int heads_of(const gdnx_paged_decode_args& a) { return a.H / a.cache.Hk > 4 ? 8 : 4; }
 
 }  // namespace
 
-size_t paged_decode_workspace_bytes(const gdnx_paged_decode_args& a) {
-  const int s = split_count(a, group_count(a));
-  return s == 1 ? 0 : (size_t)(a.B * a.H * s * (a.cache.D + 2)) * sizeof(float);
-}
+size_t paged_decode_workspace_bytes(const gdnx_paged_decode_args& a) { return plan_bytes(make_plan(a, heads_of(a))); }
 
 gdnx_status launch_paged_decode(const gdnx_paged_decode_args& a, cudaStream_t st) {
-  Dec P;
-  P.a = a;
-  P.groups = group_count(a);
-  P.splits = split_count(a, P.groups);
-  P.part = static_cast<float*>(a.workspace);
-  P.stat = P.part + a.B * a.H * P.splits * a.cache.D;
-  const dim3 grid((unsigned)P.splits, (unsigned)(a.cache.Hk * P.groups), (unsigned)a.B);
-  if (a.cache.D > 64) paged_decode_kernel<16><<<grid, NT, 0, st>>>(P);
-  else paged_decode_kernel<8><<<grid, NT, 0, st>>>(P);
-  if (cudaGetLastError() != cudaSuccess) return GDNX_ELAUNCH;
-  if (P.splits > 1) {
-    paged_decode_join_kernel<<<(unsigned)(a.B * a.H), 128, 0, st>>>(P);
-    if (cudaGetLastError() != cudaSuccess) return GDNX_ELAUNCH;
-  }
-  return GDNX_OK;
+  DecParams P;
+  fill(P, a, make_plan(a, heads_of(a)));
+  if (a.cache.D > 64) return heads_of(a) == 4 ? launch<16, 4>(P, st) : launch<16, 8>(P, st);
+  return heads_of(a) == 4 ? launch<8, 4>(P, st) : launch<8, 8>(P, st);
 }
 
 }  // namespace gdnx

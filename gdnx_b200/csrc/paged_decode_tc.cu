@@ -1,60 +1,29 @@
 // Attention of one new token per sequence over a paged cache, on the tensor cores (16-bit
 // caches).  The bytes of K and V bound it; the products only have to keep out of their way.
 //
-// Work.  A unit is one sequence and key head (and group of up to NH of its query heads); its
-// visible tokens are walked in tiles of 128 positions.  All units' tiles in a row are cut
-// evenly over the CTAs (one on each SM), so that mixed lengths leave none waiting: a CTA takes
-// the end of one unit, whole units, the beginning of another.  Whole units are written at
-// once; parts leave maximum, sum and unnormalised output, and a second kernel joins them in
-// order.  Every CTA finds its range from the lengths by itself.  Where no unit can have more
-// than four tiles, a CTA takes whole units and there is nothing to join.
-//
 // A tile.  With the keys as rows the products are narrow and nothing is padded to 128 but the
 // heads to NH:  S^T [128 keys x NH] = K Q^T,  O^T [128 dims x NH] += V^T P  (V read with its
-// rows as K; of head sizes up to 64 lanes 64.. read shifted rows and are not used).  Thread j owns key j: p_h = 2^(c s_jh - m_h), written 16-bit to shared memory as the
-// right factor.  The maxima m are those of the first tile and move only when some score lies
+// rows as K; of head sizes up to 64 lanes 64.. read shifted rows and are not used).  Thread j owns
+// key j: p_h = 2^(c s_jh - m_h), written 16-bit to shared memory as the right factor.  The maxima m are those of the first tile and move only when some score lies
 // more than 8 above (p stays below 2^8), so a tile costs one vote and no reduction; sums stay
 // in the threads until the unit ends.
 //
 // Pages come by TMA, one box for each page and 64 dims; pages that hold nothing visible are not
 // fetched.  Rows that are not visible are masked in S and zeroed in V, since what unwritten
 // and released pages hold may be NaN.
-#include "attn_tc.cuh"
-#include "kernels.h"
-#include "launch.cuh"
+#include "paged_decode.cuh"
 
 namespace gdnx {
 namespace {
 
-using namespace attn;
-
 constexpr int NTHREADS = 224;  // four warps of keys, one that issues products, one that loads, one for the queries
-constexpr int WHOLE_TILES = 4;  // units of up to so many tiles are not cut
-
-// A unit that was cut: its parts lie in CTAs c0..c1.  c1 < 0: none.
-struct Joint {
-  int b, unit, c0, c1;
-};
-
-struct DecParams {
+struct TcParams : DecParams {
   CUtensorMap kv;  // {D, Hk * page, L * 2 * pages}
-  gdnx_paged_decode_args a;
-  float* part;     // [grid][2][NH][128] unnormalised outputs of a CTA's first and last unit
-  float* stat;     // [grid][2][NH][2] maximum (log2 domain) and sum
-  Joint* joint;    // [grid] the unit cut in several parts that ends in a CTA
-  int grid, groups;
-  int whole;       // no unit is cut: a CTA takes whole units
   int vec_q;       // q's rows are 16-byte aligned
 };
 
 struct Bars {
   uint64_t full[12], empty[12], q_ready[2], q_empty[2], s_full[2], p_ready[2], pv_done[2], done;
-};
-
-// The place of a CTA in the row of all tiles: its tiles t0..t1-1, the sequence b that holds t0
-// and the tiles of the sequences before b.  Tiles are ordered by sequence, unit, tile.
-struct Range {
-  int64_t t0, t1, before, b, per;
 };
 
 template <int NH>
@@ -78,125 +47,6 @@ struct Layout {
   static constexpr int TMEM = NH == 16 ? 64 : 128;  // columns: S twice, O
 };
 
-// Visible tokens of one sequence.
-struct Seq {
-  int row, len;
-  KeyTiles kt;
-};
-
-GDNX_DEV int slot_length(const gdnx_paged_decode_args& a, int64_t b, int& row) {
-  const gdnx_cache& c = a.cache;
-  row = a.rows ? a.rows[b] : (int)b;
-  if (row < 0 || row >= c.slots) return 0;
-  const int64_t n = c.lengths[row], most = c.width * c.page;
-  return (int)(n < 0 ? 0 : (n > most ? most : n));
-}
-
-GDNX_DEV Seq make_seq(const gdnx_paged_decode_args& a, int64_t b) {
-  int row;
-  const int len = slot_length(a, b, row);
-  return {row, len, KeyTiles(len - 1, len - 1, len, (int)a.window, (int)a.sinks, TM)};
-}
-
-GDNX_DEV int tiles_of(const gdnx_paged_decode_args& a, int64_t b) { return make_seq(a, b).kt.count; }
-
-// The CTA finds its range: every thread adds up a run of sequences, and the one whose run holds
-// the range's first tile walks to its sequence.  (Whole units: t0 and t1 count units.)
-GDNX_DEV void find_range(const DecParams& P, int units, Range& out, long long* sums) {
-  if (P.whole) {
-    if (threadIdx.x == 0) {
-      const int64_t all = P.a.B * units;
-      out = {all * blockIdx.x / P.grid, all * (blockIdx.x + 1) / P.grid, 0, 0, 0};
-    }
-    __syncthreads();
-    return;
-  }
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int64_t run = (P.a.B + NTHREADS - 1) / NTHREADS;
-  const int64_t b0 = min((int64_t)threadIdx.x * run, P.a.B), b1 = min(b0 + run, P.a.B);
-  long long mine = 0;
-  for (int64_t b = b0; b < b1; ++b) mine += tiles_of(P.a, b);
-  long long s = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += y;
-  }
-  if (lane == 31) sums[warp] = s;
-  if (threadIdx.x == 0) out = {0, 0, 0, 0, 1};
-  __syncthreads();
-  long long before = s - mine, total = 0;
-#pragma unroll
-  for (int i = 0; i < NTHREADS / 32; ++i) {
-    if (i < warp) before += sums[i];
-    total += sums[i];
-  }
-  total *= units;
-  before *= units;
-  const long long per = (total + P.grid - 1) / P.grid, t0 = min(blockIdx.x * per, total);
-  if (t0 < total && t0 >= before && t0 < before + mine * units) {
-    int64_t b = b0;
-    for (; b + 1 < b1; ++b) {
-      const long long n = (long long)tiles_of(P.a, b) * units;
-      if (t0 < before + n) break;
-      before += n;
-    }
-    out = {t0, min(t0 + per, total), before, b, per};
-  }
-  __syncthreads();
-}
-
-// Walks the units of a range: every role sees the same sequence of segments.
-struct Walk {
-  const DecParams& P;
-  int units;
-  int64_t t, t1, b, before;
-  Seq seq;
-  int unit, ta, tb;  // segment: tiles ta..tb-1 of `unit` of sequence b
-  GDNX_DEV Walk(const DecParams& P_, int units_, const Range& r)
-      : P(P_), units(units_), t(r.t0), t1(r.t1), b(r.b), before(r.before), seq(), unit(0), ta(0), tb(0) {
-    if (t < t1 && !P.whole) seq = make_seq(P.a, b);
-  }
-  GDNX_DEV bool next() {
-    if (P.whole) {
-      for (; t < t1; ++t) {
-        b = t / units;
-        unit = (int)(t % units);
-        seq = make_seq(P.a, b);
-        if ((tb = seq.kt.count) == 0) continue;
-        ++t;
-        return true;
-      }
-      return false;
-    }
-    if (t >= t1) return false;
-    while (t >= before + (int64_t)seq.kt.count * units) {
-      before += (int64_t)seq.kt.count * units;
-      seq = make_seq(P.a, ++b);
-    }
-    const int n = seq.kt.count;
-    unit = (int)((t - before) / n);
-    ta = (int)((t - before) % n);
-    tb = (int)min((int64_t)n, ta + (t1 - t));
-    t += tb - ta;
-    return true;
-  }
-  GDNX_DEV bool whole() const { return ta == 0 && tb == seq.kt.count; }
-};
-
-GDNX_DEV bool key_seen(int j, int len, int window, int sinks) {
-  return j < len && (len - 1 - j < window || j < sinks);
-}
-
-// Page ids of a tile's pages, or -1 where nothing visible is there (lane < npp).
-GDNX_DEV int page_id(const DecParams& P, const Seq& s, int kt, int i) {
-  const gdnx_cache& c = P.a.cache;
-  const int64_t first = (int64_t)kt * TM + i * c.page;
-  if (first >= s.len || !(first + c.page > (int64_t)s.len - P.a.window || first < P.a.sinks)) return -1;
-  const int p = c.table[(int64_t)s.row * c.width + first / c.page];
-  return p >= 0 && p < c.pages ? p : -1;
-}
-
 GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t mbar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -204,19 +54,8 @@ GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, 
       : "memory");
 }
 
-// Zeros for the sequences that see nothing.
-GDNX_DEV void write_zeros(const DecParams& P) {
-  const gdnx_paged_decode_args& a = P.a;
-  const int D = (int)a.cache.D, n = (int)a.H * D;
-  for (int64_t b = blockIdx.x; b < a.B; b += P.grid) {
-    if (tiles_of(a, b) > 0) continue;
-    for (int x = threadIdx.x % 32; x < n; x += 32)
-      st_from_f32(a.y, a.y_dtype, b * a.y_sb + x / D * a.y_sh + x % D, 0.f);
-  }
-}
-
 template <int DB, int NH>
-GDNX_DEV void run_loads(const DecParams& P, Walk w, uint32_t smem, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void run_loads(const TcParams& P, Walk w, uint32_t smem, Bars& bar, volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   const gdnx_cache& c = P.a.cache;
   const int lane = threadIdx.x % 32, npp = TM / c.page, page = c.page;
@@ -251,7 +90,7 @@ GDNX_DEV void run_loads(const DecParams& P, Walk w, uint32_t smem, Bars& bar, vo
 }
 
 template <int DB, int NH, bool BF16>
-GDNX_DEV void run_products(const DecParams& P, Walk w, uint32_t smem, uint32_t tmem, Bars& bar,
+GDNX_DEV void run_products(const TcParams& P, Walk w, uint32_t smem, uint32_t tmem, Bars& bar,
                            volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   constexpr uint32_t ID_S = idesc16(BF16, 128, NH, false, false), ID_O = idesc16(BF16, 128, NH, true, false);
@@ -311,19 +150,9 @@ GDNX_DEV void run_products(const DecParams& P, Walk w, uint32_t smem, uint32_t t
   values();
 }
 
-// Heads of one unit.
-struct Heads {
-  int h0, n;
-  GDNX_DEV Heads(const DecParams& P, int unit, int NH) {
-    const int G = (int)(P.a.H / P.a.cache.Hk), g = unit % P.groups;
-    h0 = unit / P.groups * G + g * NH;
-    n = min(NH, G - g * NH);
-  }
-};
-
 // The unit's query rows as a K-major tile of NH rows (rows beyond its heads zero), by one warp.
 template <int DB, int NH>
-GDNX_DEV void stage_q(const DecParams& P, const Walk& w, uint8_t* dst) {
+GDNX_DEV void stage_q(const TcParams& P, const Walk& w, uint8_t* dst) {
   const gdnx_paged_decode_args& a = P.a;
   const Heads hd(P, w.unit, NH);
   const int D = (int)a.cache.D;
@@ -347,7 +176,7 @@ GDNX_DEV void stage_q(const DecParams& P, const Walk& w, uint8_t* dst) {
 }
 
 template <int DB, int NH>
-GDNX_DEV void run_queries(const DecParams& P, Walk w, uint8_t* base, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void run_queries(const TcParams& P, Walk w, uint8_t* base, Bars& bar, volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   for (uint32_t seg = 0; w.next(); ++seg) {
     if (!warp_wait(&bar.q_empty[seg & 1], (seg / 2 & 1) ^ 1, abort_flag)) return;
@@ -383,7 +212,7 @@ GDNX_DEV void tmem_st(uint32_t at, const float (&v)[NC]) {
 
 // NC: heads that a thread works on, the unit's rounded up (the others' columns are not used).
 template <int DB, int NH, int NC, bool BF16>
-GDNX_DEV void run_keys(const DecParams& P, Walk w, int64_t per, uint8_t* base, uint32_t tmem, Bars& bar, float* red,
+GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, uint32_t tmem, Bars& bar, float* red,
                        volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   const gdnx_paged_decode_args& a = P.a;
@@ -503,7 +332,7 @@ GDNX_DEV void run_keys(const DecParams& P, Walk w, int64_t per, uint8_t* base, u
 }
 
 template <int DB, int NC, bool BF16>
-__global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __grid_constant__ DecParams P) {
+__global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __grid_constant__ TcParams P) {
   constexpr int NH = NC > 16 ? 32 : 16;
   using Lo = Layout<DB, NH>;
   extern __shared__ __align__(1024) uint8_t base[];
@@ -532,7 +361,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   }
   tc::fence_before();
   wait_for_earlier();
-  find_range(P, units, sm.range, sm.sums);  // synchronises
+  find_range<NTHREADS>(P, units, sm.range, sm.sums);  // synchronises
   tc::fence_after();
   const uint32_t tmem = uniform(sm.tmem_at);
   const Walk w(P, units, sm.range);
@@ -560,101 +389,19 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
 }
 
-// Joins a cut unit's parts, CTA after CTA: block (c, g) head g of the unit that ends in CTA c.
-// Each warp sums a contiguous run of the parts; the runs are added in order.
-constexpr int JOIN_WARPS = 8;
-
-template <int NH>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_decode_join_kernel(const DecParams P) {
-  const gdnx_paged_decode_args& a = P.a;
-  __shared__ float red_m[JOIN_WARPS], red_l[JOIN_WARPS], red_o[JOIN_WARPS][128];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, D = (int)a.cache.D, g = blockIdx.y;
-  dependents_may_start();
-  wait_for_earlier();  // the parts are there
-  const Joint j = P.joint[blockIdx.x];
-  if (j.c1 < 0) return;
-  const Heads hd(P, j.unit, NH);
-  if (g >= hd.n) return;
-  const int64_t out = j.b * a.y_sb + (hd.h0 + g) * a.y_sh;
-  const auto place = [&](int c) { return ((int64_t)c * 2 + (c == j.c0)) * NH + g; };
-  const int parts = j.c1 - j.c0 + 1, run = (parts + JOIN_WARPS - 1) / JOIN_WARPS;
-  const int r0 = j.c0 + warp * run, r1 = min(r0 + run, j.c1 + 1);
-  float m = -INFINITY, l = 0.f;
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = r0 + lane; c < r1; c += 32) m = fmaxf(m, P.stat[place(c) * 2]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-  for (int c = r0; c < r1; ++c) {
-    const int64_t at = place(c);
-    const float w = exp2f(P.stat[at * 2] - ref);
-    const float4 x = *reinterpret_cast<const float4*>(P.part + at * 128 + lane * 4);
-    l = fmaf(w, P.stat[at * 2 + 1], l);
-    y.x = fmaf(w, x.x, y.x);
-    y.y = fmaf(w, x.y, y.y);
-    y.z = fmaf(w, x.z, y.z);
-    y.w = fmaf(w, x.w, y.w);
-  }
-  *reinterpret_cast<float4*>(&red_o[warp][lane * 4]) = y;
-  if (lane == 0) {
-    red_m[warp] = m;
-    red_l[warp] = l;
-  }
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= D) return;
-  float top = -INFINITY, sum = 0.f, v = 0.f;
-#pragma unroll
-  for (int i = 0; i < JOIN_WARPS; ++i) top = fmaxf(top, red_m[i]);
-  if (top == -INFINITY) top = 0.f;
-#pragma unroll
-  for (int i = 0; i < JOIN_WARPS; ++i) {
-    const float w = exp2f(red_m[i] - top);
-    sum = fmaf(w, red_l[i], sum);
-    v = fmaf(w, red_o[i][d], v);
-  }
-  st_from_f32(a.y, a.y_dtype, out + d, sum == 0.f ? 0.f : v / sum);
-}
-
-struct Plan {
-  int nh, groups, grid, whole;
-};
-
-Plan plan(const gdnx_paged_decode_args& a, int sms) {
-  Plan p;
-  const int64_t G = a.H / a.cache.Hk;
-  p.nh = G > 16 ? 32 : 16;
-  p.groups = (int)((G + p.nh - 1) / p.nh);
-  int64_t most = a.cache.width * a.cache.page;
-  if (a.max_len > 0 && a.max_len < most) most = a.max_len;
-  int64_t n = (most + TM - 1) / TM;  // tiles of a unit, at most
-  const int64_t seen = (a.window + TM - 1) / TM + 1 + (a.sinks + TM - 1) / TM;
-  if (seen < n) n = seen;
-  const int64_t units = a.B * a.cache.Hk * p.groups;
-  // Short units are not cut: a few more tiles in a row take less time than a join.
-  p.whole = n <= WHOLE_TILES;
-  const int64_t ctas = p.whole ? units : units * n;
-  p.grid = (int)(ctas < sms ? (ctas > 0 ? ctas : 1) : sms);
-  return p;
-}
-
 template <int DB, int NC, bool BF16>
-gdnx_status launch(const DecParams& P, cudaStream_t st) {
+gdnx_status launch(const TcParams& P, cudaStream_t st) {
   constexpr int NH = NC > 16 ? 32 : 16;
   const auto kernel = paged_decode_tc_kernel<DB, NC, BF16>;
   constexpr int smem = (int)Layout<DB, NH>::SMEM;
   static std::atomic<uint64_t> done;
   if (!allow_smem(kernel, smem, done)) return GDNX_ELAUNCH;
   if (launch_early(kernel, dim3((unsigned)P.grid), dim3(NTHREADS), smem, st, P) != cudaSuccess) return GDNX_ELAUNCH;
-  if (P.whole) return GDNX_OK;
-  const int64_t G = P.a.H / P.a.cache.Hk;
-  return launch_early(paged_decode_join_kernel<NH>, dim3((unsigned)P.grid, (unsigned)(G < NH ? G : NH)),
-                      dim3(JOIN_WARPS * 32), 0, st, P) == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
+  return join_parts<NH>(P, st);
 }
 
 template <int DB, bool BF16>
-gdnx_status launch_heads(const DecParams& P, cudaStream_t st) {
+gdnx_status launch_heads(const TcParams& P, cudaStream_t st) {
   const int64_t G = P.a.H / P.a.cache.Hk;
   if (G <= 4) return launch<DB, 4, BF16>(P, st);
   if (G <= 8) return launch<DB, 8, BF16>(P, st);
@@ -662,15 +409,14 @@ gdnx_status launch_heads(const DecParams& P, cudaStream_t st) {
 }
 
 template <bool BF16>
-gdnx_status launch_type(const DecParams& P, cudaStream_t st) {
+gdnx_status launch_type(const TcParams& P, cudaStream_t st) {
   return P.a.cache.D > 64 ? launch_heads<2, BF16>(P, st) : launch_heads<1, BF16>(P, st);
 }
 
 }  // namespace
 
 size_t paged_decode_tc_workspace_bytes(const gdnx_paged_decode_args& a) {
-  const Plan p = plan(a, sm_count());
-  return p.whole ? 0 : (size_t)p.grid * (2 * p.nh * (128 + 2) * sizeof(float) + sizeof(Joint));
+  return plan_bytes(make_plan(a, a.H / a.cache.Hk > 16 ? 32 : 16));
 }
 
 gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t st) {
@@ -679,7 +425,7 @@ gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t
   if (!enc) return GDNX_ELAUNCH;
   if (c.L * 2 * c.pages > ((int64_t)1 << 31) - 1 || c.Hk * c.page * c.D * 2 >= ((int64_t)1 << 40))
     return GDNX_EUNSUPPORTED;
-  DecParams P;
+  TcParams P;
   const cuuint64_t dims[3] = {(cuuint64_t)c.D, (cuuint64_t)(c.Hk * c.page), (cuuint64_t)(c.L * 2 * c.pages)};
   const cuuint64_t strides[2] = {(cuuint64_t)c.D * 2, (cuuint64_t)(c.Hk * c.page * c.D) * 2};
   const cuuint32_t box[3] = {64, (cuuint32_t)c.page, 1}, es[3] = {1, 1, 1};
@@ -687,14 +433,7 @@ gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t
           dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return GDNX_EINVAL;
-  const Plan p = plan(a, sm_count());
-  P.a = a;
-  P.grid = p.grid;
-  P.groups = p.groups;
-  P.part = static_cast<float*>(a.workspace);
-  P.stat = P.part + (size_t)p.grid * 2 * p.nh * 128;
-  P.joint = reinterpret_cast<Joint*>(P.stat + (size_t)p.grid * 2 * p.nh * 2);
-  P.whole = p.whole;
+  fill(P, a, make_plan(a, a.H / c.Hk > 16 ? 32 : 16));
   P.vec_q = reinterpret_cast<uintptr_t>(a.q.ptr) % 16 == 0 && a.q.sb % 8 == 0 && a.q.sh % 8 == 0;
   return c.dtype == GDNX_BF16 ? launch_type<true>(P, st) : launch_type<false>(P, st);
 }
