@@ -9,7 +9,8 @@
 // While one stage's rows take exponentials, the tensor cores work for the other.
 // Warps 0-3 and 4-7 are the stages' rows, warp 8 issues the products, warp 9 the TMA loads
 // (Q of each stage, K and V through one ring).  A stage's PV(t) and S(t+1) are
-// issued in order, so S(t+1) complete means PV(t) complete and O at rest.
+// issued in order, so S(t+1) complete means PV(t) complete and O at rest.  P is handed over in
+// halves of 64 keys: PV(t) starts under the second half's exponentials.
 //
 // The exponentials are what the tensor cores wait for: 128 x 128 of them a tile take the
 // special-function units as long as its two products take the tensor cores.  So an eighth of
@@ -88,7 +89,7 @@ GDNX_DEV Item make_item(const FwdParams& P, int64_t item) {
 }
 
 struct Bars {
-  uint64_t kv_full[8], kv_empty[8], q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2], fix, done;
+  uint64_t kv_full[8], kv_empty[8], q_full[2], q_empty[2], s_full[2], p_ready[2][2], o_full[2], fix, done;
 };
 
 struct Small {
@@ -215,6 +216,8 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
           uint32_t pk[32];
           weights<BF16, 64>(s + 64 * half, c2, mc, sum, pk);
           tmem_st32u(tS + 32 * half, pk);
+          tc::fence_before();
+          pipe::mbar_arrive(&bar.p_ready[st][half]);
         }
       } else {
         // chunk by chunk of 32 columns: what no row of the warp sees costs nothing
@@ -246,11 +249,13 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
             weights<BF16, 32>(s, c2, mc, sum, pk);
           }
           tc::tmem_st16u(tS + 16 * q, pk);  // over scores that have been read
+          if (q % 2) {
+            tc::fence_before();
+            pipe::mbar_arrive(&bar.p_ready[st][q / 2]);
+          }
         }
       }
       row.l += sum.x + sum.y;
-      tc::fence_before();
-      pipe::mbar_arrive(&bar.p_ready[st]);
     }
     if (w.hi(st) >= 0) {
       if (!warp_wait(&bar.o_full[st], nO++ & 1, abort_flag)) return;
@@ -321,11 +326,17 @@ GDNX_DEV void run_products(const FwdParams& P, uint32_t smem, uint32_t tmem, Bar
         const uint32_t tS = tmem + T_S + st * 128, tO = tmem + T_O + st * 128;
         const bool on = more && w.active(st, kt);
         if (on && !begun[st] && !warp_wait(&bar.q_full[st], nQ[st]++ & 1, abort_flag)) return;
-        if (pend[st] && !warp_wait(&bar.p_ready[st], nP[st]++ & 1, abort_flag)) return;
+        if (pend[st]) {  // the first half's weights, then the second's
+          if (!warp_wait(&bar.p_ready[st][0], nP[st] & 1, abort_flag)) return;
+          tc::fence_after();
+          if (elect_one()) mma_px<4>(tO, tS, v, ID_O, acc[st]);
+          __syncwarp();
+          if (!warp_wait(&bar.p_ready[st][1], nP[st]++ & 1, abort_flag)) return;
+        }
         tc::fence_after();
         if (elect_one()) {
           if (pend[st]) {
-            mma_px<8>(tO, tS, v, ID_O, acc[st]);
+            mma_px<4>(tO, tS + 32, v + 64 * 128, ID_O, true);
             if (!on) tc::commit(&bar.o_full[st]);  // a stage's tiles have no gap
           }
           if (st == 1 && i > 0) tc::commit(&bar.kv_empty[old]);
@@ -417,7 +428,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
       tc::mbar_init(&bar.q_full[s], 1);
       tc::mbar_init(&bar.q_empty[s], 1);
       tc::mbar_init(&bar.s_full[s], 1);
-      tc::mbar_init(&bar.p_ready[s], 128);
+      tc::mbar_init(&bar.p_ready[s][0], 128);
+      tc::mbar_init(&bar.p_ready[s][1], 128);
       tc::mbar_init(&bar.o_full[s], 1);
     }
     tc::mbar_init(&bar.fix, 1);
