@@ -15,12 +15,18 @@
 //
 // A key tile that holds sinks is seen by every later query, far more than the others; its
 // iterations (and all tiles' where there are few) are cut into parts that leave fp32
-// partial sums, which attn_dkv_join adds in order.
+// partial sums, added in order when attn_dkv has ended (by the blocks of attn_dq).
+//
+// attn_dkv's blocks take their key tile whole, which leaves SMs idle at its end (256 tiles on 148
+// SMs: two rounds).  So attn_dq starts there as they fall free and deals its items out by a
+// counter: together they end evenly (348 us of a step with 2 x 4096 tokens, 16 heads over 4 of
+// 128, window 1024; 378 us one after the other).
 //
 // Weights and dS are rounded to bf16 for the products, like the inputs themselves; dS of
 // float16 inputs could leave float16's range, so those take the CUDA-core kernels.
 #include "attn_tc.cuh"
 #include "kernels.h"
+#include "launch.cuh"
 
 namespace gdnx {
 namespace {
@@ -40,11 +46,12 @@ struct BwdParams {
   int qtiles, ktiles, nst;    // nst: key tiles that hold sinks
   int seg_sink, seg;          // parts of such a tile and of the others
   unsigned queries;           // items of attn_dq
+  unsigned* next;             // the next of them to take
 };
 
 struct Bars {
   uint64_t full[SLOTS], empty[SLOTS], res[2], res_empty[2], stat_full[2], stat_empty[2], s_full[2], dp_full, p_ready, ds_ready[2],
-      dp_read, o_full, fix, done;
+      dp_read, o_full, fix, done, item_full[2], item_empty[2];
 };
 
 template <int DB>
@@ -129,6 +136,8 @@ GDNX_DEV void init_bars(Bars& bar) {
     tc::mbar_init(&bar.stat_empty[i], 512);
     tc::mbar_init(&bar.s_full[i], 1);
     tc::mbar_init(&bar.ds_ready[i], 512);
+    tc::mbar_init(&bar.item_full[i], 1);
+    tc::mbar_init(&bar.item_empty[i], 512 + 1);
   }
   tc::mbar_init(&bar.dp_full, 1);
   tc::mbar_init(&bar.p_ready, 512);
@@ -397,9 +406,18 @@ GDNX_DEV QueryItem query_item(const BwdParams& P, unsigned n) {
 constexpr uint32_t Q_S = 0, Q_DP = 256, Q_DQ = 384;  // S has two buffers
 
 // A persistent CTA takes item after item: tiles are counted through (T), so that the loads and
-// the first products of an item run under the one before.
+// the first products of an item run under the one before.  CTAs start as attn_dkv leaves SMs
+// free, so items are dealt out by a counter: the loads take a number and pass it on through two
+// places (an item is computed alike whoever takes it).
+GDNX_DEV bool next_item(Bars& bar, const volatile unsigned* dealt, uint32_t k, unsigned& n, volatile int* abort_flag) {
+  if (!warp_wait(&bar.item_full[k & 1], k / 2 & 1, abort_flag)) return false;
+  n = dealt[k & 1];
+  return true;
+}
+
 template <int DB>
-GDNX_DEV void queries_rows(const BwdParams& P, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void queries_rows(const BwdParams& P, uint32_t tmem, Bars& bar, const volatile unsigned* dealt,
+                           volatile int* abort_flag) {
   const gdnx_attn_args& a = P.a;
   const int r = threadIdx.x % 128, part = threadIdx.x / 128;
   const uint32_t lane_at = (uint32_t)(r / 32 * 32) << 16;
@@ -408,11 +426,14 @@ GDNX_DEV void queries_rows(const BwdParams& P, uint32_t tmem, Bars& bar, volatil
   const float c2 = a.scale * kLog2e;
   const float2 cc = make_float2(c2, c2);
   uint32_t T = 0, items = 0;
-  for (unsigned n = blockIdx.x; n < P.queries; n += gridDim.x) {
+  for (uint32_t k = 0;; ++k) {
+    unsigned n;
+    if (!next_item(bar, dealt, k, n, abort_flag) || n >= P.queries) return;
+    pipe::mbar_arrive(&bar.item_empty[k & 1]);
     const QueryItem w = query_item(P, n);
     const int len = w.len, p = w.p0 + r, i = w.i0 + r;
     const int64_t at = ((int64_t)w.b * a.H + w.h) * P.qtiles * TM + i;
-    const float lse2 = P.lse2[at], del = P.delta[at];
+    const float lse2 = __ldcg(P.lse2 + at), del = __ldcg(P.delta + at);
     const bool one = sees_one(p, window, sinks);
     for (int t = 0; t < w.kt.count; ++t, ++T) {
       const uint32_t buf = T & 1;
@@ -476,7 +497,8 @@ GDNX_DEV void queries_rows(const BwdParams& P, uint32_t tmem, Bars& bar, volatil
 }
 
 template <int DB>
-GDNX_DEV void queries_products(const BwdParams& P, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void queries_products(const BwdParams& P, uint32_t smem, uint32_t tmem, Bars& bar,
+                               const volatile unsigned* dealt, volatile int* abort_flag) {
   using Lo = Layout<DB>;
   constexpr uint32_t ID_S = idesc16(true, 128, 128, false, false), ID_O = idesc16(true, 128, 64 * DB, false, true);
   uint32_t T = 0, items = 0;  // tiles before this item; items with tiles
@@ -508,7 +530,13 @@ GDNX_DEV void queries_products(const BwdParams& P, uint32_t smem, uint32_t tmem,
     __syncwarp();
     return true;
   };
-  for (unsigned it = blockIdx.x; it < P.queries; it += gridDim.x) {
+  for (uint32_t k = 0;; ++k) {
+    unsigned it;
+    if (!next_item(bar, dealt, k, it, abort_flag)) return;
+    __syncwarp();  // read by every lane
+    if (threadIdx.x % 32 == 0) pipe::mbar_arrive(&bar.item_empty[k & 1]);
+    it = uniform(it);
+    if (it >= P.queries) return;
     const int n = query_item(P, it).kt.count;
     if (n == 0) continue;
     if (!warp_wait(&bar.res[0], items & 1, abort_flag) || !scores(0, n == 1)) return;
@@ -534,11 +562,21 @@ GDNX_DEV void queries_products(const BwdParams& P, uint32_t smem, uint32_t tmem,
 }
 
 template <int DB>
-GDNX_DEV void queries_loads(const BwdParams& P, uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void queries_loads(const BwdParams& P, uint8_t* base, uint32_t smem, Bars& bar, volatile unsigned* dealt,
+                            volatile int* abort_flag) {
   using Lo = Layout<DB>;
   const gdnx_attn_args& a = P.a;
   uint32_t nfix = 0, T = 0, items = 0;
-  for (unsigned n = blockIdx.x; n < P.queries; n += gridDim.x) {
+  for (uint32_t k = 0;; ++k) {
+    unsigned n = 0;
+    if (!warp_wait(&bar.item_empty[k & 1], (k / 2 & 1) ^ 1, abort_flag)) return;
+    if (threadIdx.x % 32 == 0) {
+      n = atomicAdd(P.next, 1u);
+      dealt[k & 1] = n;
+      pipe::mbar_arrive(&bar.item_full[k & 1]);
+    }
+    n = uniform(n);
+    if (n >= P.queries) return;
     const QueryItem w = query_item(P, n);
     for (int t = 0; t < w.kt.count; ++t, ++T) {
       const int j0 = w.kt.tile(t) * TM;
@@ -562,7 +600,34 @@ GDNX_DEV void queries_loads(const BwdParams& P, uint8_t* base, uint32_t smem, Ba
   }
 }
 
-// The frame of both kernels.
+// Sums of cut tiles' parts, in order: one thread for each (tile, key, four values).
+template <int DB>
+GDNX_DEV void join_parts(const BwdParams& P, int first, int tiles) {
+  const gdnx_attn_args& a = P.a;
+  const int bh = (int)(a.B * a.Hk), W = 64 * DB, nseg = first == 0 && P.nst > 0 ? P.seg_sink : P.seg;
+  const int64_t item0 = first == 0 ? 0 : (int64_t)bh * P.nst * P.seg_sink;
+  const int64_t all = (int64_t)tiles * bh * 2 * TM * (W / 4);
+  for (int64_t x = (int64_t)blockIdx.x * NTHREADS + threadIdx.x; x < all; x += (int64_t)gridDim.x * NTHREADS) {
+    const int d = (int)(x % (W / 4)) * 4, r = (int)(x / (W / 4) % TM), side = (int)(x / (W / 4 * TM) % 2);
+    const int who = (int)(x / (2 * (W / 4) * TM) % bh), tile = (int)(x / ((int64_t)2 * (W / 4) * TM * bh));
+    const int64_t j = (int64_t)(first + tile) * TM + r;
+    if (j >= a.Tk || d >= a.D) continue;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < nseg; ++s) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(
+          P.part + (((item0 + ((int64_t)tile * nseg + s) * bh + who) * 2 + side) * TM + r) * W + d));
+      sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(side ? P.dk : P.dv) +
+                              ((who / a.Hk * a.Tk + j) * a.Hk + who % a.Hk) * a.D + d) =
+        make_uint2(tc::pack_bf16(sum.x, sum.y), tc::pack_bf16(sum.z, sum.w));
+  }
+}
+
+// The frame of both kernels.  attn_dkv needs the statistics; attn_dq needs them too, which every CTA
+// of attn_dkv has waited for before it lets attn_dq start.  attn_dq ends after attn_dkv, whose parts it
+// joins.
 template <int DB, bool KEYS>
 __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_constant__ BwdParams P) {
   using Lo = Layout<DB>;
@@ -570,6 +635,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_c
   Bars& bar = *reinterpret_cast<Bars*>(base + Lo::BARS);
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(base + Lo::BARS + 448);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(base + Lo::BARS + 452);
+  volatile unsigned* dealt = reinterpret_cast<volatile unsigned*>(base + Lo::BARS + 456);
   static_assert(sizeof(Bars) <= 448, "barriers fit their place");
   const uint32_t smem = uniform(tc::smem_u32(base));
   const int warp = uniform(threadIdx.x / 32);
@@ -582,6 +648,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_c
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = uniform(*tmem_at);
+  if (KEYS) {
+    wait_for_earlier();
+    dependents_may_start();
+  }
   if (smem % 1024 == 0) {
     if (KEYS) {
       const KeyItem w = key_item(P);
@@ -589,9 +659,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_c
       else if (warp == 16) keys_products<DB>(w, smem, tmem, bar, abort_flag);
       else if (warp == 17) keys_loads<DB>(P, w, base, smem, bar, abort_flag);
     } else {
-      if (warp < 16) queries_rows<DB>(P, tmem, bar, abort_flag);
-      else if (warp == 16) queries_products<DB>(P, smem, tmem, bar, abort_flag);
-      else if (warp == 17) queries_loads<DB>(P, base, smem, bar, abort_flag);
+      if (warp < 16) queries_rows<DB>(P, tmem, bar, dealt, abort_flag);
+      else if (warp == 16) queries_products<DB>(P, smem, tmem, bar, dealt, abort_flag);
+      else if (warp == 17) queries_loads<DB>(P, base, smem, bar, dealt, abort_flag);
     }
   }
   if (warp == 16) {  // every product issued has ended
@@ -607,24 +677,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_c
   tc::fence_after();
   if (warp == 16) tc::tmem_dealloc(tmem, 512);
   if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
-}
-
-// Sums of cut tiles' parts: one thread for each (tile, key, value).
-template <int DB>
-__global__ void __launch_bounds__(256) attn_dkv_join_kernel(const BwdParams P, int first, int tiles) {
-  const gdnx_attn_args& a = P.a;
-  const int bh = (int)(a.B * a.Hk), W = 64 * DB, nseg = first == 0 && P.nst > 0 ? P.seg_sink : P.seg;
-  const int64_t item0 = first == 0 ? 0 : (int64_t)bh * P.nst * P.seg_sink;
-  const int64_t all = (int64_t)tiles * bh * 2 * TM * W;
-  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
-    const int d = (int)(x % W), r = (int)(x / W % TM), side = (int)(x / (W * TM) % 2);
-    const int who = (int)(x / (2 * W * TM) % bh), tile = (int)(x / ((int64_t)2 * W * TM * bh));
-    const int64_t j = (int64_t)(first + tile) * TM + r;
-    if (j >= a.Tk || d >= a.D) continue;
-    float sum = 0.f;
-    for (int s = 0; s < nseg; ++s)
-      sum += P.part[(((item0 + ((int64_t)tile * nseg + s) * bh + who) * 2 + side) * TM + r) * W + d];
-    st_from_f32(side ? P.dk : P.dv, GDNX_BF16, ((who / a.Hk * a.Tk + j) * a.Hk + who % a.Hk) * a.D + d, sum);
+  if (!KEYS) {
+    wait_for_earlier();
+    if (P.nst > 0 && P.seg_sink > 1) join_parts<DB>(P, 0, P.nst);
+    if (P.ktiles > P.nst && P.seg > 1) join_parts<DB>(P, P.nst, P.ktiles - P.nst);
   }
 }
 
@@ -632,7 +688,9 @@ __global__ void __launch_bounds__(256) attn_dkv_join_kernel(const BwdParams P, i
 // for each row.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const gdnx_attn_bwd_args g, float* lse2, float* delta,
-                                                         int qpad) {
+                                                         unsigned* next, int qpad) {
+  dependents_may_start();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *next = 0;
   const gdnx_attn_args& a = g.fwd;
   const int64_t n = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
   if (n >= a.B * a.H * qpad) return;  // whole groups of eight
@@ -713,18 +771,16 @@ gdnx_status run(const gdnx_attn_bwd_args& g, BwdParams& P, cudaStream_t st) {
   if (!allow_smem(keys, smem, done_keys) || !allow_smem(queries, smem, done_queries)) return GDNX_ELAUNCH;
   const int64_t rows = (int64_t)stats_floats(P);
   attn_stats_kernel<__nv_bfloat16><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(
-      g, const_cast<float*>(P.lse2), const_cast<float*>(P.delta), P.qtiles * TM);
-  keys<<<(unsigned)items_of(P), NTHREADS, smem, st>>>(P);
-  const int bh = (int)(a.B * a.Hk);
-  const auto join = [&](int first, int tiles) {
-    const int64_t blocks = ((int64_t)tiles * bh * 2 * TM * 64 * DB + 255) / 256;
-    attn_dkv_join_kernel<DB><<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st>>>(P, first, tiles);
-  };
-  if (P.nst > 0 && P.seg_sink > 1) join(0, P.nst);
-  if (P.ktiles > P.nst && P.seg > 1) join(P.nst, P.ktiles - P.nst);
+      g, const_cast<float*>(P.lse2), const_cast<float*>(P.delta), P.next, P.qtiles * TM);
+  if (cudaGetLastError() != cudaSuccess ||
+      launch_early(keys, dim3((unsigned)items_of(P)), dim3(NTHREADS), smem, st, P) != cudaSuccess)
+    return GDNX_ELAUNCH;
+  const int64_t joined = ((P.seg_sink > 1 ? P.nst : 0) + (P.seg > 1 ? P.ktiles - P.nst : 0)) * a.B * a.Hk;
+  const int64_t work = joined * 8 > P.queries ? joined * 8 : P.queries;  // a block for some rows of a joined tile
   const unsigned sms = (unsigned)sm_count();
-  queries<<<P.queries < sms ? P.queries : sms, NTHREADS, smem, st>>>(P);
-  return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
+  if (launch_early(queries, dim3(work < sms ? (unsigned)work : sms), dim3(NTHREADS), smem, st, P) != cudaSuccess)
+    return GDNX_ELAUNCH;
+  return GDNX_OK;
 }
 
 }  // namespace
@@ -733,7 +789,7 @@ size_t attn_bwd_tc_workspace_bytes(const gdnx_attn_args& a) {
   BwdParams P;
   P.a = a;
   plan(P);
-  return (2 * stats_floats(P) + part_floats(P)) * sizeof(float);
+  return (2 * stats_floats(P) + 4 + part_floats(P)) * sizeof(float);
 }
 
 gdnx_status launch_attn_bwd_tc(const gdnx_attn_bwd_args& g, cudaStream_t st) {
@@ -758,7 +814,8 @@ gdnx_status launch_attn_bwd_tc(const gdnx_attn_bwd_args& g, cudaStream_t st) {
   float* ws = static_cast<float*>(g.workspace);
   P.lse2 = ws;
   P.delta = ws + stats_floats(P);
-  P.part = ws + 2 * stats_floats(P);
+  P.next = reinterpret_cast<unsigned*>(ws + 2 * stats_floats(P));  // 16 bytes
+  P.part = ws + 2 * stats_floats(P) + 4;
   return a.D > 64 ? run<2>(g, P, st) : run<1>(g, P, st);
 }
 
