@@ -2,18 +2,24 @@
 // arithmetic is fp32, so this is the path of 32-bit inputs, and of 16-bit inputs that TMA
 // cannot address.
 //
-// Forward, one block of 64 queries of one head, key tiles of 64 in sequence:
+// Forward, one block of 32 queries of one head, key tiles of 64 in sequence:
 //   s = scale log2(e) q.k;  m' = max(m, max_j s);  p = 2^(s - m');
 //   l = l 2^(m - m') + sum_j p;  o = o 2^(m - m') + p V;   y = o / l.
 // Backward, with P recomputed from lse (P = exp(scale q.k - lse)) and
 // delta_i = sum_d dy_id y_id (which is sum_j P_ij dP_ij):
 //   dP = dy V^T;  dS = P (dP - delta);  dV = P^T dy;  dQ = scale dS K;  dK = scale dS^T Q.
-// dQ has a block for each 64 queries, dK and dV one for each 64 keys, which takes the query
+// dQ has a block for each 32 queries, dK and dV one for each 32 keys, which takes the query
 // heads of its key head and the query tiles in order: no atomics, sums in a fixed order.
 //
-// A thread holds a 4 x 4 piece of the 64 x 64 score tile and a 4 x D/16 piece of the
-// accumulators.  Padding rows are loaded as zeros, so NaN in them meets no sum.
-#include "attn_common.cuh"
+// A block's own tile has 32 rows, the tiles that stream past it 64.  A thread holds a 4 x 4 piece of
+// the scores and a 4 x D/16 piece of the accumulators, a warp eight rows: so a warp's weights are its
+// own (no barrier between the two products), and it leaves out the groups of 16 columns that none of
+// its rows sees, which at the ends of the window and in the sinks' tile are most.  Several blocks of an
+// SM cover each other's loads.  Products go two d to an instruction.  Padding rows are loaded as zeros,
+// so NaN in them meets no sum.
+#include <type_traits>
+
+#include "attn_tc.cuh"
 #include "kernels.h"
 
 namespace gdnx {
@@ -21,8 +27,9 @@ namespace {
 
 using namespace attn;
 
-constexpr int BT = 64;        // rows of every tile
-constexpr int NT = 256;       // threads
+constexpr int BR = 32;        // rows of a block's own tiles
+constexpr int BT = 64;        // rows of the tiles that stream past
+constexpr int NT = 128;       // threads
 constexpr int LDP = BT + 4;   // row stride of the weight tile (16-byte rows, conflict-free)
 
 // Blocks run over heads, then batch rows, then tiles: those of one tile, which cost alike, side
@@ -45,14 +52,14 @@ GDNX_DEV float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(
 template <>
 GDNX_DEV float to_f32<__half>(__half x) { return __half2float(x); }
 
-// Rows r0..r0+63 of head h (rows at or beyond `rows` as zeros) into dst [64][DP + 4].  Aligned
+// Rows r0..r0+R-1 of head h (rows at or beyond `rows` as zeros) into dst [R][DP + 4].  Aligned
 // 32-bit rows go by 16-byte asynchronous copies (landed after `wait_tiles`), others by value.
-template <int DP, typename T>
+template <int R, int DP, typename T>
 GDNX_DEV void load_tile(float* dst, const gdnx_view& v, int64_t b, int64_t h, int r0, int rows, int D) {
   const T* base = reinterpret_cast<const T*>(v.ptr) + b * v.sb + h * v.sh;
   if (sizeof(T) == 4 && reinterpret_cast<uintptr_t>(base) % 16 == 0 && v.st % 4 == 0) {
 #pragma unroll
-    for (int k = 0; k < BT * DP / 4 / NT; ++k) {
+    for (int k = 0; k < R * DP / 4 / NT; ++k) {
       const int i = k * NT + threadIdx.x, r = i / (DP / 4), d = i % (DP / 4) * 4;
       const bool on = r0 + r < rows && d < D;
       const T* src = on ? base + (int64_t)(r0 + r) * v.st + d : base;
@@ -64,7 +71,7 @@ GDNX_DEV void load_tile(float* dst, const gdnx_view& v, int64_t b, int64_t h, in
     return;
   }
 #pragma unroll 8
-  for (int i = threadIdx.x; i < BT * DP; i += NT) {
+  for (int i = threadIdx.x; i < R * DP; i += NT) {
     const int r = i / DP, d = i % DP;
     float x = 0.f;
     if (r0 + r < rows && d < D) x = to_f32(base[(int64_t)(r0 + r) * v.st + d]);
@@ -76,40 +83,78 @@ GDNX_DEV void wait_tiles() {
   asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
 }
 
-// s[a][c] = sum_{d < D} A[ty*4+a][d] B[tx+16c][d]  (D a multiple of 8)
-template <int DP>
-GDNX_DEV void dot_tile(float (&s)[4][4], const float* A, const float* B, int ty, int tx, int D) {
-#pragma unroll
-  for (int a = 0; a < 4; ++a)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) s[a][c] = 0.f;
-#pragma unroll 4
-  for (int d = 0; d < D; d += 4) {
-    float4 x[4], y[4];
-#pragma unroll
-    for (int a = 0; a < 4; ++a) x[a] = *reinterpret_cast<const float4*>(A + (ty * 4 + a) * (DP + 4) + d);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) y[c] = *reinterpret_cast<const float4*>(B + (tx + 16 * c) * (DP + 4) + d);
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[a][c] = fmaf(x[a].x, y[c].x, s[a][c]);
-        s[a][c] = fmaf(x[a].y, y[c].y, s[a][c]);
-        s[a][c] = fmaf(x[a].z, y[c].z, s[a][c]);
-        s[a][c] = fmaf(x[a].w, y[c].w, s[a][c]);
-      }
+// The groups of 16 of a streamed tile's rows that a warp's own eight rows meet: first, first + n - 1.
+struct Groups {
+  int first, n;
+  GDNX_DEV Groups(int lo, int hi) {  // rows lo..hi of the tile, any integers
+    lo = max(lo, 0);
+    hi = min(hi, BT - 1);
+    first = lo / 16;
+    n = lo > hi ? 0 : hi / 16 - first + 1;
+  }
+};
+// Keys of the tile at j0 that the queries at positions p..p+7 see.
+GDNX_DEV Groups keys_seen(int p, int j0, int len, int window, int sinks) {
+  const int last = min(p + 7, len - 1) - j0, lo = p - window + 1 - j0;
+  if (p >= len) return Groups(1, 0);
+  if (sinks <= j0) return Groups(lo, last);
+  return Groups(0, lo <= BT - 1 ? last : min(last, sinks - 1 - j0));
+}
+// Queries of the tile at position p0 that see the keys j..j+7.
+GDNX_DEV Groups queries_seeing(int j, int p0, int len, int window, int sinks) {
+  if (j >= len) return Groups(1, 0);
+  const int last = j < sinks ? len - 1 : (int)min((int64_t)len - 1, (int64_t)j + 6 + window);
+  return Groups(j - p0, last - p0);
+}
+
+// f(std::integral_constant<int, n>) for n in 1..4: code for that many groups.
+template <typename F>
+GDNX_DEV void for_groups(int n, F f) {
+  switch (n) {
+    case 1: f(std::integral_constant<int, 1>()); break;
+    case 2: f(std::integral_constant<int, 2>()); break;
+    case 3: f(std::integral_constant<int, 3>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
   }
 }
 
-// o[a][64 g + tx*4 ..] += sum_j W[ty*4+a][j] X[j][64 g + tx*4 ..]
+// s[a][c] = sum_{d < D} A[a][d] B[16c][d]  (D a multiple of 8), two d to an instruction
+template <int DP, int NC>
+GDNX_DEV void dot_tile(float (&s)[4][4], const float* A, const float* B, int D) {
+  float2 t[4][NC];
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) t[a][c] = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int d = 0; d < D; d += 4) {
+    float4 x[4], y[NC];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) x[a] = *reinterpret_cast<const float4*>(A + a * (DP + 4) + d);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) y[c] = *reinterpret_cast<const float4*>(B + 16 * c * (DP + 4) + d);
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        t[a][c] = fma2(make_float2(x[a].x, x[a].y), make_float2(y[c].x, y[c].y), t[a][c]);
+        t[a][c] = fma2(make_float2(x[a].z, x[a].w), make_float2(y[c].z, y[c].w), t[a][c]);
+      }
+  }
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s[a][c] = t[a][c].x + t[a][c].y;
+}
+
+// o[a][64 g + tx*4 ..] += sum_j W[a][j] X[j][64 g + tx*4 ..] over the groups' j
 template <int DP>
-GDNX_DEV void acc_tile(float (&o)[4][DP / 16], const float* W, const float* X, int ty, int tx) {
+GDNX_DEV void acc_tile(float2 (&o)[4][DP / 32], const float* W, const float* X, int tx, const Groups& gr) {
 #pragma unroll 2
-  for (int j = 0; j < BT; j += 4) {
+  for (int j = 16 * gr.first; j < 16 * (gr.first + gr.n); j += 4) {
     float4 w[4];
 #pragma unroll
-    for (int a = 0; a < 4; ++a) w[a] = *reinterpret_cast<const float4*>(W + (ty * 4 + a) * LDP + j);
+    for (int a = 0; a < 4; ++a) w[a] = *reinterpret_cast<const float4*>(W + a * LDP + j);
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
 #pragma unroll
@@ -118,15 +163,22 @@ GDNX_DEV void acc_tile(float (&o)[4][DP / 16], const float* W, const float* X, i
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           const float p = jj == 0 ? w[a].x : jj == 1 ? w[a].y : jj == 2 ? w[a].z : w[a].w;
-          o[a][g * 4 + 0] = fmaf(p, x.x, o[a][g * 4 + 0]);
-          o[a][g * 4 + 1] = fmaf(p, x.y, o[a][g * 4 + 1]);
-          o[a][g * 4 + 2] = fmaf(p, x.z, o[a][g * 4 + 2]);
-          o[a][g * 4 + 3] = fmaf(p, x.w, o[a][g * 4 + 3]);
+          o[a][g * 2] = fma2(make_float2(p, p), make_float2(x.x, x.y), o[a][g * 2]);
+          o[a][g * 2 + 1] = fma2(make_float2(p, p), make_float2(x.z, x.w), o[a][g * 2 + 1]);
         }
       }
     }
   }
 }
+template <int N>
+GDNX_DEV void clear(float2 (&o)[4][N]) {
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int d = 0; d < N; ++d) o[a][d] = make_float2(0.f, 0.f);
+}
+// Value e of the four that a thread holds of a 64-wide piece.
+GDNX_DEV float part_of(const float2* o, int e) { return e % 2 ? o[e / 2].y : o[e / 2].x; }
 
 GDNX_DEV float half_warp_max(float x) {
 #pragma unroll
@@ -145,65 +197,73 @@ GDNX_DEV float rounded(float x, int dtype) {
 }
 
 template <int DP, typename T>
-__global__ void __launch_bounds__(NT) attn_fwd_simt_kernel(const gdnx_attn_args a) {
+__global__ void __launch_bounds__(NT, 3) attn_fwd_simt_kernel(const gdnx_attn_args a) {
   extern __shared__ float sm[];
   float* Q = sm;
-  float* KV = Q + BT * (DP + 4);
+  float* KV = Q + BR * (DP + 4);
   float* W = KV + BT * (DP + 4);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const Block blk = block_of(a.H, a.B);
-  const int i0 = ((int)((a.Tq + BT - 1) / BT) - 1 - blk.tile) * BT, D = (int)a.D;
+  const int i0 = ((int)((a.Tq + BR - 1) / BR) - 1 - blk.tile) * BR, D = (int)a.D;
   const int64_t h = blk.h, b = blk.b, hk = h / (a.H / a.Hk);
   const int off = (int)(a.Tk - a.Tq), len = seq_len(a, b);
   const int window = (int)a.window, sinks = (int)a.sinks;
   const float c2 = a.scale * kLog2e;
-  const KeyTiles kt(i0 + off, min(i0 + BT, (int)a.Tq) - 1 + off, len, window, sinks, BT);
-  load_tile<DP, T>(Q, a.q, b, h, i0, min((int)a.Tq, len - off), D);
-  float o[4][DP / 16], m[4], l[4];
+  const KeyTiles kt(i0 + off, min(i0 + BR, (int)a.Tq) - 1 + off, len, window, sinks, BT);
+  load_tile<BR, DP, T>(Q, a.q, b, h, i0, min((int)a.Tq, len - off), D);
+  const int pw = i0 + off + ty / 2 * 8;  // the warp's first position
+  const float* q = Q + ty * 4 * (DP + 4);
+  float* w = W + ty * 4 * LDP;
+  float2 o[4][DP / 32];
+  float m[4], l[4];
+  clear(o);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) o[r][d] = 0.f;
   }
   for (int t = 0; t < kt.count; ++t) {
     const int j0 = kt.tile(t) * BT;
+    const Groups gr = keys_seen(pw, j0, len, window, sinks);
     __syncthreads();
-    load_tile<DP, T>(KV, a.k, b, hk, j0, len, D);
+    load_tile<BT, DP, T>(KV, a.k, b, hk, j0, len, D);
     wait_tiles();
     __syncthreads();
-    float s[4][4];
-    dot_tile<DP>(s, Q, KV, ty, tx, D);
+    for_groups(gr.n, [&](auto nc) {
+      constexpr int NC = decltype(nc)::value;
+      const int col = 16 * gr.first + tx;
+      float s[4][4];
+      dot_tile<DP, NC>(s, q, KV + col * (DP + 4), D);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int p = i0 + ty * 4 + r + off;
-      float mx = m[r];
+      for (int r = 0; r < 4; ++r) {
+        const int p = i0 + ty * 4 + r + off;
+        float mx = m[r];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[r][c] = sees(p, j0 + tx + 16 * c, len, window, sinks) ? s[r][c] * c2 : -INFINITY;
-        mx = fmaxf(mx, s[r][c]);
+        for (int c = 0; c < NC; ++c) {
+          s[r][c] = sees(p, j0 + col + 16 * c, len, window, sinks) ? s[r][c] * c2 : -INFINITY;
+          mx = fmaxf(mx, s[r][c]);
+        }
+        mx = half_warp_max(mx);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        const float corr = exp2f(m[r] - base);
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          s[r][c] = exp2f(s[r][c] - base);
+          sum += s[r][c];
+          w[r * LDP + col + 16 * c] = s[r][c];
+        }
+        l[r] = l[r] * corr + half_warp_sum(sum);
+        m[r] = mx;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) o[r][d] = mul2(o[r][d], make_float2(corr, corr));
       }
-      mx = half_warp_max(mx);
-      const float base = mx == -INFINITY ? 0.f : mx;
-      const float corr = exp2f(m[r] - base);
-      float sum = 0.f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[r][c] = exp2f(s[r][c] - base);
-        sum += s[r][c];
-        W[(ty * 4 + r) * LDP + tx + 16 * c] = s[r][c];
-      }
-      l[r] = l[r] * corr + half_warp_sum(sum);
-      m[r] = mx;
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) o[r][d] *= corr;
-    }
+    });
     __syncthreads();
-    load_tile<DP, T>(KV, a.v, b, hk, j0, len, D);
+    load_tile<BT, DP, T>(KV, a.v, b, hk, j0, len, D);
     wait_tiles();
     __syncthreads();
-    acc_tile<DP>(o, W, KV, ty, tx);
+    acc_tile<DP>(o, w, KV, tx, gr);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -217,7 +277,7 @@ __global__ void __launch_bounds__(NT) attn_fwd_simt_kernel(const gdnx_attn_args 
       for (int e = 0; e < 4; ++e) {
         const int d = g * 64 + tx * 4 + e;
         if (d >= D) continue;
-        const float y = o[r][g * 4 + e] * inv;
+        const float y = part_of(&o[r][g * 2], e) * inv;
         st_from_f32(a.y, a.y_dtype, row + d, y);
         if (a.y_rest) st_from_f32(a.y_rest, a.y_dtype, ((b * a.Tq + i) * a.H + h) * D + d, y - rounded(y, a.y_dtype));
       }
@@ -236,6 +296,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const gdnx_attn_bwd_arg
   float s = 0.f;
   if (i + a.Tk - a.Tq < seq_len(a, b)) {
     const int64_t ry = b * a.y_sb + i * a.y_st + h * a.y_sh, rd = b * g.dy.sb + i * g.dy.st + h * g.dy.sh;
+#pragma unroll 4
     for (int d = lane; d < a.D; d += 32) {
       float y = ld_as_f32(a.y, a.y_dtype, ry + d);
       if (a.y_rest) y += ld_as_f32(a.y_rest, a.y_dtype, ((b * a.Tq + i) * a.H + h) * a.D + d);
@@ -250,56 +311,61 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const gdnx_attn_bwd_arg
 GDNX_DEV float weight(float s, float c2, float lse2) { return exp2f(s * c2 - lse2); }
 
 template <int DP, typename T>
-__global__ void __launch_bounds__(NT) attn_dq_simt_kernel(const gdnx_attn_bwd_args g, const float* delta) {
+__global__ void __launch_bounds__(NT, 2) attn_dq_simt_kernel(const gdnx_attn_bwd_args g, const float* delta) {
   extern __shared__ float sm[];
   const gdnx_attn_args& a = g.fwd;
   float* Q = sm;
-  float* Y = Q + BT * (DP + 4);
-  float* KV = Y + BT * (DP + 4);
-  float* W = KV + BT * (DP + 4);
+  float* Y = Q + BR * (DP + 4);
+  float* K = Y + BR * (DP + 4);
+  float* V = K + BT * (DP + 4);
+  float* W = V + BT * (DP + 4);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const Block blk = block_of(a.H, a.B);
-  const int i0 = ((int)((a.Tq + BT - 1) / BT) - 1 - blk.tile) * BT, D = (int)a.D;
+  const int i0 = ((int)((a.Tq + BR - 1) / BR) - 1 - blk.tile) * BR, D = (int)a.D;
   const int64_t h = blk.h, b = blk.b, hk = h / (a.H / a.Hk);
   const int off = (int)(a.Tk - a.Tq), len = seq_len(a, b);
   const int window = (int)a.window, sinks = (int)a.sinks;
   const float c2 = a.scale * kLog2e;
-  const KeyTiles kt(i0 + off, min(i0 + BT, (int)a.Tq) - 1 + off, len, window, sinks, BT);
+  const KeyTiles kt(i0 + off, min(i0 + BR, (int)a.Tq) - 1 + off, len, window, sinks, BT);
   const int rows = min((int)a.Tq, len - off);
-  load_tile<DP, T>(Q, a.q, b, h, i0, rows, D);
-  load_tile<DP, T>(Y, g.dy, b, h, i0, rows, D);
-  float o[4][DP / 16], lse2[4], dl[4];
+  load_tile<BR, DP, T>(Q, a.q, b, h, i0, rows, D);
+  load_tile<BR, DP, T>(Y, g.dy, b, h, i0, rows, D);
+  const int pw = i0 + off + ty / 2 * 8;  // the warp's first position
+  float* w = W + ty * 4 * LDP;
+  float2 o[4][DP / 32];
+  float lse2[4], dl[4];
+  clear(o);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = i0 + ty * 4 + r;
     lse2[r] = i < rows ? a.lse[(b * a.H + h) * a.Tq + i] * kLog2e : 0.f;
     dl[r] = i < rows ? delta[(b * a.H + h) * a.Tq + i] : 0.f;
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) o[r][d] = 0.f;
   }
   for (int t = 0; t < kt.count; ++t) {
     const int j0 = kt.tile(t) * BT;
-    float dp[4][4], s[4][4];
+    const Groups gr = keys_seen(pw, j0, len, window, sinks);
     __syncthreads();
-    load_tile<DP, T>(KV, a.v, b, hk, j0, len, D);
+    load_tile<BT, DP, T>(K, a.k, b, hk, j0, len, D);
+    load_tile<BT, DP, T>(V, a.v, b, hk, j0, len, D);
     wait_tiles();
     __syncthreads();
-    dot_tile<DP>(dp, Y, KV, ty, tx, D);
-    __syncthreads();
-    load_tile<DP, T>(KV, a.k, b, hk, j0, len, D);
-    wait_tiles();
-    __syncthreads();
-    dot_tile<DP>(s, Q, KV, ty, tx, D);
+    for_groups(gr.n, [&](auto nc) {
+      constexpr int NC = decltype(nc)::value;
+      const int col = 16 * gr.first + tx;
+      float dp[4][4], s[4][4];
+      dot_tile<DP, NC>(s, Q + ty * 4 * (DP + 4), K + col * (DP + 4), D);
+      dot_tile<DP, NC>(dp, Y + ty * 4 * (DP + 4), V + col * (DP + 4), D);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int p = i0 + ty * 4 + r + off;
-        const bool on = sees(p, j0 + tx + 16 * c, len, window, sinks) && !sees_one(p, window, sinks);
-        W[(ty * 4 + r) * LDP + tx + 16 * c] = on ? weight(s[r][c], c2, lse2[r]) * (dp[r][c] - dl[r]) : 0.f;
-      }
-    __syncthreads();
-    acc_tile<DP>(o, W, KV, ty, tx);
+        for (int c = 0; c < NC; ++c) {
+          const int p = i0 + ty * 4 + r + off;
+          const bool on = sees(p, j0 + col + 16 * c, len, window, sinks) && !sees_one(p, window, sinks);
+          w[r * LDP + col + 16 * c] = on ? weight(s[r][c], c2, lse2[r]) * (dp[r][c] - dl[r]) : 0.f;
+        }
+    });
+    __syncwarp();  // a warp's weights are its own
+    acc_tile<DP>(o, w, K, tx, gr);
   }
   T* dq = reinterpret_cast<T*>(g.dq);
 #pragma unroll
@@ -311,70 +377,86 @@ __global__ void __launch_bounds__(NT) attn_dq_simt_kernel(const gdnx_attn_bwd_ar
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = gg * 64 + tx * 4 + e;
-        if (d < D) st_from_f32(dq, a.q.dtype, ((b * a.Tq + i) * a.H + h) * D + d, o[r][gg * 4 + e] * a.scale);
+        if (d < D) st_from_f32(dq, a.q.dtype, ((b * a.Tq + i) * a.H + h) * D + d, part_of(&o[r][gg * 2], e) * a.scale);
       }
   }
 }
 
 template <int DP, typename T>
-__global__ void __launch_bounds__(NT) attn_dkv_simt_kernel(const gdnx_attn_bwd_args g, const float* delta) {
+__global__ void __launch_bounds__(NT, 2) attn_dkv_simt_kernel(const gdnx_attn_bwd_args g, const float* delta) {
   extern __shared__ float sm[];
   const gdnx_attn_args& a = g.fwd;
   float* K = sm;
-  float* V = K + BT * (DP + 4);
-  float* Q = V + BT * (DP + 4);
+  float* V = K + BR * (DP + 4);
+  float* Q = V + BR * (DP + 4);
   float* Y = Q + BT * (DP + 4);
   float* W = Y + BT * (DP + 4);  // P^T, then dS^T: [key][query]
+  float* lse = W + BR * LDP;     // of the tile's queries, in the log2 domain
+  float* dl = lse + BT;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const Block blk = block_of(a.Hk, a.B);
-  const int j0 = blk.tile * BT, D = (int)a.D;
+  const int j0 = blk.tile * BR, D = (int)a.D;
   const int64_t hk = blk.h, b = blk.b, G = a.H / a.Hk;
   const int off = (int)(a.Tk - a.Tq), len = seq_len(a, b);
   const int window = (int)a.window, sinks = (int)a.sinks;
   const float c2 = a.scale * kLog2e;
   const int rows = min((int)a.Tq, len - off);  // queries that are not padding
-  load_tile<DP, T>(K, a.k, b, hk, j0, len, D);
-  load_tile<DP, T>(V, a.v, b, hk, j0, len, D);
-  float dk[4][DP / 16], dv[4][DP / 16];
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) dk[r][d] = dv[r][d] = 0.f;
+  load_tile<BR, DP, T>(K, a.k, b, hk, j0, len, D);
+  load_tile<BR, DP, T>(V, a.v, b, hk, j0, len, D);
+  const int jw = j0 + ty / 2 * 8;  // the warp's first key
+  float* w = W + ty * 4 * LDP;
+  float2 dk[4][DP / 32], dv[4][DP / 32];
+  clear(dk);
+  clear(dv);
   // queries from position j0 on; past the window only where the tile holds sinks
   int lo = max(j0 - off, 0), hi = rows;
-  if (j0 >= sinks) hi = (int)min((int64_t)rows, (int64_t)j0 + BT - 1 + window - off);
+  if (j0 >= sinks) hi = (int)min((int64_t)rows, (int64_t)j0 + BR - 1 + window - off);
   if (j0 >= len) hi = 0;
   for (int64_t h = hk * G; h < (hk + 1) * G; ++h) {
     for (int i0 = lo / BT * BT; i0 < hi; i0 += BT) {
+      const Groups gr = queries_seeing(jw, i0 + off, len, window, sinks);
       __syncthreads();
-      load_tile<DP, T>(Q, a.q, b, h, i0, rows, D);
-      load_tile<DP, T>(Y, g.dy, b, h, i0, rows, D);
+      load_tile<BT, DP, T>(Q, a.q, b, h, i0, rows, D);
+      load_tile<BT, DP, T>(Y, g.dy, b, h, i0, rows, D);
+      if (threadIdx.x < BT) {
+        const int i = i0 + (int)threadIdx.x;
+        const int64_t at = (b * a.H + h) * a.Tq + i;
+        lse[threadIdx.x] = i < rows ? a.lse[at] * kLog2e : 0.f;
+        dl[threadIdx.x] = i < rows ? delta[at] : 0.f;
+      }
       wait_tiles();
       __syncthreads();
-      float s[4][4], dp[4][4];  // [query ty*4+r][key tx+16c]
-      dot_tile<DP>(s, Q, K, ty, tx, D);
-      dot_tile<DP>(dp, Y, V, ty, tx, D);
+      float ds[4][4];
+      for_groups(gr.n, [&](auto nc) {
+        constexpr int NC = decltype(nc)::value;
+        const int col = 16 * gr.first + tx;
+        float s[4][4];  // [key ty*4+r][query]
+        dot_tile<DP, NC>(s, K + ty * 4 * (DP + 4), Q + col * (DP + 4), D);
+        dot_tile<DP, NC>(ds, V + ty * 4 * (DP + 4), Y + col * (DP + 4), D);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = i0 + ty * 4 + r;
-        const float lse2 = i < rows ? a.lse[(b * a.H + h) * a.Tq + i] * kLog2e : 0.f;
-        const float dl = i < rows ? delta[(b * a.H + h) * a.Tq + i] : 0.f;
+        for (int c = 0; c < NC; ++c) {
+          const int p = i0 + off + col + 16 * c;
+          const float lse2 = lse[col + 16 * c], d = dl[col + 16 * c];
+          const bool one = sees_one(p, window, sinks);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float p = sees(i + off, j0 + tx + 16 * c, len, window, sinks) ? weight(s[r][c], c2, lse2) : 0.f;
-          W[(tx + 16 * c) * LDP + ty * 4 + r] = p;
-          s[r][c] = sees_one(i + off, window, sinks) ? 0.f : p * (dp[r][c] - dl);
+          for (int r = 0; r < 4; ++r) {
+            const float x = sees(p, j0 + ty * 4 + r, len, window, sinks) ? weight(s[r][c], c2, lse2) : 0.f;
+            w[r * LDP + col + 16 * c] = x;
+            ds[r][c] = one ? 0.f : x * (ds[r][c] - d);
+          }
         }
-      }
-      __syncthreads();
-      acc_tile<DP>(dv, W, Y, ty, tx);
-      __syncthreads();
+      });
+      __syncwarp();  // a warp's weights are its own
+      acc_tile<DP>(dv, w, Y, tx, gr);
+      __syncwarp();
+      for_groups(gr.n, [&](auto nc) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) W[(tx + 16 * c) * LDP + ty * 4 + r] = s[r][c];
-      __syncthreads();
-      acc_tile<DP>(dk, W, Q, ty, tx);
+          for (int c = 0; c < decltype(nc)::value; ++c) w[r * LDP + 16 * (gr.first + c) + tx] = ds[r][c];
+      });
+      __syncwarp();
+      acc_tile<DP>(dk, w, Q, tx, gr);
     }
   }
 #pragma unroll
@@ -388,16 +470,19 @@ __global__ void __launch_bounds__(NT) attn_dkv_simt_kernel(const gdnx_attn_bwd_a
         const int d = gg * 64 + tx * 4 + e;
         const int64_t at = ((b * a.Tk + j) * a.Hk + hk) * D + d;
         if (d < D) {
-          st_from_f32(g.dk, a.k.dtype, at, dk[r][gg * 4 + e] * a.scale);
-          st_from_f32(g.dv, a.k.dtype, at, dv[r][gg * 4 + e]);
+          st_from_f32(g.dk, a.k.dtype, at, part_of(&dk[r][gg * 2], e) * a.scale);
+          st_from_f32(g.dv, a.k.dtype, at, part_of(&dv[r][gg * 2], e));
         }
       }
   }
 }
 
-constexpr size_t smem_of(int dp, int tiles) { return ((size_t)tiles * BT * (dp + 4) + BT * LDP) * sizeof(float); }
+// Bytes of `own` tiles of a block, `streamed` tiles, the weights and two statistics of a streamed tile's rows.
+constexpr size_t smem_of(int dp, int own, int streamed) {
+  return ((size_t)(own * BR + streamed * BT) * (dp + 4) + BR * LDP + 2 * BT) * sizeof(float);
+}
 
-dim3 blocks(int64_t T, int64_t heads, int64_t B) { return dim3((unsigned)((T + BT - 1) / BT * heads * B)); }
+dim3 blocks(int64_t T, int64_t heads, int64_t B) { return dim3((unsigned)((T + BR - 1) / BR * heads * B)); }
 
 template <typename F>
 gdnx_status run(F kernel, dim3 grid, size_t smem, cudaStream_t st, void** args) {
@@ -414,7 +499,7 @@ gdnx_status fwd(const gdnx_attn_args& a, cudaStream_t st) {
   gdnx_attn_args arg = a;
   void* p[] = {&arg};
   return run(attn_fwd_simt_kernel<DP, T>, blocks(a.Tq, a.H, a.B),
-             smem_of(DP, 2), st, p);
+             smem_of(DP, 1, 1), st, p);
 }
 
 template <int DP, typename T>
@@ -423,10 +508,10 @@ gdnx_status bwd(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st) {
   void* p[] = {&arg, &delta};
   const gdnx_attn_args& a = g.fwd;
   gdnx_status s = run(attn_dq_simt_kernel<DP, T>,
-                      blocks(a.Tq, a.H, a.B), smem_of(DP, 3), st, p);
+                      blocks(a.Tq, a.H, a.B), smem_of(DP, 2, 2), st, p);
   if (s != GDNX_OK) return s;
   return run(attn_dkv_simt_kernel<DP, T>, blocks(a.Tk, a.Hk, a.B),
-             smem_of(DP, 4), st, p);
+             smem_of(DP, 2, 2), st, p);
 }
 
 }  // namespace
