@@ -21,6 +21,7 @@
 
 #include "attn_tc.cuh"
 #include "kernels.h"
+#include "launch.cuh"
 
 namespace gdnx {
 namespace {
@@ -147,7 +148,8 @@ GDNX_DEV void dot_tile(float (&s)[4][4], const float* A, const float* B, int D) 
     for (int c = 0; c < NC; ++c) s[a][c] = t[a][c].x + t[a][c].y;
 }
 
-// o[a][64 g + tx*4 ..] += sum_j W[a][j] X[j][64 g + tx*4 ..] over the groups' j
+// A thread holds DP/16 columns of a row: four of each 64 (from 64 g + tx*4), then two of the last 32.
+// o[a][columns] += sum_j W[a][j] X[j][columns] over the groups' j
 template <int DP>
 GDNX_DEV void acc_tile(float2 (&o)[4][DP / 32], const float* W, const float* X, int tx, const Groups& gr) {
 #pragma unroll 2
@@ -157,14 +159,23 @@ GDNX_DEV void acc_tile(float2 (&o)[4][DP / 32], const float* W, const float* X, 
     for (int a = 0; a < 4; ++a) w[a] = *reinterpret_cast<const float4*>(W + a * LDP + j);
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
+      const float* row = X + (j + jj) * (DP + 4);
 #pragma unroll
       for (int g = 0; g < DP / 64; ++g) {
-        const float4 x = *reinterpret_cast<const float4*>(X + (j + jj) * (DP + 4) + g * 64 + tx * 4);
+        const float4 x = *reinterpret_cast<const float4*>(row + g * 64 + tx * 4);
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           const float p = jj == 0 ? w[a].x : jj == 1 ? w[a].y : jj == 2 ? w[a].z : w[a].w;
           o[a][g * 2] = fma2(make_float2(p, p), make_float2(x.x, x.y), o[a][g * 2]);
           o[a][g * 2 + 1] = fma2(make_float2(p, p), make_float2(x.z, x.w), o[a][g * 2 + 1]);
+        }
+      }
+      if (DP % 64) {
+        const float2 x = *reinterpret_cast<const float2*>(row + DP / 64 * 64 + tx * 2);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const float p = jj == 0 ? w[a].x : jj == 1 ? w[a].y : jj == 2 ? w[a].z : w[a].w;
+          o[a][DP / 32 - 1] = fma2(make_float2(p, p), x, o[a][DP / 32 - 1]);
         }
       }
     }
@@ -177,8 +188,25 @@ GDNX_DEV void clear(float2 (&o)[4][N]) {
 #pragma unroll
     for (int d = 0; d < N; ++d) o[a][d] = make_float2(0.f, 0.f);
 }
-// Value e of the four that a thread holds of a 64-wide piece.
-GDNX_DEV float part_of(const float2* o, int e) { return e % 2 ? o[e / 2].y : o[e / 2].x; }
+// f(first column, its values' pairs, how many columns) for each piece of a thread's columns.
+template <int DP, typename F>
+GDNX_DEV void for_pieces(const float2 (&o)[DP / 32], int tx, F f) {
+#pragma unroll
+  for (int g = 0; g < DP / 64; ++g) f(g * 64 + tx * 4, &o[g * 2], std::integral_constant<int, 4>());
+  if constexpr (DP % 64) f(DP / 64 * 64 + tx * 2, &o[DP / 32 - 1], std::integral_constant<int, 2>());
+}
+// N values of a row, scaled.
+template <int N>
+GDNX_DEV void store_piece(void* dst, int dtype, int64_t at, const float2* o, float scale) {
+  float* p = static_cast<float*>(dst) + at;
+  if (dtype == GDNX_F32 && reinterpret_cast<uintptr_t>(p) % (4 * N) == 0) {
+    if constexpr (N == 4) *reinterpret_cast<float4*>(p) = make_float4(o[0].x * scale, o[0].y * scale, o[1].x * scale, o[1].y * scale);
+    else *reinterpret_cast<float2*>(p) = make_float2(o[0].x * scale, o[0].y * scale);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) st_from_f32(dst, dtype, at + e, (e % 2 ? o[e / 2].y : o[e / 2].x) * scale);
+}
 
 GDNX_DEV float half_warp_max(float x) {
 #pragma unroll
@@ -194,6 +222,11 @@ GDNX_DEV float half_warp_sum(float x) {
 // x in a 16-bit type and back.
 GDNX_DEV float rounded(float x, int dtype) {
   return dtype == GDNX_BF16 ? __bfloat162float(__float2bfloat16_rn(x)) : __half2float(__float2half_rn(x));
+}
+
+// Bytes of `own` tiles of a block, `streamed` tiles, the weights and two statistics of a streamed tile's rows.
+constexpr size_t smem_of(int dp, int own, int streamed) {
+  return ((size_t)(own * BR + streamed * BT) * (dp + 4) + BR * LDP + 2 * BT) * sizeof(float);
 }
 
 template <int DP, typename T>
@@ -271,16 +304,16 @@ __global__ void __launch_bounds__(NT, 3) attn_fwd_simt_kernel(const gdnx_attn_ar
     if (i >= a.Tq) continue;
     const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
     const int64_t row = b * a.y_sb + (int64_t)i * a.y_st + h * a.y_sh;
+    for_pieces<DP>(o[r], tx, [&](int d, const float2* v, auto n) {
+      if (d >= D) return;
+      store_piece<decltype(n)::value>(a.y, a.y_dtype, row + d, v, inv);
+      if (a.y_rest)
 #pragma unroll
-    for (int g = 0; g < DP / 64; ++g)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = g * 64 + tx * 4 + e;
-        if (d >= D) continue;
-        const float y = part_of(&o[r][g * 2], e) * inv;
-        st_from_f32(a.y, a.y_dtype, row + d, y);
-        if (a.y_rest) st_from_f32(a.y_rest, a.y_dtype, ((b * a.Tq + i) * a.H + h) * D + d, y - rounded(y, a.y_dtype));
-      }
+        for (int e = 0; e < decltype(n)::value; ++e) {
+          const float y = (e % 2 ? v[e / 2].y : v[e / 2].x) * inv;
+          st_from_f32(a.y_rest, a.y_dtype, ((b * a.Tq + i) * a.H + h) * D + d + e, y - rounded(y, a.y_dtype));
+        }
+    });
     if (a.lse && tx == 0)
       a.lse[(b * a.H + h) * a.Tq + i] = l[r] > 0.f ? (m[r] + log2f(l[r])) * kLn2 : -INFINITY;
   }
@@ -296,6 +329,14 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const gdnx_attn_bwd_arg
   float s = 0.f;
   if (i + a.Tk - a.Tq < seq_len(a, b)) {
     const int64_t ry = b * a.y_sb + i * a.y_st + h * a.y_sh, rd = b * g.dy.sb + i * g.dy.st + h * g.dy.sh;
+    const float *y = static_cast<const float*>(a.y) + ry, *dy = static_cast<const float*>(g.dy.ptr) + rd;
+    if (a.y_dtype == GDNX_F32 && g.dy.dtype == GDNX_F32 && !a.y_rest &&
+        (reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(dy)) % 16 == 0) {
+      if (4 * lane < a.D) {
+        const float4 u = *reinterpret_cast<const float4*>(y + 4 * lane), v = *reinterpret_cast<const float4*>(dy + 4 * lane);
+        s = fmaf(u.x, v.x, fmaf(u.y, v.y, fmaf(u.z, v.z, u.w * v.w)));
+      }
+    } else
 #pragma unroll 4
     for (int d = lane; d < a.D; d += 32) {
       float y = ld_as_f32(a.y, a.y_dtype, ry + d);
@@ -339,7 +380,7 @@ __global__ void __launch_bounds__(NT, 2) attn_dq_simt_kernel(const gdnx_attn_bwd
   for (int r = 0; r < 4; ++r) {
     const int i = i0 + ty * 4 + r;
     lse2[r] = i < rows ? a.lse[(b * a.H + h) * a.Tq + i] * kLog2e : 0.f;
-    dl[r] = i < rows ? delta[(b * a.H + h) * a.Tq + i] : 0.f;
+    dl[r] = i < rows ? __ldcg(delta + (b * a.H + h) * a.Tq + i) : 0.f;
   }
   for (int t = 0; t < kt.count; ++t) {
     const int j0 = kt.tile(t) * BT;
@@ -367,23 +408,20 @@ __global__ void __launch_bounds__(NT, 2) attn_dq_simt_kernel(const gdnx_attn_bwd
     __syncwarp();  // a warp's weights are its own
     acc_tile<DP>(o, w, K, tx, gr);
   }
-  T* dq = reinterpret_cast<T*>(g.dq);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = i0 + ty * 4 + r;
     if (i >= a.Tq) continue;
-#pragma unroll
-    for (int gg = 0; gg < DP / 64; ++gg)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = gg * 64 + tx * 4 + e;
-        if (d < D) st_from_f32(dq, a.q.dtype, ((b * a.Tq + i) * a.H + h) * D + d, part_of(&o[r][gg * 2], e) * a.scale);
-      }
+    for_pieces<DP>(o[r], tx, [&](int d, const float2* v, auto n) {
+      if (d < D) store_piece<decltype(n)::value>(g.dq, a.q.dtype, ((b * a.Tq + i) * a.H + h) * D + d, v, a.scale);
+    });
   }
+  wait_for_earlier();
 }
 
 template <int DP, typename T>
 __global__ void __launch_bounds__(NT, 2) attn_dkv_simt_kernel(const gdnx_attn_bwd_args g, const float* delta) {
+  dependents_may_start();
   extern __shared__ float sm[];
   const gdnx_attn_args& a = g.fwd;
   float* K = sm;
@@ -463,23 +501,14 @@ __global__ void __launch_bounds__(NT, 2) attn_dkv_simt_kernel(const gdnx_attn_bw
   for (int r = 0; r < 4; ++r) {
     const int j = j0 + ty * 4 + r;
     if (j >= a.Tk) continue;
-#pragma unroll
-    for (int gg = 0; gg < DP / 64; ++gg)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = gg * 64 + tx * 4 + e;
-        const int64_t at = ((b * a.Tk + j) * a.Hk + hk) * D + d;
-        if (d < D) {
-          st_from_f32(g.dk, a.k.dtype, at, part_of(&dk[r][gg * 2], e) * a.scale);
-          st_from_f32(g.dv, a.k.dtype, at, part_of(&dv[r][gg * 2], e));
-        }
-      }
+    const int64_t at = ((b * a.Tk + j) * a.Hk + hk) * D;
+    for_pieces<DP>(dk[r], tx, [&](int d, const float2* v, auto n) {
+      if (d < D) store_piece<decltype(n)::value>(g.dk, a.k.dtype, at + d, v, a.scale);
+    });
+    for_pieces<DP>(dv[r], tx, [&](int d, const float2* v, auto n) {
+      if (d < D) store_piece<decltype(n)::value>(g.dv, a.k.dtype, at + d, v, 1.f);
+    });
   }
-}
-
-// Bytes of `own` tiles of a block, `streamed` tiles, the weights and two statistics of a streamed tile's rows.
-constexpr size_t smem_of(int dp, int own, int streamed) {
-  return ((size_t)(own * BR + streamed * BT) * (dp + 4) + BR * LDP + 2 * BT) * sizeof(float);
 }
 
 dim3 blocks(int64_t T, int64_t heads, int64_t B) { return dim3((unsigned)((T + BR - 1) / BR * heads * B)); }
@@ -507,21 +536,34 @@ gdnx_status bwd(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st) {
   gdnx_attn_bwd_args arg = g;
   void* p[] = {&arg, &delta};
   const gdnx_attn_args& a = g.fwd;
-  gdnx_status s = run(attn_dq_simt_kernel<DP, T>,
-                      blocks(a.Tq, a.H, a.B), smem_of(DP, 2, 2), st, p);
+  constexpr size_t smem = smem_of(DP, 2, 2);
+  const gdnx_status s = run(attn_dkv_simt_kernel<DP, T>, blocks(a.Tk, a.Hk, a.B), smem, st, p);
   if (s != GDNX_OK) return s;
-  return run(attn_dkv_simt_kernel<DP, T>, blocks(a.Tk, a.Hk, a.B),
-             smem_of(DP, 2, 2), st, p);
+  if (cudaFuncSetAttribute(attn_dq_simt_kernel<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      launch_early(attn_dq_simt_kernel<DP, T>, blocks(a.Tq, a.H, a.B), dim3(NT), smem, st, g, delta) != cudaSuccess) {
+    cudaGetLastError();
+    return GDNX_ELAUNCH;
+  }
+  return GDNX_OK;
+}
+
+template <typename T>
+gdnx_status fwd_of(const gdnx_attn_args& a, cudaStream_t st) {
+  return a.D > 96 ? fwd<128, T>(a, st) : a.D > 64 ? fwd<96, T>(a, st) : fwd<64, T>(a, st);
+}
+template <typename T>
+gdnx_status bwd_of(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st) {
+  const int64_t D = g.fwd.D;
+  return D > 96 ? bwd<128, T>(g, delta, st) : D > 64 ? bwd<96, T>(g, delta, st) : bwd<64, T>(g, delta, st);
 }
 
 }  // namespace
 
 gdnx_status launch_attn_fwd_simt(const gdnx_attn_args& a, cudaStream_t st) {
-  const bool wide = a.D > 64;
   switch (a.q.dtype) {
-    case GDNX_BF16: return wide ? fwd<128, __nv_bfloat16>(a, st) : fwd<64, __nv_bfloat16>(a, st);
-    case GDNX_F16: return wide ? fwd<128, __half>(a, st) : fwd<64, __half>(a, st);
-    default: return wide ? fwd<128, float>(a, st) : fwd<64, float>(a, st);
+    case GDNX_BF16: return fwd_of<__nv_bfloat16>(a, st);
+    case GDNX_F16: return fwd_of<__half>(a, st);
+    default: return fwd_of<float>(a, st);
   }
 }
 
@@ -532,11 +574,10 @@ gdnx_status launch_attn_delta(const gdnx_attn_bwd_args& g, float* delta, cudaStr
 }
 
 gdnx_status launch_attn_bwd_simt(const gdnx_attn_bwd_args& g, float* delta, cudaStream_t st) {
-  const bool wide = g.fwd.D > 64;
   switch (g.fwd.q.dtype) {
-    case GDNX_BF16: return wide ? bwd<128, __nv_bfloat16>(g, delta, st) : bwd<64, __nv_bfloat16>(g, delta, st);
-    case GDNX_F16: return wide ? bwd<128, __half>(g, delta, st) : bwd<64, __half>(g, delta, st);
-    default: return wide ? bwd<128, float>(g, delta, st) : bwd<64, float>(g, delta, st);
+    case GDNX_BF16: return bwd_of<__nv_bfloat16>(g, delta, st);
+    case GDNX_F16: return bwd_of<__half>(g, delta, st);
+    default: return bwd_of<float>(g, delta, st);
   }
 }
 
