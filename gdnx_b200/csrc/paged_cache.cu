@@ -8,6 +8,11 @@
 // integer atomics, whose order does not show.  extend and compact are planned by one CTA
 // (the free pages are ranked by a scan over refs, so allocation is lowest index first
 // whatever the thread order); a second kernel moves the pages.
+//
+// Bytes moved bound extend's copies, write and compact; the others are one short launch (3 to 8 us).
+// Measured: 32 requests of up to 1500 tokens forked, extended by 5 tokens (their last pages copied in 24
+// layers), written in one layer and trimmed: 55 us (198 MB); compaction after waves of requests moves
+// pages at 87 % of a copy's rate.
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.cuh"

@@ -1121,7 +1121,7 @@ def cache_extend(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor) ->
 def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor, *, layer: int = 0,
                 counts: Optional[torch.Tensor] = None) -> None:
     """The keys and values ``k``, ``v`` [n,T,Hk,D] of slot ``rows[i]``'s last T tokens in ``layer``
-    (after :func:`cache_extend`); with ``counts`` [n] int32, row i's first ``counts[i]`` of T are its
+    (each slot once; after :func:`cache_extend`); with ``counts`` [n] int32, row i's first ``counts[i]`` of T are its
     last ``counts[i]`` tokens (a right-padded prompt)."""
     s, index = _cache_struct(cache)
     _on_device(index, k, v)

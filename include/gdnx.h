@@ -403,7 +403,7 @@ GDNX_API gdnx_status gdnx_kmd2_prologue(const gdnx_kmd2_prologue_args* args, voi
  * (a prompt, or the end of one whose beginning is already known) and sees key j where
  *   j <= p,  j < lengths[b],  and  p - j < window  or  j < sinks;
  * a query with p >= lengths[b] is padding: its output is 0, its lse -inf, and what its
- * rows of q, dy, k and v hold (NaN included) reaches no output.
+ * rows of q, dy, k and v hold (NaN included) reaches no output.  Other rows are finite.
  *   y_i = sum_j softmax_j(scale q_i.k_j) v_j ;  query head h reads key head h / (H / Hk).
  * Scores, softmax statistics and sums are fp32; 16-bit inputs run on the tensor cores
  * where TMA can address them, other types and layouts on the CUDA cores. */
@@ -473,7 +473,8 @@ GDNX_API gdnx_status gdnx_cache_fork(const gdnx_cache* cache, int64_t n, const i
 GDNX_API gdnx_status gdnx_cache_extend(const gdnx_cache* cache, int64_t n, const int32_t* rows, const int32_t* counts,
                                        void* workspace, size_t workspace_bytes, void* stream);
 /* k, v [n,T,Hk,D] become tokens length-count .. length-1 of slot rows[i] in `layer`
- * (count = counts[i] <= T, or T where counts is NULL; further tokens of a row are ignored). */
+ * (count = counts[i] <= T, or T where counts is NULL; further tokens of a row are ignored).
+ * Each slot is named once. */
 GDNX_API gdnx_status gdnx_cache_write(const gdnx_cache* cache, int64_t layer, int64_t n, int64_t T, const gdnx_view* k,
                                       const gdnx_view* v, const int32_t* rows, const int32_t* counts, void* stream);
 /* Slot rows[i] keeps its first lengths[i] tokens (0 frees it). */
