@@ -8,9 +8,9 @@
 // more than 8 above (p stays below 2^8), so a tile costs one vote and no reduction; sums stay
 // in the threads until the unit ends.
 //
-// Measured: 64 sequences of up to 8192 tokens, 16 heads over 4 of 128, pages of 64: 96 us, 5.6 TB/s of
+// Measured: 64 sequences of up to 8192 tokens, 16 heads over 4 of 128, pages of 64: 94 us, 5.7 TB/s of
 // the copy's 6.5; one sequence of 262,144 tokens over 2 key heads: 57 us, 4.7 TB/s (its start and the
-// join take 10 us); 256 sequences whose window of 1024 is read from pages of 32: 109 us.
+// join take 10 us); 256 sequences whose window of 1024 is read from pages of 32: 102 us.
 //
 // Pages come by TMA, one box for each page and 64 dims; pages that hold nothing visible are not
 // fetched.  Rows that are not visible are masked in S and zeroed in V, since what unwritten
@@ -292,8 +292,8 @@ GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, ui
         ok = warp_wait(&bar.full[sl], vc / Lo::SLOTS & 1, abort_flag);
         if (!seen && ok)
 #pragma unroll
-          for (int c = 0; c < DB * 8; ++c)
-            *reinterpret_cast<uint4*>(base + Lo::RING + sl * Lo::TILE + (c / 8) * BLOCK_BYTES + r * 128 + c % 8 * 16) =
+          for (int c = 0; c < DB * 8; ++c)  // rows begin at different pieces: no bank conflicts
+            *reinterpret_cast<uint4*>(base + Lo::RING + sl * Lo::TILE + (c / 8) * BLOCK_BYTES + r * 128 + ((c ^ r) & 7) * 16) =
                 make_uint4(0, 0, 0, 0);
       }
       tc::fence_async_smem();
