@@ -318,10 +318,11 @@ GDNX_DEV void run_products(const FwdParams& P, uint32_t smem, uint32_t tmem, Bar
   for (int64_t n = blockIdx.x; n < P.items; n += gridDim.x) {
     const Item w = make_item(P, n);
     if (w.count == 0) continue;
-    bool begun[2] = {false, false}, pend[2] = {false, false}, acc[2] = {false, false};
+    bool begun[2] = {false, false}, pend[2] = {false, false}, acc[2] = {false, false}, last[2] = {false, false};
     uint32_t old = 0;      // V's slot of the tile before
     for (int i = 0; i <= w.count; ++i) {
       const bool more = i < w.count;
+      // stage 1 may see the sinks' tile and not the next one: its last tile ends it, not its first gap
       const int kt = more ? w.tile(i) : 1 << 29;
       const uint32_t ksl = cnt % Lo::SLOTS, k = smem + Lo::KV + ksl * Lo::TILE, v = smem + Lo::KV + old * Lo::TILE;
       if (more && !warp_wait(&bar.kv_full[ksl], cnt / Lo::SLOTS & 1, abort_flag)) return;
@@ -342,7 +343,7 @@ GDNX_DEV void run_products(const FwdParams& P, uint32_t smem, uint32_t tmem, Bar
         if (elect_one()) {
           if (pend[st]) {
             mma_px<4>(tO, tS + 32, v + 64 * 128, ID_O, true);
-            if (!on) tc::commit(&bar.o_full[st]);  // a stage's tiles have no gap
+            if (last[st]) tc::commit(&bar.o_full[st]);
           }
           if (st == 1 && i > 0) tc::commit(&bar.kv_empty[old]);
           if (on) {
@@ -356,6 +357,7 @@ GDNX_DEV void run_products(const FwdParams& P, uint32_t smem, uint32_t tmem, Bar
         acc[st] = acc[st] || pend[st];
         begun[st] = begun[st] || on;
         pend[st] = on;
+        last[st] = kt == w.hi(st);
       }
       old = (cnt + 1) % Lo::SLOTS;
       if (more) cnt += 2;
@@ -446,12 +448,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
   tc::fence_after();
   const uint32_t tmem = uniform(sm.tmem_at);
   if (smem % 1024) {  // never entered: the base is aligned
-  } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 232 + 128 x 40 is just that
-    regs_up<232>();
+  } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 224 + 128 x 56 is just that
+    regs_up<224>();
     run_rows<DB, BF16, REST>(P, base, tmem, bar, abort_flag);
     if (threadIdx.x % 32 == 0) pipe::bulk_wait_all();
   } else {
-    regs_down<40>();
+    regs_down<56>();
     if (warp == 8) {
       run_products<DB, BF16>(P, smem, tmem, bar, abort_flag);
       __syncwarp();

@@ -72,6 +72,27 @@ def test_attention_and_gradients(shape, dtype):
     check(*make(B, Tq, Tk, H, Hk, D, dtype, seed=Tk), dtype, window=window, sinks=sinks)
 
 
+ODD = [  # an odd number of query heads for each key head: two consecutive blocks of queries share their tiles, and the
+    # second sees the sinks' tile but not the first of the window's; more items than SMs
+    (1, 3000, 3000, 16, 16, 64, 200, 4),
+    (3, 1100, 1100, 16, 16, 128, 130, 17),
+    (2, 2200, 2500, 15, 5, 96, 700, 130),
+    (1, 2600, 2600, 5, 1, 32, 60, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", ODD, ids=str)
+def test_blocks_that_share_tiles_with_a_gap(shape, dtype):
+    B, Tq, Tk, H, Hk, D, window, sinks = shape
+    q, k, v, dy = make(B, Tq, Tk, H, Hk, D, dtype, seed=Tk)
+    lengths = torch.arange(Tk, Tk - 70 * B, -70, device=DEV, dtype=torch.int32)
+    for _ in range(3):
+        check(q, k, v, None, dtype, window=window, sinks=sinks, lengths=lengths)
+    check(q, k, v, dy, dtype, window=window, sinks=sinks, lengths=lengths)
+    assert ops.device_status() == 0
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("Tq,Tk,D", [(260, 260, 128), (70, 260, 64)])
 def test_padding_holds_nan_and_reaches_nothing(Tq, Tk, D, dtype):
