@@ -22,12 +22,19 @@
 // P is rounded to the inputs' type, the error of which averages out over the keys like the
 // inputs' own rounding; l sums it unrounded in fp32.
 //
+// Items that do not fill a last round of the SMs go to a second kernel where they are at most half a
+// round, which starts as the first one's blocks leave SMs free: each block of queries has a CTA to itself, the
+// two stages take its key tiles in turn and stage 0 joins the two outputs, in tensor memory both.  That
+// is the whole work of a single short prompt (1024 tokens, 16 heads: 23 -> 17 us; 512 tokens after 7680,
+// window 4096: 68 -> 44 us), and balances long ones (8192 after 8192: 262 -> 246 us).
+//
 // Measured: 8 x 4096 tokens, 16 heads over 4 of 128, window 1024, 4 sinks, bf16: 272 us (888 TFLOP/s of
 // visible pairs, 53 % of a large matrix product's rate; 317 us at the 1.69 GHz of a sustained run); 8192
-// tokens after 8192, window 4096: 262 us (1066 TFLOP/s).  A pair of tiles takes the tensor cores 2048
+// tokens after 8192, window 4096: 246 us (1135 TFLOP/s).  A pair of tiles takes the tensor cores 2048
 // cycles and lasts 3350: each stage's rows take longer than the other stage's products.
 #include "attn_tc.cuh"
 #include "kernels.h"
+#include "launch.cuh"
 
 namespace gdnx {
 namespace {
@@ -40,7 +47,8 @@ constexpr uint32_t T_S = 0, T_O = 256;  // tensor-memory columns: S_0, S_1, then
 struct FwdParams {
   TileMap q, k, v, y, rest;
   gdnx_attn_args a;
-  int64_t items;
+  int64_t items;               // pairs of blocks for the first kernel
+  int split;                   // pairs that the second kernel takes, block by block
   int tma_y;                   // 16-bit outputs leave through shared memory and TMA
   int pairs, units, by_heads;  // stage pairs of a key head; blocks (or block pairs) of queries
 };
@@ -93,8 +101,27 @@ GDNX_DEV Item make_item(const FwdParams& P, int64_t item) {
   return w;
 }
 
+// The second kernel's item: one block of the last pairs, whose key tiles the two stages take in turn
+// (tile i by stage i % 2).
+GDNX_DEV Item split_item(const FwdParams& P) {
+  Item w = make_item(P, P.items + blockIdx.x / 2);
+  if (blockIdx.x & 1) {
+    w.h0 += w.dh;
+    w.i0 += w.di;
+    const int p0 = w.i0 + w.off, p1 = min(w.i0 + TM, w.Tq) - 1 + w.off;
+    w.lo0 = max(0, p0 - (int)P.a.window + 1) / TM;
+    w.hi0 = w.i0 < w.Tq && p0 < w.len ? min(p1, w.len - 1) / TM : -1;
+  }
+  w.dh = w.di = 0;
+  w.lo1 = w.lo0;
+  w.hi1 = w.hi0;
+  w.nsink = min(w.nst, w.lo0);
+  w.count = w.hi0 < 0 ? 0 : w.nsink + w.hi0 - w.lo0 + 1;
+  return w;
+}
+
 struct Bars {
-  uint64_t kv_full[8], kv_empty[8], q_full[2], q_empty[2], s_full[2], p_ready[2][2], o_full[2], fix, done;
+  uint64_t kv_full[8], kv_empty[8], q_full[2], q_empty[2], s_full[2], p_ready[2][2], o_full[2], fix, done, merge;
 };
 
 struct Small {
@@ -183,7 +210,7 @@ GDNX_DEV void pack_row(uint32_t* u, const float* o, int dtype) {
 }
 
 // One stage's rows, one for each thread.
-template <int DB, bool BF16, bool REST>
+template <int DB, bool BF16, bool REST, bool SPLIT>
 GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
   using Lo = Layout<DB>;
   const gdnx_attn_args& a = P.a;
@@ -194,12 +221,12 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
   const float c2 = a.scale * kLog2e;
   uint8_t* out = base + Lo::OUT + warp * 4096;
   uint32_t nS = 0, nO = 0;
-  for (int64_t n = blockIdx.x; n < P.items; n += gridDim.x) {
-    const Item w = make_item(P, n);
+  for (int64_t n = blockIdx.x; n < (SPLIT ? gridDim.x : P.items); n += gridDim.x) {
+    const Item w = SPLIT ? split_item(P) : make_item(P, n);
     if (!w.valid(st)) continue;
     const int i0 = w.row(st), head = w.head(st), p0 = i0 + w.off, p = p0 + r;
     Row row = {-INFINITY, 0.f};
-    for (int i = 0; i < w.count; ++i) {
+    for (int i = SPLIT ? st : 0; i < w.count; i += SPLIT ? 2 : 1) {
       const int kt = w.tile(i), j0 = kt * TM;
       if (!w.active(st, kt)) continue;
       if (!warp_wait(&bar.s_full[st], nS++ & 1, abort_flag)) return;
@@ -262,9 +289,29 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
       }
       row.l += sum.x + sum.y;
     }
-    if (w.hi(st) >= 0) {
+    if (SPLIT ? w.count > st : w.hi(st) >= 0) {
       if (!warp_wait(&bar.o_full[st], nO++ & 1, abort_flag)) return;
       tc::fence_after();
+    }
+    float f0 = 1.f, f1 = 0.f;  // SPLIT: the stages' factors
+    if (SPLIT) {  // stage 1 leaves its maximum and sum in its staging rows, stage 0 reads both outputs
+      float2* other = reinterpret_cast<float2*>(base + Lo::OUT + 4 * 4096) + r;
+      if (st == 1) {
+        *other = make_float2(row.m, row.l);
+        pipe::mbar_arrive(&bar.merge);
+        return;
+      }
+      if (!warp_wait(&bar.merge, 0, abort_flag)) return;
+      if (w.count > 1) {
+        if (!warp_wait(&bar.o_full[1], 0, abort_flag)) return;
+        tc::fence_after();
+        const float2 x = *other;
+        const float m = fmaxf(row.m, x.x);
+        f0 = row.m == -INFINITY ? 0.f : ex2((row.m - m) * c2);
+        f1 = x.x == -INFINITY ? 0.f : ex2((x.x - m) * c2);
+        row.m = m;
+        row.l = row.l * f0 + x.y * f1;
+      }
     }
     const float l = p < w.len ? row.l : 0.f;  // padding
     const int i = i0 + r, row0 = i0 + r / 32 * 32;
@@ -273,6 +320,12 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
     for (int d = 0; d < 64 * DB; d += 64) {
       float o[64];
       if (w.hi(st) >= 0) tmem_ld64(tO + d, o);
+      if (SPLIT && w.count > 1) {
+        float x[64];
+        tmem_ld64(tO + 128 + d, x);
+#pragma unroll
+        for (int e = 0; e < 64; ++e) o[e] = o[e] * f0 + x[e] * f1;
+      }
 #pragma unroll
       for (int e = 0; e < 64; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
       if (P.tma_y) {
@@ -365,6 +418,98 @@ GDNX_DEV void run_products(const FwdParams& P, uint32_t smem, uint32_t tmem, Bar
   }
 }
 
+// The same for a split item: step t holds tile 2t of stage 0 and 2t + 1 of stage 1, places 4t and
+// 4t + 1 of the ring their K, the next two their V.
+template <int DB, bool BF16>
+GDNX_DEV void split_products(const FwdParams& P, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+  using Lo = Layout<DB>;
+  constexpr uint32_t ID_S = idesc16(BF16, 128, 128, false, false), ID_O = idesc16(BF16, 128, 64 * DB, false, true);
+  const Item w = split_item(P);
+  if (w.count == 0 || !warp_wait(&bar.q_full[0], 0, abort_flag)) return;
+  for (int t = 0; t <= (w.count + 1) / 2; ++t) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const uint32_t tS = tmem + T_S + st * 128, tO = tmem + T_O + st * 128;
+      const bool pv = t > 0 && 2 * t - 2 + st < w.count, on = 2 * t + st < w.count;
+      const uint32_t kp = 4 * t + st, vp = kp - 2u, ksl = kp % Lo::SLOTS, vsl = vp % Lo::SLOTS;
+      const uint32_t k = smem + Lo::KV + ksl * Lo::TILE, v = smem + Lo::KV + vsl * Lo::TILE;
+      if (on && !warp_wait(&bar.kv_full[ksl], kp / Lo::SLOTS & 1, abort_flag)) return;
+      if (pv) {
+        if (!warp_wait(&bar.kv_full[vsl], vp / Lo::SLOTS & 1, abort_flag)) return;
+        if (!warp_wait(&bar.p_ready[st][0], (t - 1) & 1, abort_flag)) return;
+        tc::fence_after();
+        if (elect_one()) mma_px<4>(tO, tS, v, ID_O, t > 1);
+        __syncwarp();
+        if (!warp_wait(&bar.p_ready[st][1], (t - 1) & 1, abort_flag)) return;
+      }
+      tc::fence_after();
+      if (elect_one()) {
+        if (pv) {
+          mma_px<4>(tO, tS + 32, v + 64 * 128, ID_O, true);
+          tc::commit(&bar.kv_empty[vsl]);
+          if (!on) tc::commit(&bar.o_full[st]);
+        }
+        if (on) {
+          mma_abt<DB>(tS, smem + Lo::Q, k, ID_S);
+          tc::commit(&bar.s_full[st]);
+          tc::commit(&bar.kv_empty[ksl]);
+        }
+      }
+      __syncwarp();
+    }
+  }
+}
+
+// One tile of K or V (whole warp), padding rows of V to zero: they meet weights of 0, so they must not hold NaN.
+template <int DB>
+GDNX_DEV bool load_kv(const FwdParams& P, const Item& w, int side, int j0, uint32_t place, uint8_t* base, uint32_t smem,
+                      Bars& bar, volatile int* abort_flag, uint32_t& nfix) {
+  using Lo = Layout<DB>;
+  const int lane = threadIdx.x % 32;
+  const uint32_t sl = place % Lo::SLOTS, dst = smem + Lo::KV + sl * Lo::TILE;
+  if (!warp_wait(&bar.kv_empty[sl], (place / Lo::SLOTS & 1) ^ 1, abort_flag)) return false;
+  const bool fix = side == 1 && w.len < P.a.Tk && j0 + TM > w.len;
+  if (lane == 0) {
+    const uint32_t mb = tc::smem_u32(fix ? &bar.fix : &bar.kv_full[sl]);
+    pipe::expect_tx(mb, Lo::TILE);
+    load_rows<DB>(dst, side ? P.v : P.k, j0, w.hk, w.b, mb);
+  }
+  if (fix) {
+    if (!warp_wait(&bar.fix, nfix++ & 1, abort_flag)) return false;
+    for (int x = lane; x < (j0 + TM - w.len) * DB * 8; x += 32) {
+      const int row = w.len - j0 + x / (DB * 8), c = x % (DB * 8);
+      *reinterpret_cast<uint4*>(base + Lo::KV + sl * Lo::TILE + (c / 8) * BLOCK_BYTES + row * 128 + c % 8 * 16) =
+          make_uint4(0, 0, 0, 0);
+    }
+    tc::fence_async_smem();
+    __syncwarp();
+    if (lane == 0) pipe::mbar_arrive(&bar.kv_full[sl]);
+  }
+  return true;
+}
+
+// Loads of a split item.
+template <int DB>
+GDNX_DEV void split_loads(const FwdParams& P, uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag,
+                          uint32_t& issued) {
+  using Lo = Layout<DB>;
+  const Item w = split_item(P);
+  uint32_t nfix = 0;
+  for (int t = 0; 2 * t < w.count; ++t)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = 2 * t + x % 2, side = x / 2;
+      if (i >= w.count) continue;
+      if (!load_kv<DB>(P, w, side, w.tile(i) * TM, 4 * t + x, base, smem, bar, abort_flag, nfix)) return;
+      issued = 4 * t + x + 1;
+      if (t == 0 && x == 0 && threadIdx.x % 32 == 0) {
+        const uint32_t mb = tc::smem_u32(&bar.q_full[0]);
+        pipe::expect_tx(mb, Lo::TILE);
+        load_rows<DB>(smem + Lo::Q, P.q, w.i0, w.h0, w.b, mb);
+      }
+    }
+}
+
 // The warp that loads: K(0), Q, V(0), K(1), V(1), ... of each item.
 template <int DB>
 GDNX_DEV void run_loads(const FwdParams& P, uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag,
@@ -378,26 +523,7 @@ GDNX_DEV void run_loads(const FwdParams& P, uint8_t* base, uint32_t smem, Bars& 
       const int j0 = w.tile(i) * TM;
 #pragma unroll
       for (int side = 0; side < 2; ++side, ++cnt) {
-        const uint32_t sl = cnt % Lo::SLOTS, dst = smem + Lo::KV + sl * Lo::TILE;
-        if (!warp_wait(&bar.kv_empty[sl], (cnt / Lo::SLOTS & 1) ^ 1, abort_flag)) return;
-        // padding rows of V meet weights of 0, so they must not hold NaN
-        const bool fix = side == 1 && w.len < P.a.Tk && j0 + TM > w.len;
-        if (lane == 0) {
-          const uint32_t mb = tc::smem_u32(fix ? &bar.fix : &bar.kv_full[sl]);
-          pipe::expect_tx(mb, Lo::TILE);
-          load_rows<DB>(dst, side ? P.v : P.k, j0, w.hk, w.b, mb);
-        }
-        if (fix) {
-          if (!warp_wait(&bar.fix, nfix++ & 1, abort_flag)) return;
-          for (int x = lane; x < (j0 + TM - w.len) * DB * 8; x += 32) {
-            const int row = w.len - j0 + x / (DB * 8), c = x % (DB * 8);
-            *reinterpret_cast<uint4*>(base + Lo::KV + sl * Lo::TILE + (c / 8) * BLOCK_BYTES + row * 128 + c % 8 * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          tc::fence_async_smem();
-          __syncwarp();
-          if (lane == 0) pipe::mbar_arrive(&bar.kv_full[sl]);
-        }
+        if (!load_kv<DB>(P, w, side, j0, cnt, base, smem, bar, abort_flag, nfix)) return;
         issued = cnt + 1;
         if (i == 0 && side == 0) {
 #pragma unroll
@@ -416,7 +542,7 @@ GDNX_DEV void run_loads(const FwdParams& P, uint8_t* base, uint32_t smem, Bars& 
   }
 }
 
-template <int DB, bool BF16, bool REST>
+template <int DB, bool BF16, bool REST, bool SPLIT>
 __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_constant__ FwdParams P) {
   using Lo = Layout<DB>;
   extern __shared__ __align__(1024) uint8_t base[];
@@ -425,6 +551,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
   volatile int* abort_flag = &sm.abort_flag;
   const uint32_t smem = uniform(tc::smem_u32(base));
   const int warp = uniform(threadIdx.x / 32);
+  if (!SPLIT) dependents_may_start();
   if (threadIdx.x == 0) {
     *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
     for (int i = 0; i < 8; ++i) {
@@ -441,6 +568,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
     }
     tc::mbar_init(&bar.fix, 1);
     tc::mbar_init(&bar.done, 1);
+    tc::mbar_init(&bar.merge, 128);
   }
   if (warp == 8) tc::tmem_alloc(&sm.tmem_at, 512);
   tc::fence_before();
@@ -450,18 +578,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
   if (smem % 1024) {  // never entered: the base is aligned
   } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 224 + 128 x 56 is just that
     regs_up<224>();
-    run_rows<DB, BF16, REST>(P, base, tmem, bar, abort_flag);
+    run_rows<DB, BF16, REST, SPLIT>(P, base, tmem, bar, abort_flag);
     if (threadIdx.x % 32 == 0) pipe::bulk_wait_all();
   } else {
     regs_down<56>();
     if (warp == 8) {
-      run_products<DB, BF16>(P, smem, tmem, bar, abort_flag);
+      if (SPLIT) split_products<DB, BF16>(P, smem, tmem, bar, abort_flag);
+      else run_products<DB, BF16>(P, smem, tmem, bar, abort_flag);
       __syncwarp();
       if (elect_one()) tc::commit(&bar.done);  // every product issued has ended before tensor memory is freed
       tc::mbar_wait(&bar.done, 0);
     } else if (warp == 9) {
       uint32_t issued = 0;
-      run_loads<DB>(P, base, smem, bar, abort_flag, issued);
+      if (SPLIT) split_loads<DB>(P, base, smem, bar, abort_flag, issued);
+      else run_loads<DB>(P, base, smem, bar, abort_flag, issued);
       if (*abort_flag && threadIdx.x % 32 == 0) {  // let the copies in flight land
         for (uint32_t c = issued > Lo::SLOTS ? issued - Lo::SLOTS : 0; c < issued; ++c)
           tc::mbar_wait(&bar.kv_full[c % Lo::SLOTS], c / Lo::SLOTS & 1, 1u << 16);
@@ -475,15 +605,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_fwd_tc_kernel(const __grid_c
   tc::fence_after();
   if (warp == 8) tc::tmem_dealloc(tmem, 512);
   if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
+  if (SPLIT) wait_for_earlier();  // what follows may rely on both kernels
 }
 
 template <int DB, bool BF16, bool REST>
 gdnx_status launch(const FwdParams& P, int sms, cudaStream_t st) {
-  const auto kernel = attn_fwd_tc_kernel<DB, BF16, REST>;
-  static std::atomic<uint64_t> done;
-  if (!allow_smem(kernel, (int)Layout<DB>::SMEM, done)) return GDNX_ELAUNCH;
-  const unsigned grid = (unsigned)(P.items < sms ? P.items : sms);
-  kernel<<<grid, NTHREADS, Layout<DB>::SMEM, st>>>(P);
+  const auto whole = attn_fwd_tc_kernel<DB, BF16, REST, false>, split = attn_fwd_tc_kernel<DB, BF16, REST, true>;
+  constexpr int smem = (int)Layout<DB>::SMEM;
+  static std::atomic<uint64_t> done_whole, done_split;
+  if (!allow_smem(whole, smem, done_whole) || !allow_smem(split, smem, done_split)) return GDNX_ELAUNCH;
+  if (P.items > 0) whole<<<(unsigned)(P.items < sms ? P.items : sms), NTHREADS, smem, st>>>(P);
+  if (cudaGetLastError() != cudaSuccess) return GDNX_ELAUNCH;
+  if (P.split > 0 && P.items > 0)  // starts as the first kernel's blocks leave SMs free
+    return launch_early(split, dim3((unsigned)(2 * P.split)), dim3(NTHREADS), smem, st, P) == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
+  if (P.split > 0) split<<<(unsigned)(2 * P.split), NTHREADS, smem, st>>>(P);
   return cudaGetLastError() == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
 }
 
@@ -518,6 +653,11 @@ gdnx_status launch_attn_fwd_tc(const gdnx_attn_args& a, cudaStream_t st) {
   P.items = (int64_t)P.units * a.B * a.Hk * P.pairs;
   if (P.items >= ((int64_t)1 << 31)) return GDNX_EUNSUPPORTED;
   const int sms = sm_count();
+  // Pairs that do not fill a last round of the SMs: where they are at most half of them, each block has
+  // an SM to itself and its keys are split over the two stages (half a pair's time instead of a whole).
+  const int rest = (int)(P.items % sms);
+  P.split = 2 * rest <= sms ? rest : 0;
+  P.items -= P.split;
   const bool bf16 = a.q.dtype == GDNX_BF16;
   if (a.D > 64) return bf16 ? launch<2, true>(P, sms, st) : launch<2, false>(P, sms, st);
   return bf16 ? launch<1, true>(P, sms, st) : launch<1, false>(P, sms, st);

@@ -93,6 +93,29 @@ def test_blocks_that_share_tiles_with_a_gap(shape, dtype):
     assert ops.device_status() == 0
 
 
+FEW = [  # few enough blocks that each has a CTA of its own (one tile, an odd number of them, sinks apart from the window;
+    # one block too many for that), and a last round that is nearly empty
+    (1, 128, 128, 2, 2, 128, 50, 0),
+    (1, 300, 300, 1, 1, 64, 300, 0),
+    (1, 257, 900, 4, 2, 96, 130, 7),
+    (2, 640, 640, 8, 2, 128, 4000, 4),
+    (1, 128, 700, 149, 1, 64, 200, 3),
+    (1, 1280, 1280, 30, 15, 128, 60, 4),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", FEW, ids=str)
+def test_blocks_whose_keys_are_split(shape, dtype):
+    B, Tq, Tk, H, Hk, D, window, sinks = shape
+    q, k, v, dy = make(B, Tq, Tk, H, Hk, D, dtype, seed=Tq)
+    lengths = torch.arange(Tk, Tk - 70 * B, -70, device=DEV, dtype=torch.int32)
+    check(q, k, v, dy, dtype, window=window, sinks=sinks, lengths=lengths)
+    empty = torch.zeros(B, device=DEV, dtype=torch.int32)
+    assert not ops.window_attention(q, k, v, window=window, sinks=sinks, lengths=empty).any()
+    assert ops.device_status() == 0
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("Tq,Tk,D", [(260, 260, 128), (70, 260, 64)])
 def test_padding_holds_nan_and_reaches_nothing(Tq, Tk, D, dtype):
