@@ -93,7 +93,7 @@ gdnx_status check_attn_sizes(const gdnx_attn_args& a) {
   if (a.H % a.Hk || a.window < 1 || a.sinks < 0) return GDNX_EINVAL;
   if (!(a.scale > 0.f) || a.scale > 3.0e38f || !dtype_ok(a.q.dtype) || !dtype_ok(a.y_dtype)) return GDNX_EINVAL;
   if (a.D > 128 || a.D % 8 || a.Tk > kMaxTokens || a.B > 65535 || a.H > 65535) return GDNX_EUNSUPPORTED;
-  if (a.B * a.H * ((a.Tk + 63) / 64) >= ((int64_t)1 << 31)) return GDNX_EUNSUPPORTED;  // blocks of a grid
+  if (a.B * a.H * ((a.Tk + 31) / 32) >= ((int64_t)1 << 31)) return GDNX_EUNSUPPORTED;  // blocks of a grid
   return GDNX_OK;
 }
 
