@@ -249,6 +249,35 @@ def test_on_another_stream():
     assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("dtype,B,T", [("bf16", 1, 700), ("bf16", 4, 1500), ("f32", 2, 300)])
+def test_in_a_graph(dtype, B, T):
+    """A captured step (kernels that start beside their predecessors among them) replayed on new inputs."""
+    q, k, v, dy = make(B, T, T, 6, 3, 128, dtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+
+    def step():
+        y = ops.window_attention_train(*leaves, window=100, sinks=4)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (1, 2, 3):
+        with torch.no_grad():
+            for t, new in zip((*leaves, dy), make(B, T, T, 6, 3, 128, dtype, seed=seed)):
+                t.copy_(new)
+        graph.replay()
+        graph.replay()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+    assert ops.device_status() == 0
+
+
 def test_empty_sizes():
     q, k, v, _ = make(2, 3, 5, 2, 1, 64, "bf16")
     assert ops.window_attention(q[:0], k[:0], v[:0]).shape == (0, 3, 2, 64)
