@@ -170,30 +170,36 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
     if (threadIdx.x == 0) *c.status = GDNX_EINVAL;
     return;
   }
-  // what each row needs: its new pages, and one more where a shared last page is copied
-  const auto ask = [&](int64_t i, int64_t& first, int64_t& need, int& shared) {
+  // what each row needs: its new pages, and one more where a shared last page is copied; `lost`: the new
+  // tokens would begin on a page that was released (trimmed, and the slot cut back into it since)
+  const auto ask = [&](int64_t i, int64_t& first, int64_t& need, int& shared, bool& lost) {
     const int64_t len = length_of(c, rows[i]);
     const int64_t have = pages_of(c, len), want = pages_of(c, len + counts[i]);
     shared = -1;
     if (counts[i] > 0 && len % c.page) {
       const int tail = c.table[rows[i] * c.width + have - 1];
-      if (page_ok(c, tail) && c.refs[tail] > 1) shared = tail;
+      if (!page_ok(c, tail)) lost = true;
+      else if (c.refs[tail] > 1) shared = tail;
     }
     first = have - (shared >= 0);
     need = want - first;
     return want <= c.width;
   };
-  bool full = false;
+  bool full = false, lost = false;
   int64_t total = 0;
   for (int64_t base = 0; base < n; base += NT) {
     const int64_t i = base + threadIdx.x;
     int64_t first = 0, need = 0;
     int shared, sum;
-    if (i < n) full |= !ask(i, first, need, shared);
+    if (i < n) full |= !ask(i, first, need, shared, lost);
     if (full) need = 0;  // refused below; keeps the sums small
     const int at = block_scan((int)need, sums, &sum);
     if (i < n) w.off[i] = (int)(total + at);
     total += sum;
+  }
+  if (__syncthreads_or(lost)) {
+    if (threadIdx.x == 0) *c.status = GDNX_EINVAL;
+    return;
   }
   if (__syncthreads_or(full || total > c.pages)) {
     if (threadIdx.x == 0) *c.status = GDNX_ENOPAGES;
@@ -223,7 +229,7 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
     const int64_t i = i0 + warp;
     int64_t first = 0, need = 0;
     int shared = -1;
-    if (i < n) ask(i, first, need, shared);
+    if (i < n) ask(i, first, need, shared, lost);
     if (i < n) w.off[i] |= shared >= 0 ? (int)0x80000000 : 0;
   }
   __syncthreads();

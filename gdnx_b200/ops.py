@@ -1109,7 +1109,8 @@ def cache_fork(cache: PagedCache, src: torch.Tensor, dst: torch.Tensor) -> None:
 def cache_extend(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor) -> None:
     """Room for ``counts[i]`` more tokens in slot ``rows[i]`` (int32 vectors, each slot once): its
     length grows, and it takes free pages, the lowest first, in the order of ``rows``.  A partly
-    filled last page that other slots share is copied first, in every layer."""
+    filled last page that other slots share is copied first, in every layer; one that was released (the
+    slot was trimmed, then cut back into it) is refused: cut the slot back to a page's edge first."""
     s, index = _cache_struct(cache)
     at, n = _cache_rows(rows, s, index)
     more = _index32(counts, n, "counts", index)

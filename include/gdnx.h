@@ -448,7 +448,8 @@ GDNX_API gdnx_status gdnx_attn_bwd(const gdnx_attn_bwd_args* args, void* stream)
  * of every layer.  refs counts the slots that hold a page; a page with refs 0 is free.
  * The page operations below run on the device without host synchronisation.  A call that
  * cannot be carried out changes nothing and sets *status (GDNX_ENOPAGES: pool or table too
- * small; GDNX_EINVAL: a slot out of range or named twice, a negative count); while
+ * small; GDNX_EINVAL: a slot out of range or named twice, a negative count, and what an
+ * operation says below); while
  * *status is not 0 the operations do nothing, so a step can be enqueued whole and
  * checked once. */
 typedef struct {
@@ -469,7 +470,9 @@ GDNX_API gdnx_status gdnx_cache_fork(const gdnx_cache* cache, int64_t n, const i
                                      void* stream);
 /* Room for counts[i] more tokens in slot rows[i]: free pages, the lowest index first, in
  * the order of rows.  A partly filled last page that other slots share is copied first
- * (every layer), so that writes stay private. */
+ * (every layer), so that writes stay private.  GDNX_EINVAL where the partly filled last page
+ * was released (by a trim, before the slot was cut back into it): cut the slot back to a
+ * page's edge first. */
 GDNX_API gdnx_status gdnx_cache_extend(const gdnx_cache* cache, int64_t n, const int32_t* rows, const int32_t* counts,
                                        void* workspace, size_t workspace_bytes, void* stream);
 /* k, v [n,T,Hk,D] become tokens length-count .. length-1 of slot rows[i] in `layer`

@@ -122,6 +122,10 @@ class PagedCache:
     def extend(self, rows, counts):
         if self._bad(rows, *counts):
             return
+        if any(c > 0 and self.lengths[r] % self.page and self.table[r][self.lengths[r] // self.page] < 0
+               for r, c in zip(rows, counts)):  # no place for the next token on the last page
+            self.status = "invalid"
+            return
         plan, free = [], [p for p, x in enumerate(self.refs) if x == 0]
         for r, c in zip(rows, counts):
             n = self.lengths[r]

@@ -152,3 +152,18 @@ def test_oracle_cache_shares_copies_and_closes_up():
     assert c.table[2] == [-1, -1, 2]
     c.extend([0], [9])
     assert c.status == "no pages" and c.lengths[0] == 3
+
+
+def test_oracle_extend_refuses_a_released_tail():
+    kv = torch.zeros(1, 2, 8, 1, 4, 1)
+    c = A.PagedCache(kv, torch.full((1, 8), -1), torch.zeros(1, dtype=torch.int32), torch.zeros(8, dtype=torch.int32))
+    c.extend([0], [20])
+    c.trim([0], 4, 0)
+    assert c.table[0][:5] == [-1, -1, -1, -1, 4]
+    c.truncate([0], [6])
+    c.extend([0], [1])
+    assert c.status == "invalid" and c.lengths == [6] and c.table[0] == [-1] * 8
+    c.status = ""
+    c.truncate([0], [4])
+    c.extend([0], [1])
+    assert not c.status and c.lengths == [5] and c.table[0][:2] == [-1, 0]

@@ -327,3 +327,34 @@ def test_pool_beyond_32_bits(dtype):
     ops.cache_compact(c)
     assert int(c.table.max()) == 5 and torch.equal(ops.paged_decode(q, c), y)
     ops.cache_check(c)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tokens_are_not_added_behind_a_released_tail(dtype):
+    """A slot cut back into pages that a trim released has no page for the rest of its last tokens: room for more is
+    refused (with every row of the call) instead of tokens going nowhere.  At a page's edge there is nothing to miss."""
+    c = cache([200, 70, 20], width=16, D=64, dtype=dtype)
+    ops.cache_trim(c, i32(0), window=40)
+    ops.cache_truncate(c, i32(0), i32(50))  # token 49 was on page 3, which is gone
+    o = mirror(c)
+    ops.cache_extend(c, i32(1, 0), i32(3, 1))
+    o.extend([1, 0], [3, 1])
+    assert o.status == "invalid" and int(c.status) == L.GDNX_EINVAL
+    with pytest.raises(L.GdnxError):
+        ops.cache_check(c)
+    o.status = ""
+    same(c, o)
+    ops.cache_extend(c, i32(0, 1), i32(0, 3))  # nothing asked of the slot
+    ops.cache_truncate(c, i32(0), i32(48))
+    ops.cache_extend(c, i32(0), i32(5))
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(1, 5, 2, 64, generator=g).to(TYPES[dtype]).to(DEV) for _ in range(2))
+    ops.cache_write(c, k, v, i32(0), layer=1)
+    ops.cache_check(c)
+    for op, args in ((o.extend, ([0, 1], [0, 3])), (o.truncate, ([0], [48])), (o.extend, ([0], [5])), (o.write, (k, v, [0], 1))):
+        op(*args)
+    assert not o.status
+    same(c, o)
+    q = torch.randn(1, 4, 64, generator=g).to(TYPES[dtype]).to(DEV)
+    want = ops.window_attention(q[:, None], k, v)[:, 0]  # the five tokens are what is left to see
+    assert rel(ops.paged_decode(q, c, layer=1, rows=i32(0)), want) < 2 * TOL[dtype]
