@@ -210,7 +210,7 @@ gdnx_status gdnx_cache_write(const gdnx_cache* c, int64_t layer, int64_t n, int6
                              const gdnx_view* v, const int32_t* rows, const int32_t* counts, void* stream) {
   const gdnx_status s = check_cache(c);
   if (s != GDNX_OK) return s;
-  if (layer < 0 || layer >= c->L || n < 0 || T < 0 || !k || !v) return GDNX_EINVAL;
+  if (layer < 0 || layer >= c->L || n < 0 || n > c->slots || T < 0 || !k || !v) return GDNX_EINVAL;
   if (n == 0 || T == 0) return GDNX_OK;
   if (!heads_ok(*k, c->dtype, c->D) || !heads_ok(*v, c->dtype, c->D) || !is_device_ptr(rows)) return GDNX_EINVAL;
   if (counts && !is_device_ptr(counts)) return GDNX_EINVAL;

@@ -23,6 +23,7 @@ namespace {
 constexpr int NT = 1024;      // threads of a planning CTA
 constexpr int ROW_NT = 128;   // threads of a row CTA
 constexpr int COPY_NT = 256;
+constexpr int WRITE_NT = 256;
 constexpr int COPY_VEC = 4;   // 16-byte words in flight for each thread of a copy
 constexpr int HEAD = 64;      // workspace words before the lists: [0] copies, [1] live pages
 
@@ -344,26 +345,70 @@ __global__ void __launch_bounds__(COPY_NT) cache_copy_kernel(const gdnx_cache c,
   }
 }
 
-// One V-typed piece of a token's key or value for each thread.
-template <typename V>
-__global__ void __launch_bounds__(256) cache_write_kernel(const gdnx_cache c, int64_t layer, int64_t n, int64_t T,
-                                                          const gdnx_view k, const gdnx_view v, const int32_t* rows,
-                                                          const int32_t* counts, int es) {
+// Pages that a write of T tokens touches in a slot, at most.
+__host__ __device__ inline int64_t pages_touched(const gdnx_cache& c, int64_t T) {
+  const int64_t most = (T + c.page - 2) / c.page + 1;
+  return most < c.width ? most : c.width;
+}
+
+// True in every thread when a write can be carried out: no operation was refused before, each slot once and in range, 0 <= count <= T tokens
+// that the slot has, and every page they lie on held by this slot alone.  `seen` has slots bits.
+GDNX_DEV bool write_ok(uint32_t* seen, const gdnx_cache& c, int64_t n, int64_t T, const int32_t* rows,
+                       const int32_t* counts) {
+  for (int64_t i = threadIdx.x; i < (c.slots + 31) / 32; i += blockDim.x) seen[i] = 0;
+  bool bad = *c.status != 0;
+  __syncthreads();
+  const int64_t span = pages_touched(c, T);
+  for (int64_t x = threadIdx.x; x < n * span; x += blockDim.x) {
+    const int64_t i = x / span, k = x % span, count = counts ? counts[i] : T;
+    const int row = rows[i];
+    if (row < 0 || row >= c.slots || count < 0 || count > T) {
+      bad = true;
+      continue;
+    }
+    if (k == 0) bad |= (atomicOr(&seen[row / 32], 1u << (row % 32)) >> (row % 32)) & 1u;
+    const int64_t len = length_of(c, row), at = (len - count) / c.page + k;
+    if (count > len) bad = true;
+    else if (count > 0 && at <= (len - 1) / c.page) {
+      const int p = c.table[row * c.width + at];
+      bad |= !page_ok(c, p) || c.refs[p] != 1;
+    }
+  }
+  return !__syncthreads_or(bad);
+}
+
+// The check by one CTA, for writes of many pages.
+__global__ void __launch_bounds__(NT) cache_write_check_kernel(const gdnx_cache c, int64_t n, int64_t T,
+                                                               const int32_t* rows, const int32_t* counts) {
+  extern __shared__ uint32_t seen[];
   dependents_may_start();
   wait_for_earlier();
-  if (*c.status != 0) return;
+  if (!write_ok(seen, c, n, T, rows, counts) && threadIdx.x == 0 && *c.status == 0) *c.status = GDNX_EINVAL;
+}
+
+// One V-typed piece of a token's key or value for each thread.  CHECK: every CTA checks the call itself and
+// decides like the others.
+template <typename V, bool CHECK>
+__global__ void __launch_bounds__(WRITE_NT) cache_write_kernel(const gdnx_cache c, int64_t layer, int64_t n, int64_t T,
+                                                               const gdnx_view k, const gdnx_view v,
+                                                               const int32_t* rows, const int32_t* counts, int es) {
+  extern __shared__ uint32_t seen[];
+  dependents_may_start();
+  wait_for_earlier();
+  if (CHECK ? !write_ok(seen, c, n, T, rows, counts) : *c.status != 0) {
+    if (CHECK && blockIdx.x == 0 && threadIdx.x == 0 && *c.status == 0) *c.status = GDNX_EINVAL;
+    return;
+  }
   const int per = (int)(c.D * es / sizeof(V));  // pieces of one head
   const int64_t all = n * T * c.Hk * per * 2;
-  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
+  for (int64_t x = (int64_t)blockIdx.x * WRITE_NT + threadIdx.x; x < all; x += (int64_t)gridDim.x * WRITE_NT) {
     const int64_t e = x % per, h = x / per % c.Hk, t = x / (per * c.Hk) % T, i = x / (per * c.Hk * T) % n;
     const int side = (int)(x / (per * c.Hk * T * n));
     const int row = rows[i];
     const int64_t count = counts ? counts[i] : T;
-    if (row < 0 || row >= c.slots || t >= count || count > T) continue;
+    if (t >= count) continue;
     const int64_t pos = length_of(c, row) - count + t;
-    if (pos < 0) continue;
     const int p = c.table[row * c.width + pos / c.page];
-    if (!page_ok(c, p)) continue;
     const gdnx_view& in = side ? v : k;
     const V* src = reinterpret_cast<const V*>(static_cast<const char*>(in.ptr) + (i * in.sb + t * in.st + h * in.sh) * es);
     char* at = static_cast<char*>(c.kv) +
@@ -416,8 +461,11 @@ gdnx_status launch_cache_compact(const gdnx_cache& c, void* ws, cudaStream_t st)
   return copy_pages(c, ws, 0, 1, st);
 }
 
-gdnx_status launch_cache_write(const gdnx_cache& c, int64_t layer, int64_t n, int64_t T, const gdnx_view& k,
-                               const gdnx_view& v, const int32_t* rows, const int32_t* counts, cudaStream_t st) {
+namespace {
+
+template <bool CHECK>
+cudaError_t write_pieces(const gdnx_cache& c, int64_t layer, int64_t n, int64_t T, const gdnx_view& k,
+                         const gdnx_view& v, const int32_t* rows, const int32_t* counts, cudaStream_t st) {
   const int es = elem(c.dtype), vec = 16 / es;
   const auto wide = [&](const gdnx_view& x) {
     return reinterpret_cast<uintptr_t>(x.ptr) % 16 == 0 && x.sb % vec == 0 && x.st % vec == 0 && x.sh % vec == 0;
@@ -425,9 +473,24 @@ gdnx_status launch_cache_write(const gdnx_cache& c, int64_t layer, int64_t n, in
   const bool v16 = wide(k) && wide(v);
   const int64_t all = n * T * c.Hk * (v16 ? c.D / vec : c.D) * 2;
   const int64_t most = 148 * 64;
-  const unsigned grid = (unsigned)((all + 255) / 256 < most ? (all + 255) / 256 : most);
-  const auto kernel = v16 ? cache_write_kernel<uint4> : es == 4 ? cache_write_kernel<uint32_t> : cache_write_kernel<uint16_t>;
-  return launched(launch_early(kernel, dim3(grid), dim3(256), 0, st, c, layer, n, T, k, v, rows, counts, es));
+  const unsigned grid = (unsigned)((all + WRITE_NT - 1) / WRITE_NT < most ? (all + WRITE_NT - 1) / WRITE_NT : most);
+  const auto kernel = v16 ? cache_write_kernel<uint4, CHECK>
+                      : es == 4 ? cache_write_kernel<uint32_t, CHECK> : cache_write_kernel<uint16_t, CHECK>;
+  return launch_early(kernel, dim3(grid), dim3(WRITE_NT), CHECK ? seen_bytes(c) : 0, st, c, layer, n, T, k, v, rows,
+                      counts, es);
+}
+
+}  // namespace
+
+// A check that takes every thread of a CTA one step runs in the CTAs that write; longer ones run once, in a
+// CTA of their own before them.
+gdnx_status launch_cache_write(const gdnx_cache& c, int64_t layer, int64_t n, int64_t T, const gdnx_view& k,
+                               const gdnx_view& v, const int32_t* rows, const int32_t* counts, cudaStream_t st) {
+  if (n * pages_touched(c, T) <= WRITE_NT && seen_bytes(c) <= WRITE_NT * 4)
+    return launched(write_pieces<true>(c, layer, n, T, k, v, rows, counts, st));
+  if (launch_early(cache_write_check_kernel, dim3(1), dim3(NT), seen_bytes(c), st, c, n, T, rows, counts) != cudaSuccess)
+    return GDNX_ELAUNCH;
+  return launched(write_pieces<false>(c, layer, n, T, k, v, rows, counts, st));
 }
 
 }  // namespace gdnx

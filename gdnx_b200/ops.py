@@ -1123,11 +1123,11 @@ def cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, rows: torch
                 counts: Optional[torch.Tensor] = None) -> None:
     """The keys and values ``k``, ``v`` [n,T,Hk,D] of slot ``rows[i]``'s last T tokens in ``layer``
     (each slot once; after :func:`cache_extend`); with ``counts`` [n] int32, row i's first ``counts[i]`` of T are its
-    last ``counts[i]`` tokens (a right-padded prompt)."""
+    last ``counts[i]`` tokens (a right-padded prompt).  Refused where a slot has fewer tokens, or one of them lies on
+    a released page or on one that another slot holds too."""
     s, index = _cache_struct(cache)
     _on_device(index, k, v)
-    at = _index32(rows, None, "rows", index)
-    n = rows.shape[0]
+    at, n = _cache_rows(rows, s, index)
     if k.dim() != 4 or k.shape != v.shape or k.shape[0] != n or k.shape[2] != s.Hk or k.shape[3] != s.D:
         raise ValueError("k and v must be [n,T,Hk,D] with the cache's heads")
     if k.dtype is not cache.kv.dtype or v.dtype is not cache.kv.dtype:

@@ -477,7 +477,8 @@ GDNX_API gdnx_status gdnx_cache_extend(const gdnx_cache* cache, int64_t n, const
                                        void* workspace, size_t workspace_bytes, void* stream);
 /* k, v [n,T,Hk,D] become tokens length-count .. length-1 of slot rows[i] in `layer`
  * (count = counts[i] <= T, or T where counts is NULL; further tokens of a row are ignored).
- * Each slot is named once. */
+ * GDNX_EINVAL where a slot has fewer than count tokens, or one of them lies on a released page
+ * or on one that another slot holds too (extend gives the tokens that it adds pages of their own). */
 GDNX_API gdnx_status gdnx_cache_write(const gdnx_cache* cache, int64_t layer, int64_t n, int64_t T, const gdnx_view* k,
                                       const gdnx_view* v, const int32_t* rows, const int32_t* counts, void* stream);
 /* Slot rows[i] keeps its first lengths[i] tokens (0 frees it). */

@@ -146,16 +146,18 @@ class PagedCache:
             self.lengths[r] += c
 
     def write(self, k, v, rows, layer, counts=None):
-        if self.status:
+        counts = [k.shape[1]] * len(rows) if counts is None else counts
+        if self._bad(rows, *counts):
             return
-        for i, r in enumerate(rows):
-            c = k.shape[1] if counts is None else counts[i]
-            for t in range(c):
-                pos = self.lengths[r] - c + t
-                p = self.table[r][pos // self.page] if pos >= 0 else -1
-                if p >= 0:
-                    self.kv[layer, 0, p, :, pos % self.page] = k[i, t].cpu()
-                    self.kv[layer, 1, p, :, pos % self.page] = v[i, t].cpu()
+        at = [(i, t, self.lengths[r] - c + t, r) for i, (r, c) in enumerate(zip(rows, counts)) for t in range(c)]
+        if max(counts, default=0) > k.shape[1] or any(
+                pos < 0 or self.table[r][pos // self.page] < 0 or self.refs[self.table[r][pos // self.page]] != 1
+                for _, _, pos, r in at):
+            self.status = "invalid"
+            return
+        for i, t, pos, r in at:
+            for side, x in enumerate((k, v)):
+                self.kv[layer, side, self.table[r][pos // self.page], :, pos % self.page] = x[i, t].cpu()
 
     def compact(self):
         if self.status:

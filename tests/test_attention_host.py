@@ -167,3 +167,18 @@ def test_oracle_extend_refuses_a_released_tail():
     c.truncate([0], [4])
     c.extend([0], [1])
     assert not c.status and c.lengths == [5] and c.table[0][:2] == [-1, 0]
+
+
+@pytest.mark.parametrize("rows,counts,T", [([0, 3], [1, 1], 2), ([-1], [1], 2), ([0, 0], [1, 1], 2), ([0], [-1], 2),
+                                           ([0], [3], 2), ([0], None, 9), ([0], [5], 6), ([1], [8], 9)])
+def test_oracle_write_refuses(rows, counts, T):
+    """Slots out of range or twice, more tokens than given, than the slot holds, than it holds alone, than are on pages."""
+    kv = torch.zeros(1, 2, 8, 1, 4, 1)
+    c = A.PagedCache(kv, torch.full((3, 8), -1), torch.zeros(3, dtype=torch.int32), torch.zeros(8, dtype=torch.int32))
+    c.extend([0], [5])
+    c.fork([0, 0], [1, 2])
+    c.extend([1, 0], [3, 1])
+    c.trim([1], 2, 0)
+    x = torch.ones(len(rows), T, 1, 1)
+    c.write(x, x, rows, 0, counts)
+    assert c.status == "invalid" and not c.kv.any()

@@ -358,3 +358,47 @@ def test_tokens_are_not_added_behind_a_released_tail(dtype):
     q = torch.randn(1, 4, 64, generator=g).to(TYPES[dtype]).to(DEV)
     want = ops.window_attention(q[:, None], k, v)[:, 0]  # the five tokens are what is left to see
     assert rel(ops.paged_decode(q, c, layer=1, rows=i32(0)), want) < 2 * TOL[dtype]
+
+
+WRITES = {  # rows and counts of a write of T tokens that cannot be carried out; slots 0..5 hold 40, 0, 100, 100, 100, 7
+    "slot below": ([0, -1], [1, 1]), "slot beyond": ([6, 0], [1, 1]), "slot twice": ([2, 0, 2], [1, 1, 1]),
+    "negative count": ([0, 2], [1, -1]), "more than T": ([0, 2], [1, "T+1"]), "more than the slot holds": ([2, 0, 5], [1, 1, 8]),
+    "no counts, more than a slot holds": ([0, 1], None), "released page": ([0, 3], [1, 70]),
+    "page of another slot too": ([0, 4], [1, 5]), "source of a fork": ([2], [101 - 4])}
+
+
+@pytest.mark.parametrize("T", [100, 6000])  # checked by the blocks that write, and by a block of their own
+@pytest.mark.parametrize("case", WRITES)
+def test_a_write_that_cannot_be_carried_out_changes_nothing(case, T):
+    rows, counts = WRITES[case]
+    c = cache([40, 0, 100, 100, 0, 7], width=600, extra=8)
+    ops.cache_trim(c, i32(3), window=20)
+    ops.cache_fork(c, i32(2), i32(4))
+    ops.cache_extend(c, i32(2), i32(3))  # slot 2's tail is its own again, what lies before is slot 4's too
+    ops.cache_check(c)
+    before = c.kv.clone().view(torch.int16)
+    n = len(rows)
+    k = torch.ones(n, T, 2, 64, dtype=torch.bfloat16, device=DEV)
+    at = None if counts is None else i32(*(T + 1 if x == "T+1" else x for x in counts))
+    o = mirror(c)
+    ops.cache_write(c, k, k, i32(*rows), layer=1, counts=at)
+    o.write(k, k, rows, 1, None if at is None else at.tolist())
+    assert o.status == "invalid" and int(c.status) == L.GDNX_EINVAL
+    assert torch.equal(c.kv.view(torch.int16), before)
+    ops.cache_write(c, k[:1], k[:1], i32(0), counts=i32(1))  # held: the status is set
+    assert torch.equal(c.kv.view(torch.int16), before)
+    with pytest.raises(L.GdnxError) as e:
+        ops.cache_check(c)
+    assert e.value.status == L.GDNX_EINVAL
+    o.status = ""
+    ops.cache_write(c, k[:1].expand(4, -1, -1, -1), k[:1].expand(4, -1, -1, -1), i32(5, 2, 0, 1), layer=1, counts=i32(7, 3, 40, 0))
+    o.write(k[:1].expand(4, -1, -1, -1), k[:1].expand(4, -1, -1, -1), [5, 2, 0, 1], 1, [7, 3, 40, 0])
+    ops.cache_check(c)
+    same(c, o)
+
+
+def test_a_write_names_no_more_rows_than_there_are_slots():
+    c = cache([20, 5])
+    k = torch.zeros(3, 1, 2, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError):
+        ops.cache_write(c, k, k, i32(0, 1, 0))
