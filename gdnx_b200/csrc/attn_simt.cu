@@ -306,7 +306,9 @@ __global__ void __launch_bounds__(NT, 3) attn_fwd_simt_kernel(const gdnx_attn_ar
   for (int r = 0; r < 4; ++r) {
     const int i = i0 + ty * 4 + r;
     if (i >= a.Tq) continue;
-    const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
+    // every row but padding sees itself: a sum that is not positive comes of scores that are not finite
+    const float none = i + off < len ? NAN : 0.f;
+    const float inv = l[r] > 0.f ? 1.f / l[r] : none;
     const int64_t row = b * a.y_sb + (int64_t)i * a.y_st + h * a.y_sh;
     for_pieces<DP>(o[r], tx, [&](int d, const float2* v, auto n) {
       if (d >= D) return;
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(NT, 3) attn_fwd_simt_kernel(const gdnx_attn_ar
         }
     });
     if (a.lse && tx == 0)
-      a.lse[(b * a.H + h) * a.Tq + i] = l[r] > 0.f ? (m[r] + log2f(l[r])) * kLn2 : -INFINITY;
+      a.lse[(b * a.H + h) * a.Tq + i] = l[r] > 0.f ? (m[r] + log2f(l[r])) * kLn2 : none == 0.f ? -INFINITY : none;
   }
 }
 

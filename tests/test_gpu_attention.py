@@ -328,3 +328,47 @@ def test_offsets_beyond_32_bits():
     q = buf.as_strided((2, 40, 2, 64), (far, 128, 64, 1))
     q.copy_(f[0])
     assert torch.equal(ops.window_attention(q, f[1], f[2], window=9), ops.window_attention(*f, window=9))
+
+
+def _same_where_finite(got, want, tol):
+    """NaN where the other is, close elsewhere."""
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert rel(got.nan_to_num(0), want.nan_to_num(0)) < tol
+
+
+BAD_KEYS = {  # a key's first value where the queries' first value is positive, and what else its row holds
+    "nan": float("nan"), "score inf": float("inf"), "score -inf": -float("inf")}
+
+
+@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("B,T,H", [(1, 150, 2), (1, 150, 1), (5, 1000, 4)])  # keys of a block split over the stages, and not
+@pytest.mark.parametrize("what", BAD_KEYS)
+def test_scores_that_are_not_finite_show_in_their_rows(what, B, T, H, dtype):
+    """A row that sees a score of NaN or +inf is NaN whatever the key's place in its tile, one that sees -inf only too;
+    other rows do not notice.  The same for the log of the sum."""
+    for j in (0, 1, 6, 7, 45, 134) if B == 1 else (1, 6, 134):
+        q, k, v, _ = make(B, T, T, H, H, 64, dtype, seed=j)
+        q[..., 0] = 1.0
+        k[:, j] = 0.0
+        k[:, j, :, 0] = BAD_KEYS[what]
+        y, lse = ops.window_attention(q, k, v, window=40, return_lse=True)
+        yo, lo = A.window_attention(q, k, v, window=40)
+        assert yo.isnan().any() or what == "score -inf" and j > 0
+        _same_where_finite(y, yo, TOL[dtype])
+        _same_where_finite(lse, lo, 1e-5)
+
+
+@pytest.mark.parametrize("dtype", ["f32"])
+def test_scores_that_overflow_show_in_their_rows(dtype):
+    """Finite inputs whose product leaves fp32's range, at every place of a run of 16 keys."""
+    for j in range(16):
+        q, k, v, _ = make(1, 60, 60, 2, 2, 64, dtype, seed=j)
+        q[..., 0] = 1e20
+        k[:, :, :, 0] = 0.0
+        k[:, j, :, 0] = 1e20
+        y, lse = ops.window_attention(q, k, v, return_lse=True)
+        assert y[:, j:].isnan().all() and lse[..., j:].isnan().all()
+        assert y[:, :j].isfinite().all() and lse[..., :j].isfinite().all()
+        y = ops.window_attention(q, -k, v)
+        assert y[:, j + 1:].isfinite().all() and y[:, :j].isfinite().all()
