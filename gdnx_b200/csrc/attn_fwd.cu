@@ -177,10 +177,11 @@ struct Row {
 };
 
 // Takes a tile's maximum into the row, rescaling O where it lies too far above the old one.
-// Returns what the tile's scores (times c2) are taken against.
+// Returns what the tile's scores (times c2) are taken against.  A score that is NaN or +inf is the tile's maximum
+// whatever its column, and from then on l and O or the maximum itself say so (ex2_poly alone would not).
 template <int DB>
 GDNX_DEV float take_max(Row& w, float top, float c2, uint32_t tO) {
-  const bool grow = w.m != -INFINITY && (top - w.m) * c2 > 8.f;
+  const bool grow = w.m != -INFINITY && !((top - w.m) * c2 <= 8.f);
   if (__any_sync(0xffffffffu, grow)) {
     const float corr = grow ? ex2((w.m - top) * c2) : 1.f;
     w.l *= corr;
@@ -241,8 +242,8 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
 #pragma unroll
         for (int e = 4; e < 128; e += 4)
 #pragma unroll
-          for (int f = 0; f < 4; ++f) t[f] = fmaxf(t[f], s[e + f]);
-        const float mc = take_max<DB>(row, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), c2, tO);
+          for (int f = 0; f < 4; ++f) t[f] = max_nan(t[f], s[e + f]);
+        const float mc = take_max<DB>(row, max_nan(max_nan(t[0], t[1]), max_nan(t[2], t[3])), c2, tO);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t pk[32];
@@ -265,7 +266,7 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
           float s[32];
           tc::tmem_ld32(tS + 32 * q, s);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) top = fmaxf(top, on >> e & 1 ? s[e] : -INFINITY);
+          for (int e = 0; e < 32; ++e) top = max_nan(top, on >> e & 1 ? s[e] : -INFINITY);
         }
         const float mc = take_max<DB>(row, top, c2, tO);
 #pragma unroll 1
@@ -313,7 +314,8 @@ GDNX_DEV void run_rows(const FwdParams& P, uint8_t* base, uint32_t tmem, Bars& b
         row.l = row.l * f0 + x.y * f1;
       }
     }
-    const float l = p < w.len ? row.l : 0.f;  // padding
+    // every row but padding sees itself: a maximum that is not finite comes of scores that are not
+    const float l = p >= w.len ? 0.f : fabsf(row.m * c2) < INFINITY ? row.l : NAN;
     const int i = i0 + r, row0 = i0 + r / 32 * 32;
     const float inv = l > 0.f ? 1.f / l : l != l ? l : 0.f;
 #pragma unroll 1

@@ -247,7 +247,14 @@ GDNX_DEV float2 mul2(float2 a, float2 b) {
   return d;
 }
 
-// 2^x of two values on the FMA pipes, for x <= 120; below -125 it stays at 2^-125.  x = n + f with
+// The larger of two values, NaN if either is.
+GDNX_DEV float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+// 2^x of two values on the FMA pipes, for x <= 120; below -125, and for NaN, it stays at 2^-125.  x = n + f with
 // |f| <= 1/2 (n by rounding x + 1.5 2^23), 2^f by the polynomial of degree 4 whose relative
 // error over the interval is least (2.6e-6, Remez exchange), n added to the exponent.
 GDNX_DEV float2 ex2_poly(float2 x) {

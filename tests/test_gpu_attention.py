@@ -341,7 +341,7 @@ BAD_KEYS = {  # a key's first value where the queries' first value is positive, 
     "nan": float("nan"), "score inf": float("inf"), "score -inf": -float("inf")}
 
 
-@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B,T,H", [(1, 150, 2), (1, 150, 1), (5, 1000, 4)])  # keys of a block split over the stages, and not
 @pytest.mark.parametrize("what", BAD_KEYS)
 def test_scores_that_are_not_finite_show_in_their_rows(what, B, T, H, dtype):
@@ -359,7 +359,7 @@ def test_scores_that_are_not_finite_show_in_their_rows(what, B, T, H, dtype):
         _same_where_finite(lse, lo, 1e-5)
 
 
-@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_scores_that_overflow_show_in_their_rows(dtype):
     """Finite inputs whose product leaves fp32's range, at every place of a run of 16 keys."""
     for j in range(16):
