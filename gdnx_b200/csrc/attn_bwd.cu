@@ -236,10 +236,10 @@ GDNX_DEV void keys_rows(const BwdParams& P, const KeyItem& w, const uint8_t* bas
     uint32_t on = 0xffffffffu;
     const float2 cc = make_float2(c2, c2);
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) {  // every other pair on the FMA pipes
+    for (int e = 0; e < 32; e += 4) {  // every other pair on the FMA pipes; lse of NaN has to reach dV
       const float4 z = *reinterpret_cast<const float4*>(lse + e);
       const float2 x = fma2(make_float2(s[e], s[e + 1]), cc, make_float2(z.x, z.y));
-      const float2 y = ex2_poly(fma2(make_float2(s[e + 2], s[e + 3]), cc, make_float2(z.z, z.w)));
+      const float2 y = ex2_poly<true>(fma2(make_float2(s[e + 2], s[e + 3]), cc, make_float2(z.z, z.w)));
       s[e] = ex2(x.x);
       s[e + 1] = ex2(x.y);
       s[e + 2] = y.x;
@@ -450,7 +450,7 @@ GDNX_DEV void queries_rows(const BwdParams& P, uint32_t tmem, Bars& bar, const v
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {  // every other pair on the FMA pipes
         const float2 x = fma2(make_float2(s[e], s[e + 1]), cc, make_float2(lse2, lse2));
-        const float2 y = ex2_poly(fma2(make_float2(s[e + 2], s[e + 3]), cc, make_float2(lse2, lse2)));
+        const float2 y = ex2_poly<false>(fma2(make_float2(s[e + 2], s[e + 3]), cc, make_float2(lse2, lse2)));  // NaN is in del
         s[e] = ex2(x.x);
         s[e + 1] = ex2(x.y);
         s[e + 2] = y.x;

@@ -153,7 +153,7 @@ GDNX_DEV void weights(const float* s, float c2, float mc, float2& sum, uint32_t*
 #pragma unroll
   for (int e = 0; e < N / 2; ++e) {
     const float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(c2, c2), make_float2(-mc, -mc));
-    const float2 p = e % 8 == 3 ? ex2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+    const float2 p = e % 8 == 3 ? ex2_poly<false>(x) : make_float2(ex2(x.x), ex2(x.y));
     sum = add2(sum, p);
     pk[e] = pack2<BF16>(p.x, p.y);
   }

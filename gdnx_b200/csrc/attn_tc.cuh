@@ -254,13 +254,15 @@ GDNX_DEV float max_nan(float a, float b) {
   return m;
 }
 
-// 2^x of two values on the FMA pipes, for x <= 120; below -125, and for NaN, it stays at 2^-125.  x = n + f with
+// 2^x of two values on the FMA pipes, for x <= 120; below -125 it stays at 2^-125.  x = n + f with
 // |f| <= 1/2 (n by rounding x + 1.5 2^23), 2^f by the polynomial of degree 4 whose relative
-// error over the interval is least (2.6e-6, Remez exchange), n added to the exponent.
+// error over the interval is least (2.6e-6, Remez exchange), n added to the exponent.  NaN gives 2^-125 too, or with
+// KEEP_NAN NaN, for one more multiplication (n added to its bits would make a number of it).
+template <bool KEEP_NAN>
 GDNX_DEV float2 ex2_poly(float2 x) {
   constexpr float kRound = 12582912.f;
-  x.x = fmaxf(x.x, -125.f);
-  x.y = fmaxf(x.y, -125.f);
+  x.x = KEEP_NAN ? max_nan(x.x, -125.f) : fmaxf(x.x, -125.f);
+  x.y = KEEP_NAN ? max_nan(x.y, -125.f) : fmaxf(x.y, -125.f);
   const float2 r = add2(x, make_float2(kRound, kRound));
   const float2 n = add2(r, make_float2(-kRound, -kRound));
   const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
@@ -268,6 +270,9 @@ GDNX_DEV float2 ex2_poly(float2 x) {
   p = fma2(p, f, make_float2(0.2402474433f, 0.2402474433f));
   p = fma2(p, f, make_float2(0.6931217909f, 0.6931217909f));
   p = fma2(p, f, make_float2(0.9999992847f, 0.9999992847f));
+  if (KEEP_NAN)
+    return mul2(p, make_float2(__int_as_float((__float_as_int(r.x) << 23) + 0x3f800000),
+                               __int_as_float((__float_as_int(r.y) << 23) + 0x3f800000)));
   p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23));
   p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23));
   return p;

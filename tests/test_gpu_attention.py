@@ -372,3 +372,19 @@ def test_scores_that_overflow_show_in_their_rows(dtype):
         assert y[:, :j].isfinite().all() and lse[..., :j].isfinite().all()
         y = ops.window_attention(q, -k, v)
         assert y[:, j + 1:].isfinite().all() and y[:, :j].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("i", [1, 5, 6, 7, 48, 130])
+def test_a_query_that_is_not_finite_shows_in_its_gradients(i, dtype):
+    """NaN in a query: in its own dq, and in dk and dv of every key that it sees, whatever its place in the tile; nothing
+    of other heads notices."""
+    q, k, v, dy = make(1, 200, 200, 4, 2, 64, dtype, seed=i)
+    q[:, i, 1] = float("nan")
+    xs = [t.detach().requires_grad_() for t in (q, k, v)]
+    y = ops.window_attention_train(*xs, window=70, sinks=2)
+    dq, dk, dv = torch.autograd.grad(y, xs, dy)
+    seen = A.visible(200, 200, 70, 2)[i].to(DEV)
+    assert y[:, i, 1].isnan().all() and dq[:, i, 1].isnan().all()
+    assert dk[:, seen, 0].isnan().all() and dv[:, seen, 0].isnan().all()
+    assert dq[:, :, [0, 2, 3]].isfinite().all() and dk[:, :, 1].isfinite().all() and dv[:, :, 1].isfinite().all()
