@@ -21,7 +21,7 @@ GDNX_COMPACT_SVD, GDNX_COMPACT_SKETCH = 0, 1
 EXPORTED = ("gdnx_scan_fwd", "gdnx_scan_fwd_noalloc", "gdnx_scan_noalloc_status", "gdnx_scan_workspace_bytes", "gdnx_kr_scan_fwd", "gdnx_compact",
             "gdnx_decode_step", "gdnx_epilogue", "gdnx_gdn3_prologue", "gdnx_kmd2_prologue", "gdnx_scan_bwd", "gdnx_scan_bwd_workspace_bytes", "gdnx_status_string", "gdnx_version",
             "gdnx_epilogue_scatter", "gdnx_device_alloc", "gdnx_device_free", "gdnx_ipc_handle", "gdnx_ipc_open",
-            "gdnx_ipc_close", "gdnx_attn_fwd", "gdnx_attn_bwd", "gdnx_attn_bwd_workspace_bytes", "gdnx_cache_fork",
+            "gdnx_ipc_close", "gdnx_error_word", "gdnx_error_status", "gdnx_attn_fwd", "gdnx_attn_bwd", "gdnx_attn_bwd_workspace_bytes", "gdnx_cache_fork",
             "gdnx_cache_extend", "gdnx_cache_write", "gdnx_cache_truncate", "gdnx_cache_trim", "gdnx_cache_compact",
             "gdnx_cache_workspace_bytes", "gdnx_paged_decode", "gdnx_paged_decode_workspace_bytes")
 
@@ -194,6 +194,10 @@ def load(path: Path = LIB_PATH):
     lib.gdnx_ipc_close.restype = C.c_int
     lib.gdnx_scan_bwd_workspace_bytes.argtypes = [C.POINTER(ScanBwdArgs)]
     lib.gdnx_scan_bwd_workspace_bytes.restype = C.c_size_t
+    lib.gdnx_error_word.argtypes = [C.POINTER(C.c_void_p)]
+    lib.gdnx_error_word.restype = C.c_int
+    lib.gdnx_error_status.argtypes = [C.POINTER(C.c_int32), C.c_int32, C.c_void_p]
+    lib.gdnx_error_status.restype = C.c_int
     lib.gdnx_attn_fwd.argtypes = [C.POINTER(AttnArgs), C.c_void_p]
     lib.gdnx_attn_fwd.restype = C.c_int
     lib.gdnx_attn_bwd_workspace_bytes.argtypes = [C.POINTER(AttnBwdArgs)]

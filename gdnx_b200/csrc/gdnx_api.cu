@@ -79,6 +79,8 @@ Path select_path(const gdnx_scan_args& a) {
   return Path::kGeneral;
 }
 
+__device__ int g_error_word;
+
 // ---- windowed attention and the paged cache ----
 
 constexpr int64_t kMaxTokens = (int64_t)1 << 30;  // positions and their distances stay in int32
@@ -144,6 +146,32 @@ gdnx_status check_rows(const gdnx_cache* c, int64_t n, const int32_t* rows, cons
 }  // namespace
 
 extern "C" {
+
+gdnx_status gdnx_error_word(int32_t** word) {
+  if (!word) return GDNX_EINVAL;
+  void* p = nullptr;
+  if (cudaGetSymbolAddress(&p, g_error_word) != cudaSuccess) {
+    cudaGetLastError();
+    return GDNX_ELAUNCH;
+  }
+  *word = static_cast<int32_t*>(p);
+  return GDNX_OK;
+}
+
+gdnx_status gdnx_error_status(int32_t* value, int32_t clear, void* stream) {
+  int32_t *word, read = 0;
+  if (!value) return GDNX_EINVAL;
+  const gdnx_status s = gdnx_error_word(&word);
+  if (s != GDNX_OK) return s;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (cudaMemcpyAsync(&read, word, sizeof read, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+      (clear && cudaMemsetAsync(word, 0, sizeof read, st) != cudaSuccess) || cudaStreamSynchronize(st) != cudaSuccess) {
+    cudaGetLastError();
+    return GDNX_ELAUNCH;
+  }
+  *value = read;
+  return GDNX_OK;
+}
 
 gdnx_status gdnx_attn_fwd(const gdnx_attn_args* a, void* stream) {
   if (!a) return GDNX_EINVAL;

@@ -240,15 +240,26 @@ def _cached_workspace(device, need):
 def device_status(workspace: Optional[torch.Tensor] = None) -> int:
     """Device-side status of scans that used ``workspace`` (default: every workspace this
     module owns, and the attention kernels' error words): the error word the kernels write when a bounded wait gives up
-    (``GDNX_ETIMEOUT``; their outputs are then invalid), 0 otherwise.  Synchronises."""
-    wss = [workspace] if workspace is not None else list(_WORKSPACES.values()) + list(_ERRORS.values())
+    (``GDNX_ETIMEOUT``; their outputs are then invalid), 0 otherwise.  Synchronises.  An attention kernel's
+    error stays until :func:`clear_device_status`."""
+    wss = [workspace] if workspace is not None else list(_WORKSPACES.values())
     for ws in wss:
         if ws is None or ws.numel() < 4:
             continue
         code = int(ws[:4].view(torch.int32).item())
         if code:
             return code
+    for index in [] if workspace is not None else list(_ERRORS):
+        code = _read_error_word(index, False)
+        if code:
+            return code
     return 0
+
+
+def clear_device_status() -> None:
+    """Sets the attention kernels' error words to 0 (scans clear theirs when they start).  Synchronises."""
+    for index in list(_ERRORS):
+        _read_error_word(index, True)
 
 
 def check_device_status(workspace: Optional[torch.Tensor] = None) -> None:
@@ -887,18 +898,26 @@ def gdn3_scan_train(q, k, v, b_gate, w_gate, decay, *, decay_kind="gamma", state
 # windowed attention
 # ----------------------------------------------------------------------------
 
-_ERRORS = {}
+_ERRORS = {}  # device index -> address of the library's error word there
 
 
 def _error_word(index: int) -> int:
     """Address of the word that takes a device error of the attention kernels on device ``index``
-    (one per device, read by :func:`device_status`; it stays set)."""
+    (the library's own, read by :func:`device_status`; it stays set until :func:`clear_device_status`)."""
     word = _ERRORS.get(index)
     if word is None:
-        word = torch.zeros(4, dtype=torch.uint8, device=torch.device("cuda", index))
-        torch.cuda.current_stream(index).synchronize()  # other streams write it too
-        _ERRORS[index] = word
-    return word.data_ptr()
+        at = C.c_void_p()
+        with torch.cuda.device(index):
+            L.check(L.load().gdnx_error_word(C.byref(at)), "gdnx_error_word")
+        word = _ERRORS[index] = at.value
+    return word
+
+
+def _read_error_word(index: int, clear: bool) -> int:
+    value = C.c_int32(0)
+    with torch.cuda.device(index):
+        L.check(L.load().gdnx_error_status(C.byref(value), int(clear), _stream(index)), "gdnx_error_status")
+    return value.value
 
 
 def _enqueue(name: str, index: int, *args) -> None:

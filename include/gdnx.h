@@ -398,15 +398,24 @@ typedef struct {
 
 GDNX_API gdnx_status gdnx_kmd2_prologue(const gdnx_kmd2_prologue_args* args, void* stream);
 
+/* The library's own error word on the current device: one int32 that is 0 until a kernel
+ * whose `error` field points to it gives up a bounded wait (GDNX_ETIMEOUT).  The same
+ * address at every call; asking allocates nothing and may happen during a graph's capture. */
+GDNX_API gdnx_status gdnx_error_word(int32_t** word);
+/* Its value after what was enqueued on `stream` (synchronises it); with `clear` it is 0 after. */
+GDNX_API gdnx_status gdnx_error_status(int32_t* value, int32_t clear, void* stream);
+
 /* Causal attention with a sliding window and sink tokens, the exact short-range read
  * that stands beside the recurrent state.  Query i stands at position p = Tk - Tq + i
  * (a prompt, or the end of one whose beginning is already known) and sees key j where
  *   j <= p,  j < lengths[b],  and  p - j < window  or  j < sinks;
  * a query with p >= lengths[b] is padding: its output is 0, its lse -inf, and what its
- * rows of q, dy, k and v hold (NaN included) reaches no output.  Other rows are finite.
+ * rows of q, dy, k and v hold (NaN included) reaches no output.  Values of q, k, v at
+ * other positions are meant to be finite.
  *   y_i = sum_j softmax_j(scale q_i.k_j) v_j ;  query head h reads key head h / (H / Hk).
  * Scores, softmax statistics and sums are fp32; 16-bit inputs run on the tensor cores
- * where TMA can address them, other types and layouts on the CUDA cores. */
+ * where TMA can address them, other types and layouts on the CUDA cores.
+ * A row that sees a score of NaN or +inf, or only -inf, is NaN (y and lse). */
 typedef struct {
   int64_t B, Tq, Tk, H, Hk, D; /* Tq <= Tk; H a multiple of Hk; D <= 128, a multiple of 8 */
   int64_t window, sinks;       /* window >= 1 (Tk or more: plain causal), sinks >= 0       */

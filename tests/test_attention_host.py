@@ -182,3 +182,8 @@ def test_oracle_write_refuses(rows, counts, T):
     x = torch.ones(len(rows), T, 1, 1)
     c.write(x, x, rows, 0, counts)
     assert c.status == "invalid" and not c.kv.any()
+
+
+def test_error_word_refuses_a_null_place():
+    assert L.load().gdnx_error_word(None) == L.GDNX_EINVAL
+    assert L.load().gdnx_error_status(None, 0, None) == L.GDNX_EINVAL

@@ -388,3 +388,71 @@ def test_a_query_that_is_not_finite_shows_in_its_gradients(i, dtype):
     assert y[:, i, 1].isnan().all() and dq[:, i, 1].isnan().all()
     assert dk[:, seen, 0].isnan().all() and dv[:, seen, 0].isnan().all()
     assert dq[:, :, [0, 2, 3]].isfinite().all() and dk[:, :, 1].isfinite().all() and dv[:, :, 1].isfinite().all()
+
+
+def _run(code):
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True,
+                       timeout=600)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_the_first_call_may_be_captured():
+    """A process whose first attention calls happen while a graph is captured."""
+    _run("""
+import torch
+from gdnx_b200 import ops
+q, k, v = (torch.randn(1, 300, 2, 64, device="cuda").to(torch.bfloat16).requires_grad_() for _ in range(3))
+dy = torch.randn_like(q)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = ops.window_attention_train(q, k, v, window=50)
+    grads = torch.autograd.grad(y, (q, k, v), dy)
+graph.replay()
+want = ops.window_attention_train(q, k, v, window=50)
+assert torch.equal(y, want)
+assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(want, (q, k, v), dy)))
+assert ops.device_status() == 0
+""")
+
+
+def test_the_error_word_is_one_word_and_can_be_cleared():
+    """Threads that ask for it at once get the same word; what a kernel leaves there is read, told and cleared."""
+    import threading
+    ops.clear_device_status()
+    ops._ERRORS.clear()
+    words, gate, zeros = [], threading.Barrier(4), torch.zeros
+
+    def meet(*a, **kw):  # were a word made by the asking thread, all four would make theirs here
+        gate.wait(timeout=60)
+        return zeros(*a, **kw)
+
+    def ask():
+        gate.wait(timeout=60)
+        words.append(ops._error_word(0))
+
+    torch.zeros = meet
+    try:
+        threads = [threading.Thread(target=ask) for _ in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        torch.zeros = zeros
+    assert len(words) == 4 and len(set(words)) == 1
+
+    class Word:
+        __cuda_array_interface__ = dict(shape=(1,), typestr="<i4", data=(words[0], False), version=2)
+
+    word = torch.as_tensor(Word(), device=DEV)
+    assert word.data_ptr() == words[0]
+    word.fill_(L.GDNX_ETIMEOUT)
+    assert ops.device_status() == L.GDNX_ETIMEOUT
+    with pytest.raises(RuntimeError, match="ETIMEOUT"):
+        ops.check_device_status()
+    ops.clear_device_status()
+    assert ops.device_status() == 0 and int(word) == 0
+    ops.check_device_status()
