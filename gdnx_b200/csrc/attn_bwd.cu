@@ -729,7 +729,10 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const gdnx_attn_bwd_arg
 }
 
 // How the key tiles' iterations are cut: a part is about a full SM's share of all of them, at
-// least eight iterations; tiles that hold sinks are cut to the others' length.
+// least eight iterations; tiles that hold sinks are cut to the others' length, or to a quarter of an SM's
+// share where that is longer: at most eight parts an SM are kept in fp32 (155 MB), however many sinks there are
+// (16,384 tokens, 64 heads over 16 of 128, window 128, 2048 sinks: 104 MB and 5.1 ms of a training step; 2 GB and
+// 6.6 ms cut to the others' length).
 void plan(BwdParams& P) {
   const gdnx_attn_args& a = P.a;
   const int64_t G = a.H / a.Hk, bh = a.B * a.Hk;
@@ -742,14 +745,15 @@ void plan(BwdParams& P) {
   const int64_t it = G * near, it_sink = G * P.qtiles;
   const int64_t total = bh * (P.nst * it_sink + (P.ktiles - P.nst) * it);
   int64_t share = (total + 147) / 148;
+  const int64_t quarter = (share + 3) / 4;
   if (share < 8) share = 8;
   if (share > it) share = it > 8 ? it : 8;
-  const auto cut = [&](int64_t n) {
+  const auto cut = [](int64_t n, int64_t share) {
     const int64_t s = (n + share - 1) / share;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
   };
-  P.seg = cut(it);
-  P.seg_sink = cut(it_sink);
+  P.seg = cut(it, share);
+  P.seg_sink = cut(it_sink, share > quarter ? share : quarter);
 }
 
 size_t stats_floats(const BwdParams& P) { return (size_t)P.a.B * P.a.H * P.qtiles * TM; }

@@ -187,3 +187,17 @@ def test_oracle_write_refuses(rows, counts, T):
 def test_error_word_refuses_a_null_place():
     assert L.load().gdnx_error_word(None) == L.GDNX_EINVAL
     assert L.load().gdnx_error_status(None, 0, None) == L.GDNX_EINVAL
+
+
+@pytest.mark.parametrize("B,T,H,Hk,window,sinks", [
+    (1, 16384, 16, 16, 128, 2048), (1, 16384, 64, 16, 128, 2048), (4, 32768, 64, 8, 256, 32768), (64, 16384, 16, 16, 64, 16384),
+    (1, 16384, 8, 8, 128, 4), (2, 512, 16, 16, 128, 4)])
+def test_gradient_workspace_is_bounded_where_keys_are_seen_by_many_queries(B, T, H, Hk, window, sinks):
+    """Two statistics a query, and at most eight parts an SM (of 128 keys' dk and dv in fp32) beside one for each key tile
+    that holds sinks while there are fewer of those than that: 148 SMs, with or without a device to ask."""
+    a = _attn_args(B=B, Tq=T, Tk=T, H=H, Hk=Hk, D=128, window=window, sinks=sinks)
+    g = L.AttnBwdArgs(a)
+    need = L.load().gdnx_attn_bwd_workspace_bytes(C.byref(g))
+    statistics = 2 * 4 * B * H * T
+    part = 2 * 4 * 128 * 128
+    assert statistics <= need <= statistics + 16 + 8 * 148 * part
