@@ -85,9 +85,17 @@ __device__ int g_error_word;
 
 constexpr int64_t kMaxTokens = (int64_t)1 << 30;  // positions and their distances stay in int32
 
+// A device pointer on a multiple of `align` bytes.
+bool device_ptr(const void* p, size_t align) {
+  return reinterpret_cast<uintptr_t>(p) % align == 0 && is_device_ptr(p);
+}
+bool words(const int32_t* p) { return device_ptr(p, sizeof(int32_t)); }
+
+size_t bytes_of(int dtype) { return dtype == GDNX_F32 ? 4 : 2; }
+
 // A [B,T,H,D] operand: its pointer may be null where it has no elements.
 bool heads_ok(const gdnx_view& v, int dtype, int64_t D) {
-  return is_device_ptr(v.ptr) && v.dtype == dtype && v.dim == D && v.sb >= 0 && v.st >= 0 && v.sh >= 0;
+  return v.dtype == dtype && device_ptr(v.ptr, bytes_of(dtype)) && v.dim == D && v.sb >= 0 && v.st >= 0 && v.sh >= 0;
 }
 
 gdnx_status check_attn_sizes(const gdnx_attn_args& a) {
@@ -103,12 +111,12 @@ gdnx_status check_attn(const gdnx_attn_args& a) {
   const gdnx_status s = check_attn_sizes(a);
   if (s != GDNX_OK || a.B == 0 || a.Tk == 0) return s;
   if (!heads_ok(a.k, a.q.dtype, a.D) || !heads_ok(a.v, a.q.dtype, a.D)) return GDNX_EINVAL;
-  if (a.Tq > 0 && (!heads_ok(a.q, a.q.dtype, a.D) || !is_device_ptr(a.y))) return GDNX_EINVAL;
+  if (a.Tq > 0 && (!heads_ok(a.q, a.q.dtype, a.D) || !device_ptr(a.y, bytes_of(a.y_dtype)))) return GDNX_EINVAL;
   if (a.y_sb < 0 || a.y_st < 0 || a.y_sh < 0) return GDNX_EINVAL;
-  if (a.lengths && !is_device_ptr(a.lengths)) return GDNX_EINVAL;
-  if (a.lse && a.Tq > 0 && !is_device_ptr(a.lse)) return GDNX_EINVAL;
-  if (a.y_rest && a.Tq > 0 && (!is_device_ptr(a.y_rest) || a.y_dtype == GDNX_F32)) return GDNX_EINVAL;
-  if (a.error && !is_device_ptr(a.error)) return GDNX_EINVAL;
+  if (a.lengths && !words(a.lengths)) return GDNX_EINVAL;
+  if (a.lse && a.Tq > 0 && !device_ptr(a.lse, sizeof(float))) return GDNX_EINVAL;
+  if (a.y_rest && a.Tq > 0 && (!device_ptr(a.y_rest, 2) || a.y_dtype == GDNX_F32)) return GDNX_EINVAL;
+  if (a.error && !words(a.error)) return GDNX_EINVAL;
   return GDNX_OK;
 }
 
@@ -128,9 +136,8 @@ gdnx_status check_cache(const gdnx_cache* c) {
   if (c->D > 128 || c->D % 8 || c->slots > (1 << 18) || c->width > (1 << 20) || c->width * c->page > kMaxTokens ||
       c->pages > ((int64_t)1 << 30))
     return GDNX_EUNSUPPORTED;
-  if (c->pages && (!is_device_ptr(c->kv) || reinterpret_cast<uintptr_t>(c->kv) % 16 || !is_device_ptr(c->refs)))
-    return GDNX_EINVAL;
-  if (!is_device_ptr(c->table) || !is_device_ptr(c->lengths) || !is_device_ptr(c->status)) return GDNX_EINVAL;
+  if (c->pages && (!device_ptr(c->kv, 16) || !words(c->refs))) return GDNX_EINVAL;
+  if (!words(c->table) || !words(c->lengths) || !words(c->status)) return GDNX_EINVAL;
   return GDNX_OK;
 }
 
@@ -139,7 +146,7 @@ gdnx_status check_rows(const gdnx_cache* c, int64_t n, const int32_t* rows, cons
   const gdnx_status s = check_cache(c);
   if (s != GDNX_OK) return s;
   if (n < 0 || n > c->slots) return GDNX_EINVAL;
-  if (n && (!is_device_ptr(rows) || !is_device_ptr(more))) return GDNX_EINVAL;
+  if (n && (!words(rows) || !words(more))) return GDNX_EINVAL;
   return GDNX_OK;
 }
 
@@ -197,15 +204,16 @@ gdnx_status gdnx_attn_bwd(const gdnx_attn_bwd_args* g, void* stream) {
   const gdnx_attn_args& a = g->fwd;
   const gdnx_status s = check_attn(a);
   if (s != GDNX_OK || a.B == 0 || a.Tk == 0) return s;
-  if (!is_device_ptr(g->dk) || !is_device_ptr(g->dv)) return GDNX_EINVAL;
+  const size_t es = bytes_of(a.q.dtype);
+  if (!device_ptr(g->dk, es) || !device_ptr(g->dv, es)) return GDNX_EINVAL;
   const cudaStream_t st = (cudaStream_t)stream;
   if (a.Tq == 0) {  // nothing was read: the gradients are zero
-    const size_t bytes = (size_t)(a.B * a.Tk * a.Hk * a.D) * (a.k.dtype == GDNX_F32 ? 4 : 2);
+    const size_t bytes = (size_t)(a.B * a.Tk * a.Hk * a.D) * es;
     return cudaMemsetAsync(g->dk, 0, bytes, st) == cudaSuccess && cudaMemsetAsync(g->dv, 0, bytes, st) == cudaSuccess
                ? GDNX_OK : GDNX_ELAUNCH;
   }
-  if (!heads_ok(g->dy, a.q.dtype, a.D) || !is_device_ptr(g->dq) || !a.lse) return GDNX_EINVAL;
-  if (g->workspace_bytes < gdnx_attn_bwd_workspace_bytes(g) || !is_device_ptr(g->workspace)) return GDNX_EWORKSPACE;
+  if (!heads_ok(g->dy, a.q.dtype, a.D) || !device_ptr(g->dq, es) || !a.lse) return GDNX_EINVAL;
+  if (g->workspace_bytes < gdnx_attn_bwd_workspace_bytes(g) || !device_ptr(g->workspace, sizeof(float))) return GDNX_EWORKSPACE;
   gdnx_attn_bwd_args c = *g;
   c.fwd = clamp_attn(a);
   if (a.q.dtype == GDNX_BF16) {
@@ -230,7 +238,7 @@ gdnx_status gdnx_cache_extend(const gdnx_cache* c, int64_t n, const int32_t* row
                               void* workspace, size_t workspace_bytes, void* stream) {
   const gdnx_status s = check_rows(c, n, rows, counts);
   if (s != GDNX_OK || n == 0) return s;
-  if (workspace_bytes < gdnx_cache_workspace_bytes(c, n) || !is_device_ptr(workspace)) return GDNX_EWORKSPACE;
+  if (workspace_bytes < gdnx_cache_workspace_bytes(c, n) || !device_ptr(workspace, sizeof(int32_t))) return GDNX_EWORKSPACE;
   return gdnx::launch_cache_extend(*c, n, rows, counts, workspace, (cudaStream_t)stream);
 }
 
@@ -240,8 +248,8 @@ gdnx_status gdnx_cache_write(const gdnx_cache* c, int64_t layer, int64_t n, int6
   if (s != GDNX_OK) return s;
   if (layer < 0 || layer >= c->L || n < 0 || n > c->slots || T < 0 || !k || !v) return GDNX_EINVAL;
   if (n == 0 || T == 0) return GDNX_OK;
-  if (!heads_ok(*k, c->dtype, c->D) || !heads_ok(*v, c->dtype, c->D) || !is_device_ptr(rows)) return GDNX_EINVAL;
-  if (counts && !is_device_ptr(counts)) return GDNX_EINVAL;
+  if (!heads_ok(*k, c->dtype, c->D) || !heads_ok(*v, c->dtype, c->D) || !words(rows)) return GDNX_EINVAL;
+  if (counts && !words(counts)) return GDNX_EINVAL;
   return gdnx::launch_cache_write(*c, layer, n, T, *k, *v, rows, counts, (cudaStream_t)stream);
 }
 
@@ -262,7 +270,7 @@ gdnx_status gdnx_cache_trim(const gdnx_cache* c, int64_t n, const int32_t* rows,
 gdnx_status gdnx_cache_compact(const gdnx_cache* c, void* workspace, size_t workspace_bytes, void* stream) {
   const gdnx_status s = check_cache(c);
   if (s != GDNX_OK || c->pages == 0) return s;
-  if (workspace_bytes < gdnx_cache_workspace_bytes(c, 0) || !is_device_ptr(workspace)) return GDNX_EWORKSPACE;
+  if (workspace_bytes < gdnx_cache_workspace_bytes(c, 0) || !device_ptr(workspace, sizeof(int32_t))) return GDNX_EWORKSPACE;
   return gdnx::launch_cache_compact(*c, workspace, (cudaStream_t)stream);
 }
 
@@ -284,9 +292,9 @@ static gdnx_status check_decode(const gdnx_paged_decode_args& a) {
   if (a.B > 65535 || a.H > 65535) return GDNX_EUNSUPPORTED;
   if (!a.rows && a.B > a.cache.slots) return GDNX_EINVAL;
   if (a.B == 0) return GDNX_OK;
-  if (!heads_ok(a.q, a.cache.dtype, a.cache.D) || !is_device_ptr(a.y) || a.y_sb < 0 || a.y_sh < 0) return GDNX_EINVAL;
-  if (a.rows && !is_device_ptr(a.rows)) return GDNX_EINVAL;
-  if (a.error && !is_device_ptr(a.error)) return GDNX_EINVAL;
+  if (!heads_ok(a.q, a.cache.dtype, a.cache.D) || !device_ptr(a.y, bytes_of(a.y_dtype)) || a.y_sb < 0 || a.y_sh < 0) return GDNX_EINVAL;
+  if (a.rows && !words(a.rows)) return GDNX_EINVAL;
+  if (a.error && !words(a.error)) return GDNX_EINVAL;
   return GDNX_OK;
 }
 
@@ -302,7 +310,7 @@ gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* a, void* stream) {
   const gdnx_status s = check_decode(*a);
   if (s != GDNX_OK || a->B == 0) return s;
   const size_t need = gdnx_paged_decode_workspace_bytes(a);
-  if (need && (a->workspace_bytes < need || !is_device_ptr(a->workspace))) return GDNX_EWORKSPACE;
+  if (need && (a->workspace_bytes < need || !device_ptr(a->workspace, 16))) return GDNX_EWORKSPACE;
   const gdnx_paged_decode_args c = clamp_decode(*a);
   return c.cache.dtype == GDNX_F32 ? gdnx::launch_paged_decode(c, (cudaStream_t)stream)
                                    : gdnx::launch_paged_decode_tc(c, (cudaStream_t)stream);

@@ -415,7 +415,9 @@ GDNX_API gdnx_status gdnx_error_status(int32_t* value, int32_t clear, void* stre
  *   y_i = sum_j softmax_j(scale q_i.k_j) v_j ;  query head h reads key head h / (H / Hk).
  * Scores, softmax statistics and sums are fp32; 16-bit inputs run on the tensor cores
  * where TMA can address them, other types and layouts on the CUDA cores.
- * A row that sees a score of NaN or +inf, or only -inf, is NaN (y and lse). */
+ * A row that sees a score of NaN or +inf, or only -inf, is NaN (y and lse).
+ * Here and below, pointers that are not on a multiple of their elements' size are GDNX_EINVAL
+ * (a workspace: GDNX_EWORKSPACE). */
 typedef struct {
   int64_t B, Tq, Tk, H, Hk, D; /* Tq <= Tk; H a multiple of Hk; D <= 128, a multiple of 8 */
   int64_t window, sinks;       /* window >= 1 (Tk or more: plain causal), sinks >= 0       */
@@ -518,7 +520,7 @@ typedef struct {
   int32_t y_dtype;
   int64_t y_sb, y_sh;
   int32_t* error;              /* device word that takes GDNX_ETIMEOUT; NULL = none */
-  void* workspace;
+  void* workspace;             /* 16-byte aligned */
   size_t workspace_bytes;
 } gdnx_paged_decode_args;
 

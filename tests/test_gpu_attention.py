@@ -456,3 +456,71 @@ def test_the_error_word_is_one_word_and_can_be_cleared():
     ops.clear_device_status()
     assert ops.device_status() == 0 and int(word) == 0
     ops.check_device_status()
+
+
+def _forward_args(q, k, v, lengths):
+    a, index = ops._attn_args(q, k, v, 16, 2, None, lengths)
+    y, lse = torch.empty_like(q), torch.empty(q.shape[0], q.shape[2], q.shape[1], device=DEV)
+    a.y, a.y_dtype, a.lse = y.data_ptr(), ops._DT[y.dtype], lse.data_ptr()
+    a.y_sb, a.y_st, a.y_sh, _ = y.stride()
+    return a, (y, lse)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_c_entries_refuse_pointers_between_elements(dtype):
+    """Refused on the host, before any launch.  (Every address asked for lies inside its tensor.)"""
+    import ctypes as C
+    lib = L.load()
+    lengths = torch.full((2,), 24, dtype=torch.int32, device=DEV)
+    q, k, v, dy = make(2, 32, 32, 4, 2, 64, dtype)
+
+    def moved(s, field, by, call, status=L.GDNX_EINVAL):
+        at = s
+        *path, last = field.split(".")
+        for name in path:
+            at = getattr(at, name)
+        was = getattr(at, last)
+        setattr(at, last, was + by)
+        assert call() == status, field
+        setattr(at, last, was)
+
+    a, keep = _forward_args(q, k, v, lengths)
+    forward = lambda: lib.gdnx_attn_fwd(C.byref(a), None)  # noqa: E731
+    for field in ("q.ptr", "k.ptr", "v.ptr", "y", "lse", "lengths", "error"):
+        moved(a, field, 1, forward)
+    g = L.AttnBwdArgs(a, ops._heads_view(dy))
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    g.dq, g.dk, g.dv = (t.data_ptr() for t in grads)
+    ws = torch.empty(lib.gdnx_attn_bwd_workspace_bytes(C.byref(g)) + 16, dtype=torch.uint8, device=DEV)
+    g.workspace, g.workspace_bytes = ws.data_ptr(), ws.numel() - 16
+    backward = lambda: lib.gdnx_attn_bwd(C.byref(g), None)  # noqa: E731
+    for field in ("fwd.q.ptr", "fwd.lse", "dy.ptr", "dq", "dk", "dv"):
+        moved(g, field, 1, backward)
+    moved(g, "workspace", 1, backward, L.GDNX_EWORKSPACE)
+
+    c = ops.PagedCache.zeros(1, 200, 2, 16, 64, slots=2, width=100, dtype=TYPES[dtype], device=DEV)
+    rows = torch.arange(2, dtype=torch.int32, device=DEV)
+    s, _ = ops._cache_struct(c)
+    y = torch.empty_like(q[:, 0])
+    d = L.PagedDecodeArgs(s, 2, 4, 0, 1 << 40, 0, 0, 0.125, ops._heads_view(q[:, :1]), rows.data_ptr(), y.data_ptr(),
+                          ops._DT[y.dtype], 256, 64, ops._error_word(0))
+    room = torch.empty(lib.gdnx_paged_decode_workspace_bytes(C.byref(d)) + 16, dtype=torch.uint8, device=DEV)
+    assert room.numel() > 16
+    d.workspace, d.workspace_bytes = room.data_ptr(), room.numel() - 16
+    decode = lambda: lib.gdnx_paged_decode(C.byref(d), None)  # noqa: E731
+    for field in ("q.ptr", "y", "rows", "error", "cache.table", "cache.lengths", "cache.refs", "cache.status"):
+        moved(d, field, 1, decode)
+    moved(d, "cache.kv", 8, decode)
+    moved(d, "workspace", 8, decode, L.GDNX_EWORKSPACE)
+    kv = ops._heads_view(k)
+    for by in ((1, 0, 0), (0, 1, 0), (0, 0, 1)):
+        at = L.View.from_buffer_copy(kv)
+        at.ptr += by[0]
+        assert lib.gdnx_cache_write(C.byref(s), 0, 2, 32, C.byref(at), C.byref(kv), rows.data_ptr() + by[1],
+                                    lengths.data_ptr() + by[2], None) == L.GDNX_EINVAL
+    assert lib.gdnx_cache_truncate(C.byref(s), 1, rows.data_ptr() + 2, rows.data_ptr(), None) == L.GDNX_EINVAL
+    assert lib.gdnx_cache_extend(C.byref(s), 1, rows.data_ptr(), rows.data_ptr(), room.data_ptr() + 1, 1 << 40,
+                                 None) == L.GDNX_EWORKSPACE
+    assert lib.gdnx_cache_compact(C.byref(s), room.data_ptr() + 2, 1 << 40, None) == L.GDNX_EWORKSPACE
+    torch.cuda.synchronize()
+    ops.cache_check(c)
