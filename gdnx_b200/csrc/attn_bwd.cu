@@ -1,4 +1,4 @@
-// Windowed attention, gradients, on the tensor cores (16-bit inputs that TMA can address).
+// Windowed attention, gradients, on the tensor cores (bfloat16 inputs that TMA can address).
 //
 // Two kernels recompute P from lse and write every gradient once, in a fixed order: seven
 // products of a tile instead of five, against atomics (whose order would show in the bits)
@@ -65,13 +65,6 @@ struct Layout {
                             END = BARS + 512;
   static constexpr size_t SMEM = END + 512;  // the base is 1024-aligned: there is no static shared memory
 };
-
-// Bits lo..hi (inclusive) of the 32-bit word that holds columns 32w..32w+31.
-GDNX_DEV uint32_t range_bits(int lo, int hi, int w) {
-  lo = max(lo - 32 * w, 0);
-  hi = min(hi - 32 * w, 31);
-  return lo > hi ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
-}
 
 // D (+)= P X with P's columns in four quarters, each over the start of its 32 of 128 columns.
 GDNX_DEV void mma_quarters(uint32_t d, uint32_t p, uint32_t x, uint32_t idesc, bool acc) {
@@ -690,7 +683,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_bwd_tc_kernel(const __grid_c
 
 // Minus lse in the log2 domain and minus delta = sum_d dy y, padded to whole tiles of queries: eight lanes
 // for each row.
-template <typename T>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const gdnx_attn_bwd_args g, float* lse2, float* delta,
                                                          unsigned* next, int qpad) {
   dependents_may_start();
@@ -778,7 +770,7 @@ gdnx_status run(const gdnx_attn_bwd_args& g, BwdParams& P, cudaStream_t st) {
   static std::atomic<uint64_t> done_keys, done_queries;
   if (!allow_smem(keys, smem, done_keys) || !allow_smem(queries, smem, done_queries)) return GDNX_ELAUNCH;
   const int64_t rows = (int64_t)stats_floats(P);
-  attn_stats_kernel<__nv_bfloat16><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(
+  attn_stats_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(
       g, const_cast<float*>(P.lse2), const_cast<float*>(P.delta), P.next, P.qtiles * TM);
   if (cudaGetLastError() != cudaSuccess ||
       launch_early(keys, dim3((unsigned)items_of(P)), dim3(NTHREADS), smem, st, P) != cudaSuccess)

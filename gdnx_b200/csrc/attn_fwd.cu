@@ -139,13 +139,6 @@ struct Layout {
   static constexpr size_t SMEM = SMALL + sizeof(Small);  // no static shared memory: the base is 1024-aligned
 };
 
-// Bits lo..hi (inclusive, any integers) of the 32-bit word that holds columns 32w..32w+31.
-GDNX_DEV uint32_t range_bits(int lo, int hi, int w) {
-  lo = max(lo - 32 * w, 0);
-  hi = min(hi - 32 * w, 31);
-  return lo > hi ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
-}
-
 // Weights of N columns: p = 2^(c2 s - mc), summed, packed 16-bit.  One pair in eight is taken on
 // the FMA pipes (where masked scores give 2^-125: nothing beside a weight that counts).
 template <bool BF16, int N>

@@ -62,8 +62,8 @@ GDNX_DEV bool elect_one() {
   return ok != 0;
 }
 
-// The issuing thread is one thread: descriptors are built once and stepped by constants (their
-// address field counts 16-byte units), which keeps a product's issue well below its run time.
+// Descriptors are built once and stepped by constants (their address field counts 16-byte units), which
+// keeps a product's issue well below its run time.
 
 // D[128 x N] = A B^T over the head dimension: both tiles K-major in shared memory.
 template <int DB>
@@ -165,29 +165,7 @@ GDNX_DEV void tmem_ld64(uint32_t taddr, float* v) {
       : "memory");
 }
 
-// 32 lanes x n columns of raw words.
-GDNX_DEV void tmem_st64u(uint32_t taddr, const uint32_t (&v)[64]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x64.b32 [%0], {"
-      "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,"
-      "%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,"
-      "%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,%64"
-      "};\n\t"
-      "tcgen05.wait::st.sync.aligned;"
-      :
-      : "r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
-        "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
-        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]),
-        "r"(v[32]), "r"(v[33]), "r"(v[34]), "r"(v[35]), "r"(v[36]), "r"(v[37]), "r"(v[38]), "r"(v[39]),
-        "r"(v[40]), "r"(v[41]), "r"(v[42]), "r"(v[43]), "r"(v[44]), "r"(v[45]), "r"(v[46]), "r"(v[47]),
-        "r"(v[48]), "r"(v[49]), "r"(v[50]), "r"(v[51]), "r"(v[52]), "r"(v[53]), "r"(v[54]), "r"(v[55]),
-        "r"(v[56]), "r"(v[57]), "r"(v[58]), "r"(v[59]), "r"(v[60]), "r"(v[61]), "r"(v[62]), "r"(v[63])
-      : "memory");
-}
-
+// 32 lanes x 32 columns of raw words.
 GDNX_DEV void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
@@ -204,20 +182,18 @@ GDNX_DEV void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
       : "memory");
 }
 
-GDNX_DEV void tmem_st8u(uint32_t taddr, const uint32_t (&v)[8]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n\t"
-      "tcgen05.wait::st.sync.aligned;"
-      :
-      : "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-      : "memory");
-}
-
 GDNX_DEV void tma_store_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
                "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(src)
                : "memory");
+}
+
+// Bits lo..hi (inclusive, any integers) of the 32-bit word that holds columns 32w..32w+31.
+GDNX_DEV uint32_t range_bits(int lo, int hi, int w) {
+  lo = max(lo - 32 * w, 0);
+  hi = min(hi - 32 * w, 31);
+  return lo > hi ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
 }
 
 // Two fp32 operations in one instruction.
@@ -296,22 +272,8 @@ inline EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// The device's number of SMs, and whether a kernel may use `smem` bytes of dynamic shared memory
-// there (set on its first launch on a device: `done` has a bit for each).
-inline int sm_count() {
-  static std::atomic<int> sms[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 148;
-  int n = sms[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-      cudaGetLastError();
-      return 148;
-    }
-    sms[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
+// Whether a kernel may use `smem` bytes of dynamic shared memory on the current device (set on its first launch
+// there: `done` has a bit for each).
 template <typename F>
 bool allow_smem(F kernel, int smem, std::atomic<uint64_t>& done) {
   int dev = 0;

@@ -4,9 +4,29 @@
 // every kernel before it has ended and its writes are visible.
 #pragma once
 
+#include <atomic>
 #include <cuda_runtime.h>
 
 namespace gdnx {
+
+// The current device's number of SMs (148 where it cannot be asked).
+inline int sm_count() {
+  static std::atomic<int> sms[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) {
+    cudaGetLastError();
+    return 148;
+  }
+  int n = sms[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+      cudaGetLastError();
+      return 148;
+    }
+    sms[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
 __device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
