@@ -736,7 +736,8 @@ void plan(BwdParams& P) {
   if (near > P.qtiles) near = P.qtiles;
   const int64_t it = G * near, it_sink = G * P.qtiles;
   const int64_t total = bh * (P.nst * it_sink + (P.ktiles - P.nst) * it);
-  int64_t share = (total + 147) / 148;
+  const int64_t sms = sm_count();
+  int64_t share = (total + sms - 1) / sms;
   const int64_t quarter = (share + 3) / 4;
   if (share < 8) share = 8;
   if (share > it) share = it > 8 ? it : 8;

@@ -425,7 +425,7 @@ int elem(int dtype) { return dtype == GDNX_F32 ? 4 : 2; }
 
 gdnx_status copy_pages(const gdnx_cache& c, void* ws, int64_t n, int rename, cudaStream_t st) {
   const int64_t run = c.Hk * c.page * c.D * elem(c.dtype);
-  return launched(launch_early(cache_copy_kernel, dim3(148 * 8), dim3(COPY_NT), 0, st, c, ws, n, run, rename));
+  return launched(launch_early(cache_copy_kernel, dim3(sm_count() * 8), dim3(COPY_NT), 0, st, c, ws, n, run, rename));
 }
 
 }  // namespace
@@ -472,7 +472,7 @@ cudaError_t write_pieces(const gdnx_cache& c, int64_t layer, int64_t n, int64_t 
   };
   const bool v16 = wide(k) && wide(v);
   const int64_t all = n * T * c.Hk * (v16 ? c.D / vec : c.D) * 2;
-  const int64_t most = 148 * 64;
+  const int64_t most = sm_count() * 64;
   const unsigned grid = (unsigned)((all + WRITE_NT - 1) / WRITE_NT < most ? (all + WRITE_NT - 1) / WRITE_NT : most);
   const auto kernel = v16 ? cache_write_kernel<uint4, CHECK>
                       : es == 4 ? cache_write_kernel<uint32_t, CHECK> : cache_write_kernel<uint16_t, CHECK>;
