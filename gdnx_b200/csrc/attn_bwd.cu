@@ -19,15 +19,17 @@
 //
 // attn_dkv's blocks take their key tile whole, which leaves SMs idle at its end (256 tiles on 148
 // SMs: two rounds).  So attn_dq starts there as they fall free and deals its items out by a
-// counter: together they end evenly (348 us of a step with 2 x 4096 tokens, 16 heads over 4 of
-// 128, window 1024; 378 us one after the other).
+// counter: together they end evenly (2 x 4096 tokens, 16 heads over 4 of 128, window 1024: 8 % less of a whole
+// step than one after the other).
 //
-// Measured at those sizes: 24 us for delta (y, what its rounding left, and dy: 4.1 TB/s), 147 us until
-// dK, dV are done, 229 us in all.  An iteration of dK, dV takes 2850 cycles where its four products take
-// 2048: the rows hold the products up between P and dS.
+// Measured at those sizes: a step with its forward takes 388 us in a sustained run (under the 1000 W cap), 352 to
+// 358 us by itself.  Of the latter 24 us are delta's (y, what its rounding left, and dy: 4.1 TB/s), 147 us
+// pass until dK, dV are done, 229 us in all.  An iteration of dK, dV takes 2850 cycles where its four products
+// take 2048: the rows hold the products up between P and dS.
 //
-// Weights and dS are rounded to bf16 for the products, like the inputs themselves; dS of
-// float16 inputs could leave float16's range, so those take the CUDA-core kernels.
+// Weights and dS are rounded to bf16 for the products, like the inputs themselves (the tensor cores take both factors
+// in one type; it leaves dq, dk, dv 1.4 times as far from 64 bits as rounding the results alone would); dS of
+// float16 inputs could leave float16's range, so those take the CUDA-core kernels (9.9 ms at the sizes above).
 #include "attn_tc.cuh"
 #include "kernels.h"
 #include "launch.cuh"

@@ -26,12 +26,13 @@
 // round, which starts as the first one's blocks leave SMs free: each block of queries has a CTA to itself, the
 // two stages take its key tiles in turn and stage 0 joins the two outputs, in tensor memory both.  That
 // is the whole work of a single short prompt (1024 tokens, 16 heads: 23 -> 17 us; 512 tokens after 7680,
-// window 4096: 68 -> 44 us), and balances long ones (8192 after 8192: 262 -> 246 us).
+// window 4096: 68 -> 44 us), and balances long ones (8192 after 8192: 6 % less).
 //
-// Measured: 8 x 4096 tokens, 16 heads over 4 of 128, window 1024, 4 sinks, bf16: 272 us (888 TFLOP/s of
-// visible pairs, 53 % of a large matrix product's rate; 317 us at the 1.69 GHz of a sustained run); 8192
-// tokens after 8192, window 4096: 246 us (1135 TFLOP/s).  A pair of tiles takes the tensor cores 2048
-// cycles and lasts 3350: each stage's rows take longer than the other stage's products.
+// Measured: 8 x 4096 tokens, 16 heads over 4 of 128, window 1024, 4 sinks, bf16: 322 us in a sustained run, which the
+// 1000 W cap holds at 1.69 GHz (749 TFLOP/s of visible pairs, 45 % of a large matrix product's rate), 286 us for a
+// call by itself; 8192 tokens after 8192, window 4096: 287 us (973 TFLOP/s), 257 us by itself.  A pair of tiles
+// takes the tensor cores 2048 cycles and lasts 3350: each stage's rows take longer than the other stage's products.
+// Maxima that keep NaN cost 2 us of these.
 #include "attn_tc.cuh"
 #include "kernels.h"
 #include "launch.cuh"

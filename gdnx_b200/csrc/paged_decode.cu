@@ -10,7 +10,9 @@
 // with the maximum m moved only where a score lies more than 8 above it (a vote of the warp).
 // The groups' (m, l, o) are joined when the unit ends.
 //
-// Measured: 64 sequences of 4096 tokens, 16 heads over 4 of 128: 223 us, 4.8 TB/s; one of 16,384 tokens: 27 us.
+// Measured: 64 sequences of 4096 tokens, 16 heads over 4 of 128: 228 us, 4.7 TB/s; one of 16,384 tokens: 34 us with
+// nothing in L2.  Two warps a scheduler issue in 52 % of cycles and have one ready in as many: a warp's chain of
+// dot product, exponential and sums, not the loads, is what the ring waits for.
 #include "paged_decode.cuh"
 
 namespace gdnx {

@@ -4,7 +4,9 @@
 // A tile.  With the keys as rows the products are narrow and nothing is padded to 128 but the
 // heads to NH:  S^T [128 keys x NH] = K Q^T,  O^T [128 dims x NH] += V^T P  (V read with its
 // rows as K; of head sizes up to 64 lanes 64.. read shifted rows and are not used).  Thread j owns
-// key j: p_h = 2^(c s_jh - m_h), written 16-bit to shared memory as the right factor.  The maxima m are those of the first tile and move only when some score lies
+// key j: p_h = 2^(c s_jh - m_h), written to shared memory as the right factor, in the cache's type (both
+// factors of a product have one; a weight's rounding averages out over the keys like V's own, and the
+// sums take it unrounded).  The maxima m are those of the first tile and move only when some score lies
 // more than 8 above (p stays below 2^8), so a tile costs one vote and no reduction; sums stay
 // in the threads until the unit ends.
 //

@@ -992,7 +992,8 @@ def window_attention(q, k, v, *, window: Optional[int] = None, sinks: int = 0, s
     Query i stands at position p = Tk - Tq + i and sees key j where j <= p and p - j < ``window``
     (None: no window) or j < ``sinks``.  ``lengths`` [B] int32 are the valid tokens of right-padded
     sequences: keys from there on are not seen, and queries from there on give zeros, whatever the
-    padding holds.  ``scale`` defaults to D ** -0.5.  Returns y [B,Tq,H,D] (and the log of the sum
+    padding holds.  Elsewhere values are meant to be finite; a row that sees a score of NaN or +inf, or only
+    -inf, is NaN.  ``scale`` defaults to D ** -0.5.  Returns y [B,Tq,H,D] (and the log of the sum
     of exponentials [B,H,Tq] fp32 if asked, -inf where a row is padding)."""
     y, lse, _ = _window_attention(q, k, v, window, sinks, scale, lengths, out, out_dtype, return_lse, False)
     return (y, lse) if return_lse else y
