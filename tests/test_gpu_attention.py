@@ -524,3 +524,9 @@ def test_c_entries_refuse_pointers_between_elements(dtype):
     assert lib.gdnx_cache_compact(C.byref(s), room.data_ptr() + 2, 1 << 40, None) == L.GDNX_EWORKSPACE
     torch.cuda.synchronize()
     ops.cache_check(c)
+
+
+@pytest.mark.parametrize("T,H,Hk,window,sinks", [(1500, 64, 16, 60, 900), (1100, 16, 16, 40, 1100), (900, 12, 4, 128, 300)])
+def test_gradients_where_many_keys_are_sinks(T, H, Hk, window, sinks):
+    """Key tiles that every later query sees, cut into parts of more than a tile's own length, into such parts, and whole."""
+    check(*make(1, T, T, H, Hk, 64, "bf16", seed=T), "bf16", window=window, sinks=sinks)
