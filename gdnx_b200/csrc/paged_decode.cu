@@ -10,7 +10,7 @@
 // with the maximum m moved only where a score lies more than 8 above it (a vote of the warp).
 // The groups' (m, l, o) are joined when the unit ends.
 //
-// Measured: 64 sequences of 4096 tokens, 16 heads over 4 of 128: 228 us, 4.7 TB/s; one of 16,384 tokens: 34 us with
+// Measured: 64 sequences of 4096 tokens, 16 heads over 4 of 128: 230 us, 4.7 TB/s; one of 16,384 tokens: 34 us with
 // nothing in L2.  Two warps a scheduler issue in 52 % of cycles and have one ready in as many: a warp's chain of
 // dot product, exponential and sums, not the loads, is what the ring waits for.
 #include "paged_decode.cuh"
@@ -96,6 +96,7 @@ GDNX_DEV void use_stages(const DecParams& P, Walk w, int64_t per, const uint8_t*
   while (w.next()) {
     const Heads hd(P, w.unit, NH);
     float q[NH][8], o[NH][8], m[NH], l[NH];
+    bool any = false;  // this lane's group saw a token
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       m[h] = -INFINITY;
@@ -125,6 +126,7 @@ GDNX_DEV void use_stages(const DecParams& P, Walk w, int64_t per, const uint8_t*
         for (int i = 0; i < PASSES; ++i) {
           const int r = warp * (SUB / WARPS) + i * KPW + sub, j = j0 + r;
           seen[i] = key_seen(j, w.seq.len, window, sinks) && (on_page >> (r / 16) & 1);
+          any |= seen[i];
           float4 k0 = make_float4(0.f, 0.f, 0.f, 0.f), k1 = k0;
           if (seen[i] && d0 < D) k0 = *reinterpret_cast<const float4*>(kt + r * D + d0);
           if (seen[i] && d1 < D) k1 = *reinterpret_cast<const float4*>(kt + r * D + d1);
@@ -184,6 +186,7 @@ GDNX_DEV void use_stages(const DecParams& P, Walk w, int64_t per, const uint8_t*
     // the groups of a warp, then the warps in order
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
+      if (any) m[h] = fmaxf(m[h], kNoScore);
       float top = m[h];
 #pragma unroll
       for (int z = LPK; z < 32; z <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, z));
@@ -223,7 +226,7 @@ GDNX_DEV void use_stages(const DecParams& P, Walk w, int64_t per, const uint8_t*
         y = fmaf(z, sm.o[k][h][d], y);
       }
       if (whole) {
-        st_from_f32(a.y, a.y_dtype, w.b * a.y_sb + (hd.h0 + h) * a.y_sh + d, sum == 0.f ? 0.f : y / sum);
+        st_from_f32(a.y, a.y_dtype, w.b * a.y_sb + (hd.h0 + h) * a.y_sh + d, sum == 0.f ? no_weights(top) : y / sum);
       } else {
         P.part[(at + h) * 128 + d] = y;
         if (d == 0) {

@@ -162,6 +162,12 @@ GDNX_DEV int page_id(const DecParams& P, const Seq& s, int kt, int i) {
   return p >= 0 && p < c.pages ? p : -1;
 }
 
+// What stands for the maximum where something is seen but no score lies above -inf (nothing seen: -inf).
+constexpr float kNoScore = -3.402823466e38f;
+
+// The output where the weights' sum is 0.
+GDNX_DEV float no_weights(float top) { return top == -INFINITY ? 0.f : NAN; }
+
 // Zeros for the sequences that see nothing.
 GDNX_DEV void write_zeros(const DecParams& P) {
   const gdnx_paged_decode_args& a = P.a;
@@ -207,11 +213,11 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_decode_join_kernel(cons
   for (int c = r0 + lane; c < r1; c += 32) m = fmaxf(m, P.stat[place(c) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float ref = m == -INFINITY ? 0.f : m;
+  const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll 4
   for (int c = r0; c < r1; ++c) {
     const int64_t at = place(c);
-    const float w = exp2f(P.stat[at * 2] - ref);
+    const float w = exp2f(P.stat[at * 2] - base);
     const float4 x = *reinterpret_cast<const float4*>(P.part + at * 128 + lane * 4);
     l = fmaf(w, P.stat[at * 2 + 1], l);
     y.x = fmaf(w, x.x, y.x);
@@ -230,14 +236,14 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_decode_join_kernel(cons
   float top = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll
   for (int i = 0; i < JOIN_WARPS; ++i) top = fmaxf(top, red_m[i]);
-  if (top == -INFINITY) top = 0.f;
+  const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
   for (int i = 0; i < JOIN_WARPS; ++i) {
-    const float w = exp2f(red_m[i] - top);
+    const float w = exp2f(red_m[i] - ref);
     sum = fmaf(w, red_l[i], sum);
     v = fmaf(w, red_o[i][d], v);
   }
-  st_from_f32(a.y, a.y_dtype, out + d, sum == 0.f ? 0.f : v / sum);
+  st_from_f32(a.y, a.y_dtype, out + d, sum == 0.f ? no_weights(top) : v / sum);
 }
 
 // The plan of a call with groups of `nh` query heads.

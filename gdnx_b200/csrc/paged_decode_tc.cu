@@ -232,6 +232,7 @@ GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, ui
   while (w.next()) {
     const Heads hd(P, w.unit, NH);
     float m[NC], l[NC];
+    bool any = false;  // this thread saw a key
 #pragma unroll
     for (int h = 0; h < NC; ++h) {
       m[h] = -INFINITY;
@@ -245,6 +246,7 @@ GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, ui
         const int p = a.cache.table[(int64_t)w.seq.row * a.cache.width + j / a.cache.page];
         seen = p >= 0 && p < a.cache.pages;
       }
+      any |= seen;
       ok = ok && warp_wait(&bar.s_full[nt & 1], nt / 2 & 1, abort_flag);
       tc::fence_after();
       float s[NC];
@@ -302,10 +304,11 @@ GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, ui
       tc::fence_before();
       pipe::mbar_arrive(&bar.p_ready[nt & 1]);
     }
-    // the unit's sums, then its output: lane d of tensor memory holds dimension d
+    // the unit's sums, then its output: lane d of tensor memory holds dimension d.  (Without a score above -inf
+    // the sums tell whether a key was seen.)
 #pragma unroll
     for (int h = 0; h < NC; ++h) {
-      const float x = warp_sum(l[h]);
+      const float x = warp_sum(any && m[h] == -INFINITY ? l[h] + 1.f : l[h]);
       if (lane == 0) red[warp * NH + h] = x;
     }
     if (pipe::group_any(1, 128, !ok)) return;
@@ -319,14 +322,19 @@ GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, ui
 #pragma unroll
     for (int h = 0; h < NC; ++h) {
       if (h >= hd.n) continue;
-      const float sum = red[h] + red[NH + h] + red[2 * NH + h] + red[3 * NH + h];
+      float sum = red[h] + red[NH + h] + red[2 * NH + h] + red[3 * NH + h], top = m[h];
+      if (top == -INFINITY && sum > 0.f) {
+        top = kNoScore;
+        sum = 0.f;
+      }
       if (whole) {
-        const float inv = sum > 0.f ? 1.f / sum : sum != sum ? sum : 0.f;
-        if (r < D) st_from_f32(a.y, a.y_dtype, w.b * a.y_sb + (hd.h0 + h) * a.y_sh + r, sum == 0.f ? 0.f : o[h] * inv);
+        if (r < D)
+          st_from_f32(a.y, a.y_dtype, w.b * a.y_sb + (hd.h0 + h) * a.y_sh + r,
+                      sum == 0.f ? no_weights(top) : o[h] * (1.f / sum));
       } else {
         P.part[(at + h) * 128 + r] = o[h];
         if (r == 0) {
-          P.stat[(at + h) * 2] = m[h];
+          P.stat[(at + h) * 2] = top;
           P.stat[(at + h) * 2 + 1] = sum;
         }
       }

@@ -1193,7 +1193,7 @@ def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Op
     """Attention of one new token per sequence over a paged cache: ``q`` [B,H,D], row i for slot
     ``rows[i]`` (int32; default slot i), whose last token it is (written before this call).  It sees
     the slot's tokens within ``window`` (None: all) and the first ``sinks``; tokens on released pages
-    are not seen.  A slot of length 0 gives zeros.  ``max_len``, if known, is the longest slot's
+    are not seen.  A slot of length 0 gives zeros, scores of NaN or +inf, or only -inf, give NaN.  ``max_len``, if known, is the longest slot's
     length; it only sizes the split over the cache's length.  Returns [B,H,D]."""
     s, index = _cache_struct(cache)
     _on_device(index, q)

@@ -506,8 +506,8 @@ GDNX_API gdnx_status gdnx_cache_compact(const gdnx_cache* cache, void* workspace
 /* Attention of one new token per query row over a cache: row i of q reads slot rows[i],
  * whose last token it is (the token's own key and value are written before the call).
  * It sees token j < length where length - 1 - j < window or j < sinks; tokens on released
- * pages are not seen.  A row that sees nothing (length 0, a slot out of range), or scores of
- * -inf only, gives 0; one that sees a score of NaN or +inf is NaN.
+ * pages are not seen.  A row that sees nothing (length 0, a slot out of range) gives 0;
+ * one that sees a score of NaN or +inf, or only -inf, is NaN.
  * The visible tokens are split over CTAs, and the parts joined in a fixed order. */
 typedef struct {
   gdnx_cache cache;

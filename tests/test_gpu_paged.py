@@ -402,3 +402,34 @@ def test_a_write_names_no_more_rows_than_there_are_slots():
     k = torch.zeros(3, 1, 2, 64, dtype=torch.bfloat16, device=DEV)
     with pytest.raises(ValueError):
         ops.cache_write(c, k, k, i32(0, 1, 0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", ["nan", "inf", "-inf"])
+def test_decode_of_scores_that_are_not_finite(what, dtype):
+    """A token that sees a score of NaN or +inf, or only -inf, is NaN, in units of few tiles and in cut ones; other
+    sequences, -inf among finite scores and slots that see nothing are not."""
+    bad = float(what)
+    for lengths, at, heads in (([300, 0, 90], 77, 4), ([5000, 3, 4000], 4097, 2), ([5000, 0, 3], 130, 6)):
+        c = cache(lengths, Hk=2, page=16, D=64, width=400, dtype=dtype, seed=at)
+        q = torch.randn(3, heads, 64, generator=torch.Generator().manual_seed(1)).to(TYPES[dtype]).to(DEV)
+        q[..., 0] = 1.0
+        page = c.table[0, at // 16]
+        c.kv[1, 0, page, :, at % 16] = 0
+        c.kv[1, 0, page, :, at % 16, 0] = bad
+        y = ops.paged_decode(q, c, layer=1)
+        yo = mirror(c).decode(q, 1)
+        assert torch.equal(y.isnan().cpu(), yo.isnan()) and bool(y[0].isnan().all()) == (what != "-inf")
+        assert rel(y.nan_to_num(0), yo.nan_to_num(0)) < TOL[dtype]
+        last = c.table[2, (lengths[2] - 1) // 16]  # a window of one token, whose score is bad
+        c.kv[1, 0, last, :, (lengths[2] - 1) % 16] = 0
+        c.kv[1, 0, last, :, (lengths[2] - 1) % 16, 0] = bad
+        y = ops.paged_decode(q, c, layer=1, window=1)
+        assert y[2].isnan().all() and y[:2].isfinite().all()
+        k = c.kv[1, 0].clone()
+        c.kv[1, 0] = 0  # every score
+        c.kv[1, 0, ..., 0] = bad
+        y = ops.paged_decode(q, c, layer=1)
+        assert torch.equal(y.isnan().flatten(1).all(1).cpu(), torch.tensor(lengths) > 0)
+        assert torch.equal(y.isnan().flatten(1).any(1).cpu(), torch.tensor(lengths) > 0)
+        assert not ops.paged_decode(q[:1], c, rows=i32(-1)).any()
