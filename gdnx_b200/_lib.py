@@ -23,6 +23,8 @@ EXPORTED = ("gdnx_scan_fwd", "gdnx_scan_fwd_noalloc", "gdnx_scan_noalloc_status"
             "gdnx_epilogue_scatter", "gdnx_device_alloc", "gdnx_device_free", "gdnx_ipc_handle", "gdnx_ipc_open",
             "gdnx_ipc_close", "gdnx_error_word", "gdnx_error_status", "gdnx_attn_fwd", "gdnx_attn_bwd", "gdnx_attn_bwd_workspace_bytes", "gdnx_cache_fork",
             "gdnx_cache_extend", "gdnx_cache_write", "gdnx_cache_truncate", "gdnx_cache_trim", "gdnx_cache_compact",
+            "gdnx_cache_compact_bounds", "gdnx_cache_step", "gdnx_cache_append", "gdnx_cache_bounds",
+            "gdnx_paged_select", "gdnx_paged_select_workspace_bytes",
             "gdnx_cache_workspace_bytes", "gdnx_paged_decode", "gdnx_paged_decode_workspace_bytes")
 
 
@@ -143,6 +145,19 @@ class PagedDecodeArgs(C.Structure):
                 ("window", C.c_int64), ("sinks", C.c_int64), ("max_len", C.c_int64), ("scale", C.c_float),
                 ("q", View), ("rows", C.c_void_p), ("y", C.c_void_p), ("y_dtype", C.c_int32),
                 ("y_sb", C.c_int64), ("y_sh", C.c_int64), ("error", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("positions", C.c_void_p), ("pages", C.c_void_p), ("listed", C.c_int64)]
+
+
+class Step(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("starts", C.c_void_p), ("first", C.c_void_p), ("token_rows", C.c_void_p),
+                ("positions", C.c_void_p), ("places", C.c_void_p)]
+
+
+class PagedSelectArgs(C.Structure):
+    _fields_ = [("cache", Cache), ("bounds", C.c_void_p), ("B", C.c_int64), ("H", C.c_int64), ("layer", C.c_int64),
+                ("k", C.c_int64), ("window", C.c_int64), ("sinks", C.c_int64), ("max_len", C.c_int64), ("q", View),
+                ("rows", C.c_void_p), ("positions", C.c_void_p), ("selected", C.c_void_p),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
@@ -210,13 +225,20 @@ def load(path: Path = LIB_PATH):
     for name, types in (("fork", [cache, i64, ptr, ptr, ptr]), ("extend", [cache, i64, ptr, ptr, ptr, size, ptr]),
                         ("write", [cache, i64, i64, i64, C.POINTER(View), C.POINTER(View), ptr, ptr, ptr]),
                         ("truncate", [cache, i64, ptr, ptr, ptr]), ("trim", [cache, i64, ptr, i64, i64, ptr]),
-                        ("compact", [cache, ptr, size, ptr])):
+                        ("compact", [cache, ptr, size, ptr]), ("compact_bounds", [cache, ptr, ptr, size, ptr]),
+                        ("step", [cache, i64, ptr, ptr, C.POINTER(Step), ptr, size, ptr]),
+                        ("append", [cache, i64, i64, C.POINTER(View), C.POINTER(View), ptr, ptr]),
+                        ("bounds", [cache, i64, i64, ptr, ptr, ptr, ptr])):
         fn = getattr(lib, "gdnx_cache_" + name)
         fn.argtypes, fn.restype = types, C.c_int
     lib.gdnx_paged_decode_workspace_bytes.argtypes = [C.POINTER(PagedDecodeArgs)]
     lib.gdnx_paged_decode_workspace_bytes.restype = size
     lib.gdnx_paged_decode.argtypes = [C.POINTER(PagedDecodeArgs), C.c_void_p]
     lib.gdnx_paged_decode.restype = C.c_int
+    lib.gdnx_paged_select_workspace_bytes.argtypes = [C.POINTER(PagedSelectArgs)]
+    lib.gdnx_paged_select_workspace_bytes.restype = size
+    lib.gdnx_paged_select.argtypes = [C.POINTER(PagedSelectArgs), C.c_void_p]
+    lib.gdnx_paged_select.restype = C.c_int
     lib.gdnx_status_string.argtypes = [C.c_int]
     lib.gdnx_status_string.restype = C.c_char_p
     lib.gdnx_version.argtypes = []

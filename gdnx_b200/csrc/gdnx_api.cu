@@ -84,6 +84,7 @@ __device__ int g_error_word;
 // ---- windowed attention and the paged cache ----
 
 constexpr int64_t kMaxTokens = (int64_t)1 << 30;  // positions and their distances stay in int32
+constexpr int64_t kMaxPacked = (int64_t)1 << 20;  // rows of a packed batch: a thousand of them add up in int32
 
 // A device pointer on a multiple of `align` bytes.
 bool device_ptr(const void* p, size_t align) {
@@ -271,7 +272,82 @@ gdnx_status gdnx_cache_compact(const gdnx_cache* c, void* workspace, size_t work
   const gdnx_status s = check_cache(c);
   if (s != GDNX_OK || c->pages == 0) return s;
   if (workspace_bytes < gdnx_cache_workspace_bytes(c, 0) || !device_ptr(workspace, sizeof(int32_t))) return GDNX_EWORKSPACE;
-  return gdnx::launch_cache_compact(*c, workspace, (cudaStream_t)stream);
+  return gdnx::launch_cache_compact(*c, nullptr, workspace, (cudaStream_t)stream);
+}
+
+gdnx_status gdnx_cache_compact_bounds(const gdnx_cache* c, void* bounds, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
+  const gdnx_status s = check_cache(c);
+  if (s != GDNX_OK || c->pages == 0) return s;
+  if (!device_ptr(bounds, 16)) return GDNX_EINVAL;
+  if (workspace_bytes < gdnx_cache_workspace_bytes(c, 0) || !device_ptr(workspace, sizeof(int32_t))) return GDNX_EWORKSPACE;
+  return gdnx::launch_cache_compact(*c, bounds, workspace, (cudaStream_t)stream);
+}
+
+gdnx_status gdnx_cache_step(const gdnx_cache* c, int64_t n, const int32_t* rows, const int32_t* counts,
+                            const gdnx_step* step, void* workspace, size_t workspace_bytes, void* stream) {
+  const gdnx_status s = check_rows(c, n, rows, counts);
+  if (s != GDNX_OK) return s;
+  if (!step || step->tokens < 0 || !words(step->starts) || (n && !words(step->first))) return GDNX_EINVAL;
+  if (step->tokens > kMaxPacked) return GDNX_EUNSUPPORTED;
+  if (step->tokens && (!words(step->token_rows) || !words(step->positions) || !device_ptr(step->places, 8))) return GDNX_EINVAL;
+  if (workspace_bytes < gdnx_cache_workspace_bytes(c, n) || !device_ptr(workspace, sizeof(int32_t))) return GDNX_EWORKSPACE;
+  return gdnx::launch_cache_step(*c, n, rows, counts, *step, workspace, (cudaStream_t)stream);
+}
+
+gdnx_status gdnx_cache_append(const gdnx_cache* c, int64_t layer, int64_t tokens, const gdnx_view* k,
+                              const gdnx_view* v, const int64_t* places, void* stream) {
+  const gdnx_status s = check_cache(c);
+  if (s != GDNX_OK) return s;
+  if (layer < 0 || layer >= c->L || tokens < 0 || !k || !v) return GDNX_EINVAL;
+  if (tokens > kMaxPacked || c->Hk > 65535) return GDNX_EUNSUPPORTED;
+  if (tokens == 0 || c->pages == 0) return GDNX_OK;
+  if (!heads_ok(*k, c->dtype, c->D) || !heads_ok(*v, c->dtype, c->D) || !device_ptr(places, 8)) return GDNX_EINVAL;
+  return gdnx::launch_cache_append(*c, layer, tokens, *k, *v, places, (cudaStream_t)stream);
+}
+
+gdnx_status gdnx_cache_bounds(const gdnx_cache* c, int64_t layer, int64_t n, const int32_t* rows, const int32_t* counts,
+                              void* bounds, void* stream) {
+  const gdnx_status s = check_rows(c, n, rows, counts);
+  if (s != GDNX_OK) return s;
+  if (layer < 0 || layer >= c->L) return GDNX_EINVAL;
+  if (n == 0 || c->pages == 0) return GDNX_OK;
+  if (!device_ptr(bounds, 16)) return GDNX_EINVAL;
+  return gdnx::launch_cache_bounds(*c, layer, n, rows, counts, bounds, (cudaStream_t)stream);
+}
+
+// Pages that hold one of the first `sinks` or the last `window` tokens, at most.
+static int64_t always_taken(const gdnx_paged_select_args& a) {
+  const int64_t page = a.cache.page;
+  return (a.sinks + page - 1) / page + (a.window + page - 2) / page + 1;
+}
+
+static gdnx_status check_select(const gdnx_paged_select_args& a) {
+  const gdnx_status s = check_cache(&a.cache);
+  if (s != GDNX_OK) return s;
+  if (a.cache.pages < 1 || a.B < 0 || a.H <= 0 || a.H % a.cache.Hk || a.layer < 0 || a.layer >= a.cache.L ||
+      a.k < 1 || a.window < 1 || a.sinks < 0 || a.max_len < 0)
+    return GDNX_EINVAL;
+  if (a.window > kMaxTokens || a.sinks > kMaxTokens || always_taken(a) > a.k) return GDNX_EINVAL;
+  if (a.B > kMaxPacked || a.H > 65535 || a.k > kMaxPacked || a.B * a.cache.Hk >= ((int64_t)1 << 31))
+    return GDNX_EUNSUPPORTED;
+  return !a.rows && a.B > a.cache.slots ? GDNX_EINVAL : GDNX_OK;
+}
+
+size_t gdnx_paged_select_workspace_bytes(const gdnx_paged_select_args* a) {
+  return !a || check_select(*a) != GDNX_OK || a->B == 0 ? 0 : gdnx::paged_select_workspace_bytes(*a);
+}
+
+gdnx_status gdnx_paged_select(const gdnx_paged_select_args* a, void* stream) {
+  if (!a) return GDNX_EINVAL;
+  const gdnx_status s = check_select(*a);
+  if (s != GDNX_OK || a->B == 0) return s;
+  if (!heads_ok(a->q, a->cache.dtype, a->cache.D) || !device_ptr(a->bounds, 16) || !words(a->selected) ||
+      (a->rows && !words(a->rows)) || (a->positions && !words(a->positions)))
+    return GDNX_EINVAL;
+  const size_t need = gdnx_paged_select_workspace_bytes(a);
+  if (need && (a->workspace_bytes < need || !device_ptr(a->workspace, 16))) return GDNX_EWORKSPACE;
+  return gdnx::launch_paged_select(*a, (cudaStream_t)stream);
 }
 
 // The decode's arguments with window and sinks kept within the longest sequence.
@@ -294,6 +370,8 @@ static gdnx_status check_decode(const gdnx_paged_decode_args& a) {
   if (a.B == 0) return GDNX_OK;
   if (!heads_ok(a.q, a.cache.dtype, a.cache.D) || !device_ptr(a.y, bytes_of(a.y_dtype)) || a.y_sb < 0 || a.y_sh < 0) return GDNX_EINVAL;
   if (a.rows && !words(a.rows)) return GDNX_EINVAL;
+  if (a.positions && !words(a.positions)) return GDNX_EINVAL;
+  if (a.pages && (!words(a.pages) || a.listed < 1)) return GDNX_EINVAL;
   if (a.error && !words(a.error)) return GDNX_EINVAL;
   return GDNX_OK;
 }

@@ -34,7 +34,16 @@ gdnx_status launch_cache_truncate(const gdnx_cache& c, int64_t n, const int32_t*
                                   cudaStream_t st);
 gdnx_status launch_cache_trim(const gdnx_cache& c, int64_t n, const int32_t* rows, int64_t window, int64_t sinks,
                               cudaStream_t st);
-gdnx_status launch_cache_compact(const gdnx_cache& c, void* ws, cudaStream_t st);
+// `bounds`: moved along where given.
+gdnx_status launch_cache_compact(const gdnx_cache& c, void* bounds, void* ws, cudaStream_t st);
+gdnx_status launch_cache_step(const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* counts,
+                              const gdnx_step& step, void* ws, cudaStream_t st);
+gdnx_status launch_cache_append(const gdnx_cache& c, int64_t layer, int64_t tokens, const gdnx_view& k,
+                                const gdnx_view& v, const int64_t* places, cudaStream_t st);
+gdnx_status launch_cache_bounds(const gdnx_cache& c, int64_t layer, int64_t n, const int32_t* rows,
+                                const int32_t* counts, void* bounds, cudaStream_t st);
+size_t paged_select_workspace_bytes(const gdnx_paged_select_args& a);
+gdnx_status launch_paged_select(const gdnx_paged_select_args& a, cudaStream_t st);
 size_t paged_decode_workspace_bytes(const gdnx_paged_decode_args& a);
 gdnx_status launch_paged_decode(const gdnx_paged_decode_args& a, cudaStream_t st);
 // 16-bit caches, on the tensor cores (paged_decode_tc.cu).

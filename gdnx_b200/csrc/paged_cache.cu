@@ -18,9 +18,7 @@
 // layers), written in one layer and trimmed: 57 us (198 MB); compaction after waves of requests moves
 // pages at 85 % of a copy's rate; write of 64 x 1 tokens 4.2 us (its checks: 1.1), of 8 x 4096 tokens of 4 heads of
 // 128 in bf16 56 us.
-#include "common.cuh"
-#include "kernels.h"
-#include "launch.cuh"
+#include "paged_cache.cuh"
 
 namespace gdnx {
 namespace {
@@ -50,39 +48,6 @@ struct Plan {
     return (size_t)(HEAD + 2 * m + pages + n) * sizeof(int32_t);
   }
 };
-
-// True in every thread when all rows are slots and none is named twice (and, where
-// `other` is given, its rows are slots not among `rows`).  `seen` has slots bits.
-GDNX_DEV bool rows_ok(uint32_t* seen, const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* other,
-                      const int32_t* counts) {
-  for (int64_t i = threadIdx.x; i < (c.slots + 31) / 32; i += blockDim.x) seen[i] = 0;
-  __syncthreads();
-  bool bad = false;
-  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-    const int r = rows[i];
-    if (r < 0 || r >= c.slots) bad = true;
-    else bad |= (atomicOr(&seen[r / 32], 1u << (r % 32)) >> (r % 32)) & 1u;
-    if (counts) bad |= counts[i] < 0;
-  }
-  __syncthreads();
-  if (other)
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-      const int r = other[i];
-      if (r < 0 || r >= c.slots) bad = true;
-      else bad |= (seen[r / 32] >> (r % 32)) & 1u;
-    }
-  return !__syncthreads_or(bad);
-}
-
-GDNX_DEV bool page_ok(const gdnx_cache& c, int p) { return p >= 0 && p < c.pages; }
-
-GDNX_DEV int64_t pages_of(const gdnx_cache& c, int64_t tokens) { return (tokens + c.page - 1) / c.page; }
-
-// A slot's length, kept within what its row can hold.
-GDNX_DEV int64_t length_of(const gdnx_cache& c, int row) {
-  const int64_t n = c.lengths[row], most = c.width * c.page;
-  return n < 0 ? 0 : (n > most ? most : n);
-}
 
 enum RowOp { kFork, kTruncate, kTrim };
 
@@ -159,8 +124,10 @@ GDNX_DEV void load4(int (&r)[4], const gdnx_cache& c, int64_t p, int fill) {
   for (int e = 0; e < 4; ++e) r[e] = p + e < c.pages ? c.refs[p + e] : fill;
 }
 
+// STEP: also where the new tokens stand in a packed batch (`out.starts`, `out.first`; zeros where refused).
+template <bool STEP>
 __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, int64_t n, const int32_t* rows,
-                                                          const int32_t* counts, void* ws) {
+                                                          const int32_t* counts, void* ws, const gdnx_step out) {
   extern __shared__ uint32_t seen[];
   __shared__ int sums[32];
   __shared__ int ncopy;
@@ -171,11 +138,17 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
     w.head[0] = 0;
     ncopy = 0;
   }
-  if (*c.status != 0) return;
-  if (!rows_ok(seen, c, n, rows, nullptr, counts)) {
-    if (threadIdx.x == 0) *c.status = GDNX_EINVAL;
-    return;
-  }
+  // each entry of starts and first is written by one thread only, so that the last value written stays
+  const auto refuse = [&](int status) {
+    if (STEP)
+      for (int64_t i = threadIdx.x; i <= n; i += NT) {
+        out.starts[i] = 0;
+        if (i < n) out.first[i] = 0;
+      }
+    if (threadIdx.x == 0 && status) *c.status = status;
+  };
+  if (*c.status != 0) return refuse(0);
+  if (!rows_ok(seen, c, n, rows, nullptr, counts)) return refuse(GDNX_EINVAL);
   // what each row needs: its new pages, and one more where a shared last page is copied; `lost`: the new
   // tokens would begin on a page that was released (trimmed, and the slot cut back into it since)
   const auto ask = [&](int64_t i, int64_t& first, int64_t& need, int& shared, bool& lost) {
@@ -192,7 +165,7 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
     return want <= c.width;
   };
   bool full = false, lost = false;
-  int64_t total = 0;
+  int64_t total = 0, packed = 0;
   for (int64_t base = 0; base < n; base += NT) {
     const int64_t i = base + threadIdx.x;
     int64_t first = 0, need = 0;
@@ -202,15 +175,18 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
     const int at = block_scan((int)need, sums, &sum);
     if (i < n) w.off[i] = (int)(total + at);
     total += sum;
+    if (STEP) {  // counts beyond the batch are refused below; cut, their sums stay small
+      const int start = block_scan(i < n ? (int)min((int64_t)counts[i], out.tokens + 1) : 0, sums, &sum);
+      if (i < n) {
+        out.starts[i] = (int)(packed + start);
+        out.first[i] = (int)length_of(c, rows[i]);
+      }
+      packed += sum;
+    }
   }
-  if (__syncthreads_or(lost)) {
-    if (threadIdx.x == 0) *c.status = GDNX_EINVAL;
-    return;
-  }
-  if (__syncthreads_or(full || total > c.pages)) {
-    if (threadIdx.x == 0) *c.status = GDNX_ENOPAGES;
-    return;
-  }
+  if (STEP && threadIdx.x == n % NT) out.starts[n] = (int)packed;
+  if (__syncthreads_or(lost || (STEP && packed > out.tokens))) return refuse(GDNX_EINVAL);
+  if (__syncthreads_or(full || total > c.pages)) return refuse(GDNX_ENOPAGES);
   int64_t found = 0;
   for (int64_t base = 0; base < c.pages && found < total; base += 4 * NT) {
     int r[4], sum;
@@ -224,10 +200,7 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
       }
     found += sum;
   }
-  if (found < total) {
-    if (threadIdx.x == 0) *c.status = GDNX_ENOPAGES;
-    return;
-  }
+  if (found < total) return refuse(GDNX_ENOPAGES);
   __syncthreads();  // the list is whole
   // refs of shared pages are read above and below by every row before any is changed
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -311,17 +284,45 @@ __global__ void __launch_bounds__(NT) cache_compact_kernel(const gdnx_cache c, v
   }
 }
 
-// Moves the planned pages in every layer; for compact also renames them in the table.
-// A page of one layer's keys or values is one contiguous run.  Sources and destinations
-// are different pages, so the moves are independent.
+// Where each packed token stands: its sequence by bisection of the starts, and its page's place there.
+GDNX_DEV void place_tokens(const gdnx_cache& c, int64_t n, const int32_t* rows, const gdnx_step& s) {
+  const int packed = s.starts[n];
+  for (int64_t t = (int64_t)blockIdx.x * COPY_NT + threadIdx.x; t < s.tokens; t += (int64_t)gridDim.x * COPY_NT) {
+    int row = -1, pos = -1;
+    int64_t place = -1;
+    if (t < packed) {
+      int64_t lo = 0, hi = n;  // starts[lo] <= t < starts[hi]
+      while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) / 2;
+        if (s.starts[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      row = rows[lo];
+      pos = s.first[lo] + (int)(t - s.starts[lo]);
+      place = (int64_t)c.table[row * c.width + pos / c.page] * c.page + pos % c.page;
+    }
+    s.token_rows[t] = row;
+    s.positions[t] = pos;
+    s.places[t] = place;
+  }
+}
+
+// Moves the planned pages in every layer; for compact (RENAME) also renames them in the table, for a step (PLACE)
+// finds the new tokens' places.  A page of one layer's keys or values is one contiguous run of `run` bytes (a page
+// of bounds another, shorter one: kv is then their tensor).  Sources and destinations are different pages, so the
+// moves are independent.
+enum CopyKind { kMove, kRename, kPlace };
+
+template <int KIND>
 __global__ void __launch_bounds__(COPY_NT) cache_copy_kernel(const gdnx_cache c, void* ws, int64_t n, int64_t run,
-                                                             int rename) {
+                                                             void* pages, const int32_t* rows, const gdnx_step step) {
   const Plan w(ws, c.pages, n);
   dependents_may_start();
   wait_for_earlier();
+  if (KIND == kPlace) place_tokens(c, n, rows, step);
   const int m = w.head[0];
   if (m == 0) return;
-  if (rename) {
+  if (KIND == kRename) {
     const int live = w.head[1];
     for (int64_t i = (int64_t)blockIdx.x * COPY_NT + threadIdx.x; i < c.slots * c.width;
          i += (int64_t)gridDim.x * COPY_NT) {
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(COPY_NT) cache_copy_kernel(const gdnx_cache c,
   }
   constexpr int UNIT = COPY_NT * COPY_VEC;  // 16-byte words
   const int64_t words = run / 16, per = (words + UNIT - 1) / UNIT, sides = c.L * 2;
-  uint4* kv = static_cast<uint4*>(c.kv);
+  uint4* kv = static_cast<uint4*>(pages);
   for (int64_t u = blockIdx.x; u < per * sides * m; u += gridDim.x) {
     const int64_t part = u % per, side = u / per % sides, k = u / (per * sides);
     const uint4* src = kv + (side * c.pages + w.src[k]) * words;
@@ -422,15 +423,12 @@ __global__ void __launch_bounds__(WRITE_NT) cache_write_kernel(const gdnx_cache 
   }
 }
 
-size_t seen_bytes(const gdnx_cache& c) { return (size_t)((c.slots + 31) / 32) * 4; }
-
-gdnx_status launched(cudaError_t e) { return e == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH; }
-
-int elem(int dtype) { return dtype == GDNX_F32 ? 4 : 2; }
-
-gdnx_status copy_pages(const gdnx_cache& c, void* ws, int64_t n, int rename, cudaStream_t st) {
+template <int KIND>
+gdnx_status copy_pages(const gdnx_cache& c, void* ws, int64_t n, cudaStream_t st, const int32_t* rows = nullptr,
+                       const gdnx_step& step = {}) {
   const int64_t run = c.Hk * c.page * c.D * elem(c.dtype);
-  return launched(launch_early(cache_copy_kernel, dim3(sm_count() * 8), dim3(COPY_NT), 0, st, c, ws, n, run, rename));
+  return launched(launch_early(cache_copy_kernel<KIND>, dim3(sm_count() * 8), dim3(COPY_NT), 0, st, c, ws, n, run, c.kv,
+                               rows, step));
 }
 
 }  // namespace
@@ -456,14 +454,26 @@ gdnx_status launch_cache_trim(const gdnx_cache& c, int64_t n, const int32_t* row
 
 gdnx_status launch_cache_extend(const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* counts, void* ws,
                                 cudaStream_t st) {
-  if (launch_early(cache_extend_kernel, dim3(1), dim3(NT), seen_bytes(c), st, c, n, rows, counts, ws) != cudaSuccess)
+  if (launch_early(cache_extend_kernel<false>, dim3(1), dim3(NT), seen_bytes(c), st, c, n, rows, counts, ws,
+                   gdnx_step{}) != cudaSuccess)
     return GDNX_ELAUNCH;
-  return copy_pages(c, ws, n, 0, st);
+  return copy_pages<kMove>(c, ws, n, st);
 }
 
-gdnx_status launch_cache_compact(const gdnx_cache& c, void* ws, cudaStream_t st) {
+gdnx_status launch_cache_step(const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* counts,
+                              const gdnx_step& step, void* ws, cudaStream_t st) {
+  if (launch_early(cache_extend_kernel<true>, dim3(1), dim3(NT), seen_bytes(c), st, c, n, rows, counts, ws, step) !=
+      cudaSuccess)
+    return GDNX_ELAUNCH;
+  return copy_pages<kPlace>(c, ws, n, st, rows, step);
+}
+
+gdnx_status launch_cache_compact(const gdnx_cache& c, void* bounds, void* ws, cudaStream_t st) {
   if (launch_early(cache_compact_kernel, dim3(1), dim3(NT), 0, st, c, ws) != cudaSuccess) return GDNX_ELAUNCH;
-  return copy_pages(c, ws, 0, 1, st);
+  const gdnx_status s = copy_pages<kRename>(c, ws, 0, st);
+  if (s != GDNX_OK || !bounds) return s;
+  return launched(launch_early(cache_copy_kernel<kMove>, dim3(sm_count() * 8), dim3(COPY_NT), 0, st, c, ws, 0,
+                               c.Hk * c.D * elem(c.dtype), bounds, nullptr, gdnx_step{}));
 }
 
 namespace {

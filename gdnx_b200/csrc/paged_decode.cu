@@ -31,13 +31,16 @@ struct Small {
   uint64_t full[STAGES], empty[STAGES];
   Range range;
   long long sums[NTHREADS / 32];
+  int at[STAGES][2];  // places of a stage's two halves
   int ok[STAGES];  // which halves of a stage's tokens lie on pages
   int abort_flag;
 };
 
-// Does the sequence's newest token see any of tokens j..j+31?
-GDNX_DEV bool sub_seen(int j, int len, int64_t window, int64_t sinks) {
-  return j < len && (j + SUB > (int64_t)len - window || j < sinks);
+// Does the sequence's newest token see any of a tile's tokens 32 s .. 32 s + 31?  (Of listed pages: is one there?)
+GDNX_DEV bool sub_seen(const DecParams& P, const Seq& q, int tile, int s) {
+  const int j = tile * TM + s * SUB;
+  if (P.a.pages) return j < q.listed * P.a.cache.page;
+  return j < q.len && (j + SUB > (int64_t)q.len - P.a.window || j < P.a.sinks);
 }
 
 template <int NH>
@@ -54,11 +57,11 @@ GDNX_DEV void load_stages(const DecParams& P, Walk w, uint8_t* ring, Small<NH>& 
       const int k = (t - w.ta) % ahead;
       if (k == 0) {
         const int mine = t + lane / npp;
-        ids = mine < w.tb ? page_id(P, w.seq, w.seq.kt.tile(mine), lane % npp) : -1;
+        ids = mine < w.tb ? page_id(P, w.seq, w.b, w.unit, w.seq.kt.tile(mine), lane % npp) : -1;
       }
       for (int s = 0; s < TM / SUB; ++s) {
-        const int j = w.seq.kt.tile(t) * TM + s * SUB;
-        if (!sub_seen(j, w.seq.len, P.a.window, P.a.sinks)) continue;
+        const int tile = w.seq.kt.tile(t);
+        if (!sub_seen(P, w.seq, tile, s)) continue;
         const uint32_t st = n % STAGES;
         if (!warp_wait(&sm.empty[st], (n / STAGES & 1) ^ 1, &sm.abort_flag)) return;
         ++n;
@@ -69,12 +72,17 @@ GDNX_DEV void load_stages(const DecParams& P, Walk w, uint8_t* ring, Small<NH>& 
         const uint32_t got = __ballot_sync(0xffffffffu, go);
         const uint32_t bar = tc::smem_u32(&sm.full[st]), bytes = (uint32_t)(tokens * D * 4);
         if (lane == 0) {
+          // places of a stage's two halves in the sequence
+          const int64_t a = page_first(P, w.seq, w.b, w.unit, tile, s * SUB / page);
+          const int64_t b = runs == 1 ? a + 16 : page_first(P, w.seq, w.b, w.unit, tile, s * SUB / page + 1);
+          sm.at[st][0] = (int)(a + (runs == 1 ? s * SUB % page : 0));
+          sm.at[st][1] = (int)(b + (runs == 1 ? s * SUB % page : 0));
           sm.ok[st] = runs == 1 ? (got & 1 ? 3 : 0) : (int)((got & 1) | (got >> 1 & 2));
           pipe::expect_tx(bar, __popc(got) * bytes);
         }
         __syncwarp();
         if (go) {
-          const int64_t row = ((((P.a.layer * 2 + side) * c.pages + id) * c.Hk + hk) * page + (j + run * tokens) % page);
+          const int64_t row = ((((P.a.layer * 2 + side) * c.pages + id) * c.Hk + hk) * page + (s * SUB + run * tokens) % page);
           pipe::bulk_load(tc::smem_u32(ring) + st * 2 * SIDE + side * SIDE + run * tokens * D * 4, kv + row * D, bytes, bar);
         }
       }
@@ -111,20 +119,20 @@ GDNX_DEV void use_stages(const DecParams& P, Walk w, int64_t per, const uint8_t*
     }
     for (int t = w.ta; t < w.tb; ++t) {
       for (int s = 0; s < TM / SUB; ++s) {
-        const int j0 = w.seq.kt.tile(t) * TM + s * SUB;
-        if (!sub_seen(j0, w.seq.len, a.window, a.sinks)) continue;
+        if (!sub_seen(P, w.seq, w.seq.kt.tile(t), s)) continue;
         const uint32_t st = n % STAGES;
         ok = ok && warp_wait(&sm.full[st], n / STAGES & 1, &sm.abort_flag);
         ++n;
         if (!ok) continue;
         const int on_page = *const_cast<volatile int*>(&sm.ok[st]);
+        const int at[2] = {*const_cast<volatile int*>(&sm.at[st][0]), *const_cast<volatile int*>(&sm.at[st][1])};
         const float* kt = reinterpret_cast<const float*>(ring + st * 2 * SIDE);
         const float* vt = reinterpret_cast<const float*>(ring + st * 2 * SIDE + SIDE);
         float x[PASSES][NH];
         bool seen[PASSES], over = false;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-          const int r = warp * (SUB / WARPS) + i * KPW + sub, j = j0 + r;
+          const int r = warp * (SUB / WARPS) + i * KPW + sub, j = (r < 16 ? at[0] : at[1]) + r % 16;
           seen[i] = key_seen(j, w.seq.len, window, sinks) && (on_page >> (r / 16) & 1);
           any |= seen[i];
           float4 k0 = make_float4(0.f, 0.f, 0.f, 0.f), k1 = k0;

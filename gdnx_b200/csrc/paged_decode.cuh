@@ -42,24 +42,33 @@ struct Range {
   int64_t t0, t1, before, b, per;
 };
 
-// Visible tokens of one sequence.
+// Visible tokens of one sequence.  Where the call names pages, its tiles hold the first `listed` pages of each
+// key head's list in their order, not the tokens in theirs.
 struct Seq {
   int row, len;
   KeyTiles kt;
+  int listed;
 };
 
 GDNX_DEV int slot_length(const gdnx_paged_decode_args& a, int64_t b, int& row) {
   const gdnx_cache& c = a.cache;
   row = a.rows ? a.rows[b] : (int)b;
   if (row < 0 || row >= c.slots) return 0;
-  const int64_t n = c.lengths[row], most = c.width * c.page;
+  int64_t n = c.lengths[row];
+  const int64_t most = c.width * c.page;
+  if (a.positions) n = min(n, (int64_t)a.positions[b] + 1);
   return (int)(n < 0 ? 0 : (n > most ? most : n));
 }
 
 GDNX_DEV Seq make_seq(const gdnx_paged_decode_args& a, int64_t b) {
   int row;
   const int len = slot_length(a, b, row);
-  return {row, len, KeyTiles(len - 1, len - 1, len, (int)a.window, (int)a.sinks, TM)};
+  if (a.pages) {
+    Seq s = {row, len, KeyTiles(), (int)min(a.listed, (int64_t)(len + a.cache.page - 1) / a.cache.page)};
+    s.kt.count = (s.listed * a.cache.page + TM - 1) / TM;
+    return s;
+  }
+  return {row, len, KeyTiles(len - 1, len - 1, len, (int)a.window, (int)a.sinks, TM), 0};
 }
 
 GDNX_DEV int tiles_of(const gdnx_paged_decode_args& a, int64_t b) { return make_seq(a, b).kt.count; }
@@ -153,11 +162,20 @@ GDNX_DEV bool key_seen(int j, int len, int window, int sinks) {
   return j < len && (len - 1 - j < window || j < sinks);
 }
 
-// Page ids of a tile's pages, or -1 where nothing visible is there (lane < npp).
-GDNX_DEV int page_id(const DecParams& P, const Seq& s, int kt, int i) {
+// First token of the i-th page of a unit's tile kt (-1: the list has none there).
+GDNX_DEV int64_t page_first(const DecParams& P, const Seq& s, int64_t b, int unit, int kt, int i) {
   const gdnx_cache& c = P.a.cache;
-  const int64_t first = (int64_t)kt * TM + i * c.page;
-  if (first >= s.len || !(first + c.page > (int64_t)s.len - P.a.window || first < P.a.sinks)) return -1;
+  if (!P.a.pages) return (int64_t)kt * TM + i * c.page;
+  const int e = kt * (TM / c.page) + i;
+  const int x = e < s.listed ? P.a.pages[(b * c.Hk + unit / P.groups) * P.a.listed + e] : -1;
+  return x < 0 || x >= c.width ? -1 : (int64_t)x * c.page;
+}
+
+// Page ids of a tile's pages, or -1 where nothing visible is there (lane < npp).
+GDNX_DEV int page_id(const DecParams& P, const Seq& s, int64_t b, int unit, int kt, int i) {
+  const gdnx_cache& c = P.a.cache;
+  const int64_t first = page_first(P, s, b, unit, kt, i);
+  if (first < 0 || first >= s.len || !(first + c.page > (int64_t)s.len - P.a.window || first < P.a.sinks)) return -1;
   const int p = c.table[(int64_t)s.row * c.width + first / c.page];
   return p >= 0 && p < c.pages ? p : -1;
 }
@@ -258,9 +276,10 @@ inline Plan make_plan(const gdnx_paged_decode_args& a, int nh) {
   p.groups = (int)((G + nh - 1) / nh);
   int64_t most = a.cache.width * a.cache.page;
   if (a.max_len > 0 && a.max_len < most) most = a.max_len;
+  if (a.pages && a.listed * a.cache.page < most) most = a.listed * a.cache.page;
   int64_t n = (most + TM - 1) / TM;  // tiles of a unit, at most
   const int64_t seen = (a.window + TM - 1) / TM + 1 + (a.sinks + TM - 1) / TM;
-  if (seen < n) n = seen;
+  if (!a.pages && seen < n) n = seen;
   const int64_t units = a.B * a.cache.Hk * p.groups;
   // Short units are not cut: a few more tiles in a row take less time than a join.
   p.whole = n <= WHOLE_TILES;

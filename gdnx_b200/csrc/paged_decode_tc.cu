@@ -75,7 +75,7 @@ GDNX_DEV void run_loads(const TcParams& P, Walk w, uint32_t smem, Bars& bar, vol
       const int k = (t - w.ta) % ahead;
       if (k == 0) {
         const int mine = t + lane / npp;
-        ids = mine < w.tb ? page_id(P, w.seq, w.seq.kt.tile(mine), lane % npp) : -1;
+        ids = mine < w.tb ? page_id(P, w.seq, w.b, w.unit, w.seq.kt.tile(mine), lane % npp) : -1;
       }
       const int pg = lane / DB, d = lane % DB;
       const int id = __shfl_sync(0xffffffffu, ids, (k * npp + pg) & 31);
@@ -239,9 +239,10 @@ GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, ui
       l[h] = 0.f;
     }
     for (int t = w.ta; t < w.tb; ++t, ++nt) {
-      const int j0 = w.seq.kt.tile(t) * TM, j = j0 + r;
+      const int page = a.cache.page, first = (int)page_first(P, w.seq, w.b, w.unit, w.seq.kt.tile(t), r / page);
+      const int j = first + r % page;
       // a released page inside the visible range is not seen either
-      bool seen = key_seen(j, w.seq.len, window, sinks);
+      bool seen = first >= 0 && key_seen(j, w.seq.len, window, sinks);
       if (seen) {
         const int p = a.cache.table[(int64_t)w.seq.row * a.cache.width + j / a.cache.page];
         seen = p >= 0 && p < a.cache.pages;

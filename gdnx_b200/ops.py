@@ -1068,20 +1068,23 @@ class PagedCache:
     """A paged key/value cache on the device.  A slot is one sequence; page ``table[s, i]`` holds its
     tokens ``i*page .. i*page+page-1`` in every layer.  ``refs`` counts the slots that hold a page (0:
     free).  ``status`` is a device word: an operation that cannot be carried out changes nothing and
-    sets it, and while it is set the operations do nothing (:func:`cache_check` reads it)."""
+    sets it, and while it is set the operations do nothing (:func:`cache_check` reads it).  ``bounds``, where the
+    cache has them, are those of each page's keys (:func:`cache_bounds`), which :func:`paged_select` reads."""
     kv: torch.Tensor       # [L, 2, pages, Hk, page, D] (keys, values)
     table: torch.Tensor    # [slots, width] int32, -1 = no page
     lengths: torch.Tensor  # [slots] int32
     refs: torch.Tensor     # [pages] int32
     status: torch.Tensor   # [1] int32
+    bounds: Optional[torch.Tensor] = None  # [L, 2, pages, Hk, D] (least, greatest)
 
     @staticmethod
-    def zeros(L_, pages, Hk, page, D, *, slots, width, dtype=torch.bfloat16, device="cuda"):
+    def zeros(L_, pages, Hk, page, D, *, slots, width, dtype=torch.bfloat16, device="cuda", bounds=False):
         """An empty cache of ``pages`` pages for ``slots`` sequences of up to ``width`` pages."""
         i32 = dict(dtype=torch.int32, device=device)
         return PagedCache(torch.zeros(L_, 2, pages, Hk, page, D, dtype=dtype, device=device),
                           torch.full((slots, width), -1, **i32), torch.zeros(slots, **i32),
-                          torch.zeros(pages, **i32), torch.zeros(1, **i32))
+                          torch.zeros(pages, **i32), torch.zeros(1, **i32),
+                          torch.zeros(L_, 2, pages, Hk, D, dtype=dtype, device=device) if bounds else None)
 
 
 def _cache_struct(c: PagedCache):
@@ -1099,6 +1102,17 @@ def _cache_struct(c: PagedCache):
     return L.Cache(kv.data_ptr(), _DT[kv.dtype], page, layers, pages, hk, d, slots, width, table.data_ptr(),
                    _index32(c.lengths, slots, "lengths", index), _index32(c.refs, pages, "refs", index),
                    _index32(c.status, 1, "status", index)), index
+
+
+def _cache_bounds(c: PagedCache, index: int) -> int:
+    """Address of the cache's bounds."""
+    b, kv = c.bounds, c.kv
+    if b is None:
+        raise ValueError("the cache has no bounds")
+    if b.shape != kv.shape[:4] + kv.shape[5:] or b.dtype is not kv.dtype or not b.is_contiguous():
+        raise ValueError("bounds must be contiguous [L, 2, pages, Hk, D] in the cache's type")
+    _on_device(index, b)
+    return b.data_ptr()
 
 
 def _cache_rows(rows, s, index, name="rows"):
@@ -1179,22 +1193,151 @@ def cache_trim(cache: PagedCache, rows: torch.Tensor, *, window: int, sinks: int
 
 def cache_compact(cache: PagedCache) -> None:
     """Moves the live pages down so that they are the pool's first: page for page in order, those
-    above the live count into the free ones below it."""
+    above the live count into the free ones below it (and their bounds with them)."""
     s, index = _cache_struct(cache)
     need = L.load().gdnx_cache_workspace_bytes(C.byref(s), 0)
     ws = cache.table.new_empty(need, dtype=torch.uint8)
-    _enqueue("gdnx_cache_compact", index, C.byref(s), ws.data_ptr(), need)
+    if cache.bounds is None:
+        _enqueue("gdnx_cache_compact", index, C.byref(s), ws.data_ptr(), need)
+    else:
+        _enqueue("gdnx_cache_compact_bounds", index, C.byref(s), _cache_bounds(cache, index), ws.data_ptr(), need)
+
+
+@dataclass
+class PagedStep:
+    """A serving step's new tokens, packed: sequence i's are rows ``starts[i]`` .. ``starts[i+1]-1`` of a packed tensor, the
+    first of them at position ``first[i]`` of slot ``rows[i]``; rows from ``starts[-1]`` on are padding, -1 in the lists
+    of the packed rows.  One step serves every layer."""
+    rows: torch.Tensor        # [n] int32
+    starts: torch.Tensor      # [n + 1] int32
+    first: torch.Tensor       # [n] int32
+    token_rows: torch.Tensor  # [tokens] int32: each row's slot
+    positions: torch.Tensor   # [tokens] int32: its position there
+    places: torch.Tensor      # [tokens] int64: page * page size + offset
+
+
+def cache_step(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor, tokens: int) -> PagedStep:
+    """:func:`cache_extend`, and where the new tokens stand in packed tensors of ``tokens`` rows (at least the sum of
+    ``counts``, at most 2**20): sequence after sequence in the order of ``rows``.  A step that is refused, or follows a
+    refused operation, has no tokens."""
+    s, index = _cache_struct(cache)
+    at, n = _cache_rows(rows, s, index)
+    more = _index32(counts, n, "counts", index)
+    if tokens < 0:
+        raise ValueError("tokens must not be negative")
+    i32 = dict(dtype=torch.int32)
+    step = PagedStep(rows, rows.new_empty(n + 1, **i32), rows.new_empty(n, **i32), rows.new_empty(tokens, **i32),
+                     rows.new_empty(tokens, **i32), rows.new_empty(tokens, dtype=torch.int64))
+    out = L.Step(tokens, step.starts.data_ptr(), step.first.data_ptr(), step.token_rows.data_ptr(),
+                 step.positions.data_ptr(), step.places.data_ptr())
+    need = L.load().gdnx_cache_workspace_bytes(C.byref(s), n)
+    ws = rows.new_empty(need, dtype=torch.uint8)
+    _enqueue("gdnx_cache_step", index, C.byref(s), n, at, more, C.byref(out), ws.data_ptr(), need)
+    return step
+
+
+def _packed_view(t: torch.Tensor) -> L.View:
+    """View of a packed [tokens,H,D] tensor."""
+    st, sh, sd = t.stride()
+    d = t.shape[2]
+    if sd != 1 and d > 1:
+        raise ValueError("the last dim of every input must be contiguous")
+    return L.View(t.data_ptr(), _DT[t.dtype], d, 0, st, sh)
+
+
+def cache_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, step: PagedStep, *, layer: int = 0) -> None:
+    """The packed keys and values ``k``, ``v`` [tokens,Hk,D] of a step's new tokens go to their places in ``layer``
+    (what padding rows hold goes nowhere).  Meant for the step's own cache before its slots change again."""
+    s, index = _cache_struct(cache)
+    _on_device(index, k, v)
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != s.Hk or k.shape[2] != s.D:
+        raise ValueError("k and v must be [tokens,Hk,D] with the cache's heads")
+    if k.dtype is not cache.kv.dtype or v.dtype is not cache.kv.dtype:
+        raise TypeError("k and v must have the cache's type")
+    if not 0 <= layer < s.L:
+        raise ValueError("no such layer")
+    places = step.places
+    if places.dtype is not torch.int64 or places.dim() != 1 or not places.is_contiguous() or places.shape[0] != k.shape[0]:
+        raise ValueError("the step must have k's rows")
+    _on_device(index, places)
+    _enqueue("gdnx_cache_append", index, C.byref(s), layer, k.shape[0], C.byref(_packed_view(k)), C.byref(_packed_view(v)),
+             places.data_ptr())
+
+
+def cache_bounds(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor, *, layer: int = 0) -> None:
+    """Brings ``cache.bounds`` up to date in ``layer`` after the last ``counts[i]`` tokens of slots ``rows`` were written
+    (int32 vectors, each slot once): for every page on which one of them lies, the least and the greatest value of each
+    dim among its tokens' keys, NaN where a key's is.  Exact.  Refused where a slot has fewer tokens, or its last page is
+    partly filled and held by another slot too (bring the bounds up to date before the fork)."""
+    s, index = _cache_struct(cache)
+    at, n = _cache_rows(rows, s, index)
+    if not 0 <= layer < s.L:
+        raise ValueError("no such layer")
+    _enqueue("gdnx_cache_bounds", index, C.byref(s), layer, n, at, _index32(counts, n, "counts", index),
+             _cache_bounds(cache, index))
+
+
+def paged_select(q: torch.Tensor, cache: PagedCache, k: int, *, layer: int = 0, rows: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None, window: int = 1, sinks: int = 0,
+                 max_len: Optional[int] = None) -> torch.Tensor:
+    """The ``k`` pages that each query's key heads are to read, for :func:`paged_decode`'s ``pages``: [B,Hk,k] int32
+    indexes into the slot's table row, rising, -1 behind them.
+
+    ``q`` [B,H,D], row i for slot ``rows[i]`` (int32; default slot i), at ``positions[i]`` (int32; default: the slot's last
+    token).  A page's score, from ``cache.bounds``, is the greatest of its query heads' sums over d of
+    max(q_d lo_d, q_d hi_d): no key on the page has a greater product with a query (NaN counts as +inf; summed in 64
+    bits).  Taken are the pages that hold one of the first ``sinks`` or the last ``window`` tokens (no more than ``k``
+    pages), then those of largest score, the lower page first among equals.  Released pages are not taken.  ``max_len``,
+    if known, is the longest slot's length; it only sizes the launch."""
+    s, index = _cache_struct(cache)
+    _on_device(index, q)
+    if q.dim() != 3:
+        raise ValueError("q must be [B,H,D]")
+    B, H, D = q.shape
+    if D != s.D or H == 0 or H % s.Hk:
+        raise ValueError("q must be [B,H,D] with the cache's head size and H a multiple of its heads")
+    if q.dtype is not cache.kv.dtype:
+        raise TypeError("q must have the cache's type")
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be at least 1, sinks at least 0")
+    if k < -(-sinks // s.page) + (window + s.page - 2) // s.page + 1:
+        raise ValueError("k must be at least the pages of the window and the sinks")
+    if not 0 <= layer < s.L:
+        raise ValueError("no such layer")
+    qb, qh, qd = q.stride()
+    if qd != 1:
+        raise ValueError("the last dim of every input must be contiguous")
+    if rows is None and B > s.slots:
+        raise ValueError("more queries than slots")
+    out = q.new_empty((B, s.Hk, k), dtype=torch.int32)
+    a = L.PagedSelectArgs(s, _cache_bounds(cache, index), B, H, layer, k, window, sinks, max_len or 0,
+                          L.View(q.data_ptr(), _DT[q.dtype], D, qb, 0, qh),
+                          None if rows is None else _index32(rows, B, "rows", index),
+                          None if positions is None else _index32(positions, B, "positions", index), out.data_ptr())
+    need = L.load().gdnx_paged_select_workspace_bytes(C.byref(a))
+    ws = None
+    if need:
+        ws = q.new_empty(need, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    _enqueue("gdnx_paged_select", index, C.byref(a))
+    return out
 
 
 def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Optional[torch.Tensor] = None,
                  window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
                  max_len: Optional[int] = None, out: Optional[torch.Tensor] = None,
-                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+                 out_dtype: Optional[torch.dtype] = None, positions: Optional[torch.Tensor] = None,
+                 pages: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token per sequence over a paged cache: ``q`` [B,H,D], row i for slot
     ``rows[i]`` (int32; default slot i), whose last token it is (written before this call).  It sees
     the slot's tokens within ``window`` (None: all) and the first ``sinks``; tokens on released pages
     are not seen.  A slot of length 0 gives zeros, scores of NaN or +inf, or only -inf, give NaN.  ``max_len``, if known, is the longest slot's
-    length; it only sizes the split over the cache's length.  Returns [B,H,D]."""
+    length; it only sizes the split over the cache's length.
+
+    ``positions`` [B] int32: row i stands at that position of its slot instead (-1: nowhere) and sees no later token.
+    ``pages`` [B,Hk,k] int32, as :func:`paged_select` gives them: row i's key heads see of these tokens only those on the
+    pages that their lists name, as indexes into the slot's table row, each once.  As many entries of a list are read as
+    the slot has pages up to the position; others than the slot's are passed over.  Returns [B,H,D]."""
     s, index = _cache_struct(cache)
     _on_device(index, q)
     if q.dim() != 3:
@@ -1227,6 +1370,13 @@ def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Op
                           D ** -0.5 if scale is None else scale, L.View(q.data_ptr(), _DT[q.dtype], D, qb, 0, qh),
                           None if rows is None else _index32(rows, B, "rows", index), y.data_ptr(), _DT[y.dtype], yb, yh,
                           _error_word(index))
+    if positions is not None:
+        a.positions = _index32(positions, B, "positions", index)
+    if pages is not None:
+        if pages.dtype is not torch.int32 or pages.dim() != 3 or pages.shape[:2] != (B, s.Hk) or pages.shape[2] < 1 or not pages.is_contiguous():
+            raise ValueError("pages must be a contiguous int32 tensor [B,Hk,k]")
+        _on_device(index, pages)
+        a.pages, a.listed = pages.data_ptr(), pages.shape[2]
     need = L.load().gdnx_paged_decode_workspace_bytes(C.byref(a))
     ws = None
     if need:

@@ -502,12 +502,67 @@ GDNX_API gdnx_status gdnx_cache_trim(const gdnx_cache* cache, int64_t n, const i
 /* Moves the live pages at or above index n_live down into the free ones below it (in
  * order), so that the n_live live pages are the pool's first. */
 GDNX_API gdnx_status gdnx_cache_compact(const gdnx_cache* cache, void* workspace, size_t workspace_bytes, void* stream);
+/* The same with a tensor of bounds (gdnx_cache_bounds), whose pages move along. */
+GDNX_API gdnx_status gdnx_cache_compact_bounds(const gdnx_cache* cache, void* bounds, void* workspace,
+                                               size_t workspace_bytes, void* stream);
+
+/* A serving step's new tokens, of different numbers in different slots, packed behind one another: sequence i has
+ * rows starts[i] .. starts[i+1]-1 of a packed tensor, its first token at position first[i] of slot rows[i].  Rows
+ * from starts[n] on are padding. */
+typedef struct {
+  int64_t tokens;              /* rows of the packed tensors, at most 2^20 */
+  int32_t* starts;             /* [n + 1] */
+  int32_t* first;              /* [n] */
+  int32_t* token_rows;         /* [tokens] a row's slot, -1 for padding */
+  int32_t* positions;          /* [tokens] its position in the slot, -1 for padding */
+  int64_t* places;             /* [tokens] page * page size + offset of its place in the pool, -1 for padding */
+} gdnx_step;
+
+/* gdnx_cache_extend, and where the new tokens stand (everything in `step` is written).  More tokens than the packed
+ * tensors have rows are refused (GDNX_EINVAL); a step that is refused, or follows a refused operation, has no tokens. */
+GDNX_API gdnx_status gdnx_cache_step(const gdnx_cache* cache, int64_t n, const int32_t* rows, const int32_t* counts,
+                                     const gdnx_step* step, void* workspace, size_t workspace_bytes, void* stream);
+/* k, v [tokens,Hk,D] (st, sh) go to a step's places in `layer`; padding goes nowhere. */
+GDNX_API gdnx_status gdnx_cache_append(const gdnx_cache* cache, int64_t layer, int64_t tokens, const gdnx_view* k,
+                                       const gdnx_view* v, const int64_t* places, void* stream);
+/* bounds [L, 2, pages, Hk, D] in the cache's type, 16-byte aligned: of each page on which one of the last counts[i]
+ * tokens of slot rows[i] lies, the least and the greatest value of each dim among the keys of the page's tokens in
+ * `layer` (NaN where a key's is).  Released pages are left out.  GDNX_EINVAL where a slot has fewer tokens, or its
+ * last page is partly filled and held by another slot too. */
+GDNX_API gdnx_status gdnx_cache_bounds(const gdnx_cache* cache, int64_t layer, int64_t n, const int32_t* rows,
+                                       const int32_t* counts, void* bounds, void* stream);
+
+/* The pages that each query's key heads are to read, by their bounds.  Query b stands at position positions[b] of slot
+ * rows[b] (its last token where positions is NULL) and has the pages up to that position.  A page's score is the
+ * greatest of the head's query heads' sums over d of max(q_d lo_d, q_d hi_d), in 64 bits (NaN counts as +inf).  Taken
+ * are the pages that hold one of the first `sinks` or the last `window` tokens, then those of largest score, the lower
+ * page first among equals, k in all; released pages are not taken.
+ * selected [B,Hk,k]: indexes into the slot's table row, rising, -1 behind them. */
+typedef struct {
+  gdnx_cache cache;
+  const void* bounds;          /* as gdnx_cache_bounds leaves them */
+  int64_t B, H, layer, k;
+  int64_t window, sinks;       /* window >= 1; their pages are at most k */
+  int64_t max_len;             /* no slot is longer: sizes the launch; 0 = width * page */
+  gdnx_view q;                 /* [B,H,D] (sb, sh), the cache's type */
+  const int32_t* rows;         /* [B] device; NULL = slots 0..B-1 */
+  const int32_t* positions;    /* [B] device; NULL = the slots' last tokens */
+  int32_t* selected;
+  void* workspace;             /* 16-byte aligned */
+  size_t workspace_bytes;
+} gdnx_paged_select_args;
+
+GDNX_API size_t gdnx_paged_select_workspace_bytes(const gdnx_paged_select_args* args);
+GDNX_API gdnx_status gdnx_paged_select(const gdnx_paged_select_args* args, void* stream);
 
 /* Attention of one new token per query row over a cache: row i of q reads slot rows[i],
  * whose last token it is (the token's own key and value are written before the call).
  * It sees token j < length where length - 1 - j < window or j < sinks; tokens on released
  * pages are not seen.  A row that sees nothing (length 0, a slot out of range) gives 0;
  * one that sees a score of NaN or +inf, or only -inf, is NaN.
+ * With `positions`, row i of q stands at that position of its slot instead (-1: nowhere) and sees no later token.
+ * With `pages`, it sees of these only the tokens on the pages that its key head's list names: indexes into the
+ * slot's table row, each once, of which as many are read as the slot has pages; others than the slot's are passed over.
  * The visible tokens are split over CTAs, and the parts joined in a fixed order. */
 typedef struct {
   gdnx_cache cache;
@@ -523,6 +578,9 @@ typedef struct {
   int32_t* error;              /* device word that takes GDNX_ETIMEOUT; NULL = none */
   void* workspace;             /* 16-byte aligned */
   size_t workspace_bytes;
+  const int32_t* positions;    /* [B] device; NULL = the slots' last tokens */
+  const int32_t* pages;        /* [B,Hk,listed] device; NULL = all */
+  int64_t listed;
 } gdnx_paged_decode_args;
 
 GDNX_API size_t gdnx_paged_decode_workspace_bytes(const gdnx_paged_decode_args* args);

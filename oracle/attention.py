@@ -174,25 +174,119 @@ class PagedCache:
 
     def tokens(self, r, layer, window=None, sinks=0):
         """Keys and values [n, Hk, D] in 64 bits of what the last token of slot r sees."""
-        n = self.lengths[r]
+        return self.seen(r, self.lengths[r], layer, window, sinks)
+
+    def seen(self, r, n, layer, window=None, sinks=0, pages=None):
+        """The same of the last of its first n tokens (`pages`: on these pages only)."""
         window = n if window is None else window
-        at = [(self.table[r][j // self.page], j % self.page) for j in range(n) if n - 1 - j < window or j < sinks]
+        at = [(self.table[r][j // self.page], j % self.page) for j in range(n)
+              if (n - 1 - j < window or j < sinks) and (pages is None or j // self.page in pages)]
         at = [(p, o) for p, o in at if p >= 0]
         pick = lambda side: torch.stack([self.kv[layer, side, p, :, o].double() for p, o in at])  # noqa: E731
         return (pick(0), pick(1)) if at else (None, None)
 
-    def decode(self, q, layer=0, rows=None, window=None, sinks=0, scale=None):
+    def decode(self, q, layer=0, rows=None, window=None, sinks=0, scale=None, positions=None, pages=None):
         """y [B,H,D] in 64 bits."""
         B, H, D = q.shape
         q = q.detach().double().cpu()
         y = torch.zeros(B, H, D, dtype=torch.float64)
         for b in range(B):
             r = b if rows is None else rows[b]
-            k, v = self.tokens(r, layer, window, sinks) if 0 <= r < len(self.table) else (None, None)
-            if k is None:
+            if not 0 <= r < len(self.table):
                 continue
+            n = self.lengths[r] if positions is None else max(0, min(self.lengths[r], positions[b] + 1))
+            Hk = self.kv.shape[3]
             for h in range(H):
-                g = h // (H // k.shape[1])
+                g = h // (H // Hk)
+                k, v = self.seen(r, n, layer, window, sinks, None if pages is None else pages[b][g])
+                if k is None:
+                    continue
                 p = torch.softmax(k[:, g] @ q[b, h] * (D ** -0.5 if scale is None else scale), 0)
                 y[b, h] = p @ v[:, g]
         return y
+
+    def step(self, rows, counts, tokens):
+        """extend, and (starts, first, slot of each packed row, position, place); nothing new where refused."""
+        first = [self.lengths[r] if 0 <= r < len(self.lengths) else 0 for r in rows]
+        if not self._bad(rows, *counts) and sum(counts) > tokens:
+            self.status = "invalid"
+        self.extend(rows, counts)
+        if self.status:
+            first, counts = [0] * len(rows), [0] * len(rows)
+        starts, slots, positions, places = [0], [], [], []
+        for r, f, c in zip(rows, first, counts):
+            starts.append(starts[-1] + c)
+            for p in range(f, f + c):
+                slots.append(r)
+                positions.append(p)
+                places.append(self.table[r][p // self.page] * self.page + p % self.page)
+        pad = [-1] * (tokens - len(slots))
+        return starts, first, slots + pad, positions + pad, places + pad
+
+    def append(self, k, v, places, layer):
+        if self.status:
+            return
+        for t, at in enumerate(places):
+            if at >= 0:
+                for side, x in enumerate((k, v)):
+                    self.kv[layer, side, at // self.page, :, at % self.page] = x[t].cpu()
+
+    def page_bounds(self, r, i, layer):
+        """(lo, hi) [Hk, D] of the keys on page i of slot r."""
+        n = min(self.page, self.lengths[r] - i * self.page)
+        k = self.kv[layer, 0, self.table[r][i], :, :n].double()
+        return k.amin(1), k.amax(1)
+
+    def update_bounds(self, bounds, rows, counts, layer):
+        """Writes the bounds [L, 2, pages, Hk, D] of the pages that the slots' last tokens lie on."""
+        if self._bad(rows, *counts):
+            return
+        last = [self.table[r][self.lengths[r] // self.page] if self.lengths[r] % self.page else -1 for r in rows]
+        if any(c > self.lengths[r] or (c > 0 and p >= 0 and self.refs[p] > 1) for r, c, p in zip(rows, counts, last)):
+            self.status = "invalid"
+            return
+        for r, c in zip(rows, counts):
+            for i in range((self.lengths[r] - c) // self.page, self._pages(self.lengths[r])) if c else ():
+                if self.table[r][i] >= 0:
+                    for side, x in enumerate(self.page_bounds(r, i, layer)):
+                        bounds[layer, side, self.table[r][i]] = x.to(bounds.dtype)
+
+    def select(self, q, bounds, k, layer=0, rows=None, positions=None, window=1, sinks=0):
+        """[B, Hk, k] lists of pages, from given bounds."""
+        B, H, _ = q.shape
+        Hk = bounds.shape[3]
+        q, lo, hi = q.detach().double().cpu(), bounds[layer, 0].double().cpu(), bounds[layer, 1].double().cpu()
+        out = []
+        for b in range(B):
+            r = b if rows is None else rows[b]
+            n = self.lengths[r] if 0 <= r < len(self.table) else 0
+            if positions is not None:
+                n = max(0, min(n, positions[b] + 1))
+            have = [i for i in range(self._pages(n)) if self.table[r][i] >= 0]
+            out.append([])
+            for h in range(Hk):
+                def score(i):
+                    p = self.table[r][i]
+                    x = q[b, h * (H // Hk):(h + 1) * (H // Hk)]
+                    s = torch.where(x >= 0, x * hi[p, h], x * lo[p, h]).sum(1)
+                    return torch.where(s.isnan(), math.inf, s).max().item()
+                always = [i for i in have if i * self.page < sinks or (i + 1) * self.page > n - window]
+                rest = sorted((i for i in have if i not in always), key=lambda i: (-score(i), i))
+                take = sorted(always + rest[: k - len(always)])
+                out[-1].append(take + [-1] * (k - len(take)))
+        return out
+
+    def attend(self, q, step, layer=0, window=None, sinks=0, scale=None):
+        """(y [tokens,H,D], lse [tokens,H]) in 64 bits of a step's packed queries; padding rows 0 and -inf."""
+        starts, _, slots, positions = step[:4]
+        N, H, D = q.shape
+        q = q.detach().double().cpu()
+        y, lse = torch.zeros(N, H, D, dtype=torch.float64), torch.full((N, H), -math.inf, dtype=torch.float64)
+        for t in range(starts[-1]):
+            k, v = self.seen(slots[t], positions[t] + 1, layer, window, sinks)
+            if k is None:
+                continue
+            s = torch.einsum("hgd,nhd->hgn", q[t].view(k.shape[1], -1, D), k) * (D ** -0.5 if scale is None else scale)
+            y[t] = torch.einsum("hgn,nhd->hgd", torch.softmax(s, -1), v).reshape(H, D)
+            lse[t] = torch.logsumexp(s, -1).reshape(H)
+        return y, lse
