@@ -24,7 +24,7 @@ EXPORTED = ("gdnx_scan_fwd", "gdnx_scan_fwd_noalloc", "gdnx_scan_noalloc_status"
             "gdnx_ipc_close", "gdnx_error_word", "gdnx_error_status", "gdnx_attn_fwd", "gdnx_attn_bwd", "gdnx_attn_bwd_workspace_bytes", "gdnx_cache_fork",
             "gdnx_cache_extend", "gdnx_cache_write", "gdnx_cache_truncate", "gdnx_cache_trim", "gdnx_cache_compact",
             "gdnx_cache_compact_bounds", "gdnx_cache_step", "gdnx_cache_append", "gdnx_cache_bounds",
-            "gdnx_paged_select", "gdnx_paged_select_workspace_bytes",
+            "gdnx_paged_attn", "gdnx_paged_attn_workspace_bytes", "gdnx_paged_select", "gdnx_paged_select_workspace_bytes",
             "gdnx_cache_workspace_bytes", "gdnx_paged_decode", "gdnx_paged_decode_workspace_bytes")
 
 
@@ -154,6 +154,14 @@ class Step(C.Structure):
                 ("positions", C.c_void_p), ("places", C.c_void_p)]
 
 
+class PagedAttnArgs(C.Structure):
+    _fields_ = [("cache", Cache), ("n", C.c_int64), ("tokens", C.c_int64), ("H", C.c_int64), ("layer", C.c_int64),
+                ("window", C.c_int64), ("sinks", C.c_int64), ("max_len", C.c_int64), ("scale", C.c_float), ("q", View),
+                ("rows", C.c_void_p), ("starts", C.c_void_p), ("first", C.c_void_p), ("y", C.c_void_p),
+                ("y_dtype", C.c_int32), ("y_st", C.c_int64), ("y_sh", C.c_int64), ("lse", C.c_void_p),
+                ("error", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 class PagedSelectArgs(C.Structure):
     _fields_ = [("cache", Cache), ("bounds", C.c_void_p), ("B", C.c_int64), ("H", C.c_int64), ("layer", C.c_int64),
                 ("k", C.c_int64), ("window", C.c_int64), ("sinks", C.c_int64), ("max_len", C.c_int64), ("q", View),
@@ -235,6 +243,10 @@ def load(path: Path = LIB_PATH):
     lib.gdnx_paged_decode_workspace_bytes.restype = size
     lib.gdnx_paged_decode.argtypes = [C.POINTER(PagedDecodeArgs), C.c_void_p]
     lib.gdnx_paged_decode.restype = C.c_int
+    lib.gdnx_paged_attn_workspace_bytes.argtypes = [C.POINTER(PagedAttnArgs)]
+    lib.gdnx_paged_attn_workspace_bytes.restype = size
+    lib.gdnx_paged_attn.argtypes = [C.POINTER(PagedAttnArgs), C.c_void_p]
+    lib.gdnx_paged_attn.restype = C.c_int
     lib.gdnx_paged_select_workspace_bytes.argtypes = [C.POINTER(PagedSelectArgs)]
     lib.gdnx_paged_select_workspace_bytes.restype = size
     lib.gdnx_paged_select.argtypes = [C.POINTER(PagedSelectArgs), C.c_void_p]

@@ -394,6 +394,43 @@ gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* a, void* stream) {
                                    : gdnx::launch_paged_decode_tc(c, (cudaStream_t)stream);
 }
 
+static gdnx_status check_paged_attn(const gdnx_paged_attn_args& a) {
+  const gdnx_status s = check_cache(&a.cache);
+  if (s != GDNX_OK) return s;
+  if (a.cache.pages < 1 || a.n < 0 || a.n > a.cache.slots || a.tokens < 0 || a.H <= 0 || a.H % a.cache.Hk || a.layer < 0 ||
+      a.layer >= a.cache.L || a.window < 1 || a.sinks < 0 || a.max_len < 0 || !(a.scale > 0.f) || a.scale > 3.0e38f ||
+      !dtype_ok(a.y_dtype))
+    return GDNX_EINVAL;
+  return a.tokens > kMaxPacked || a.H > 65535 ? GDNX_EUNSUPPORTED : GDNX_OK;
+}
+
+// Window and sinks beyond the longest sequence say no more than its length does.
+static gdnx_paged_attn_args clamp_paged(const gdnx_paged_attn_args& a) {
+  gdnx_paged_attn_args c = a;
+  const int64_t most = a.cache.width * a.cache.page;
+  if (c.window > most) c.window = most;
+  if (c.sinks > most) c.sinks = most;
+  return c;
+}
+
+size_t gdnx_paged_attn_workspace_bytes(const gdnx_paged_attn_args* a) {
+  if (!a || check_paged_attn(*a) != GDNX_OK || a->tokens == 0) return 0;
+  return gdnx::paged_attn_simt_workspace_bytes(clamp_paged(*a));
+}
+
+gdnx_status gdnx_paged_attn(const gdnx_paged_attn_args* a, void* stream) {
+  if (!a) return GDNX_EINVAL;
+  const gdnx_status s = check_paged_attn(*a);
+  if (s != GDNX_OK || a->tokens == 0) return s;
+  if (!heads_ok(a->q, a->cache.dtype, a->cache.D) || !device_ptr(a->y, bytes_of(a->y_dtype)) || a->y_st < 0 || a->y_sh < 0)
+    return GDNX_EINVAL;
+  if (!words(a->starts) || (a->n && (!words(a->rows) || !words(a->first)))) return GDNX_EINVAL;
+  if ((a->lse && !device_ptr(a->lse, sizeof(float))) || (a->error && !words(a->error))) return GDNX_EINVAL;
+  const size_t need = gdnx_paged_attn_workspace_bytes(a);
+  if (need && (a->workspace_bytes < need || !device_ptr(a->workspace, 16))) return GDNX_EWORKSPACE;
+  return gdnx::launch_paged_attn_simt(clamp_paged(*a), (cudaStream_t)stream);
+}
+
 const char* gdnx_status_string(gdnx_status s) {
   switch (s) {
     case GDNX_OK: return "GDNX_OK";

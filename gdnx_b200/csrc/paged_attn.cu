@@ -1,0 +1,209 @@
+// Attention of a chunk of new tokens over a paged cache, on the CUDA cores (all arithmetic fp32).
+//
+// Blocks of 32 rows (tokens times the heads of a group, paged_attn.cuh) walk key tiles of 64 as windowed attention's
+// forward does (attn_simt.cuh):  s = scale log2(e) q.k;  m' = max(m, max_j s);  p = 2^(s - m');
+//   l = l 2^(m - m') + sum_j p;  o = o 2^(m - m') + p V;   y = o / l.
+// A tile's tokens come from up to four pages by 16-byte asynchronous copies; what lies on no page, or behind the
+// sequence's last token, is zero and not seen.
+#include "attn_simt.cuh"
+#include "paged_attn.cuh"
+
+namespace gdnx {
+namespace {
+
+using Simt = Shape<BR, BT, false>;
+constexpr int GRANULES = BT / 16;  // of 16 tokens: the smallest page
+
+struct Ids {
+  int id[GRANULES];  // page of each granule, -1 where there is none
+};
+
+// Tokens j0.. of keys or values (side) into dst [BT][DP + 4].
+template <int DP, typename T>
+GDNX_DEV void load_paged(float* dst, const gdnx_cache& c, int64_t layer, int side, int hk, const int* ids, int j0, int len) {
+  const int D = (int)c.D;
+  const T* base = static_cast<const T*>(c.kv) + (layer * 2 + side) * c.pages * c.Hk * c.page * D;
+  constexpr int V = 16 / sizeof(T);  // values of a copy
+#pragma unroll
+  for (int k = 0; k < (BT * DP / V + NT - 1) / NT; ++k) {
+    const int i = k * NT + threadIdx.x, r = i / (DP / V), d = i % (DP / V) * V;
+    if (BT * DP / V % NT && r >= BT) break;
+    const int id = ids[r / 16];
+    const bool on = id >= 0 && j0 + r < len && d < D;
+    const T* src = on ? base + (((int64_t)id * c.Hk + hk) * c.page + (j0 + r) % c.page) * D + d : base;
+    float* to = dst + r * (DP + 4) + d;
+    if constexpr (sizeof(T) == 4) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                       static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                   "l"(src), "r"(on ? 16 : 0)
+                   : "memory");
+    } else {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (on) u = *reinterpret_cast<const uint4*>(src);
+      const T* x = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int e = 0; e < V; ++e) to[e] = to_f32(x[e]);
+    }
+  }
+}
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParams P) {
+  extern __shared__ float sm[];
+  __shared__ Share share;
+  __shared__ long long sums[NT / 32];
+  __shared__ Ids ids;
+  const gdnx_paged_attn_args& a = P.a;
+  const gdnx_cache& c = a.cache;
+  float* Q = sm;
+  float* KV = Q + BR * (DP + 4);
+  float* W = KV + BT * (DP + 4);
+  dependents_may_start();
+  wait_for_earlier();
+  find_share<Simt, NT>(P, share, sums);
+  if (threadIdx.x == 0 && P.cut) P.joint[blockIdx.x] = {0, 0, 0, 0, -1};
+  write_padding(P, threadIdx.x, NT);
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, D = (int)c.D;
+  const int window = (int)a.window, sinks = (int)a.sinks;
+  const float c2 = a.scale * kLog2e;
+  const float* q = Q + ty * 4 * (DP + 4);
+  float* w = W + ty * 4 * LDP;
+  Walk<Simt> x(P, share);
+  while (x.next()) {
+    const int heads = x.heads(), h0 = x.head0(), len = x.s.len(), t0 = x.x.t0;
+    __syncthreads();  // the unit before has read its tiles
+    for (int i = threadIdx.x; i < BR * DP; i += NT) {
+      const int r = i / DP, d = i % DP, t = t0 + r / P.gs, g = r % P.gs;
+      float v = 0.f;
+      if (r / P.gs < P.tb && g < heads && t < x.s.count && d < D)
+        v = ld_as_f32(a.q.ptr, a.q.dtype, (int64_t)(x.s.start + t) * a.q.st + (int64_t)(h0 + g) * a.q.sh + d);
+      Q[r * (DP + 4) + d] = v;
+    }
+    int p[4];  // positions of this thread's rows, -1: no query
+    float m[4], l[4];
+    bool any[4];
+    float2 o[4][DP / 32];
+    clear(o);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = ty * 4 + r, t = t0 + i / P.gs;
+      p[r] = i / P.gs < P.tb && i % P.gs < heads && t < x.s.count ? x.s.first + t : -1;
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+      any[r] = false;
+    }
+    // positions of the warp's eight rows
+    const int pw = x.s.first + t0 + ty / 2 * 8 / P.gs, pz = min(x.s.first + t0 + (ty / 2 * 8 + 7) / P.gs, len - 1);
+    for (int k = x.ta; k < x.tb; ++k) {
+      const int j0 = x.x.kt.tile(k) * BT;
+      // columns that some of the warp's rows see
+      const int lo = pw - window + 1 - j0;
+      const Groups gr = pw >= len ? Groups(1, 0) : sinks <= j0 ? Groups(lo, pz - j0)
+                                                               : Groups(0, lo <= BT - 1 ? pz - j0 : min(pz - j0, sinks - 1 - j0));
+      __syncthreads();
+      if (threadIdx.x < GRANULES) {
+        const int64_t page = (j0 + 16 * threadIdx.x) / c.page;
+        const int id = page < c.width ? c.table[(int64_t)x.s.row * c.width + page] : -1;
+        ids.id[threadIdx.x] = id >= 0 && id < c.pages ? id : -1;
+      }
+      __syncthreads();
+      load_paged<DP, T>(KV, c, a.layer, 0, x.hk(), ids.id, j0, len);
+      wait_tiles();
+      __syncthreads();
+      for_groups(gr.n, [&](auto nc) {
+        constexpr int NC = decltype(nc)::value;
+        const int col = 16 * gr.first + tx;
+        float s[4][4];
+        dot_tile<DP, NC>(s, q, KV + col * (DP + 4), D);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float mx = m[r];
+#pragma unroll
+          for (int e = 0; e < NC; ++e) {
+            const bool on = sees(p[r], j0 + col + 16 * e, len, window, sinks) && ids.id[gr.first + e] >= 0;
+            any[r] |= on;
+            s[r][e] = on ? s[r][e] * c2 : -INFINITY;
+            mx = fmaxf(mx, s[r][e]);
+          }
+          mx = half_warp_max(mx);
+          const float base = mx == -INFINITY ? 0.f : mx;
+          const float corr = exp2f(m[r] - base);
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < NC; ++e) {
+            s[r][e] = exp2f(s[r][e] - base);
+            sum += s[r][e];
+            w[r * LDP + col + 16 * e] = s[r][e];
+          }
+          l[r] = l[r] * corr + half_warp_sum(sum);
+          m[r] = mx;
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) o[r][d] = mul2(o[r][d], make_float2(corr, corr));
+        }
+      });
+      __syncthreads();
+      load_paged<DP, T>(KV, c, a.layer, 1, x.hk(), ids.id, j0, len);
+      wait_tiles();
+      __syncthreads();
+      acc_tile<DP>(o, w, KV, tx, gr);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = ty * 4 + r;
+      const uint32_t half = 0xffffu << (threadIdx.x % 32 / 16 * 16);
+      const bool seen = __ballot_sync(0xffffffffu, any[r]) & half;
+      if (p[r] < 0) continue;
+      const float top = seen ? fmaxf(m[r], kNoScore) : -INFINITY;
+      if (x.whole()) {
+        const int64_t tok = x.s.start + t0 + i / P.gs, h = h0 + i % P.gs;
+        const float f = scale_of(top, l[r]);
+        for_pieces<DP>(o[r], tx, [&](int d, const float2* v, auto n) {
+          if (d < D) store_piece<decltype(n)::value>(a.y, a.y_dtype, tok * a.y_st + h * a.y_sh + d, v, f);
+        });
+        if (a.lse && tx == 0) a.lse[tok * a.H + h] = lse_of(top, l[r]);
+      } else {
+        const int64_t at = x.part() + i;
+        for_pieces<DP>(o[r], tx, [&](int d, const float2* v, auto n) {
+          if (d < D) store_piece<decltype(n)::value>(P.part, GDNX_F32, at * D + d, v, 1.f);
+        });
+        if (tx == 0) {
+          P.stat[at * 2] = top;
+          P.stat[at * 2 + 1] = l[r];
+        }
+      }
+    }
+    if (threadIdx.x == 0 && x.ends_cut()) P.joint[blockIdx.x] = x.joint(share.per);
+  }
+}
+
+template <int DP, typename T>
+gdnx_status run(const ChunkParams& P, cudaStream_t st) {
+  constexpr int smem = ((BR + BT) * (DP + 4) + BR * LDP) * (int)sizeof(float);
+  static std::atomic<uint64_t> done;
+  if (!allow_smem(paged_attn_simt_kernel<DP, T>, smem, done)) return GDNX_ELAUNCH;
+  if (launch_early(paged_attn_simt_kernel<DP, T>, dim3((unsigned)P.grid), dim3(NT), smem, st, P) != cudaSuccess)
+    return GDNX_ELAUNCH;
+  return join_chunks<Simt>(P, st);
+}
+template <typename T>
+gdnx_status run_of(const ChunkParams& P, cudaStream_t st) {
+  const int64_t D = P.a.cache.D;
+  return D > 96 ? run<128, T>(P, st) : D > 64 ? run<96, T>(P, st) : run<64, T>(P, st);
+}
+
+ChunkParams plan(const gdnx_paged_attn_args& a) { return plan_chunks<Simt>(a, sm_count() * 3); }
+
+}  // namespace
+
+size_t paged_attn_simt_workspace_bytes(const gdnx_paged_attn_args& a) { return chunk_bytes(plan(a)); }
+
+gdnx_status launch_paged_attn_simt(const gdnx_paged_attn_args& a, cudaStream_t st) {
+  const ChunkParams P = plan(a);
+  switch (a.cache.dtype) {
+    case GDNX_BF16: return run_of<__nv_bfloat16>(P, st);
+    case GDNX_F16: return run_of<__half>(P, st);
+    default: return run_of<float>(P, st);
+  }
+}
+
+}  // namespace gdnx

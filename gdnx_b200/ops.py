@@ -1264,6 +1264,61 @@ def cache_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, step: Page
              places.data_ptr())
 
 
+def paged_attention(q: torch.Tensor, cache: PagedCache, step: PagedStep, *, layer: int = 0, window: Optional[int] = None,
+                    sinks: int = 0, scale: Optional[float] = None, max_len: Optional[int] = None,
+                    out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, return_lse: bool = False):
+    """Attention of a step's packed new tokens (chunks of prompts, proposals, single tokens, mixed) over the cache that
+    holds them (:func:`cache_append`) and what came before.  ``q`` [tokens,H,D] in the cache's type, any strides with a
+    contiguous last dim, H a multiple of the cache's heads.
+
+    The token at position p of its slot sees the slot's token j <= p where p - j < ``window`` (None: no window) or
+    j < ``sinks``; tokens on released pages are not seen.  Padding rows give zeros.  A row that sees a score of NaN or
+    +inf, or only -inf, is NaN.  ``scale`` defaults to D ** -0.5.  ``max_len``, if known, is the longest slot's length;
+    it only sizes the split over the cache's length.  Returns y [tokens,H,D] (and the log of the sum of exponentials
+    [tokens,H] fp32 if asked, -inf where a row is padding or sees nothing)."""
+    s, index = _cache_struct(cache)
+    _on_device(index, q)
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens,H,D]")
+    N, H, D = q.shape
+    if D != s.D or H == 0 or H % s.Hk:
+        raise ValueError("q must be [tokens,H,D] with the cache's head size and H a multiple of its heads")
+    if q.dtype is not cache.kv.dtype:
+        raise TypeError("q must have the cache's type")
+    if step.positions.shape[0] != N:
+        raise ValueError("the step must have q's rows")
+    if window is None:
+        window = 1 << 62
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be at least 1 (None: no window), sinks at least 0")
+    if not 0 <= layer < s.L:
+        raise ValueError("no such layer")
+    if out is None:
+        y = q.new_empty(q.shape) if out_dtype is None else q.new_empty(q.shape, dtype=out_dtype)
+    else:
+        y = out
+        _on_device(index, y)
+        if y.shape != q.shape or y.dtype not in _DT or (D > 1 and y.stride(-1) != 1):
+            raise ValueError("out must be [tokens,H,D] with a contiguous last dim")
+    yt, yh, _ = y.stride()
+    rows, n = _cache_rows(step.rows, s, index)
+    a = L.PagedAttnArgs(s, n, N, H, layer, min(window, 1 << 62), min(sinks, 1 << 62), max_len or 0,
+                        D ** -0.5 if scale is None else scale, _packed_view(q), rows,
+                        _index32(step.starts, n + 1, "starts", index), _index32(step.first, n, "first", index),
+                        y.data_ptr(), _DT[y.dtype], yt, yh)
+    lse = q.new_empty((N, H), dtype=torch.float32) if return_lse else None
+    if return_lse:
+        a.lse = lse.data_ptr()
+    a.error = _error_word(index)
+    need = L.load().gdnx_paged_attn_workspace_bytes(C.byref(a))
+    ws = None
+    if need:
+        ws = q.new_empty(need, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    _enqueue("gdnx_paged_attn", index, C.byref(a))
+    return (y, lse) if return_lse else y
+
+
 def cache_bounds(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor, *, layer: int = 0) -> None:
     """Brings ``cache.bounds`` up to date in ``layer`` after the last ``counts[i]`` tokens of slots ``rows`` were written
     (int32 vectors, each slot once): for every page on which one of them lies, the least and the greatest value of each

@@ -586,6 +586,35 @@ typedef struct {
 GDNX_API size_t gdnx_paged_decode_workspace_bytes(const gdnx_paged_decode_args* args);
 GDNX_API gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* args, void* stream);
 
+/* Attention of a step's packed new tokens (of chunks of prompts, proposals, single tokens, mixed) over the cache that
+ * holds them and what came before: row starts[i] + t of q stands at position p = first[i] + t of slot rows[i] (keys and
+ * values written before the call) and sees the slot's token j <= p where p - j < window or j < sinks; tokens on released
+ * pages are not seen.  Rows in no sequence (behind starts[n], or of a sequence that is no slot's or ends beyond the
+ * table) give 0, their lse is -inf; so does a row that sees nothing.  A row that sees a score of NaN or +inf, or only
+ * -inf, is NaN.  Scores, softmax statistics and sums are fp32; 16-bit caches run on the tensor cores.
+ * The work is split over CTAs by the lengths that it finds, and the parts joined in a fixed order. */
+typedef struct {
+  gdnx_cache cache;
+  int64_t n, tokens, H, layer; /* tokens at most 2^20 */
+  int64_t window, sinks;       /* window >= 1 */
+  int64_t max_len;             /* no sequence ends beyond it: sizes the split; 0 = width * page */
+  float scale;
+  gdnx_view q;                 /* [tokens,H,D] (st, sh), the cache's type */
+  const int32_t* rows;         /* [n] device, as gdnx_step leaves them */
+  const int32_t* starts;       /* [n + 1] */
+  const int32_t* first;        /* [n] */
+  void* y;                     /* [tokens,H,D] */
+  int32_t y_dtype;
+  int64_t y_st, y_sh;
+  float* lse;                  /* [tokens,H] log of the sum of exponentials; NULL = not kept */
+  int32_t* error;              /* device word that takes GDNX_ETIMEOUT; NULL = none */
+  void* workspace;             /* 16-byte aligned */
+  size_t workspace_bytes;
+} gdnx_paged_attn_args;
+
+GDNX_API size_t gdnx_paged_attn_workspace_bytes(const gdnx_paged_attn_args* args);
+GDNX_API gdnx_status gdnx_paged_attn(const gdnx_paged_attn_args* args, void* stream);
+
 GDNX_API const char* gdnx_status_string(gdnx_status s);
 
 /* Library build identification (for load checks). */

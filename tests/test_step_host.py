@@ -12,7 +12,8 @@ from gdnx_b200 import ops
 from oracle import attention as A
 
 ROOT = Path(__file__).resolve().parents[1]
-STRUCTS = {"gdnx_step": L.Step, "gdnx_paged_select_args": L.PagedSelectArgs, "gdnx_paged_decode_args": L.PagedDecodeArgs}
+STRUCTS = {"gdnx_step": L.Step, "gdnx_paged_select_args": L.PagedSelectArgs, "gdnx_paged_decode_args": L.PagedDecodeArgs,
+           "gdnx_paged_attn_args": L.PagedAttnArgs}
 
 
 def test_ctypes_layout_matches_c(tmp_path):
@@ -33,7 +34,8 @@ def test_ctypes_layout_matches_c(tmp_path):
 
 def test_null_arguments_are_refused():
     lib = L.load()
-    assert lib.gdnx_paged_select(None, None) == L.GDNX_EINVAL
+    assert lib.gdnx_paged_select(None, None) == L.GDNX_EINVAL and lib.gdnx_paged_attn(None, None) == L.GDNX_EINVAL
+    assert lib.gdnx_paged_attn_workspace_bytes(None) == 0
     assert lib.gdnx_paged_select_workspace_bytes(None) == 0
     assert lib.gdnx_cache_step(None, 0, None, None, None, None, 0, None) == L.GDNX_EINVAL
     assert lib.gdnx_cache_append(None, 0, 0, None, None, None, None) == L.GDNX_EINVAL
@@ -47,7 +49,8 @@ def test_cpu_tensors_and_absent_bounds_are_refused():
     x = torch.zeros(2, 4, 64)
     step = ops.PagedStep(c.lengths, c.lengths, c.lengths, c.lengths, c.lengths, torch.zeros(2, dtype=torch.int64))
     for call in (lambda: ops.cache_step(c, c.lengths, c.lengths, 2), lambda: ops.cache_append(c, x, x, step),
-                 lambda: ops.cache_bounds(c, c.lengths, c.lengths), lambda: ops.paged_select(x, c, 2)):
+                 lambda: ops.cache_bounds(c, c.lengths, c.lengths), lambda: ops.paged_select(x, c, 2),
+                 lambda: ops.paged_attention(x, c, step)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
 
