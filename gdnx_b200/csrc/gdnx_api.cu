@@ -415,7 +415,8 @@ static gdnx_paged_attn_args clamp_paged(const gdnx_paged_attn_args& a) {
 
 size_t gdnx_paged_attn_workspace_bytes(const gdnx_paged_attn_args* a) {
   if (!a || check_paged_attn(*a) != GDNX_OK || a->tokens == 0) return 0;
-  return gdnx::paged_attn_simt_workspace_bytes(clamp_paged(*a));
+  const gdnx_paged_attn_args c = clamp_paged(*a);
+  return c.cache.dtype == GDNX_F32 ? gdnx::paged_attn_simt_workspace_bytes(c) : gdnx::paged_attn_tc_workspace_bytes(c);
 }
 
 gdnx_status gdnx_paged_attn(const gdnx_paged_attn_args* a, void* stream) {
@@ -428,7 +429,9 @@ gdnx_status gdnx_paged_attn(const gdnx_paged_attn_args* a, void* stream) {
   if ((a->lse && !device_ptr(a->lse, sizeof(float))) || (a->error && !words(a->error))) return GDNX_EINVAL;
   const size_t need = gdnx_paged_attn_workspace_bytes(a);
   if (need && (a->workspace_bytes < need || !device_ptr(a->workspace, 16))) return GDNX_EWORKSPACE;
-  return gdnx::launch_paged_attn_simt(clamp_paged(*a), (cudaStream_t)stream);
+  const gdnx_paged_attn_args c = clamp_paged(*a);
+  return c.cache.dtype == GDNX_F32 ? gdnx::launch_paged_attn_simt(c, (cudaStream_t)stream)
+                                   : gdnx::launch_paged_attn_tc(c, (cudaStream_t)stream);
 }
 
 const char* gdnx_status_string(gdnx_status s) {

@@ -52,6 +52,9 @@ gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t
 // Attention of packed new tokens over a paged cache (paged_attn.cu).
 size_t paged_attn_simt_workspace_bytes(const gdnx_paged_attn_args& a);
 gdnx_status launch_paged_attn_simt(const gdnx_paged_attn_args& a, cudaStream_t st);
+// 16-bit caches, on the tensor cores (paged_attn_tc.cu).
+size_t paged_attn_tc_workspace_bytes(const gdnx_paged_attn_args& a);
+gdnx_status launch_paged_attn_tc(const gdnx_paged_attn_args& a, cudaStream_t st);
 // Backward of the dense scan (scan_backward.cu).
 bool scan_bwd_supported(const gdnx_scan_bwd_args& a);
 size_t scan_bwd_workspace_bytes(const gdnx_scan_bwd_args& a);

@@ -1,4 +1,5 @@
-// Attention of a chunk of new tokens over a paged cache, on the CUDA cores (all arithmetic fp32).
+// Attention of a chunk of new tokens over a paged cache of 32-bit values, on the CUDA cores
+// (all arithmetic fp32).
 //
 // Blocks of 32 rows (tokens times the heads of a group, paged_attn.cuh) walk key tiles of 64 as windowed attention's
 // forward does (attn_simt.cuh):  s = scale log2(e) q.k;  m' = max(m, max_j s);  p = 2^(s - m');
@@ -19,35 +20,24 @@ struct Ids {
 };
 
 // Tokens j0.. of keys or values (side) into dst [BT][DP + 4].
-template <int DP, typename T>
+template <int DP>
 GDNX_DEV void load_paged(float* dst, const gdnx_cache& c, int64_t layer, int side, int hk, const int* ids, int j0, int len) {
   const int D = (int)c.D;
-  const T* base = static_cast<const T*>(c.kv) + (layer * 2 + side) * c.pages * c.Hk * c.page * D;
-  constexpr int V = 16 / sizeof(T);  // values of a copy
+  const float* base = static_cast<const float*>(c.kv) + (layer * 2 + side) * c.pages * c.Hk * c.page * D;
 #pragma unroll
-  for (int k = 0; k < (BT * DP / V + NT - 1) / NT; ++k) {
-    const int i = k * NT + threadIdx.x, r = i / (DP / V), d = i % (DP / V) * V;
-    if (BT * DP / V % NT && r >= BT) break;
+  for (int k = 0; k < BT * DP / 4 / NT; ++k) {
+    const int i = k * NT + threadIdx.x, r = i / (DP / 4), d = i % (DP / 4) * 4;
     const int id = ids[r / 16];
     const bool on = id >= 0 && j0 + r < len && d < D;
-    const T* src = on ? base + (((int64_t)id * c.Hk + hk) * c.page + (j0 + r) % c.page) * D + d : base;
-    float* to = dst + r * (DP + 4) + d;
-    if constexpr (sizeof(T) == 4) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                       static_cast<uint32_t>(__cvta_generic_to_shared(to))),
-                   "l"(src), "r"(on ? 16 : 0)
-                   : "memory");
-    } else {
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (on) u = *reinterpret_cast<const uint4*>(src);
-      const T* x = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int e = 0; e < V; ++e) to[e] = to_f32(x[e]);
-    }
+    const float* src = on ? base + (((int64_t)id * c.Hk + hk) * c.page + (j0 + r) % c.page) * D + d : base;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(dst + r * (DP + 4) + d))),
+                 "l"(src), "r"(on ? 16 : 0)
+                 : "memory");
   }
 }
 
-template <int DP, typename T>
+template <int DP>
 __global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParams P) {
   extern __shared__ float sm[];
   __shared__ Share share;
@@ -76,7 +66,7 @@ __global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParam
       const int r = i / DP, d = i % DP, t = t0 + r / P.gs, g = r % P.gs;
       float v = 0.f;
       if (r / P.gs < P.tb && g < heads && t < x.s.count && d < D)
-        v = ld_as_f32(a.q.ptr, a.q.dtype, (int64_t)(x.s.start + t) * a.q.st + (int64_t)(h0 + g) * a.q.sh + d);
+        v = static_cast<const float*>(a.q.ptr)[(int64_t)(x.s.start + t) * a.q.st + (int64_t)(h0 + g) * a.q.sh + d];
       Q[r * (DP + 4) + d] = v;
     }
     int p[4];  // positions of this thread's rows, -1: no query
@@ -107,7 +97,7 @@ __global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParam
         ids.id[threadIdx.x] = id >= 0 && id < c.pages ? id : -1;
       }
       __syncthreads();
-      load_paged<DP, T>(KV, c, a.layer, 0, x.hk(), ids.id, j0, len);
+      load_paged<DP>(KV, c, a.layer, 0, x.hk(), ids.id, j0, len);
       wait_tiles();
       __syncthreads();
       for_groups(gr.n, [&](auto nc) {
@@ -142,7 +132,7 @@ __global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParam
         }
       });
       __syncthreads();
-      load_paged<DP, T>(KV, c, a.layer, 1, x.hk(), ids.id, j0, len);
+      load_paged<DP>(KV, c, a.layer, 1, x.hk(), ids.id, j0, len);
       wait_tiles();
       __syncthreads();
       acc_tile<DP>(o, w, KV, tx, gr);
@@ -176,21 +166,15 @@ __global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParam
   }
 }
 
-template <int DP, typename T>
+template <int DP>
 gdnx_status run(const ChunkParams& P, cudaStream_t st) {
   constexpr int smem = ((BR + BT) * (DP + 4) + BR * LDP) * (int)sizeof(float);
   static std::atomic<uint64_t> done;
-  if (!allow_smem(paged_attn_simt_kernel<DP, T>, smem, done)) return GDNX_ELAUNCH;
-  if (launch_early(paged_attn_simt_kernel<DP, T>, dim3((unsigned)P.grid), dim3(NT), smem, st, P) != cudaSuccess)
+  if (!allow_smem(paged_attn_simt_kernel<DP>, smem, done)) return GDNX_ELAUNCH;
+  if (launch_early(paged_attn_simt_kernel<DP>, dim3((unsigned)P.grid), dim3(NT), smem, st, P) != cudaSuccess)
     return GDNX_ELAUNCH;
   return join_chunks<Simt>(P, st);
 }
-template <typename T>
-gdnx_status run_of(const ChunkParams& P, cudaStream_t st) {
-  const int64_t D = P.a.cache.D;
-  return D > 96 ? run<128, T>(P, st) : D > 64 ? run<96, T>(P, st) : run<64, T>(P, st);
-}
-
 ChunkParams plan(const gdnx_paged_attn_args& a) { return plan_chunks<Simt>(a, sm_count() * 3); }
 
 }  // namespace
@@ -199,11 +183,7 @@ size_t paged_attn_simt_workspace_bytes(const gdnx_paged_attn_args& a) { return c
 
 gdnx_status launch_paged_attn_simt(const gdnx_paged_attn_args& a, cudaStream_t st) {
   const ChunkParams P = plan(a);
-  switch (a.cache.dtype) {
-    case GDNX_BF16: return run_of<__nv_bfloat16>(P, st);
-    case GDNX_F16: return run_of<__half>(P, st);
-    default: return run_of<float>(P, st);
-  }
+  return a.cache.D > 96 ? run<128>(P, st) : a.cache.D > 64 ? run<96>(P, st) : run<64>(P, st);
 }
 
 }  // namespace gdnx

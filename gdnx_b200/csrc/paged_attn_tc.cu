@@ -1,0 +1,665 @@
+// Attention of a chunk of new tokens over a paged cache, on the tensor cores (16-bit caches).
+//
+// A persistent CTA walks its share of units (paged_attn.cuh): one or two blocks of 128 rows, a row being one query head
+// of one token.  Two stages, each a warpgroup with one row a thread, take turns with the tensor cores:
+//   S_s = Q_s K^T (tcgen05, fp32 in tensor memory) -> registers:  m = max, p = 2^(c (s - m)), l += p ->
+//   P_s packed 16-bit over S_s's columns -> O_s += P_s V (tcgen05, P from tensor memory, V read with its rows as K).
+// A unit of two blocks gives each stage one, and each tile of 128 keys serves both.  A unit of one block gives its
+// tiles to the two stages in turn, whose outputs stage 0 joins at the end.  The maximum is lazy and the weights are
+// rounded as in windowed attention's forward (attn_fwd.cu).
+//
+// Keys and values come by TMA, a box for each page and 64 dims.  Pages that are not there are not fetched; rows of V
+// that no query may see (those, and rows behind the last token, which may hold NaN) are cleared by the loading warp.
+// Warps 0-3 and 4-7 are the stages' rows, warp 8 issues the products, warp 9 the loads, 10 and 11 clear padding rows
+// of the output.
+#include "paged_attn.cuh"
+
+namespace gdnx {
+namespace {
+
+using Tc = Shape<128, TM, true>;
+
+constexpr int NTHREADS = 384;
+constexpr uint32_t T_S = 0, T_O = 256;  // tensor-memory columns: S_0, S_1, then O_0, O_1
+
+struct TcParams : ChunkParams {
+  CUtensorMap kv;  // {D, Hk * page, L * 2 * pages}
+  CUtensorMap q;   // {D, H, tokens}, box {64, gs, tb}
+  int tma_q;       // q's layout is one that TMA can address, and heads come in whole groups
+  int vec_q, vec_y;  // rows are 16-byte aligned
+};
+
+struct Bars {
+  uint64_t kv_full[8], kv_empty[8], q_full[2], q_empty[2], s_full[2], p_ready[2][2], o_full[2], fix, done, left, joined;
+};
+
+struct Small {
+  Bars bar;
+  Share share;
+  long long sums[NTHREADS / 32];
+  float2 stat[128];  // stage 1's maxima and sums
+  uint32_t tmem_at;
+  int abort_flag;
+};
+
+template <int DB>
+struct Layout {
+  static constexpr int SLOTS = DB == 2 ? 4 : 8;  // K and V tiles in flight
+  static constexpr uint32_t TILE = DB * BLOCK_BYTES;
+  // Q of both stages, the ring, and for each row warp 32 rows x 64 values on their way out
+  static constexpr uint32_t Q = 0, KV = 2 * TILE, OUT = KV + SLOTS * TILE, SMALL = OUT + 8 * 4096;
+  static constexpr size_t SMEM = SMALL + sizeof(Small);  // no static shared memory: the base is 1024-aligned
+};
+
+GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(mbar)
+      : "memory");
+}
+
+// A segment's n tiles in the ring, counted from its first place.  Two blocks: K0 V0 K1 V1 ...  One block: two tiles at
+// a time, K0 K1 V0 V1 K2 K3 ...; a last odd one K V.
+GDNX_DEV int k_place(bool pair, int i) { return pair ? 2 * i : i / 2 * 4 + i % 2; }
+GDNX_DEV int v_place(bool pair, int i, int n) {
+  return pair || (i == n - 1 && n % 2) ? 2 * i + 1 : i / 2 * 4 + 2 + i % 2;
+}
+
+// What a segment asks of its stages.
+struct Seg {
+  int n;        // tiles
+  bool pair;    // each stage has its own block
+  int lo1, hi0, hi1, nst;  // block 1's first window tile, the blocks' last tiles, and how many tiles hold sinks
+  int last0, last1;        // the last tile of each stage, counted from the segment's first; -1: none
+  GDNX_DEV Seg(const ChunkParams& P, const Walk<Tc>& w) {
+    n = w.tb - w.ta;
+    pair = w.x.blocks == 2;
+    nst = (int)((P.a.sinks + TM - 1) / TM);
+    if (!pair) {
+      last0 = (n - 1) & ~1;
+      last1 = n > 1 ? ((n - 2) | 1) : -1;
+      lo1 = hi0 = hi1 = 0;
+      return;
+    }
+    const int p = w.s.first + w.x.t0 + P.tb;  // block 1's first position
+    lo1 = max(0, p - (int)P.a.window + 1) / TM;
+    hi0 = (p - 1) / TM;
+    hi1 = (w.s.first + min(w.x.t0 + 2 * P.tb, w.s.count) - 1) / TM;
+    const KeyTiles& k = w.x.kt;
+    last0 = min(w.tb - 1, k.nsink + hi0 - k.lo) - w.ta;  // block 0 has every tile up to its last
+    if (last0 < 0) last0 = -1;
+    int e = w.tb - 1;  // block 1: but those between the sinks and its window
+    if (e >= k.nsink && k.tile(e) < lo1 && k.tile(e) >= nst) e = nst - 1 >= k.lo ? k.nsink + nst - 1 - k.lo : k.nsink - 1;
+    last1 = e < w.ta ? -1 : e - w.ta;
+  }
+  GDNX_DEV int last(int st) const { return st ? last1 : last0; }
+  // Does stage st work on the segment's i-th tile, number kt?
+  GDNX_DEV bool on(int st, int i, int kt) const {
+    if (!pair) return (i & 1) == st;
+    return st ? kt <= hi1 && (kt >= lo1 || kt < nst) : kt <= hi0;
+  }
+};
+
+// Weights of N columns: p = 2^(c2 s - mc), summed, packed 16-bit.  One pair in eight is taken on the FMA pipes (where
+// masked scores give 2^-125: nothing beside a weight that counts).
+template <bool BF16, int N>
+GDNX_DEV void weights(const float* s, float c2, float mc, float2& sum, uint32_t* pk) {
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e) {
+    const float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), make_float2(c2, c2), make_float2(-mc, -mc));
+    const float2 p = e % 8 == 3 ? ex2_poly<false>(x) : make_float2(ex2(x.x), ex2(x.y));
+    sum = add2(sum, p);
+    pk[e] = pack2<BF16>(p.x, p.y);
+  }
+}
+
+// A row's running state: the maximum that O and l are scaled to, the sum, and whether it saw a key.
+struct Row {
+  float m, l;
+  bool any;
+};
+
+// Takes a tile's maximum into the row, rescaling O where it lies too far above the old one.
+// Returns what the tile's scores (times c2) are taken against.  A score that is NaN or +inf is the tile's maximum
+// whatever its column, and from then on l and O or the maximum itself say so (ex2_poly alone would not).
+template <int DB>
+GDNX_DEV float take_max(Row& w, float top, float c2, uint32_t tO) {
+  const bool grow = w.m != -INFINITY && !((top - w.m) * c2 <= 8.f);
+  if (__any_sync(0xffffffffu, grow)) {
+    const float corr = grow ? ex2((w.m - top) * c2) : 1.f;
+    w.l *= corr;
+    if (grow) w.m = top;
+#pragma unroll 1
+    for (int d = 0; d < 64 * DB; d += 16) {
+      float o[16];
+      tc::tmem_ld16(tO + d, o);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] *= corr;
+      tc::tmem_st16u(tO + d, reinterpret_cast<const uint32_t*>(o));
+    }
+  }
+  if (w.m == -INFINITY) w.m = top;
+  return w.m == -INFINITY ? 0.f : w.m * c2;
+}
+
+// 32 values of a row as 16-bit words.
+GDNX_DEV void pack_row(uint32_t* u, const float* o, int dtype) {
+  if (dtype == GDNX_BF16) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) u[e] = pack2<true>(o[2 * e], o[2 * e + 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) u[e] = pack2<false>(o[2 * e], o[2 * e + 1]);
+  }
+}
+
+// Bits of a word of 32 columns (word q of a tile) on pages that are not there: bit i of `gone` is the tile's i-th page.
+GDNX_DEV uint32_t gone_bits(uint32_t gone, int page, int q) {
+  if (page >= 32) return gone >> (32 * q / page) & 1 ? 0xffffffffu : 0u;
+  return (gone >> (2 * q) & 1 ? 0xffffu : 0u) | (gone >> (2 * q + 1) & 1 ? 0xffff0000u : 0u);
+}
+
+// One stage's rows, one for each thread.
+template <int DB, bool BF16>
+GDNX_DEV void run_rows(const TcParams& P, const Share& share, uint8_t* base, Small& sm, uint32_t tmem) {
+  using Lo = Layout<DB>;
+  const gdnx_paged_attn_args& a = P.a;
+  const gdnx_cache& c = a.cache;
+  Bars& bar = sm.bar;
+  volatile int* abort_flag = &sm.abort_flag;
+  const int r = threadIdx.x % 128, lane = r % 32, warp = threadIdx.x / 32, st = warp / 4;
+  const uint32_t lane_at = (uint32_t)(r / 32 * 32) << 16;
+  const uint32_t tS = tmem + T_S + st * 128 + lane_at, tO = tmem + T_O + st * 128 + lane_at;
+  const int window = (int)a.window, sinks = (int)a.sinks, D = (int)c.D, npp = TM / c.page;
+  const float c2 = a.scale * kLog2e;
+  const int tok = r / P.gs, head = r % P.gs;  // this thread's row
+  uint8_t* out = base + Lo::OUT + warp * 4096;
+  uint32_t nS = 0, nO = 0, nj = 0;
+  if (threadIdx.x == 0 && P.cut) P.joint[blockIdx.x] = {0, 0, 0, 0, -1};
+  Walk<Tc> w(P, share);
+  while (w.next()) {
+    const Seg g(P, w);
+    const int len = w.s.len(), t0 = w.x.t0 + (g.pair && st ? P.tb : 0), t = t0 + tok;
+    const bool valid = tok < P.tb && head < w.heads() && t < w.s.count;
+    const int p = valid ? w.s.first + t : -1;
+    const bool some = __any_sync(0xffffffffu, valid);
+    const int p0 = w.s.first + t0, p1 = w.s.first + min(t0 + P.tb, w.s.count) - 1;  // of the block
+    const int32_t* table = c.table + (int64_t)w.s.row * c.width;
+    Row row = {-INFINITY, 0.f, false};
+    bool worked = false;
+    for (int i = 0; i < g.n; ++i) {
+      const int kt = w.x.kt.tile(w.ta + i), j0 = kt * TM;
+      if (!g.on(st, i, kt)) continue;
+      worked = true;
+      // the tile's pages that are not there
+      int id = 0;
+      if (lane < npp) {
+        const int64_t x = (int64_t)kt * npp + lane;
+        id = x < c.width ? table[x] : -1;
+      }
+      const uint32_t gone = __ballot_sync(0xffffffffu, id < 0 || id >= c.pages);
+      if (!warp_wait(&bar.s_full[st], nS++ & 1, abort_flag)) return;
+      tc::fence_after();
+      if (!some) {  // no row of the warp is a query: what its weights are does not matter
+        pipe::mbar_arrive(&bar.p_ready[st][0]);
+        pipe::mbar_arrive(&bar.p_ready[st][1]);
+        continue;
+      }
+      float2 sum = make_float2(0.f, 0.f);
+      // does every row see the whole tile?
+      if (!gone && j0 + TM - 1 <= p0 && (p1 - j0 < window || j0 + TM <= sinks)) {
+        row.any = true;
+        float s[128], t4[4];
+        tmem_ld128(tS, s);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) t4[f] = s[f];
+#pragma unroll
+        for (int e = 4; e < 128; e += 4)
+#pragma unroll
+          for (int f = 0; f < 4; ++f) t4[f] = max_nan(t4[f], s[e + f]);
+        const float mc = take_max<DB>(row, max_nan(max_nan(t4[0], t4[1]), max_nan(t4[2], t4[3])), c2, tO);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[32];
+          weights<BF16, 64>(s + 64 * half, c2, mc, sum, pk);
+          tmem_st32u(tS + 32 * half, pk);
+          tc::fence_before();
+          pipe::mbar_arrive(&bar.p_ready[st][half]);
+        }
+      } else {
+        // chunk by chunk of 32 columns: what no row of the warp sees costs nothing
+        // visible columns: lo..hi, and those up to sk
+        const int hi = p - j0, lo = p - window + 1 - j0, sk = min(sinks - 1 - j0, hi);
+        uint32_t used = 0;
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t on = (range_bits(lo, hi, q) | range_bits(0, sk, q)) & ~gone_bits(gone, c.page, q);
+          if (!__any_sync(0xffffffffu, on)) continue;
+          used |= 1u << q;
+          row.any |= on != 0;
+          float s[32];
+          tc::tmem_ld32(tS + 32 * q, s);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) top = max_nan(top, on >> e & 1 ? s[e] : -INFINITY);
+        }
+        const float mc = take_max<DB>(row, top, c2, tO);
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          uint32_t pk[16] = {};
+          if (used >> q & 1) {
+            const uint32_t on = (range_bits(lo, hi, q) | range_bits(0, sk, q)) & ~gone_bits(gone, c.page, q);
+            float s[32];
+            tc::tmem_ld32(tS + 32 * q, s);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(on >> e & 1)) s[e] = -INFINITY;
+            weights<BF16, 32>(s, c2, mc, sum, pk);
+          }
+          tc::tmem_st16u(tS + 16 * q, pk);  // over scores that have been read
+          if (q % 2) {
+            tc::fence_before();
+            pipe::mbar_arrive(&bar.p_ready[st][q / 2]);
+          }
+        }
+      }
+      row.l += sum.x + sum.y;
+    }
+    if (worked) {
+      if (!warp_wait(&bar.o_full[st], nO++ & 1, abort_flag)) return;
+      tc::fence_after();
+    }
+    const bool both = !g.pair && g.n > 1;  // both stages worked on the one block
+    if (!g.pair) {
+      if (st == 1) {
+        if (!both) continue;
+        // stage 1 leaves its maximum and sum, and its output until stage 0 has read it
+        sm.stat[r] = make_float2(row.m, row.any ? row.l : -1.f);
+        tc::fence_before();
+        pipe::mbar_arrive(&bar.left);
+        if (!warp_wait(&bar.joined, nj++ & 1, abort_flag)) return;
+        continue;
+      }
+    }
+    float f0 = 1.f, f1 = 0.f;  // the stages' factors
+    if (both) {
+      if (!warp_wait(&bar.left, nj++ & 1, abort_flag)) return;
+      tc::fence_after();
+      const float2 x = sm.stat[r];
+      const bool other = !(x.y < 0.f);  // (NaN: it saw something)
+      // a maximum that is NaN stays one
+      const float m = max_nan(row.m, x.x);
+      f0 = row.m == -INFINITY ? 0.f : ex2((row.m - m) * c2);
+      f1 = x.x == -INFINITY ? 0.f : ex2((x.x - m) * c2);
+      row.m = m;
+      row.l = row.l * f0 + (other ? x.y * f1 : 0.f);
+      row.any |= other;
+    }
+    if (!some && !both) continue;
+    // the maximum in the log2 domain and the sum as the join takes them: a maximum that is not finite comes of scores
+    // that are not, and shows in the sum
+    const float mc = row.m * c2;
+    const bool finite = fabsf(mc) < INFINITY;
+    const float top = !row.any ? -INFINITY : finite ? mc : kNoScore;
+    const float l = !row.any || row.m == -INFINITY ? 0.f : finite ? row.l : NAN;
+    const bool whole = w.whole();
+    const float f = whole ? scale_of(top, l) : 1.f;
+    const int64_t row_at = (int64_t)(w.s.start + t) * a.y_st + (int64_t)(w.head0() + head) * a.y_sh;
+    const int64_t part = w.part() + (g.pair ? st * 128 : 0) + r;
+    const uint32_t live = __ballot_sync(0xffffffffu, valid);
+#pragma unroll 1
+    for (int d = 0; d < 64 * DB; d += 64) {
+      float o[64];
+      if (worked) tmem_ld64(tO + d, o);
+      else
+#pragma unroll
+        for (int e = 0; e < 64; ++e) o[e] = 0.f;
+      if (both) {
+        float x[64];
+        tmem_ld64(tO + 128 + d, x);
+#pragma unroll
+        for (int e = 0; e < 64; ++e) o[e] = o[e] * f0 + x[e] * f1;
+      }
+      if (!whole) {
+        if (valid)
+#pragma unroll
+          for (int e = 0; e < 64; e += 4)
+            if (d + e < D) *reinterpret_cast<float4*>(P.part + part * D + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 64; ++e) o[e] = f == 0.f ? 0.f : o[e] * f;
+      if (a.y_dtype != GDNX_F32 && P.vec_y) {  // through shared memory: four rows' 128 bytes to a store
+        uint32_t u[32];
+        pack_row(u, o, a.y_dtype);
+        pack_row(u + 16, o + 32, a.y_dtype);
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4*>(out + tc::sw128(lane, e, 32)) =
+              make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int from = e * 4 + lane / 8, x = lane % 8;
+          const int64_t at = __shfl_sync(0xffffffffu, row_at, from);
+          if ((live >> from & 1) && d + x * 8 < D)
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + at + d + x * 8) =
+                *reinterpret_cast<const uint4*>(out + tc::sw128(from, x, 32));
+        }
+      } else if (valid) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (d + e < D) st_from_f32(a.y, a.y_dtype, row_at + d + e, o[e]);
+      }
+    }
+    if (valid && whole && a.lse) a.lse[(int64_t)(w.s.start + t) * a.H + w.head0() + head] = lse_of(top, l);
+    if (valid && !whole) {
+      P.stat[part * 2] = top;
+      P.stat[part * 2 + 1] = l;
+    }
+    if (both) {  // stage 1's output may be written again
+      tc::fence_before();
+      pipe::mbar_arrive(&bar.joined);
+    }
+    if (threadIdx.x == 0 && w.ends_cut()) P.joint[blockIdx.x] = w.joint(share.per);
+  }
+}
+
+// The warp that issues the products: for each step and stage PV of the step before, once its weights are there, and S of
+// this one, in one run.  In order, S of a step complete means PV of the one before complete.
+template <int DB, bool BF16>
+GDNX_DEV void run_products(const TcParams& P, const Share& share, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+  using Lo = Layout<DB>;
+  constexpr uint32_t ID_S = idesc16(BF16, 128, 128, false, false), ID_O = idesc16(BF16, 128, 64 * DB, false, true);
+  uint32_t cnt = 0, nP[2] = {0, 0}, nQ[2] = {0, 0};
+  Walk<Tc> w(P, share);
+  while (w.next()) {
+    const Seg g(P, w);
+    const int steps = g.pair ? g.n : (g.n + 1) / 2;
+    // a block's tiles go to both stages: one Q serves them
+    bool begun[2] = {false, false}, pend[2] = {false, false}, acc[2] = {false, false};
+    int was[2] = {0, 0};  // the stage's tile of the step before
+    for (int s = 0; s <= steps; ++s) {
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const uint32_t tS = tmem + T_S + st * 128, tO = tmem + T_O + st * 128;
+        const int i = g.pair ? s : 2 * s + st;
+        const bool there = i < g.n, on = there && g.on(st, i, w.x.kt.tile(w.ta + i));
+        const uint32_t kp = cnt + k_place(g.pair, i), ksl = kp % Lo::SLOTS;
+        const uint32_t vp = cnt + v_place(g.pair, was[st], g.n), vsl = vp % Lo::SLOTS;
+        if (on) {
+          if (!begun[st] && (g.pair || st == 0) && !warp_wait(&bar.q_full[st], nQ[st]++ & 1, abort_flag)) return;
+          if (!warp_wait(&bar.kv_full[ksl], kp / Lo::SLOTS & 1, abort_flag)) return;
+        }
+        if (pend[st]) {  // the first half's weights, then the second's
+          const uint32_t v = smem + Lo::KV + vsl * Lo::TILE;
+          if (!warp_wait(&bar.kv_full[vsl], vp / Lo::SLOTS & 1, abort_flag)) return;
+          if (!warp_wait(&bar.p_ready[st][0], nP[st] & 1, abort_flag)) return;
+          tc::fence_after();
+          if (elect_one()) mma_px<4>(tO, tS, v, ID_O, acc[st]);
+          __syncwarp();
+          if (!warp_wait(&bar.p_ready[st][1], nP[st]++ & 1, abort_flag)) return;
+        }
+        tc::fence_after();
+        if (elect_one()) {
+          if (pend[st]) {
+            mma_px<4>(tO, tS + 32, smem + Lo::KV + vsl * Lo::TILE + 64 * 128, ID_O, true);
+            if (was[st] == g.last(st)) tc::commit(&bar.o_full[st]);
+          }
+          // V of the step before is done with: by both stages, or by the one whose it is
+          if (s > 0 && g.pair && st == 1) tc::commit(&bar.kv_empty[(cnt + v_place(true, s - 1, g.n)) % Lo::SLOTS]);
+          if (pend[st] && !g.pair) tc::commit(&bar.kv_empty[vsl]);
+          if (on) {
+            mma_abt<DB>(tS, smem + Lo::Q + (g.pair ? st : 0) * Lo::TILE, smem + Lo::KV + ksl * Lo::TILE, ID_S);
+            tc::commit(&bar.s_full[st]);
+            // the last product that reads a Q
+            if (i == (g.pair ? g.last(st) : g.n - 1)) tc::commit(&bar.q_empty[g.pair ? st : 0]);
+          }
+          if (there && (g.pair ? st == 1 : true)) tc::commit(&bar.kv_empty[ksl]);
+        }
+        __syncwarp();
+        acc[st] = acc[st] || pend[st];
+        begun[st] = begun[st] || on;
+        // (a stage's gap between the sinks' tile and its window ends nothing)
+        pend[st] = on;
+        if (on) was[st] = i;
+      }
+    }
+    cnt += 2 * g.n;
+  }
+}
+
+// Page ids of tile kt's pages for the lanes below npp, -1 where there is none.
+GDNX_DEV int page_of(const ChunkParams& P, const Chunk& s, int kt, int i) {
+  const gdnx_cache& c = P.a.cache;
+  const int64_t x = (int64_t)kt * (TM / c.page) + i;
+  if (x >= c.width || x * c.page >= s.len()) return -1;
+  const int p = c.table[(int64_t)s.row * c.width + x];
+  return p >= 0 && p < c.pages ? p : -1;
+}
+
+// The warp that loads: a segment's first K, its Q, then the tiles in their places' order.
+template <int DB>
+GDNX_DEV void run_loads(const TcParams& P, const Share& share, uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag,
+                        uint32_t& issued) {
+  using Lo = Layout<DB>;
+  const gdnx_cache& c = P.a.cache;
+  const int lane = threadIdx.x % 32, page = c.page, npp = TM / page, ahead = 32 / npp;
+  const uint32_t box = (uint32_t)page * 128;
+  uint32_t cnt = 0, nQ[2] = {0, 0}, nfix = 0;
+  Walk<Tc> w(P, share);
+  while (w.next()) {
+    const Seg g(P, w);
+    const int hk = w.hk();
+    int ids = -1, from = -1;  // page ids of tiles from .. from + ahead - 1
+    for (int x = 0; x < 2 * g.n; ++x) {
+      // the tile and side at place x
+      int i, side;
+      if (g.pair || (g.n % 2 && x >= 2 * g.n - 2)) {
+        i = x / 2;
+        side = x % 2;
+      } else {
+        i = x / 4 * 2 + x % 2;
+        side = x % 4 / 2;
+      }
+      // (a step's two tiles lie in one reading of ids: their count is even, or one)
+      const int group = (i / ahead) * ahead;
+      if (group != from) {
+        from = group;
+        const int mine = from + lane / npp;
+        ids = mine < g.n ? page_of(P, w.s, w.x.kt.tile(w.ta + mine), lane % npp) : -1;
+      }
+      const int j0 = w.x.kt.tile(w.ta + i) * TM, pg = lane / DB, d = lane % DB;
+      const int id = __shfl_sync(0xffffffffu, ids, ((i - from) * npp + pg) & 31);
+      const bool go = pg < npp && id >= 0;
+      const uint32_t got = __ballot_sync(0xffffffffu, go);
+      const uint32_t place = cnt + x, sl = place % Lo::SLOTS, dst = smem + Lo::KV + sl * Lo::TILE;
+      if (!warp_wait(&bar.kv_empty[sl], (place / Lo::SLOTS & 1) ^ 1, abort_flag)) return;
+      const bool fix = side == 1 && (__popc(got) < npp * DB || j0 + TM > w.s.len());
+      uint64_t* full = fix ? &bar.fix : &bar.kv_full[sl];
+      const uint32_t mb = tc::smem_u32(full);
+      if (lane == 0) pipe::expect_tx(mb, __popc(got) * box);
+      __syncwarp();
+      if (go)
+        tma_load_3d(dst + d * BLOCK_BYTES + pg * box, &P.kv, d * 64, hk * page, (int)((P.a.layer * 2 + side) * c.pages + id), mb);
+      issued = place + 1;
+      if (fix) {  // rows that no query may see meet weights of 0, so they must not hold NaN
+        if (!warp_wait(&bar.fix, nfix++ & 1, abort_flag)) return;
+        const int end = w.s.len() - j0;  // rows from here on are behind the last token
+        for (int y = lane; y < TM * DB * 8; y += 32) {
+          const int row = y / (DB * 8), e = y % (DB * 8);
+          if (row < end && (got >> (row / page * DB) & 1)) continue;
+          *reinterpret_cast<uint4*>(base + Lo::KV + sl * Lo::TILE + (e / 8) * BLOCK_BYTES + row * 128 + e % 8 * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        tc::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) pipe::mbar_arrive(&bar.kv_full[sl]);
+      }
+      if (x == 0) {
+        const gdnx_view& q = P.a.q;
+        for (int b = 0; b < (g.pair ? 2 : 1); ++b) {
+          if (g.last(b) < 0) continue;
+          if (!warp_wait(&bar.q_empty[b], (nQ[b]++ & 1) ^ 1, abort_flag)) return;
+          const uint32_t at = smem + Lo::Q + b * Lo::TILE, qb = tc::smem_u32(&bar.q_full[b]);
+          const int t0 = w.x.t0 + b * P.tb, row0 = w.s.start + t0;
+          if (P.tma_q) {
+            if (lane == 0) {
+              pipe::expect_tx(qb, DB * (uint32_t)(P.gs * P.tb) * 128);
+#pragma unroll
+              for (int e = 0; e < DB; ++e) tma_load_3d(at + e * BLOCK_BYTES, &P.q, e * 64, w.head0(), row0, qb);
+            }
+            __syncwarp();
+          } else {
+            const int heads = w.heads(), n = min(P.tb, w.s.count - t0), D = (int)c.D;
+            for (int y = lane; y < 128 * DB * 8; y += 32) {
+              const int row = y / (DB * 8), e = y % (DB * 8), t = row / P.gs, h = row % P.gs;
+              uint4 u = make_uint4(0, 0, 0, 0);
+              if (t < n && h < heads && e * 8 < D) {
+                const uint16_t* src = static_cast<const uint16_t*>(q.ptr) + (int64_t)(row0 + t) * q.st + (w.head0() + h) * q.sh + e * 8;
+                if (P.vec_q) {
+                  u = *reinterpret_cast<const uint4*>(src);
+                } else {
+                  u.x = src[0] | (uint32_t)src[1] << 16;
+                  u.y = src[2] | (uint32_t)src[3] << 16;
+                  u.z = src[4] | (uint32_t)src[5] << 16;
+                  u.w = src[6] | (uint32_t)src[7] << 16;
+                }
+              }
+              *reinterpret_cast<uint4*>(base + Lo::Q + b * Lo::TILE + tc::sw128(row, e, 128)) = u;
+            }
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) pipe::mbar_arrive(&bar.q_full[b]);
+          }
+        }
+      }
+    }
+    cnt += 2 * g.n;
+  }
+}
+
+template <int DB, bool BF16>
+__global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid_constant__ TcParams P) {
+  using Lo = Layout<DB>;
+  extern __shared__ __align__(1024) uint8_t base[];
+  Small& sm = *reinterpret_cast<Small*>(base + Lo::SMALL);
+  Bars& bar = sm.bar;
+  volatile int* abort_flag = &sm.abort_flag;
+  const uint32_t smem = uniform(tc::smem_u32(base));
+  const int warp = uniform(threadIdx.x / 32);
+  dependents_may_start();
+  if (threadIdx.x == 0) {
+    *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
+    for (int i = 0; i < 8; ++i) {
+      tc::mbar_init(&bar.kv_full[i], 1);
+      tc::mbar_init(&bar.kv_empty[i], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      tc::mbar_init(&bar.q_full[s], 1);
+      tc::mbar_init(&bar.q_empty[s], 1);
+      tc::mbar_init(&bar.s_full[s], 1);
+      tc::mbar_init(&bar.p_ready[s][0], 128);
+      tc::mbar_init(&bar.p_ready[s][1], 128);
+      tc::mbar_init(&bar.o_full[s], 1);
+    }
+    tc::mbar_init(&bar.fix, 1);
+    tc::mbar_init(&bar.done, 1);
+    tc::mbar_init(&bar.left, 128);
+    tc::mbar_init(&bar.joined, 128);
+  }
+  if (warp == 8) tc::tmem_alloc(&sm.tmem_at, 512);
+  // rows of Q that no load writes stay zero
+  for (uint32_t i = threadIdx.x; i < 2 * Lo::TILE / 16; i += NTHREADS)
+    *reinterpret_cast<uint4*>(base + Lo::Q + i * 16) = make_uint4(0, 0, 0, 0);
+  tc::fence_async_smem();
+  tc::fence_before();
+  wait_for_earlier();
+  find_share<Tc, NTHREADS>(P, sm.share, sm.sums);  // synchronises
+  tc::fence_after();
+  const uint32_t tmem = uniform(sm.tmem_at);
+  if (smem % 1024) {  // never entered: the base is aligned
+  } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 224 + 128 x 56 is just that
+    regs_up<224>();
+    run_rows<DB, BF16>(P, sm.share, base, sm, tmem);
+  } else {
+    regs_down<56>();
+    if (warp == 8) {
+      run_products<DB, BF16>(P, sm.share, smem, tmem, bar, abort_flag);
+      __syncwarp();
+      if (elect_one()) tc::commit(&bar.done);  // every product issued has ended before tensor memory is freed
+      tc::mbar_wait(&bar.done, 0);
+    } else if (warp == 9) {
+      uint32_t issued = 0;
+      run_loads<DB>(P, sm.share, base, smem, bar, abort_flag, issued);
+      if (*abort_flag && threadIdx.x % 32 == 0) {  // let the copies in flight land
+        for (uint32_t c = issued > Lo::SLOTS ? issued - Lo::SLOTS : 0; c < issued; ++c)
+          tc::mbar_wait(&bar.kv_full[c % Lo::SLOTS], c / Lo::SLOTS & 1, 1u << 16);
+        for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
+      }
+    } else {
+      write_padding(P, threadIdx.x - 320, 64);
+    }
+  }
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 8) tc::tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
+}
+
+template <int DB, bool BF16>
+gdnx_status launch(const TcParams& P, cudaStream_t st) {
+  const auto kernel = paged_attn_tc_kernel<DB, BF16>;
+  constexpr int smem = (int)Layout<DB>::SMEM;
+  static std::atomic<uint64_t> done;
+  if (!allow_smem(kernel, smem, done)) return GDNX_ELAUNCH;
+  if (launch_early(kernel, dim3((unsigned)P.grid), dim3(NTHREADS), smem, st, P) != cudaSuccess) return GDNX_ELAUNCH;
+  return join_chunks<Tc>(P, st);
+}
+
+ChunkParams plan(const gdnx_paged_attn_args& a) { return plan_chunks<Tc>(a, sm_count()); }
+
+}  // namespace
+
+size_t paged_attn_tc_workspace_bytes(const gdnx_paged_attn_args& a) { return chunk_bytes(plan(a)); }
+
+gdnx_status launch_paged_attn_tc(const gdnx_paged_attn_args& a, cudaStream_t st) {
+  const gdnx_cache& c = a.cache;
+  const EncodeTiledFn enc = encode_fn();
+  if (!enc) return GDNX_ELAUNCH;
+  if (c.L * 2 * c.pages > ((int64_t)1 << 31) - 1 || c.Hk * c.page * c.D * 2 >= ((int64_t)1 << 40)) return GDNX_EUNSUPPORTED;
+  TcParams P;
+  static_cast<ChunkParams&>(P) = plan(a);
+  const CUtensorMapDataType type = c.dtype == GDNX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cuuint32_t es[3] = {1, 1, 1};
+  {
+    const cuuint64_t dims[3] = {(cuuint64_t)c.D, (cuuint64_t)(c.Hk * c.page), (cuuint64_t)(c.L * 2 * c.pages)};
+    const cuuint64_t strides[2] = {(cuuint64_t)c.D * 2, (cuuint64_t)(c.Hk * c.page * c.D) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)c.page, 1};
+    if (enc(&P.kv, type, 3, c.kv, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return GDNX_EINVAL;
+  }
+  P.vec_q = reinterpret_cast<uintptr_t>(a.q.ptr) % 16 == 0 && a.q.st % 8 == 0 && a.q.sh % 8 == 0;
+  P.vec_y = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_st % 8 == 0 && a.y_sh % 8 == 0;
+  // TMA takes 16-byte strides below 2^40, none of them 0 where there is more than one; a last group of fewer heads would
+  // read the next key head's
+  P.tma_q = P.vec_q && P.groups == 1 && (a.q.sh > 0 || a.H == 1) && (a.q.st > 0 || a.tokens == 1) &&
+            a.q.st < ((int64_t)1 << 39) && a.q.sh < ((int64_t)1 << 39);
+  if (P.tma_q) {
+    const cuuint64_t one = (cuuint64_t)((c.D + 7) / 8 * 16);
+    const cuuint64_t dims[3] = {(cuuint64_t)c.D, (cuuint64_t)a.H, (cuuint64_t)a.tokens};
+    const cuuint64_t strides[2] = {a.H > 1 ? (cuuint64_t)a.q.sh * 2 : one, a.tokens > 1 ? (cuuint64_t)a.q.st * 2 : one};
+    const cuuint32_t box[3] = {64, (cuuint32_t)P.gs, (cuuint32_t)P.tb};
+    if (enc(&P.q, type, 3, const_cast<void*>(a.q.ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      P.tma_q = 0;
+  }
+  if (c.D > 64) return c.dtype == GDNX_BF16 ? launch<2, true>(P, st) : launch<2, false>(P, st);
+  return c.dtype == GDNX_BF16 ? launch<1, true>(P, st) : launch<1, false>(P, st);
+}
+
+}  // namespace gdnx
