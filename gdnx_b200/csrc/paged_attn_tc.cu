@@ -29,8 +29,10 @@ struct TcParams : ChunkParams {
   int vec_q, vec_y;  // rows are 16-byte aligned
 };
 
+constexpr int MOST_SLOTS = 14;
+
 struct Bars {
-  uint64_t kv_full[8], kv_empty[8], q_full[2], q_empty[2], s_full[2], p_ready[2][2], o_full[2], fix, done, left, joined;
+  uint64_t full[MOST_SLOTS], empty[MOST_SLOTS], s_full[2], p_ready[2][2], o_full[2], fix, done, left, joined;
 };
 
 struct Small {
@@ -42,13 +44,48 @@ struct Small {
   int abort_flag;
 };
 
+// Shared memory is slots of one tile.  The first holds the block's Q, the second a second block's; the others, and the
+// second where there is one block, are the ring that K and V go round, from its first slot in every segment.
 template <int DB>
 struct Layout {
-  static constexpr int SLOTS = DB == 2 ? 4 : 8;  // K and V tiles in flight
-  static constexpr uint32_t TILE = DB * BLOCK_BYTES;
-  // Q of both stages, the ring, and for each row warp 32 rows x 64 values on their way out
-  static constexpr uint32_t Q = 0, KV = 2 * TILE, OUT = KV + SLOTS * TILE, SMALL = OUT + 8 * 4096;
+  static constexpr int SLOTS = DB == 2 ? 7 : 14;
+  static constexpr uint32_t TILE = DB * BLOCK_BYTES, SMALL = SLOTS * TILE;
   static constexpr size_t SMEM = SMALL + sizeof(Small);  // no static shared memory: the base is 1024-aligned
+};
+
+// A place of a segment's ring: its slot behind the ring's first, and whether an odd number of rounds lies behind it.
+struct Place {
+  int at;
+  uint32_t odd;
+};
+
+// What a role knows of the slots: a bit for each, the parity of its next use in this segment.
+template <int DB>
+struct Ring {
+  uint32_t bits = 0;
+  int first = 1, size = 1;  // of the segment's ring
+  GDNX_DEV void begin(bool pair) {
+    first = pair ? 2 : 1;
+    size = Layout<DB>::SLOTS - first;
+  }
+  // The place n (at most a round) behind p.
+  GDNX_DEV Place behind(Place p, int n) const {
+    p.at += n;
+    if (p.at >= size) {
+      p.at -= size;
+      p.odd ^= 1;
+    }
+    return p;
+  }
+  GDNX_DEV int slot(Place p) const { return first + p.at; }
+  GDNX_DEV uint32_t parity(Place p) const { return (bits >> (first + p.at) ^ p.odd) & 1; }
+  GDNX_DEV uint32_t q_parity(int b) const { return bits >> b & 1; }
+  // A segment of n places and these Qs is over.
+  GDNX_DEV void end(int n, bool q0, bool q1) {
+    // slots before n % size have had one use more than the others
+    const uint32_t all = ((1u << size) - 1) << first, more = ((1u << n % size) - 1) << first;
+    bits ^= (n / size & 1 ? all : 0) ^ more ^ (q0 ? 1 : 0) ^ (q1 ? 2 : 0);
+  }
 };
 
 GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t mbar) {
@@ -58,12 +95,8 @@ GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, 
       : "memory");
 }
 
-// A segment's n tiles in the ring, counted from its first place.  Two blocks: K0 V0 K1 V1 ...  One block: two tiles at
-// a time, K0 K1 V0 V1 K2 K3 ...; a last odd one K V.
-GDNX_DEV int k_place(bool pair, int i) { return pair ? 2 * i : i / 2 * 4 + i % 2; }
-GDNX_DEV int v_place(bool pair, int i, int n) {
-  return pair || (i == n - 1 && n % 2) ? 2 * i + 1 : i / 2 * 4 + 2 + i % 2;
-}
+// A segment's tiles in the ring.  Two blocks: K0 V0 K1 V1 ...  One block: two tiles at a time, K0 K1 V0 V1 K2 K3 ...; a
+// last odd one K V.
 
 // What a segment asks of its stages.
 struct Seg {
@@ -71,10 +104,14 @@ struct Seg {
   bool pair;    // each stage has its own block
   int lo1, hi0, hi1, nst;  // block 1's first window tile, the blocks' last tiles, and how many tiles hold sinks
   int last0, last1;        // the last tile of each stage, counted from the segment's first; -1: none
+  int from, nsink, lo;     // the unit's tile that the segment begins with; its tiles' numbers (KeyTiles)
   GDNX_DEV Seg(const ChunkParams& P, const Walk<Tc>& w) {
     n = w.tb - w.ta;
     pair = w.x.blocks == 2;
     nst = (int)((P.a.sinks + TM - 1) / TM);
+    from = w.ta;
+    nsink = w.x.kt.nsink;
+    lo = w.x.kt.lo;
     if (!pair) {
       last0 = (n - 1) & ~1;
       last1 = n > 1 ? ((n - 2) | 1) : -1;
@@ -92,6 +129,21 @@ struct Seg {
     if (e >= k.nsink && k.tile(e) < lo1 && k.tile(e) >= nst) e = nst - 1 >= k.lo ? k.nsink + nst - 1 - k.lo : k.nsink - 1;
     last1 = e < w.ta ? -1 : e - w.ta;
   }
+  // The same in a form that the compiler knows to be uniform: what products are issued from.
+  GDNX_DEV void make_uniform() {
+    n = uniform(n);
+    pair = uniform((int)pair);
+    lo1 = uniform(lo1);
+    hi0 = uniform(hi0);
+    hi1 = uniform(hi1);
+    last0 = uniform(last0);
+    last1 = uniform(last1);
+    from = uniform(from);
+    nsink = uniform(nsink);
+    lo = uniform(lo);
+  }
+  // Number of the segment's i-th tile.
+  GDNX_DEV int tile(int i) const { return from + i < nsink ? from + i : lo + from + i - nsink; }
   GDNX_DEV int last(int st) const { return st ? last1 : last0; }
   // Does stage st work on the segment's i-th tile, number kt?
   GDNX_DEV bool on(int st, int i, int kt) const {
@@ -113,10 +165,11 @@ GDNX_DEV void weights(const float* s, float c2, float mc, float2& sum, uint32_t*
   }
 }
 
-// A row's running state: the maximum that O and l are scaled to, the sum, and whether it saw a key.
+// A row's running state: the maximum that O and l are scaled to, the sum, whether it saw a key, and whether it is a
+// query at all (another may hold anything, and rescales nothing).
 struct Row {
   float m, l;
-  bool any;
+  bool any, query;
 };
 
 // Takes a tile's maximum into the row, rescaling O where it lies too far above the old one.
@@ -124,7 +177,7 @@ struct Row {
 // whatever its column, and from then on l and O or the maximum itself say so (ex2_poly alone would not).
 template <int DB>
 GDNX_DEV float take_max(Row& w, float top, float c2, uint32_t tO) {
-  const bool grow = w.m != -INFINITY && !((top - w.m) * c2 <= 8.f);
+  const bool grow = w.query && w.m != -INFINITY && !((top - w.m) * c2 <= 8.f);
   if (__any_sync(0xffffffffu, grow)) {
     const float corr = grow ? ex2((w.m - top) * c2) : 1.f;
     w.l *= corr;
@@ -161,8 +214,7 @@ GDNX_DEV uint32_t gone_bits(uint32_t gone, int page, int q) {
 
 // One stage's rows, one for each thread.
 template <int DB, bool BF16>
-GDNX_DEV void run_rows(const TcParams& P, const Share& share, uint8_t* base, Small& sm, uint32_t tmem) {
-  using Lo = Layout<DB>;
+GDNX_DEV void run_rows(const TcParams& P, const Share& share, Small& sm, uint32_t tmem) {
   const gdnx_paged_attn_args& a = P.a;
   const gdnx_cache& c = a.cache;
   Bars& bar = sm.bar;
@@ -173,7 +225,6 @@ GDNX_DEV void run_rows(const TcParams& P, const Share& share, uint8_t* base, Sma
   const int window = (int)a.window, sinks = (int)a.sinks, D = (int)c.D, npp = TM / c.page;
   const float c2 = a.scale * kLog2e;
   const int tok = r / P.gs, head = r % P.gs;  // this thread's row
-  uint8_t* out = base + Lo::OUT + warp * 4096;
   uint32_t nS = 0, nO = 0, nj = 0;
   if (threadIdx.x == 0 && P.cut) P.joint[blockIdx.x] = {0, 0, 0, 0, -1};
   Walk<Tc> w(P, share);
@@ -185,19 +236,25 @@ GDNX_DEV void run_rows(const TcParams& P, const Share& share, uint8_t* base, Sma
     const bool some = __any_sync(0xffffffffu, valid);
     const int p0 = w.s.first + t0, p1 = w.s.first + min(t0 + P.tb, w.s.count) - 1;  // of the block
     const int32_t* table = c.table + (int64_t)w.s.row * c.width;
-    Row row = {-INFINITY, 0.f, false};
+    Row row = {-INFINITY, 0.f, false, valid};
     bool worked = false;
-    for (int i = 0; i < g.n; ++i) {
-      const int kt = w.x.kt.tile(w.ta + i), j0 = kt * TM;
-      if (!g.on(st, i, kt)) continue;
+    // the stage's next tile from i on, and the lane's page of it
+    const auto next_tile = [&](int i) {
+      while (i < g.n && !g.on(st, i, g.tile(i))) ++i;
+      return i;
+    };
+    const auto page_there = [&](int i) {
+      const int64_t x = (int64_t)g.tile(i) * npp + lane;
+      return i < g.n && lane < npp ? (x < c.width ? table[x] : -1) : 0;
+    };
+    int after = next_tile(0), id = page_there(after);
+    while (after < g.n) {
+      const int i = after, j0 = g.tile(i) * TM;
       worked = true;
       // the tile's pages that are not there
-      int id = 0;
-      if (lane < npp) {
-        const int64_t x = (int64_t)kt * npp + lane;
-        id = x < c.width ? table[x] : -1;
-      }
       const uint32_t gone = __ballot_sync(0xffffffffu, id < 0 || id >= c.pages);
+      after = next_tile(i + 1);
+      id = page_there(after);
       if (!warp_wait(&bar.s_full[st], nS++ & 1, abort_flag)) return;
       tc::fence_after();
       if (!some) {  // no row of the warp is a query: what its weights are does not matter
@@ -306,7 +363,6 @@ GDNX_DEV void run_rows(const TcParams& P, const Share& share, uint8_t* base, Sma
     const float f = whole ? scale_of(top, l) : 1.f;
     const int64_t row_at = (int64_t)(w.s.start + t) * a.y_st + (int64_t)(w.head0() + head) * a.y_sh;
     const int64_t part = w.part() + (g.pair ? st * 128 : 0) + r;
-    const uint32_t live = __ballot_sync(0xffffffffu, valid);
 #pragma unroll 1
     for (int d = 0; d < 64 * DB; d += 64) {
       float o[64];
@@ -329,24 +385,15 @@ GDNX_DEV void run_rows(const TcParams& P, const Share& share, uint8_t* base, Sma
       }
 #pragma unroll
       for (int e = 0; e < 64; ++e) o[e] = f == 0.f ? 0.f : o[e] * f;
-      if (a.y_dtype != GDNX_F32 && P.vec_y) {  // through shared memory: four rows' 128 bytes to a store
+      if (a.y_dtype != GDNX_F32 && P.vec_y) {
         uint32_t u[32];
         pack_row(u, o, a.y_dtype);
         pack_row(u + 16, o + 32, a.y_dtype);
-        __syncwarp();
+        uint16_t* dst = static_cast<uint16_t*>(a.y) + row_at + d;
+        if (valid)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          *reinterpret_cast<uint4*>(out + tc::sw128(lane, e, 32)) =
-              make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
-        __syncwarp();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int from = e * 4 + lane / 8, x = lane % 8;
-          const int64_t at = __shfl_sync(0xffffffffu, row_at, from);
-          if ((live >> from & 1) && d + x * 8 < D)
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + at + d + x * 8) =
-                *reinterpret_cast<const uint4*>(out + tc::sw128(from, x, 32));
-        }
+          for (int e = 0; e < 8; ++e)
+            if (d + e * 8 < D) *reinterpret_cast<uint4*>(dst + e * 8) = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
       } else if (valid) {
 #pragma unroll
         for (int e = 0; e < 64; ++e)
@@ -367,66 +414,77 @@ GDNX_DEV void run_rows(const TcParams& P, const Share& share, uint8_t* base, Sma
 }
 
 // The warp that issues the products: for each step and stage PV of the step before, once its weights are there, and S of
-// this one, in one run.  In order, S of a step complete means PV of the one before complete.
-template <int DB, bool BF16>
-GDNX_DEV void run_products(const TcParams& P, const Share& share, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+// this one, in one run.  In order, S of a step complete means PV of the one before complete.  A step is a tile of two
+// blocks, or two tiles of one.
+template <int DB, bool BF16, bool PAIR>
+GDNX_DEV bool segment_products(const Seg& g, Ring<DB>& ring, uint32_t (&nP)[2], uint32_t smem, uint32_t tmem, Bars& bar,
+                               volatile int* abort_flag) {
   using Lo = Layout<DB>;
   constexpr uint32_t ID_S = idesc16(BF16, 128, 128, false, false), ID_O = idesc16(BF16, 128, 64 * DB, false, true);
-  uint32_t cnt = 0, nP[2] = {0, 0}, nQ[2] = {0, 0};
+  const int steps = PAIR ? g.n : (g.n + 1) / 2;
+  bool begun[2] = {false, false}, pend[2] = {false, false}, acc[2] = {false, false};
+  ring.begin(PAIR);
+  Place now = {0, 0}, before = {0, 0};  // where the step's tiles begin, and those of the one before
+  for (int s = 0; s <= steps; ++s) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const uint32_t tS = tmem + T_S + st * 128, tO = tmem + T_O + st * 128;
+      const int i = PAIR ? s : 2 * s + st, was = PAIR ? s - 1 : i - 2;
+      const bool there = i < g.n, on = there && (!PAIR || g.on(st, i, g.tile(i)));
+      const Place kp = ring.behind(now, PAIR ? 0 : st);
+      const Place vp = ring.behind(before, PAIR ? 1 : was == g.n - 1 && st == 0 ? 1 : 2 + st);
+      const uint32_t ksl = ring.slot(kp), vsl = ring.slot(vp), k = smem + ksl * Lo::TILE, v = smem + vsl * Lo::TILE;
+      if (on) {
+        if (!begun[st] && (PAIR || st == 0) && !warp_wait(&bar.full[st], ring.q_parity(st), abort_flag)) return false;
+        if (!warp_wait(&bar.full[ksl], ring.parity(kp), abort_flag)) return false;
+      }
+      if (pend[st]) {  // the first half's weights, then the second's
+        if (!warp_wait(&bar.full[vsl], ring.parity(vp), abort_flag)) return false;
+        if (!warp_wait(&bar.p_ready[st][0], nP[st] & 1, abort_flag)) return false;
+        tc::fence_after();
+        if (elect_one()) mma_px<4>(tO, tS, v, ID_O, acc[st]);
+        __syncwarp();
+        if (!warp_wait(&bar.p_ready[st][1], nP[st]++ & 1, abort_flag)) return false;
+      }
+      tc::fence_after();
+      if (elect_one()) {
+        if (pend[st]) {
+          mma_px<4>(tO, tS + 32, v + 64 * 128, ID_O, true);
+          if (was == g.last(st)) tc::commit(&bar.o_full[st]);
+        }
+        // V of the step before is done with: by both stages, or by the one whose it is
+        if (PAIR ? s > 0 && st == 1 : pend[st]) tc::commit(&bar.empty[vsl]);
+        if (on) {
+          mma_abt<DB>(tS, smem + (PAIR ? st : 0) * Lo::TILE, k, ID_S);
+          tc::commit(&bar.s_full[st]);
+          // the last product that reads a Q
+          if (i == (PAIR ? g.last(st) : g.n - 1)) tc::commit(&bar.empty[PAIR ? st : 0]);
+        }
+        if (there && (!PAIR || st == 1)) tc::commit(&bar.empty[ksl]);
+      }
+      __syncwarp();
+      acc[st] = acc[st] || pend[st];
+      begun[st] = begun[st] || on;
+      pend[st] = on;  // (a stage's gap between the sinks' tile and its window ends nothing)
+    }
+    before = now;
+    now = ring.behind(now, PAIR ? 2 : 4);
+  }
+  ring.end(2 * g.n, g.last0 >= 0, PAIR && g.last1 >= 0);
+  return true;
+}
+
+template <int DB, bool BF16>
+GDNX_DEV void run_products(const TcParams& P, const Share& share, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+  uint32_t nP[2] = {0, 0};
+  Ring<DB> ring;
   Walk<Tc> w(P, share);
   while (w.next()) {
-    const Seg g(P, w);
-    const int steps = g.pair ? g.n : (g.n + 1) / 2;
-    // a block's tiles go to both stages: one Q serves them
-    bool begun[2] = {false, false}, pend[2] = {false, false}, acc[2] = {false, false};
-    int was[2] = {0, 0};  // the stage's tile of the step before
-    for (int s = 0; s <= steps; ++s) {
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const uint32_t tS = tmem + T_S + st * 128, tO = tmem + T_O + st * 128;
-        const int i = g.pair ? s : 2 * s + st;
-        const bool there = i < g.n, on = there && g.on(st, i, w.x.kt.tile(w.ta + i));
-        const uint32_t kp = cnt + k_place(g.pair, i), ksl = kp % Lo::SLOTS;
-        const uint32_t vp = cnt + v_place(g.pair, was[st], g.n), vsl = vp % Lo::SLOTS;
-        if (on) {
-          if (!begun[st] && (g.pair || st == 0) && !warp_wait(&bar.q_full[st], nQ[st]++ & 1, abort_flag)) return;
-          if (!warp_wait(&bar.kv_full[ksl], kp / Lo::SLOTS & 1, abort_flag)) return;
-        }
-        if (pend[st]) {  // the first half's weights, then the second's
-          const uint32_t v = smem + Lo::KV + vsl * Lo::TILE;
-          if (!warp_wait(&bar.kv_full[vsl], vp / Lo::SLOTS & 1, abort_flag)) return;
-          if (!warp_wait(&bar.p_ready[st][0], nP[st] & 1, abort_flag)) return;
-          tc::fence_after();
-          if (elect_one()) mma_px<4>(tO, tS, v, ID_O, acc[st]);
-          __syncwarp();
-          if (!warp_wait(&bar.p_ready[st][1], nP[st]++ & 1, abort_flag)) return;
-        }
-        tc::fence_after();
-        if (elect_one()) {
-          if (pend[st]) {
-            mma_px<4>(tO, tS + 32, smem + Lo::KV + vsl * Lo::TILE + 64 * 128, ID_O, true);
-            if (was[st] == g.last(st)) tc::commit(&bar.o_full[st]);
-          }
-          // V of the step before is done with: by both stages, or by the one whose it is
-          if (s > 0 && g.pair && st == 1) tc::commit(&bar.kv_empty[(cnt + v_place(true, s - 1, g.n)) % Lo::SLOTS]);
-          if (pend[st] && !g.pair) tc::commit(&bar.kv_empty[vsl]);
-          if (on) {
-            mma_abt<DB>(tS, smem + Lo::Q + (g.pair ? st : 0) * Lo::TILE, smem + Lo::KV + ksl * Lo::TILE, ID_S);
-            tc::commit(&bar.s_full[st]);
-            // the last product that reads a Q
-            if (i == (g.pair ? g.last(st) : g.n - 1)) tc::commit(&bar.q_empty[g.pair ? st : 0]);
-          }
-          if (there && (g.pair ? st == 1 : true)) tc::commit(&bar.kv_empty[ksl]);
-        }
-        __syncwarp();
-        acc[st] = acc[st] || pend[st];
-        begun[st] = begun[st] || on;
-        // (a stage's gap between the sinks' tile and its window ends nothing)
-        pend[st] = on;
-        if (on) was[st] = i;
-      }
-    }
-    cnt += 2 * g.n;
+    Seg g(P, w);
+    g.make_uniform();
+    if (!(g.pair ? segment_products<DB, BF16, true>(g, ring, nP, smem, tmem, bar, abort_flag)
+                 : segment_products<DB, BF16, false>(g, ring, nP, smem, tmem, bar, abort_flag)))
+      return;
   }
 }
 
@@ -441,19 +499,21 @@ GDNX_DEV int page_of(const ChunkParams& P, const Chunk& s, int kt, int i) {
 
 // The warp that loads: a segment's first K, its Q, then the tiles in their places' order.
 template <int DB>
-GDNX_DEV void run_loads(const TcParams& P, const Share& share, uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag,
-                        uint32_t& issued) {
+GDNX_DEV void run_loads(const TcParams& P, const Share& share, uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag) {
   using Lo = Layout<DB>;
   const gdnx_cache& c = P.a.cache;
   const int lane = threadIdx.x % 32, page = c.page, npp = TM / page, ahead = 32 / npp;
   const uint32_t box = (uint32_t)page * 128;
-  uint32_t cnt = 0, nQ[2] = {0, 0}, nfix = 0;
+  uint32_t nfix = 0;
+  Ring<DB> ring;
   Walk<Tc> w(P, share);
   while (w.next()) {
     const Seg g(P, w);
     const int hk = w.hk();
+    ring.begin(g.pair);
+    Place at = {0, 0};
     int ids = -1, from = -1;  // page ids of tiles from .. from + ahead - 1
-    for (int x = 0; x < 2 * g.n; ++x) {
+    for (int x = 0; x < 2 * g.n; ++x, at = ring.behind(at, 1)) {
       // the tile and side at place x
       int i, side;
       if (g.pair || (g.n % 2 && x >= 2 * g.n - 2)) {
@@ -468,47 +528,47 @@ GDNX_DEV void run_loads(const TcParams& P, const Share& share, uint8_t* base, ui
       if (group != from) {
         from = group;
         const int mine = from + lane / npp;
-        ids = mine < g.n ? page_of(P, w.s, w.x.kt.tile(w.ta + mine), lane % npp) : -1;
+        ids = mine < g.n ? page_of(P, w.s, g.tile(mine), lane % npp) : -1;
       }
-      const int j0 = w.x.kt.tile(w.ta + i) * TM, pg = lane / DB, d = lane % DB;
+      const int j0 = g.tile(i) * TM, pg = lane / DB, d = lane % DB;
       const int id = __shfl_sync(0xffffffffu, ids, ((i - from) * npp + pg) & 31);
       const bool go = pg < npp && id >= 0;
       const uint32_t got = __ballot_sync(0xffffffffu, go);
-      const uint32_t place = cnt + x, sl = place % Lo::SLOTS, dst = smem + Lo::KV + sl * Lo::TILE;
-      if (!warp_wait(&bar.kv_empty[sl], (place / Lo::SLOTS & 1) ^ 1, abort_flag)) return;
+      const int sl = ring.slot(at);
+      const uint32_t dst = smem + sl * Lo::TILE;
+      if (!warp_wait(&bar.empty[sl], ring.parity(at) ^ 1, abort_flag)) return;
       const bool fix = side == 1 && (__popc(got) < npp * DB || j0 + TM > w.s.len());
-      uint64_t* full = fix ? &bar.fix : &bar.kv_full[sl];
+      uint64_t* full = fix ? &bar.fix : &bar.full[sl];
       const uint32_t mb = tc::smem_u32(full);
       if (lane == 0) pipe::expect_tx(mb, __popc(got) * box);
       __syncwarp();
       if (go)
         tma_load_3d(dst + d * BLOCK_BYTES + pg * box, &P.kv, d * 64, hk * page, (int)((P.a.layer * 2 + side) * c.pages + id), mb);
-      issued = place + 1;
       if (fix) {  // rows that no query may see meet weights of 0, so they must not hold NaN
         if (!warp_wait(&bar.fix, nfix++ & 1, abort_flag)) return;
         const int end = w.s.len() - j0;  // rows from here on are behind the last token
         for (int y = lane; y < TM * DB * 8; y += 32) {
           const int row = y / (DB * 8), e = y % (DB * 8);
           if (row < end && (got >> (row / page * DB) & 1)) continue;
-          *reinterpret_cast<uint4*>(base + Lo::KV + sl * Lo::TILE + (e / 8) * BLOCK_BYTES + row * 128 + e % 8 * 16) =
+          *reinterpret_cast<uint4*>(base + sl * Lo::TILE + (e / 8) * BLOCK_BYTES + row * 128 + e % 8 * 16) =
               make_uint4(0, 0, 0, 0);
         }
         tc::fence_async_smem();
         __syncwarp();
-        if (lane == 0) pipe::mbar_arrive(&bar.kv_full[sl]);
+        if (lane == 0) pipe::mbar_arrive(&bar.full[sl]);
       }
       if (x == 0) {
         const gdnx_view& q = P.a.q;
         for (int b = 0; b < (g.pair ? 2 : 1); ++b) {
           if (g.last(b) < 0) continue;
-          if (!warp_wait(&bar.q_empty[b], (nQ[b]++ & 1) ^ 1, abort_flag)) return;
-          const uint32_t at = smem + Lo::Q + b * Lo::TILE, qb = tc::smem_u32(&bar.q_full[b]);
+          if (!warp_wait(&bar.empty[b], ring.q_parity(b) ^ 1, abort_flag)) return;
+          const uint32_t to = smem + b * Lo::TILE, qb = tc::smem_u32(&bar.full[b]);
           const int t0 = w.x.t0 + b * P.tb, row0 = w.s.start + t0;
           if (P.tma_q) {
             if (lane == 0) {
               pipe::expect_tx(qb, DB * (uint32_t)(P.gs * P.tb) * 128);
 #pragma unroll
-              for (int e = 0; e < DB; ++e) tma_load_3d(at + e * BLOCK_BYTES, &P.q, e * 64, w.head0(), row0, qb);
+              for (int e = 0; e < DB; ++e) tma_load_3d(to + e * BLOCK_BYTES, &P.q, e * 64, w.head0(), row0, qb);
             }
             __syncwarp();
           } else {
@@ -527,16 +587,16 @@ GDNX_DEV void run_loads(const TcParams& P, const Share& share, uint8_t* base, ui
                   u.w = src[6] | (uint32_t)src[7] << 16;
                 }
               }
-              *reinterpret_cast<uint4*>(base + Lo::Q + b * Lo::TILE + tc::sw128(row, e, 128)) = u;
+              *reinterpret_cast<uint4*>(base + b * Lo::TILE + tc::sw128(row, e, 128)) = u;
             }
             tc::fence_async_smem();
             __syncwarp();
-            if (lane == 0) pipe::mbar_arrive(&bar.q_full[b]);
+            if (lane == 0) pipe::mbar_arrive(&bar.full[b]);
           }
         }
       }
     }
-    cnt += 2 * g.n;
+    ring.end(2 * g.n, g.last0 >= 0, g.pair && g.last1 >= 0);
   }
 }
 
@@ -552,13 +612,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
   dependents_may_start();
   if (threadIdx.x == 0) {
     *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
-    for (int i = 0; i < 8; ++i) {
-      tc::mbar_init(&bar.kv_full[i], 1);
-      tc::mbar_init(&bar.kv_empty[i], 1);
+    for (int i = 0; i < Lo::SLOTS; ++i) {
+      tc::mbar_init(&bar.full[i], 1);
+      tc::mbar_init(&bar.empty[i], 1);
     }
     for (int s = 0; s < 2; ++s) {
-      tc::mbar_init(&bar.q_full[s], 1);
-      tc::mbar_init(&bar.q_empty[s], 1);
       tc::mbar_init(&bar.s_full[s], 1);
       tc::mbar_init(&bar.p_ready[s][0], 128);
       tc::mbar_init(&bar.p_ready[s][1], 128);
@@ -570,10 +628,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
     tc::mbar_init(&bar.joined, 128);
   }
   if (warp == 8) tc::tmem_alloc(&sm.tmem_at, 512);
-  // rows of Q that no load writes stay zero
-  for (uint32_t i = threadIdx.x; i < 2 * Lo::TILE / 16; i += NTHREADS)
-    *reinterpret_cast<uint4*>(base + Lo::Q + i * 16) = make_uint4(0, 0, 0, 0);
-  tc::fence_async_smem();
   tc::fence_before();
   wait_for_earlier();
   find_share<Tc, NTHREADS>(P, sm.share, sm.sums);  // synchronises
@@ -582,7 +636,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
   if (smem % 1024) {  // never entered: the base is aligned
   } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 224 + 128 x 56 is just that
     regs_up<224>();
-    run_rows<DB, BF16>(P, sm.share, base, sm, tmem);
+    run_rows<DB, BF16>(P, sm.share, sm, tmem);
   } else {
     regs_down<56>();
     if (warp == 8) {
@@ -591,13 +645,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
       if (elect_one()) tc::commit(&bar.done);  // every product issued has ended before tensor memory is freed
       tc::mbar_wait(&bar.done, 0);
     } else if (warp == 9) {
-      uint32_t issued = 0;
-      run_loads<DB>(P, sm.share, base, smem, bar, abort_flag, issued);
-      if (*abort_flag && threadIdx.x % 32 == 0) {  // let the copies in flight land
-        for (uint32_t c = issued > Lo::SLOTS ? issued - Lo::SLOTS : 0; c < issued; ++c)
-          tc::mbar_wait(&bar.kv_full[c % Lo::SLOTS], c / Lo::SLOTS & 1, 1u << 16);
+      run_loads<DB>(P, sm.share, base, smem, bar, abort_flag);
+      if (*abort_flag)  // let the copies in flight land
         for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
-      }
     } else {
       write_padding(P, threadIdx.x - 320, 64);
     }
