@@ -4,7 +4,7 @@
 // A block of ROWS rows holds the queries of one key head (a group of at most ROWS of its query heads) at `tb` tokens in
 // sequence: row r is token r / gs, head r % gs.  So a chunk of a few tokens fills a tile with its heads, and keys and
 // values are read once for all of them.  A unit is one block (PAIR: two, where the chunk has them) of one sequence;
-// its tiles of KEYS keys weigh one a block, and it weighs OVER more for its start and end.  Units are ordered by
+// its tiles of KEYS keys have a weight each, its start and end another.  Units are ordered by
 // sequence, head group, tokens.  Every CTA finds its share of the row from the lengths by itself, without a word to
 // the host: mixed batches of whole chunks and single tokens leave no SM waiting, and one token over a long cache has
 // all of them.  Units of up to SMALL in weight stay whole: a few more tiles in a row take less time than a join.
@@ -58,22 +58,25 @@ template <int ROWS_, int KEYS_, bool PAIR_>
 struct Shape {
   static constexpr int ROWS = ROWS_, KEYS = KEYS_;
   static constexpr bool PAIR = PAIR_;
-  static constexpr int OVER = 2, SMALL = 8, LEAST = 4;  // LEAST: of a CTA's share, so that few tiles are not cut into less
+  // Weights: of a unit's start and end, of a tile of one block and of two, of a unit that stays whole, and of a CTA's
+  // share at least, so that few tiles are not cut into less.
+  static constexpr int OVER = 12, ONE = 2, TWO = 4, SMALL = 24, LEAST = 8;
 };
 
 // A unit of a sequence: its key tiles, blocks and weight.
 template <class S>
 struct Unit {
   KeyTiles kt;
-  int t0, blocks, w;  // first token of the chunk
-  GDNX_DEV Unit() : kt(), t0(0), blocks(0), w(0) {}
+  int t0, blocks, each, w;  // first token of the chunk; weights of a tile and in all
+  GDNX_DEV Unit() : kt(), t0(0), blocks(0), each(0), w(0) {}
   GDNX_DEV Unit(const ChunkParams& P, const Chunk& s, int u) {
     const int step = S::PAIR ? 2 * P.tb : P.tb;
     t0 = u * step;
     const int n = min(step, s.count - t0);
     blocks = n > P.tb ? 2 : 1;
     kt = KeyTiles(s.first + t0, s.first + t0 + n - 1, s.len(), (int)P.a.window, (int)P.a.sinks, S::KEYS);
-    w = S::OVER + blocks * kt.count;
+    each = blocks == 2 ? S::TWO : S::ONE;
+    w = S::OVER + each * kt.count;
   }
 };
 
@@ -228,10 +231,10 @@ struct Walk {
         ta = 0;
         tb = before >= t0 ? x.kt.count : 0;
       } else {
-        // tile i lies at before + OVER + i * blocks, and belongs to the share that this lies in
+        // tile i lies at before + OVER + i * each, and belongs to the share that this lies in
         const long long lo = t0 - before - S::OVER, hi = t1 - before - S::OVER;
-        ta = lo <= 0 ? 0 : (int)min((lo + x.blocks - 1) / x.blocks, (long long)x.kt.count);
-        tb = hi <= 0 ? 0 : (int)min((hi + x.blocks - 1) / x.blocks, (long long)x.kt.count);
+        ta = lo <= 0 ? 0 : (int)min((lo + x.each - 1) / x.each, (long long)x.kt.count);
+        tb = hi <= 0 ? 0 : (int)min((hi + x.each - 1) / x.each, (long long)x.kt.count);
       }
       if (ta < tb) return true;
     }
@@ -387,9 +390,10 @@ ChunkParams plan_chunks(const gdnx_paged_attn_args& a, int ctas) {
   int64_t tiles = (most + S::KEYS - 1) / S::KEYS;  // of a unit, at most
   const int64_t seen = (a.window + (S::PAIR ? 2 : 1) * P.tb + S::KEYS - 1) / S::KEYS + 1 + (a.sinks + S::KEYS - 1) / S::KEYS;
   if (seen < tiles) tiles = seen;
-  P.cut = S::OVER + tiles * (P.rows / S::ROWS) > S::SMALL;
+  const int64_t w = S::OVER + tiles * (P.rows > S::ROWS ? S::TWO : S::ONE);  // of a unit, at most
+  P.cut = w > S::SMALL;
   // a CTA's share is LEAST in weight, or a unit
-  const int64_t units = (a.tokens / P.tb + a.n) * a.cache.Hk * P.groups, w = S::OVER + tiles * (P.rows / S::ROWS);
+  const int64_t units = (a.tokens / P.tb + a.n) * a.cache.Hk * P.groups;
   const int64_t want = P.cut ? (units * w + S::LEAST - 1) / S::LEAST : units;
   P.grid = (int)(want < ctas ? (want > 0 ? want : 1) : ctas);
   P.part = static_cast<float*>(a.workspace);
