@@ -161,7 +161,7 @@ GDNX_DEV void find_share(const ChunkParams& P, Share& out, long long* sums) {
   if (__any_sync(0xffffffffu, here)) {
     bool found = false;
     for (int64_t k = 0; k < run; ++k) {
-      const long long w = weight(b0 + k) * hgs;
+      const long long w = (run == 1 ? mine : weight(b0 + k)) * hgs;
       if (here && !found && t0 < before + w) {
         found = true;
         out = {t0, min(t0 + per, total), before, per, w / hgs, (int)(b0 + k), 0, 0};

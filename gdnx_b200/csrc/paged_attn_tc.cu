@@ -9,9 +9,10 @@
 // rounded as in windowed attention's forward (attn_fwd.cu).
 //
 // Keys and values come by TMA, a box for each page and 64 dims.  Pages that are not there are not fetched; rows of V
-// that no query may see (those, and rows behind the last token, which may hold NaN) are cleared by the loading warp.
-// Warps 0-3 and 4-7 are the stages' rows, warp 8 issues the products, warp 9 the loads, 10 and 11 clear padding rows
-// of the output.
+// that no query may see (those, and rows behind the last token) may hold NaN and are cleared.
+// Warps 0-3 and 4-7 are the stages' rows, warp 8 issues the products, warp 9 the loads, warp 11 clears rows of V.  Warp
+// 10 walks the share ahead of them all and leaves what they need of each segment in a short queue, so that none waits
+// for lengths and page tables where one segment ends and the next begins; then it clears padding rows of the output.
 #include "paged_attn.cuh"
 
 namespace gdnx {
@@ -32,71 +33,9 @@ struct TcParams : ChunkParams {
 constexpr int MOST_SLOTS = 14;
 
 struct Bars {
-  uint64_t full[MOST_SLOTS], empty[MOST_SLOTS], s_full[2], p_ready[2][2], o_full[2], fix, done, left, joined;
+  uint64_t full[MOST_SLOTS], empty[MOST_SLOTS], landed[MOST_SLOTS], s_full[2], p_ready[2][2], o_full[2], done, left, joined;
+  uint64_t item_full[4], item_empty[4], job_full[4], job_empty[4];
 };
-
-struct Small {
-  Bars bar;
-  Share share;
-  long long sums[NTHREADS / 32];
-  float2 stat[128];  // stage 1's maxima and sums
-  uint32_t tmem_at;
-  int abort_flag;
-};
-
-// Shared memory is slots of one tile.  The first holds the block's Q, the second a second block's; the others, and the
-// second where there is one block, are the ring that K and V go round, from its first slot in every segment.
-template <int DB>
-struct Layout {
-  static constexpr int SLOTS = DB == 2 ? 7 : 14;
-  static constexpr uint32_t TILE = DB * BLOCK_BYTES, SMALL = SLOTS * TILE;
-  static constexpr size_t SMEM = SMALL + sizeof(Small);  // no static shared memory: the base is 1024-aligned
-};
-
-// A place of a segment's ring: its slot behind the ring's first, and whether an odd number of rounds lies behind it.
-struct Place {
-  int at;
-  uint32_t odd;
-};
-
-// What a role knows of the slots: a bit for each, the parity of its next use in this segment.
-template <int DB>
-struct Ring {
-  uint32_t bits = 0;
-  int first = 1, size = 1;  // of the segment's ring
-  GDNX_DEV void begin(bool pair) {
-    first = pair ? 2 : 1;
-    size = Layout<DB>::SLOTS - first;
-  }
-  // The place n (at most a round) behind p.
-  GDNX_DEV Place behind(Place p, int n) const {
-    p.at += n;
-    if (p.at >= size) {
-      p.at -= size;
-      p.odd ^= 1;
-    }
-    return p;
-  }
-  GDNX_DEV int slot(Place p) const { return first + p.at; }
-  GDNX_DEV uint32_t parity(Place p) const { return (bits >> (first + p.at) ^ p.odd) & 1; }
-  GDNX_DEV uint32_t q_parity(int b) const { return bits >> b & 1; }
-  // A segment of n places and these Qs is over.
-  GDNX_DEV void end(int n, bool q0, bool q1) {
-    // slots before n % size have had one use more than the others
-    const uint32_t all = ((1u << size) - 1) << first, more = ((1u << n % size) - 1) << first;
-    bits ^= (n / size & 1 ? all : 0) ^ more ^ (q0 ? 1 : 0) ^ (q1 ? 2 : 0);
-  }
-};
-
-GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t mbar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(mbar)
-      : "memory");
-}
-
-// A segment's tiles in the ring.  Two blocks: K0 V0 K1 V1 ...  One block: two tiles at a time, K0 K1 V0 V1 K2 K3 ...; a
-// last odd one K V.
 
 // What a segment asks of its stages.
 struct Seg {
@@ -151,6 +90,91 @@ struct Seg {
     return st ? kt <= hi1 && (kt >= lo1 || kt < nst) : kt <= hi0;
   }
 };
+
+// A segment in the queue; the last has no tiles.
+struct Item {
+  Seg g;
+  int row, start, first, count, t0;  // the chunk, and the segment's first token in it
+  int hk, head0, heads;
+  int part, whole;  // rows of its part; or it is a whole unit
+  int ids[32];      // page ids of its first tiles, a lane's each
+  GDNX_DEV int len() const { return first + count; }
+};
+constexpr int ITEMS = 4, JOBS = 4, MASKS = 32;
+
+// A tile of V to be cleared, once it has landed, of the rows from `end` on and of the pages that are not there; slot < 0:
+// there are no more.
+struct Job {
+  int slot, end;
+  uint32_t there;
+};
+
+struct Small {
+  Bars bar;
+  Item item[ITEMS];
+  Job job[JOBS];
+  Share share;
+  long long sums[NTHREADS / 32];
+  float2 stat[128];  // stage 1's maxima and sums
+  uint8_t there[MASKS];  // pages of the tiles that are there, tile after tile
+  uint32_t tmem_at;
+  int abort_flag;
+};
+
+// Shared memory is slots of one tile.  The first holds the block's Q, the second a second block's; the others, and the
+// second where there is one block, are the ring that K and V go round, from its first slot in every segment.
+template <int DB>
+struct Layout {
+  static constexpr int SLOTS = DB == 2 ? 7 : 14;
+  static constexpr uint32_t TILE = DB * BLOCK_BYTES, SMALL = SLOTS * TILE;
+  static constexpr size_t SMEM = SMALL + sizeof(Small);  // no static shared memory: the base is 1024-aligned
+  static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
+};
+
+// A place of a segment's ring: its slot behind the ring's first, and whether an odd number of rounds lies behind it.
+struct Place {
+  int at;
+  uint32_t odd;
+};
+
+// What a role knows of the slots: a bit for each, the parity of its next use in this segment.
+template <int DB>
+struct Ring {
+  uint32_t bits = 0;
+  int first = 1, size = 1;  // of the segment's ring
+  GDNX_DEV void begin(bool pair) {
+    first = pair ? 2 : 1;
+    size = Layout<DB>::SLOTS - first;
+  }
+  // The place n (at most a round) behind p.
+  GDNX_DEV Place behind(Place p, int n) const {
+    p.at += n;
+    if (p.at >= size) {
+      p.at -= size;
+      p.odd ^= 1;
+    }
+    return p;
+  }
+  GDNX_DEV int slot(Place p) const { return first + p.at; }
+  GDNX_DEV uint32_t parity(Place p) const { return (bits >> (first + p.at) ^ p.odd) & 1; }
+  GDNX_DEV uint32_t q_parity(int b) const { return bits >> b & 1; }
+  // A segment of n places and these Qs is over.
+  GDNX_DEV void end(int n, bool q0, bool q1) {
+    // slots before n % size have had one use more than the others
+    const uint32_t all = ((1u << size) - 1) << first, more = ((1u << n % size) - 1) << first;
+    bits ^= (n / size & 1 ? all : 0) ^ more ^ (q0 ? 1 : 0) ^ (q1 ? 2 : 0);
+  }
+};
+
+GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(mbar)
+      : "memory");
+}
+
+// A segment's tiles in the ring.  Two blocks: K0 V0 K1 V1 ...  One block: two tiles at a time, K0 K1 V0 V1 K2 K3 ...; a
+// last odd one K V.
 
 // Weights of N columns: p = 2^(c2 s - mc), summed, packed 16-bit.  One pair in eight is taken on the FMA pipes (where
 // masked scores give 2^-125: nothing beside a weight that counts).
@@ -214,7 +238,7 @@ GDNX_DEV uint32_t gone_bits(uint32_t gone, int page, int q) {
 
 // One stage's rows, one for each thread.
 template <int DB, bool BF16>
-GDNX_DEV void run_rows(const TcParams& P, const Share& share, Small& sm, uint32_t tmem) {
+GDNX_DEV void run_rows(const TcParams& P, Small& sm, uint32_t tmem) {
   const gdnx_paged_attn_args& a = P.a;
   const gdnx_cache& c = a.cache;
   Bars& bar = sm.bar;
@@ -222,39 +246,31 @@ GDNX_DEV void run_rows(const TcParams& P, const Share& share, Small& sm, uint32_
   const int r = threadIdx.x % 128, lane = r % 32, warp = threadIdx.x / 32, st = warp / 4;
   const uint32_t lane_at = (uint32_t)(r / 32 * 32) << 16;
   const uint32_t tS = tmem + T_S + st * 128 + lane_at, tO = tmem + T_O + st * 128 + lane_at;
-  const int window = (int)a.window, sinks = (int)a.sinks, D = (int)c.D, npp = TM / c.page;
+  const int window = (int)a.window, sinks = (int)a.sinks, D = (int)c.D;
+  const uint32_t all_pages = (1u << TM / c.page) - 1;
   const float c2 = a.scale * kLog2e;
   const int tok = r / P.gs, head = r % P.gs;  // this thread's row
-  uint32_t nS = 0, nO = 0, nj = 0;
-  if (threadIdx.x == 0 && P.cut) P.joint[blockIdx.x] = {0, 0, 0, 0, -1};
-  Walk<Tc> w(P, share);
-  while (w.next()) {
-    const Seg g(P, w);
-    const int len = w.s.len(), t0 = w.x.t0 + (g.pair && st ? P.tb : 0), t = t0 + tok;
-    const bool valid = tok < P.tb && head < w.heads() && t < w.s.count;
-    const int p = valid ? w.s.first + t : -1;
+  uint32_t nS = 0, nO = 0, nj = 0, tiles = 0;
+  for (uint32_t k = 0;; ++k) {
+    __syncwarp();  // the segment before is done with
+    if (k > 0 && lane == 0) pipe::mbar_arrive(&bar.item_empty[(k - 1) % ITEMS]);
+    if (!warp_wait(&bar.item_full[k % ITEMS], k / ITEMS & 1, abort_flag)) return;
+    const Item& w = sm.item[k % ITEMS];
+    const Seg g = w.g;
+    if (g.n == 0) return;
+    const int t0 = w.t0 + (g.pair && st ? P.tb : 0), t = t0 + tok, first = w.first, count = w.count;
+    const bool valid = tok < P.tb && head < w.heads && t < count;
+    const int p = valid ? first + t : -1;
     const bool some = __any_sync(0xffffffffu, valid);
-    const int p0 = w.s.first + t0, p1 = w.s.first + min(t0 + P.tb, w.s.count) - 1;  // of the block
-    const int32_t* table = c.table + (int64_t)w.s.row * c.width;
+    const int p0 = first + t0, p1 = first + min(t0 + P.tb, count) - 1;  // of the block
     Row row = {-INFINITY, 0.f, false, valid};
     bool worked = false;
-    // the stage's next tile from i on, and the lane's page of it
-    const auto next_tile = [&](int i) {
-      while (i < g.n && !g.on(st, i, g.tile(i))) ++i;
-      return i;
-    };
-    const auto page_there = [&](int i) {
-      const int64_t x = (int64_t)g.tile(i) * npp + lane;
-      return i < g.n && lane < npp ? (x < c.width ? table[x] : -1) : 0;
-    };
-    int after = next_tile(0), id = page_there(after);
-    while (after < g.n) {
-      const int i = after, j0 = g.tile(i) * TM;
+    const uint32_t from = tiles;
+    tiles += g.n;
+    for (int i = 0; i < g.n; ++i) {
+      const int kt = g.tile(i), j0 = kt * TM;
+      if (!g.on(st, i, kt)) continue;
       worked = true;
-      // the tile's pages that are not there
-      const uint32_t gone = __ballot_sync(0xffffffffu, id < 0 || id >= c.pages);
-      after = next_tile(i + 1);
-      id = page_there(after);
       if (!warp_wait(&bar.s_full[st], nS++ & 1, abort_flag)) return;
       tc::fence_after();
       if (!some) {  // no row of the warp is a query: what its weights are does not matter
@@ -262,63 +278,40 @@ GDNX_DEV void run_rows(const TcParams& P, const Share& share, Small& sm, uint32_
         pipe::mbar_arrive(&bar.p_ready[st][1]);
         continue;
       }
+      // the tile's pages that are not there
+      const uint32_t gone = ~*const_cast<volatile uint8_t*>(&sm.there[(from + i) % MASKS]) & all_pages;
       float2 sum = make_float2(0.f, 0.f);
+      float s[128], t4[4];
+      tmem_ld128(tS, s);
       // does every row see the whole tile?
       if (!gone && j0 + TM - 1 <= p0 && (p1 - j0 < window || j0 + TM <= sinks)) {
         row.any = true;
-        float s[128], t4[4];
-        tmem_ld128(tS, s);
-#pragma unroll
-        for (int f = 0; f < 4; ++f) t4[f] = s[f];
-#pragma unroll
-        for (int e = 4; e < 128; e += 4)
-#pragma unroll
-          for (int f = 0; f < 4; ++f) t4[f] = max_nan(t4[f], s[e + f]);
-        const float mc = take_max<DB>(row, max_nan(max_nan(t4[0], t4[1]), max_nan(t4[2], t4[3])), c2, tO);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t pk[32];
-          weights<BF16, 64>(s + 64 * half, c2, mc, sum, pk);
-          tmem_st32u(tS + 32 * half, pk);
-          tc::fence_before();
-          pipe::mbar_arrive(&bar.p_ready[st][half]);
-        }
       } else {
-        // chunk by chunk of 32 columns: what no row of the warp sees costs nothing
         // visible columns: lo..hi, and those up to sk
         const int hi = p - j0, lo = p - window + 1 - j0, sk = min(sinks - 1 - j0, hi);
-        uint32_t used = 0;
-        float top = -INFINITY;
-#pragma unroll 1
+#pragma unroll
         for (int q = 0; q < 4; ++q) {
           const uint32_t on = (range_bits(lo, hi, q) | range_bits(0, sk, q)) & ~gone_bits(gone, c.page, q);
-          if (!__any_sync(0xffffffffu, on)) continue;
-          used |= 1u << q;
           row.any |= on != 0;
-          float s[32];
-          tc::tmem_ld32(tS + 32 * q, s);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) top = max_nan(top, on >> e & 1 ? s[e] : -INFINITY);
+          for (int e = 0; e < 32; ++e)
+            if (!(on >> e & 1)) s[32 * q + e] = -INFINITY;
         }
-        const float mc = take_max<DB>(row, top, c2, tO);
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          uint32_t pk[16] = {};
-          if (used >> q & 1) {
-            const uint32_t on = (range_bits(lo, hi, q) | range_bits(0, sk, q)) & ~gone_bits(gone, c.page, q);
-            float s[32];
-            tc::tmem_ld32(tS + 32 * q, s);
+      }
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(on >> e & 1)) s[e] = -INFINITY;
-            weights<BF16, 32>(s, c2, mc, sum, pk);
-          }
-          tc::tmem_st16u(tS + 16 * q, pk);  // over scores that have been read
-          if (q % 2) {
-            tc::fence_before();
-            pipe::mbar_arrive(&bar.p_ready[st][q / 2]);
-          }
-        }
+      for (int f = 0; f < 4; ++f) t4[f] = s[f];
+#pragma unroll
+      for (int e = 4; e < 128; e += 4)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) t4[f] = max_nan(t4[f], s[e + f]);
+      const float mc = take_max<DB>(row, max_nan(max_nan(t4[0], t4[1]), max_nan(t4[2], t4[3])), c2, tO);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t pk[32];
+        weights<BF16, 64>(s + 64 * half, c2, mc, sum, pk);
+        tmem_st32u(tS + 32 * half, pk);
+        tc::fence_before();
+        pipe::mbar_arrive(&bar.p_ready[st][half]);
       }
       row.l += sum.x + sum.y;
     }
@@ -352,17 +345,20 @@ GDNX_DEV void run_rows(const TcParams& P, const Share& share, Small& sm, uint32_
       row.l = row.l * f0 + (other ? x.y * f1 : 0.f);
       row.any |= other;
     }
-    if (!some && !both) continue;
+    if (!some) {
+      if (both) pipe::mbar_arrive(&bar.joined);
+      continue;
+    }
     // the maximum in the log2 domain and the sum as the join takes them: a maximum that is not finite comes of scores
     // that are not, and shows in the sum
     const float mc = row.m * c2;
     const bool finite = fabsf(mc) < INFINITY;
     const float top = !row.any ? -INFINITY : finite ? mc : kNoScore;
     const float l = !row.any || row.m == -INFINITY ? 0.f : finite ? row.l : NAN;
-    const bool whole = w.whole();
+    const bool whole = w.whole;
     const float f = whole ? scale_of(top, l) : 1.f;
-    const int64_t row_at = (int64_t)(w.s.start + t) * a.y_st + (int64_t)(w.head0() + head) * a.y_sh;
-    const int64_t part = w.part() + (g.pair ? st * 128 : 0) + r;
+    const int64_t row_at = (int64_t)(w.start + t) * a.y_st + (int64_t)(w.head0 + head) * a.y_sh;
+    const int64_t part = (int64_t)w.part + (g.pair ? st * 128 : 0) + r;
 #pragma unroll 1
     for (int d = 0; d < 64 * DB; d += 64) {
       float o[64];
@@ -375,6 +371,10 @@ GDNX_DEV void run_rows(const TcParams& P, const Share& share, Small& sm, uint32_
         tmem_ld64(tO + 128 + d, x);
 #pragma unroll
         for (int e = 0; e < 64; ++e) o[e] = o[e] * f0 + x[e] * f1;
+        if (d + 64 == 64 * DB) {  // stage 1's output may be written again
+          tc::fence_before();
+          pipe::mbar_arrive(&bar.joined);
+        }
       }
       if (!whole) {
         if (valid)
@@ -400,16 +400,11 @@ GDNX_DEV void run_rows(const TcParams& P, const Share& share, Small& sm, uint32_
           if (d + e < D) st_from_f32(a.y, a.y_dtype, row_at + d + e, o[e]);
       }
     }
-    if (valid && whole && a.lse) a.lse[(int64_t)(w.s.start + t) * a.H + w.head0() + head] = lse_of(top, l);
+    if (valid && whole && a.lse) a.lse[(int64_t)(w.start + t) * a.H + w.head0 + head] = lse_of(top, l);
     if (valid && !whole) {
       P.stat[part * 2] = top;
       P.stat[part * 2 + 1] = l;
     }
-    if (both) {  // stage 1's output may be written again
-      tc::fence_before();
-      pipe::mbar_arrive(&bar.joined);
-    }
-    if (threadIdx.x == 0 && w.ends_cut()) P.joint[blockIdx.x] = w.joint(share.per);
   }
 }
 
@@ -475,109 +470,157 @@ GDNX_DEV bool segment_products(const Seg& g, Ring<DB>& ring, uint32_t (&nP)[2], 
 }
 
 template <int DB, bool BF16>
-GDNX_DEV void run_products(const TcParams& P, const Share& share, uint32_t smem, uint32_t tmem, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void run_products(Small& sm, uint32_t smem, uint32_t tmem) {
+  Bars& bar = sm.bar;
+  volatile int* abort_flag = &sm.abort_flag;
   uint32_t nP[2] = {0, 0};
   Ring<DB> ring;
-  Walk<Tc> w(P, share);
-  while (w.next()) {
-    Seg g(P, w);
+  for (uint32_t k = 0;; ++k) {
+    if (!warp_wait(&bar.item_full[k % ITEMS], k / ITEMS & 1, abort_flag)) return;
+    Seg g = sm.item[k % ITEMS].g;
     g.make_uniform();
+    if (g.n == 0) return;
+    __syncwarp();
+    if (threadIdx.x % 32 == 0) pipe::mbar_arrive(&bar.item_empty[k % ITEMS]);
     if (!(g.pair ? segment_products<DB, BF16, true>(g, ring, nP, smem, tmem, bar, abort_flag)
                  : segment_products<DB, BF16, false>(g, ring, nP, smem, tmem, bar, abort_flag)))
       return;
   }
 }
 
-// Page ids of tile kt's pages for the lanes below npp, -1 where there is none.
-GDNX_DEV int page_of(const ChunkParams& P, const Chunk& s, int kt, int i) {
-  const gdnx_cache& c = P.a.cache;
+// The page of tile kt's i-th page in the cache, -1 where there is none.
+GDNX_DEV int page_of(const gdnx_cache& c, int row, int len, int kt, int i) {
   const int64_t x = (int64_t)kt * (TM / c.page) + i;
-  if (x >= c.width || x * c.page >= s.len()) return -1;
-  const int p = c.table[(int64_t)s.row * c.width + x];
+  if (x >= c.width || x * c.page >= len) return -1;
+  const int p = c.table[(int64_t)row * c.width + x];
   return p >= 0 && p < c.pages ? p : -1;
+}
+
+// The warp that walks the share.
+GDNX_DEV void run_schedule(const TcParams& P, Small& sm) {
+  Bars& bar = sm.bar;
+  const int lane = threadIdx.x % 32, npp = TM / P.a.cache.page;
+  if (lane == 0 && P.cut) P.joint[blockIdx.x] = {0, 0, 0, 0, -1};
+  Walk<Tc> w(P, sm.share);
+  for (uint32_t k = 0;; ++k) {
+    const bool more = w.next();
+    if (!warp_wait(&bar.item_empty[k % ITEMS], (k / ITEMS & 1) ^ 1, &sm.abort_flag)) return;
+    Item& x = sm.item[k % ITEMS];
+    if (more) {
+      const Seg g(P, w);
+      const int i = lane / npp;
+      x.ids[lane] = i < g.n ? page_of(P.a.cache, w.s.row, w.s.len(), g.tile(i), lane % npp) : -1;
+      if (lane == 0) {
+        x.g = g;
+        x.row = w.s.row;
+        x.start = w.s.start;
+        x.first = w.s.first;
+        x.count = w.s.count;
+        x.t0 = w.x.t0;
+        x.hk = w.hk();
+        x.head0 = w.head0();
+        x.heads = w.heads();
+        x.part = (int)w.part();
+        x.whole = w.whole();
+        if (w.ends_cut()) P.joint[blockIdx.x] = w.joint(sm.share.per);
+      }
+    } else if (lane == 0) {
+      x.g.n = 0;
+    }
+    __syncwarp();
+    if (lane == 0) pipe::mbar_arrive(&bar.item_full[k % ITEMS]);
+    if (!more) return;
+  }
+}
+
+// A segment's places in order: f(tile, side (0: K, 1: V), place), until that is false.
+template <int DB, typename F>
+GDNX_DEV bool for_places(const Ring<DB>& ring, const Seg& g, F f) {
+  Place at = {0, 0};
+  for (int x = 0; x < 2 * g.n; ++x, at = ring.behind(at, 1)) {
+    const bool two = g.pair || (g.n % 2 && x >= 2 * g.n - 2);
+    if (!f(two ? x / 2 : x / 4 * 2 + x % 2, two ? x % 2 : x % 4 / 2, at)) return false;
+  }
+  return true;
 }
 
 // The warp that loads: a segment's first K, its Q, then the tiles in their places' order.
 template <int DB>
-GDNX_DEV void run_loads(const TcParams& P, const Share& share, uint8_t* base, uint32_t smem, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void run_loads(const TcParams& P, Small& sm, uint8_t* base, uint32_t smem) {
   using Lo = Layout<DB>;
   const gdnx_cache& c = P.a.cache;
-  const int lane = threadIdx.x % 32, page = c.page, npp = TM / page, ahead = 32 / npp;
-  const uint32_t box = (uint32_t)page * 128;
-  uint32_t nfix = 0;
+  Bars& bar = sm.bar;
+  volatile int* abort_flag = &sm.abort_flag;
+  const int lane = threadIdx.x % 32, page = c.page, npp = TM / page, ahead = 32 / npp, pg = lane / DB, d = lane % DB;
+  const uint32_t box = (uint32_t)page * 128, all_pages = (1u << npp) - 1;
+  uint32_t tiles = 0, jobs = 0;
+  const auto post = [&](const Job& j) {  // to the warp that clears
+    if (!warp_wait(&bar.job_empty[jobs % JOBS], (jobs / JOBS & 1) ^ 1, abort_flag)) return false;
+    if (lane == 0) {
+      sm.job[jobs % JOBS] = j;
+      pipe::mbar_arrive(&bar.job_full[jobs % JOBS]);
+    }
+    __syncwarp();
+    ++jobs;
+    return true;
+  };
   Ring<DB> ring;
-  Walk<Tc> w(P, share);
-  while (w.next()) {
-    const Seg g(P, w);
-    const int hk = w.hk();
+  for (uint32_t k = 0;; ++k) {
+    if (!warp_wait(&bar.item_full[k % ITEMS], k / ITEMS & 1, abort_flag)) return;
+    const Item& w = sm.item[k % ITEMS];
+    const Seg g = w.g;
+    if (g.n == 0) break;
+    const int hk = w.hk, row = w.row, len = w.len();
     ring.begin(g.pair);
-    Place at = {0, 0};
-    int ids = -1, from = -1;  // page ids of tiles from .. from + ahead - 1
-    for (int x = 0; x < 2 * g.n; ++x, at = ring.behind(at, 1)) {
-      // the tile and side at place x
-      int i, side;
-      if (g.pair || (g.n % 2 && x >= 2 * g.n - 2)) {
-        i = x / 2;
-        side = x % 2;
-      } else {
-        i = x / 4 * 2 + x % 2;
-        side = x % 4 / 2;
+    // page ids of tiles from .. from + ahead - 1, a lane's each, and of those behind them
+    const auto read = [&](int first) {
+      const int i = first + lane / npp;
+      return i < g.n ? page_of(c, row, len, g.tile(i), lane % npp) : -1;
+    };
+    int from = 0, ids = w.ids[lane], next = ahead < g.n ? read(ahead) : -1;
+    const auto load = [&](int i, int side, Place at) {
+      if (i >= from + ahead) {  // (a step's two tiles lie in one reading: their number is even, or one)
+        from += ahead;
+        ids = next;
+        if (from + ahead < g.n) next = read(from + ahead);
       }
-      // (a step's two tiles lie in one reading of ids: their count is even, or one)
-      const int group = (i / ahead) * ahead;
-      if (group != from) {
-        from = group;
-        const int mine = from + lane / npp;
-        ids = mine < g.n ? page_of(P, w.s, g.tile(mine), lane % npp) : -1;
-      }
-      const int j0 = g.tile(i) * TM, pg = lane / DB, d = lane % DB;
       const int id = __shfl_sync(0xffffffffu, ids, ((i - from) * npp + pg) & 31);
-      const bool go = pg < npp && id >= 0;
-      const uint32_t got = __ballot_sync(0xffffffffu, go);
-      const int sl = ring.slot(at);
-      const uint32_t dst = smem + sl * Lo::TILE;
-      if (!warp_wait(&bar.empty[sl], ring.parity(at) ^ 1, abort_flag)) return;
-      const bool fix = side == 1 && (__popc(got) < npp * DB || j0 + TM > w.s.len());
-      uint64_t* full = fix ? &bar.fix : &bar.full[sl];
-      const uint32_t mb = tc::smem_u32(full);
-      if (lane == 0) pipe::expect_tx(mb, __popc(got) * box);
-      __syncwarp();
-      if (go)
-        tma_load_3d(dst + d * BLOCK_BYTES + pg * box, &P.kv, d * 64, hk * page, (int)((P.a.layer * 2 + side) * c.pages + id), mb);
-      if (fix) {  // rows that no query may see meet weights of 0, so they must not hold NaN
-        if (!warp_wait(&bar.fix, nfix++ & 1, abort_flag)) return;
-        const int end = w.s.len() - j0;  // rows from here on are behind the last token
-        for (int y = lane; y < TM * DB * 8; y += 32) {
-          const int row = y / (DB * 8), e = y % (DB * 8);
-          if (row < end && (got >> (row / page * DB) & 1)) continue;
-          *reinterpret_cast<uint4*>(base + sl * Lo::TILE + (e / 8) * BLOCK_BYTES + row * 128 + e % 8 * 16) =
-              make_uint4(0, 0, 0, 0);
-        }
-        tc::fence_async_smem();
-        __syncwarp();
-        if (lane == 0) pipe::mbar_arrive(&bar.full[sl]);
+      const uint32_t there = __ballot_sync(0xffffffffu, ids >= 0) >> ((i - from) * npp) & all_pages;
+      const int sl = ring.slot(at), j0 = g.tile(i) * TM;
+      if (!warp_wait(&bar.empty[sl], ring.parity(at) ^ 1, abort_flag)) return false;
+      // rows of V that no query may see meet weights of 0, so they must not hold NaN
+      const bool clear = side == 1 && (there != all_pages || j0 + TM > len);
+      const uint32_t mb = tc::smem_u32(clear ? &bar.landed[sl] : &bar.full[sl]);
+      if (lane == 0) {
+        if (side == 0) *const_cast<volatile uint8_t*>(&sm.there[(tiles + i) % MASKS]) = (uint8_t)there;
+        pipe::expect_tx(mb, __popc(there) * DB * box);
       }
-      if (x == 0) {
+      __syncwarp();
+      if (pg < npp && id >= 0)
+        tma_load_3d(smem + sl * Lo::TILE + d * BLOCK_BYTES + pg * box, &P.kv, d * 64, hk * page,
+                    (int)((P.a.layer * 2 + side) * c.pages + id), mb);
+      if (clear && !post({sl, len - j0, there})) return false;
+      if (side == 0 && i == 0) {
         const gdnx_view& q = P.a.q;
         for (int b = 0; b < (g.pair ? 2 : 1); ++b) {
           if (g.last(b) < 0) continue;
-          if (!warp_wait(&bar.empty[b], ring.q_parity(b) ^ 1, abort_flag)) return;
+          if (!warp_wait(&bar.empty[b], ring.q_parity(b) ^ 1, abort_flag)) return false;
           const uint32_t to = smem + b * Lo::TILE, qb = tc::smem_u32(&bar.full[b]);
-          const int t0 = w.x.t0 + b * P.tb, row0 = w.s.start + t0;
+          const int t0 = w.t0 + b * P.tb, row0 = w.start + t0;
           if (P.tma_q) {
             if (lane == 0) {
               pipe::expect_tx(qb, DB * (uint32_t)(P.gs * P.tb) * 128);
 #pragma unroll
-              for (int e = 0; e < DB; ++e) tma_load_3d(to + e * BLOCK_BYTES, &P.q, e * 64, w.head0(), row0, qb);
+              for (int e = 0; e < DB; ++e) tma_load_3d(to + e * BLOCK_BYTES, &P.q, e * 64, w.head0, row0, qb);
             }
             __syncwarp();
           } else {
-            const int heads = w.heads(), n = min(P.tb, w.s.count - t0), D = (int)c.D;
+            const int heads = w.heads, n = min(P.tb, w.count - t0), D = (int)c.D;
             for (int y = lane; y < 128 * DB * 8; y += 32) {
-              const int row = y / (DB * 8), e = y % (DB * 8), t = row / P.gs, h = row % P.gs;
+              const int r = y / (DB * 8), e = y % (DB * 8), t = r / P.gs, h = r % P.gs;
               uint4 u = make_uint4(0, 0, 0, 0);
               if (t < n && h < heads && e * 8 < D) {
-                const uint16_t* src = static_cast<const uint16_t*>(q.ptr) + (int64_t)(row0 + t) * q.st + (w.head0() + h) * q.sh + e * 8;
+                const uint16_t* src = static_cast<const uint16_t*>(q.ptr) + (int64_t)(row0 + t) * q.st + (w.head0 + h) * q.sh + e * 8;
                 if (P.vec_q) {
                   u = *reinterpret_cast<const uint4*>(src);
                 } else {
@@ -587,7 +630,7 @@ GDNX_DEV void run_loads(const TcParams& P, const Share& share, uint8_t* base, ui
                   u.w = src[6] | (uint32_t)src[7] << 16;
                 }
               }
-              *reinterpret_cast<uint4*>(base + b * Lo::TILE + tc::sw128(row, e, 128)) = u;
+              *reinterpret_cast<uint4*>(base + b * Lo::TILE + tc::sw128(r, e, 128)) = u;
             }
             tc::fence_async_smem();
             __syncwarp();
@@ -595,8 +638,39 @@ GDNX_DEV void run_loads(const TcParams& P, const Share& share, uint8_t* base, ui
           }
         }
       }
-    }
+      return true;
+    };
+    if (!for_places(ring, g, load)) return;
     ring.end(2 * g.n, g.last0 >= 0, g.pair && g.last1 >= 0);
+    tiles += g.n;
+    __syncwarp();
+    if (lane == 0) pipe::mbar_arrive(&bar.item_empty[k % ITEMS]);
+  }
+  post({-1, 0, 0});
+}
+
+// The warp that clears rows of V.
+template <int DB>
+GDNX_DEV void run_clears(const TcParams& P, Small& sm, uint8_t* base) {
+  using Lo = Layout<DB>;
+  Bars& bar = sm.bar;
+  const int lane = threadIdx.x % 32, page = P.a.cache.page, e = lane % (8 * DB);
+  uint32_t bits = 0;  // a bit for each slot: the parity of its next clearing
+  for (uint32_t k = 0;; ++k) {
+    if (!warp_wait(&bar.job_full[k % JOBS], k / JOBS & 1, &sm.abort_flag)) return;
+    const Job j = sm.job[k % JOBS];
+    __syncwarp();
+    if (lane == 0) pipe::mbar_arrive(&bar.job_empty[k % JOBS]);
+    if (j.slot < 0) return;
+    if (!warp_wait(&bar.landed[j.slot], bits >> j.slot & 1, &sm.abort_flag)) return;
+    bits ^= 1u << j.slot;
+    for (int row = lane / (8 * DB); row < TM; row += 32 / (8 * DB)) {
+      if (row < j.end && (j.there >> (row / page) & 1)) continue;
+      *reinterpret_cast<uint4*>(base + j.slot * Lo::TILE + (e / 8) * BLOCK_BYTES + row * 128 + e % 8 * 16) = make_uint4(0, 0, 0, 0);
+    }
+    tc::fence_async_smem();
+    __syncwarp();
+    if (lane == 0) pipe::mbar_arrive(&bar.full[j.slot]);
   }
 }
 
@@ -615,6 +689,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
     for (int i = 0; i < Lo::SLOTS; ++i) {
       tc::mbar_init(&bar.full[i], 1);
       tc::mbar_init(&bar.empty[i], 1);
+      tc::mbar_init(&bar.landed[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      tc::mbar_init(&bar.item_full[i], 1);
+      tc::mbar_init(&bar.item_empty[i], 10);  // eight warps of rows, the products', the loads'
+      tc::mbar_init(&bar.job_full[i], 1);
+      tc::mbar_init(&bar.job_empty[i], 1);
     }
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(&bar.s_full[s], 1);
@@ -622,7 +703,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
       tc::mbar_init(&bar.p_ready[s][1], 128);
       tc::mbar_init(&bar.o_full[s], 1);
     }
-    tc::mbar_init(&bar.fix, 1);
     tc::mbar_init(&bar.done, 1);
     tc::mbar_init(&bar.left, 128);
     tc::mbar_init(&bar.joined, 128);
@@ -634,22 +714,25 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
   tc::fence_after();
   const uint32_t tmem = uniform(sm.tmem_at);
   if (smem % 1024) {  // never entered: the base is aligned
-  } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 224 + 128 x 56 is just that
-    regs_up<224>();
-    run_rows<DB, BF16>(P, sm.share, sm, tmem);
+  } else if (warp < 8) {  // 384 threads start with 168 registers each: 2 x 128 x 216 + 128 x 72 is just that
+    regs_up<216>();
+    run_rows<DB, BF16>(P, sm, tmem);
   } else {
-    regs_down<56>();
+    regs_down<72>();
     if (warp == 8) {
-      run_products<DB, BF16>(P, sm.share, smem, tmem, bar, abort_flag);
+      run_products<DB, BF16>(sm, smem, tmem);
       __syncwarp();
       if (elect_one()) tc::commit(&bar.done);  // every product issued has ended before tensor memory is freed
       tc::mbar_wait(&bar.done, 0);
     } else if (warp == 9) {
-      run_loads<DB>(P, sm.share, base, smem, bar, abort_flag);
+      run_loads<DB>(P, sm, base, smem);
       if (*abort_flag)  // let the copies in flight land
         for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
+    } else if (warp == 10) {
+      run_schedule(P, sm);
+      write_padding(P, threadIdx.x % 32, 32);
     } else {
-      write_padding(P, threadIdx.x - 320, 64);
+      run_clears<DB>(P, sm, base);
     }
   }
   __syncwarp();
