@@ -684,6 +684,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
   const uint32_t smem = uniform(tc::smem_u32(base));
   const int warp = uniform(threadIdx.x / 32);
   dependents_may_start();
+  if (threadIdx.x == 288) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&P.kv)) : "memory");
+    if (P.tma_q) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&P.q)) : "memory");
+  }
   if (threadIdx.x == 0) {
     *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
     for (int i = 0; i < Lo::SLOTS; ++i) {

@@ -4,21 +4,28 @@
 // tokens, then those with the largest scores, the lower page first among equals, `k` in all; they come in rising order.
 //
 // A score decides by comparison, so a rounding could change which page is taken: products and sums are in 64 bits
-// (exact products of 16-bit values, and sums whose error is far below the scores' distances), and score pages at 4
-// lanes a page with a fixed order of sums, so that equal pages have equal scores.  max(q lo, q hi) is q hi for q >= 0,
-// else q lo.  The scores are kept as 64-bit words that order alike: all ones for a page that is always taken, 0 for one
-// that the sequence does not hold.
+// (exact products of 16-bit values, and sums whose error is far below the scores' distances) with a fixed order of sums,
+// so that equal pages have equal scores.  max(q lo, q hi) is q hi for q >= 0, else q lo.  The scores are kept as 64-bit
+// words that order alike: all ones for a page that is always taken, 0 for one that the sequence does not hold.
 //
-// The k-th largest word is found bit by bit from the highest in which the words differ: a bit stays set where at least k
-// words lie at or above; the search ends as soon as just k do.
+// The 64-bit pipe bounds it.  A lane holds the queries of four dims in registers and reads 8 or 16 bytes of a page's
+// bounds; the sums of several pages and heads are reduced over the lanes together, each step handing half of them to
+// the lane's partner.  (With a page to four lanes and the queries in shared memory, the reads of these took 70 us for
+// 64 x 4 key heads of up to 256 pages; now MEASURED.)
+//
+// Of up to RANKED words each thread ranks one against all others.  Of more, the k-th largest is found two bits at a
+// time from the highest in which the words differ; the search ends as soon as just k lie at or above.
+#include <type_traits>
+
+#include "attn_tc.cuh"
 #include "paged_cache.cuh"
 
 namespace gdnx {
 namespace {
 
-constexpr int NT = 256;
-constexpr int LANES = 4;      // of a page
-constexpr int GH = 8;         // query heads that one reading of the bounds serves
+constexpr int NT = 256;         // threads of a CTA that scores
+constexpr int TAKE_NT = 1024;   // of one that only takes
+constexpr int RANKED = 256;
 constexpr int SMEM_KEYS = 24 * 1024;
 
 struct SelParams {
@@ -49,133 +56,205 @@ GDNX_DEV unsigned long long ordered(double x) {
   return u < 0 ? ~(unsigned long long)u : (unsigned long long)u | 0x8000000000000000ull;
 }
 
+// Four values of a row of bounds, as they lie and widened.
 template <typename T>
-struct Vec {
-  static constexpr int N = 16 / sizeof(T);
+struct Four {
+  uint2 u;
+  GDNX_DEV void clear() { u = make_uint2(0, 0); }
+  GDNX_DEV void load(const void* base, int64_t at) { u = *reinterpret_cast<const uint2*>(static_cast<const char*>(base) + at * 2); }
+  GDNX_DEV void widen(double (&x)[4]) const {
+    if constexpr (std::is_same<T, __half>::value) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+      x[0] = a.x;
+      x[1] = a.y;
+      x[2] = b.x;
+      x[3] = b.y;
+    } else {
+      x[0] = __uint_as_float(u.x << 16);
+      x[1] = __uint_as_float(u.x & 0xffff0000u);
+      x[2] = __uint_as_float(u.y << 16);
+      x[3] = __uint_as_float(u.y & 0xffff0000u);
+    }
+  }
 };
-GDNX_DEV void widen(float (&x)[4], uint4 u, float) {
-  x[0] = __uint_as_float(u.x);
-  x[1] = __uint_as_float(u.y);
-  x[2] = __uint_as_float(u.z);
-  x[3] = __uint_as_float(u.w);
-}
-GDNX_DEV void widen(float (&x)[8], uint4 u, __nv_bfloat16) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+template <>
+struct Four<float> {
+  float4 u;
+  GDNX_DEV void clear() { u = make_float4(0.f, 0.f, 0.f, 0.f); }
+  GDNX_DEV void load(const void* base, int64_t at) { u = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at); }
+  GDNX_DEV void widen(double (&x)[4]) const {
+    x[0] = u.x;
+    x[1] = u.y;
+    x[2] = u.z;
+    x[3] = u.w;
   }
-}
-GDNX_DEV void widen(float (&x)[8], uint4 u, __half) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-  }
-}
+};
 
-// The words of this CTA's pages x, x = first, first + stride, ... of NT / LANES at a time.
-template <typename T>
-GDNX_DEV void score_pages(const SelParams& P, const Query& q, int64_t b, int64_t hk, double (*qs)[128],
-                          unsigned long long* keys) {
+constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
+
+// The words of this CTA's share of the pages.  LANES lanes share a page, 32 / LANES pages lie side by side, and a warp
+// takes PB of these at a time; GH query heads at a time.
+template <typename T, int LANES, int GH>
+GDNX_DEV void score_pages(const SelParams& P, const Query& q, int64_t b, int64_t hk, unsigned long long* keys) {
+  constexpr int PB = GH == 1 ? 8 : 16 / GH, V = PB * GH, SIDE = 32 / LANES;
+  // of the sums' number v = page GH + head, the lane's upper bits are the upper ones, REST sums stay with a lane
+  constexpr int LV = log2_of(V), LG = log2_of(LANES), L = LV < LG ? LV : LG, REST = 1 << (LV - L);
+  static_assert(REST <= GH, "a lane's sums are one page's");
   const gdnx_paged_select_args& a = P.a;
   const gdnx_cache& c = a.cache;
-  const int G = (int)(a.H / c.Hk), D = (int)c.D, per = D / Vec<T>::N, lane = threadIdx.x % LANES;
-  const uint4* bounds = static_cast<const uint4*>(a.bounds);
+  const int G = (int)(a.H / c.Hk), D = (int)c.D, in = threadIdx.x % LANES, sub = threadIdx.x % 32 / LANES, d = in * 4;
   const int64_t lo0 = a.layer * 2 * c.pages, hi0 = lo0 + c.pages;
-  constexpr int STEP = NT / LANES;
+  const int32_t* table = c.table + (int64_t)q.row * c.width;
+  constexpr int STEP = NT / 32 * SIDE * PB;
   for (int g0 = 0; g0 < G; g0 += GH) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < GH * D; i += NT) {
-      const int g = i / D, d = i % D;
-      // a head that is not there repeats the first
-      qs[g][d] = ld_as_f32(a.q.ptr, a.q.dtype, b * a.q.sb + (hk * G + (g0 + g < G ? g0 + g : 0)) * a.q.sh + d);
-    }
-    __syncthreads();
-    for (int x0 = blockIdx.x * STEP; x0 < q.pages; x0 += P.splits * STEP) {
-      const int x = x0 + threadIdx.x / LANES;
-      const int p = x < q.pages ? c.table[(int64_t)q.row * c.width + x] : -1;
-      double s[GH];
+    double x[GH][4];
+    uint32_t minus = 0;  // a bit for each query value below 0
 #pragma unroll
-      for (int g = 0; g < GH; ++g) s[g] = 0.0;
-      if (page_ok(c, p)) {
-        const uint4* lo = bounds + ((lo0 + p) * c.Hk + hk) * per;
-        const uint4* hi = bounds + ((hi0 + p) * c.Hk + hk) * per;
-        for (int e = lane; e < per; e += LANES) {
-          float l[Vec<T>::N], h[Vec<T>::N];
-          widen(l, lo[e], T());
-          widen(h, hi[e], T());
+    for (int g = 0; g < GH; ++g)
 #pragma unroll
-          for (int i = 0; i < Vec<T>::N; ++i) {
-            const double dl = l[i], dh = h[i];
+      for (int i = 0; i < 4; ++i) {
+        // a head that is not there repeats the first; a dim that is not there counts nothing
+        const float v = d < D ? ld_as_f32(a.q.ptr, a.q.dtype, b * a.q.sb + (hk * G + (g0 + g < G ? g0 + g : 0)) * a.q.sh + d + i) : 0.f;
+        x[g][i] = v;
+        if (!(v >= 0.f)) minus |= 1u << (g * 4 + i);
+      }
+    for (int x0 = ((int)blockIdx.x * (NT / 32) + (int)threadIdx.x / 32) * SIDE * PB; x0 < q.pages; x0 += P.splits * STEP) {
+      int id[PB];
+      Four<T> lo[PB], hi[PB];
 #pragma unroll
-            for (int g = 0; g < GH; ++g) {
-              const double v = qs[g][e * Vec<T>::N + i];
-              s[g] = fma(v, v >= 0.0 ? dh : dl, s[g]);
+      for (int j = 0; j < PB; ++j) {
+        const int at = x0 + j * SIDE + sub;
+        id[j] = at < q.pages ? table[at] : -1;
+      }
+#pragma unroll
+      for (int j = 0; j < PB; ++j) {
+        lo[j].clear();
+        hi[j].clear();
+        if (page_ok(c, id[j]) && d < D) {
+          lo[j].load(a.bounds, ((lo0 + id[j]) * c.Hk + hk) * D + d);
+          hi[j].load(a.bounds, ((hi0 + id[j]) * c.Hk + hk) * D + d);
+        }
+      }
+      double s[V];
+#pragma unroll
+      for (int j = 0; j < PB; ++j) {
+        double l[4], h[4];
+        lo[j].widen(l);
+        hi[j].widen(h);
+#pragma unroll
+        for (int g = 0; g < GH; ++g) {
+          double t = x[g][0] * (minus >> (g * 4) & 1 ? l[0] : h[0]);
+#pragma unroll
+          for (int i = 1; i < 4; ++i) t = fma(x[g][i], minus >> (g * 4 + i) & 1 ? l[i] : h[i], t);
+          s[j * GH + g] = t;
+        }
+      }
+      int left = V;
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) {
+        if (left > 1) {
+          left /= 2;
+          const bool up = in & o;
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i)
+            if (i < left) {
+              const double give = up ? s[i] : s[i + left], keep = up ? s[i + left] : s[i];
+              s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
             }
-          }
+        } else {
+          s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
         }
       }
       unsigned long long key = 0;
 #pragma unroll
-      for (int g = 0; g < GH; ++g) {
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
-        const unsigned long long w = ordered(s[g]);
+      for (int i = 0; i < REST; ++i) {
+        const unsigned long long w = ordered(s[i]);
         key = w > key ? w : key;
       }
-      if (lane == 0 && x < q.pages) {
-        const int64_t at = (int64_t)x * c.page;
-        if (!page_ok(c, p)) key = 0;
-        else if (at < a.sinks || at + c.page > q.len - a.window) key = ~0ull;
-        else if (g0 > 0) key = key > keys[x] ? key : keys[x];
-        keys[x] = key;
+#pragma unroll
+      for (int n = REST, o = 1 << (LG - L); n < GH; n *= 2, o *= 2) {
+        const unsigned long long w = __shfl_xor_sync(0xffffffffu, key, o);
+        key = w > key ? w : key;
+      }
+      const int v = (in >> (LG - L)) << (LV - L), j = v / GH;
+      if (v % GH == 0 && (in & ((1 << (LG - L)) - 1)) == 0) {
+        const int at = x0 + j * SIDE + sub;
+        int p = -1;
+#pragma unroll
+        for (int e = 0; e < PB; ++e) p = e == j ? id[e] : p;
+        if (at < q.pages) {
+          const int64_t first = (int64_t)at * c.page;
+          if (!page_ok(c, p)) key = 0;
+          else if (first < a.sinks || first + c.page > q.len - a.window) key = ~0ull;
+          else if (g0 > 0) key = key > keys[at] ? key : keys[at];
+          keys[at] = key;
+        }
       }
     }
   }
 }
 
 // Exclusive prefix sum of 0 or 1 per thread over the CTA, and the total.
+template <int THREADS>
 GDNX_DEV int rank_of(bool on, int* warp_sums, int* total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const uint32_t bits = __ballot_sync(0xffffffffu, on);
   __syncthreads();
   if (lane == 0) warp_sums[warp] = __popc(bits);
   __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 32; ++i) {
-    before += i < warp ? warp_sums[i] : 0;
-    all += warp_sums[i];
-  }
-  *total = all;
-  return before + __popc(bits & ((1u << lane) - 1));
-}
-
-// f(word) summed over the n words, in every thread.
-template <typename F>
-GDNX_DEV int count_words(const unsigned long long* keys, int n, int* warp_sums, F f) {
-  int mine = 0;
-  for (int i = threadIdx.x; i < n; i += NT) mine += f(keys[i]);
-  mine = __reduce_add_sync(0xffffffffu, mine);
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) warp_sums[threadIdx.x / 32] = mine;
-  __syncthreads();
-  int all = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 32; ++i) all += warp_sums[i];
-  return all;
+  const int mine = lane < THREADS / 32 ? warp_sums[lane] : 0;
+  *total = __reduce_add_sync(0xffffffffu, mine);
+  return __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0) + __popc(bits & ((1u << lane) - 1));
 }
 
 // The k largest of n words (0: none), the lower index first among equals, in rising order; -1 behind them.
+template <int THREADS>
 GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t* out) {
-  __shared__ int sums[NT / 32];
-  __shared__ unsigned long long ends[2][NT / 32];
+  constexpr int WARPS = THREADS / 32;
+  static_assert(RANKED <= THREADS, "a word for each thread");
+  __shared__ int sums[2][3][WARPS];
+  __shared__ unsigned long long ends[2][WARPS];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  if (n <= RANKED) {
+    const unsigned long long w = (int)threadIdx.x < n ? keys[threadIdx.x] : 0;
+    int above = 0;
+    if (warp * 32 < n && n > k) {
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const unsigned long long x = keys[i];
+        above += x > w || (x == w && i < (int)threadIdx.x);
+      }
+    }
+    int all;
+    const bool on = w != 0 && above < k;
+    const int r = rank_of<THREADS>(on, sums[0][0], &all);
+    if (on) out[r] = (int)threadIdx.x;
+    for (int i = all + threadIdx.x; i < k; i += THREADS) out[i] = -1;
+    return;
+  }
+  // f(word): three truth values, counted over the n words, in every thread.  (Two places for the sums in turn: one
+  // barrier a count.)
+  int turn = 0;
+  const auto count = [&](auto f, int (&total)[3]) {
+    int mine[3] = {0, 0, 0};
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      bool on[3];
+      f(keys[i], on);
+#pragma unroll
+      for (int e = 0; e < 3; ++e) mine[e] += on[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+      const int s = __reduce_add_sync(0xffffffffu, mine[e]);
+      if (lane == 0) sums[turn][e][warp] = s;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 3; ++e) total[e] = __reduce_add_sync(0xffffffffu, lane < WARPS ? sums[turn][e][lane] : 0);
+    turn ^= 1;
+  };
   unsigned long long least = ~0ull, most = 0;
-  for (int i = threadIdx.x; i < n; i += NT) {
+  for (int i = threadIdx.x; i < n; i += THREADS) {
     const unsigned long long w = keys[i];
     if (w == 0) continue;
     least = w < least ? w : least;
@@ -187,70 +266,103 @@ GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t
     least = x < least ? x : least;
     most = y > most ? y : most;
   }
-  if (threadIdx.x % 32 == 0) {
-    ends[0][threadIdx.x / 32] = least;
-    ends[1][threadIdx.x / 32] = most;
+  if (lane == 0) {
+    ends[0][warp] = least;
+    ends[1][warp] = most;
   }
-  const int there = count_words(keys, n, sums, [](unsigned long long w) { return w != 0; });  // synchronises
-#pragma unroll
-  for (int i = 0; i < NT / 32; ++i) {
-    least = ends[0][i] < least ? ends[0][i] : least;
-    most = ends[1][i] > most ? ends[1][i] : most;
-  }
+  int got[3];
+  // words that are there, and those always taken (which the search leaves out: they differ in the highest bits)
+  count([](unsigned long long w, bool (&on)[3]) { on[0] = w != 0; on[1] = w == ~0ull; on[2] = false; }, got);
+  const int there = got[0], always = got[1];
   unsigned long long bar = 1;  // at least this is taken
   int above = there;           // words at or above it
-  if (there > k) {
+  if (there > k && always >= k) {
+    bar = ~0ull;
+    above = always;
+  } else if (there > k) {
+    // the ends of the others: all ones are above them all
+    unsigned long long top_word = 0;
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      const unsigned long long w = keys[i];
+      if (w != ~0ull && w > top_word) top_word = w;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long y = __shfl_xor_sync(0xffffffffu, top_word, o);
+      top_word = y > top_word ? y : top_word;
+    }
+    __syncthreads();  // the ends have been written
+    least = ends[0][0];
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) least = ends[0][i] < least ? ends[0][i] : least;
+    __syncthreads();
+    if (lane == 0) ends[1][warp] = top_word;
+    __syncthreads();
+    most = ends[1][0];
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) most = ends[1][i] > most ? ends[1][i] : most;
     const int top = least == most ? -1 : 63 - __clzll(least ^ most);
     bar = top < 0 ? most : most >> top >> 1 << top << 1;
-    for (int bit = top; bit >= 0 && above != k; --bit) {
-      const unsigned long long t = bar | 1ull << bit;
-      const int m = count_words(keys, n, sums, [=](unsigned long long w) { return w >= t; });
-      if (m >= k) {
-        bar = t;
-        above = m;
+    for (int bit = top; bit >= 0 && above != k; bit -= 2) {
+      // the two bits bit, bit - 1 (the last may be one bit alone)
+      const int low = bit > 0 ? bit - 1 : 0;
+      const unsigned long long one = 1ull << low;
+      const unsigned long long t1 = bar + one, t2 = bit > 0 ? bar + 2 * one : t1, t3 = bit > 0 ? bar + 3 * one : t1;
+      count([=](unsigned long long w, bool (&on)[3]) { on[0] = w >= t1; on[1] = w >= t2; on[2] = w >= t3; }, got);
+      if (got[2] >= k) {
+        bar = t3;
+        above = got[2];
+      } else if (got[1] >= k) {
+        bar = t2;
+        above = got[1];
+      } else if (got[0] >= k) {
+        bar = t1;
+        above = got[0];
       }
     }
   }
   // of the words equal to the bar, the first ones
   int equal = n;
-  if (above > k) equal = k - count_words(keys, n, sums, [=](unsigned long long w) { return w > bar; });
+  if (above > k) {
+    count([=](unsigned long long w, bool (&on)[3]) { on[0] = w > bar; on[1] = on[2] = false; }, got);
+    equal = k - got[0];
+  }
   int taken = 0, ties = 0;
-  for (int i0 = 0; i0 < n && taken < k; i0 += NT) {
+  for (int i0 = 0; i0 < n && taken < k; i0 += THREADS) {
     const int i = i0 + threadIdx.x;
     const unsigned long long w = i < n ? keys[i] : 0;
     int all;
     bool on = w >= bar;
     if (above > k) {
-      const int r = rank_of(w == bar, sums, &all);
+      const int r = rank_of<THREADS>(w == bar, sums[0][0], &all);
       if (w == bar) on = ties + r < equal;
       ties += all;
     }
-    const int r = rank_of(on, sums, &all);
+    const int r = rank_of<THREADS>(on, sums[1][0], &all);
     if (on) out[taken + r] = i;
     taken += all;
   }
-  for (int i = taken + threadIdx.x; i < k; i += NT) out[i] = -1;
+  for (int i = taken + threadIdx.x; i < k; i += THREADS) out[i] = -1;
 }
 
 // FUSED: one CTA for each query and key head scores its pages and takes the largest; else CTA (x, unit) leaves the
 // words of its share of the pages to the next kernel.
-template <typename T, bool FUSED>
+template <typename T, int LANES, int GH, bool FUSED>
 __global__ void __launch_bounds__(NT) paged_select_kernel(const SelParams P) {
   extern __shared__ unsigned long long words[];
-  __shared__ double qs[GH][128];
   dependents_may_start();
   wait_for_earlier();
   const int64_t unit = blockIdx.y + (int64_t)blockIdx.z * gridDim.y, Hk = P.a.cache.Hk;
   if (unit >= P.a.B * Hk) return;
   const Query q = query_of(P.a, unit / Hk);
   unsigned long long* keys = FUSED ? words : P.keys + unit * P.a.cache.width;
-  score_pages<T>(P, q, unit / Hk, unit % Hk, qs, keys);
+  score_pages<T, LANES, GH>(P, q, unit / Hk, unit % Hk, keys);
   if (!FUSED) return;
   __syncthreads();
-  take_largest(keys, q.pages, (int)P.a.k, P.a.selected + unit * P.a.k);
+  take_largest<NT>(keys, q.pages, (int)P.a.k, P.a.selected + unit * P.a.k);
 }
 
-__global__ void __launch_bounds__(NT) paged_take_kernel(const SelParams P) {
+__global__ void __launch_bounds__(TAKE_NT) paged_take_kernel(const SelParams P) {
   extern __shared__ unsigned long long words[];
   dependents_may_start();
   wait_for_earlier();
@@ -258,11 +370,11 @@ __global__ void __launch_bounds__(NT) paged_take_kernel(const SelParams P) {
   const Query q = query_of(P.a, unit / Hk);
   const unsigned long long* keys = P.keys + unit * P.a.cache.width;
   if (q.pages <= SMEM_KEYS) {
-    for (int i = threadIdx.x; i < q.pages; i += NT) words[i] = keys[i];
+    for (int i = threadIdx.x; i < q.pages; i += TAKE_NT) words[i] = keys[i];
     __syncthreads();
     keys = words;
   }
-  take_largest(keys, q.pages, (int)P.a.k, P.a.selected + unit * P.a.k);
+  take_largest<TAKE_NT>(keys, q.pages, (int)P.a.k, P.a.selected + unit * P.a.k);
 }
 
 // Pages that a sequence can have.
@@ -274,32 +386,41 @@ int64_t most_pages(const gdnx_paged_select_args& a) {
 // One kernel does both where the query heads fill the device by themselves, or have few pages each.
 bool fused(const gdnx_paged_select_args& a) {
   const int64_t n = most_pages(a);
-  return a.cache.width <= SMEM_KEYS && (a.B * a.cache.Hk >= sm_count() || n <= 4 * NT / LANES);
+  return a.cache.width <= SMEM_KEYS && (a.B * a.cache.Hk >= sm_count() || n <= RANKED);
 }
 
-template <typename F>
-bool allow(F kernel, size_t bytes) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess) return true;
-  cudaGetLastError();
-  return false;
-}
-
-template <typename T>
+template <typename T, int LANES, int GH>
 gdnx_status select_of(const gdnx_paged_select_args& a, cudaStream_t st) {
+  static std::atomic<uint64_t> done[2];
   const int64_t units = a.B * a.cache.Hk, n = most_pages(a);
   SelParams P = {a, static_cast<unsigned long long*>(a.workspace), 1};
   const unsigned y = (unsigned)(units < 65535 ? units : 65535), z = (unsigned)((units + y - 1) / y);
   const size_t bytes = (size_t)(a.cache.width < SMEM_KEYS ? a.cache.width : SMEM_KEYS) * 8;
   if (fused(a)) {
-    if (!allow(paged_select_kernel<T, true>, SMEM_KEYS * 8)) return GDNX_ELAUNCH;
-    return launched(launch_early(paged_select_kernel<T, true>, dim3(1, y, z), dim3(NT), bytes, st, P));
+    const auto kernel = paged_select_kernel<T, LANES, GH, true>;
+    if (bytes > 32 * 1024 && !attn::allow_smem(kernel, SMEM_KEYS * 8, done[0])) return GDNX_ELAUNCH;
+    return launched(launch_early(kernel, dim3(1, y, z), dim3(NT), bytes, st, P));
   }
-  const int64_t want = ((int64_t)sm_count() * 4 + units - 1) / units, have = (n + NT / LANES - 1) / (NT / LANES);
+  // CTAs that fill the device four times over, of a batch of pages for each warp at least
+  constexpr int64_t STEP = NT / LANES * (GH == 1 ? 8 : 16 / GH);
+  const int64_t want = ((int64_t)sm_count() * 4 + units - 1) / units, have = (n + STEP - 1) / STEP;
   P.splits = (int)(want < have ? want : have);
-  if (launch_early(paged_select_kernel<T, false>, dim3((unsigned)P.splits, y, z), dim3(NT), 0, st, P) != cudaSuccess)
+  if (launch_early(paged_select_kernel<T, LANES, GH, false>, dim3((unsigned)P.splits, y, z), dim3(NT), 0, st, P) != cudaSuccess)
     return GDNX_ELAUNCH;
-  if (!allow(paged_take_kernel, SMEM_KEYS * 8)) return GDNX_ELAUNCH;
-  return launched(launch_early(paged_take_kernel, dim3((unsigned)units), dim3(NT), bytes, st, P));
+  if (bytes > 32 * 1024 && !attn::allow_smem(paged_take_kernel, SMEM_KEYS * 8, done[1])) return GDNX_ELAUNCH;
+  return launched(launch_early(paged_take_kernel, dim3((unsigned)units), dim3(TAKE_NT), bytes, st, P));
+}
+
+template <typename T, int LANES>
+gdnx_status select_heads(const gdnx_paged_select_args& a, cudaStream_t st) {
+  const int64_t G = a.H / a.cache.Hk;
+  return G == 1 ? select_of<T, LANES, 1>(a, st) : G <= 4 ? select_of<T, LANES, 4>(a, st) : select_of<T, LANES, 8>(a, st);
+}
+
+template <typename T>
+gdnx_status select_type(const gdnx_paged_select_args& a, cudaStream_t st) {
+  const int64_t D = a.cache.D;
+  return D > 64 ? select_heads<T, 32>(a, st) : D > 32 ? select_heads<T, 16>(a, st) : select_heads<T, 8>(a, st);
 }
 
 }  // namespace
@@ -310,9 +431,9 @@ size_t paged_select_workspace_bytes(const gdnx_paged_select_args& a) {
 
 gdnx_status launch_paged_select(const gdnx_paged_select_args& a, cudaStream_t st) {
   switch (a.cache.dtype) {
-    case GDNX_BF16: return select_of<__nv_bfloat16>(a, st);
-    case GDNX_F16: return select_of<__half>(a, st);
-    default: return select_of<float>(a, st);
+    case GDNX_BF16: return select_type<__nv_bfloat16>(a, st);
+    case GDNX_F16: return select_type<__half>(a, st);
+    default: return select_type<float>(a, st);
   }
 }
 
