@@ -14,7 +14,8 @@
 // 64 x 4 key heads of up to 256 pages; now MEASURED.)
 //
 // Of up to RANKED words each thread ranks one against all others.  Of more, the k-th largest is found two bits at a
-// time from the highest in which the words differ; the search ends as soon as just k lie at or above.
+// time among their places between the least and the greatest, in 32 bits from registers; the search ends as soon as just
+// k lie at or above, and goes on in 64 bits where places fall together.
 #include <type_traits>
 
 #include "attn_tc.cuh"
@@ -32,6 +33,7 @@ struct SelParams {
   gdnx_paged_select_args a;
   unsigned long long* keys;  // [B, Hk, width]; null: the words stay in shared memory
   int splits;                // CTAs that share a query head's pages
+  int vec_q;                 // four values of q lie aligned
 };
 
 struct Query {
@@ -62,6 +64,10 @@ struct Four {
   uint2 u;
   GDNX_DEV void clear() { u = make_uint2(0, 0); }
   GDNX_DEV void load(const void* base, int64_t at) { u = *reinterpret_cast<const uint2*>(static_cast<const char*>(base) + at * 2); }
+  GDNX_DEV void gather(const void* base, int64_t at) {  // not aligned
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    u = make_uint2(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16);
+  }
   GDNX_DEV void widen(double (&x)[4]) const {
     if constexpr (std::is_same<T, __half>::value) {
       const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
@@ -82,6 +88,10 @@ struct Four<float> {
   float4 u;
   GDNX_DEV void clear() { u = make_float4(0.f, 0.f, 0.f, 0.f); }
   GDNX_DEV void load(const void* base, int64_t at) { u = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at); }
+  GDNX_DEV void gather(const void* base, int64_t at) {
+    const float* p = static_cast<const float*>(base) + at;
+    u = make_float4(p[0], p[1], p[2], p[3]);
+  }
   GDNX_DEV void widen(double (&x)[4]) const {
     x[0] = u.x;
     x[1] = u.y;
@@ -110,14 +120,18 @@ GDNX_DEV void score_pages(const SelParams& P, const Query& q, int64_t b, int64_t
     double x[GH][4];
     uint32_t minus = 0;  // a bit for each query value below 0
 #pragma unroll
-    for (int g = 0; g < GH; ++g)
+    for (int g = 0; g < GH; ++g) {
+      // a head that is not there repeats the first; a dim that is not there counts nothing
+      const int64_t at = b * a.q.sb + (hk * G + (g0 + g < G ? g0 + g : 0)) * a.q.sh + d;
+      Four<T> w;
+      w.clear();
+      if (d < D && P.vec_q) w.load(a.q.ptr, at);
+      else if (d < D) w.gather(a.q.ptr, at);
+      w.widen(x[g]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // a head that is not there repeats the first; a dim that is not there counts nothing
-        const float v = d < D ? ld_as_f32(a.q.ptr, a.q.dtype, b * a.q.sb + (hk * G + (g0 + g < G ? g0 + g : 0)) * a.q.sh + d + i) : 0.f;
-        x[g][i] = v;
-        if (!(v >= 0.f)) minus |= 1u << (g * 4 + i);
-      }
+      for (int i = 0; i < 4; ++i)
+        if (!(x[g][i] >= 0.0)) minus |= 1u << (g * 4 + i);
+    }
     for (int x0 = ((int)blockIdx.x * (NT / 32) + (int)threadIdx.x / 32) * SIDE * PB; x0 < q.pages; x0 += P.splits * STEP) {
       int id[PB];
       Four<T> lo[PB], hi[PB];
@@ -210,7 +224,7 @@ GDNX_DEV int rank_of(bool on, int* warp_sums, int* total) {
 // The k largest of n words (0: none), the lower index first among equals, in rising order; -1 behind them.
 template <int THREADS>
 GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t* out) {
-  constexpr int WARPS = THREADS / 32;
+  constexpr int WARPS = THREADS / 32, HELD = 8;
   static_assert(RANKED <= THREADS, "a word for each thread");
   __shared__ int sums[2][3][WARPS];
   __shared__ unsigned long long ends[2][WARPS];
@@ -219,11 +233,14 @@ GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t
     const unsigned long long w = (int)threadIdx.x < n ? keys[threadIdx.x] : 0;
     int above = 0;
     if (warp * 32 < n && n > k) {
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const unsigned long long x = keys[i];
-        above += x > w || (x == w && i < (int)threadIdx.x);
-      }
+      // those before this warp's words go first among equals, those behind them do not
+      const int a0 = warp * 32, a1 = min(a0 + 32, n);
+#pragma unroll 8
+      for (int i = 0; i < a0; ++i) above += keys[i] >= w;
+#pragma unroll 8
+      for (int i = a0; i < a1; ++i) above += keys[i] > w || (keys[i] == w && i < (int)threadIdx.x);
+#pragma unroll 8
+      for (int i = a1; i < n; ++i) above += keys[i] > w;
     }
     int all;
     const bool on = w != 0 && above < k;
@@ -232,31 +249,14 @@ GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t
     for (int i = all + threadIdx.x; i < k; i += THREADS) out[i] = -1;
     return;
   }
-  // f(word): three truth values, counted over the n words, in every thread.  (Two places for the sums in turn: one
-  // barrier a count.)
-  int turn = 0;
-  const auto count = [&](auto f, int (&total)[3]) {
-    int mine[3] = {0, 0, 0};
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-      bool on[3];
-      f(keys[i], on);
-#pragma unroll
-      for (int e = 0; e < 3; ++e) mine[e] += on[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 3; ++e) {
-      const int s = __reduce_add_sync(0xffffffffu, mine[e]);
-      if (lane == 0) sums[turn][e][warp] = s;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 3; ++e) total[e] = __reduce_add_sync(0xffffffffu, lane < WARPS ? sums[turn][e][lane] : 0);
-    turn ^= 1;
-  };
+  // The ends of the words that are there and not taken always, and the numbers of both.
   unsigned long long least = ~0ull, most = 0;
+  int there = 0, always = 0;
   for (int i = threadIdx.x; i < n; i += THREADS) {
     const unsigned long long w = keys[i];
-    if (w == 0) continue;
+    there += w != 0;
+    always += w == ~0ull;
+    if (w == 0 || w == ~0ull) continue;
     least = w < least ? w : least;
     most = w > most ? w : most;
   }
@@ -266,76 +266,108 @@ GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t
     least = x < least ? x : least;
     most = y > most ? y : most;
   }
+  there = __reduce_add_sync(0xffffffffu, there);
+  always = __reduce_add_sync(0xffffffffu, always);
   if (lane == 0) {
     ends[0][warp] = least;
     ends[1][warp] = most;
+    sums[1][0][warp] = there;
+    sums[1][1][warp] = always;
   }
-  int got[3];
-  // words that are there, and those always taken (which the search leaves out: they differ in the highest bits)
-  count([](unsigned long long w, bool (&on)[3]) { on[0] = w != 0; on[1] = w == ~0ull; on[2] = false; }, got);
-  const int there = got[0], always = got[1];
-  unsigned long long bar = 1;  // at least this is taken
-  int above = there;           // words at or above it
-  if (there > k && always >= k) {
-    bar = ~0ull;
-    above = always;
-  } else if (there > k) {
-    // the ends of the others: all ones are above them all
-    unsigned long long top_word = 0;
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-      const unsigned long long w = keys[i];
-      if (w != ~0ull && w > top_word) top_word = w;
+  __syncthreads();
+  there = always = 0;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) {
+    least = ends[0][i] < least ? ends[0][i] : least;
+    most = ends[1][i] > most ? ends[1][i] : most;
+    there += sums[1][0][i];
+    always += sums[1][1][i];
+  }
+  // A word's place between the ends in 32 bits: 0 for one that is not there, all ones for one always taken.  The
+  // first words' places stay in registers.
+  const int shift = most > least ? max(0, 33 - __clzll(most - least)) : 0;
+  const auto place = [&](unsigned long long w) {
+    return w == 0 ? 0u : w == ~0ull ? 0xffffffffu : (uint32_t)((w - least) >> shift) + 1;
+  };
+  uint32_t held[HELD];
+#pragma unroll
+  for (int e = 0; e < HELD; ++e) {
+    const int i = e * THREADS + threadIdx.x;
+    held[e] = i < n ? place(keys[i]) : 0;
+  }
+  // Words whose place is at least t + 1, + 2, + 3 times `one`, in every thread.  (Two places for the sums in turn: one
+  // barrier a count.)
+  int turn = 0;
+  const auto total = [&](int (&mine)[3]) {
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+      const int s = __reduce_add_sync(0xffffffffu, mine[e]);
+      if (lane == 0) sums[turn][e][warp] = s;
     }
+    __syncthreads();
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long y = __shfl_xor_sync(0xffffffffu, top_word, o);
-      top_word = y > top_word ? y : top_word;
+    for (int e = 0; e < 3; ++e) mine[e] = __reduce_add_sync(0xffffffffu, lane < WARPS ? sums[turn][e][lane] : 0);
+    turn ^= 1;
+  };
+  uint32_t bar = 1;   // places from here on are taken
+  int above = there;  // words there
+  if (there > k) {
+    bar = 0;
+    above = n;
+    for (int bit = 30; bit >= 0 && above != k; bit -= 2) {
+      int got[3] = {0, 0, 0};
+      const auto look = [&](uint32_t w) {
+#pragma unroll
+        for (int e = 0; e < 3; ++e) got[e] += w >= bar + ((uint32_t)(e + 1) << bit);
+      };
+#pragma unroll
+      for (int e = 0; e < HELD; ++e) look(held[e]);
+      for (int i = HELD * THREADS + threadIdx.x; i < n; i += THREADS) look(place(keys[i]));
+      total(got);
+#pragma unroll
+      for (int e = 2; e >= 0; --e)
+        if (got[e] >= k) {
+          bar += (uint32_t)(e + 1) << bit;
+          above = got[e];
+          break;
+        }
     }
-    __syncthreads();  // the ends have been written
-    least = ends[0][0];
-#pragma unroll
-    for (int i = 1; i < WARPS; ++i) least = ends[0][i] < least ? ends[0][i] : least;
-    __syncthreads();
-    if (lane == 0) ends[1][warp] = top_word;
-    __syncthreads();
-    most = ends[1][0];
-#pragma unroll
-    for (int i = 1; i < WARPS; ++i) most = ends[1][i] > most ? ends[1][i] : most;
-    const int top = least == most ? -1 : 63 - __clzll(least ^ most);
-    bar = top < 0 ? most : most >> top >> 1 << top << 1;
-    for (int bit = top; bit >= 0 && above != k; bit -= 2) {
-      // the two bits bit, bit - 1 (the last may be one bit alone)
-      const int low = bit > 0 ? bit - 1 : 0;
-      const unsigned long long one = 1ull << low;
-      const unsigned long long t1 = bar + one, t2 = bit > 0 ? bar + 2 * one : t1, t3 = bit > 0 ? bar + 3 * one : t1;
-      count([=](unsigned long long w, bool (&on)[3]) { on[0] = w >= t1; on[1] = w >= t2; on[2] = w >= t3; }, got);
-      if (got[2] >= k) {
-        bar = t3;
-        above = got[2];
-      } else if (got[1] >= k) {
-        bar = t2;
-        above = got[1];
-      } else if (got[0] >= k) {
-        bar = t1;
+  }
+  // More than k at or above: those at the bar itself are told apart by what their places leave out.
+  unsigned long long edge = 0;  // of the words at the bar's place, those from here on
+  if (above > k && shift > 0) {
+    edge = least + ((unsigned long long)(bar - 1) << shift);
+    for (int bit = shift - 1; bit >= 0; --bit) {
+      int got[3] = {0, 0, 0};
+      for (int i = threadIdx.x; i < n; i += THREADS) got[0] += keys[i] >= edge + (1ull << bit);
+      total(got);
+      if (got[0] >= k) {
+        edge += 1ull << bit;
         above = got[0];
+        if (above == k) break;
       }
     }
   }
-  // of the words equal to the bar, the first ones
+  // Of the words equal to the last that is taken, the first ones.
+  const auto taken_from = [&](unsigned long long w, uint32_t p) { return edge ? w >= edge : p >= bar; };
   int equal = n;
   if (above > k) {
-    count([=](unsigned long long w, bool (&on)[3]) { on[0] = w > bar; on[1] = on[2] = false; }, got);
+    int got[3] = {0, 0, 0};
+    for (int i = threadIdx.x; i < n; i += THREADS) got[0] += edge ? keys[i] > edge : place(keys[i]) > bar;
+    total(got);
     equal = k - got[0];
   }
   int taken = 0, ties = 0;
   for (int i0 = 0; i0 < n && taken < k; i0 += THREADS) {
     const int i = i0 + threadIdx.x;
     const unsigned long long w = i < n ? keys[i] : 0;
+    const uint32_t p = place(w);
     int all;
-    bool on = w >= bar;
+    bool on = i < n && w != 0 && taken_from(w, p);
     if (above > k) {
-      const int r = rank_of<THREADS>(w == bar, sums[0][0], &all);
-      if (w == bar) on = ties + r < equal;
+      const bool same = on && (edge ? w == edge : p == bar);
+      const int r = rank_of<THREADS>(same, sums[0][0], &all);
+      if (same) on = ties + r < equal;
       ties += all;
     }
     const int r = rank_of<THREADS>(on, sums[1][0], &all);
@@ -393,7 +425,9 @@ template <typename T, int LANES, int GH>
 gdnx_status select_of(const gdnx_paged_select_args& a, cudaStream_t st) {
   static std::atomic<uint64_t> done[2];
   const int64_t units = a.B * a.cache.Hk, n = most_pages(a);
-  SelParams P = {a, static_cast<unsigned long long*>(a.workspace), 1};
+  const size_t four = 4 * sizeof(T);
+  SelParams P = {a, static_cast<unsigned long long*>(a.workspace), 1,
+                 reinterpret_cast<uintptr_t>(a.q.ptr) % four == 0 && a.q.sb % 4 == 0 && a.q.sh % 4 == 0};
   const unsigned y = (unsigned)(units < 65535 ? units : 65535), z = (unsigned)((units + y - 1) / y);
   const size_t bytes = (size_t)(a.cache.width < SMEM_KEYS ? a.cache.width : SMEM_KEYS) * 8;
   if (fused(a)) {
@@ -401,9 +435,9 @@ gdnx_status select_of(const gdnx_paged_select_args& a, cudaStream_t st) {
     if (bytes > 32 * 1024 && !attn::allow_smem(kernel, SMEM_KEYS * 8, done[0])) return GDNX_ELAUNCH;
     return launched(launch_early(kernel, dim3(1, y, z), dim3(NT), bytes, st, P));
   }
-  // CTAs that fill the device four times over, of a batch of pages for each warp at least
-  constexpr int64_t STEP = NT / LANES * (GH == 1 ? 8 : 16 / GH);
-  const int64_t want = ((int64_t)sm_count() * 4 + units - 1) / units, have = (n + STEP - 1) / STEP;
+  // CTAs that fill the device twice over, of two batches of pages for each warp at least: reading q costs about one
+  constexpr int64_t STEP = 2 * NT / LANES * (GH == 1 ? 8 : 16 / GH);
+  const int64_t want = ((int64_t)sm_count() * 2 + units - 1) / units, have = (n + STEP - 1) / STEP;
   P.splits = (int)(want < have ? want : have);
   if (launch_early(paged_select_kernel<T, LANES, GH, false>, dim3((unsigned)P.splits, y, z), dim3(NT), 0, st, P) != cudaSuccess)
     return GDNX_ELAUNCH;
