@@ -8,7 +8,7 @@
 // so that equal pages have equal scores.  max(q lo, q hi) is q hi for q >= 0, else q lo.  The scores are kept as 64-bit
 // words that order alike: all ones for a page that is always taken, 0 for one that the sequence does not hold.
 //
-// The 64-bit pipe bounds it.  A lane holds the queries of four dims in registers and reads 8 or 16 bytes of a page's
+// Issue slots bound it.  A lane holds the queries of four dims in registers and reads 8 or 16 bytes of a page's
 // bounds; the sums of several pages and heads are reduced over the lanes together, each step handing half of them to
 // the lane's partner.  (With a page to four lanes and the queries in shared memory, the reads of these took 70 us for
 // 64 x 4 key heads of up to 256 pages; now MEASURED.)
@@ -115,10 +115,14 @@ GDNX_DEV void score_pages(const SelParams& P, const Query& q, int64_t b, int64_t
   const int G = (int)(a.H / c.Hk), D = (int)c.D, in = threadIdx.x % LANES, sub = threadIdx.x % 32 / LANES, d = in * 4;
   const int64_t lo0 = a.layer * 2 * c.pages, hi0 = lo0 + c.pages;
   const int32_t* table = c.table + (int64_t)q.row * c.width;
-  constexpr int STEP = NT / 32 * SIDE * PB;
+  constexpr int BATCH = SIDE * PB;
+  static_assert(32 % BATCH == 0, "a batch's ids lie in one reading");
+  // the warp's pages r0..r1-1: an even share in whole batches
+  const int lane = threadIdx.x % 32, warps = P.splits * (NT / 32), warp = (int)blockIdx.x * (NT / 32) + (int)threadIdx.x / 32;
+  const int share = ((q.pages + BATCH - 1) / BATCH + warps - 1) / warps * BATCH;
+  const int r0 = min(warp * share, q.pages), r1 = min(r0 + share, q.pages);
   for (int g0 = 0; g0 < G; g0 += GH) {
-    double x[GH][4];
-    uint32_t minus = 0;  // a bit for each query value below 0
+    double up[GH][4], dn[GH][4];  // the queries' values from 0 on (the others 0), and those below
 #pragma unroll
     for (int g = 0; g < GH; ++g) {
       // a head that is not there repeats the first; a dim that is not there counts nothing
@@ -127,58 +131,87 @@ GDNX_DEV void score_pages(const SelParams& P, const Query& q, int64_t b, int64_t
       w.clear();
       if (d < D && P.vec_q) w.load(a.q.ptr, at);
       else if (d < D) w.gather(a.q.ptr, at);
-      w.widen(x[g]);
+      double x[4];
+      w.widen(x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!(x[g][i] >= 0.0)) minus |= 1u << (g * 4 + i);
+      for (int i = 0; i < 4; ++i) {
+        up[g][i] = x[i] >= 0.0 ? x[i] : 0.0;
+        dn[g][i] = x[i] >= 0.0 ? 0.0 : x[i];
+      }
     }
-    for (int x0 = ((int)blockIdx.x * (NT / 32) + (int)threadIdx.x / 32) * SIDE * PB; x0 < q.pages; x0 += P.splits * STEP) {
-      int id[PB];
-      Four<T> lo[PB], hi[PB];
-#pragma unroll
-      for (int j = 0; j < PB; ++j) {
-        const int at = x0 + j * SIDE + sub;
-        id[j] = at < q.pages ? table[at] : -1;
+    // ids of 32 of the warp's pages, a lane's each, and of the 32 behind them; bounds of a batch, read one ahead
+    const auto read = [&](int x) { return x + lane < r1 ? table[x + lane] : -1; };
+    int base = r0, ids = read(r0), more = read(r0 + 32);
+    int id[PB], next_id[PB];
+    Four<T> lo[PB], hi[PB], next_lo[PB], next_hi[PB];
+    const auto fetch = [&](int x0) {
+      if (x0 >= base + 32) {
+        base += 32;
+        ids = more;
+        more = read(base + 32);
       }
 #pragma unroll
       for (int j = 0; j < PB; ++j) {
-        lo[j].clear();
-        hi[j].clear();
-        if (page_ok(c, id[j]) && d < D) {
-          lo[j].load(a.bounds, ((lo0 + id[j]) * c.Hk + hk) * D + d);
-          hi[j].load(a.bounds, ((hi0 + id[j]) * c.Hk + hk) * D + d);
+        next_id[j] = __shfl_sync(0xffffffffu, ids, (x0 - base + j * SIDE + sub) & 31);
+        next_lo[j].clear();
+        next_hi[j].clear();
+        if (page_ok(c, next_id[j]) && d < D) {
+          next_lo[j].load(a.bounds, ((lo0 + next_id[j]) * c.Hk + hk) * D + d);
+          next_hi[j].load(a.bounds, ((hi0 + next_id[j]) * c.Hk + hk) * D + d);
         }
       }
+    };
+    if (r0 < r1) fetch(r0);
+    for (int x0 = r0; x0 < r1; x0 += BATCH) {
+#pragma unroll
+      for (int j = 0; j < PB; ++j) {
+        id[j] = next_id[j];
+        lo[j] = next_lo[j];
+        hi[j] = next_hi[j];
+      }
+      if (x0 + BATCH < r1) fetch(x0 + BATCH);
       double s[V];
+      const auto sum = [&](auto term) {
 #pragma unroll
-      for (int j = 0; j < PB; ++j) {
-        double l[4], h[4];
-        lo[j].widen(l);
-        hi[j].widen(h);
+        for (int j = 0; j < PB; ++j) {
+          double l[4], h[4];
+          lo[j].widen(l);
+          hi[j].widen(h);
 #pragma unroll
-        for (int g = 0; g < GH; ++g) {
-          double t = x[g][0] * (minus >> (g * 4) & 1 ? l[0] : h[0]);
+          for (int g = 0; g < GH; ++g) {
+            double t = 0.0;
 #pragma unroll
-          for (int i = 1; i < 4; ++i) t = fma(x[g][i], minus >> (g * 4 + i) & 1 ? l[i] : h[i], t);
-          s[j * GH + g] = t;
+            for (int i = 0; i < 4; ++i) t = term(t, g, i, l[i], h[i]);
+            s[j * GH + g] = t;
+          }
         }
-      }
-      int left = V;
+        int left = V;
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) {
-        if (left > 1) {
-          left /= 2;
-          const bool up = in & o;
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+          if (left > 1) {
+            left /= 2;
+            const bool upper = in & o;
 #pragma unroll
-          for (int i = 0; i < V / 2; ++i)
-            if (i < left) {
-              const double give = up ? s[i] : s[i + left], keep = up ? s[i + left] : s[i];
-              s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-            }
-        } else {
-          s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+            for (int i = 0; i < V / 2; ++i)
+              if (i < left) {
+                const double give = upper ? s[i] : s[i + left], keep = upper ? s[i + left] : s[i];
+                s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+              }
+          } else {
+            s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+          }
         }
-      }
+      };
+      // one of the two products is 0; with a bound that is not finite it may be NaN, which shows in the sum
+      sum([&](double t, int g, int i, double l, double h) { return fma(dn[g][i], l, fma(up[g][i], h, t)); });
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < REST; ++i) odd |= !(fabs(s[i]) < INFINITY);
+      if (__any_sync(0xffffffffu, odd))
+        sum([&](double t, int g, int i, double l, double h) {
+          const bool below = !(dn[g][i] == 0.0);
+          return fma(below ? dn[g][i] : up[g][i], below ? l : h, t);
+        });
       unsigned long long key = 0;
 #pragma unroll
       for (int i = 0; i < REST; ++i) {
@@ -196,7 +229,7 @@ GDNX_DEV void score_pages(const SelParams& P, const Query& q, int64_t b, int64_t
         int p = -1;
 #pragma unroll
         for (int e = 0; e < PB; ++e) p = e == j ? id[e] : p;
-        if (at < q.pages) {
+        if (at < r1) {
           const int64_t first = (int64_t)at * c.page;
           if (!page_ok(c, p)) key = 0;
           else if (first < a.sinks || first + c.page > q.len - a.window) key = ~0ull;
@@ -224,7 +257,7 @@ GDNX_DEV int rank_of(bool on, int* warp_sums, int* total) {
 // The k largest of n words (0: none), the lower index first among equals, in rising order; -1 behind them.
 template <int THREADS>
 GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t* out) {
-  constexpr int WARPS = THREADS / 32, HELD = 8;
+  constexpr int WARPS = THREADS / 32, HELD = 4;
   static_assert(RANKED <= THREADS, "a word for each thread");
   __shared__ int sums[2][3][WARPS];
   __shared__ unsigned long long ends[2][WARPS];
@@ -260,12 +293,15 @@ GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t
     least = w < least ? w : least;
     most = w > most ? w : most;
   }
+  const auto span = [](unsigned long long& a, unsigned long long& z) {  // over the warp
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long x = __shfl_xor_sync(0xffffffffu, least, o), y = __shfl_xor_sync(0xffffffffu, most, o);
-    least = x < least ? x : least;
-    most = y > most ? y : most;
-  }
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long x = __shfl_xor_sync(0xffffffffu, a, o), y = __shfl_xor_sync(0xffffffffu, z, o);
+      a = x < a ? x : a;
+      z = y > z ? y : z;
+    }
+  };
+  span(least, most);
   there = __reduce_add_sync(0xffffffffu, there);
   always = __reduce_add_sync(0xffffffffu, always);
   if (lane == 0) {
@@ -275,14 +311,11 @@ GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t
     sums[1][1][warp] = always;
   }
   __syncthreads();
-  there = always = 0;
-#pragma unroll
-  for (int i = 0; i < WARPS; ++i) {
-    least = ends[0][i] < least ? ends[0][i] : least;
-    most = ends[1][i] > most ? ends[1][i] : most;
-    there += sums[1][0][i];
-    always += sums[1][1][i];
-  }
+  least = lane < WARPS ? ends[0][lane] : ~0ull;
+  most = lane < WARPS ? ends[1][lane] : 0;
+  span(least, most);
+  there = __reduce_add_sync(0xffffffffu, lane < WARPS ? sums[1][0][lane] : 0);
+  always = __reduce_add_sync(0xffffffffu, lane < WARPS ? sums[1][1][lane] : 0);
   // A word's place between the ends in 32 bits: 0 for one that is not there, all ones for one always taken.  The
   // first words' places stay in registers.
   const int shift = most > least ? max(0, 33 - __clzll(most - least)) : 0;
@@ -448,7 +481,7 @@ gdnx_status select_of(const gdnx_paged_select_args& a, cudaStream_t st) {
 template <typename T, int LANES>
 gdnx_status select_heads(const gdnx_paged_select_args& a, cudaStream_t st) {
   const int64_t G = a.H / a.cache.Hk;
-  return G == 1 ? select_of<T, LANES, 1>(a, st) : G <= 4 ? select_of<T, LANES, 4>(a, st) : select_of<T, LANES, 8>(a, st);
+  return G == 1 ? select_of<T, LANES, 1>(a, st) : select_of<T, LANES, 4>(a, st);
 }
 
 template <typename T>
