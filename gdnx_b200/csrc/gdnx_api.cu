@@ -129,7 +129,7 @@ gdnx_attn_args clamp_attn(const gdnx_attn_args& a) {
   return c;
 }
 
-gdnx_status check_cache(const gdnx_cache* c) {
+gdnx_status check_cache_sizes(const gdnx_cache* c) {
   if (!c) return GDNX_EINVAL;
   if (!dtype_ok(c->dtype) || c->L <= 0 || c->pages < 0 || c->Hk <= 0 || c->D <= 0 || c->slots <= 0 || c->width <= 0)
     return GDNX_EINVAL;
@@ -137,6 +137,12 @@ gdnx_status check_cache(const gdnx_cache* c) {
   if (c->D > 128 || c->D % 8 || c->slots > (1 << 18) || c->width > (1 << 20) || c->width * c->page > kMaxTokens ||
       c->pages > ((int64_t)1 << 30))
     return GDNX_EUNSUPPORTED;
+  return GDNX_OK;
+}
+
+gdnx_status check_cache(const gdnx_cache* c) {
+  const gdnx_status s = check_cache_sizes(c);
+  if (s != GDNX_OK) return s;
   if (c->pages && (!device_ptr(c->kv, 16) || !words(c->refs))) return GDNX_EINVAL;
   if (!words(c->table) || !words(c->lengths) || !words(c->status)) return GDNX_EINVAL;
   return GDNX_OK;
@@ -322,8 +328,8 @@ static int64_t always_taken(const gdnx_paged_select_args& a) {
   return (a.sinks + page - 1) / page + (a.window + page - 2) / page + 1;
 }
 
-static gdnx_status check_select(const gdnx_paged_select_args& a) {
-  const gdnx_status s = check_cache(&a.cache);
+static gdnx_status check_select_sizes(const gdnx_paged_select_args& a) {
+  const gdnx_status s = check_cache_sizes(&a.cache);
   if (s != GDNX_OK) return s;
   if (a.cache.pages < 1 || a.B < 0 || a.H <= 0 || a.H % a.cache.Hk || a.layer < 0 || a.layer >= a.cache.L ||
       a.k < 1 || a.window < 1 || a.sinks < 0 || a.max_len < 0)
@@ -335,12 +341,14 @@ static gdnx_status check_select(const gdnx_paged_select_args& a) {
 }
 
 size_t gdnx_paged_select_workspace_bytes(const gdnx_paged_select_args* a) {
-  return !a || check_select(*a) != GDNX_OK || a->B == 0 ? 0 : gdnx::paged_select_workspace_bytes(*a);
+  return !a || check_select_sizes(*a) != GDNX_OK || a->B == 0 ? 0 : gdnx::paged_select_workspace_bytes(*a);
 }
 
 gdnx_status gdnx_paged_select(const gdnx_paged_select_args* a, void* stream) {
   if (!a) return GDNX_EINVAL;
-  const gdnx_status s = check_select(*a);
+  const gdnx_status z = check_select_sizes(*a);
+  if (z != GDNX_OK) return z;
+  const gdnx_status s = check_cache(&a->cache);
   if (s != GDNX_OK || a->B == 0) return s;
   if (!heads_ok(a->q, a->cache.dtype, a->cache.D) || !device_ptr(a->bounds, 16) || !words(a->selected) ||
       (a->rows && !words(a->rows)) || (a->positions && !words(a->positions)))
@@ -378,7 +386,7 @@ static gdnx_status check_decode(const gdnx_paged_decode_args& a) {
 
 size_t gdnx_paged_decode_workspace_bytes(const gdnx_paged_decode_args* a) {
   if (!a || a->B <= 0 || a->H <= 0 || a->cache.Hk <= 0 || a->window < 1 || a->sinks < 0) return 0;
-  if (check_cache(&a->cache) != GDNX_OK || a->H % a->cache.Hk) return 0;
+  if (check_cache_sizes(&a->cache) != GDNX_OK || a->H % a->cache.Hk) return 0;
   const gdnx_paged_decode_args c = clamp_decode(*a);
   return c.cache.dtype == GDNX_F32 ? gdnx::paged_decode_workspace_bytes(c) : gdnx::paged_decode_tc_workspace_bytes(c);
 }
@@ -394,8 +402,8 @@ gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* a, void* stream) {
                                    : gdnx::launch_paged_decode_tc(c, (cudaStream_t)stream);
 }
 
-static gdnx_status check_paged_attn(const gdnx_paged_attn_args& a) {
-  const gdnx_status s = check_cache(&a.cache);
+static gdnx_status check_paged_attn_sizes(const gdnx_paged_attn_args& a) {
+  const gdnx_status s = check_cache_sizes(&a.cache);
   if (s != GDNX_OK) return s;
   if (a.cache.pages < 1 || a.n < 0 || a.n > a.cache.slots || a.tokens < 0 || a.H <= 0 || a.H % a.cache.Hk || a.layer < 0 ||
       a.layer >= a.cache.L || a.window < 1 || a.sinks < 0 || a.max_len < 0 || !(a.scale > 0.f) || a.scale > 3.0e38f ||
@@ -414,14 +422,16 @@ static gdnx_paged_attn_args clamp_paged(const gdnx_paged_attn_args& a) {
 }
 
 size_t gdnx_paged_attn_workspace_bytes(const gdnx_paged_attn_args* a) {
-  if (!a || check_paged_attn(*a) != GDNX_OK || a->tokens == 0) return 0;
+  if (!a || check_paged_attn_sizes(*a) != GDNX_OK || a->tokens == 0) return 0;
   const gdnx_paged_attn_args c = clamp_paged(*a);
   return c.cache.dtype == GDNX_F32 ? gdnx::paged_attn_simt_workspace_bytes(c) : gdnx::paged_attn_tc_workspace_bytes(c);
 }
 
 gdnx_status gdnx_paged_attn(const gdnx_paged_attn_args* a, void* stream) {
   if (!a) return GDNX_EINVAL;
-  const gdnx_status s = check_paged_attn(*a);
+  const gdnx_status z = check_paged_attn_sizes(*a);
+  if (z != GDNX_OK) return z;
+  const gdnx_status s = check_cache(&a->cache);
   if (s != GDNX_OK || a->tokens == 0) return s;
   if (!heads_ok(a->q, a->cache.dtype, a->cache.D) || !device_ptr(a->y, bytes_of(a->y_dtype)) || a->y_st < 0 || a->y_sh < 0)
     return GDNX_EINVAL;

@@ -920,15 +920,27 @@ def _read_error_word(index: int, clear: bool) -> int:
     return value.value
 
 
+_ENTRIES = {}  # name -> the library's function
+
+
+def _entry(name: str):
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = _ENTRIES[name] = getattr(L.load(), name)
+    return fn
+
+
 def _enqueue(name: str, index: int, *args) -> None:
     """Call a C entry point with device ``index`` current and that device's current stream."""
-    fn = getattr(L.load(), name)
+    fn = _entry(name)
     stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch.cuda.current_device() == index:
-        L.check(fn(*args, stream), name)
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(index):
-            L.check(fn(*args, stream), name)
+            status = fn(*args, stream)
+    if status != L.GDNX_OK:
+        L.check(status, name)
 
 
 def _heads_view(t: torch.Tensor) -> L.View:
@@ -948,11 +960,15 @@ def _on_device(index: int, *ts) -> None:
             raise ValueError("all tensors must be on one device")
 
 
+_I32 = torch.int32
+
+
 def _index32(t, n, name, index):
     """Address of a contiguous int32 vector of n (any n where None) on device ``index``."""
-    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+    if t.dtype is not _I32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
         raise ValueError(f"{name} must be a contiguous int32 vector" + ("" if n is None else f" of {n}"))
-    _on_device(index, t)
+    if t.get_device() != index:
+        _on_device(index, t)
     return t.data_ptr()
 
 
@@ -1089,19 +1105,23 @@ class PagedCache:
 
 def _cache_struct(c: PagedCache):
     """The cache as the C ABI takes it, and its device's index."""
-    kv, table = c.kv, c.table
-    _require_cuda(kv)
+    kv, table, lengths, refs, status = c.kv, c.table, c.lengths, c.refs, c.status
     index = kv.get_device()
-    if kv.dim() != 6 or kv.shape[1] != 2 or not kv.is_contiguous() or kv.dtype not in _DT:
+    if index < 0:
+        _require_cuda(kv)
+    if kv.dim() != 6 or kv.dtype not in _DT or not kv.is_contiguous():
         raise ValueError("kv must be contiguous [L, 2, pages, Hk, page, D] in float32, bfloat16 or float16")
-    if table.dtype is not torch.int32 or table.dim() != 2 or not table.is_contiguous():
+    layers, sides, pages, hk, page, d = kv.shape
+    if sides != 2:
+        raise ValueError("kv must be contiguous [L, 2, pages, Hk, page, D] in float32, bfloat16 or float16")
+    if table.dtype is not _I32 or table.dim() != 2 or not table.is_contiguous():
         raise ValueError("table must be a contiguous int32 tensor [slots, width]")
-    _on_device(index, table)
-    layers, _, pages, hk, page, d = kv.shape
+    if table.get_device() != index:
+        _on_device(index, table)
     slots, width = table.shape
     return L.Cache(kv.data_ptr(), _DT[kv.dtype], page, layers, pages, hk, d, slots, width, table.data_ptr(),
-                   _index32(c.lengths, slots, "lengths", index), _index32(c.refs, pages, "refs", index),
-                   _index32(c.status, 1, "status", index)), index
+                   _index32(lengths, slots, "lengths", index), _index32(refs, pages, "refs", index),
+                   _index32(status, 1, "status", index)), index
 
 
 def _cache_bounds(c: PagedCache, index: int) -> int:
@@ -1118,10 +1138,16 @@ def _cache_bounds(c: PagedCache, index: int) -> int:
 def _cache_rows(rows, s, index, name="rows"):
     """Address and number of a list of slots."""
     at = _index32(rows, None, name, index)
-    n = rows.shape[0]
+    n = rows.numel()
     if n > s.slots:
         raise ValueError(f"{name} names more slots than there are")
     return at, n
+
+
+def _cache_workspace(s, n, like):
+    """Workspace of a page operation on n rows, and its bytes."""
+    need = _entry("gdnx_cache_workspace_bytes")(C.byref(s), n)
+    return like.new_empty(need, dtype=torch.uint8), need
 
 
 def cache_check(cache: PagedCache) -> None:
@@ -1148,8 +1174,7 @@ def cache_extend(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor) ->
     s, index = _cache_struct(cache)
     at, n = _cache_rows(rows, s, index)
     more = _index32(counts, n, "counts", index)
-    need = L.load().gdnx_cache_workspace_bytes(C.byref(s), n)
-    ws = rows.new_empty(need, dtype=torch.uint8)
+    ws, need = _cache_workspace(s, n, rows)
     _enqueue("gdnx_cache_extend", index, C.byref(s), n, at, more, ws.data_ptr(), need)
 
 
@@ -1195,8 +1220,7 @@ def cache_compact(cache: PagedCache) -> None:
     """Moves the live pages down so that they are the pool's first: page for page in order, those
     above the live count into the free ones below it (and their bounds with them)."""
     s, index = _cache_struct(cache)
-    need = L.load().gdnx_cache_workspace_bytes(C.byref(s), 0)
-    ws = cache.table.new_empty(need, dtype=torch.uint8)
+    ws, need = _cache_workspace(s, 0, cache.table)
     if cache.bounds is None:
         _enqueue("gdnx_cache_compact", index, C.byref(s), ws.data_ptr(), need)
     else:
@@ -1225,13 +1249,11 @@ def cache_step(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor, toke
     more = _index32(counts, n, "counts", index)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
-    i32 = dict(dtype=torch.int32)
-    step = PagedStep(rows, rows.new_empty(n + 1, **i32), rows.new_empty(n, **i32), rows.new_empty(tokens, **i32),
-                     rows.new_empty(tokens, **i32), rows.new_empty(tokens, dtype=torch.int64))
-    out = L.Step(tokens, step.starts.data_ptr(), step.first.data_ptr(), step.token_rows.data_ptr(),
-                 step.positions.data_ptr(), step.places.data_ptr())
-    need = L.load().gdnx_cache_workspace_bytes(C.byref(s), n)
-    ws = rows.new_empty(need, dtype=torch.uint8)
+    starts, first, token_rows, positions = rows.new_empty(2 * (n + tokens) + 1).split_with_sizes((n + 1, n, tokens, tokens))
+    step = PagedStep(rows, starts, first, token_rows, positions, rows.new_empty(tokens, dtype=torch.int64))
+    at32 = starts.data_ptr()
+    out = L.Step(tokens, at32, at32 + 4 * (n + 1), at32 + 4 * (2 * n + 1), at32 + 4 * (2 * n + 1 + tokens), step.places.data_ptr())
+    ws, need = _cache_workspace(s, n, rows)
     _enqueue("gdnx_cache_step", index, C.byref(s), n, at, more, C.byref(out), ws.data_ptr(), need)
     return step
 
@@ -1310,7 +1332,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, step: PagedStep, *, laye
     if return_lse:
         a.lse = lse.data_ptr()
     a.error = _error_word(index)
-    need = L.load().gdnx_paged_attn_workspace_bytes(C.byref(a))
+    need = _entry("gdnx_paged_attn_workspace_bytes")(C.byref(a))
     ws = None
     if need:
         ws = q.new_empty(need, dtype=torch.uint8)
@@ -1369,7 +1391,7 @@ def paged_select(q: torch.Tensor, cache: PagedCache, k: int, *, layer: int = 0, 
                           L.View(q.data_ptr(), _DT[q.dtype], D, qb, 0, qh),
                           None if rows is None else _index32(rows, B, "rows", index),
                           None if positions is None else _index32(positions, B, "positions", index), out.data_ptr())
-    need = L.load().gdnx_paged_select_workspace_bytes(C.byref(a))
+    need = _entry("gdnx_paged_select_workspace_bytes")(C.byref(a))
     ws = None
     if need:
         ws = q.new_empty(need, dtype=torch.uint8)
@@ -1432,7 +1454,7 @@ def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Op
             raise ValueError("pages must be a contiguous int32 tensor [B,Hk,k]")
         _on_device(index, pages)
         a.pages, a.listed = pages.data_ptr(), pages.shape[2]
-    need = L.load().gdnx_paged_decode_workspace_bytes(C.byref(a))
+    need = _entry("gdnx_paged_decode_workspace_bytes")(C.byref(a))
     ws = None
     if need:
         ws = q.new_empty(need, dtype=torch.uint8)
