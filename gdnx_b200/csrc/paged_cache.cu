@@ -204,12 +204,11 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
   __syncthreads();  // the list is whole
   // refs of shared pages are read above and below by every row before any is changed
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  for (int64_t i0 = 0; i0 < n; i0 += NT / 32) {
-    const int64_t i = i0 + warp;
+  for (int64_t i = threadIdx.x; i < n; i += NT) {
     int64_t first = 0, need = 0;
     int shared = -1;
-    if (i < n) ask(i, first, need, shared, lost);
-    if (i < n) w.off[i] |= shared >= 0 ? (int)0x80000000 : 0;
+    ask(i, first, need, shared, lost);
+    w.off[i] |= shared >= 0 ? (int)0x80000000 : 0;
   }
   __syncthreads();
   for (int64_t i = warp; i < n; i += NT / 32) {
@@ -284,22 +283,33 @@ __global__ void __launch_bounds__(NT) cache_compact_kernel(const gdnx_cache c, v
   }
 }
 
-// Where each packed token stands: its sequence by bisection of the starts, and its page's place there.
+constexpr int STARTS = 4096;  // of a step that fit shared memory
+
+// Where each packed token stands: its sequence by bisection of the starts (from shared memory where they fit), and its
+// page's place there.
 GDNX_DEV void place_tokens(const gdnx_cache& c, int64_t n, const int32_t* rows, const gdnx_step& s) {
-  const int packed = s.starts[n];
+  __shared__ int32_t mine[STARTS];
+  if ((int64_t)blockIdx.x * COPY_NT >= s.tokens) return;
+  const int32_t* starts = s.starts;
+  if (n < STARTS) {
+    for (int i = threadIdx.x; i <= n; i += COPY_NT) mine[i] = s.starts[i];
+    __syncthreads();
+    starts = mine;
+  }
+  const int packed = starts[n], shift = 31 - __clz(c.page);
   for (int64_t t = (int64_t)blockIdx.x * COPY_NT + threadIdx.x; t < s.tokens; t += (int64_t)gridDim.x * COPY_NT) {
     int row = -1, pos = -1;
     int64_t place = -1;
     if (t < packed) {
-      int64_t lo = 0, hi = n;  // starts[lo] <= t < starts[hi]
+      int lo = 0, hi = (int)n;  // starts[lo] <= t < starts[hi]
       while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) / 2;
-        if (s.starts[mid] <= t) lo = mid;
+        const int mid = (lo + hi) / 2;
+        if (starts[mid] <= t) lo = mid;
         else hi = mid;
       }
       row = rows[lo];
-      pos = s.first[lo] + (int)(t - s.starts[lo]);
-      place = (int64_t)c.table[row * c.width + pos / c.page] * c.page + pos % c.page;
+      pos = s.first[lo] + (int)t - starts[lo];
+      place = ((int64_t)c.table[row * c.width + (pos >> shift)] << shift) + (pos & (c.page - 1));
     }
     s.token_rows[t] = row;
     s.positions[t] = pos;
