@@ -53,11 +53,12 @@ GDNX_DEV void load_stages(const DecParams& P, Walk w, uint8_t* ring, Small<NH>& 
   while (w.next()) {
     const int hk = w.unit / P.groups;
     int ids = -1;
+    int64_t first;
     for (int t = w.ta; t < w.tb; ++t) {
       const int k = (t - w.ta) % ahead;
       if (k == 0) {
         const int mine = t + lane / npp;
-        ids = mine < w.tb ? page_id(P, w.seq, w.b, w.unit, w.seq.kt.tile(mine), lane % npp) : -1;
+        ids = mine < w.tb ? page_id(P, w.seq, w.b, w.unit, w.seq.kt.tile(mine), lane % npp, first) : -1;
       }
       for (int s = 0; s < TM / SUB; ++s) {
         const int tile = w.seq.kt.tile(t);

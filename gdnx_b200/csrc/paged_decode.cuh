@@ -171,10 +171,10 @@ GDNX_DEV int64_t page_first(const DecParams& P, const Seq& s, int64_t b, int uni
   return x < 0 || x >= c.width ? -1 : (int64_t)x * c.page;
 }
 
-// Page ids of a tile's pages, or -1 where nothing visible is there (lane < npp).
-GDNX_DEV int page_id(const DecParams& P, const Seq& s, int64_t b, int unit, int kt, int i) {
+// Page ids of a tile's pages, or -1 where nothing visible is there (lane < npp), and their first tokens.
+GDNX_DEV int page_id(const DecParams& P, const Seq& s, int64_t b, int unit, int kt, int i, int64_t& first) {
   const gdnx_cache& c = P.a.cache;
-  const int64_t first = page_first(P, s, b, unit, kt, i);
+  first = page_first(P, s, b, unit, kt, i);
   if (first < 0 || first >= s.len || !(first + c.page > (int64_t)s.len - P.a.window || first < P.a.sinks)) return -1;
   const int p = c.table[(int64_t)s.row * c.width + first / c.page];
   return p >= 0 && p < c.pages ? p : -1;

@@ -28,6 +28,8 @@ struct TcParams : DecParams {
   int vec_q;       // q's rows are 16-byte aligned
 };
 
+constexpr int TILES = 16;  // more than can be between the loads and the keys
+
 struct Bars {
   uint64_t full[12], empty[12], q_ready[2], q_empty[2], s_full[2], p_ready[2], pv_done[2], done;
 };
@@ -38,6 +40,7 @@ struct Small {
   Range range;
   long long sums[NTHREADS / 32];
   float red[4 * NH];
+  int at[TILES][8];  // first tokens of a tile's pages, -1 where nothing visible is there; tile after tile
   uint32_t tmem_at;
   int abort_flag;
 };
@@ -61,7 +64,7 @@ GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, 
 }
 
 template <int DB, int NH>
-GDNX_DEV void run_loads(const TcParams& P, Walk w, uint32_t smem, Bars& bar, volatile int* abort_flag) {
+GDNX_DEV void run_loads(const TcParams& P, Walk w, uint32_t smem, Bars& bar, int (*at)[8], volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   const gdnx_cache& c = P.a.cache;
   const int lane = threadIdx.x % 32, npp = TM / c.page, page = c.page;
@@ -71,16 +74,21 @@ GDNX_DEV void run_loads(const TcParams& P, Walk w, uint32_t smem, Bars& bar, vol
   while (w.next()) {
     const int hk = w.unit / P.groups;
     int ids = -1;
+    int64_t first = -1;
     for (int t = w.ta; t < w.tb; ++t) {
       const int k = (t - w.ta) % ahead;
       if (k == 0) {
         const int mine = t + lane / npp;
-        ids = mine < w.tb ? page_id(P, w.seq, w.b, w.unit, w.seq.kt.tile(mine), lane % npp) : -1;
+        ids = mine < w.tb ? page_id(P, w.seq, w.b, w.unit, w.seq.kt.tile(mine), lane % npp, first) : -1;
       }
       const int pg = lane / DB, d = lane % DB;
       const int id = __shfl_sync(0xffffffffu, ids, (k * npp + pg) & 31);
       const bool go = pg < npp && id >= 0;
       const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, go)) * box;
+      // handed to the keys with the tile's barrier
+      const int begin = __shfl_sync(0xffffffffu, ids >= 0 ? (int)first : -1, (k * npp + lane) & 31);
+      if (lane < npp) const_cast<volatile int*>(at[cnt / 2 % TILES])[lane] = begin;
+      __syncwarp();
 #pragma unroll
       for (int side = 0; side < 2; ++side, ++cnt) {
         const uint32_t sl = cnt % Lo::SLOTS, mb = tc::smem_u32(&bar.full[sl]);
@@ -219,13 +227,13 @@ GDNX_DEV void tmem_st(uint32_t at, const float (&v)[NC]) {
 // NC: heads that a thread works on, the unit's rounded up (the others' columns are not used).
 template <int DB, int NH, int NC, bool BF16>
 GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, uint32_t tmem, Bars& bar, float* red,
-                       volatile int* abort_flag) {
+                       const int (*at)[8], volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   const gdnx_paged_decode_args& a = P.a;
   const int r = threadIdx.x, lane = r % 32, warp = r / 32, D = (int)a.cache.D;
   const uint32_t lane_at = (uint32_t)(warp * 32) << 16;
   const float c2 = a.scale * kLog2e;
-  const int window = (int)a.window, sinks = (int)a.sinks;
+  const int window = (int)a.window, sinks = (int)a.sinks, on_page = r / a.cache.page, in_page = r % a.cache.page;
   uint32_t nt = 0;
   bool ok = true;  // a wait that gave up is told at the next vote, where all four warps leave
   if (r == 0 && !P.whole) P.joint[blockIdx.x] = {0, 0, 0, -1};
@@ -239,17 +247,12 @@ GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, ui
       l[h] = 0.f;
     }
     for (int t = w.ta; t < w.tb; ++t, ++nt) {
-      const int page = a.cache.page, first = (int)page_first(P, w.seq, w.b, w.unit, w.seq.kt.tile(t), r / page);
-      const int j = first + r % page;
-      // a released page inside the visible range is not seen either
-      bool seen = first >= 0 && key_seen(j, w.seq.len, window, sinks);
-      if (seen) {
-        const int p = a.cache.table[(int64_t)w.seq.row * a.cache.width + j / a.cache.page];
-        seen = p >= 0 && p < a.cache.pages;
-      }
-      any |= seen;
       ok = ok && warp_wait(&bar.s_full[nt & 1], nt / 2 & 1, abort_flag);
       tc::fence_after();
+      // a released page inside the visible range is not seen either
+      const int first = *const_cast<volatile int*>(&at[nt % TILES][on_page]);
+      const bool seen = first >= 0 && key_seen(first + in_page, w.seq.len, window, sinks);
+      any |= seen;
       float s[NC];
       tmem_ld(tmem + lane_at + (nt & 1) * NH, s);
       bool over = t == w.ta || !ok;
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   const Walk w(P, units, sm.range);
   if (smem % 1024) {  // never entered: the base is aligned
   } else if (warp < 4) {
-    run_keys<DB, NH, NC, BF16>(P, w, sm.range.per, base, tmem, bar, sm.red, abort_flag);
+    run_keys<DB, NH, NC, BF16>(P, w, sm.range.per, base, tmem, bar, sm.red, sm.at, abort_flag);
   } else if (warp == 4) {
     run_products<DB, NH, BF16>(P, w, smem, tmem, bar, abort_flag);
     __syncwarp();
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   } else if (warp == 6) {
     run_queries<DB, NH>(P, w, base, bar, abort_flag);
   } else {
-    run_loads<DB, NH>(P, w, smem, bar, abort_flag);
+    run_loads<DB, NH>(P, w, smem, bar, sm.at, abort_flag);
     write_zeros(P);
     if (*abort_flag)  // let the copies in flight land
       for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);

@@ -106,7 +106,8 @@ GDNX_DEV bool bounds_ok(uint32_t* seen, const gdnx_cache& c, int64_t n, const in
   return !__syncthreads_or(bad);
 }
 
-// CTA (h, i, z): head h of every gridDim.z-th page that holds one of the newest tokens of slot rows[i].
+// CTA (h, i, z): head h of every gridDim.z-th page that holds one of the newest tokens of slot rows[i].  A CTA reads
+// its first page's keys before it checks the call, and writes after.
 template <typename T>
 __global__ void __launch_bounds__(BOUNDS_NT) cache_bounds_kernel(const gdnx_cache c, int64_t layer, int64_t n,
                                                                  const int32_t* rows, const int32_t* counts,
@@ -115,28 +116,46 @@ __global__ void __launch_bounds__(BOUNDS_NT) cache_bounds_kernel(const gdnx_cach
   __shared__ uint4 part[2][BOUNDS_NT];
   dependents_may_start();
   wait_for_earlier();
-  if (!bounds_ok(seen, c, n, rows, counts)) {
-    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && *c.status == 0) *c.status = GDNX_EINVAL;
-    return;
-  }
   const int per = (int)(c.D * sizeof(T) / 16), groups = BOUNDS_NT / per;  // pieces of a row, rows side by side
   const int piece = threadIdx.x % per, group = threadIdx.x / per, h = blockIdx.x;
+  const bool first_cta = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
+  bool checked = false;
   for (int64_t i = blockIdx.y; i < n; i += gridDim.y) {
-    const int64_t len = length_of(c, rows[i]), count = counts[i];
-    if (count == 0) continue;
+    const int row = rows[i];
+    if (row < 0 || row >= c.slots) continue;  // refused by the CTAs that have work
+    const int64_t len = length_of(c, row), count = min((int64_t)counts[i], len);
+    if (count <= 0) continue;
     for (int64_t x = (len - count) / c.page + blockIdx.z; x * c.page < len; x += gridDim.z) {
-      const int p = c.table[rows[i] * c.width + x];
+      const int p = c.table[row * c.width + x];
       if (!page_ok(c, p)) continue;
       const int have = (int)min((int64_t)c.page, len - x * c.page);
       const uint4* src = static_cast<const uint4*>(c.kv) + ((layer * 2 * c.pages + p) * c.Hk + h) * c.page * per + piece;
+      constexpr int AHEAD = 8;  // rows in flight, those of the first page under the checks
+      uint4 k[AHEAD];
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e)
+        if (group < groups && group + e * groups < have) k[e] = src[(group + e * groups) * per];
+      if (!checked) {
+        if (!bounds_ok(seen, c, n, rows, counts)) {
+          if (first_cta && threadIdx.x == 0 && *c.status == 0) *c.status = GDNX_EINVAL;
+          return;
+        }
+        checked = true;
+      }
       if (group < groups) {
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        if (group < have) lo = hi = src[group * per];
-#pragma unroll 8
-        for (int r = group + groups; r < have; r += groups) {
-          const uint4 k = src[r * per];
-          lo = least4<T>(lo, k);
-          hi = most4<T>(hi, k);
+        uint4 lo = k[0], hi = k[0];
+        for (int r = group; r < have; r += AHEAD * groups) {
+          if (r > group) {
+#pragma unroll
+            for (int e = 0; e < AHEAD; ++e)
+              if (r + e * groups < have) k[e] = src[(r + e * groups) * per];
+          }
+#pragma unroll
+          for (int e = 0; e < AHEAD; ++e)
+            if (r + e * groups < have) {
+              lo = least4<T>(lo, k[e]);
+              hi = most4<T>(hi, k[e]);
+            }
         }
         part[0][threadIdx.x] = lo;
         part[1][threadIdx.x] = hi;
@@ -154,6 +173,8 @@ __global__ void __launch_bounds__(BOUNDS_NT) cache_bounds_kernel(const gdnx_cach
       __syncthreads();
     }
   }
+  if (!checked && first_cta && !bounds_ok(seen, c, n, rows, counts) && threadIdx.x == 0 && *c.status == 0)
+    *c.status = GDNX_EINVAL;
 }
 
 template <typename T>
