@@ -5,49 +5,53 @@
 // forward does (attn_simt.cuh):  s = scale log2(e) q.k;  m' = max(m, max_j s);  p = 2^(s - m');
 //   l = l 2^(m - m') + sum_j p;  o = o 2^(m - m') + p V;   y = o / l.
 // A tile's tokens come from up to four pages by 16-byte asynchronous copies; what lies on no page, or behind the
-// sequence's last token, is zero and not seen.
+// sequence's last token, is zero and not seen.  The next tile's keys come under the product with the values, its values
+// under the product with its keys, its page ids under both.
 #include "attn_simt.cuh"
 #include "paged_attn.cuh"
 
 namespace gdnx {
 namespace {
 
-using Simt = Shape<BR, BT, false>;
+struct Simt : Shape<BR, BT, false> {
+  static constexpr int OVER = 4, SMALL = 12, LEAST = 4;
+};
 constexpr int GRANULES = BT / 16;  // of 16 tokens: the smallest page
 
-struct Ids {
-  int id[GRANULES];  // page of each granule, -1 where there is none
-};
-
-// Tokens j0.. of keys or values (side) into dst [BT][DP + 4].
+// Tokens j0.. of keys or values (side) into dst [BT][DP + 4], as one group of asynchronous copies.  ids: page of each
+// granule, -1 where there is none.
 template <int DP>
 GDNX_DEV void load_paged(float* dst, const gdnx_cache& c, int64_t layer, int side, int hk, const int* ids, int j0, int len) {
-  const int D = (int)c.D;
-  const float* base = static_cast<const float*>(c.kv) + (layer * 2 + side) * c.pages * c.Hk * c.page * D;
+  const int D = (int)c.D, mask = c.page - 1, row = c.page * D;
+  const float* base = static_cast<const float*>(c.kv) + ((layer * 2 + side) * c.pages * c.Hk + hk) * row;
 #pragma unroll
   for (int k = 0; k < BT * DP / 4 / NT; ++k) {
     const int i = k * NT + threadIdx.x, r = i / (DP / 4), d = i % (DP / 4) * 4;
     const int id = ids[r / 16];
     const bool on = id >= 0 && j0 + r < len && d < D;
-    const float* src = on ? base + (((int64_t)id * c.Hk + hk) * c.page + (j0 + r) % c.page) * D + d : base;
+    const float* src = on ? base + (int64_t)id * c.Hk * row + ((j0 + r) & mask) * D + d : base;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                      static_cast<uint32_t>(__cvta_generic_to_shared(dst + r * (DP + 4) + d))),
                  "l"(src), "r"(on ? 16 : 0)
                  : "memory");
   }
+  asm volatile("cp.async.commit_group;" ::: "memory");
 }
+// This thread's groups but the newest have landed (a barrier makes them everyone's).
+GDNX_DEV void wait_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 
 template <int DP>
 __global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParams P) {
   extern __shared__ float sm[];
   __shared__ Share share;
   __shared__ long long sums[NT / 32];
-  __shared__ Ids ids;
+  __shared__ int ids[2][GRANULES];
   const gdnx_paged_attn_args& a = P.a;
   const gdnx_cache& c = a.cache;
   float* Q = sm;
-  float* KV = Q + BR * (DP + 4);
-  float* W = KV + BT * (DP + 4);
+  float* K = Q + BR * (DP + 4);
+  float* V = K + BT * (DP + 4);
+  float* W = V + BT * (DP + 4);
   dependents_may_start();
   wait_for_earlier();
   find_share<Simt, NT>(P, share, sums);
@@ -60,8 +64,19 @@ __global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParam
   float* w = W + ty * 4 * LDP;
   Walk<Simt> x(P, share);
   while (x.next()) {
-    const int heads = x.heads(), h0 = x.head0(), len = x.s.len(), t0 = x.x.t0;
+    const int heads = x.heads(), h0 = x.head0(), len = x.s.len(), t0 = x.x.t0, hk = x.hk();
+    const auto read_ids = [&](int k) {  // of tile k, by the first threads
+      if (threadIdx.x < GRANULES && k < x.tb) {
+        const int64_t page = (x.x.kt.tile(k) * BT + 16 * threadIdx.x) / c.page;
+        const int id = page < c.width ? c.table[(int64_t)x.s.row * c.width + page] : -1;
+        ids[k & 1][threadIdx.x] = id >= 0 && id < c.pages ? id : -1;
+      }
+    };
     __syncthreads();  // the unit before has read its tiles
+    read_ids(x.ta);
+    __syncthreads();
+    load_paged<DP>(K, c, a.layer, 0, hk, ids[x.ta & 1], x.x.kt.tile(x.ta) * BT, len);
+    load_paged<DP>(V, c, a.layer, 1, hk, ids[x.ta & 1], x.x.kt.tile(x.ta) * BT, len);
     for (int i = threadIdx.x; i < BR * DP; i += NT) {
       const int r = i / DP, d = i % DP, t = t0 + r / P.gs, g = r % P.gs;
       float v = 0.f;
@@ -90,27 +105,22 @@ __global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParam
       const int lo = pw - window + 1 - j0;
       const Groups gr = pw >= len ? Groups(1, 0) : sinks <= j0 ? Groups(lo, pz - j0)
                                                                : Groups(0, lo <= BT - 1 ? pz - j0 : min(pz - j0, sinks - 1 - j0));
-      __syncthreads();
-      if (threadIdx.x < GRANULES) {
-        const int64_t page = (j0 + 16 * threadIdx.x) / c.page;
-        const int id = page < c.width ? c.table[(int64_t)x.s.row * c.width + page] : -1;
-        ids.id[threadIdx.x] = id >= 0 && id < c.pages ? id : -1;
-      }
-      __syncthreads();
-      load_paged<DP>(KV, c, a.layer, 0, x.hk(), ids.id, j0, len);
-      wait_tiles();
-      __syncthreads();
+      const int* here = ids[k & 1];
+      const int next0 = k + 1 < x.tb ? x.x.kt.tile(k + 1) * BT : 0;
+      wait_but_one();
+      __syncthreads();  // K (and, of the first tile, Q)
+      read_ids(k + 1);
       for_groups(gr.n, [&](auto nc) {
         constexpr int NC = decltype(nc)::value;
         const int col = 16 * gr.first + tx;
         float s[4][4];
-        dot_tile<DP, NC>(s, q, KV + col * (DP + 4), D);
+        dot_tile<DP, NC>(s, q, K + col * (DP + 4), D);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float mx = m[r];
 #pragma unroll
           for (int e = 0; e < NC; ++e) {
-            const bool on = sees(p[r], j0 + col + 16 * e, len, window, sinks) && ids.id[gr.first + e] >= 0;
+            const bool on = sees(p[r], j0 + col + 16 * e, len, window, sinks) && here[gr.first + e] >= 0;
             any[r] |= on;
             s[r][e] = on ? s[r][e] * c2 : -INFINITY;
             mx = fmaxf(mx, s[r][e]);
@@ -131,11 +141,14 @@ __global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParam
           for (int d = 0; d < DP / 32; ++d) o[r][d] = mul2(o[r][d], make_float2(corr, corr));
         }
       });
+      __syncthreads();  // K has been read, and the next tile's ids are there
+      if (k + 1 < x.tb) load_paged<DP>(K, c, a.layer, 0, hk, ids[(k + 1) & 1], next0, len);
+      else asm volatile("cp.async.commit_group;" ::: "memory");
+      wait_but_one();
+      __syncthreads();  // V
+      acc_tile<DP>(o, w, V, tx, gr);
       __syncthreads();
-      load_paged<DP>(KV, c, a.layer, 1, x.hk(), ids.id, j0, len);
-      wait_tiles();
-      __syncthreads();
-      acc_tile<DP>(o, w, KV, tx, gr);
+      if (k + 1 < x.tb) load_paged<DP>(V, c, a.layer, 1, hk, ids[(k + 1) & 1], next0, len);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -168,14 +181,15 @@ __global__ void __launch_bounds__(NT, 3) paged_attn_simt_kernel(const ChunkParam
 
 template <int DP>
 gdnx_status run(const ChunkParams& P, cudaStream_t st) {
-  constexpr int smem = ((BR + BT) * (DP + 4) + BR * LDP) * (int)sizeof(float);
+  constexpr int smem = ((BR + 2 * BT) * (DP + 4) + BR * LDP) * (int)sizeof(float);
   static std::atomic<uint64_t> done;
   if (!allow_smem(paged_attn_simt_kernel<DP>, smem, done)) return GDNX_ELAUNCH;
   if (launch_early(paged_attn_simt_kernel<DP>, dim3((unsigned)P.grid), dim3(NT), smem, st, P) != cudaSuccess)
     return GDNX_ELAUNCH;
   return join_chunks<Simt>(P, st);
 }
-ChunkParams plan(const gdnx_paged_attn_args& a) { return plan_chunks<Simt>(a, sm_count() * 3); }
+// As many CTAs as shared memory has room for.
+ChunkParams plan(const gdnx_paged_attn_args& a) { return plan_chunks<Simt>(a, sm_count() * (a.cache.D > 96 ? 2 : 3)); }
 
 }  // namespace
 
