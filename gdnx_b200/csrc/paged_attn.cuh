@@ -67,16 +67,15 @@ struct Shape {
 template <class S>
 struct Unit {
   KeyTiles kt;
-  int t0, blocks, each, w;  // first token of the chunk; weights of a tile and in all
-  GDNX_DEV Unit() : kt(), t0(0), blocks(0), each(0), w(0) {}
+  int t0, blocks, w;  // first token of the chunk
+  GDNX_DEV Unit() : kt(), t0(0), blocks(0), w(0) {}
   GDNX_DEV Unit(const ChunkParams& P, const Chunk& s, int u) {
     const int step = S::PAIR ? 2 * P.tb : P.tb;
     t0 = u * step;
     const int n = min(step, s.count - t0);
     blocks = n > P.tb ? 2 : 1;
     kt = KeyTiles(s.first + t0, s.first + t0 + n - 1, s.len(), (int)P.a.window, (int)P.a.sinks, S::KEYS);
-    each = blocks == 2 ? S::TWO : S::ONE;
-    w = S::OVER + each * kt.count;
+    w = S::OVER + (blocks == 2 ? S::TWO : S::ONE) * kt.count;
   }
 };
 
@@ -231,13 +230,19 @@ struct Walk {
         ta = 0;
         tb = before >= t0 ? x.kt.count : 0;
       } else {
-        // tile i lies at before + OVER + i * each, and belongs to the share that this lies in
+        // tile i lies at before + OVER + i of its weights, and belongs to the share that this lies in
         const long long lo = t0 - before - S::OVER, hi = t1 - before - S::OVER;
-        ta = lo <= 0 ? 0 : (int)min((lo + x.each - 1) / x.each, (long long)x.kt.count);
-        tb = hi <= 0 ? 0 : (int)min((hi + x.each - 1) / x.each, (long long)x.kt.count);
+        ta = tiles_before(lo);
+        tb = tiles_before(hi);
       }
       if (ta < tb) return true;
     }
+  }
+  // Tiles of the unit that begin before weight z behind its start.
+  GDNX_DEV int tiles_before(long long z) const {
+    if (z <= 0) return 0;
+    const int most = (int)min(z, (long long)x.w);  // (a tile weighs 1 or more)
+    return min(x.blocks == 2 ? (most + S::TWO - 1) / S::TWO : (most + S::ONE - 1) / S::ONE, x.kt.count);
   }
   GDNX_DEV bool whole() const { return ta == 0 && tb == x.kt.count; }
   // Where this segment's part lies: one that goes on in the next CTA is this CTA's last, any other its first.
