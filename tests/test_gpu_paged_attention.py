@@ -110,6 +110,28 @@ def test_chunks_against_the_formula(case):
     assert torch.equal(ops.paged_attention(q, c, step, **kw), y)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (70, 20)])
+def test_more_sequences_than_a_block_has_threads(dtype, window, sinks):
+    """Each thread adds up the weights of several sequences, some of many units, some with nothing new."""
+    g = torch.Generator().manual_seed(11)
+    n = 900
+    lengths = torch.randint(0, 60, (n,), generator=g).tolist()
+    for i, x in ((0, 700), (1, 1), (401, 1500), (402, 900), (899, 300)):
+        lengths[i] = x
+    counts = [min(x, c) for x, c in zip(lengths, torch.randint(0, 4, (n,), generator=g).tolist())]
+    counts[0], counts[401], counts[402], counts[899] = 650, 333, 0, 300
+    c = cache(lengths, Hk=2, page=16, D=32, dtype=dtype, width=100)
+    order = torch.randperm(n, generator=g).tolist()
+    step = packed(c, order, [counts[i] for i in order], pad=9)
+    N = step.positions.shape[0]
+    q = torch.randn(N, 6, 32, generator=g).to(TYPES[dtype]).to(DEV)
+    y, lse = ops.paged_attention(q, c, step, layer=1, window=window, sinks=sinks, return_lse=True)
+    want, want_lse = plain(q, c, step, layer=1, window=window, sinks=sinks)
+    close(y, want, dtype)
+    assert torch.allclose(lse[:-9].double(), want_lse[:-9], rtol=1e-5, atol=1e-4) and (y[-9:] == 0).all()
+
+
 def test_chunks_against_the_oracle():
     for dtype in TYPES:
         c = cache([40, 7, 100, 0, 17], page=16, dtype=dtype, width=8)

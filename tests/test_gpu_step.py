@@ -283,6 +283,42 @@ def test_selection_among_more_pages_than_shared_memory_holds():
         assert ops.paged_select(q, c, k, rows=i32(1))[0, 0].tolist() == want
 
 
+def test_more_units_than_a_grid_dimension_holds():
+    """20,000 queries of four key heads: 80,000 selections, each against the formula."""
+    page, n, Hk, H, D, B, k = 16, 12, 4, 4, 8, 20000, 5
+    c = cache([page * n - 3, page * 7], Hk=Hk, page=page, D=D, dtype="f32", width=n)
+    o = mirror(c)
+    with_bounds(c, o)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    q = torch.randn(B, H, D, generator=g, device=DEV)
+    rows = torch.randint(0, 2, (B,), generator=g, device=DEV, dtype=torch.int32)
+    pages = ops.paged_select(q, c, k, rows=rows)
+    at = c.table.long()[rows.long()].clamp_min(0)  # [B, n]
+    lo, hi = (c.bounds[0, s][at].double() for s in (0, 1))  # [B, n, Hk, D]
+    x = q.double()[:, None]
+    score = torch.where(x >= 0, x * hi, x * lo).sum(-1).transpose(1, 2)  # [B, Hk, n]
+    have = (c.lengths.long()[rows.long()] + page - 1) // page
+    i = torch.arange(n, device=DEV)
+    score = torch.where(i == have[:, None, None] - 1, torch.inf, torch.where(i < have[:, None, None], score, -torch.inf))
+    want = torch.sort(score, dim=-1, descending=True, stable=True).indices[..., :k].sort(-1).values
+    assert torch.equal(pages.long(), want)
+
+
+def test_bounds_of_many_slots():
+    g = torch.Generator().manual_seed(6)
+    lengths = torch.randint(0, 70, (700,), generator=g).tolist()
+    c = cache(lengths, Hk=1, D=8, page=32, width=3)
+    o = mirror(c)
+    mine = with_bounds(c, o)
+    rows = torch.randperm(700, generator=g).tolist()[:600]
+    counts = [min(lengths[r], x) for r, x in zip(rows, torch.randint(0, 50, (600,), generator=g).tolist())]
+    c.kv[:, 0] = c.kv[:, 0].flip(-1)
+    o.kv = c.kv.cpu()
+    ops.cache_bounds(c, i32(*rows), i32(*counts), layer=1)
+    o.update_bounds(mine, rows, counts, 1)
+    assert int(c.status) == 0 and not o.status and torch.equal(c.bounds.cpu(), mine)
+
+
 def test_listed_pages_that_are_not_the_slots_are_passed_over():
     for dtype in ("bf16", "f32"):
         c = cache([100, 37], page=16, width=8, dtype=dtype)
