@@ -174,7 +174,12 @@ GDNX_DEV void find_share(const ChunkParams& P, Share& out, long long* sums) {
     const int nu = units_of<S>(P, c);
     const int hg = (int)((t0 - out.before) / out.one);
     long long at = out.before + hg * out.one;
-    for (int u0 = 0; u0 < nu; u0 += 32) {
+    if (nu == 1 && lane == 0) {
+      out.before = at;
+      out.hg = hg;
+      out.u = 0;
+    }
+    for (int u0 = 0; nu > 1 && u0 < nu; u0 += 32) {
       const long long w = u0 + lane < nu ? Unit<S>(P, c, u0 + lane).w : 0, in = warp_scan64(w);
       const uint32_t behind = __ballot_sync(0xffffffffu, t0 < at + in);
       if (behind) {

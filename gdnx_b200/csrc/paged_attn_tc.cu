@@ -488,12 +488,11 @@ GDNX_DEV void run_products(Small& sm, uint32_t smem, uint32_t tmem) {
   }
 }
 
-// The page of tile kt's i-th page in the cache, -1 where there is none.
-GDNX_DEV int page_of(const gdnx_cache& c, int row, int len, int kt, int i) {
+// What the table says of tile kt's i-th page, -1 where it says nothing.  (Checked against the pool when it is used: the
+// warp that reads ahead then does not wait for what it read.)
+GDNX_DEV int table_entry(const gdnx_cache& c, int row, int len, int kt, int i) {
   const int64_t x = (int64_t)kt * (TM / c.page) + i;
-  if (x >= c.width || x * c.page >= len) return -1;
-  const int p = c.table[(int64_t)row * c.width + x];
-  return p >= 0 && p < c.pages ? p : -1;
+  return x < c.width && x * c.page < len ? c.table[(int64_t)row * c.width + x] : -1;
 }
 
 // The warp that walks the share.
@@ -509,7 +508,7 @@ GDNX_DEV void run_schedule(const TcParams& P, Small& sm) {
     if (more) {
       const Seg g(P, w);
       const int i = lane / npp;
-      x.ids[lane] = i < g.n ? page_of(P.a.cache, w.s.row, w.s.len(), g.tile(i), lane % npp) : -1;
+      x.ids[lane] = i < g.n ? table_entry(P.a.cache, w.s.row, w.s.len(), g.tile(i), lane % npp) : -1;
       if (lane == 0) {
         x.g = g;
         x.row = w.s.row;
@@ -575,13 +574,14 @@ GDNX_DEV void run_loads(const TcParams& P, Small& sm, uint8_t* base, uint32_t sm
     // page ids of tiles from .. from + ahead - 1, a lane's each, and of those behind them
     const auto read = [&](int first) {
       const int i = first + lane / npp;
-      return i < g.n ? page_of(c, row, len, g.tile(i), lane % npp) : -1;
+      return i < g.n ? table_entry(c, row, len, g.tile(i), lane % npp) : -1;
     };
-    int from = 0, ids = w.ids[lane], next = ahead < g.n ? read(ahead) : -1;
+    const auto in_pool = [&](int id) { return id < c.pages ? id : -1; };
+    int from = 0, ids = in_pool(w.ids[lane]), next = ahead < g.n ? read(ahead) : -1;
     const auto load = [&](int i, int side, Place at) {
       if (i >= from + ahead) {  // (a step's two tiles lie in one reading: their number is even, or one)
         from += ahead;
-        ids = next;
+        ids = in_pool(next);
         if (from + ahead < g.n) next = read(from + ahead);
       }
       const int id = __shfl_sync(0xffffffffu, ids, ((i - from) * npp + pg) & 31);
@@ -685,6 +685,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
   const int warp = uniform(threadIdx.x / 32);
   dependents_may_start();
   if (threadIdx.x == 288) {
+    // what is read first is looked up (and its pages' addresses) under the set-up
+    for (const int32_t* p : {P.a.starts, P.a.first, P.a.rows, (const int32_t*)P.a.cache.table})
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&P.kv)) : "memory");
     if (P.tma_q) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&P.q)) : "memory");
   }
