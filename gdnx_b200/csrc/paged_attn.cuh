@@ -33,6 +33,7 @@ struct ChunkParams {
   int groups, gs, tb;  // groups of a key head's queries, heads of a group, tokens of a block
   int rows;            // rows of a part
   int cut;             // some unit may be cut
+  int vec_join;        // four values of y lie aligned
 };
 
 // The new tokens of one sequence: rows start .. start + count - 1 of the packed tensors, at positions first ...
@@ -292,9 +293,11 @@ GDNX_DEV float lse_of(float top, float sum) {
   return sum > 0.f ? (top + log2f(sum)) * kLn2 : top == -INFINITY ? -INFINITY : NAN;
 }
 
-// Joins a cut unit's parts, CTA after CTA: block (c, y) rows 8 y .. 8 y + 7 of the unit that ends in CTA c.  A warp
-// takes a row; where there are many parts, all eight warps take each row, a run of the parts each, joined in order.
-constexpr int JOIN_WARPS = 8;
+// Joins a cut unit's parts, CTA after CTA: block (c, y) rows JOIN_ROWS y .. of the unit that ends in CTA c.  Eight lanes
+// share a row, which keeps the work that a row needs once to an eighth of a warp (a row to a warp took 26 us where 4096
+// tokens of 16 heads are cut for 148 CTAs, now JOINED).  Where there are many parts, all eight warps take each row, a
+// run of the parts each, joined in order.
+constexpr int JOIN_WARPS = 8, JOIN_ROWS = 64;
 
 template <class S>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_attn_join_kernel(const ChunkParams P) {
@@ -309,16 +312,65 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_attn_join_kernel(const 
   const int G = (int)(a.H / a.cache.Hk), h0 = j.hg / P.groups * G + j.hg % P.groups * P.gs;
   const int heads = min(P.gs, G - j.hg % P.groups * P.gs), t0 = j.u * (S::PAIR ? 2 * P.tb : P.tb);
   const auto place = [&](int c, int r) { return ((int64_t)c * 2 + (c == j.c0)) * P.rows + r; };
-  // the token of row r in the chunk, or -1
-  const auto token = [&](int r) {
-    const int q = r % S::ROWS, t = t0 + r / S::ROWS * P.tb + q / P.gs;
-    return q / P.gs < P.tb && q % P.gs < heads && t < s.count ? t : -1;
+  // the packed row and head of row r, or -1
+  const auto query = [&](int r, int& head) {
+    const int q = r % S::ROWS, tok = q / P.gs, t = t0 + r / S::ROWS * P.tb + tok;
+    head = h0 + q - tok * P.gs;
+    return tok < P.tb && head < h0 + heads && t < s.count ? s.start + t : -1;
   };
-  // maximum, sum and four values of parts c = from..to-1 of row r
-  const auto add = [&](int r, int from, int to, float& m, float& l, float4& y) {
-    m = -INFINITY;
-    l = 0.f;
-    y = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int parts = j.c1 - j.c0 + 1, r0 = blockIdx.y * JOIN_ROWS, r1 = min(r0 + JOIN_ROWS, P.rows);
+  if (parts <= 8) {
+    const int d0 = lane % 8 * 4;  // this lane's values: four of each 32
+    for (int r = r0 + warp * 4 + lane / 8; r < r1; r += JOIN_WARPS * 4) {
+      int head;
+      const int64_t tok = query(r, head);
+      if (tok < 0) continue;
+      float m = -INFINITY, l = 0.f;
+      for (int c = j.c0; c <= j.c1; ++c) m = fmaxf(m, P.stat[place(c, r) * 2]);
+      const float base = m == -INFINITY ? 0.f : m;
+      float4 y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = j.c0; c <= j.c1; ++c) {
+        const int64_t at = place(c, r);
+        const float2 st = *reinterpret_cast<const float2*>(P.stat + at * 2);
+        const float w = exp2f(st.x - base);
+        const float* x = P.part + at * D + d0;
+        l = fmaf(w, st.y, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d0 + 32 * e < D) {
+            const float4 v = *reinterpret_cast<const float4*>(x + 32 * e);
+            y[e] = make_float4(fmaf(w, v.x, y[e].x), fmaf(w, v.y, y[e].y), fmaf(w, v.z, y[e].z), fmaf(w, v.w, y[e].w));
+          }
+      }
+      const float f = scale_of(m, l);
+      const int64_t out = tok * a.y_st + head * a.y_sh + d0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d0 + 32 * e < D) {
+          const float v[4] = {y[e].x * f, y[e].y * f, y[e].z * f, y[e].w * f};
+          if (P.vec_join && a.y_dtype != GDNX_F32) {
+            const bool bf = a.y_dtype == GDNX_BF16;
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + out + 32 * e) =
+                make_uint2(bf ? pack2<true>(v[0], v[1]) : pack2<false>(v[0], v[1]), bf ? pack2<true>(v[2], v[3]) : pack2<false>(v[2], v[3]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st_from_f32(a.y, a.y_dtype, out + 32 * e + i, v[i]);
+          }
+        }
+      if (a.lse && d0 == 0) a.lse[tok * a.H + head] = lse_of(m, l);
+    }
+    return;
+  }
+  const int run = (parts + JOIN_WARPS - 1) / JOIN_WARPS;
+  const int from = min(j.c0 + warp * run, j.c1 + 1), to = min(from + run, j.c1 + 1);
+  for (int r = r0; r < r1; ++r) {
+    int head;
+    const int64_t tok = query(r, head);
+    if (tok < 0) continue;
+    float m = -INFINITY, l = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = from + lane; c < to; c += 32) m = fmaxf(m, P.stat[place(c, r) * 2]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -330,35 +382,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_attn_join_kernel(const 
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (lane * 4 < D) x = *reinterpret_cast<const float4*>(P.part + at * D + lane * 4);
       l = fmaf(w, P.stat[at * 2 + 1], l);
-      y.x = fmaf(w, x.x, y.x);
-      y.y = fmaf(w, x.y, y.y);
-      y.z = fmaf(w, x.z, y.z);
-      y.w = fmaf(w, x.w, y.w);
+      y = make_float4(fmaf(w, x.x, y.x), fmaf(w, x.y, y.y), fmaf(w, x.z, y.z), fmaf(w, x.w, y.w));
     }
-  };
-  const int parts = j.c1 - j.c0 + 1, r0 = blockIdx.y * JOIN_WARPS;
-  if (parts <= 8) {
-    const int r = r0 + warp, t = token(r);
-    if (t < 0) return;
-    float m, l;
-    float4 y;
-    add(r, j.c0, j.c1 + 1, m, l, y);
-    const float f = scale_of(m, l), v[4] = {y.x, y.y, y.z, y.w};
-    const int64_t tok = s.start + t, h = h0 + r % S::ROWS % P.gs;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane * 4 + e < D) st_from_f32(a.y, a.y_dtype, tok * a.y_st + h * a.y_sh + lane * 4 + e, v[e] * f);
-    if (a.lse && lane == 0) a.lse[tok * a.H + h] = lse_of(m, l);
-    return;
-  }
-  const int run = (parts + JOIN_WARPS - 1) / JOIN_WARPS;
-  for (int r = r0; r < r0 + JOIN_WARPS; ++r) {
-    const int t = token(r);
-    if (t < 0) continue;
-    const int from = min(j.c0 + warp * run, j.c1 + 1), to = min(from + run, j.c1 + 1);
-    float m, l;
-    float4 y;
-    add(r, from, to, m, l, y);
     *reinterpret_cast<float4*>(&red_o[warp][lane * 4]) = y;
     if (lane == 0) {
       red_m[warp] = m;
@@ -377,9 +402,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_attn_join_kernel(const 
         sum = fmaf(w, red_l[i], sum);
         v = fmaf(w, red_o[i][d], v);
       }
-      const int64_t tok = s.start + t, h = h0 + r % S::ROWS % P.gs;
-      st_from_f32(a.y, a.y_dtype, tok * a.y_st + h * a.y_sh + d, v * scale_of(top, sum));
-      if (a.lse && d == 0) a.lse[tok * a.H + h] = lse_of(top, sum);
+      st_from_f32(a.y, a.y_dtype, tok * a.y_st + head * a.y_sh + d, v * scale_of(top, sum));
+      if (a.lse && d == 0) a.lse[tok * a.H + head] = lse_of(top, sum);
     }
     __syncthreads();
   }
@@ -406,6 +430,7 @@ ChunkParams plan_chunks(const gdnx_paged_attn_args& a, int ctas) {
   const int64_t units = (a.tokens / P.tb + a.n) * a.cache.Hk * P.groups;
   const int64_t want = P.cut ? (units * w + S::LEAST - 1) / S::LEAST : units;
   P.grid = (int)(want < ctas ? (want > 0 ? want : 1) : ctas);
+  P.vec_join = reinterpret_cast<uintptr_t>(a.y) % 8 == 0 && a.y_st % 4 == 0 && a.y_sh % 4 == 0;
   P.part = static_cast<float*>(a.workspace);
   P.stat = P.part + (size_t)P.grid * 2 * P.rows * a.cache.D;
   P.joint = reinterpret_cast<Joint*>(P.stat + (size_t)P.grid * 2 * P.rows * 2);
@@ -420,7 +445,7 @@ inline size_t chunk_bytes(const ChunkParams& P) {
 template <class S>
 gdnx_status join_chunks(const ChunkParams& P, cudaStream_t st) {
   if (!P.cut) return GDNX_OK;
-  const cudaError_t e = launch_early(paged_attn_join_kernel<S>, dim3((unsigned)P.grid, (unsigned)(P.rows / JOIN_WARPS)),
+  const cudaError_t e = launch_early(paged_attn_join_kernel<S>, dim3((unsigned)P.grid, (unsigned)((P.rows + JOIN_ROWS - 1) / JOIN_ROWS)),
                                      dim3(JOIN_WARPS * 32), 0, st, P);
   return e == cudaSuccess ? GDNX_OK : GDNX_ELAUNCH;
 }

@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
     const int64_t len = length_of(c, rows[i]);
     const int64_t have = pages_of(c, len), want = pages_of(c, len + counts[i]);
     shared = -1;
-    if (counts[i] > 0 && len % c.page) {
+    if (counts[i] > 0 && (len & (c.page - 1))) {
       const int tail = c.table[rows[i] * c.width + have - 1];
       if (!page_ok(c, tail)) lost = true;
       else if (c.refs[tail] > 1) shared = tail;

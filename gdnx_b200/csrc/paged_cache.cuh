@@ -33,7 +33,8 @@ GDNX_DEV bool rows_ok(uint32_t* seen, const gdnx_cache& c, int64_t n, const int3
 
 GDNX_DEV bool page_ok(const gdnx_cache& c, int p) { return p >= 0 && p < c.pages; }
 
-GDNX_DEV int64_t pages_of(const gdnx_cache& c, int64_t tokens) { return (tokens + c.page - 1) / c.page; }
+// (A page has a power of two tokens.)
+GDNX_DEV int64_t pages_of(const gdnx_cache& c, int64_t tokens) { return (tokens + c.page - 1) >> (31 - __clz(c.page)); }
 
 // A slot's length, kept within what its row can hold.
 GDNX_DEV int64_t length_of(const gdnx_cache& c, int row) {

@@ -13,9 +13,8 @@
 // the lane's partner.  (With a page to four lanes and the queries in shared memory, the reads of these took 70 us for
 // 64 x 4 key heads of up to 256 pages; now MEASURED.)
 //
-// Of up to RANKED words each thread ranks one against all others.  Of more, the k-th largest is found two bits at a
-// time among their places between the least and the greatest, in 32 bits from registers; the search ends as soon as just
-// k lie at or above, and goes on in 64 bits where places fall together.
+// Of up to RANKED words each thread ranks one against all others.  Of more, the words are counted in 256 parts of their
+// range, and those of the part that the k-th largest lies in again, until they are few enough to be ranked.
 #include <type_traits>
 
 #include "attn_tc.cuh"
@@ -257,10 +256,11 @@ GDNX_DEV int rank_of(bool on, int* warp_sums, int* total) {
 // The k largest of n words (0: none), the lower index first among equals, in rising order; -1 behind them.
 template <int THREADS>
 GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t* out) {
-  constexpr int WARPS = THREADS / 32, HELD = 4;
+  constexpr int WARPS = THREADS / 32;
   static_assert(RANKED <= THREADS, "a word for each thread");
-  __shared__ int sums[2][3][WARPS];
-  __shared__ unsigned long long ends[2][WARPS];
+  __shared__ int sums[2][WARPS];
+  __shared__ unsigned long long ends[2][WARPS], few[RANKED], last;
+  __shared__ int few_at[RANKED], hist[256], found[3];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   if (n <= RANKED) {
     const unsigned long long w = (int)threadIdx.x < n ? keys[threadIdx.x] : 0;
@@ -277,7 +277,7 @@ GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t
     }
     int all;
     const bool on = w != 0 && above < k;
-    const int r = rank_of<THREADS>(on, sums[0][0], &all);
+    const int r = rank_of<THREADS>(on, sums[0], &all);
     if (on) out[r] = (int)threadIdx.x;
     for (int i = all + threadIdx.x; i < k; i += THREADS) out[i] = -1;
     return;
@@ -307,107 +307,110 @@ GDNX_DEV void take_largest(const unsigned long long* keys, int n, int k, int32_t
   if (lane == 0) {
     ends[0][warp] = least;
     ends[1][warp] = most;
-    sums[1][0][warp] = there;
-    sums[1][1][warp] = always;
+    sums[0][warp] = there;
+    sums[1][warp] = always;
   }
   __syncthreads();
   least = lane < WARPS ? ends[0][lane] : ~0ull;
   most = lane < WARPS ? ends[1][lane] : 0;
   span(least, most);
-  there = __reduce_add_sync(0xffffffffu, lane < WARPS ? sums[1][0][lane] : 0);
-  always = __reduce_add_sync(0xffffffffu, lane < WARPS ? sums[1][1][lane] : 0);
-  // A word's place between the ends in 32 bits: 0 for one that is not there, all ones for one always taken.  The
-  // first words' places stay in registers.
-  const int shift = most > least ? max(0, 33 - __clzll(most - least)) : 0;
-  const auto place = [&](unsigned long long w) {
-    return w == 0 ? 0u : w == ~0ull ? 0xffffffffu : (uint32_t)((w - least) >> shift) + 1;
-  };
-  uint32_t held[HELD];
-#pragma unroll
-  for (int e = 0; e < HELD; ++e) {
-    const int i = e * THREADS + threadIdx.x;
-    held[e] = i < n ? place(keys[i]) : 0;
-  }
-  // Words whose place is at least t + 1, + 2, + 3 times `one`, in every thread.  (Two places for the sums in turn: one
-  // barrier a count.)
-  int turn = 0;
-  const auto total = [&](int (&mine)[3]) {
-#pragma unroll
-    for (int e = 0; e < 3; ++e) {
-      const int s = __reduce_add_sync(0xffffffffu, mine[e]);
-      if (lane == 0) sums[turn][e][warp] = s;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 3; ++e) mine[e] = __reduce_add_sync(0xffffffffu, lane < WARPS ? sums[turn][e][lane] : 0);
-    turn ^= 1;
-  };
-  uint32_t bar = 1;   // places from here on are taken
-  int above = there;  // words there
+  there = __reduce_add_sync(0xffffffffu, lane < WARPS ? sums[0][lane] : 0);
+  always = __reduce_add_sync(0xffffffffu, lane < WARPS ? sums[1][lane] : 0);
+  // Taken is what lies above `bar`, and of the words equal to it those up to index `end`.
+  unsigned long long bar = 0;
+  int end = -1;
   if (there > k) {
-    bar = 0;
-    above = n;
-    for (int bit = 30; bit >= 0 && above != k; bit -= 2) {
-      int got[3] = {0, 0, 0};
-      const auto look = [&](uint32_t w) {
-#pragma unroll
-        for (int e = 0; e < 3; ++e) got[e] += w >= bar + ((uint32_t)(e + 1) << bit);
-      };
-#pragma unroll
-      for (int e = 0; e < HELD; ++e) look(held[e]);
-      for (int i = HELD * THREADS + threadIdx.x; i < n; i += THREADS) look(place(keys[i]));
-      total(got);
-#pragma unroll
-      for (int e = 2; e >= 0; --e)
-        if (got[e] >= k) {
-          bar += (uint32_t)(e + 1) << bit;
-          above = got[e];
-          break;
-        }
-    }
-  }
-  // More than k at or above: those at the bar itself are told apart by what their places leave out.
-  unsigned long long edge = 0;  // of the words at the bar's place, those from here on
-  if (above > k && shift > 0) {
-    edge = least + ((unsigned long long)(bar - 1) << shift);
-    for (int bit = shift - 1; bit >= 0; --bit) {
-      int got[3] = {0, 0, 0};
-      for (int i = threadIdx.x; i < n; i += THREADS) got[0] += keys[i] >= edge + (1ull << bit);
-      total(got);
-      if (got[0] >= k) {
-        edge += 1ull << bit;
-        above = got[0];
-        if (above == k) break;
+    // the need-th largest of the `inside` words from least to most is the last that is taken
+    int need = k - always, inside = there - always;
+    while (need > 0 && inside > RANKED && least < most) {
+      // how many of them lie in each 256th of their range
+      const int shift = max(0, 56 - __clzll(most - least));
+      for (int i = threadIdx.x; i < 256; i += THREADS) hist[i] = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += THREADS) {
+        const unsigned long long w = keys[i];
+        if (w >= least && w <= most) atomicAdd(&hist[(int)((w - least) >> shift)], 1);
       }
+      __syncthreads();
+      if (warp == 0) {  // from the highest: a lane has eight parts
+        int mine = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mine += hist[255 - (lane * 8 + e)];
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += x;
+        }
+        if (upto >= need && upto - mine < need) {
+          int before = upto - mine, e = 0;
+          while (before + hist[255 - (lane * 8 + e)] < need) before += hist[255 - (lane * 8 + e++)];
+          found[0] = 255 - (lane * 8 + e);
+          found[1] = before;
+          found[2] = hist[255 - (lane * 8 + e)];
+        }
+      }
+      __syncthreads();
+      need -= found[1];
+      inside = found[2];
+      least += (unsigned long long)found[0] << shift;
+      const unsigned long long top = least + ((1ull << shift) - 1);
+      most = top < most ? top : most;
+      __syncthreads();  // found and hist may be written again
+    }
+    if (need <= 0) {
+      bar = ~0ull - 1;  // those always taken are all
+    } else if (inside <= RANKED) {
+      if (threadIdx.x == 0) found[0] = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += THREADS) {
+        const unsigned long long w = keys[i];
+        if (w >= least && w <= most) {
+          const int at = atomicAdd(&found[0], 1);  // in any order: the ranks do not depend on it
+          few[at] = w;
+          few_at[at] = i;
+        }
+      }
+      __syncthreads();
+      if ((int)threadIdx.x < inside) {
+        const unsigned long long w = few[threadIdx.x];
+        const int at = few_at[threadIdx.x];
+        int above = 0;
+        for (int i = 0; i < inside; ++i) above += few[i] > w || (few[i] == w && few_at[i] < at);
+        if (above == need - 1) {
+          last = w;
+          found[1] = at;
+        }
+      }
+      __syncthreads();
+      bar = last;
+      end = found[1];
+    } else {  // all alike: the need-th of them
+      bar = least;
+      int before = 0;
+      for (int i0 = 0; i0 < n && before < need; i0 += THREADS) {
+        const int i = i0 + threadIdx.x;
+        const bool on = i < n && keys[i] == bar;
+        int all;
+        const int r = rank_of<THREADS>(on, sums[0], &all);
+        if (on && before + r == need - 1) found[1] = i;
+        before += all;
+      }
+      __syncthreads();
+      end = found[1];
     }
   }
-  // Of the words equal to the last that is taken, the first ones.
-  const auto taken_from = [&](unsigned long long w, uint32_t p) { return edge ? w >= edge : p >= bar; };
-  int equal = n;
-  if (above > k) {
-    int got[3] = {0, 0, 0};
-    for (int i = threadIdx.x; i < n; i += THREADS) got[0] += edge ? keys[i] > edge : place(keys[i]) > bar;
-    total(got);
-    equal = k - got[0];
-  }
-  int taken = 0, ties = 0;
+  int taken = 0;
   for (int i0 = 0; i0 < n && taken < k; i0 += THREADS) {
     const int i = i0 + threadIdx.x;
     const unsigned long long w = i < n ? keys[i] : 0;
-    const uint32_t p = place(w);
+    const bool on = w > bar || (w == bar && w != 0 && i <= end);
     int all;
-    bool on = i < n && w != 0 && taken_from(w, p);
-    if (above > k) {
-      const bool same = on && (edge ? w == edge : p == bar);
-      const int r = rank_of<THREADS>(same, sums[0][0], &all);
-      if (same) on = ties + r < equal;
-      ties += all;
-    }
-    const int r = rank_of<THREADS>(on, sums[1][0], &all);
-    if (on) out[taken + r] = i;
+    const int r = rank_of<THREADS>(on, sums[0], &all);
+    if (on && taken + r < k) out[taken + r] = i;
     taken += all;
   }
-  for (int i = taken + threadIdx.x; i < k; i += THREADS) out[i] = -1;
+  for (int i = min(taken, k) + threadIdx.x; i < k; i += THREADS) out[i] = -1;
 }
 
 // FUSED: one CTA for each query and key head scores its pages and takes the largest; else CTA (x, unit) leaves the

@@ -181,7 +181,7 @@ template <typename T>
 cudaError_t bounds_of(const gdnx_cache& c, int64_t layer, int64_t n, const int32_t* rows, const int32_t* counts,
                       void* bounds, cudaStream_t st) {
   // as many CTAs as keep the device busy; where the pages of a call are fewer, the others find none
-  const int64_t y = n < 65535 ? n : 65535, fill = (int64_t)sm_count() * 16 / (c.Hk * y), z = fill < 1 ? 1 : fill < c.width ? fill : c.width;
+  const int64_t y = n < 65535 ? n : 65535, fill = (int64_t)sm_count() * 8 / (c.Hk * y), z = fill < 1 ? 1 : fill < c.width ? fill : c.width;
   return launch_early(cache_bounds_kernel<T>, dim3((unsigned)c.Hk, (unsigned)y, (unsigned)(z < 65535 ? z : 65535)),
                       dim3(BOUNDS_NT), seen_bytes(c), st, c, layer, n, rows, counts, static_cast<uint4*>(bounds));
 }
