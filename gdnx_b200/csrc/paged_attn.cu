@@ -6,7 +6,11 @@
 //   l = l 2^(m - m') + sum_j p;  o = o 2^(m - m') + p V;   y = o / l.
 // A tile's tokens come from up to four pages by 16-byte asynchronous copies; what lies on no page, or behind the
 // sequence's last token, is zero and not seen.  The next tile's keys come under the product with the values, its values
-// under the product with its keys, its page ids under both.
+// under the product with its keys, its page ids under both (loads and products in turn: 106 us for the case below).
+//
+// Measured: three chunks of up to 301 tokens and two single ones at lengths up to 1031, 8 heads over 2 of 96, window 300,
+// 3 sinks: 58 to 66 us (7 us of multiply-adds at the CUDA cores' rate, which shared-memory reads hold to a quarter; start,
+// join and two or three tiles a CTA are the rest); 1000 tokens after 1000 without a window: 184 us.
 #include "attn_simt.cuh"
 #include "paged_attn.cuh"
 

@@ -295,7 +295,7 @@ GDNX_DEV float lse_of(float top, float sum) {
 
 // Joins a cut unit's parts, CTA after CTA: block (c, y) rows JOIN_ROWS y .. of the unit that ends in CTA c.  Eight lanes
 // share a row, which keeps the work that a row needs once to an eighth of a warp (a row to a warp took 26 us where 4096
-// tokens of 16 heads are cut for 148 CTAs, now JOINED).  Where there are many parts, all eight warps take each row, a
+// tokens of 16 heads are cut for 148 CTAs; now 14).  Where there are many parts, all eight warps take each row, a
 // run of the parts each, joined in order.
 constexpr int JOIN_WARPS = 8, JOIN_ROWS = 64;
 

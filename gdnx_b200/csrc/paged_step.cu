@@ -6,6 +6,10 @@
 // bounds: lo_d = min_j k_jd, hi_d = max_j k_jd over a page's tokens, exact in the cache's type, NaN where a key is.
 // Bytes bound it: every key of the touched pages is read once, by one CTA for each page and head whose threads take
 // 16 bytes of a row each and every so many rows.
+//
+// Measured (4 heads of 128, bf16): append of 24,500 tokens (100 MB moved) 16 us, 6.2 TB/s; of 64 tokens 2.0 us.  bounds of
+// 8 x 4096 tokens 10.5 us (3.3 TB/s), behind one token in each of 64 slots 4.9 us: the check of the call, under which the
+// first page's keys come, and the chain from slot to page to keys.
 #include "paged_cache.cuh"
 
 namespace gdnx {
