@@ -700,8 +700,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
   dependents_may_start();
   if (threadIdx.x == 288) {
     // what is read first is looked up (and its pages' addresses) under the set-up
-    for (const int32_t* p : {P.a.starts, P.a.first, P.a.rows, (const int32_t*)P.a.cache.table})
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+    if (P.a.n > 0)
+      for (const int32_t* p : {P.a.starts, P.a.first, P.a.rows, (const int32_t*)P.a.cache.table})
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&P.kv)) : "memory");
     if (P.tma_q) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&P.q)) : "memory");
   }

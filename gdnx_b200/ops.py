@@ -1103,6 +1103,13 @@ class PagedCache:
                           torch.zeros(L_, 2, pages, Hk, D, dtype=dtype, device=device) if bounds else None)
 
 
+def _output(q, dtype):
+    """A contiguous tensor of q's shape (dtype None: and type), by the cheapest call."""
+    if dtype is not None:
+        return q.new_empty(q.shape, dtype=dtype)
+    return torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
+
+
 def _cache_struct(c: PagedCache):
     """The cache as the C ABI takes it, and its device's index."""
     kv, table, lengths, refs, status = c.kv, c.table, c.lengths, c.refs, c.status
@@ -1279,7 +1286,7 @@ def cache_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, step: Page
     if not 0 <= layer < s.L:
         raise ValueError("no such layer")
     places = step.places
-    if places.dtype is not torch.int64 or places.dim() != 1 or not places.is_contiguous() or places.shape[0] != k.shape[0]:
+    if places.dtype is not torch.int64 or places.dim() != 1 or not places.is_contiguous() or places.numel() != k.shape[0]:
         raise ValueError("the step must have k's rows")
     _on_device(index, places)
     _enqueue("gdnx_cache_append", index, C.byref(s), layer, k.shape[0], C.byref(_packed_view(k)), C.byref(_packed_view(v)),
@@ -1299,7 +1306,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, step: PagedStep, *, laye
     it only sizes the split over the cache's length.  Returns y [tokens,H,D] (and the log of the sum of exponentials
     [tokens,H] fp32 if asked, -inf where a row is padding or sees nothing)."""
     s, index = _cache_struct(cache)
-    _on_device(index, q)
+    if q.get_device() != index:
+        _on_device(index, q)
     if q.dim() != 3:
         raise ValueError("q must be [tokens,H,D]")
     N, H, D = q.shape
@@ -1307,7 +1315,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, step: PagedStep, *, laye
         raise ValueError("q must be [tokens,H,D] with the cache's head size and H a multiple of its heads")
     if q.dtype is not cache.kv.dtype:
         raise TypeError("q must have the cache's type")
-    if step.positions.shape[0] != N:
+    if step.positions.numel() != N:
         raise ValueError("the step must have q's rows")
     if window is None:
         window = 1 << 62
@@ -1316,7 +1324,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, step: PagedStep, *, laye
     if not 0 <= layer < s.L:
         raise ValueError("no such layer")
     if out is None:
-        y = q.new_empty(q.shape) if out_dtype is None else q.new_empty(q.shape, dtype=out_dtype)
+        y = _output(q, out_dtype)
     else:
         y = out
         _on_device(index, y)
@@ -1367,7 +1375,8 @@ def paged_select(q: torch.Tensor, cache: PagedCache, k: int, *, layer: int = 0, 
     pages), then those of largest score, the lower page first among equals.  Released pages are not taken.  ``max_len``,
     if known, is the longest slot's length; it only sizes the launch."""
     s, index = _cache_struct(cache)
-    _on_device(index, q)
+    if q.get_device() != index:
+        _on_device(index, q)
     if q.dim() != 3:
         raise ValueError("q must be [B,H,D]")
     B, H, D = q.shape
@@ -1416,7 +1425,8 @@ def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Op
     pages that their lists name, as indexes into the slot's table row, each once.  As many entries of a list are read as
     the slot has pages up to the position; others than the slot's are passed over.  Returns [B,H,D]."""
     s, index = _cache_struct(cache)
-    _on_device(index, q)
+    if q.get_device() != index:
+        _on_device(index, q)
     if q.dim() != 3:
         raise ValueError("q must be [B,H,D]")
     B, H, D = q.shape
@@ -1431,7 +1441,7 @@ def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Op
     if not 0 <= layer < s.L:
         raise ValueError("no such layer")
     if out is None:
-        y = q.new_empty(q.shape) if out_dtype is None else q.new_empty(q.shape, dtype=out_dtype)
+        y = _output(q, out_dtype)
     else:
         y = out
         _on_device(index, y)
