@@ -275,10 +275,12 @@ GDNX_DEV void zero_rows(const ChunkParams& P, int64_t r0, int64_t r1, int i, int
       if (a.lse && x % D == 0) a.lse[t * a.H + x / D] = -INFINITY;
     }
 }
-// Padding rows: those behind the last sequence, and sequences that have no tokens after all.
+// Padding rows: those before the first sequence and behind the last, and sequences that have no tokens after all.
 GDNX_DEV void write_padding(const ChunkParams& P, int i, int threads) {
   const gdnx_paged_attn_args& a = P.a;
+  const int64_t begin = a.n ? min((int64_t)max(a.starts[0], 0), a.tokens) : 0;
   const int64_t end = a.n ? min((int64_t)max(a.starts[a.n], 0), a.tokens) : 0;
+  for (int64_t t = blockIdx.x; t < begin; t += P.grid) zero_rows(P, t, t + 1, i, threads);
   for (int64_t t = end + blockIdx.x; t < a.tokens; t += P.grid) zero_rows(P, t, t + 1, i, threads);
   for (int64_t b = blockIdx.x; b < a.n; b += P.grid) {
     const Chunk s = make_chunk(a, b);

@@ -187,9 +187,6 @@ GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, 
       : "memory");
 }
 
-// A segment's tiles in the ring.  Two blocks: K0 V0 K1 V1 ...  One block: two tiles at a time, K0 K1 V0 V1 K2 K3 ...; a
-// last odd one K V.
-
 // Weights of N columns: p = 2^(c2 s - mc), summed, packed 16-bit.  One pair in eight is taken on the FMA pipes (where
 // masked scores give 2^-125: nothing beside a weight that counts).
 template <bool BF16, int N>
@@ -546,7 +543,8 @@ GDNX_DEV void run_schedule(const TcParams& P, Small& sm) {
   }
 }
 
-// A segment's places in order: f(tile, side (0: K, 1: V), place), until that is false.
+// A segment's places in order: f(tile, side (0: K, 1: V), place), until that is false.  Two blocks: K0 V0 K1 V1 ...  One
+// block: two tiles at a time, K0 K1 V0 V1 K2 K3 ...; a last odd one K V.
 template <int DB, typename F>
 GDNX_DEV bool for_places(const Ring<DB>& ring, const Seg& g, F f) {
   Place at = {0, 0};

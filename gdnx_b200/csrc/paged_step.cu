@@ -97,8 +97,8 @@ GDNX_DEV uint4 most4(uint4 a, uint4 b) {
 // once and in range, no more tokens than the slot has, and no partly filled last page that another slot holds too (which
 // may see more of it).
 GDNX_DEV bool bounds_ok(uint32_t* seen, const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* counts) {
-  if (*c.status != 0 || !rows_ok(seen, c, n, rows, nullptr, counts)) return false;
-  bool bad = false;
+  bool bad = *c.status != 0;  // (voted on below: another CTA may set it meanwhile)
+  if (!rows_ok(seen, c, n, rows, nullptr, counts)) return false;
   for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
     const int64_t len = length_of(c, rows[i]);
     bad |= counts[i] > len;

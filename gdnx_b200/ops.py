@@ -1301,10 +1301,11 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, step: PagedStep, *, laye
     contiguous last dim, H a multiple of the cache's heads.
 
     The token at position p of its slot sees the slot's token j <= p where p - j < ``window`` (None: no window) or
-    j < ``sinks``; tokens on released pages are not seen.  Padding rows give zeros.  A row that sees a score of NaN or
-    +inf, or only -inf, is NaN.  ``scale`` defaults to D ** -0.5.  ``max_len``, if known, is the longest slot's length;
-    it only sizes the split over the cache's length.  Returns y [tokens,H,D] (and the log of the sum of exponentials
-    [tokens,H] fp32 if asked, -inf where a row is padding or sees nothing)."""
+    j < ``sinks``; tokens on released pages are not seen.  Padding rows give zeros.  What lies on released pages or
+    behind a sequence's last token (NaN included) reaches no output; other values are meant to be finite.  A row that sees
+    a score of NaN or +inf, or only -inf, is NaN.  ``scale`` defaults to D ** -0.5.  ``max_len``, if known, is the longest
+    slot's length; it only sizes the split over the cache's length.  For serving: no gradients.  Returns y [tokens,H,D]
+    (and the log of the sum of exponentials [tokens,H] fp32 if asked, -inf where a row is padding or sees nothing)."""
     s, index = _cache_struct(cache)
     if q.get_device() != index:
         _on_device(index, q)
@@ -1353,7 +1354,8 @@ def cache_bounds(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor, *,
     """Brings ``cache.bounds`` up to date in ``layer`` after the last ``counts[i]`` tokens of slots ``rows`` were written
     (int32 vectors, each slot once): for every page on which one of them lies, the least and the greatest value of each
     dim among its tokens' keys, NaN where a key's is.  Exact.  Refused where a slot has fewer tokens, or its last page is
-    partly filled and held by another slot too (bring the bounds up to date before the fork)."""
+    partly filled and held by another slot too (bring the bounds up to date before the fork).  A page that
+    :func:`cache_step` or :func:`cache_extend` gives a slot, a copy of a shared one too, has no bounds before this."""
     s, index = _cache_struct(cache)
     at, n = _cache_rows(rows, s, index)
     if not 0 <= layer < s.L:

@@ -589,9 +589,10 @@ GDNX_API gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* args, void*
 /* Attention of a step's packed new tokens (of chunks of prompts, proposals, single tokens, mixed) over the cache that
  * holds them and what came before: row starts[i] + t of q stands at position p = first[i] + t of slot rows[i] (keys and
  * values written before the call) and sees the slot's token j <= p where p - j < window or j < sinks; tokens on released
- * pages are not seen.  Rows in no sequence (behind starts[n], or of a sequence that is no slot's or ends beyond the
- * table) give 0, their lse is -inf; so does a row that sees nothing.  A row that sees a score of NaN or +inf, or only
- * -inf, is NaN.  Scores, softmax statistics and sums are fp32; 16-bit caches run on the tensor cores.
+ * pages are not seen.  Rows in no sequence (before starts[0], behind starts[n], or of a sequence that is no slot's or
+ * ends beyond the table) give 0, their lse is -inf; so does a row that sees nothing.  A row that sees a score of NaN or +inf, or only
+ * -inf, is NaN.  What lies on released pages or behind a sequence's last token (NaN included) reaches no output; other
+ * values are meant to be finite.  Scores, softmax statistics and sums are fp32; 16-bit caches run on the tensor cores.
  * The work is split over CTAs by the lengths that it finds, and the parts joined in a fixed order. */
 typedef struct {
   gdnx_cache cache;

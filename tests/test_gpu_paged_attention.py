@@ -232,6 +232,20 @@ def test_steps_that_name_no_slots_give_zeros():
     assert (ops.paged_attention(q, c, none) == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_before_the_first_sequence_are_padding(dtype):
+    c = cache([100, 37], page=16, width=8, dtype=dtype)
+    good = packed(c, [0, 1], [20, 10])
+    q = torch.randn(47, 4, 64).to(TYPES[dtype]).to(DEV)
+    step = ops.PagedStep(good.rows, good.starts + 7, good.first, i32(*[0] * 47), i32(*[0] * 47), good.places)
+    y = torch.full_like(q, math.nan)
+    _, lse = ops.paged_attention(q, c, step, out=y, return_lse=True)
+    none = torch.arange(47, device=DEV)
+    none = (none < 7) | (none >= 37)
+    assert (y[none] == 0).all() and (lse[none] == -math.inf).all()
+    close(y[7:37], plain(q[7:37], c, good)[0], dtype)
+
+
 def test_one_token_agrees_with_decode_and_prompts_with_window_attention():
     for dtype in TYPES:
         c = cache([200, 64, 1, 90], page=16, Hk=2, D=64, dtype=dtype, width=14)
