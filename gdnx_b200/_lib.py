@@ -23,7 +23,7 @@ EXPORTED = ("gdnx_scan_fwd", "gdnx_scan_fwd_noalloc", "gdnx_scan_noalloc_status"
             "gdnx_epilogue_scatter", "gdnx_device_alloc", "gdnx_device_free", "gdnx_ipc_handle", "gdnx_ipc_open",
             "gdnx_ipc_close", "gdnx_error_word", "gdnx_error_status", "gdnx_attn_fwd", "gdnx_attn_bwd", "gdnx_attn_bwd_workspace_bytes", "gdnx_cache_fork",
             "gdnx_cache_extend", "gdnx_cache_write", "gdnx_cache_truncate", "gdnx_cache_trim", "gdnx_cache_compact",
-            "gdnx_cache_compact_bounds", "gdnx_cache_step", "gdnx_cache_append", "gdnx_cache_bounds",
+            "gdnx_cache_compact_bounds", "gdnx_cache_step", "gdnx_cache_step_rows", "gdnx_cache_append", "gdnx_cache_bounds",
             "gdnx_paged_attn", "gdnx_paged_attn_workspace_bytes", "gdnx_paged_select", "gdnx_paged_select_workspace_bytes",
             "gdnx_cache_workspace_bytes", "gdnx_paged_decode", "gdnx_paged_decode_workspace_bytes")
 
@@ -235,6 +235,7 @@ def load(path: Path = LIB_PATH):
                         ("truncate", [cache, i64, ptr, ptr, ptr]), ("trim", [cache, i64, ptr, i64, i64, ptr]),
                         ("compact", [cache, ptr, size, ptr]), ("compact_bounds", [cache, ptr, ptr, size, ptr]),
                         ("step", [cache, i64, ptr, ptr, C.POINTER(Step), ptr, size, ptr]),
+                        ("step_rows", [cache, i64, ptr, ptr, C.POINTER(Step), ptr, ptr, size, ptr]),
                         ("append", [cache, i64, i64, C.POINTER(View), C.POINTER(View), ptr, ptr]),
                         ("bounds", [cache, i64, i64, ptr, ptr, ptr, ptr])):
         fn = getattr(lib, "gdnx_cache_" + name)

@@ -290,15 +290,28 @@ gdnx_status gdnx_cache_compact_bounds(const gdnx_cache* c, void* bounds, void* w
   return gdnx::launch_cache_compact(*c, bounds, workspace, (cudaStream_t)stream);
 }
 
-gdnx_status gdnx_cache_step(const gdnx_cache* c, int64_t n, const int32_t* rows, const int32_t* counts,
-                            const gdnx_step* step, void* workspace, size_t workspace_bytes, void* stream) {
+static gdnx_status cache_step(const gdnx_cache* c, int64_t n, const int32_t* rows, const int32_t* counts,
+                              const gdnx_step* step, int32_t* rows_out, void* workspace, size_t workspace_bytes,
+                              void* stream) {
   const gdnx_status s = check_rows(c, n, rows, counts);
   if (s != GDNX_OK) return s;
   if (!step || step->tokens < 0 || !words(step->starts) || (n && !words(step->first))) return GDNX_EINVAL;
   if (step->tokens > kMaxPacked) return GDNX_EUNSUPPORTED;
   if (step->tokens && (!words(step->token_rows) || !words(step->positions) || !device_ptr(step->places, 8))) return GDNX_EINVAL;
   if (workspace_bytes < gdnx_cache_workspace_bytes(c, n) || !device_ptr(workspace, sizeof(int32_t))) return GDNX_EWORKSPACE;
-  return gdnx::launch_cache_step(*c, n, rows, counts, *step, workspace, (cudaStream_t)stream);
+  return gdnx::launch_cache_step(*c, n, rows, counts, *step, rows_out, workspace, (cudaStream_t)stream);
+}
+
+gdnx_status gdnx_cache_step(const gdnx_cache* c, int64_t n, const int32_t* rows, const int32_t* counts,
+                            const gdnx_step* step, void* workspace, size_t workspace_bytes, void* stream) {
+  return cache_step(c, n, rows, counts, step, nullptr, workspace, workspace_bytes, stream);
+}
+
+gdnx_status gdnx_cache_step_rows(const gdnx_cache* c, int64_t n, const int32_t* rows, const int32_t* counts,
+                                 const gdnx_step* step, int32_t* rows_out, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  if (n > 0 && !words(rows_out)) return GDNX_EINVAL;
+  return cache_step(c, n, rows, counts, step, rows_out, workspace, workspace_bytes, stream);
 }
 
 gdnx_status gdnx_cache_append(const gdnx_cache* c, int64_t layer, int64_t tokens, const gdnx_view* k,

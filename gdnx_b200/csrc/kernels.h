@@ -36,8 +36,9 @@ gdnx_status launch_cache_trim(const gdnx_cache& c, int64_t n, const int32_t* row
                               cudaStream_t st);
 // `bounds`: moved along where given.
 gdnx_status launch_cache_compact(const gdnx_cache& c, void* bounds, void* ws, cudaStream_t st);
+// `rows_out`: takes a copy of `rows` where given.
 gdnx_status launch_cache_step(const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* counts,
-                              const gdnx_step& step, void* ws, cudaStream_t st);
+                              const gdnx_step& step, int32_t* rows_out, void* ws, cudaStream_t st);
 gdnx_status launch_cache_append(const gdnx_cache& c, int64_t layer, int64_t tokens, const gdnx_view& k,
                                 const gdnx_view& v, const int64_t* places, cudaStream_t st);
 gdnx_status launch_cache_bounds(const gdnx_cache& c, int64_t layer, int64_t n, const int32_t* rows,

@@ -125,10 +125,12 @@ GDNX_DEV void load4(int (&r)[4], const gdnx_cache& c, int64_t p, int fill) {
   for (int e = 0; e < 4; ++e) r[e] = p + e < c.pages ? c.refs[p + e] : fill;
 }
 
-// STEP: also where the new tokens stand in a packed batch (`out.starts`, `out.first`; zeros where refused).
+// STEP: also where the new tokens stand in a packed batch (`out.starts`, `out.first`; zeros where refused), and a copy of
+// `rows` where the caller wants one.
 template <bool STEP>
 __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, int64_t n, const int32_t* rows,
-                                                          const int32_t* counts, void* ws, const gdnx_step out) {
+                                                          const int32_t* counts, void* ws, const gdnx_step out,
+                                                          int32_t* rows_out) {
   extern __shared__ uint32_t seen[];
   __shared__ int sums[32];
   __shared__ int ncopy;
@@ -145,6 +147,7 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
       for (int64_t i = threadIdx.x; i <= n; i += NT) {
         out.starts[i] = 0;
         if (i < n) out.first[i] = 0;
+        if (i < n && rows_out) rows_out[i] = rows[i];
       }
     if (threadIdx.x == 0 && status) *c.status = status;
   };
@@ -181,6 +184,7 @@ __global__ void __launch_bounds__(NT) cache_extend_kernel(const gdnx_cache c, in
       if (i < n) {
         out.starts[i] = (int)(packed + start);
         out.first[i] = (int)length_of(c, rows[i]);
+        if (rows_out) rows_out[i] = rows[i];
       }
       packed += sum;
     }
@@ -466,15 +470,15 @@ gdnx_status launch_cache_trim(const gdnx_cache& c, int64_t n, const int32_t* row
 gdnx_status launch_cache_extend(const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* counts, void* ws,
                                 cudaStream_t st) {
   if (launch_early(cache_extend_kernel<false>, dim3(1), dim3(NT), seen_bytes(c), st, c, n, rows, counts, ws,
-                   gdnx_step{}) != cudaSuccess)
+                   gdnx_step{}, nullptr) != cudaSuccess)
     return GDNX_ELAUNCH;
   return copy_pages<kMove>(c, ws, n, st);
 }
 
 gdnx_status launch_cache_step(const gdnx_cache& c, int64_t n, const int32_t* rows, const int32_t* counts,
-                              const gdnx_step& step, void* ws, cudaStream_t st) {
-  if (launch_early(cache_extend_kernel<true>, dim3(1), dim3(NT), seen_bytes(c), st, c, n, rows, counts, ws, step) !=
-      cudaSuccess)
+                              const gdnx_step& step, int32_t* rows_out, void* ws, cudaStream_t st) {
+  if (launch_early(cache_extend_kernel<true>, dim3(1), dim3(NT), seen_bytes(c), st, c, n, rows, counts, ws, step,
+                   rows_out) != cudaSuccess)
     return GDNX_ELAUNCH;
   return copy_pages<kPlace>(c, ws, n, st, rows, step);
 }

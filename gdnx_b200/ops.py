@@ -1238,7 +1238,8 @@ def cache_compact(cache: PagedCache) -> None:
 class PagedStep:
     """A serving step's new tokens, packed: sequence i's are rows ``starts[i]`` .. ``starts[i+1]-1`` of a packed tensor, the
     first of them at position ``first[i]`` of slot ``rows[i]``; rows from ``starts[-1]`` on are padding, -1 in the lists
-    of the packed rows.  One step serves every layer."""
+    of the packed rows.  One step serves every layer.  Its tensors are its own: what becomes of the lists that it was
+    made from does not change it."""
     rows: torch.Tensor        # [n] int32
     starts: torch.Tensor      # [n + 1] int32
     first: torch.Tensor       # [n] int32
@@ -1256,12 +1257,13 @@ def cache_step(cache: PagedCache, rows: torch.Tensor, counts: torch.Tensor, toke
     more = _index32(counts, n, "counts", index)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
-    starts, first, token_rows, positions = rows.new_empty(2 * (n + tokens) + 1).split_with_sizes((n + 1, n, tokens, tokens))
-    step = PagedStep(rows, starts, first, token_rows, positions, rows.new_empty(tokens, dtype=torch.int64))
+    starts, first, own, token_rows, positions = rows.new_empty(3 * n + 2 * tokens + 1).split_with_sizes(
+        (n + 1, n, n, tokens, tokens))
+    step = PagedStep(own, starts, first, token_rows, positions, rows.new_empty(tokens, dtype=torch.int64))
     at32 = starts.data_ptr()
-    out = L.Step(tokens, at32, at32 + 4 * (n + 1), at32 + 4 * (2 * n + 1), at32 + 4 * (2 * n + 1 + tokens), step.places.data_ptr())
+    out = L.Step(tokens, at32, at32 + 4 * (n + 1), at32 + 4 * (3 * n + 1), at32 + 4 * (3 * n + 1 + tokens), step.places.data_ptr())
     ws, need = _cache_workspace(s, n, rows)
-    _enqueue("gdnx_cache_step", index, C.byref(s), n, at, more, C.byref(out), ws.data_ptr(), need)
+    _enqueue("gdnx_cache_step_rows", index, C.byref(s), n, at, more, C.byref(out), at32 + 4 * (2 * n + 1), ws.data_ptr(), need)
     return step
 
 

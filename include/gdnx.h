@@ -522,6 +522,10 @@ typedef struct {
  * tensors have rows are refused (GDNX_EINVAL); a step that is refused, or follows a refused operation, has no tokens. */
 GDNX_API gdnx_status gdnx_cache_step(const gdnx_cache* cache, int64_t n, const int32_t* rows, const int32_t* counts,
                                      const gdnx_step* step, void* workspace, size_t workspace_bytes, void* stream);
+/* The same with a copy of `rows` in rows_out [n], for a plan that outlives the caller's list. */
+GDNX_API gdnx_status gdnx_cache_step_rows(const gdnx_cache* cache, int64_t n, const int32_t* rows, const int32_t* counts,
+                                          const gdnx_step* step, int32_t* rows_out, void* workspace,
+                                          size_t workspace_bytes, void* stream);
 /* k, v [tokens,Hk,D] (st, sh) go to a step's places in `layer`; padding goes nowhere. */
 GDNX_API gdnx_status gdnx_cache_append(const gdnx_cache* cache, int64_t layer, int64_t tokens, const gdnx_view* k,
                                        const gdnx_view* v, const int64_t* places, void* stream);
