@@ -89,6 +89,10 @@ GDNX_DEV void mma_px(uint32_t d, uint32_t p, uint32_t x, uint32_t idesc, bool ac
 GDNX_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, pipe::wait_or_abort(bar, parity, abort_flag));
 }
+// One that may last as long as other warps' work, which changes `moved` as it goes on.
+GDNX_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const volatile uint32_t* moved) {
+  return __all_sync(0xffffffffu, pipe::wait_or_abort(bar, parity, abort_flag, moved));
+}
 
 // Registers of the executing warpgroup from here on (the block's sum stays within its launch's).
 template <int N>

@@ -13,6 +13,9 @@
 // Warps 0-3 and 4-7 are the stages' rows, warp 8 issues the products, warp 9 the loads, warp 11 clears rows of V.  Warp
 // 10 walks the share ahead of them all and leaves what they need of each segment in a short queue, so that none waits
 // for lengths and page tables where one segment ends and the next begins; then it clears padding rows of the output.
+// Warps 10 and 11 may have nothing to do for as long as a whole segment, or the whole share, takes (38 s for 2^20 tokens of
+// 80 heads): the bound of their waits counts from the last tile that the loads asked for.  All other waits last some tiles,
+// or the walk over sequences without tokens.
 //
 // The shape: a small chunk is bound by the bytes of K and V, of which 192 KB are on their way or in use, a long one by the
 // rows' chain (scores out of tensor memory, maximum, exponentials), which two stages cover in part.  Products are issued
@@ -131,6 +134,7 @@ struct Small {
   long long sums[NTHREADS / 32];
   float2 stat[128];  // stage 1's maxima and sums
   uint8_t there[MASKS];  // pages of the tiles that are there, tile after tile
+  uint32_t asked;        // changes with every tile that the loads ask for
   uint32_t tmem_at;
   int abort_flag;
 };
@@ -514,7 +518,7 @@ GDNX_DEV void run_schedule(const TcParams& P, Small& sm) {
   Walk<Tc> w(P, sm.share);
   for (uint32_t k = 0;; ++k) {
     const bool more = w.next();
-    if (!warp_wait(&bar.item_empty[k % ITEMS], (k / ITEMS & 1) ^ 1, &sm.abort_flag)) return;
+    if (!warp_wait(&bar.item_empty[k % ITEMS], (k / ITEMS & 1) ^ 1, &sm.abort_flag, &sm.asked)) return;
     Item& x = sm.item[k % ITEMS];
     if (more) {
       const Seg g(P, w);
@@ -604,7 +608,10 @@ GDNX_DEV void run_loads(const TcParams& P, Small& sm, uint8_t* base, uint32_t sm
       const bool clear = side == 1 && (there != all_pages || j0 + TM > len);
       const uint32_t mb = tc::smem_u32(clear ? &bar.landed[sl] : &bar.full[sl]);
       if (lane == 0) {
-        if (side == 0) *const_cast<volatile uint8_t*>(&sm.there[(tiles + i) % MASKS]) = (uint8_t)there;
+        if (side == 0) {
+          *const_cast<volatile uint8_t*>(&sm.there[(tiles + i) % MASKS]) = (uint8_t)there;
+          *const_cast<volatile uint32_t*>(&sm.asked) = tiles + i + 1;
+        }
         pipe::expect_tx(mb, __popc(there) * DB * box);
       }
       __syncwarp();
@@ -669,7 +676,7 @@ GDNX_DEV void run_clears(const TcParams& P, Small& sm, uint8_t* base) {
   const int lane = threadIdx.x % 32, page = P.a.cache.page, e = lane % (8 * DB);
   uint32_t bits = 0;  // a bit for each slot: the parity of its next clearing
   for (uint32_t k = 0;; ++k) {
-    if (!warp_wait(&bar.job_full[k % JOBS], k / JOBS & 1, &sm.abort_flag)) return;
+    if (!warp_wait(&bar.job_full[k % JOBS], k / JOBS & 1, &sm.abort_flag, &sm.asked)) return;
     const Job j = sm.job[k % JOBS];
     __syncwarp();
     if (lane == 0) pipe::mbar_arrive(&bar.job_empty[k % JOBS]);
@@ -706,6 +713,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_attn_tc_kernel(const __grid
   }
   if (threadIdx.x == 0) {
     *abort_flag = smem % 1024 ? 1 : 0;  // swizzled tiles need an aligned base
+    sm.asked = 0;
     for (int i = 0; i < Lo::SLOTS; ++i) {
       tc::mbar_init(&bar.full[i], 1);
       tc::mbar_init(&bar.empty[i], 1);

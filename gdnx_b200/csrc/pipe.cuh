@@ -6,6 +6,7 @@
 
 #include <stdint.h>
 
+#include "bounded_wait.h"
 #include "tc.cuh"
 
 namespace gdnx {
@@ -43,12 +44,22 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
 // on running out it raises the flag itself.
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   const uint32_t a = tc::smem_u32(bar);
-  for (uint32_t it = 0; it < (1u << 22); ++it) {
+  for (uint32_t it = 0; it < kPolls; ++it) {
     if (try_wait(a, parity)) return true;
     if (*abort_flag) return false;
   }
   *abort_flag = 1;
   return false;
+}
+// The same for a wait that may last as long as other threads' work: `moved`, a word of shared memory that these change as
+// they go on, starts the count anew.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                              const volatile uint32_t* moved) {
+  const uint32_t a = tc::smem_u32(bar);
+  const Wait w = wait_while_moving([&] { return try_wait(a, parity); }, [&] { return *abort_flag != 0; },
+                                   [&] { return *moved; }, kPolls);
+  if (w == Wait::kRanOut) *abort_flag = 1;
+  return w == Wait::kDone;
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
