@@ -25,7 +25,8 @@ EXPORTED = ("gdnx_scan_fwd", "gdnx_scan_fwd_noalloc", "gdnx_scan_noalloc_status"
             "gdnx_cache_extend", "gdnx_cache_write", "gdnx_cache_truncate", "gdnx_cache_trim", "gdnx_cache_compact",
             "gdnx_cache_compact_bounds", "gdnx_cache_step", "gdnx_cache_step_rows", "gdnx_cache_append", "gdnx_cache_bounds",
             "gdnx_paged_attn", "gdnx_paged_attn_workspace_bytes", "gdnx_paged_select", "gdnx_paged_select_workspace_bytes",
-            "gdnx_cache_workspace_bytes", "gdnx_paged_decode", "gdnx_paged_decode_workspace_bytes")
+            "gdnx_cache_workspace_bytes", "gdnx_paged_decode", "gdnx_paged_decode_workspace_bytes",
+            "gdnx_paged_decode_listed", "gdnx_paged_decode_listed_workspace_bytes")
 
 
 class View(C.Structure):
@@ -145,8 +146,11 @@ class PagedDecodeArgs(C.Structure):
                 ("window", C.c_int64), ("sinks", C.c_int64), ("max_len", C.c_int64), ("scale", C.c_float),
                 ("q", View), ("rows", C.c_void_p), ("y", C.c_void_p), ("y_dtype", C.c_int32),
                 ("y_sb", C.c_int64), ("y_sh", C.c_int64), ("error", C.c_void_p),
-                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
-                ("positions", C.c_void_p), ("pages", C.c_void_p), ("listed", C.c_int64)]
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class PagedDecodeListedArgs(C.Structure):
+    _fields_ = [("decode", PagedDecodeArgs), ("positions", C.c_void_p), ("pages", C.c_void_p), ("listed", C.c_int64)]
 
 
 class Step(C.Structure):
@@ -244,6 +248,10 @@ def load(path: Path = LIB_PATH):
     lib.gdnx_paged_decode_workspace_bytes.restype = size
     lib.gdnx_paged_decode.argtypes = [C.POINTER(PagedDecodeArgs), C.c_void_p]
     lib.gdnx_paged_decode.restype = C.c_int
+    lib.gdnx_paged_decode_listed_workspace_bytes.argtypes = [C.POINTER(PagedDecodeListedArgs)]
+    lib.gdnx_paged_decode_listed_workspace_bytes.restype = size
+    lib.gdnx_paged_decode_listed.argtypes = [C.POINTER(PagedDecodeListedArgs), C.c_void_p]
+    lib.gdnx_paged_decode_listed.restype = C.c_int
     lib.gdnx_paged_attn_workspace_bytes.argtypes = [C.POINTER(PagedAttnArgs)]
     lib.gdnx_paged_attn_workspace_bytes.restype = size
     lib.gdnx_paged_attn.argtypes = [C.POINTER(PagedAttnArgs), C.c_void_p]

@@ -372,15 +372,22 @@ gdnx_status gdnx_paged_select(const gdnx_paged_select_args* a, void* stream) {
 }
 
 // The decode's arguments with window and sinks kept within the longest sequence.
-static gdnx_paged_decode_args clamp_decode(const gdnx_paged_decode_args& a) {
-  gdnx_paged_decode_args c = a;
-  const int64_t most = a.cache.width * a.cache.page;
-  if (c.window > most) c.window = most;
-  if (c.sinks > most) c.sinks = most;
+static gdnx::DecodeArgs decode_args(const gdnx_paged_decode_args& a, const int32_t* positions = nullptr,
+                                    const int32_t* pages = nullptr, int64_t listed = 0) {
+  gdnx::DecodeArgs c;
+  static_cast<gdnx_paged_decode_args&>(c) = a;
+  if (check_cache_sizes(&a.cache) == GDNX_OK) {
+    const int64_t most = a.cache.width * a.cache.page;
+    if (c.window > most) c.window = most;
+    if (c.sinks > most) c.sinks = most;
+  }
+  c.positions = positions;
+  c.pages = pages;
+  c.listed = listed;
   return c;
 }
 
-static gdnx_status check_decode(const gdnx_paged_decode_args& a) {
+static gdnx_status check_decode(const gdnx::DecodeArgs& a) {
   const gdnx_status s = check_cache(&a.cache);
   if (s != GDNX_OK) return s;
   if (a.cache.pages < 1 || a.B < 0 || a.H <= 0 || a.H % a.cache.Hk || a.layer < 0 || a.layer >= a.cache.L || a.window < 1 || a.sinks < 0 ||
@@ -397,22 +404,33 @@ static gdnx_status check_decode(const gdnx_paged_decode_args& a) {
   return GDNX_OK;
 }
 
-size_t gdnx_paged_decode_workspace_bytes(const gdnx_paged_decode_args* a) {
-  if (!a || a->B <= 0 || a->H <= 0 || a->cache.Hk <= 0 || a->window < 1 || a->sinks < 0) return 0;
-  if (check_cache_sizes(&a->cache) != GDNX_OK || a->H % a->cache.Hk) return 0;
-  const gdnx_paged_decode_args c = clamp_decode(*a);
-  return c.cache.dtype == GDNX_F32 ? gdnx::paged_decode_workspace_bytes(c) : gdnx::paged_decode_tc_workspace_bytes(c);
+static size_t decode_bytes(const gdnx::DecodeArgs& a) {
+  if (a.B <= 0 || a.H <= 0 || a.cache.Hk <= 0 || a.window < 1 || a.sinks < 0) return 0;
+  if (check_cache_sizes(&a.cache) != GDNX_OK || a.H % a.cache.Hk) return 0;
+  return a.cache.dtype == GDNX_F32 ? gdnx::paged_decode_workspace_bytes(a) : gdnx::paged_decode_tc_workspace_bytes(a);
 }
 
+static gdnx_status decode(const gdnx::DecodeArgs& a, void* stream) {
+  const gdnx_status s = check_decode(a);
+  if (s != GDNX_OK || a.B == 0) return s;
+  const size_t need = decode_bytes(a);
+  if (need && (a.workspace_bytes < need || !device_ptr(a.workspace, 16))) return GDNX_EWORKSPACE;
+  return a.cache.dtype == GDNX_F32 ? gdnx::launch_paged_decode(a, (cudaStream_t)stream)
+                                   : gdnx::launch_paged_decode_tc(a, (cudaStream_t)stream);
+}
+
+size_t gdnx_paged_decode_workspace_bytes(const gdnx_paged_decode_args* a) { return a ? decode_bytes(decode_args(*a)) : 0; }
+
 gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* a, void* stream) {
-  if (!a) return GDNX_EINVAL;
-  const gdnx_status s = check_decode(*a);
-  if (s != GDNX_OK || a->B == 0) return s;
-  const size_t need = gdnx_paged_decode_workspace_bytes(a);
-  if (need && (a->workspace_bytes < need || !device_ptr(a->workspace, 16))) return GDNX_EWORKSPACE;
-  const gdnx_paged_decode_args c = clamp_decode(*a);
-  return c.cache.dtype == GDNX_F32 ? gdnx::launch_paged_decode(c, (cudaStream_t)stream)
-                                   : gdnx::launch_paged_decode_tc(c, (cudaStream_t)stream);
+  return a ? decode(decode_args(*a), stream) : GDNX_EINVAL;
+}
+
+size_t gdnx_paged_decode_listed_workspace_bytes(const gdnx_paged_decode_listed_args* a) {
+  return a ? decode_bytes(decode_args(a->decode, a->positions, a->pages, a->listed)) : 0;
+}
+
+gdnx_status gdnx_paged_decode_listed(const gdnx_paged_decode_listed_args* a, void* stream) {
+  return a ? decode(decode_args(a->decode, a->positions, a->pages, a->listed), stream) : GDNX_EINVAL;
 }
 
 static gdnx_status check_paged_attn_sizes(const gdnx_paged_attn_args& a) {
@@ -470,7 +488,7 @@ const char* gdnx_status_string(gdnx_status s) {
   return "GDNX_UNKNOWN";
 }
 
-const char* gdnx_version(void) { return "gdnx-b200 0.1 sm_100a"; }
+const char* gdnx_version(void) { return "gdnx-b200 0.2 sm_100a"; }
 
 size_t gdnx_scan_workspace_bytes(const gdnx_scan_args* a) {
   if (!a) return 0;

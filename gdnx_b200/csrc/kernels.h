@@ -45,11 +45,17 @@ gdnx_status launch_cache_bounds(const gdnx_cache& c, int64_t layer, int64_t n, c
                                 const int32_t* counts, void* bounds, cudaStream_t st);
 size_t paged_select_workspace_bytes(const gdnx_paged_select_args& a);
 gdnx_status launch_paged_select(const gdnx_paged_select_args& a, cudaStream_t st);
-size_t paged_decode_workspace_bytes(const gdnx_paged_decode_args& a);
-gdnx_status launch_paged_decode(const gdnx_paged_decode_args& a, cudaStream_t st);
+// A decode's arguments, dense (no positions, no pages) or not.
+struct DecodeArgs : gdnx_paged_decode_args {
+  const int32_t* positions;
+  const int32_t* pages;
+  int64_t listed;
+};
+size_t paged_decode_workspace_bytes(const DecodeArgs& a);
+gdnx_status launch_paged_decode(const DecodeArgs& a, cudaStream_t st);
 // 16-bit caches, on the tensor cores (paged_decode_tc.cu).
-size_t paged_decode_tc_workspace_bytes(const gdnx_paged_decode_args& a);
-gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t st);
+size_t paged_decode_tc_workspace_bytes(const DecodeArgs& a);
+gdnx_status launch_paged_decode_tc(const DecodeArgs& a, cudaStream_t st);
 // Attention of packed new tokens over a paged cache (paged_attn.cu).
 size_t paged_attn_simt_workspace_bytes(const gdnx_paged_attn_args& a);
 gdnx_status launch_paged_attn_simt(const gdnx_paged_attn_args& a, cudaStream_t st);

@@ -94,7 +94,7 @@ GDNX_DEV void load_stages(const DecParams& P, Walk w, uint8_t* ring, Small<NH>& 
 template <int LPK, int NH>
 GDNX_DEV void use_stages(const DecParams& P, Walk w, int64_t per, const uint8_t* ring, Small<NH>& sm) {
   constexpr int KPW = 32 / LPK, PASSES = SUB / WARPS / KPW;
-  const gdnx_paged_decode_args& a = P.a;
+  const DecodeArgs& a = P.a;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, sub = lane / LPK, dl = lane % LPK, D = (int)a.cache.D;
   const int d0 = 4 * dl, d1 = 4 * (LPK + dl);  // this lane's two runs of four values
   const int window = (int)a.window, sinks = (int)a.sinks;
@@ -289,13 +289,13 @@ gdnx_status launch(const DecParams& P, cudaStream_t st) {
 }
 
 // Query heads of a unit.
-int heads_of(const gdnx_paged_decode_args& a) { return a.H / a.cache.Hk > 4 ? 8 : 4; }
+int heads_of(const DecodeArgs& a) { return a.H / a.cache.Hk > 4 ? 8 : 4; }
 
 }  // namespace
 
-size_t paged_decode_workspace_bytes(const gdnx_paged_decode_args& a) { return plan_bytes(make_plan(a, heads_of(a))); }
+size_t paged_decode_workspace_bytes(const DecodeArgs& a) { return plan_bytes(make_plan(a, heads_of(a))); }
 
-gdnx_status launch_paged_decode(const gdnx_paged_decode_args& a, cudaStream_t st) {
+gdnx_status launch_paged_decode(const DecodeArgs& a, cudaStream_t st) {
   DecParams P;
   fill(P, a, make_plan(a, heads_of(a)));
   if (a.cache.D > 64) return heads_of(a) == 4 ? launch<16, 4>(P, st) : launch<16, 8>(P, st);

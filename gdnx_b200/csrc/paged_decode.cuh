@@ -28,7 +28,7 @@ struct Joint {
 };
 
 struct DecParams {
-  gdnx_paged_decode_args a;
+  DecodeArgs a;
   float* part;     // [grid][2][NH][128] unnormalised outputs of a CTA's first and last unit
   float* stat;     // [grid][2][NH][2] maximum (log2 domain) and sum
   Joint* joint;    // [grid] the unit cut in several parts that ends in a CTA
@@ -50,7 +50,7 @@ struct Seq {
   int listed;
 };
 
-GDNX_DEV int slot_length(const gdnx_paged_decode_args& a, int64_t b, int& row) {
+GDNX_DEV int slot_length(const DecodeArgs& a, int64_t b, int& row) {
   const gdnx_cache& c = a.cache;
   row = a.rows ? a.rows[b] : (int)b;
   if (row < 0 || row >= c.slots) return 0;
@@ -60,7 +60,7 @@ GDNX_DEV int slot_length(const gdnx_paged_decode_args& a, int64_t b, int& row) {
   return (int)(n < 0 ? 0 : (n > most ? most : n));
 }
 
-GDNX_DEV Seq make_seq(const gdnx_paged_decode_args& a, int64_t b) {
+GDNX_DEV Seq make_seq(const DecodeArgs& a, int64_t b) {
   int row;
   const int len = slot_length(a, b, row);
   if (a.pages) {
@@ -71,7 +71,7 @@ GDNX_DEV Seq make_seq(const gdnx_paged_decode_args& a, int64_t b) {
   return {row, len, KeyTiles(len - 1, len - 1, len, (int)a.window, (int)a.sinks, TM), 0};
 }
 
-GDNX_DEV int tiles_of(const gdnx_paged_decode_args& a, int64_t b) { return make_seq(a, b).kt.count; }
+GDNX_DEV int tiles_of(const DecodeArgs& a, int64_t b) { return make_seq(a, b).kt.count; }
 
 // The CTA finds its range: every thread adds up a run of sequences, and the one whose run holds
 // the range's first tile walks to its sequence.  (Whole units: t0 and t1 count units.)
@@ -188,7 +188,7 @@ GDNX_DEV float no_weights(float top) { return top == -INFINITY ? 0.f : NAN; }
 
 // Zeros for the sequences that see nothing.
 GDNX_DEV void write_zeros(const DecParams& P) {
-  const gdnx_paged_decode_args& a = P.a;
+  const DecodeArgs& a = P.a;
   const int D = (int)a.cache.D, n = (int)a.H * D;
   for (int64_t b = blockIdx.x; b < a.B; b += P.grid) {
     if (tiles_of(a, b) > 0) continue;
@@ -213,7 +213,7 @@ constexpr int JOIN_WARPS = 8;
 
 template <int NH>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_decode_join_kernel(const DecParams P) {
-  const gdnx_paged_decode_args& a = P.a;
+  const DecodeArgs& a = P.a;
   __shared__ float red_m[JOIN_WARPS], red_l[JOIN_WARPS], red_o[JOIN_WARPS][128];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, D = (int)a.cache.D, g = blockIdx.y;
   dependents_may_start();
@@ -269,7 +269,7 @@ struct Plan {
   int nh, groups, grid, whole;
 };
 
-inline Plan make_plan(const gdnx_paged_decode_args& a, int nh) {
+inline Plan make_plan(const DecodeArgs& a, int nh) {
   Plan p;
   const int64_t G = a.H / a.cache.Hk, sms = sm_count();
   p.nh = nh;
@@ -292,7 +292,7 @@ inline size_t plan_bytes(const Plan& p) {
   return p.whole ? 0 : (size_t)p.grid * (2 * p.nh * (128 + 2) * sizeof(float) + sizeof(Joint));
 }
 
-inline void fill(DecParams& P, const gdnx_paged_decode_args& a, const Plan& p) {
+inline void fill(DecParams& P, const DecodeArgs& a, const Plan& p) {
   P.a = a;
   P.grid = p.grid;
   P.groups = p.groups;

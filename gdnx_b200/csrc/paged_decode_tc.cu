@@ -167,7 +167,7 @@ GDNX_DEV void run_products(const TcParams& P, Walk w, uint32_t smem, uint32_t tm
 // The unit's query rows as a K-major tile of NH rows (rows beyond its heads zero), by one warp.
 template <int DB, int NH>
 GDNX_DEV void stage_q(const TcParams& P, const Walk& w, uint8_t* dst) {
-  const gdnx_paged_decode_args& a = P.a;
+  const DecodeArgs& a = P.a;
   const Heads hd(P, w.unit, NH);
   const int D = (int)a.cache.D;
 #pragma unroll 4
@@ -229,7 +229,7 @@ template <int DB, int NH, int NC, bool BF16>
 GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, uint32_t tmem, Bars& bar, float* red,
                        const int (*at)[8], volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
-  const gdnx_paged_decode_args& a = P.a;
+  const DecodeArgs& a = P.a;
   const int r = threadIdx.x, lane = r % 32, warp = r / 32, D = (int)a.cache.D;
   const uint32_t lane_at = (uint32_t)(warp * 32) << 16;
   const float c2 = a.scale * kLog2e;
@@ -433,11 +433,11 @@ gdnx_status launch_type(const TcParams& P, cudaStream_t st) {
 
 }  // namespace
 
-size_t paged_decode_tc_workspace_bytes(const gdnx_paged_decode_args& a) {
+size_t paged_decode_tc_workspace_bytes(const DecodeArgs& a) {
   return plan_bytes(make_plan(a, a.H / a.cache.Hk > 16 ? 32 : 16));
 }
 
-gdnx_status launch_paged_decode_tc(const gdnx_paged_decode_args& a, cudaStream_t st) {
+gdnx_status launch_paged_decode_tc(const DecodeArgs& a, cudaStream_t st) {
   const gdnx_cache& c = a.cache;
   const EncodeTiledFn enc = encode_fn();
   if (!enc) return GDNX_ELAUNCH;

@@ -1461,17 +1461,21 @@ def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Op
                           D ** -0.5 if scale is None else scale, L.View(q.data_ptr(), _DT[q.dtype], D, qb, 0, qh),
                           None if rows is None else _index32(rows, B, "rows", index), y.data_ptr(), _DT[y.dtype], yb, yh,
                           _error_word(index))
+    name, call = "gdnx_paged_decode", a
+    if positions is not None or pages is not None:
+        name, call = "gdnx_paged_decode_listed", L.PagedDecodeListedArgs(a)
+        a = call.decode
     if positions is not None:
-        a.positions = _index32(positions, B, "positions", index)
+        call.positions = _index32(positions, B, "positions", index)
     if pages is not None:
         if pages.dtype is not torch.int32 or pages.dim() != 3 or pages.shape[:2] != (B, s.Hk) or pages.shape[2] < 1 or not pages.is_contiguous():
             raise ValueError("pages must be a contiguous int32 tensor [B,Hk,k]")
         _on_device(index, pages)
-        a.pages, a.listed = pages.data_ptr(), pages.shape[2]
-    need = _entry("gdnx_paged_decode_workspace_bytes")(C.byref(a))
+        call.pages, call.listed = pages.data_ptr(), pages.shape[2]
+    need = _entry(name + "_workspace_bytes")(C.byref(call))
     ws = None
     if need:
         ws = q.new_empty(need, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    _enqueue("gdnx_paged_decode", index, C.byref(a))
+    _enqueue(name, index, C.byref(call))
     return y

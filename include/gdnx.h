@@ -564,9 +564,6 @@ GDNX_API gdnx_status gdnx_paged_select(const gdnx_paged_select_args* args, void*
  * It sees token j < length where length - 1 - j < window or j < sinks; tokens on released
  * pages are not seen.  A row that sees nothing (length 0, a slot out of range) gives 0;
  * one that sees a score of NaN or +inf, or only -inf, is NaN.
- * With `positions`, row i of q stands at that position of its slot instead (-1: nowhere) and sees no later token.
- * With `pages`, it sees of these only the tokens on the pages that its key head's list names: indexes into the
- * slot's table row, each once, of which as many are read as the slot has pages; others than the slot's are passed over.
  * The visible tokens are split over CTAs, and the parts joined in a fixed order. */
 typedef struct {
   gdnx_cache cache;
@@ -582,13 +579,24 @@ typedef struct {
   int32_t* error;              /* device word that takes GDNX_ETIMEOUT; NULL = none */
   void* workspace;             /* 16-byte aligned */
   size_t workspace_bytes;
-  const int32_t* positions;    /* [B] device; NULL = the slots' last tokens */
-  const int32_t* pages;        /* [B,Hk,listed] device; NULL = all */
-  int64_t listed;
 } gdnx_paged_decode_args;
 
 GDNX_API size_t gdnx_paged_decode_workspace_bytes(const gdnx_paged_decode_args* args);
 GDNX_API gdnx_status gdnx_paged_decode(const gdnx_paged_decode_args* args, void* stream);
+
+/* The same at given positions and over listed pages.
+ * With `positions`, row i of q stands at that position of its slot instead (-1: nowhere) and sees no later token.
+ * With `pages`, it sees of these only the tokens on the pages that its key head's list names: indexes into the
+ * slot's table row, each once, of which as many are read as the slot has pages; others than the slot's are passed over. */
+typedef struct {
+  gdnx_paged_decode_args decode;
+  const int32_t* positions;    /* [B] device; NULL = the slots' last tokens */
+  const int32_t* pages;        /* [B,Hk,listed] device; NULL = all */
+  int64_t listed;
+} gdnx_paged_decode_listed_args;
+
+GDNX_API size_t gdnx_paged_decode_listed_workspace_bytes(const gdnx_paged_decode_listed_args* args);
+GDNX_API gdnx_status gdnx_paged_decode_listed(const gdnx_paged_decode_listed_args* args, void* stream);
 
 /* Attention of a step's packed new tokens (of chunks of prompts, proposals, single tokens, mixed) over the cache that
  * holds them and what came before: row starts[i] + t of q stands at position p = first[i] + t of slot rows[i] (keys and

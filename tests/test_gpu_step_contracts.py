@@ -1,10 +1,11 @@
 """What the serving step's operators promise beyond their formulas: a plan is its own, foreign plans stay within the
 tensors, and what a call is not given it refuses."""
-import math
+import ctypes as C
 
 import pytest
 import torch
 
+from gdnx_b200 import _lib as L
 from gdnx_b200 import ops
 from test_gpu_paged import DEV, TYPES, cache, i32
 from test_gpu_paged_attention import close, plain
@@ -44,3 +45,24 @@ def test_a_refused_plan_keeps_its_rows():
     assert step.rows.tolist() == [0, 7] and step.starts.tolist() == [0, 0, 0] and step.first.tolist() == [0, 0]
     with pytest.raises(Exception, match="GDNX_EINVAL"):
         ops.cache_check(c)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_dense_decode_reads_its_own_struct_only(dtype):
+    """Words behind the struct that are neither null nor addresses, as a program built before listed pages may have."""
+    lib = L.load()
+    c = cache([300, 20], Hk=2, page=16, D=64, dtype=dtype, width=20, extra=0)
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(4)).to(TYPES[dtype]).to(DEV)
+    want = ops.paged_decode(q, c)
+    y = torch.empty_like(q)
+    s, _ = ops._cache_struct(c)
+    a = L.PagedDecodeArgs(s, 2, 4, 0, 1 << 40, 0, 0, 0.125, L.View(q.data_ptr(), ops._DT[q.dtype], 64, 256, 0, 64), None,
+                          y.data_ptr(), ops._DT[y.dtype], 256, 64, ops._error_word(0))
+    ws = torch.empty(lib.gdnx_paged_decode_workspace_bytes(C.byref(a)), dtype=torch.uint8, device=DEV)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    size = C.sizeof(L.PagedDecodeArgs)
+    room = (C.c_char * (size + 64))(*([b"\x01"] * (size + 64)))
+    C.memmove(room, C.byref(a), size)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.gdnx_paged_decode(C.cast(room, C.POINTER(L.PagedDecodeArgs)), stream) == L.GDNX_OK
+    assert torch.equal(y, want)
