@@ -9,7 +9,8 @@
 //
 // Measured (4 heads of 128, bf16): append of 24,500 tokens (100 MB moved) 16 us, 6.2 TB/s; of 64 tokens 2.0 us.  bounds of
 // 8 x 4096 tokens 10.5 us (3.3 TB/s), behind one token in each of 64 slots 4.9 us: the check of the call, under which the
-// first page's keys come, and the chain from slot to page to keys.
+// first page's keys come, and the chain from slot to page to keys.  Behind one token in each of 4096 slots 63 us: checked
+// by every CTA, such a call took 599, which grew with the square of the rows.
 #include "paged_cache.cuh"
 
 namespace gdnx {
@@ -18,6 +19,7 @@ namespace {
 constexpr int APPEND_NT = 256;
 constexpr int TOKENS = 4;  // of a thread in flight
 constexpr int BOUNDS_NT = 128;
+constexpr int CHECK_NT = 1024;
 
 template <typename V>
 __global__ void __launch_bounds__(APPEND_NT) cache_append_kernel(const gdnx_cache c, int64_t layer, int64_t tokens,
@@ -110,9 +112,18 @@ GDNX_DEV bool bounds_ok(uint32_t* seen, const gdnx_cache& c, int64_t n, const in
   return !__syncthreads_or(bad);
 }
 
-// CTA (h, i, z): head h of every gridDim.z-th page that holds one of the newest tokens of slot rows[i].  A CTA reads
-// its first page's keys before it checks the call, and writes after.
-template <typename T>
+// The check by one CTA, for calls of many rows.
+__global__ void __launch_bounds__(CHECK_NT) cache_bounds_check_kernel(const gdnx_cache c, int64_t n, const int32_t* rows,
+                                                                      const int32_t* counts) {
+  extern __shared__ uint32_t seen[];
+  dependents_may_start();
+  wait_for_earlier();
+  if (!bounds_ok(seen, c, n, rows, counts) && threadIdx.x == 0 && *c.status == 0) *c.status = GDNX_EINVAL;
+}
+
+// CTA (h, i, z): head h of every gridDim.z-th page that holds one of the newest tokens of slot rows[i].  CHECK: every CTA
+// checks the call itself and decides like the others; it reads its first page's keys before, and writes after.
+template <typename T, bool CHECK>
 __global__ void __launch_bounds__(BOUNDS_NT) cache_bounds_kernel(const gdnx_cache c, int64_t layer, int64_t n,
                                                                  const int32_t* rows, const int32_t* counts,
                                                                  uint4* bounds) {
@@ -123,7 +134,8 @@ __global__ void __launch_bounds__(BOUNDS_NT) cache_bounds_kernel(const gdnx_cach
   const int per = (int)(c.D * sizeof(T) / 16), groups = BOUNDS_NT / per;  // pieces of a row, rows side by side
   const int piece = threadIdx.x % per, group = threadIdx.x / per, h = blockIdx.x;
   const bool first_cta = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
-  bool checked = false;
+  bool checked = !CHECK;
+  if (!CHECK && *c.status != 0) return;
   for (int64_t i = blockIdx.y; i < n; i += gridDim.y) {
     const int row = rows[i];
     if (row < 0 || row >= c.slots) continue;  // refused by the CTAs that have work
@@ -181,13 +193,25 @@ __global__ void __launch_bounds__(BOUNDS_NT) cache_bounds_kernel(const gdnx_cach
     *c.status = GDNX_EINVAL;
 }
 
-template <typename T>
+template <typename T, bool CHECK>
 cudaError_t bounds_of(const gdnx_cache& c, int64_t layer, int64_t n, const int32_t* rows, const int32_t* counts,
                       void* bounds, cudaStream_t st) {
   // as many CTAs as keep the device busy; where the pages of a call are fewer, the others find none
   const int64_t y = n < 65535 ? n : 65535, fill = (int64_t)sm_count() * 8 / (c.Hk * y), z = fill < 1 ? 1 : fill < c.width ? fill : c.width;
-  return launch_early(cache_bounds_kernel<T>, dim3((unsigned)c.Hk, (unsigned)y, (unsigned)(z < 65535 ? z : 65535)),
-                      dim3(BOUNDS_NT), seen_bytes(c), st, c, layer, n, rows, counts, static_cast<uint4*>(bounds));
+  return launch_early(cache_bounds_kernel<T, CHECK>, dim3((unsigned)c.Hk, (unsigned)y, (unsigned)(z < 65535 ? z : 65535)),
+                      dim3(BOUNDS_NT), CHECK ? seen_bytes(c) : 0, st, c, layer, n, rows, counts, static_cast<uint4*>(bounds));
+}
+
+// A check that takes every thread of a CTA one step runs in the CTAs that find the bounds; longer ones run once, in a CTA
+// of their own before them (one new token in each of 128 slots: 4.8 us in the CTAs; of 200 slots 9.7 in the CTAs, 6.6 in
+// its own; of 1024 slots 53 and 16).
+template <typename T>
+gdnx_status bounds_call(const gdnx_cache& c, int64_t layer, int64_t n, const int32_t* rows, const int32_t* counts,
+                        void* bounds, cudaStream_t st) {
+  if (n <= BOUNDS_NT && seen_bytes(c) <= BOUNDS_NT * 4) return launched(bounds_of<T, true>(c, layer, n, rows, counts, bounds, st));
+  if (launch_early(cache_bounds_check_kernel, dim3(1), dim3(CHECK_NT), seen_bytes(c), st, c, n, rows, counts) != cudaSuccess)
+    return GDNX_ELAUNCH;
+  return launched(bounds_of<T, false>(c, layer, n, rows, counts, bounds, st));
 }
 
 }  // namespace
@@ -209,9 +233,9 @@ gdnx_status launch_cache_append(const gdnx_cache& c, int64_t layer, int64_t toke
 gdnx_status launch_cache_bounds(const gdnx_cache& c, int64_t layer, int64_t n, const int32_t* rows,
                                 const int32_t* counts, void* bounds, cudaStream_t st) {
   switch (c.dtype) {
-    case GDNX_BF16: return launched(bounds_of<__nv_bfloat16>(c, layer, n, rows, counts, bounds, st));
-    case GDNX_F16: return launched(bounds_of<__half>(c, layer, n, rows, counts, bounds, st));
-    default: return launched(bounds_of<float>(c, layer, n, rows, counts, bounds, st));
+    case GDNX_BF16: return bounds_call<__nv_bfloat16>(c, layer, n, rows, counts, bounds, st);
+    case GDNX_F16: return bounds_call<__half>(c, layer, n, rows, counts, bounds, st);
+    default: return bounds_call<float>(c, layer, n, rows, counts, bounds, st);
   }
 }
 

@@ -1,6 +1,7 @@
 """What the serving step's operators promise beyond their formulas: a plan is its own, foreign plans stay within the
 tensors, and what a call is not given it refuses."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -66,3 +67,77 @@ def test_a_dense_decode_reads_its_own_struct_only(dtype):
     stream = torch.cuda.current_stream().cuda_stream
     assert lib.gdnx_paged_decode(C.cast(room, C.POINTER(L.PagedDecodeArgs)), stream) == L.GDNX_OK
     assert torch.equal(y, want)
+
+
+def many_slots(n, Hk=2, page=16, D=8):
+    """n slots of 1 to 2 page tokens each, written."""
+    g = torch.Generator().manual_seed(n)
+    c = ops.PagedCache.zeros(1, 2 * n, Hk, page, D, slots=n, width=3, bounds=True, device=DEV)
+    rows = torch.randperm(n, generator=g).int().to(DEV)
+    counts = torch.randint(1, 2 * page + 1, (n,), generator=g).int().to(DEV)
+    ops.cache_extend(c, rows, counts)
+    c.kv.copy_(torch.randn(c.kv.shape, generator=g))
+    return c, rows, counts
+
+
+def bounds_of_all(c):
+    """The bounds of every page that a slot holds (each by one slot), a token that is not there leaving no trace."""
+    L_, _, pages, Hk, page, D = c.kv.shape
+    have = torch.zeros(pages, dtype=torch.long, device=DEV)
+    at = torch.arange(c.table.shape[1], device=DEV) * page
+    held = (c.lengths[:, None] - at).clamp(0, page).long()
+    on = (c.table >= 0) & (held > 0)
+    have[c.table[on].long()] = held[on]
+    there = (torch.arange(page, device=DEV) < have[:, None])[None, :, None, :, None]
+    k = c.kv[:, 0].float()
+    lo = torch.where(there, k, math.inf).amin(3)
+    hi = torch.where(there, k, -math.inf).amax(3)
+    want = torch.stack([lo, hi], 1)
+    return torch.where((have > 0)[None, None, :, None, None], want, 0.0).to(c.kv.dtype)
+
+
+@pytest.mark.parametrize("n", [128, 129, 1500])
+def test_bounds_of_many_slots_and_their_refusals(n):
+    """On both sides of the size from which a call is checked by a CTA of its own."""
+    c, rows, counts = many_slots(n)
+    ops.cache_bounds(c, rows, counts)
+    ops.cache_check(c)
+    want = bounds_of_all(c)
+    assert torch.equal(c.bounds, want)
+    # refused: nothing is written, the status says so, and while it is set nothing happens
+    c.bounds.fill_(3.0)
+    bad_row, twice, more = rows.clone(), rows.clone(), counts.clone()
+    bad_row[n - 1] = n
+    twice[n - 1] = twice[0]
+    more[n // 2] = 3 * 16
+    for r, k in ((bad_row, counts), (twice, counts), (rows, more), (rows, -counts)):
+        ops.cache_bounds(c, r, k)
+        assert int(c.status) == L.GDNX_EINVAL
+        ops.cache_bounds(c, rows, counts)
+        assert int(c.status) == L.GDNX_EINVAL and (c.bounds == 3.0).all()
+        c.status.zero_()
+    # a partly filled last page that another slot holds too
+    part = int((counts.cpu() % 16 != 0).nonzero()[0])
+    other = 0 if part else 1
+    ops.cache_fork(c, rows[part:part + 1], rows[other:other + 1])
+    ops.cache_bounds(c, rows, c.lengths[rows.long()].contiguous())
+    assert int(c.status) == L.GDNX_EINVAL and (c.bounds == 3.0).all()
+
+
+def test_bounds_take_time_by_rows_not_by_their_square():
+    """Four times the rows take about four times as long (checked by every CTA they took fifteen times)."""
+    took = []
+    for n in (2048, 8192):
+        c, rows, counts = many_slots(n)
+        best = math.inf
+        for _ in range(8):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(5):
+                ops.cache_bounds(c, rows, counts)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        ops.cache_check(c)
+        took.append(best)
+    assert took[1] < 8 * took[0]
