@@ -37,14 +37,15 @@ struct Small {
 };
 
 // Does the sequence's newest token see any of a tile's tokens 32 s .. 32 s + 31?  (Of listed pages: is one there?)
+template <bool LISTED>
 GDNX_DEV bool sub_seen(const DecParams& P, const Seq& q, int tile, int s) {
   const int j = tile * TM + s * SUB;
-  if (P.a.pages) return j < q.listed * P.a.cache.page;
+  if (LISTED && P.a.pages) return j < q.listed * P.a.cache.page;
   return j < q.len && (j + SUB > (int64_t)q.len - P.a.window || j < P.a.sinks);
 }
 
-template <int NH>
-GDNX_DEV void load_stages(const DecParams& P, Walk w, uint8_t* ring, Small<NH>& sm) {
+template <bool LISTED, int NH>
+GDNX_DEV void load_stages(const DecParams& P, Walk<LISTED> w, uint8_t* ring, Small<NH>& sm) {
   const gdnx_cache& c = P.a.cache;
   const int lane = threadIdx.x % 32, page = c.page, npp = TM / page, ahead = 32 / npp, D = (int)c.D;
   const int runs = page < SUB ? SUB / page : 1, tokens = SUB / runs;  // contiguous runs of a stage
@@ -53,16 +54,16 @@ GDNX_DEV void load_stages(const DecParams& P, Walk w, uint8_t* ring, Small<NH>& 
   while (w.next()) {
     const int hk = w.unit / P.groups;
     int ids = -1;
-    int64_t first;
+    int64_t first = -1;
     for (int t = w.ta; t < w.tb; ++t) {
       const int k = (t - w.ta) % ahead;
       if (k == 0) {
         const int mine = t + lane / npp;
-        ids = mine < w.tb ? page_id(P, w.seq, w.b, w.unit, w.seq.kt.tile(mine), lane % npp, first) : -1;
+        ids = mine < w.tb ? page_id<LISTED>(P, w.seq, w.b, w.unit, w.seq.kt.tile(mine), lane % npp, first) : -1;
       }
       for (int s = 0; s < TM / SUB; ++s) {
         const int tile = w.seq.kt.tile(t);
-        if (!sub_seen(P, w.seq, tile, s)) continue;
+        if (!sub_seen<LISTED>(P, w.seq, tile, s)) continue;
         const uint32_t st = n % STAGES;
         if (!warp_wait(&sm.empty[st], (n / STAGES & 1) ^ 1, &sm.abort_flag)) return;
         ++n;
@@ -73,11 +74,12 @@ GDNX_DEV void load_stages(const DecParams& P, Walk w, uint8_t* ring, Small<NH>& 
         const uint32_t got = __ballot_sync(0xffffffffu, go);
         const uint32_t bar = tc::smem_u32(&sm.full[st]), bytes = (uint32_t)(tokens * D * 4);
         if (lane == 0) {
-          // places of a stage's two halves in the sequence
-          const int64_t a = page_first(P, w.seq, w.b, w.unit, tile, s * SUB / page);
-          const int64_t b = runs == 1 ? a + 16 : page_first(P, w.seq, w.b, w.unit, tile, s * SUB / page + 1);
-          sm.at[st][0] = (int)(a + (runs == 1 ? s * SUB % page : 0));
-          sm.at[st][1] = (int)(b + (runs == 1 ? s * SUB % page : 0));
+          if (LISTED) {  // places of a stage's two halves in the sequence
+            const int64_t a = page_first<LISTED>(P, w.seq, w.b, w.unit, tile, s * SUB / page);
+            const int64_t b = runs == 1 ? a + 16 : page_first<LISTED>(P, w.seq, w.b, w.unit, tile, s * SUB / page + 1);
+            sm.at[st][0] = (int)(a + (runs == 1 ? s * SUB % page : 0));
+            sm.at[st][1] = (int)(b + (runs == 1 ? s * SUB % page : 0));
+          }
           sm.ok[st] = runs == 1 ? (got & 1 ? 3 : 0) : (int)((got & 1) | (got >> 1 & 2));
           pipe::expect_tx(bar, __popc(got) * bytes);
         }
@@ -91,8 +93,8 @@ GDNX_DEV void load_stages(const DecParams& P, Walk w, uint8_t* ring, Small<NH>& 
   }
 }
 
-template <int LPK, int NH>
-GDNX_DEV void use_stages(const DecParams& P, Walk w, int64_t per, const uint8_t* ring, Small<NH>& sm) {
+template <bool LISTED, int LPK, int NH>
+GDNX_DEV void use_stages(const DecParams& P, Walk<LISTED> w, int64_t per, const uint8_t* ring, Small<NH>& sm) {
   constexpr int KPW = 32 / LPK, PASSES = SUB / WARPS / KPW;
   const DecodeArgs& a = P.a;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, sub = lane / LPK, dl = lane % LPK, D = (int)a.cache.D;
@@ -120,20 +122,25 @@ GDNX_DEV void use_stages(const DecParams& P, Walk w, int64_t per, const uint8_t*
     }
     for (int t = w.ta; t < w.tb; ++t) {
       for (int s = 0; s < TM / SUB; ++s) {
-        if (!sub_seen(P, w.seq, w.seq.kt.tile(t), s)) continue;
+        if (!sub_seen<LISTED>(P, w.seq, w.seq.kt.tile(t), s)) continue;
         const uint32_t st = n % STAGES;
         ok = ok && warp_wait(&sm.full[st], n / STAGES & 1, &sm.abort_flag);
         ++n;
         if (!ok) continue;
         const int on_page = *const_cast<volatile int*>(&sm.ok[st]);
-        const int at[2] = {*const_cast<volatile int*>(&sm.at[st][0]), *const_cast<volatile int*>(&sm.at[st][1])};
+        const int j0 = w.seq.kt.tile(t) * TM + s * SUB;
+        int at[2] = {0, 0};
+        if (LISTED) {
+          at[0] = *const_cast<volatile int*>(&sm.at[st][0]);
+          at[1] = *const_cast<volatile int*>(&sm.at[st][1]);
+        }
         const float* kt = reinterpret_cast<const float*>(ring + st * 2 * SIDE);
         const float* vt = reinterpret_cast<const float*>(ring + st * 2 * SIDE + SIDE);
         float x[PASSES][NH];
         bool seen[PASSES], over = false;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-          const int r = warp * (SUB / WARPS) + i * KPW + sub, j = (r < 16 ? at[0] : at[1]) + r % 16;
+          const int r = warp * (SUB / WARPS) + i * KPW + sub, j = LISTED ? (r < 16 ? at[0] : at[1]) + r % 16 : j0 + r;
           seen[i] = key_seen(j, w.seq.len, window, sinks) && (on_page >> (r / 16) & 1);
           any |= seen[i];
           float4 k0 = make_float4(0.f, 0.f, 0.f, 0.f), k1 = k0;
@@ -250,7 +257,7 @@ GDNX_DEV void use_stages(const DecParams& P, Walk w, int64_t per, const uint8_t*
   }
 }
 
-template <int LPK, int NH>
+template <bool LISTED, int LPK, int NH>
 __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_kernel(const DecParams P) {
   extern __shared__ __align__(128) uint8_t ring[];
   Small<NH>& sm = *reinterpret_cast<Small<NH>*>(ring + STAGES * 2 * SIDE);
@@ -264,13 +271,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_kernel(const DecPara
     }
   }
   wait_for_earlier();
-  find_range<NTHREADS>(P, units, sm.range, sm.sums);  // synchronises
-  const Walk w(P, units, sm.range);
+  find_range<LISTED, NTHREADS>(P, units, sm.range, sm.sums);  // synchronises
+  const Walk<LISTED> w(P, units, sm.range);
   if (warp < WARPS) {
-    use_stages<LPK, NH>(P, w, sm.range.per, ring, sm);
+    use_stages<LISTED, LPK, NH>(P, w, sm.range.per, ring, sm);
   } else {
-    load_stages<NH>(P, w, ring, sm);
-    write_zeros(P);
+    load_stages<LISTED, NH>(P, w, ring, sm);
+    write_zeros<LISTED>(P);
     if (*const_cast<volatile int*>(&sm.abort_flag))  // let the copies in flight land
       for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
   }
@@ -278,14 +285,19 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_kernel(const DecPara
   if (threadIdx.x == 0 && sm.abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
 }
 
-template <int LPK, int NH>
-gdnx_status launch(const DecParams& P, cudaStream_t st) {
+template <bool LISTED, int LPK, int NH>
+gdnx_status launch_as(const DecParams& P, cudaStream_t st) {
   constexpr int smem = (int)(STAGES * 2 * SIDE + sizeof(Small<NH>));
-  const auto kernel = paged_decode_kernel<LPK, NH>;
+  const auto kernel = paged_decode_kernel<LISTED, LPK, NH>;
   static std::atomic<uint64_t> done;
   if (!allow_smem(kernel, smem, done)) return GDNX_ELAUNCH;
   if (launch_early(kernel, dim3((unsigned)P.grid), dim3(NTHREADS), smem, st, P) != cudaSuccess) return GDNX_ELAUNCH;
   return join_parts<NH>(P, st);
+}
+
+template <int LPK, int NH>
+gdnx_status launch(const DecParams& P, cudaStream_t st) {
+  return P.a.positions || P.a.pages ? launch_as<true, LPK, NH>(P, st) : launch_as<false, LPK, NH>(P, st);
 }
 
 // Query heads of a unit.

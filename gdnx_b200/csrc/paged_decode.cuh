@@ -44,26 +44,30 @@ struct Range {
 
 // Visible tokens of one sequence.  Where the call names pages, its tiles hold the first `listed` pages of each
 // key head's list in their order, not the tokens in theirs.
+// LISTED, here and below: the call may name pages or positions.  Asked for at run time, what these need on the way to
+// the first load and for every tile cost the calls that have neither 2 to 7 % (4 tokens 8.7 instead of 8.1 us).
 struct Seq {
   int row, len;
   KeyTiles kt;
   int listed;
 };
 
+template <bool LISTED>
 GDNX_DEV int slot_length(const DecodeArgs& a, int64_t b, int& row) {
   const gdnx_cache& c = a.cache;
   row = a.rows ? a.rows[b] : (int)b;
   if (row < 0 || row >= c.slots) return 0;
   int64_t n = c.lengths[row];
   const int64_t most = c.width * c.page;
-  if (a.positions) n = min(n, (int64_t)a.positions[b] + 1);
+  if (LISTED && a.positions) n = min(n, (int64_t)a.positions[b] + 1);
   return (int)(n < 0 ? 0 : (n > most ? most : n));
 }
 
+template <bool LISTED>
 GDNX_DEV Seq make_seq(const DecodeArgs& a, int64_t b) {
   int row;
-  const int len = slot_length(a, b, row);
-  if (a.pages) {
+  const int len = slot_length<LISTED>(a, b, row);
+  if (LISTED && a.pages) {
     Seq s = {row, len, KeyTiles(), (int)min(a.listed, (int64_t)(len + a.cache.page - 1) / a.cache.page)};
     s.kt.count = (s.listed * a.cache.page + TM - 1) / TM;
     return s;
@@ -71,11 +75,12 @@ GDNX_DEV Seq make_seq(const DecodeArgs& a, int64_t b) {
   return {row, len, KeyTiles(len - 1, len - 1, len, (int)a.window, (int)a.sinks, TM), 0};
 }
 
-GDNX_DEV int tiles_of(const DecodeArgs& a, int64_t b) { return make_seq(a, b).kt.count; }
+template <bool LISTED>
+GDNX_DEV int tiles_of(const DecodeArgs& a, int64_t b) { return make_seq<LISTED>(a, b).kt.count; }
 
 // The CTA finds its range: every thread adds up a run of sequences, and the one whose run holds
 // the range's first tile walks to its sequence.  (Whole units: t0 and t1 count units.)
-template <int THREADS>
+template <bool LISTED, int THREADS>
 GDNX_DEV void find_range(const DecParams& P, int units, Range& out, long long* sums) {
   if (P.whole) {
     if (threadIdx.x == 0) {
@@ -89,7 +94,7 @@ GDNX_DEV void find_range(const DecParams& P, int units, Range& out, long long* s
   const int64_t run = (P.a.B + THREADS - 1) / THREADS;
   const int64_t b0 = min((int64_t)threadIdx.x * run, P.a.B), b1 = min(b0 + run, P.a.B);
   long long mine = 0;
-  for (int64_t b = b0; b < b1; ++b) mine += tiles_of(P.a, b);
+  for (int64_t b = b0; b < b1; ++b) mine += tiles_of<LISTED>(P.a, b);
   long long s = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -111,7 +116,7 @@ GDNX_DEV void find_range(const DecParams& P, int units, Range& out, long long* s
   if (t0 < total && t0 >= before && t0 < before + mine * units) {
     int64_t b = b0;
     for (; b + 1 < b1; ++b) {
-      const long long n = (long long)tiles_of(P.a, b) * units;
+      const long long n = (long long)tiles_of<LISTED>(P.a, b) * units;
       if (t0 < before + n) break;
       before += n;
     }
@@ -121,6 +126,7 @@ GDNX_DEV void find_range(const DecParams& P, int units, Range& out, long long* s
 }
 
 // Walks the units of a range: every role sees the same sequence of segments.
+template <bool LISTED>
 struct Walk {
   const DecParams& P;
   int units;
@@ -129,14 +135,14 @@ struct Walk {
   int unit, ta, tb;  // segment: tiles ta..tb-1 of `unit` of sequence b
   GDNX_DEV Walk(const DecParams& P_, int units_, const Range& r)
       : P(P_), units(units_), t(r.t0), t1(r.t1), b(r.b), before(r.before), seq(), unit(0), ta(0), tb(0) {
-    if (t < t1 && !P.whole) seq = make_seq(P.a, b);
+    if (t < t1 && !P.whole) seq = make_seq<LISTED>(P.a, b);
   }
   GDNX_DEV bool next() {
     if (P.whole) {
       for (; t < t1; ++t) {
         b = t / units;
         unit = (int)(t % units);
-        seq = make_seq(P.a, b);
+        seq = make_seq<LISTED>(P.a, b);
         if ((tb = seq.kt.count) == 0) continue;
         ++t;
         return true;
@@ -146,7 +152,7 @@ struct Walk {
     if (t >= t1) return false;
     while (t >= before + (int64_t)seq.kt.count * units) {
       before += (int64_t)seq.kt.count * units;
-      seq = make_seq(P.a, ++b);
+      seq = make_seq<LISTED>(P.a, ++b);
     }
     const int n = seq.kt.count;
     unit = (int)((t - before) / n);
@@ -163,18 +169,20 @@ GDNX_DEV bool key_seen(int j, int len, int window, int sinks) {
 }
 
 // First token of the i-th page of a unit's tile kt (-1: the list has none there).
+template <bool LISTED>
 GDNX_DEV int64_t page_first(const DecParams& P, const Seq& s, int64_t b, int unit, int kt, int i) {
   const gdnx_cache& c = P.a.cache;
-  if (!P.a.pages) return (int64_t)kt * TM + i * c.page;
+  if (!LISTED || !P.a.pages) return (int64_t)kt * TM + i * c.page;
   const int e = kt * (TM / c.page) + i;
   const int x = e < s.listed ? P.a.pages[(b * c.Hk + unit / P.groups) * P.a.listed + e] : -1;
   return x < 0 || x >= c.width ? -1 : (int64_t)x * c.page;
 }
 
 // Page ids of a tile's pages, or -1 where nothing visible is there (lane < npp), and their first tokens.
+template <bool LISTED>
 GDNX_DEV int page_id(const DecParams& P, const Seq& s, int64_t b, int unit, int kt, int i, int64_t& first) {
   const gdnx_cache& c = P.a.cache;
-  first = page_first(P, s, b, unit, kt, i);
+  first = page_first<LISTED>(P, s, b, unit, kt, i);
   if (first < 0 || first >= s.len || !(first + c.page > (int64_t)s.len - P.a.window || first < P.a.sinks)) return -1;
   const int p = c.table[(int64_t)s.row * c.width + first / c.page];
   return p >= 0 && p < c.pages ? p : -1;
@@ -187,11 +195,12 @@ constexpr float kNoScore = -3.402823466e38f;
 GDNX_DEV float no_weights(float top) { return top == -INFINITY ? 0.f : NAN; }
 
 // Zeros for the sequences that see nothing.
+template <bool LISTED>
 GDNX_DEV void write_zeros(const DecParams& P) {
   const DecodeArgs& a = P.a;
   const int D = (int)a.cache.D, n = (int)a.H * D;
   for (int64_t b = blockIdx.x; b < a.B; b += P.grid) {
-    if (tiles_of(a, b) > 0) continue;
+    if (tiles_of<LISTED>(a, b) > 0) continue;
     for (int x = threadIdx.x % 32; x < n; x += 32)
       st_from_f32(a.y, a.y_dtype, b * a.y_sb + x / D * a.y_sh + x % D, 0.f);
   }

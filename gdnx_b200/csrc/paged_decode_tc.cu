@@ -63,8 +63,8 @@ GDNX_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, 
       : "memory");
 }
 
-template <int DB, int NH>
-GDNX_DEV void run_loads(const TcParams& P, Walk w, uint32_t smem, Bars& bar, int (*at)[8], volatile int* abort_flag) {
+template <bool LISTED, int DB, int NH>
+GDNX_DEV void run_loads(const TcParams& P, Walk<LISTED> w, uint32_t smem, Bars& bar, int (*at)[8], volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   const gdnx_cache& c = P.a.cache;
   const int lane = threadIdx.x % 32, npp = TM / c.page, page = c.page;
@@ -79,7 +79,7 @@ GDNX_DEV void run_loads(const TcParams& P, Walk w, uint32_t smem, Bars& bar, int
       const int k = (t - w.ta) % ahead;
       if (k == 0) {
         const int mine = t + lane / npp;
-        ids = mine < w.tb ? page_id(P, w.seq, w.b, w.unit, w.seq.kt.tile(mine), lane % npp, first) : -1;
+        ids = mine < w.tb ? page_id<LISTED>(P, w.seq, w.b, w.unit, w.seq.kt.tile(mine), lane % npp, first) : -1;
       }
       const int pg = lane / DB, d = lane % DB;
       const int id = __shfl_sync(0xffffffffu, ids, (k * npp + pg) & 31);
@@ -103,8 +103,8 @@ GDNX_DEV void run_loads(const TcParams& P, Walk w, uint32_t smem, Bars& bar, int
   }
 }
 
-template <int DB, int NH, bool BF16>
-GDNX_DEV void run_products(const TcParams& P, Walk w, uint32_t smem, uint32_t tmem, Bars& bar,
+template <bool LISTED, int DB, int NH, bool BF16>
+GDNX_DEV void run_products(const TcParams& P, Walk<LISTED> w, uint32_t smem, uint32_t tmem, Bars& bar,
                            volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   constexpr uint32_t ID_S = idesc16(BF16, 128, NH, false, false), ID_O = idesc16(BF16, 128, NH, true, false);
@@ -165,8 +165,8 @@ GDNX_DEV void run_products(const TcParams& P, Walk w, uint32_t smem, uint32_t tm
 }
 
 // The unit's query rows as a K-major tile of NH rows (rows beyond its heads zero), by one warp.
-template <int DB, int NH>
-GDNX_DEV void stage_q(const TcParams& P, const Walk& w, uint8_t* dst) {
+template <bool LISTED, int DB, int NH>
+GDNX_DEV void stage_q(const TcParams& P, const Walk<LISTED>& w, uint8_t* dst) {
   const DecodeArgs& a = P.a;
   const Heads hd(P, w.unit, NH);
   const int D = (int)a.cache.D;
@@ -189,12 +189,12 @@ GDNX_DEV void stage_q(const TcParams& P, const Walk& w, uint8_t* dst) {
   }
 }
 
-template <int DB, int NH>
-GDNX_DEV void run_queries(const TcParams& P, Walk w, uint8_t* base, Bars& bar, volatile int* abort_flag) {
+template <bool LISTED, int DB, int NH>
+GDNX_DEV void run_queries(const TcParams& P, Walk<LISTED> w, uint8_t* base, Bars& bar, volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   for (uint32_t seg = 0; w.next(); ++seg) {
     if (!warp_wait(&bar.q_empty[seg & 1], (seg / 2 & 1) ^ 1, abort_flag)) return;
-    stage_q<DB, NH>(P, w, base + Lo::Q + (seg & 1) * Lo::QB);
+    stage_q<LISTED, DB, NH>(P, w, base + Lo::Q + (seg & 1) * Lo::QB);
     tc::fence_async_smem();
     pipe::mbar_arrive(&bar.q_ready[seg & 1]);
   }
@@ -225,8 +225,8 @@ GDNX_DEV void tmem_st(uint32_t at, const float (&v)[NC]) {
 }
 
 // NC: heads that a thread works on, the unit's rounded up (the others' columns are not used).
-template <int DB, int NH, int NC, bool BF16>
-GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, uint32_t tmem, Bars& bar, float* red,
+template <bool LISTED, int DB, int NH, int NC, bool BF16>
+GDNX_DEV void run_keys(const TcParams& P, Walk<LISTED> w, int64_t per, uint8_t* base, uint32_t tmem, Bars& bar, float* red,
                        const int (*at)[8], volatile int* abort_flag) {
   using Lo = Layout<DB, NH>;
   const DecodeArgs& a = P.a;
@@ -349,7 +349,7 @@ GDNX_DEV void run_keys(const TcParams& P, Walk w, int64_t per, uint8_t* base, ui
   }
 }
 
-template <int DB, int NC, bool BF16>
+template <bool LISTED, int DB, int NC, bool BF16>
 __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __grid_constant__ TcParams P) {
   constexpr int NH = NC > 16 ? 32 : 16;
   using Lo = Layout<DB, NH>;
@@ -379,23 +379,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   }
   tc::fence_before();
   wait_for_earlier();
-  find_range<NTHREADS>(P, units, sm.range, sm.sums);  // synchronises
+  find_range<LISTED, NTHREADS>(P, units, sm.range, sm.sums);  // synchronises
   tc::fence_after();
   const uint32_t tmem = uniform(sm.tmem_at);
-  const Walk w(P, units, sm.range);
+  const Walk<LISTED> w(P, units, sm.range);
   if (smem % 1024) {  // never entered: the base is aligned
   } else if (warp < 4) {
-    run_keys<DB, NH, NC, BF16>(P, w, sm.range.per, base, tmem, bar, sm.red, sm.at, abort_flag);
+    run_keys<LISTED, DB, NH, NC, BF16>(P, w, sm.range.per, base, tmem, bar, sm.red, sm.at, abort_flag);
   } else if (warp == 4) {
-    run_products<DB, NH, BF16>(P, w, smem, tmem, bar, abort_flag);
+    run_products<LISTED, DB, NH, BF16>(P, w, smem, tmem, bar, abort_flag);
     __syncwarp();
     if (elect_one()) tc::commit(&bar.done);  // every product issued has ended before tensor memory is freed
     tc::mbar_wait(&bar.done, 0);
   } else if (warp == 6) {
-    run_queries<DB, NH>(P, w, base, bar, abort_flag);
+    run_queries<LISTED, DB, NH>(P, w, base, bar, abort_flag);
   } else {
-    run_loads<DB, NH>(P, w, smem, bar, sm.at, abort_flag);
-    write_zeros(P);
+    run_loads<LISTED, DB, NH>(P, w, smem, bar, sm.at, abort_flag);
+    write_zeros<LISTED>(P);
     if (*abort_flag)  // let the copies in flight land
       for (uint32_t it = 0; it < (1u << 12); ++it) __nanosleep(100);
   }
@@ -407,15 +407,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) paged_decode_tc_kernel(const __gr
   if (threadIdx.x == 0 && *abort_flag && P.a.error) *P.a.error = GDNX_ETIMEOUT;
 }
 
-template <int DB, int NC, bool BF16>
-gdnx_status launch(const TcParams& P, cudaStream_t st) {
+template <bool LISTED, int DB, int NC, bool BF16>
+gdnx_status launch_as(const TcParams& P, cudaStream_t st) {
   constexpr int NH = NC > 16 ? 32 : 16;
-  const auto kernel = paged_decode_tc_kernel<DB, NC, BF16>;
+  const auto kernel = paged_decode_tc_kernel<LISTED, DB, NC, BF16>;
   constexpr int smem = (int)Layout<DB, NH>::SMEM;
   static std::atomic<uint64_t> done;
   if (!allow_smem(kernel, smem, done)) return GDNX_ELAUNCH;
   if (launch_early(kernel, dim3((unsigned)P.grid), dim3(NTHREADS), smem, st, P) != cudaSuccess) return GDNX_ELAUNCH;
   return join_parts<NH>(P, st);
+}
+
+template <int DB, int NC, bool BF16>
+gdnx_status launch(const TcParams& P, cudaStream_t st) {
+  return P.a.positions || P.a.pages ? launch_as<true, DB, NC, BF16>(P, st) : launch_as<false, DB, NC, BF16>(P, st);
 }
 
 template <int DB, bool BF16>
