@@ -141,3 +141,80 @@ def test_bounds_take_time_by_rows_not_by_their_square():
         ops.cache_check(c)
         took.append(best)
     assert took[1] < 8 * took[0]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_foreign_plans_stay_within_the_tensors(dtype):
+    """Starts out of range or falling, and rows and positions that are none: what lies around the output is untouched, and
+    the rows that the clamped plan defines are what they are."""
+    c = cache([100, 37], page=16, D=64, dtype=dtype, width=8)
+    N, H, D = 40, 4, 64
+    starts, first, rows = i32(0, 20, 30), i32(80, 27), i32(0, 1)
+    lists = (torch.zeros(N, dtype=torch.int32, device=DEV),) * 2 + (torch.zeros(N, dtype=torch.int64, device=DEV),)
+    q = torch.randn(N, H, D, generator=torch.Generator().manual_seed(5)).to(TYPES[dtype]).to(DEV)
+    want = ops.paged_attention(q, c, ops.PagedStep(rows, starts, first, *lists))
+    assert (want[30:] == 0).all() and not (want[:30] == 0).all(-1).any()
+    zero = torch.zeros_like(want)
+    nobody = torch.cat([want[:20], zero[20:]])
+    plans = [  # starts, first, rows, what rows are defined, and as what
+        ((-5, 20, 30), first, rows, slice(0, N), want),
+        ((30, 10, 5), first, rows, slice(0, N), zero),
+        ((0, 20, 1 << 30), first, rows, slice(0, 20), want),
+        ((0, 20, -(1 << 31)), first, rows, slice(0, 0), want),
+        ((1 << 30, (1 << 31) - 1, 1 << 30), first, rows, slice(0, N), zero),
+        ((0, 20, 30), i32(80, (1 << 31) - 1), rows, slice(0, N), nobody),
+        ((0, 20, 30), i32(80, -(1 << 31)), rows, slice(0, N), nobody),
+        ((0, 20, 30), first, i32(0, (1 << 31) - 1), slice(0, N), nobody),
+        ((0, 20, 30), first, i32(0, -(1 << 31)), slice(0, N), nobody),
+    ]
+    for s, f, r, known, value in plans:
+        room = torch.full((N + 8, H + 2, D + 32), 7.0, dtype=TYPES[dtype], device=DEV)
+        out = room[4:4 + N, 1:1 + H, 16:16 + D]
+        assert ops.paged_attention(q, c, ops.PagedStep(r, i32(*s), f, *lists), out=out) is out
+        assert torch.equal(out[known], value[known]), (s, f, r)
+        inside = torch.zeros(room.shape, dtype=torch.bool, device=DEV)
+        inside[4:4 + N, 1:1 + H, 16:16 + D] = True
+        assert (room[~inside] == 7.0).all(), (s, f, r)
+    ops.check_device_status()
+
+
+@pytest.mark.parametrize("dtype,st", [("bf16", 0), ("f32", 0), ("f16", 1)])
+def test_places_that_are_none_are_passed_over(dtype, st):
+    """Places before, behind and far outside the pool (st 1: rows that are not aligned) write nothing."""
+    c = cache([100, 37], page=16, D=64, dtype=dtype, width=8)
+    most = c.kv.shape[2] * 16
+    places = torch.tensor([3, -1, most, -(1 << 62), most - 1, 1 << 62, -2, 17], device=DEV)
+    n, Hk = places.numel(), c.kv.shape[3]
+    k, v = (torch.randn(n, Hk, 64 + st, device=DEV).to(TYPES[dtype])[..., st:] for _ in range(2))
+    want = c.kv.clone()
+    for t in (0, 4, 7):
+        p = int(places[t])
+        want[1, 0, p // 16, :, p % 16], want[1, 1, p // 16, :, p % 16] = k[t], v[t]
+    ops.cache_append(c, k, v, ops.PagedStep(c.lengths, c.lengths, c.lengths, c.lengths, c.lengths, places), layer=1)
+    ops.cache_check(c)
+    assert torch.equal(c.kv.view(torch.uint8), want.view(torch.uint8))  # (what is unwritten may be NaN)
+
+
+def test_absent_and_wrong_bounds_are_refused():
+    c = cache([100, 37], page=16, D=64, width=8)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=DEV)
+    rows, counts = i32(0, 1), i32(1, 1)
+    good = torch.zeros(c.kv.shape[:4] + c.kv.shape[5:], dtype=c.kv.dtype, device=DEV)
+    calls = [lambda: ops.cache_bounds(c, rows, counts), lambda: ops.paged_select(q, c, 2), lambda: ops.cache_compact(c)]
+    c.bounds = None
+    for call in calls[:2]:
+        with pytest.raises(ValueError, match="no bounds"):
+            call()
+    calls[2]()  # a cache without bounds is compacted without
+    wide = torch.zeros(good.shape[:-1] + (128,), dtype=good.dtype, device=DEV)
+    for bad, message in ((good[:, :, :-1].contiguous(), "bounds must be"), (good.half(), "bounds must be"),
+                         (good[..., :32].contiguous(), "bounds must be"), (wide[..., :64], "bounds must be"),
+                         (good.cpu(), "CUDA|device")):
+        c.bounds = bad
+        for call in calls:
+            with pytest.raises(ValueError, match=message):
+                call()
+    c.bounds = good
+    for call in calls:
+        call()
+    ops.cache_check(c)
