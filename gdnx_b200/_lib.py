@@ -149,8 +149,8 @@ class PagedDecodeArgs(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
-class PagedDecodeListedArgs(C.Structure):
-    _fields_ = [("decode", PagedDecodeArgs), ("positions", C.c_void_p), ("pages", C.c_void_p), ("listed", C.c_int64)]
+class PagedDecodeListedArgs(PagedDecodeArgs):  # the C struct's member `decode` lies first
+    _fields_ = [("positions", C.c_void_p), ("pages", C.c_void_p), ("listed", C.c_int64)]
 
 
 class Step(C.Structure):

@@ -1457,25 +1457,24 @@ def paged_decode(q: torch.Tensor, cache: PagedCache, *, layer: int = 0, rows: Op
     if rows is None and B > s.slots:
         raise ValueError("more queries than slots")
     yb, yh, _ = y.stride()
-    a = L.PagedDecodeArgs(s, B, H, layer, min(window, 1 << 62), min(sinks, 1 << 62), max_len or 0,
-                          D ** -0.5 if scale is None else scale, L.View(q.data_ptr(), _DT[q.dtype], D, qb, 0, qh),
-                          None if rows is None else _index32(rows, B, "rows", index), y.data_ptr(), _DT[y.dtype], yb, yh,
-                          _error_word(index))
-    name, call = "gdnx_paged_decode", a
+    name, args = "gdnx_paged_decode", L.PagedDecodeArgs
     if positions is not None or pages is not None:
-        name, call = "gdnx_paged_decode_listed", L.PagedDecodeListedArgs(a)
-        a = call.decode
+        name, args = "gdnx_paged_decode_listed", L.PagedDecodeListedArgs
+    a = args(s, B, H, layer, min(window, 1 << 62), min(sinks, 1 << 62), max_len or 0,
+             D ** -0.5 if scale is None else scale, L.View(q.data_ptr(), _DT[q.dtype], D, qb, 0, qh),
+             None if rows is None else _index32(rows, B, "rows", index), y.data_ptr(), _DT[y.dtype], yb, yh,
+             _error_word(index))
     if positions is not None:
-        call.positions = _index32(positions, B, "positions", index)
+        a.positions = _index32(positions, B, "positions", index)
     if pages is not None:
         if pages.dtype is not torch.int32 or pages.dim() != 3 or pages.shape[:2] != (B, s.Hk) or pages.shape[2] < 1 or not pages.is_contiguous():
             raise ValueError("pages must be a contiguous int32 tensor [B,Hk,k]")
         _on_device(index, pages)
-        call.pages, call.listed = pages.data_ptr(), pages.shape[2]
-    need = _entry(name + "_workspace_bytes")(C.byref(call))
+        a.pages, a.listed = pages.data_ptr(), pages.shape[2]
+    need = _entry(name + "_workspace_bytes")(C.byref(a))
     ws = None
     if need:
         ws = q.new_empty(need, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    _enqueue(name, index, C.byref(call))
+    _enqueue(name, index, C.byref(a))
     return y

@@ -67,9 +67,9 @@ def test_the_idle_warps_of_chunk_attention_wait_that_way():
     assert all("&sm.asked" in line for line in re.findall(r"warp_wait\(&bar\.(?:job_full|item_empty)\[[^;]*;", src))
 
 
-def decode_args(page=64):
+def decode_args(struct=L.PagedDecodeArgs, page=64):
     """A 16-bit decode of one query over a long sequence (no pointer is read for its workspace)."""
-    a = L.PagedDecodeArgs()
+    a = struct()
     a.cache.dtype, a.cache.page, a.cache.L, a.cache.pages, a.cache.Hk, a.cache.D = 1, page, 1, 4096, 2, 128
     a.cache.slots, a.cache.width = 4, 4096
     a.B, a.H, a.window, a.scale, a.y_dtype = 1, 16, 1 << 40, 0.125, 1
@@ -91,19 +91,19 @@ def test_the_decode_reads_its_own_struct_only():
 
 def test_listed_decode_layout_and_refusals(tmp_path):
     py, cname = L.PagedDecodeListedArgs, "gdnx_paged_decode_listed_args"
+    fields = [("decode." + f, f) for f, _ in L.PagedDecodeArgs._fields_] + [(f, f) for f, _ in py._fields_]
     lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "gdnx.h"', "int main(void){",
              f'printf("%zu\\n", sizeof({cname}));']
-    lines += [f'printf("%zu\\n", offsetof({cname}, {f}));' for f, _ in py._fields_]
+    lines += [f'printf("%zu\\n", offsetof({cname}, {f}));' for f, _ in fields]
     src = tmp_path / "probe.c"
     src.write_text("\n".join(lines + ["return 0;}"]))
     subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(tmp_path / "probe")], check=True)
     got = [int(x) for x in subprocess.run([str(tmp_path / "probe")], capture_output=True, text=True).stdout.split()]
-    assert got == [C.sizeof(py)] + [getattr(py, f).offset for f, _ in py._fields_]
+    assert got == [C.sizeof(py)] + [getattr(py, f).offset for _, f in fields]
     lib = L.load()
     assert lib.gdnx_paged_decode_listed(None, None) == L.GDNX_EINVAL
     assert lib.gdnx_paged_decode_listed_workspace_bytes(None) == 0
-    a = L.PagedDecodeListedArgs(decode_args())
-    dense = lib.gdnx_paged_decode_listed_workspace_bytes(C.byref(a))
-    assert dense == lib.gdnx_paged_decode_workspace_bytes(C.byref(a.decode)) > 0
+    a = decode_args(L.PagedDecodeListedArgs)
+    assert lib.gdnx_paged_decode_listed_workspace_bytes(C.byref(a)) == lib.gdnx_paged_decode_workspace_bytes(C.byref(a)) > 0
     a.pages, a.listed = 1 << 20, 4  # two tiles of 128 tokens: not cut, no parts
     assert lib.gdnx_paged_decode_listed_workspace_bytes(C.byref(a)) == 0
