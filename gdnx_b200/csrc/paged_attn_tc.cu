@@ -23,13 +23,13 @@
 // instead of 959), K, V and Q share one pool of slots, a unit's start and end weigh six tiles in the cut (one tile: 148 and
 // 246 us instead of 114 and 189 for the second and third case below).
 //
-// Measured: 4096 tokens after 28,672, 16 heads over 2 of 128, f16: 876 us (1177 TFLOP/s of visible pairs, 71 % of a large
-// product's burst rate and 84 % of its rate under the power cap; tensor pipes busy 59 % of cycles); 64 sequences of up
-// to 8192 tokens with 2 to 5 new ones each, 16 heads over 4, bf16, pages of 64: 112 us (4.8 TB/s of the copy's 6.5); 4
-// chunks of up to 512 beside 60 single tokens over as many: 175 us (DRAM 47 %: its chunks' products and its tokens'
-// bytes come one after the other on an SM); 33 tokens after 467, 4 heads of 64, pages of 16: 18 us, of which the first
-// key tile arrives after 7 (one load after the other: lengths, page table, keys) and its 64 boxes of 2 KB take 5 to ask
-// for.
+// Measured: 4096 tokens after 28,672, 16 heads over 2 of 128, f16: 990 us under sustained load (1041 TFLOP/s of visible
+// pairs, 74 % of a large product's rate under the power cap), 876 us for the first 40 ms after a pause (1177 TFLOP/s, 71 %
+// of a product's burst rate); tensor pipes busy 59 % of cycles; 64 sequences of up to 8192 tokens with 2 to 5 new ones
+// each, 16 heads over 4, bf16, pages of 64: 112 us (4.8 TB/s of the copy's 6.5); 4 chunks of up to 512 beside 60 single
+// tokens over as many: 175 to 179 us (DRAM 47 %: its chunks' products and its tokens' bytes come one after the other on an
+// SM); 33 tokens after 467, 4 heads of 64, pages of 16: 18 us, of which the first key tile arrives after 7 (one load after
+// the other: lengths, page table, keys) and its 64 boxes of 2 KB take 5 to ask for.
 #include "paged_attn.cuh"
 
 namespace gdnx {
